@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define KVSSD_HIP_ABI_VERSION 5
+#define KVSSD_HIP_ABI_VERSION 6
 
 /* Query element types accepted by kvssd_hip_fused_decode (the reference
  * dispatches fp32/fp64/fp16/bf16 queries: csrc/fused_decode.cu:131-133). */
@@ -261,6 +261,138 @@ int kvssd_hip_read_probe(const void* data, size_t bytes, uint32_t* sink, size_t 
  * page-locked for the copy to be asynchronous.  The staging copy of
  * KVSSDPipeline._stage (src/kvssd/pipeline.py:110-114). */
 int kvssd_hip_memcpy_h2d_async(void* dst, const void* src, size_t bytes, void* stream);
+
+/* ------------------------------------------------------------- generation ---
+ * Operators of a decode loop over many sequences: rotary positions, and a
+ * paged packed cache that grows token by token.  No counterparts in the
+ * reference, whose cache is written once and then only read.  The pool's pages
+ * have the PackedBatch layout (src/kvssd/backends/base.py:19-27), so that a
+ * page is a block of that layout and kvssd_hip_fused_decode reads it as one. */
+
+/* Rotation by position p of the first rotary_dim values of a head: pair i
+ * (values i and i + rotary_dim / 2, or 2 i and 2 i + 1 where `interleaved`)
+ * turns by p * frequencies[i] and is multiplied by `magnitude`; the other
+ * values are left as they are.  `inverse` turns back (the rotation's
+ * transpose).  Angles, sines and products are formed in 64 bits and rounded
+ * once to the values' type. */
+typedef struct kvssd_rotary_spec {
+  const double* frequencies; /* device, [rotary_dim / 2] */
+  double magnitude;
+  int32_t head_dim;
+  int32_t rotary_dim; /* even, 2 <= rotary_dim <= head_dim <= 1024 */
+  int32_t interleaved;
+  int32_t inverse;
+} kvssd_rotary_spec;
+
+/* A [tokens, heads, head_dim] tensor: values of a head side by side, strides
+ * in elements. */
+typedef struct kvssd_heads {
+  const void* data;
+  void* out; /* where results go; may equal data with the same strides */
+  int64_t token_stride, head_stride;
+  int64_t out_token_stride, out_head_stride;
+  int32_t heads;
+  int32_t reserved;
+} kvssd_heads;
+
+/* out[t] = data[t] rotated by positions[t] (int32, or int64 where positions_64)
+ * for the `count` (1 or 2) tensors of `tensors`, both of `dtype` (F16, BF16,
+ * F32) and `tokens` tokens. */
+int kvssd_hip_rotary(const kvssd_rotary_spec* spec, const void* positions, int positions_64, int64_t tokens, int dtype,
+                     const kvssd_heads* tensors, int count, void* stream);
+
+/* A paged packed cache.  Pool: packed_k/v uint8 [num_pages, page_tokens,
+ * kv_heads, head_dim*bits/8] and scales fp16 [num_pages, page_tokens,
+ * kv_heads, head_dim/group_size], C-contiguous, 16-byte aligned.  Slot s of
+ * sequence b lies in page page_table[b][s / page_tokens], row
+ * s % page_tokens; sequence b holds slots 0 .. lengths[b]-1 (clamped to
+ * [0, max_pages*page_tokens]).  Pages outside [0, num_pages) are skipped:
+ * their slots are neither read nor written.  head_dim is a multiple of 32 up
+ * to 256, group_size a power of two, 32 or more, that divides it. */
+typedef struct kvssd_paged_cache {
+  int32_t bits, kv_heads, head_dim, group_size;
+  int32_t num_pages, page_tokens;
+  int32_t sequences, max_pages;
+  uint8_t* packed_k;
+  uint8_t* packed_v;
+  uint16_t* scales_k;
+  uint16_t* scales_v;
+  const int32_t* page_table; /* [sequences, max_pages] */
+  const int32_t* lengths;    /* [sequences] */
+  float* weights;            /* [sequences, max_pages*page_tokens] or NULL: summed attention weights */
+  int32_t* positions;        /* same shape or NULL: each slot's position */
+} kvssd_paged_cache;
+
+/* New tokens into their sequences' pages.  Token t of keys/values [tokens,
+ * kv_heads, head_dim] belongs to the sequence b with offsets[b] <= t <
+ * offsets[b+1] (offsets NULL: tokens == sequences, one each), goes to slot
+ * lengths[b] + i with i its place in the sequence's run, and has position
+ * first_positions[b] + i (first_positions NULL: its slot).  Keys are rotated
+ * (rotary not NULL) and rounded to their type, then keys and values are
+ * quantised as by kvssd_hip_quantize.  Slots past the table's end are
+ * dropped.  `query` (data NULL: none) is rotated by the same positions.
+ * Where the cache has them, the new slots' weights become 0 and their
+ * positions are stored.  lengths_out[b] = lengths[b] + count, at most the
+ * table's capacity; it may be the cache's own lengths where offsets is NULL. */
+typedef struct kvssd_paged_append_args {
+  kvssd_heads keys, values, query; /* keys.out and values.out are not used */
+  int64_t tokens;
+  const int32_t* offsets;         /* [sequences + 1] or NULL */
+  const int32_t* first_positions; /* [sequences] or NULL */
+  const kvssd_rotary_spec* rotary;
+  int32_t* lengths_out; /* or NULL */
+  int32_t dtype;        /* F16, BF16 or F32, of keys, values and query */
+  int32_t reserved;
+} kvssd_paged_append_args;
+int kvssd_hip_paged_append(const kvssd_paged_cache* cache, const kvssd_paged_append_args* args, void* stream);
+
+/* Attention of one query [sequences, query_heads, head_dim] (contiguous, F16,
+ * BF16 or F32) per sequence over its slots: out (fp32, or query_dtype with
+ * out_query_dtype = 1) and lse fp32 [sequences, query_heads].  A sequence of
+ * length 0 gives out = 0 and lse = -inf.  With `accumulate`, weights[b][s] +=
+ * sum over the query heads of exp(score - lse).  max_length and total_tokens
+ * size the split (0: the table's capacity, for every sequence); lengths beyond
+ * them are answered all the same.  fp32 outputs come from 32-bit-grade
+ * arithmetic; 16-bit ones round the softmax weights times the value scales to
+ * fp16. */
+typedef struct kvssd_paged_decode_args {
+  const void* query;
+  void* out;
+  float* lse;
+  void* workspace; /* kvssd_hip_paged_decode_workspace_bytes, 256-byte aligned */
+  size_t workspace_bytes;
+  double sm_scale;
+  int64_t total_tokens;
+  int32_t max_length;
+  int32_t query_heads;
+  int32_t query_dtype;
+  int32_t out_query_dtype;
+  int32_t accumulate;
+  int32_t reserved;
+} kvssd_paged_decode_args;
+int kvssd_hip_paged_decode_workspace_bytes(const kvssd_paged_cache* cache, const kvssd_paged_decode_args* args,
+                                           size_t* bytes);
+int kvssd_hip_paged_decode(const kvssd_paged_cache* cache, const kvssd_paged_decode_args* args, void* stream);
+
+/* Cuts every sequence to at most `budget` slots.  Kept are, in this order, the
+ * slots with a position below `sink` or above (largest position - recent), then
+ * those of the largest weights (NaN counts as -inf); of equals the lower slot.
+ * The n-th kept slot at or past the budget moves into the n-th freed slot
+ * before it, so that only those rows are copied, in place.  lengths_out,
+ * weights_out and positions_out (the cache's shapes, not its own arrays)
+ * describe the result; slots past the new length get weight 0 and position
+ * -1.  Needs the cache's weights and positions. */
+typedef struct kvssd_paged_evict_args {
+  int32_t budget, sink, recent, reserved;
+  int32_t* lengths_out;
+  float* weights_out;
+  int32_t* positions_out;
+  void* workspace; /* kvssd_hip_paged_evict_workspace_bytes */
+  size_t workspace_bytes;
+} kvssd_paged_evict_args;
+int kvssd_hip_paged_evict_workspace_bytes(const kvssd_paged_cache* cache, const kvssd_paged_evict_args* args,
+                                          size_t* bytes);
+int kvssd_hip_paged_evict(const kvssd_paged_cache* cache, const kvssd_paged_evict_args* args, void* stream);
 
 /* Message of the last failed call on this host thread ("" if none). */
 const char* kvssd_hip_last_error(void);

@@ -1,0 +1,35 @@
+// Shared by the generation operators: rotary positions and the paged packed
+// cache (rotary.hip, paged_append.hip, paged_decode*.hip, paged_evict.hip).
+#pragma once
+
+#include "common.hpp"
+
+namespace kvssd {
+
+inline int64_t paged_capacity(const kvssd_paged_cache& c) { return static_cast<int64_t>(c.max_pages) * c.page_tokens; }
+
+// the checks every paged entry point makes of a cache
+int check_paged_cache(const kvssd_paged_cache* c);
+int check_rotary(const kvssd_rotary_spec* r);
+
+inline size_t dtype_bytes(int dtype) { return dtype == KVSSD_DTYPE_F32 ? 4 : 2; }
+inline bool paged_dtype(int dtype) {
+  return dtype == KVSSD_DTYPE_F16 || dtype == KVSSD_DTYPE_BF16 || dtype == KVSSD_DTYPE_F32;
+}
+
+int launch_rotary(const kvssd_rotary_spec& r, const void* positions, int positions_64, int64_t tokens, int dtype,
+                  const kvssd_heads* tensors, int count, hipStream_t stream);
+int launch_paged_append(const kvssd_paged_cache& c, const kvssd_paged_append_args& a, hipStream_t stream);
+int paged_decode_bytes(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, size_t* bytes);
+int launch_paged_decode(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, hipStream_t stream);
+int launch_paged_evict(const kvssd_paged_cache& c, const kvssd_paged_evict_args& a, hipStream_t stream);
+
+// ------------------------------------------------------------ device side ---
+
+// Length of sequence b as every kernel takes it.
+__device__ __forceinline__ int paged_length(const int32_t* lengths, int b, int capacity) {
+  const int n = lengths[b];
+  return n < 0 ? 0 : (n > capacity ? capacity : n);
+}
+
+}  // namespace kvssd

@@ -1,0 +1,237 @@
+// Paged decode: the split plan, the join of a sequence's runs, the sum of its
+// attention weights, and the C entry points.
+//
+// Join, per (sequence, query head): with partials (O_r unnormalised, m_r in
+// log2 units, l_r) of the sequence's runs r,
+//   M = max m_r, L = sum l_r 2^(m_r - M), out = sum O_r 2^(m_r - M) / L,
+//   lse = ln 2 (M + log2 L);
+// runs with l = 0 (no slot took part) add nothing.  The number of runs follows
+// from the sequence's length on the device, as in the decode kernel.
+//
+// Weights: slot t of sequence b gains sum over heads of 2^(s_bht - lse2_bh) from
+// the scores that the decode left (4 bytes a slot and head): a second pass
+// over the keys would read head_dim * bits / 8 + scales per kv head instead.
+#include "paged_decode.hpp"
+
+#include <string>
+
+namespace kvssd {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSlice = 64;  // dims of a workgroup: 16 lanes of 4, 16 runs side by side
+
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams p) {
+  __shared__ float w_s[kMaxSplits];
+  __shared__ float red[2][kThreads / kWave];
+  __shared__ float4v sum_s[kThreads / kWave][16];
+  const int seq = blockIdx.x / p.query_heads, h = blockIdx.x % p.query_heads;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int length = paged_length(p.c.lengths, seq, p.capacity);
+  const int run = run_of(length, p.chunk, p.splits);
+  const int n = length > 0 ? (length + run - 1) / run : 0;
+  const int64_t row0 = static_cast<int64_t>(seq) * p.splits * p.query_heads + h;  // run r: row0 + r * query_heads
+  const int d0 = blockIdx.y * kSlice + 4 * (tid & 15);
+  const int d = p.c.head_dim;
+  float big = -INFINITY;
+  for (int r = tid; r < n; r += kThreads) {
+    const float* ml = p.part_ml + 2 * (row0 + static_cast<int64_t>(r) * p.query_heads);
+    w_s[r] = ml[1] != 0.0f ? ml[0] : -INFINITY;  // (a NaN sum keeps its run)
+    if (ml[1] != 0.0f) big = fmaxf(big, ml[0]);
+  }
+  big = wave_max(big);
+  if (lane == 0) red[0][wave] = big;
+  __syncthreads();
+  big = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float total = 0.0f;
+  for (int r = tid; r < n; r += kThreads) {
+    const float l = p.part_ml[2 * (row0 + static_cast<int64_t>(r) * p.query_heads) + 1];
+    const float w = l != 0.0f ? exp2f(w_s[r] - big) : 0.0f;
+    w_s[r] = w;
+    total += w * l;
+  }
+  total = wave_sum(total);
+  if (lane == 0) red[1][wave] = total;
+  __syncthreads();
+  total = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (d0 < d) {
+    const float* o = p.part_o + row0 * d + d0;
+    const int64_t step = static_cast<int64_t>(p.query_heads) * d;
+#pragma unroll 4
+    for (int r = tid / 16; r < n; r += kThreads / 16) {
+      const float w = w_s[r];
+      const float4v v = *reinterpret_cast<const float4v*>(o + r * step);
+      if (w != 0.0f) acc += w * v;  // (NaN weights take part)
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    acc[i] += __shfl_xor(acc[i], 16, kWave);
+    acc[i] += __shfl_xor(acc[i], 32, kWave);
+  }
+  if (lane < 16) sum_s[wave][lane] = acc;
+  __syncthreads();
+  const int64_t row = static_cast<int64_t>(seq) * p.query_heads + h;
+  if (tid < 16 && d0 < d) {
+    const float4v v = (sum_s[0][tid] + sum_s[1][tid]) + (sum_s[2][tid] + sum_s[3][tid]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_out(p.out, p.out_dtype, row * d + d0 + i, total == 0.0f ? 0.0f : v[i] / total);
+  }
+  if (tid == 0 && blockIdx.y == 0) p.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (big + log2f(total));
+}
+
+__global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodeParams p) {
+  const int seq = blockIdx.y;
+  const int length = paged_length(p.c.lengths, seq, p.capacity);
+  const float* lse = p.lse + static_cast<int64_t>(seq) * p.query_heads;
+  for (int64_t t = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 4; t < length;
+       t += static_cast<int64_t>(gridDim.x) * kThreads * 4) {
+    const float* s = p.scores + static_cast<int64_t>(seq) * p.query_heads * p.score_stride + t;
+    float4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int h = 0; h < p.query_heads; ++h) {
+      const float4v v = *reinterpret_cast<const float4v*>(s + h * p.score_stride);
+      const float e = lse[h] * kLog2e;
+      if (e == -INFINITY) continue;  // no slot took part
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] += exp2f(v[i] - e);
+    }
+    float* w = p.c.weights + static_cast<int64_t>(seq) * p.capacity + t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (t + i < length) w[i] += sum[i];
+  }
+}
+
+// Runs and shapes of a decode; the workspace's arrays as offsets from its start.
+struct Plan {
+  PagedDecodeParams p;
+  int dp, nt;
+  size_t o_bytes, ml_bytes, score_bytes;
+};
+
+size_t aligned(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+int plan_of(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, Plan* out) {
+  if (a.query_heads <= 0 || a.query_heads % c.kv_heads) return arg_error("query heads must be divisible by KV heads");
+  if (!paged_dtype(a.query_dtype)) return arg_error("unsupported query dtype");
+  if (a.out_query_dtype != 0 && a.out_query_dtype != 1) return arg_error("out_query_dtype must be 0 or 1");
+  if (a.max_length < 0 || a.total_tokens < 0) return arg_error("max_length and total_tokens must be >= 0");
+  if (a.accumulate && !c.weights) return arg_error("accumulate needs a cache with weights");
+  PagedDecodeParams& p = out->p;
+  p = PagedDecodeParams{};
+  p.c = c;
+  p.query = a.query;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.capacity = static_cast<int>(paged_capacity(c));
+  p.query_heads = a.query_heads;
+  p.gq = a.query_heads / c.kv_heads;
+  p.query_dtype = a.query_dtype;
+  p.out_dtype = a.out_query_dtype ? a.query_dtype : KVSSD_DTYPE_F32;
+  p.scale_log2 = static_cast<float>(a.sm_scale) * kLog2e;
+  p.groups = c.head_dim / c.group_size;
+  while ((1 << p.gp_log2) < p.groups) ++p.gp_log2;
+  const int heads = 16 >> p.gp_log2;
+  p.tiles = (p.gq + heads - 1) / heads;
+  out->dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+  // two head tiles share a tile's codes; at 256 dims their sums would not fit the registers
+  out->nt = p.tiles > 1 && out->dp < 256 ? 2 : 1;
+  p.tile_sets = (p.tiles + out->nt - 1) / out->nt;
+  p.head_groups = (c.kv_heads + kDecodeWaves - 1) / kDecodeWaves;
+  p.heads_of_group = (c.kv_heads + p.head_groups - 1) / p.head_groups;
+  if (static_cast<int64_t>(p.head_groups) * p.tile_sets > 65535) return arg_error("too many heads");
+
+  int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
+  int64_t all = a.total_tokens > 0 ? a.total_tokens : longest * c.sequences;
+  if (all > longest * c.sequences) all = longest * c.sequences;
+  constexpr int64_t kWaves = 4096;
+  auto tiles_up = [](int64_t n) { return (n + kTile - 1) / kTile * kTile; };
+  int64_t chunk = tiles_up((all * c.kv_heads * p.tile_sets + kWaves - 1) / kWaves);
+  if (chunk < 64) chunk = 64;
+  if ((longest + chunk - 1) / chunk > kMaxSplits) chunk = tiles_up((longest + kMaxSplits - 1) / kMaxSplits);
+  p.chunk = static_cast<int>(chunk);
+  p.splits = static_cast<int>((longest + chunk - 1) / chunk);
+  if (p.splits < 1) p.splits = 1;
+  p.group_splits = kDecodeWaves / p.heads_of_group;
+  if (p.group_splits > p.splits) p.group_splits = p.splits;
+
+  const size_t rows = static_cast<size_t>(c.sequences) * p.query_heads * p.splits;
+  out->o_bytes = p.splits > 1 ? aligned(rows * c.head_dim * sizeof(float)) : 0;
+  out->ml_bytes = p.splits > 1 ? aligned(rows * 2 * sizeof(float)) : 0;
+  p.score_stride = tiles_up(p.capacity);
+  out->score_bytes =
+      a.accumulate ? static_cast<size_t>(c.sequences) * p.query_heads * p.score_stride * sizeof(float) : 0;
+  const int64_t wgs = static_cast<int64_t>(c.sequences) * ((p.splits + p.group_splits - 1) / p.group_splits);
+  if (wgs * kDecodeWaves * kWave > 0xFFFFFFFFll || static_cast<int64_t>(c.sequences) * p.query_heads * kThreads > 0xFFFFFFFFll)
+    return arg_error("too many sequences for one call");
+  return 0;
+}
+
+}  // namespace
+
+int launch_paged_merge(const PagedDecodeParams& p, hipStream_t stream) {
+  const dim3 grid(p.c.sequences * p.query_heads, (p.c.head_dim + kSlice - 1) / kSlice);
+  hipLaunchKernelGGL(paged_merge_kernel, grid, dim3(kThreads), 0, stream, p);
+  return hip_status(hipGetLastError(), "paged_merge launch");
+}
+
+int paged_decode_bytes(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, size_t* bytes) {
+  Plan plan{};
+  if (int rc = plan_of(c, a, &plan)) return rc;
+  *bytes = plan.o_bytes + plan.ml_bytes + plan.score_bytes;
+  return 0;
+}
+
+int launch_paged_decode(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, hipStream_t stream) {
+  Plan plan{};
+  if (int rc = plan_of(c, a, &plan)) return rc;
+  PagedDecodeParams& p = plan.p;
+  const size_t need = plan.o_bytes + plan.ml_bytes + plan.score_bytes;
+  if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need))
+    return arg_error("workspace too small: need " + std::to_string(need) + " bytes");
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 256) return arg_error("workspace must be 256-byte aligned");
+  char* ws = static_cast<char*>(a.workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + plan.o_bytes);
+  if (a.accumulate) p.scores = reinterpret_cast<float*>(ws + plan.o_bytes + plan.ml_bytes);
+  const bool precise = p.out_dtype == KVSSD_DTYPE_F32 || p.query_dtype == KVSSD_DTYPE_F32;
+  if (int rc = c.bits == 4 ? launch_paged_int4(p, plan.dp, plan.nt, precise, stream)
+                           : launch_paged_int2(p, plan.dp, plan.nt, precise, stream))
+    return rc;
+  if (p.splits > 1)
+    if (int rc = launch_paged_merge(p, stream)) return rc;
+  if (a.accumulate) {
+    const int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
+    const int64_t blocks = (longest + 4 * kThreads - 1) / (4 * kThreads);
+    hipLaunchKernelGGL(paged_weights_kernel, dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024), c.sequences),
+                       dim3(kThreads), 0, stream, p);
+    return hip_status(hipGetLastError(), "paged_weights launch");
+  }
+  return 0;
+}
+
+}  // namespace kvssd
+
+using namespace kvssd;
+
+extern "C" {
+
+__attribute__((visibility("default"))) int kvssd_hip_paged_decode_workspace_bytes(const kvssd_paged_cache* cache,
+                                                                                  const kvssd_paged_decode_args* args,
+                                                                                  size_t* bytes) {
+  if (int rc = check_paged_cache(cache)) return rc;
+  if (args == nullptr || bytes == nullptr) return arg_error("arguments are NULL");
+  return paged_decode_bytes(*cache, *args, bytes);
+}
+
+__attribute__((visibility("default"))) int kvssd_hip_paged_decode(const kvssd_paged_cache* cache,
+                                                                  const kvssd_paged_decode_args* args, void* stream) {
+  if (int rc = check_paged_cache(cache)) return rc;
+  if (args == nullptr) return arg_error("arguments are NULL");
+  if (!args->query || !args->out || !args->lse) return arg_error("a required buffer pointer is NULL");
+  return launch_paged_decode(*cache, *args, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,123 @@
+// Rotary positions of queries and keys (rotary_ops.hpp has the arithmetic).
+//
+// A workgroup takes one token, or a few of a long prompt: its threads form the
+// tokens' sines once (LDS), then take items of 2 x 16 bytes -- the two
+// partners of 8 (16-bit types) or 4 pairs -- over all heads of both tensors.
+#include "paged.hpp"
+#include "rotary_ops.hpp"
+
+namespace kvssd {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTurns = 512;  // of a workgroup: 8 KB of LDS
+
+struct RotaryParams {
+  const double* frequencies;
+  const void* positions;
+  double magnitude;
+  kvssd_heads t[2];
+  RotaryShape shape;
+  int64_t tokens;
+  int count, inverse, positions_64, per_group;  // tokens of a workgroup
+};
+
+template <typename T, int PV>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p) {
+  __shared__ Turn turns[kMaxTurns];
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.per_group;
+  const int n = static_cast<int>(p.tokens - t0 < p.per_group ? p.tokens - t0 : p.per_group);
+  for (int i = threadIdx.x; i < n * p.shape.pairs; i += kThreads) {
+    const int64_t t = t0 + i / p.shape.pairs;
+    const double pos = p.positions_64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[t])
+                                      : static_cast<double>(static_cast<const int32_t*>(p.positions)[t]);
+    turns[i] = make_turn(pos, p.frequencies[i % p.shape.pairs], p.magnitude, p.inverse);
+  }
+  __syncthreads();
+  for (int k = 0; k < p.count; ++k) {
+    const kvssd_heads& h = p.t[k];
+    const int per_token = h.heads * p.shape.items;
+    for (int i = threadIdx.x; i < n * per_token; i += kThreads) {
+      const int tok = i / per_token, rest = i % per_token;
+      const int head = rest / p.shape.items, item = rest % p.shape.items;
+      rotary_item<T, PV>(p.shape, item,
+                         static_cast<const T*>(h.data) + (t0 + tok) * h.token_stride + head * h.head_stride,
+                         static_cast<T*>(h.out) + (t0 + tok) * h.out_token_stride + head * h.out_head_stride,
+                         turns + tok * p.shape.pairs);
+    }
+  }
+}
+
+template <typename T>
+void launch_typed(RotaryParams& p, const kvssd_rotary_spec& r, hipStream_t stream) {
+  constexpr int kVec = 16 / sizeof(T);
+  bool vec = (r.rotary_dim / 2) % kVec == 0 && (r.head_dim - r.rotary_dim) % kVec == 0;
+  for (int k = 0; k < p.count; ++k) vec = vec && heads_vector(p.t[k], sizeof(T), true);
+  p.shape = rotary_shape(r, vec ? kVec : 1);
+  int per = kMaxTurns / p.shape.pairs;  // >= 1: at most 512 pairs
+  // long prompts: the sines of 4 tokens at a time give every thread one; short
+  // ones: a workgroup a token, so that more CUs take part
+  per = p.tokens >= 2048 ? (per < 4 ? per : 4) : 1;
+  p.per_group = per;
+  const dim3 grid(static_cast<unsigned>((p.tokens + per - 1) / per));
+  if (vec) hipLaunchKernelGGL((rotary_kernel<T, kVec>), grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((rotary_kernel<T, 1>), grid, dim3(kThreads), 0, stream, p);
+}
+
+}  // namespace
+
+int check_rotary(const kvssd_rotary_spec* r) {
+  if (r == nullptr || r->frequencies == nullptr) return arg_error("a required buffer pointer is NULL");
+  if (r->rotary_dim < 2 || r->rotary_dim % 2 || r->rotary_dim > r->head_dim)
+    return arg_error("rotary_dim must be even and between 2 and head_dim");
+  if (r->head_dim > 1024) return arg_error("rotary head_dim must be <= 1024");
+  return 0;
+}
+
+int launch_rotary(const kvssd_rotary_spec& r, const void* positions, int positions_64, int64_t tokens, int dtype,
+                  const kvssd_heads* tensors, int count, hipStream_t stream) {
+  RotaryParams p{};
+  p.frequencies = r.frequencies;
+  p.positions = positions;
+  p.magnitude = r.magnitude;
+  for (int k = 0; k < count; ++k) p.t[k] = tensors[k];
+  p.tokens = tokens;
+  p.count = count;
+  p.inverse = r.inverse;
+  p.positions_64 = positions_64;
+  switch (dtype) {
+    case KVSSD_DTYPE_F16:
+      launch_typed<_Float16>(p, r, stream);
+      break;
+    case KVSSD_DTYPE_BF16:
+      launch_typed<uint16_t>(p, r, stream);
+      break;
+    default:
+      launch_typed<float>(p, r, stream);
+  }
+  return hip_status(hipGetLastError(), "rotary launch");
+}
+
+}  // namespace kvssd
+
+using namespace kvssd;
+
+extern "C" __attribute__((visibility("default"))) int kvssd_hip_rotary(const kvssd_rotary_spec* spec,
+                                                                       const void* positions, int positions_64,
+                                                                       int64_t tokens, int dtype,
+                                                                       const kvssd_heads* tensors, int count,
+                                                                       void* stream) {
+  if (int rc = check_rotary(spec)) return rc;
+  if (!paged_dtype(dtype)) return arg_error("unsupported dtype");
+  if (count < 1 || count > 2 || tensors == nullptr) return arg_error("rotary takes one or two tensors");
+  if (tokens < 0 || tokens > (int64_t{1} << 23)) return arg_error("rotary takes at most 2^23 tokens a call");
+  for (int k = 0; k < count; ++k) {
+    if (tensors[k].heads < 0 || tensors[k].heads > 65536) return arg_error("rotary takes at most 65536 heads");
+    if (tokens > 0 && tensors[k].heads > 0 && (!tensors[k].data || !tensors[k].out))
+      return arg_error("a required buffer pointer is NULL");
+  }
+  if (tokens == 0) return 0;
+  if (positions == nullptr) return arg_error("a required buffer pointer is NULL");
+  return launch_rotary(*spec, positions, positions_64, tokens, dtype, tensors, count,
+                       static_cast<hipStream_t>(stream));
+}

@@ -23,7 +23,7 @@ LIB_PATH = Path(os.environ.get("KVSSD_HIP_LIBRARY") or Path(__file__).resolve().
 LIB_PATH_OVERRIDDEN = bool(os.environ.get("KVSSD_HIP_LIBRARY"))
 # the sources the in-tree build comes from (absent in an installed copy)
 BUILD_SCRIPT = Path(__file__).resolve().parent.parent / "csrc" / "build.py"
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_F64 = 0, 1, 2, 3
 KERNEL_AUTO, KERNEL_GENERAL, KERNEL_MFMA, KERNEL_STAGED = 0, 1, 2, 3
@@ -65,6 +65,64 @@ class RecordLayout(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("bits", "block_tokens", "kv_heads", "head_dim", "group_size")]
 
 
+_P, _I32, _LL = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+
+
+class RotarySpec(ctypes.Structure):
+    """kvssd_rotary_spec (include/kvssd_hip.h)."""
+
+    _fields_ = [("frequencies", _P), ("magnitude", ctypes.c_double)] + [
+        (n, _I32) for n in ("head_dim", "rotary_dim", "interleaved", "inverse")
+    ]
+
+
+class Heads(ctypes.Structure):
+    """kvssd_heads."""
+
+    _fields_ = [("data", _P), ("out", _P)] + [
+        (n, _LL) for n in ("token_stride", "head_stride", "out_token_stride", "out_head_stride")
+    ] + [("heads", _I32), ("reserved", _I32)]
+
+
+class PagedCache(ctypes.Structure):
+    """kvssd_paged_cache."""
+
+    _fields_ = [
+        (n, _I32)
+        for n in ("bits", "kv_heads", "head_dim", "group_size", "num_pages", "page_tokens", "sequences", "max_pages")
+    ] + [
+        (n, _P)
+        for n in ("packed_k", "packed_v", "scales_k", "scales_v", "page_table", "lengths", "weights", "positions")
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """kvssd_paged_append_args."""
+
+    _fields_ = [
+        ("keys", Heads), ("values", Heads), ("query", Heads), ("tokens", _LL), ("offsets", _P),
+        ("first_positions", _P), ("rotary", ctypes.POINTER(RotarySpec)), ("lengths_out", _P), ("dtype", _I32),
+        ("reserved", _I32),
+    ]
+
+
+class PagedDecodeArgs(ctypes.Structure):
+    """kvssd_paged_decode_args."""
+
+    _fields_ = [
+        ("query", _P), ("out", _P), ("lse", _P), ("workspace", _P), ("workspace_bytes", ctypes.c_size_t),
+        ("sm_scale", ctypes.c_double), ("total_tokens", _LL),
+    ] + [(n, _I32) for n in ("max_length", "query_heads", "query_dtype", "out_query_dtype", "accumulate", "reserved")]
+
+
+class PagedEvictArgs(ctypes.Structure):
+    """kvssd_paged_evict_args."""
+
+    _fields_ = [(n, _I32) for n in ("budget", "sink", "recent", "reserved")] + [
+        (n, _P) for n in ("lengths_out", "weights_out", "positions_out", "workspace")
+    ] + [("workspace_bytes", ctypes.c_size_t)]
+
+
 # (name, restype, argtypes) for every entry point in include/kvssd_hip.h
 _VP, _SZ, _I, _I64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_int64
 SIGNATURES = {
@@ -90,6 +148,13 @@ SIGNATURES = {
     "kvssd_hip_vllm_encode": (_I, [_VP, _I, _I64, _I, _I, _VP, _VP, _VP, _SZ, _VP]),
     "kvssd_hip_vllm_decode": (_I, [_VP, _I64, _I, _I, ctypes.c_uint32, _I, _VP, _VP, _VP, _SZ, _VP]),
     "kvssd_hip_memcpy_h2d_async": (_I, [_VP, _VP, _SZ, _VP]),
+    # structures by address: ctypes.byref(s), or an address kept for many calls
+    "kvssd_hip_rotary": (_I, [_VP, _VP, _I, _I64, _I, _VP, _I, _VP]),
+    "kvssd_hip_paged_append": (_I, [_VP, _VP, _VP]),
+    "kvssd_hip_paged_decode_workspace_bytes": (_I, [_VP, _VP, ctypes.POINTER(_SZ)]),
+    "kvssd_hip_paged_decode": (_I, [_VP, _VP, _VP]),
+    "kvssd_hip_paged_evict_workspace_bytes": (_I, [_VP, _VP, ctypes.POINTER(_SZ)]),
+    "kvssd_hip_paged_evict": (_I, [_VP, _VP, _VP]),
     "kvssd_hip_read_probe": (_I, [_VP, _SZ, _VP, _SZ, _VP]),
     "kvssd_hip_last_error": (ctypes.c_char_p, []),
 }

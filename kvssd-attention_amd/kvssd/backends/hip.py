@@ -22,7 +22,8 @@ from collections.abc import Sequence
 import torch
 
 from .. import _native
-from .base import BackendAvailability, PackedBatch
+from .base import BackendAvailability, PackedBatch, PagedBatch
+from .paged import PreparedPagedDecode
 
 _device_state: dict[int, tuple[bool, str]] = {}
 
@@ -191,6 +192,40 @@ class HipAttentionBackend:
         if min(ids) < 0 or max(ids) >= num_blocks:
             raise ValueError(f"block ids must lie in [0, {num_blocks})")
         return torch.tensor(ids, dtype=torch.int32).pin_memory().to(device, non_blocking=True)
+
+    # ----------------------------------------------------------- paged ---
+    def run_paged(
+        self,
+        query: torch.Tensor,
+        batch: PagedBatch,
+        sm_scale: float,
+        out_dtype: torch.dtype | None = None,
+        accumulate: bool = False,
+        max_length: int = 0,
+        total_tokens: int = 0,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """Attention of one query per sequence, [sequences, query_heads, head_dim], over its pages: (out, lse).
+
+        ``out`` is fp32 unless ``out_dtype`` is the query's dtype.  A sequence of length 0 gives out = 0 and
+        lse = -inf.  ``accumulate`` adds each slot's attention weight, summed over the query heads, to
+        ``batch.weights``.  ``max_length`` and ``total_tokens``, the longest length and their sum where the caller
+        knows them (0: the page table's capacity), size the split over the sequences; lengths past them are answered
+        too."""
+        return PreparedPagedDecode(query, batch, sm_scale, out_dtype, accumulate, max_length, total_tokens, rows=1)(query)
+
+    def prepare_paged(
+        self,
+        query: torch.Tensor,
+        batch: PagedBatch,
+        sm_scale: float,
+        out_dtype: torch.dtype | None = None,
+        accumulate: bool = False,
+        max_length: int = 0,
+        total_tokens: int = 0,
+    ) -> PreparedPagedDecode:
+        """Every check and plan of ``run_paged`` done once; calling the result with a query of that shape, dtype and
+        device decodes over the batch's arrays as they are at the call (what a decode loop repeats)."""
+        return PreparedPagedDecode(query, batch, sm_scale, out_dtype, accumulate, max_length, total_tokens)
 
     # ----------------------------------------------------------- merge ---
     def merge_chunks(

@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from ..quant import unpack_codes
-from .base import BackendAvailability, PackedBatch
+from .base import BackendAvailability, PackedBatch, PagedBatch
 
 
 class ReferenceAttentionBackend:
@@ -46,3 +46,47 @@ class ReferenceAttentionBackend:
         lse = torch.logsumexp(scores, dim=-1)
         out = torch.einsum("ht,thd->hd", torch.softmax(scores, dim=-1), values[:, head_map])
         return out, lse
+
+    def run_paged(
+        self,
+        query: torch.Tensor,
+        batch: PagedBatch,
+        sm_scale: float,
+        out_dtype: torch.dtype | None = None,
+        accumulate: bool = False,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """Attention of one query per sequence over its pages, sequence by sequence (what
+        HipAttentionBackend.run_paged computes); see there for the arguments."""
+        batch.validate()
+        batch.validate_query(query)
+        if accumulate and batch.weights is None:
+            raise ValueError("accumulate needs a cache with weights")
+        page_tokens = batch.packed_k.shape[1]
+        outs, lses = [], []
+        for b, length in enumerate(batch.lengths.tolist()):
+            slots = torch.arange(max(0, min(length, batch.capacity)), device=query.device)
+            pages = batch.page_table[b].long()[slots // page_tokens]
+            slots = slots[(pages >= 0) & (pages < batch.packed_k.shape[0])]
+            rows = batch.page_table[b].long()[slots // page_tokens] * page_tokens + slots % page_tokens
+            one = PackedBatch(
+                *(t.flatten(0, 1)[rows].unsqueeze(0)
+                  for t in (batch.packed_k, batch.packed_v, batch.scales_k, batch.scales_v)),
+                torch.tensor([len(slots)], dtype=torch.int32, device=query.device), batch.bits, batch.group_size,
+            )
+            if len(slots) == 0:
+                outs.append(torch.zeros_like(query[b], dtype=torch.float32))
+                lses.append(torch.full((query.shape[1],), -torch.inf, device=query.device))
+                continue
+            out, lse = self.run(query[b], one, sm_scale)
+            outs.append(out)
+            lses.append(lse)
+            if accumulate:
+                mid = 1 << (batch.bits - 1)
+                keys = unpack_codes(one.packed_k[0], batch.bits, query.shape[2]).float() - mid
+                keys = keys * one.scales_k[0].float().repeat_interleave(batch.group_size, dim=-1)
+                grouped = query[b].float().reshape(keys.shape[1], -1, keys.shape[2])
+                scores = torch.matmul(grouped, keys.permute(1, 2, 0).contiguous()) * sm_scale
+                weights = torch.exp(scores - lse.reshape(*scores.shape[:2], 1)).sum((0, 1))
+                batch.weights[b, slots] += weights
+        out = torch.stack(outs)
+        return out.to(out_dtype or torch.float32), torch.stack(lses)

@@ -33,6 +33,7 @@ import torch
 from .attention import packed_attention, resolve_required
 from .backends import AttentionBackend, PackedBatch
 from .loader import AsyncBlockLoader
+from .paged import PagedKVCache
 from .records_hip import gather_records, raise_for_status
 from .selectors import AllBlocks, BlockSelector
 from .staging import HostRecords, RecordStager
@@ -161,6 +162,21 @@ class KVSSDPipeline:
     def release_resident(self, layers: Sequence[int] | None = None) -> None:
         for layer in list(self._resident) if layers is None else layers:
             self._resident.pop(layer, None)
+
+    def paged_cache(self, layer: int, *, spare_pages: int = 0, track_weights: bool = False) -> PagedKVCache:
+        """A resident layer as a paged cache of one sequence that can grow: its blocks copied into pages of
+        block_tokens tokens, with ``spare_pages`` free ones behind them."""
+        res = self._resident.get(layer)
+        if res is None:
+            raise ValueError(f"layer {layer} is not resident")
+        spec = self.store.spec
+        cache = PagedKVCache(
+            len(res.ids) + spare_pages, spec.block_tokens, spec.kv_heads, spec.head_dim, bits=spec.bits,
+            group_size=spec.group_size, track_weights=track_weights, device=self.device,
+            attention_backend=self.attention_backend,
+        )
+        cache.load(0, res.batch)
+        return cache
 
     def _table(self, res: _Resident, selected: list[int]) -> torch.Tensor | None:
         """Device block table for ``selected``; None when it is every row in order."""

@@ -1,0 +1,96 @@
+"""Rotary frequencies, and what the operator refuses (no GPU)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from kvssd import Rotary, RotaryScaling
+from kvssd.rotary import _overlaps_itself, refuse_grad, rotary_frequencies
+
+
+def test_plain_frequencies():
+    f = rotary_frequencies(8, 10000.0)
+    assert f == [1.0, 10000.0 ** -0.25, 10000.0 ** -0.5, 10000.0 ** -0.75]
+
+
+def test_scaled_frequencies():
+    plain = rotary_frequencies(128, 500000.0)
+    assert rotary_frequencies(128, 500000.0, RotaryScaling("linear", 4.0)) == [f / 4.0 for f in plain]
+    ntk = rotary_frequencies(128, 500000.0, RotaryScaling("ntk", 4.0))
+    # the first pair stays, the last is divided by the factor (64 bits: pow is good to a few 2^-53)
+    assert ntk[0] == plain[0] and ntk[-1] == pytest.approx(plain[-1] / 4.0, rel=1e-13)
+    for kind, low, high in (("yarn", 1.0, 32.0), ("wavelength", 1.0, 4.0)):
+        s = RotaryScaling(kind, 8.0, 8192)
+        got = rotary_frequencies(128, 500000.0, s)
+        assert s.bounds == (low, high)
+        turns = [8192 * f / (2 * math.pi) for f in plain]
+        for f, g, n in zip(plain, got, turns):
+            assert f / 8.0 * (1 - 1e-12) <= g <= f * (1 + 1e-12)
+            if n > high * 1.3:
+                assert g == pytest.approx(f, rel=1e-15)
+            if n < low / 1.3:
+                assert g == pytest.approx(f / 8.0, rel=1e-15)
+        assert all(a > b for a, b in zip(got, got[1:]))
+    assert RotaryScaling("yarn", 4.0).magnitude == 0.1 * math.log(4.0) + 1.0
+    assert RotaryScaling("linear", 4.0).magnitude == 1.0
+
+
+def test_a_ramp_that_is_a_step():
+    # a context so short that the ramp's ends meet: still a frequency per pair, all within a factor of 8
+    f = rotary_frequencies(4, 10000.0, RotaryScaling("yarn", 8.0, 1))
+    assert len(f) == 2 and all(0 < x <= 1 for x in f)
+
+
+@pytest.mark.parametrize(("args", "kwargs", "match"), [
+    ((64,), dict(rotary_dim=0), "even and between"),
+    ((64,), dict(rotary_dim=7), "even and between"),
+    ((64,), dict(rotary_dim=66), "even and between"),
+    ((63,), dict(), "even and between"),
+    ((2048,), dict(), "<= 1024"),
+    ((64,), dict(layout="pairs"), "unknown rotary layout"),
+    ((64,), dict(base=1.0), "base"),
+    ((64,), dict(base=float("nan")), "base"),
+    ((2,), dict(scaling=RotaryScaling("ntk", 2.0)), "ntk"),
+])
+def test_refused_layouts(args, kwargs, match):
+    with pytest.raises(ValueError, match=match):
+        Rotary(*args, device="cpu", **kwargs)
+
+
+@pytest.mark.parametrize(("args", "match"), [
+    (("cubic", 2.0), "unknown rotary scaling"),
+    (("linear", 0.5), "at least 1"),
+    (("linear", float("inf")), "at least 1"),
+    (("yarn", 2.0, 0), "positive"),
+    (("yarn", 2.0, 10, 4.0, 2.0), "low < high"),
+    (("yarn", 2.0, 10, 0.0), "low < high"),
+])
+def test_refused_scalings(args, match):
+    with pytest.raises(ValueError, match=match):
+        RotaryScaling(*args)
+
+
+def test_cpu_tensors_are_refused():
+    rot = Rotary(8, device="cpu")
+    with pytest.raises(ValueError, match="GPU"):
+        rot(torch.arange(3), torch.zeros(3, 1, 8))
+
+
+def test_gradients_are_refused_not_cut():
+    x = torch.zeros(2, requires_grad=True)
+    with pytest.raises(ValueError, match="no backward pass"):
+        refuse_grad(None, x)
+    with torch.no_grad():
+        refuse_grad(x)
+    refuse_grad(x.detach(), None)
+
+
+def test_tensors_that_hold_an_element_twice_are_seen():
+    t = torch.zeros(4, 6, 8)
+    assert not _overlaps_itself(t) and not _overlaps_itself(t.transpose(0, 1)) and not _overlaps_itself(t[:, ::2])
+    assert _overlaps_itself(t[:, :1].expand(4, 3, 8))
+    assert _overlaps_itself(torch.zeros(20).as_strided((3, 2, 8), (4, 2, 1)))
+    assert not _overlaps_itself(torch.zeros(0, 2, 8)) and not _overlaps_itself(t[:1].expand(1, 6, 8))
