@@ -26,10 +26,16 @@ int launch_paged_evict(const kvssd_paged_cache& c, const kvssd_paged_evict_args&
 
 // ------------------------------------------------------------ device side ---
 
+// *p for a wave-uniform p of memory that the launch does not write: a scalar load
+__device__ __forceinline__ int32_t uniform_load(const int32_t* p) {
+  typedef const __attribute__((address_space(4))) int32_t* constant_ptr;
+  return __builtin_amdgcn_readfirstlane(*(constant_ptr)(uintptr_t)p);
+}
+
 // Length of sequence b as every kernel takes it.
+__device__ __forceinline__ int clamp_length(int n, int capacity) { return n < 0 ? 0 : (n > capacity ? capacity : n); }
 __device__ __forceinline__ int paged_length(const int32_t* lengths, int b, int capacity) {
-  const int n = lengths[b];
-  return n < 0 ? 0 : (n > capacity ? capacity : n);
+  return clamp_length(lengths[b], capacity);
 }
 
 }  // namespace kvssd

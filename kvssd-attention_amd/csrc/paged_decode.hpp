@@ -9,47 +9,55 @@
 //
 // Work split.  A wave owns one kv head, up to 16 / GP of its query heads (GP:
 // scale groups per head, rounded up to a power of two; NT such head tiles) and
-// one run of a sequence's slots, 32 slots (a tile) at a time.  The waves of a
+// one run of a sequence's slots, 64 slots (a stage) at a time.  The waves of a
 // workgroup take neighbouring kv heads of the same run, whose rows lie side by
 // side in a page, so that whole cache lines are used.  Waves do not meet: each
 // leaves an unnormalised partial (O, m, l), which paged_merge.hip joins.
 //
-// QK (v_mfma_f32_16x16x32_f16, two per 32 dims and tile): rows = 16 tokens'
-//   codes, columns = (query head, group): the query masked to one group, so
-//   that a column's sum is one group's and its scale multiplies in 32 bits
-//   afterwards.  A code enters as the fp16 number 1 + c / 2^6 (INT4) or
-//   1 + c / 2^2 (two bit operations for a pair); the offset's share,
-//   -(1 + mid/2^6) sum q, is the accumulator's initial value.  The query is
-//   scaled by a power of two per head into fp16's range (exact for fp16 and
-//   bf16) and, with 32-bit queries, taken as a sum of two fp16 parts.
-// Softmax in the columns' lanes: a lane holds its (head, group)'s scores of 8
-//   slots; the groups' shares meet by lane exchanges within 8 lanes.  The
-//   running maximum is lazy: scores up to 2^6 above the reference are summed as
-//   they are (no wave-wide maximum per tile); where one exceeds that, all lanes
-//   take the new maximum and rescale.  The reference also holds the exponent of
-//   the largest value scale met, so that W = 2^(s - m) sv lies in fp16's normal
-//   range (at most 2^15) whatever the scales' size.
-// PV: rows = (head, group) weights W, columns = 16 column units of a V row, K =
-//   the tile's 32 slots.  The QK result's layout (lane: column (head, group),
-//   rows 4 (lane / 16) + i of both halves) is the A operand's layout if slots are
-//   taken in that order, so W needs no exchange; V's codes of two slots form an
-//   operand pair.  V codes enter as the exact numbers (c - mid) / 2^6: an offset
-//   taken out of the sums afterwards would cost a share of their precision that
-//   grows with the number of slots.  Of a unit's 16 rows those of its own group
-//   count.  Where 32-bit grade is asked for, W is a sum of two fp16 parts.
+// Copies.  A stage's codes go from memory straight to LDS (16 bytes a lane), one
+// stage ahead of the arithmetic, into the wave's own two buffers: 128 KB of a
+// CU in flight or in use without a register.  A row's 16-byte chunks are stored
+// in an order turned by the row's number, so that neither the key rows' nor the
+// value columns' reads meet in a bank.  Scales come through registers (one slot
+// a lane) and are laid out by group in LDS.
+//
+// QK (v_mfma_f32_16x16x32_f16): rows = 16 slots' codes, columns = (query head,
+//   group): the query masked to one group, so that a column's sum is one group's
+//   and its scale multiplies in 32 bits afterwards.  A code enters as the fp16
+//   number 1 + c / 2^6 (INT4) or 1 + c / 2^2 (a bit operation for a pair); the
+//   offset's share, -(1 + mid/2^6) sum q, is the accumulator's initial value.
+//   The query is scaled by a power of two per head into fp16's range (exact for
+//   fp16 and bf16) and, with 32-bit results, taken as a sum of two fp16 parts.
+//   Tile u's row r is slot 16 (r / 4) + 4 u + r % 4: a lane's results are then
+//   its (head, group)'s scores of the 16 slots 16 (lane / 16) + e.
+// Softmax in the columns' lanes; the groups' shares meet by lane exchanges
+//   within 8 lanes.  The running maximum is lazy: scores up to 2^6 above the
+//   reference are summed as they are (no wave-wide maximum per stage); where one
+//   exceeds that, all lanes take the new maximum and rescale.  The reference
+//   also holds the exponent of the largest value scale met, so that W =
+//   2^(s - m) sv lies in fp16's normal range (at most 2^15) whatever the scales'
+//   size.
+// PV: rows = (head, group) weights W, columns = 16 dims, K = 32 slots.  The QK
+//   results' lanes are the A operand's, so W needs no exchange; V's codes come
+//   transposed from LDS (ds_read_b64_tr_b4: a dim's codes of 16 slots a lane)
+//   and enter as the exact numbers (c - mid) / 2^6: an offset taken out of the
+//   sums afterwards would cost a share of their precision that grows with the
+//   number of slots.  Of a column's 16 rows those of its own group count.
+//   Where 32-bit grade is asked for, W is a sum of two fp16 parts.
 #pragma once
 
+#include <type_traits>
+
 #include "paged.hpp"
+#include "staged_ops.hpp"
 
 namespace kvssd {
 
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-typedef float float4v __attribute__((ext_vector_type(4)));
-
-constexpr int kTile = 32;        // slots of a tile
-constexpr int kDecodeWaves = 8;  // most waves of a workgroup
+constexpr int kTile = 64;        // slots of a stage
 constexpr int kMaxSplits = 1024;
+
+// waves of a workgroup: two stages of codes each fit the CU's LDS
+constexpr int decode_waves(int dp) { return dp == 256 ? 4 : 8; }
 
 struct PagedDecodeParams {
   kvssd_paged_cache c;
@@ -62,10 +70,10 @@ struct PagedDecodeParams {
   int64_t score_stride;
   int capacity, chunk, splits;  // slots of a run at least, runs of a sequence at most
   int group_splits;             // runs of a workgroup (waves beyond one per kv head)
-  int heads_of_group, head_groups;  // kv heads of a workgroup, workgroups over the kv heads
+  int group_units, groups_of_units;  // units (kv head, head tile) of a workgroup, workgroups over them
   int query_heads, gq, query_dtype, out_dtype;
-  int tiles, tile_sets;  // head tiles of a kv head, sets of NT
-  int gp_log2, groups;   // log2 of GP, groups per head
+  int tiles;             // head tiles of a kv head
+  int groups;            // scale groups per head
   float scale_log2;
 };
 
@@ -87,13 +95,64 @@ __device__ __forceinline__ void store_out(void* out, int dtype, int64_t at, floa
 }
 
 int launch_paged_merge(const PagedDecodeParams& p, hipStream_t stream);
-int launch_paged_int2(const PagedDecodeParams& p, int dp, int nt, bool precise, hipStream_t stream);
-int launch_paged_int4(const PagedDecodeParams& p, int dp, int nt, bool precise, hipStream_t stream);
+// dp: head_dim padded to 64, 128 or 256; gp: groups padded to a power of two
+template <int BITS, int DP>
+int launch_paged_dims(const PagedDecodeParams& p, int gp, bool precise, hipStream_t stream);
+template <>
+int launch_paged_dims<4, 64>(const PagedDecodeParams& p, int gp, bool precise, hipStream_t stream);
+template <>
+int launch_paged_dims<4, 128>(const PagedDecodeParams& p, int gp, bool precise, hipStream_t stream);
+template <>
+int launch_paged_dims<4, 256>(const PagedDecodeParams& p, int gp, bool precise, hipStream_t stream);
+template <>
+int launch_paged_dims<2, 64>(const PagedDecodeParams& p, int gp, bool precise, hipStream_t stream);
+template <>
+int launch_paged_dims<2, 128>(const PagedDecodeParams& p, int gp, bool precise, hipStream_t stream);
+template <>
+int launch_paged_dims<2, 256>(const PagedDecodeParams& p, int gp, bool precise, hipStream_t stream);
 
 // ------------------------------------------------------------------ kernel ---
 
-__device__ __forceinline__ uint32_t sub_pair(uint32_t w, half2v off) {
-  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, w) - off);
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+// v * a + b for an fp16 pair
+__device__ __forceinline__ uint32_t fma_pair(uint32_t v, _Float16 a, _Float16 b) {
+  const half2v r = __builtin_elementwise_fma(__builtin_bit_cast(half2v, v), half2v{a, a}, half2v{b, b});
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+// A word of 8 slots' transposed codes (nibble e: slot e) as PV operand pairs
+// (e, e + 4): INT4, the dim's (c - 8) / 64; INT2, (c - 2) / 4 of the nibble's
+// even (odd = 0) or odd dim.  Codes stay where they are in their half, at
+// 1 + c / F for the F of that place; one fused multiply-add takes out the 1 and
+// the offset and brings all to one F, exactly.
+template <int BITS>
+__device__ __forceinline__ u32x4 value_operand(uint32_t x, int odd, const Masks& k, uint32_t m01, uint32_t m23) {
+  const uint32_t y = x >> 8;
+  if constexpr (BITS == 4) {
+    const _Float16 f = 16.0f, fo = -16.125f, o = -1.125f;
+    return u32x4{fma_pair(ao(x, k.m03), f, fo), fma_pair(ao(x, k.m47), 1.0f, o), fma_pair(ao(y, k.m03), f, fo),
+                 fma_pair(ao(y, k.m47), 1.0f, o)};
+  } else if (odd == 0) {
+    const _Float16 f0 = 256.0f, o0 = -256.5f, f1 = 16.0f, o1 = -16.5f;
+    return u32x4{fma_pair(ao(x, m01), f0, o0), fma_pair(ao(x, k.m45), f1, o1), fma_pair(ao(y, m01), f0, o0),
+                 fma_pair(ao(y, k.m45), f1, o1)};
+  } else {
+    const _Float16 f0 = 64.0f, o0 = -64.5f, f1 = 4.0f, o1 = -4.5f;
+    return u32x4{fma_pair(ao(x, m23), f0, o0), fma_pair(ao(x, k.m67), f1, o1), fma_pair(ao(y, m23), f0, o0),
+                 fma_pair(ao(y, k.m67), f1, o1)};
+  }
+}
+
+// A word of key codes as QK operands, one (INT4) or two (INT2) slices
+template <int BITS>
+__device__ __forceinline__ u32x4 key_operand(uint32_t x, int odd, const Masks& k) {
+  if constexpr (BITS == 4) {
+    return u32x4{ao(x << 4, k.m47), ao(x, k.m47), ao(x >> 4, k.m47), ao(x >> 8, k.m47)};
+  } else {
+    if (odd == 0) return u32x4{ao(x << 8, k.m89), ao(x << 6, k.m89), ao(x << 4, k.m89), ao(x << 2, k.m89)};
+    return u32x4{ao(x, k.m89), ao(x >> 2, k.m89), ao(x >> 4, k.m89), ao(x >> 6, k.m89)};
+  }
 }
 
 template <int CTRL>
@@ -101,87 +160,217 @@ __device__ __forceinline__ float dpp_add(float v) {
   return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
 }
 
-__device__ __forceinline__ float query_value(const void* q, int dtype, int64_t at) {
-  if (dtype == KVSSD_DTYPE_F32) return static_cast<const float*>(q)[at];
-  if (dtype == KVSSD_DTYPE_F16) return static_cast<float>(static_cast<const _Float16*>(q)[at]);
-  return __builtin_bit_cast(float, static_cast<uint32_t>(static_cast<const uint16_t*>(q)[at]) << 16);
+// As dma16 / dma4 with a 64-bit address per lane.
+__device__ __forceinline__ void dma16_at(const uint8_t* src, uint32_t lds_dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_dst) : "memory");
+}
+__device__ __forceinline__ void dma4_at(const uint8_t* src, uint32_t lds_dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds_dst) : "memory");
 }
 
-// Codes, scales and slot validity of one tile in a lane's registers.
-template <int BITS, int DP>
-struct PagedTile {
-  static constexpr int kKeyWords = DP * BITS / 128;                       // a lane's quarter of a key row
-  static constexpr int kUnit = DP / 16;                                   // codes of a V column unit
-  static constexpr int kValueWords = kUnit * BITS > 32 ? kUnit * BITS / 32 : 1;  // (a unit below 32 bits: in one register)
-  uint32_t k[2][kKeyWords];
-  uint32_t v[8][kValueWords];
-  uint32_t s[4];  // lanes 0-31: the slot's key scales, 32-63: its value scales (8 fp16)
-  uint32_t live;  // bit e: slot tau(lane / 16, e) takes part
-};
+// N consecutive query values (16-byte aligned) in 32 bits
+template <int N>
+__device__ __forceinline__ void query_span(const void* q, int dtype, int64_t at, float* v) {
+  if (dtype == KVSSD_DTYPE_F32) {
+    __builtin_memcpy(v, __builtin_assume_aligned(static_cast<const float*>(q) + at, 16), 4 * N);
+    return;
+  }
+  uint32_t w[N / 2];
+  __builtin_memcpy(w, __builtin_assume_aligned(static_cast<const uint16_t*>(q) + at, 16), 2 * N);
+  if (dtype == KVSSD_DTYPE_F16) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i % 2 ? half_hi(w[i / 2]) : half_lo(w[i / 2]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __builtin_bit_cast(float, i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+  }
+}
 
-template <int BITS, int DP, int NT, bool PREC, bool UNI>
-__global__ __launch_bounds__(kDecodeWaves * kWave) void paged_decode_kernel(PagedDecodeParams p) {
-  using Tile = PagedTile<BITS, DP>;
-  constexpr int kSlices = DP / 32;  // QK products of a half tile
-  constexpr int kUnit = Tile::kUnit;
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// UNI: pages hold whole halves (32 slots) of a stage and rows whole 16-byte
+// chunks, so that a copy's rows have one uniform base; else every lane finds
+// its own row's address.
+template <int BITS, int DP, int GP, bool PREC, bool UNI>
+__global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(PagedDecodeParams p) {
+  constexpr int kWaves = decode_waves(DP);
+  constexpr int kRow = DP * BITS / 8;      // bytes of a (padded) row in LDS
+  constexpr int kChunks = kRow / 16;       // 16-byte chunks of a row; also the copies of a stage's keys or values
+  constexpr int kArray = kTile * kRow;
+  constexpr int kRowsOfCopy = kTile / kChunks;
+  constexpr int kSlices = DP / 32;         // QK products of 16 slots
+  constexpr int kSpan = DP / 4;            // dims of a lane in QK
+  constexpr int kCols = DP / 16;           // PV column tiles
   constexpr int kParts = PREC ? 2 : 1;
+  constexpr int NT = 1;
+  constexpr int kHeads = 16 / GP;          // query heads of a head tile
   constexpr float kF = kUnpackScale<BITS>;
   constexpr float kOff = kUnpackOffset<BITS>;
-  constexpr float kLazy = 6.0f;  // log2 units a score may exceed the reference by
-  __shared__ uint16_t scale_lds[kDecodeWaves][2][8][kTile];  // [keys, values][group][slot order]
+  constexpr float kLazy = 6.0f;            // log2 units a score may exceed the reference by
+  __shared__ __attribute__((aligned(1024))) uint8_t codes_lds[kWaves][2][2 * kArray];
+  __shared__ __attribute__((aligned(16))) uint16_t scale_lds[kWaves][2][GP][kTile];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int col = lane & 15, lg = lane >> 4;
-  const int group_splits = p.group_splits;
-  const int wg_splits = (p.splits + group_splits - 1) / group_splits;
-  const int seq = blockIdx.x / wg_splits;
-  const int split = (blockIdx.x % wg_splits) * group_splits + wave / p.heads_of_group;
-  const int kvh = (blockIdx.y / p.tile_sets) * p.heads_of_group + wave % p.heads_of_group;
-  const int set = blockIdx.y % p.tile_sets;
+  const int wg_splits = (p.splits + p.group_splits - 1) / p.group_splits;
+  // (quotients are formed in vector registers: back to scalars, as the copies' bases have to be)
+  const int seq = scalar(blockIdx.x / wg_splits);
+  const int split = scalar((blockIdx.x % wg_splits) * p.group_splits + wave / p.group_units);
+  const int unit = scalar(blockIdx.y * p.group_units + wave % p.group_units);
+  const int kvh = scalar(unit / p.tiles);
+  const int set = unit - kvh * p.tiles;
   const kvssd_paged_cache& c = p.c;
   if (split >= p.splits || kvh >= c.kv_heads) return;
-  const int length = paged_length(c.lengths, seq, p.capacity);
-  const int run = run_of(length, p.chunk, p.splits);
-  const int begin = split * run;  // < 2^31: splits * run < length + splits * (chunk + 32)
-  if (begin >= length && (split > 0 || p.splits > 1)) return;  // the merge knows which runs exist
+  const int length = clamp_length(uniform_load(c.lengths + seq), p.capacity);
+  const int run = scalar(run_of(length, p.chunk, p.splits));
+  const int begin = split * run;  // < 2^31: splits * run < length + splits * (chunk + 64)
+  if (begin >= length && p.splits > 1) return;  // the merge knows which runs exist
   const int end = min(length, begin + run);
 
-  const int d = c.head_dim, gs = c.group_size, gp_log2 = p.gp_log2;
-  const int gp = 1 << gp_log2, hpt = 16 >> gp_log2;  // heads of a tile
+  const int d = c.head_dim, gs = c.group_size;
   const int row_bytes = d * BITS / 8;
   const int64_t slot_bytes = static_cast<int64_t>(c.kv_heads) * row_bytes;
-  const int own_g = col & (gp - 1);
-  const int gq0 = set * NT * hpt;  // first query head of this wave within its kv head
+  const int64_t slot_scales = static_cast<int64_t>(c.kv_heads) * p.groups;
+  const int own_g = col & (GP - 1);
+  const int gq0 = set * NT * kHeads;  // first query head of this wave within its kv head
 
-  // ---- query operand, its scale and the accumulator's initial value
-  // dims of the lane in slice j: granule A (j < kSlices / pieces) and, in DP 256, granule B
-  half8 q[kParts][NT][kSlices];
+  // ---- copies of a stage
+  const uint8_t* pk = c.packed_k + static_cast<int64_t>(kvh) * row_bytes;
+  const uint8_t* pv = c.packed_v + static_cast<int64_t>(kvh) * row_bytes;
+  const uint16_t* sk = c.scales_k + static_cast<int64_t>(kvh) * p.groups;
+  const uint16_t* sv = c.scales_v + static_cast<int64_t>(kvh) * p.groups;
+  const int32_t* pages = c.page_table + static_cast<int64_t>(seq) * c.max_pages;
+  const int bt = c.page_tokens;
+  // a row's chunk i lies at place i ^ turned(row)
+  auto turned = [](int row) { return ((row / (256 / kRow)) ^ (row >> 4)) & (kChunks - 1); };
+  uint32_t copy_at[kChunks];  // of copy n: the lane's chunk, from its row's start (not UNI) or the copy's first row's
+#pragma unroll
+  for (int n = 0; n < kChunks; ++n) {
+    const int lr = lane / kChunks;
+    const int chunk = (lane % kChunks) ^ turned(n * kRowsOfCopy + lr);
+    const int byte = chunk * 16 < row_bytes ? chunk * 16 : 0;  // (padding: the row's start again)
+    copy_at[n] = UNI ? static_cast<uint32_t>(lr * slot_bytes) + byte : byte;
+  }
+  uint32_t scale_k[4], scale_v[4];  // of slot `lane` of the stage last issued
+  uint32_t live = 0;                // whether that slot takes part
+  auto load_scales = [&](const uint16_t* row, uint32_t* s) {
+    if (GP >= 4 && p.groups == 4) {
+      __builtin_memcpy(s, __builtin_assume_aligned(row, 8), 8);
+    } else if (GP == 2) {
+      __builtin_memcpy(s, __builtin_assume_aligned(row, 4), 4);
+    } else if (GP == 8 && p.groups == 8) {
+      __builtin_memcpy(s, __builtin_assume_aligned(row, 16), 16);
+    } else {
+#pragma unroll
+      for (int g = 0; g < GP; ++g) {
+        const uint32_t x = row[g < p.groups ? g : 0];
+        s[g / 2] = g % 2 ? s[g / 2] | x << 16 : x;
+      }
+    }
+  };
+  const uint32_t lds0 = lds_addr(codes_lds[wave][0]);
+  // the page of the next half to be issued, fetched one half ahead
+  int half_page = 0, half_off = 0;  // index into `pages`, slot within the page
+  if constexpr (UNI) {
+    half_page = scalar(begin / bt);
+    half_off = begin - half_page * bt;
+  }
+  int next_page[2] = {-1, -1}, next_off[2] = {0, 0};
+  auto fetch_pages = [&](int base) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      next_page[h] = base + 32 * h < end ? uniform_load(pages + half_page) : -1;
+      next_off[h] = half_off;
+      half_off += 32;
+      if (half_off == bt) {
+        half_off = 0;
+        ++half_page;
+      }
+    }
+  };
+  auto issue = [&](int base, int buf) {
+    const uint32_t dst = lds0 + buf * (2 * kArray);
+    if constexpr (UNI) {
+      int64_t row[2];
+      bool ok[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ok[h] = next_page[h] >= 0 && next_page[h] < c.num_pages;
+        row[h] = static_cast<int64_t>(ok[h] ? next_page[h] : 0) * bt + next_off[h];
+      }
+      const int64_t mine = (lane < 32 ? row[0] : row[1]) + (lane & 31);
+      load_scales(sk + mine * slot_scales, scale_k);
+      load_scales(sv + mine * slot_scales, scale_v);
+      live = base + lane < end && (lane < 32 ? ok[0] : ok[1]);
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) {
+        const int64_t at = (row[n * kRowsOfCopy / 32] + n * kRowsOfCopy % 32) * slot_bytes;
+        dma16<true>(pk + at, copy_at[n], dst + n * 1024);
+      }
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) {
+        const int64_t at = (row[n * kRowsOfCopy / 32] + n * kRowsOfCopy % 32) * slot_bytes;
+        dma16<true>(pv + at, copy_at[n], dst + kArray + n * 1024);
+      }
+    } else {
+      const int slot = base + lane;
+      int mine = -1;
+      if (slot < end) {
+        const int page = pages[slot / bt];
+        if (page >= 0 && page < c.num_pages) mine = page * bt + slot % bt;
+      }
+      live = mine >= 0;
+      const int64_t row = max(mine, 0);
+      load_scales(sk + row * slot_scales, scale_k);
+      load_scales(sv + row * slot_scales, scale_v);
+      if (row_bytes % 16 == 0) {
+#pragma unroll
+        for (int n = 0; n < kChunks; ++n) {
+          const int64_t at = static_cast<int64_t>(__shfl(static_cast<int>(row), n * kRowsOfCopy + lane / kChunks, kWave)) * slot_bytes + copy_at[n];
+          dma16_at(pk + at, dst + n * 1024);
+          dma16_at(pv + at, dst + kArray + n * 1024);
+        }
+      } else {  // INT2 rows of an odd number of 8-byte pieces: 4 bytes a lane
+        constexpr int kUnits = kRow / 4;
+        for (int n = 0; n < kUnits; ++n) {
+          const int r = n * (kWave / kUnits) + lane / kUnits, unit = lane % kUnits;
+          int byte = ((unit / 4) ^ turned(r)) * 16 + unit % 4 * 4;
+          byte = byte < row_bytes ? byte : 0;
+          const int64_t at = static_cast<int64_t>(__shfl(static_cast<int>(row), r, kWave)) * slot_bytes + byte;
+          dma4_at(pk + at, dst + n * 256);
+          dma4_at(pv + at, dst + kArray + n * 256);
+        }
+      }
+    }
+  };
+  if (begin < end) {
+    if constexpr (UNI) fetch_pages(begin);
+    issue(begin, 0);
+    if constexpr (UNI) fetch_pages(begin + kTile);
+  }
+
+  // ---- query operand, its scale and the accumulator's initial value (while the first stage arrives)
+  u32x4 q[kParts][NT][kSlices];
   float c_init[NT], s_factor[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int hh = gq0 + t * hpt + (col >> gp_log2);
-    const bool has = hh < p.gq && own_g < p.groups;
+    const int hh = gq0 + t * kHeads + col / GP;
     const int64_t q0 = (static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq + (hh < p.gq ? hh : 0)) * d;
-    float qv[kSlices][8];
+    float x[kSpan];
     float big = 0.0f;
+    constexpr int kPieces = DP == 256 ? 2 : 1, kPiece = kSpan / kPieces;
 #pragma unroll
-    for (int j = 0; j < kSlices; ++j)
+    for (int g = 0; g < kPieces; ++g) {
+      const int dim = g * 128 + lg * kPiece;
+      float* v = x + g * kPiece;
+      query_span<kPiece>(p.query, p.query_dtype, q0 + (dim < d ? dim : 0), v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        // dim of operand element (j, e): the codes' order in unpack_int4_f16 / unpack_int2_f16
-        int dim;
-        if constexpr (BITS == 4) {
-          const int in = (e >> 1) + (e & 1) * 4;
-          dim = DP == 64 ? lg * 16 + j * 8 + in : (j / 4) * 128 + lg * 32 + (j % 4) * 8 + in;
-        } else {
-          const int in = (j & 1) * 4 + (e >> 1) + (e & 1) * 8;
-          dim = DP == 64 ? lg * 16 + in : (j / 4) * 128 + lg * 32 + ((j % 4) / 2) * 16 + in;
-        }
-        const float x = dim < d ? query_value(p.query, p.query_dtype, q0 + dim) : 0.0f;
-        big = fmaxf(big, fabsf(x));
-        qv[j][e] = has && dim < d && dim / gs == own_g ? x : 0.0f;
-      }
+      for (int i = 0; i < kPiece; ++i) big = fmaxf(big, fabsf(v[i]));
+      const bool mine = hh < p.gq && dim < d && dim / gs == own_g;
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) v[i] = mine ? v[i] : 0.0f;
+    }
     big = fmaxf(big, __shfl_xor(big, 16, kWave));
     big = fmaxf(big, __shfl_xor(big, 32, kWave));
     int ex = static_cast<int>((__builtin_bit_cast(uint32_t, big) >> 23) & 255u);
@@ -194,15 +383,18 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void paged_decode_kernel(Page
 #pragma unroll
     for (int j = 0; j < kSlices; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = qv[j][e] * scale_up;
-        const _Float16 hi = static_cast<_Float16>(x);
-        q[0][t][j][e] = hi;
-        sum += static_cast<float>(hi);
+      for (int w = 0; w < 4; ++w) {
+        // the codes' order in key_operand: pairs (i, i + 4) of a word's 8, (i, i + 8) of its 16
+        const int lo = BITS == 4 ? j * 8 + w : j / 2 * 16 + j % 2 * 4 + w;
+        const float a = x[lo] * scale_up, b = x[lo + (BITS == 4 ? 4 : 8)] * scale_up;
+        const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
+        q[0][t][j][w] = pack_half2(ah, bh);
+        sum += static_cast<float>(ah) + static_cast<float>(bh);
         if constexpr (PREC) {
-          const _Float16 lo = static_cast<_Float16>(x - static_cast<float>(hi));
-          q[kParts - 1][t][j][e] = lo;
-          sum += static_cast<float>(lo);
+          const _Float16 al = static_cast<_Float16>(a - static_cast<float>(ah));
+          const _Float16 bl = static_cast<_Float16>(b - static_cast<float>(bh));
+          q[kParts - 1][t][j][w] = pack_half2(al, bl);
+          sum += static_cast<float>(al) + static_cast<float>(bl);
         }
       }
     sum += __shfl_xor(sum, 16, kWave);
@@ -210,192 +402,90 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void paged_decode_kernel(Page
     c_init[t] = -kOff * sum;
   }
 
-  // ---- where the lane's loads lie within a slot's rows (units past head_dim read from the row's start)
-  const uint8_t* pk = c.packed_k + static_cast<int64_t>(kvh) * row_bytes;
-  const uint8_t* pv = c.packed_v + static_cast<int64_t>(kvh) * row_bytes;
-  int k_at[DP == 256 ? 2 : 1];
-  if constexpr (DP == 64) {
-    k_at[0] = lg * 16 < d ? lg * 2 * BITS : 0;
-  } else {
+  // ---- where the lane reads a stage's codes
+  int key_at[4];  // tile u: slot 16 (col / 4) + 4 u + col % 4 (and, in DP 256, chunks kChunks / 2 on)
 #pragma unroll
-    for (int g = 0; g < DP / 128; ++g) k_at[g] = g * 128 + lg * 32 < d ? (g * 128 + lg * 32) * BITS / 8 : 0;
+  for (int u = 0; u < 4; ++u) {
+    const int slot = 16 * (col / 4) + 4 * u + col % 4;
+    constexpr int kLaneBytes = (DP == 256 ? 128 : DP) * BITS / 32;  // of a lane's piece: 16, 8 or 4
+    key_at[u] = slot * kRow + ((lg * kLaneBytes / 16) ^ turned(slot)) * 16 + lg * kLaneBytes % 16;
   }
-  const int v_at = col * kUnit < d ? col * kUnit * BITS / 8 : 0;
-  const uint16_t* scales = (lane < 32 ? c.scales_k : c.scales_v) + static_cast<int64_t>(kvh) * p.groups;
-  const int64_t slot_scales = static_cast<int64_t>(c.kv_heads) * p.groups;
-  const int32_t* pages = c.page_table + static_cast<int64_t>(seq) * c.max_pages;
-  const int bt = c.page_tokens;
+  const int value_turn = turned(lane);  // slot 16 lg + col
+  const int value_at = kArray + lane * kRow;
+  uint32_t zero = 0;
+  asm("" : "+v"(zero));
+  const Masks masks = make_masks(zero);
+  const uint32_t m01 = 0x00030003u | zero, m23 = 0x000C000Cu | zero;
 
-  auto load_key = [&](const uint8_t* row, uint32_t* k) {
-    if constexpr (DP == 64) {
-      __builtin_memcpy(k, __builtin_assume_aligned(row + k_at[0], 4 * Tile::kKeyWords), 4 * Tile::kKeyWords);
-    } else {
-#pragma unroll
-      for (int g = 0; g < DP / 128; ++g)
-        __builtin_memcpy(k + g * BITS, __builtin_assume_aligned(row + k_at[g], 4 * BITS), 4 * BITS);
-    }
-  };
-  auto load_value = [&](const uint8_t* row, uint32_t* v) {
-    constexpr int kBytes = kUnit * BITS / 8;
-    if constexpr (kBytes >= 4) {
-      __builtin_memcpy(v, __builtin_assume_aligned(row + v_at, kBytes), kBytes);
-    } else if constexpr (kBytes == 2) {
-      v[0] = *reinterpret_cast<const uint16_t*>(row + v_at);
-    } else {
-      v[0] = row[v_at];
-    }
-  };
-  auto load_scales = [&](const uint16_t* row, uint32_t* s) {
-    if (p.groups == 4) {
-      __builtin_memcpy(s, __builtin_assume_aligned(row, 8), 8);
-    } else if (p.groups == 2) {
-      __builtin_memcpy(s, __builtin_assume_aligned(row, 4), 4);
-    } else if (p.groups == 8) {
-      __builtin_memcpy(s, __builtin_assume_aligned(row, 16), 16);
-    } else {
-#pragma unroll
-      for (int g = 0; g < 8; ++g)
-        if (g < p.groups) {
-          const uint32_t x = row[g];
-          s[g / 2] = g % 2 ? s[g / 2] | x << 16 : x;
-        }
-    }
-  };
-
-  // slot of the tile that operand element e of this lane stands for
-  auto tau = [&](int e) { return (e < 4 ? 0 : 12) + 4 * lg + e; };
-
-  // Every load of a tile.  UNI: pages of whole tiles, so that a tile lies in one page.
-  auto load_tile = [&](int base, Tile& tile) {
-    uint32_t live = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) live |= (base + tau(e) < end ? 1u : 0u) << e;
-    if constexpr (UNI) {
-      int page = pages[base / bt];
-      if (page < 0 || page >= c.num_pages) {
-        page = 0;
-        live = 0;
-      }
-      const int64_t row0 = static_cast<int64_t>(page) * bt + base % bt;
-      const uint8_t* kb = pk + row0 * slot_bytes;
-      const uint8_t* vb = pv + row0 * slot_bytes;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) load_key(kb + (16 * u + col) * static_cast<int>(slot_bytes), tile.k[u]);
-      load_scales(scales + (row0 + (lane & 31)) * slot_scales, tile.s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) load_value(vb + tau(e) * static_cast<int>(slot_bytes), tile.v[e]);
-    } else {
-      const int slot = base + (lane & 31);
-      int row = -1;
-      if (slot < end) {
-        const int page = pages[slot / bt];
-        if (page >= 0 && page < c.num_pages) row = page * bt + slot % bt;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        load_key(pk + static_cast<int64_t>(max(__shfl(row, 16 * u + col, kWave), 0)) * slot_bytes, tile.k[u]);
-      load_scales(scales + static_cast<int64_t>(max(row, 0)) * slot_scales, tile.s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int r = __shfl(row, tau(e), kWave);
-        if (r < 0) live &= ~(1u << e);
-        load_value(pv + static_cast<int64_t>(max(r, 0)) * slot_bytes, tile.v[e]);
-      }
-    }
-    tile.live = live;
-  };
-
-  float4v acc[NT][kUnit];
+  f32x4 acc[NT][kCols];
   float m_ref[NT], l[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     m_ref[t] = -INFINITY;
     l[t] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) acc[t][i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < kCols; ++i) acc[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
   int w_exp = -32;  // W = 2^(s - m_ref) sv, m_ref = maximum + w_exp: sv < 2^(w_exp + 9)
   bool first = true;
 
-  auto compute = [&](int base, const Tile& tile) {
-    // scales into the lanes that use them: [group][lg][e]
-    {
-      const int x = lane & 31;
-      const int at = (x & 12) * 2 + (x & 3) + (x & 16) / 4;  // 8 (x % 16 / 4) + x % 4 + 4 (x / 16)
-      uint16_t(*dst)[kTile] = scale_lds[wave][lane >> 5];
-      __builtin_amdgcn_wave_barrier();
+  auto compute = [&](int base, int buf, uint64_t live_mask, auto ragged_tag) {
+    constexpr bool kRagged = decltype(ragged_tag)::value;
+    const uint8_t* stage = codes_lds[wave][buf];
+    const uint32_t mask16 = static_cast<uint32_t>(live_mask >> (16 * lg)) & 0xFFFFu;  // slots 16 lg + e
+    uint32_t skw[8], svw[8];
+    __builtin_memcpy(skw, __builtin_assume_aligned(&scale_lds[wave][0][own_g][16 * lg], 16), 32);
+    __builtin_memcpy(svw, __builtin_assume_aligned(&scale_lds[wave][1][own_g][16 * lg], 16), 32);
+    if constexpr (kRagged) {  // value scales of slots that take no part may be anything: 0 (codes are always finite)
 #pragma unroll
-      for (int g = 0; g < 8; ++g)
-        if (g < p.groups) dst[g][at] = static_cast<uint16_t>(tile.s[g / 2] >> (16 * (g % 2)));
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    }
-    const int g_read = own_g < p.groups ? own_g : 0;
-    uint32_t skw[4], svw[4];
-    __builtin_memcpy(skw, __builtin_assume_aligned(&scale_lds[wave][0][g_read][8 * lg], 16), 16);
-    __builtin_memcpy(svw, __builtin_assume_aligned(&scale_lds[wave][1][g_read][8 * lg], 16), 16);
-    const bool ragged = !__all(tile.live == 255u);
-    if (ragged) {  // value scales of slots that take no part may be anything: 0 (codes are always finite)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (!(tile.live >> e & 1u)) svw[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+      for (int e = 0; e < 16; ++e)
+        if (!(mask16 >> e & 1u)) svw[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
     }
     // ---- scores
-    float4v s_acc[NT][2];
+    f32x4 s_acc[NT][4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      half8 a[kSlices];
+    for (int u = 0; u < 4; ++u) {
+      uint32_t kw[kSpan * BITS / 32];
+      constexpr int kBytes = (DP == 256 ? 128 : DP) * BITS / 32;
+      __builtin_memcpy(kw, __builtin_assume_aligned(stage + key_at[u], kBytes), kBytes);
+      if constexpr (DP == 256)
+        __builtin_memcpy(kw + kBytes / 4, __builtin_assume_aligned(stage + (key_at[u] ^ (kRow / 2)), kBytes), kBytes);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s_acc[t][u] = f32x4{c_init[t], c_init[t], c_init[t], c_init[t]};
 #pragma unroll
       for (int j = 0; j < kSlices; ++j) {
-        uint32_t w[8];
-        if constexpr (BITS == 4) {
-          unpack_int4_f16(tile.k[u][j], w);
-          __builtin_memcpy(&a[j], w, 16);
-        } else if (j % 2 == 0) {
-          unpack_int2_f16(tile.k[u][j / 2], w);
-          __builtin_memcpy(&a[j], w, 16);
-          __builtin_memcpy(&a[j + 1], w + 4, 16);
-        }
-      }
+        const u32x4 a = BITS == 4 ? key_operand<BITS>(kw[j], 0, masks) : key_operand<BITS>(kw[j / 2], j % 2, masks);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float4v s = {c_init[t], c_init[t], c_init[t], c_init[t]};
-#pragma unroll
-        for (int j = 0; j < kSlices; ++j) {
-          s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[j], q[0][t][j], s, 0, 0, 0);
-          if constexpr (PREC) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[j], q[kParts - 1][t][j], s, 0, 0, 0);
+        for (int t = 0; t < NT; ++t) {
+          s_acc[t][u] = mfma16(a, q[0][t][j], s_acc[t][u]);
+          if constexpr (PREC) s_acc[t][u] = mfma16(a, q[kParts - 1][t][j], s_acc[t][u]);
         }
-        s_acc[t][u] = s;
       }
     }
-    // ---- V operands are formed per column unit below; weights first
     uint32_t sv_top;
     {
       typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-      u16x2 m = __builtin_elementwise_max(__builtin_bit_cast(u16x2, svw[0] & 0x7FFF7FFFu), __builtin_bit_cast(u16x2, svw[1] & 0x7FFF7FFFu));
-      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, svw[2] & 0x7FFF7FFFu));
-      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, svw[3] & 0x7FFF7FFFu));
+      u16x2 m = __builtin_bit_cast(u16x2, svw[0] & 0x7FFF7FFFu);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, svw[i] & 0x7FFF7FFFu));
       sv_top = m[0] > m[1] ? m[0] : m[1];
     }
-    float s2[NT][8];  // scores over s_factor, summed over the groups
-    float tv[NT][8];
+    float s2[NT][16];  // scores over s_factor, summed over the groups
     bool over = static_cast<int>(sv_top >> 10) - 23 > w_exp;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float top = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const _Float16 sk = __builtin_bit_cast(half2v, skw[e / 2])[e % 2];
-        float x = s_acc[t][e / 4][e % 4] * static_cast<float>(sk);
-        if (own_g >= p.groups) x = 0.0f;
-        if (gp_log2 > 0) x = dpp_add<0xB1>(x);
-        if (gp_log2 > 1) x = dpp_add<0x4E>(x);
-        if (gp_log2 > 2) x = dpp_add<0x141>(x);
-        if (ragged && !(tile.live >> e & 1u)) x = -INFINITY;
+      for (int e = 0; e < 16; ++e) {
+        float x = s_acc[t][e / 4][e % 4] * static_cast<float>(__builtin_bit_cast(half2v, skw[e / 2])[e % 2]);
+        if constexpr (GP > 1) x = dpp_add<0xB1>(x);
+        if constexpr (GP > 2) x = dpp_add<0x4E>(x);
+        if constexpr (GP > 4) x = dpp_add<0x141>(x);
+        if (kRagged && !(mask16 >> e & 1u)) x = -INFINITY;
         s2[t][e] = x;
-        tv[t][e] = __builtin_fmaf(x, s_factor[t], -m_ref[t]);
-        if (ragged && !(tile.live >> e & 1u)) tv[t][e] = -INFINITY;
-        top = fmaxf(top, tv[t][e]);
+        // (s_factor is negative or zero for a scale that is: the mask stays a mask below)
+        const float s = kRagged && !(mask16 >> e & 1u) ? -INFINITY : __builtin_fmaf(x, s_factor[t], -m_ref[t]);
+        top = fmaxf(top, s);
       }
       over = over || top > kLazy - static_cast<float>(w_exp);
     }
@@ -409,13 +499,12 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void paged_decode_kernel(Page
       for (int t = 0; t < NT; ++t) {
         float top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (!ragged || (tile.live >> e & 1u)) top = fmaxf(top, s2[t][e] * s_factor[t]);
+        for (int e = 0; e < 16; ++e)
+          if (!kRagged || (mask16 >> e & 1u)) top = fmaxf(top, s2[t][e] * s_factor[t]);
         top = fmaxf(top, __shfl_xor(top, 16, kWave));
         top = fmaxf(top, __shfl_xor(top, 32, kWave));
         const float m_old = m_ref[t] - static_cast<float>(w_exp);
-        const float m_new = fmaxf(first ? -INFINITY : m_old, top);
-        const float ref = m_new + static_cast<float>(e_new);
+        const float ref = fmaxf(first ? -INFINITY : m_old, top) + static_cast<float>(e_new);
         const float alpha = first ? 0.0f : (ref == m_ref[t] ? 1.0f : exp2f(m_ref[t] - ref));
         m_ref[t] = ref;
         if (!first) {
@@ -424,13 +513,8 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void paged_decode_kernel(Page
           for (int i = 0; i < 4; ++i) {
             const float a = __shfl(alpha, 4 * lg + i, kWave);
 #pragma unroll
-            for (int k = 0; k < kUnit; ++k) acc[t][k][i] *= a;
+            for (int k = 0; k < kCols; ++k) acc[t][k][i] *= a;
           }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          tv[t][e] = __builtin_fmaf(s2[t][e], s_factor[t], -ref);
-          if (ragged && !(tile.live >> e & 1u)) tv[t][e] = -INFINITY;
         }
       }
       w_exp = e_new;
@@ -439,113 +523,114 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void paged_decode_kernel(Page
     if (p.scores != nullptr) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int hh = gq0 + t * hpt + (col >> gp_log2);
+        const int hh = gq0 + t * kHeads + col / GP;
         if (own_g == 0 && hh < p.gq) {
-          float* dst = p.scores + (static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq + hh) * p.score_stride + base + 4 * lg;
+          float* dst = p.scores + (static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq + hh) * p.score_stride + base + 16 * lg;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float4v v;
+          for (int u = 0; u < 4; ++u) {
+            f32x4 v;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              v[i] = ragged && !(tile.live >> (4 * u + i) & 1u) ? -INFINITY : s2[t][4 * u + i] * s_factor[t];
-            *reinterpret_cast<float4v*>(dst + 16 * u) = v;
+              v[i] = kRagged && !(mask16 >> (4 * u + i) & 1u) ? -INFINITY : s2[t][4 * u + i] * s_factor[t];
+            *reinterpret_cast<f32x4*>(dst + 4 * u) = v;
           }
         }
       }
     }
-    half8 w[kParts][NT];
+    // ---- weights: pairs (e, e + 4) of each step's 8 slots, the order of the values' pairs
+    u32x4 w[kParts][NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float sum = 0.0f;
+      float x[16];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float pe = __builtin_amdgcn_exp2f(tv[t][e]);
+      for (int e = 0; e < 16; ++e) {
+        const float tv = kRagged && !(mask16 >> e & 1u) ? -INFINITY : __builtin_fmaf(s2[t][e], s_factor[t], -m_ref[t]);
+        const float pe = __builtin_amdgcn_exp2f(tv);
         sum += pe;
-        const float x = pe * static_cast<float>(__builtin_bit_cast(half2v, svw[e / 2])[e % 2]);
-        const _Float16 hi = static_cast<_Float16>(x);
-        w[0][t][e] = hi;
-        if constexpr (PREC) w[kParts - 1][t][e] = static_cast<_Float16>(x - static_cast<float>(hi));
+        x[e] = pe * static_cast<float>(__builtin_bit_cast(half2v, svw[e / 2])[e % 2]);
+        // one product in 32 bits for both parts: a first part rounded straight from the factors (v_fma_mixlo_f16)
+        // may be the other of its two neighbours, and the parts' sum then a step of it off
+        if constexpr (PREC) asm("" : "+v"(x[e]));
       }
       l[t] += sum;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float a = x[8 * s + k], b = x[8 * s + k + 4];
+          const half2v hi = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+          w[0][t][s][k] = __builtin_bit_cast(uint32_t, hi);
+          if constexpr (PREC) {
+            const half2v lo = {static_cast<_Float16>(a - static_cast<float>(hi[0])),
+                               static_cast<_Float16>(b - static_cast<float>(hi[1]))};
+            w[kParts - 1][t][s][k] = __builtin_bit_cast(uint32_t, lo);
+          }
+        }
     }
-    // ---- weights times values
-    const half2v off = {static_cast<_Float16>(kOff), static_cast<_Float16>(kOff)};
-    constexpr int kCodes = kUnit < 16 / BITS ? kUnit : 16 / BITS;  // codes of a 16-bit piece of a unit
+    // ---- weights times values: 8 bytes of a row a read, 16 (INT4) or 32 (INT2) dims
 #pragma unroll
-    for (int piece = 0; piece < kUnit / kCodes; ++piece) {
-      uint32_t b[kCodes][4];
+    for (int r = 0; r < kRow / 8; ++r) {
+      const i32x2 x = lds_read_tr4(stage, value_at + (((r / 2) ^ value_turn) * 16) + r % 2 * 8);
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const uint32_t x0 = tile.v[2 * m][piece / 2], x1 = tile.v[2 * m + 1][piece / 2];
-        uint32_t y;
-        if constexpr (kUnit * BITS >= 32) {
-          y = __builtin_amdgcn_perm(x1, x0, piece % 2 ? 0x07060302u : 0x05040100u);
-        } else {
-          y = x0 | (x1 << 16);
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int odd = 0; odd < (BITS == 4 ? 1 : 2); ++odd) {
+          const u32x4 b = value_operand<BITS>(static_cast<uint32_t>(x[s]), odd, masks, m01, m23);
+          const int tile = BITS == 4 ? r : 2 * r + odd;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            acc[t][tile] = mfma16(w[0][t][s], b, acc[t][tile]);
+            if constexpr (PREC) acc[t][tile] = mfma16(w[kParts - 1][t][s], b, acc[t][tile]);
+          }
         }
-        uint32_t u[8];
-        if constexpr (BITS == 4) unpack_int4_f16(y, u);
-        else unpack_int2_f16(y, u);
-#pragma unroll
-        for (int k = 0; k < kCodes; ++k) b[k][m] = sub_pair(u[k], off);
-      }
-#pragma unroll
-      for (int k = 0; k < kCodes; ++k) {
-        half8 bv;
-        __builtin_memcpy(&bv, b[k], 16);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          float4v& o = acc[t][piece * kCodes + k];
-          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[0][t], bv, o, 0, 0, 0);
-          if constexpr (PREC) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[kParts - 1][t], bv, o, 0, 0, 0);
-        }
-      }
     }
   };
 
-  if (begin < end) {
-    // two tiles' registers: one is loaded while the other is worked on
-    const int last = begin + (end - begin - 1) / kTile * kTile;
-    Tile a, b;
-    load_tile(begin, a);
-    for (int base = begin; base <= last; base += 2 * kTile) {
-      load_tile(min(base + kTile, last), b);
-      compute(base, a);
-      if (base + kTile > last) break;
-      load_tile(min(base + 2 * kTile, last), a);
-      compute(base + kTile, b);
+  int buf = 0;
+  for (int base = begin; base < end; base += kTile, buf ^= 1) {
+    // the stage's copies (and scales) have landed, and nothing reads the buffer that the next one goes to
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int g = 0; g < GP; ++g) {
+      scale_lds[wave][0][g][lane] = static_cast<uint16_t>(g < p.groups ? scale_k[g / 2] >> (16 * (g % 2)) : 0u);
+      scale_lds[wave][1][g][lane] = static_cast<uint16_t>(g < p.groups ? scale_v[g / 2] >> (16 * (g % 2)) : 0u);
     }
+    const uint64_t live_mask = __ballot(live != 0);
+    if (base + kTile < end) {
+      issue(base + kTile, buf ^ 1);
+      if constexpr (UNI) fetch_pages(base + 2 * kTile);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (live_mask == ~0ull) compute(base, buf, live_mask, std::false_type{});
+    else compute(base, buf, live_mask, std::true_type{});
+    __builtin_amdgcn_wave_barrier();
   }
 
   // ---- this run's partial, or the result where a sequence has one run
   const bool whole = p.splits == 1;
+  const int64_t head0 = static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq;
+  const int64_t part0 = (static_cast<int64_t>(seq) * p.splits + split) * p.query_heads + kvh * p.gq;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     float lt = l[t] + __shfl_xor(l[t], 16, kWave);
     lt += __shfl_xor(lt, 32, kWave);
-    const int unit_g = col * kUnit / gs;  // group of this lane's column unit
-    const int64_t head0 = static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq;
-    const int64_t part0 = (static_cast<int64_t>(seq) * p.splits + split) * p.query_heads + kvh * p.gq;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 4 * lg + i;
-      const int hh = gq0 + t * hpt + (r >> gp_log2);
+      const int hh = gq0 + t * kHeads + r / GP;
       const float l_row = __shfl(lt, r, kWave);
-      if ((r & (gp - 1)) != unit_g || hh >= p.gq || col * kUnit >= d) continue;
-      if (whole) {
-        const float inv = l_row == 0.0f ? 0.0f : kF / l_row;
+      const float inv = l_row == 0.0f ? 0.0f : kF / l_row;
 #pragma unroll
-        for (int k = 0; k < kUnit; ++k)
-          store_out(p.out, p.out_dtype, (head0 + hh) * d + col * kUnit + k, l_row == 0.0f ? 0.0f : acc[t][k][i] * inv);
-      } else {
-        float* o = p.part_o + (part0 + hh) * d + col * kUnit;
-#pragma unroll
-        for (int k = 0; k < kUnit; k += 4)
-          *reinterpret_cast<float4v*>(o + k) =
-              float4v{kF * acc[t][k][i], kF * acc[t][k + 1][i], kF * acc[t][k + 2][i], kF * acc[t][k + 3][i]};
+      for (int k = 0; k < kCols; ++k) {
+        const int dim = BITS == 4 ? 16 * k + col : 32 * (k / 2) + 2 * col + k % 2;
+        if (hh >= p.gq || dim >= d || dim / gs != (r & (GP - 1))) continue;
+        if (whole) store_out(p.out, p.out_dtype, (head0 + hh) * d + dim, l_row == 0.0f ? 0.0f : acc[t][k][i] * inv);
+        else p.part_o[(part0 + hh) * d + dim] = kF * acc[t][k][i];
       }
     }
-    const int hh = gq0 + t * hpt + (col >> gp_log2);
+    const int hh = gq0 + t * kHeads + col / GP;
     if (lg == 0 && own_g == 0 && hh < p.gq) {
       if (whole) {
         p.lse[head0 + hh] = lt == 0.0f ? -INFINITY : kLn2 * (m_ref[t] + log2f(lt));
@@ -557,30 +642,24 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void paged_decode_kernel(Page
   }
 }
 
-template <int BITS, int DP, int NT, bool PREC>
+template <int BITS, int DP, int GP, bool PREC>
 int launch_paged_kernel(const PagedDecodeParams& p, hipStream_t stream) {
   const int wg_splits = (p.splits + p.group_splits - 1) / p.group_splits;
-  const dim3 grid(static_cast<unsigned>(p.c.sequences) * wg_splits, p.head_groups * p.tile_sets);
-  const dim3 block(p.heads_of_group * p.group_splits * kWave);
-  if (p.c.page_tokens % kTile == 0)
-    hipLaunchKernelGGL((paged_decode_kernel<BITS, DP, NT, PREC, true>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((paged_decode_kernel<BITS, DP, NT, PREC, false>), grid, block, 0, stream, p);
+  const dim3 grid(static_cast<unsigned>(p.c.sequences) * wg_splits, p.groups_of_units);
+  const dim3 block(p.group_units * p.group_splits * kWave);
+  if constexpr (DP * BITS >= 256) {
+    if (p.c.page_tokens % 32 == 0 && p.c.head_dim * BITS % 128 == 0) {
+      hipLaunchKernelGGL((paged_decode_kernel<BITS, DP, GP, PREC, true>), grid, block, 0, stream, p);
+      return hip_status(hipGetLastError(), "paged_decode launch");
+    }
+  }
+  hipLaunchKernelGGL((paged_decode_kernel<BITS, DP, GP, PREC, false>), grid, block, 0, stream, p);
   return hip_status(hipGetLastError(), "paged_decode launch");
 }
 
-template <int BITS>
-int launch_paged_bits(const PagedDecodeParams& p, int dp, int nt, bool precise, hipStream_t stream) {
-  if (dp == 64) {
-    if (nt == 1) return precise ? launch_paged_kernel<BITS, 64, 1, true>(p, stream) : launch_paged_kernel<BITS, 64, 1, false>(p, stream);
-    return precise ? launch_paged_kernel<BITS, 64, 2, true>(p, stream) : launch_paged_kernel<BITS, 64, 2, false>(p, stream);
-  }
-  if (dp == 128) {
-    if (nt == 1) return precise ? launch_paged_kernel<BITS, 128, 1, true>(p, stream) : launch_paged_kernel<BITS, 128, 1, false>(p, stream);
-    return precise ? launch_paged_kernel<BITS, 128, 2, true>(p, stream) : launch_paged_kernel<BITS, 128, 2, false>(p, stream);
-  }
-  if (nt == 1) return precise ? launch_paged_kernel<BITS, 256, 1, true>(p, stream) : launch_paged_kernel<BITS, 256, 1, false>(p, stream);
-  return precise ? launch_paged_kernel<BITS, 256, 2, true>(p, stream) : launch_paged_kernel<BITS, 256, 2, false>(p, stream);
+template <int BITS, int DP, int GP>
+int launch_paged_shape(const PagedDecodeParams& p, bool precise, hipStream_t stream) {
+  return precise ? launch_paged_kernel<BITS, DP, GP, true>(p, stream) : launch_paged_kernel<BITS, DP, GP, false>(p, stream);
 }
 
 }  // namespace kvssd

@@ -1,0 +1,12 @@
+// INT4 instances of the paged decode kernel, head_dim up to 256 (paged_decode.hpp).
+#include "paged_decode.hpp"
+
+namespace kvssd {
+template <>
+int launch_paged_dims<4, 256>(const PagedDecodeParams& p, int gp, bool precise, hipStream_t stream) {
+  if (gp == 1) return launch_paged_shape<4, 256, 1>(p, precise, stream);
+  if (gp == 2) return launch_paged_shape<4, 256, 2>(p, precise, stream);
+  if (gp == 4) return launch_paged_shape<4, 256, 4>(p, precise, stream);
+  return launch_paged_shape<4, 256, 8>(p, precise, stream);
+}
+}  // namespace kvssd

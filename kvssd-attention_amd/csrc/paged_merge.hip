@@ -24,7 +24,7 @@ constexpr int kSlice = 64;  // dims of a workgroup: 16 lanes of 4, 16 runs side 
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams p) {
   __shared__ float w_s[kMaxSplits];
   __shared__ float red[2][kThreads / kWave];
-  __shared__ float4v sum_s[kThreads / kWave][16];
+  __shared__ f32x4 sum_s[kThreads / kWave][16];
   const int seq = blockIdx.x / p.query_heads, h = blockIdx.x % p.query_heads;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int length = paged_length(p.c.lengths, seq, p.capacity);
@@ -54,14 +54,14 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
   if (lane == 0) red[1][wave] = total;
   __syncthreads();
   total = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-  float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   if (d0 < d) {
     const float* o = p.part_o + row0 * d + d0;
     const int64_t step = static_cast<int64_t>(p.query_heads) * d;
 #pragma unroll 4
     for (int r = tid / 16; r < n; r += kThreads / 16) {
       const float w = w_s[r];
-      const float4v v = *reinterpret_cast<const float4v*>(o + r * step);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(o + r * step);
       if (w != 0.0f) acc += w * v;  // (NaN weights take part)
     }
   }
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
   __syncthreads();
   const int64_t row = static_cast<int64_t>(seq) * p.query_heads + h;
   if (tid < 16 && d0 < d) {
-    const float4v v = (sum_s[0][tid] + sum_s[1][tid]) + (sum_s[2][tid] + sum_s[3][tid]);
+    const f32x4 v = (sum_s[0][tid] + sum_s[1][tid]) + (sum_s[2][tid] + sum_s[3][tid]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) store_out(p.out, p.out_dtype, row * d + d0 + i, total == 0.0f ? 0.0f : v[i] / total);
   }
@@ -88,10 +88,10 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodePara
   for (int64_t t = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 4; t < length;
        t += static_cast<int64_t>(gridDim.x) * kThreads * 4) {
     const float* s = p.scores + static_cast<int64_t>(seq) * p.query_heads * p.score_stride + t;
-    float4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int h = 0; h < p.query_heads; ++h) {
-      const float4v v = *reinterpret_cast<const float4v*>(s + h * p.score_stride);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(s + h * p.score_stride);
       const float e = lse[h] * kLog2e;
       if (e == -INFINITY) continue;  // no slot took part
 #pragma unroll
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodePara
 // Runs and shapes of a decode; the workspace's arrays as offsets from its start.
 struct Plan {
   PagedDecodeParams p;
-  int dp, nt;
+  int dp, gp = 1;
   size_t o_bytes, ml_bytes, score_bytes;
 };
 
@@ -132,29 +132,28 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, Plan* 
   p.out_dtype = a.out_query_dtype ? a.query_dtype : KVSSD_DTYPE_F32;
   p.scale_log2 = static_cast<float>(a.sm_scale) * kLog2e;
   p.groups = c.head_dim / c.group_size;
-  while ((1 << p.gp_log2) < p.groups) ++p.gp_log2;
-  const int heads = 16 >> p.gp_log2;
+  while (out->gp < p.groups) out->gp *= 2;
+  const int heads = 16 / out->gp;
   p.tiles = (p.gq + heads - 1) / heads;
   out->dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
-  // two head tiles share a tile's codes; at 256 dims their sums would not fit the registers
-  out->nt = p.tiles > 1 && out->dp < 256 ? 2 : 1;
-  p.tile_sets = (p.tiles + out->nt - 1) / out->nt;
-  p.head_groups = (c.kv_heads + kDecodeWaves - 1) / kDecodeWaves;
-  p.heads_of_group = (c.kv_heads + p.head_groups - 1) / p.head_groups;
-  if (static_cast<int64_t>(p.head_groups) * p.tile_sets > 65535) return arg_error("too many heads");
+  const int waves = decode_waves(out->dp);
+  const int64_t units = static_cast<int64_t>(c.kv_heads) * p.tiles;
+  if (units > (1 << 18)) return arg_error("too many heads");
+  p.groups_of_units = static_cast<int>((units + waves - 1) / waves);
+  p.group_units = static_cast<int>((units + p.groups_of_units - 1) / p.groups_of_units);
 
   int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
   int64_t all = a.total_tokens > 0 ? a.total_tokens : longest * c.sequences;
   if (all > longest * c.sequences) all = longest * c.sequences;
   constexpr int64_t kWaves = 4096;
   auto tiles_up = [](int64_t n) { return (n + kTile - 1) / kTile * kTile; };
-  int64_t chunk = tiles_up((all * c.kv_heads * p.tile_sets + kWaves - 1) / kWaves);
+  int64_t chunk = tiles_up((all * units + kWaves - 1) / kWaves);
   if (chunk < 64) chunk = 64;
   if ((longest + chunk - 1) / chunk > kMaxSplits) chunk = tiles_up((longest + kMaxSplits - 1) / kMaxSplits);
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((longest + chunk - 1) / chunk);
   if (p.splits < 1) p.splits = 1;
-  p.group_splits = kDecodeWaves / p.heads_of_group;
+  p.group_splits = waves / p.group_units;
   if (p.group_splits > p.splits) p.group_splits = p.splits;
 
   const size_t rows = static_cast<size_t>(c.sequences) * p.query_heads * p.splits;
@@ -164,7 +163,7 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, Plan* 
   out->score_bytes =
       a.accumulate ? static_cast<size_t>(c.sequences) * p.query_heads * p.score_stride * sizeof(float) : 0;
   const int64_t wgs = static_cast<int64_t>(c.sequences) * ((p.splits + p.group_splits - 1) / p.group_splits);
-  if (wgs * kDecodeWaves * kWave > 0xFFFFFFFFll || static_cast<int64_t>(c.sequences) * p.query_heads * kThreads > 0xFFFFFFFFll)
+  if (wgs * waves * kWave > 0xFFFFFFFFll || static_cast<int64_t>(c.sequences) * p.query_heads * kThreads > 0xFFFFFFFFll)
     return arg_error("too many sequences for one call");
   return 0;
 }
@@ -197,9 +196,14 @@ int launch_paged_decode(const kvssd_paged_cache& c, const kvssd_paged_decode_arg
   p.part_ml = reinterpret_cast<float*>(ws + plan.o_bytes);
   if (a.accumulate) p.scores = reinterpret_cast<float*>(ws + plan.o_bytes + plan.ml_bytes);
   const bool precise = p.out_dtype == KVSSD_DTYPE_F32 || p.query_dtype == KVSSD_DTYPE_F32;
-  if (int rc = c.bits == 4 ? launch_paged_int4(p, plan.dp, plan.nt, precise, stream)
-                           : launch_paged_int2(p, plan.dp, plan.nt, precise, stream))
-    return rc;
+  if (reinterpret_cast<uintptr_t>(a.query) % 16) return arg_error("query must be 16-byte aligned");
+  const auto launch = c.bits == 4 ? (plan.dp == 64    ? launch_paged_dims<4, 64>
+                                     : plan.dp == 128 ? launch_paged_dims<4, 128>
+                                                      : launch_paged_dims<4, 256>)
+                                  : (plan.dp == 64    ? launch_paged_dims<2, 64>
+                                     : plan.dp == 128 ? launch_paged_dims<2, 128>
+                                                      : launch_paged_dims<2, 256>);
+  if (int rc = launch(p, plan.gp, precise, stream)) return rc;
   if (p.splits > 1)
     if (int rc = launch_paged_merge(p, stream)) return rc;
   if (a.accumulate) {

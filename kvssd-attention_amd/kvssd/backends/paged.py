@@ -96,7 +96,8 @@ class PreparedPagedDecode:
             )
         if query.requires_grad and torch.is_grad_enabled():
             raise ValueError("this operator has no backward pass; call it under torch.no_grad() or on detached tensors")
-        query = query if query.is_contiguous() else query.contiguous()
+        if not query.is_contiguous() or query.data_ptr() % 16:  # the kernel reads 16 bytes at a time
+            query = query.clone(memory_format=torch.contiguous_format)
         if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self._index):
                 return self._launch(query)
