@@ -68,20 +68,111 @@ struct PagedDecodeParams {
   float* part_ml;
   float* scores;  // nullptr unless weights are summed: [sequences][query_heads][score_stride], log2 units
   int64_t score_stride;
-  int capacity, chunk, splits;  // slots of a run at least, runs of a sequence at most
-  int group_splits;             // runs of a workgroup (waves beyond one per kv head)
+  int capacity;
+  int run_tiles;    // stages of a run, unless the lengths call for more
+  int runs;         // runs of all sequences that the grid and the workspace hold; == sequences: one run each
+  int group_runs;   // runs of a workgroup (waves beyond one per unit)
   int group_units, groups_of_units;  // units (kv head, head tile) of a workgroup, workgroups over them
   int query_heads, gq, query_dtype, out_dtype;
   int tiles;             // head tiles of a kv head
   int groups;            // scale groups per head
+  int group_log2;        // log2 of the group size
   float scale_log2;
 };
 
-// a sequence's slots per run, and its runs
-__device__ __forceinline__ int run_of(int length, int chunk, int splits) {
-  const int per = (length + splits - 1) / splits;
-  const int up = (per + kTile - 1) / kTile * kTile;
-  return up > chunk ? up : chunk;
+// Where the runs of a ragged batch lie.  Every sequence is cut into runs of the
+// same number of stages (its last may be shorter); run r of the batch is the
+// r-th in the order of the sequences.  Worked out from the lengths on the
+// device, by every wave for itself (64 lengths a step), so that a grid of about
+// as many runs as there are serves any lengths: p.run_tiles comes from the
+// caller's hints, and grows here where the lengths would need more runs than
+// the grid has (sum of runs <= stages / run_tiles + sequences) or a sequence
+// more than its join takes.
+struct RunMap {
+  int tiles;  // stages of a run
+  int seq;    // of run r; -1: there is no such run
+  int nth;    // its place among the sequence's
+};
+
+// x of a lane before this one (0 where there is none): CTRL 0x110 + n, n lanes
+// before in the row of 16; 0x142 / 0x143, lane 15 of the row before / lane 31
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int lane_before(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_prefix(int x) {  // inclusive sum over the lanes
+  x += lane_before<0x111, 0xF>(x);
+  x += lane_before<0x112, 0xF>(x);
+  x += lane_before<0x114, 0xF>(x);
+  x += lane_before<0x118, 0xF>(x);
+  x += lane_before<0x142, 0xA>(x);
+  return x + lane_before<0x143, 0xC>(x);
+}
+__device__ __forceinline__ int wave_most(int x) {  // of numbers that are not negative
+  x = max(x, lane_before<0x111, 0xF>(x));
+  x = max(x, lane_before<0x112, 0xF>(x));
+  x = max(x, lane_before<0x114, 0xF>(x));
+  x = max(x, lane_before<0x118, 0xF>(x));
+  x = max(x, lane_before<0x142, 0xA>(x));
+  return __builtin_amdgcn_readlane(max(x, lane_before<0x143, 0xC>(x)), kWave - 1);
+}
+
+__device__ __forceinline__ int length_tiles(const PagedDecodeParams& p, int seq) {
+  return seq < p.c.sequences ? (paged_length(p.c.lengths, seq, p.capacity) + kTile - 1) / kTile : 0;
+}
+
+__device__ __forceinline__ int tiles_of_runs(const PagedDecodeParams& p) {
+  const int lane = threadIdx.x % kWave;
+  int sum = 0, most = 0;
+  for (int s = lane; s - lane < p.c.sequences; s += kWave) {
+    const int n = length_tiles(p, s);
+    sum += n;
+    most = max(most, n);
+  }
+  sum = __builtin_amdgcn_readlane(wave_prefix(sum), kWave - 1);
+  most = wave_most(most);
+  if (p.runs <= p.c.sequences) return max(most, 1);  // one run a sequence
+  const int room = p.runs - p.c.sequences;
+  return max(p.run_tiles, max((sum + room - 1) / room, (most + kMaxSplits - 1) / kMaxSplits));
+}
+
+__device__ __forceinline__ RunMap find_run(const PagedDecodeParams& p, int r) {
+  RunMap m{tiles_of_runs(p), -1, 0};
+  if (p.runs <= p.c.sequences) {
+    if (r < p.c.sequences) m.seq = r;
+    return m;
+  }
+  const int lane = threadIdx.x % kWave;
+  for (int s0 = 0; s0 < p.c.sequences; s0 += kWave) {
+    const int n = (length_tiles(p, s0 + lane) + m.tiles - 1) / m.tiles;
+    const int upto = wave_prefix(n);
+    const uint64_t past = __ballot(r < upto);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      m.seq = s0 + at;
+      m.nth = r - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
+      return m;
+    }
+    r -= __builtin_amdgcn_readlane(upto, kWave - 1);
+  }
+  return m;
+}
+
+// first run of a sequence, and its number of runs
+__device__ __forceinline__ RunMap runs_of(const PagedDecodeParams& p, int seq, int* first, int* count) {
+  const RunMap m{tiles_of_runs(p), seq, 0};
+  const int lane = threadIdx.x % kWave;
+  int before = 0;
+  for (int s0 = 0; s0 <= seq; s0 += kWave) {
+    const int n = (length_tiles(p, s0 + lane) + m.tiles - 1) / m.tiles;
+    const int upto = wave_prefix(n);
+    if (seq < s0 + kWave) {
+      *count = __builtin_amdgcn_readlane(n, seq - s0);
+      *first = before + __builtin_amdgcn_readlane(upto, seq - s0) - *count;
+    }
+    before += __builtin_amdgcn_readlane(upto, kWave - 1);
+  }
+  return m;
 }
 
 template <typename T>
@@ -213,22 +304,21 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int col = lane & 15, lg = lane >> 4;
-  const int wg_splits = (p.splits + p.group_splits - 1) / p.group_splits;
   // (quotients are formed in vector registers: back to scalars, as the copies' bases have to be)
-  const int seq = scalar(blockIdx.x / wg_splits);
-  const int split = scalar((blockIdx.x % wg_splits) * p.group_splits + wave / p.group_units);
+  const int run = scalar(blockIdx.x * p.group_runs + wave / p.group_units);
   const int unit = scalar(blockIdx.y * p.group_units + wave % p.group_units);
   const int kvh = scalar(unit / p.tiles);
   const int set = unit - kvh * p.tiles;
   const kvssd_paged_cache& c = p.c;
-  if (split >= p.splits || kvh >= c.kv_heads) return;
+  if (kvh >= c.kv_heads) return;
+  const RunMap map = find_run(p, run);
+  if (map.seq < 0) return;
+  const int seq = scalar(map.seq);
   const int length = clamp_length(uniform_load(c.lengths + seq), p.capacity);
-  const int run = scalar(run_of(length, p.chunk, p.splits));
-  const int begin = split * run;  // < 2^31: splits * run < length + splits * (chunk + 64)
-  if (begin >= length && p.splits > 1) return;  // the merge knows which runs exist
-  const int end = min(length, begin + run);
+  const int begin = scalar(map.nth * map.tiles) * kTile;
+  const int end = min(length, begin + scalar(map.tiles) * kTile);  // (at most 2^30 + 64 each)
 
-  const int d = c.head_dim, gs = c.group_size;
+  const int d = c.head_dim;
   const int row_bytes = d * BITS / 8;
   const int64_t slot_bytes = static_cast<int64_t>(c.kv_heads) * row_bytes;
   const int64_t slot_scales = static_cast<int64_t>(c.kv_heads) * p.groups;
@@ -367,7 +457,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       query_span<kPiece>(p.query, p.query_dtype, q0 + (dim < d ? dim : 0), v);
 #pragma unroll
       for (int i = 0; i < kPiece; ++i) big = fmaxf(big, fabsf(v[i]));
-      const bool mine = hh < p.gq && dim < d && dim / gs == own_g;
+      const bool mine = hh < p.gq && dim < d && dim >> p.group_log2 == own_g;
 #pragma unroll
       for (int i = 0; i < kPiece; ++i) v[i] = mine ? v[i] : 0.0f;
     }
@@ -492,9 +582,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     if (first || __any(over)) {
       // new reference points: the largest score so far and the largest value scale so far
       int e_new = static_cast<int>(sv_top >> 10) - 23;
-#pragma unroll
-      for (int k = 1; k < kWave; k <<= 1) e_new = max(e_new, __shfl_xor(e_new, k, kWave));
-      e_new = max(e_new, w_exp);
+      e_new = max(wave_most(e_new + 32) - 32, w_exp);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float top = -INFINITY;
@@ -609,9 +697,9 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   }
 
   // ---- this run's partial, or the result where a sequence has one run
-  const bool whole = p.splits == 1;
+  const bool whole = p.runs <= c.sequences;
   const int64_t head0 = static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq;
-  const int64_t part0 = (static_cast<int64_t>(seq) * p.splits + split) * p.query_heads + kvh * p.gq;
+  const int64_t part0 = static_cast<int64_t>(run) * p.query_heads + kvh * p.gq;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     float lt = l[t] + __shfl_xor(l[t], 16, kWave);
@@ -625,7 +713,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
 #pragma unroll
       for (int k = 0; k < kCols; ++k) {
         const int dim = BITS == 4 ? 16 * k + col : 32 * (k / 2) + 2 * col + k % 2;
-        if (hh >= p.gq || dim >= d || dim / gs != (r & (GP - 1))) continue;
+        if (hh >= p.gq || dim >= d || dim >> p.group_log2 != (r & (GP - 1))) continue;
         if (whole) store_out(p.out, p.out_dtype, (head0 + hh) * d + dim, l_row == 0.0f ? 0.0f : acc[t][k][i] * inv);
         else p.part_o[(part0 + hh) * d + dim] = kF * acc[t][k][i];
       }
@@ -644,9 +732,8 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
 
 template <int BITS, int DP, int GP, bool PREC>
 int launch_paged_kernel(const PagedDecodeParams& p, hipStream_t stream) {
-  const int wg_splits = (p.splits + p.group_splits - 1) / p.group_splits;
-  const dim3 grid(static_cast<unsigned>(p.c.sequences) * wg_splits, p.groups_of_units);
-  const dim3 block(p.group_units * p.group_splits * kWave);
+  const dim3 grid((p.runs + p.group_runs - 1) / p.group_runs, p.groups_of_units);
+  const dim3 block(p.group_units * p.group_runs * kWave);
   if constexpr (DP * BITS >= 256) {
     if (p.c.page_tokens % 32 == 0 && p.c.head_dim * BITS % 128 == 0) {
       hipLaunchKernelGGL((paged_decode_kernel<BITS, DP, GP, PREC, true>), grid, block, 0, stream, p);

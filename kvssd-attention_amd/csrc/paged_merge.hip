@@ -27,10 +27,9 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
   __shared__ f32x4 sum_s[kThreads / kWave][16];
   const int seq = blockIdx.x / p.query_heads, h = blockIdx.x % p.query_heads;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int length = paged_length(p.c.lengths, seq, p.capacity);
-  const int run = run_of(length, p.chunk, p.splits);
-  const int n = length > 0 ? (length + run - 1) / run : 0;
-  const int64_t row0 = static_cast<int64_t>(seq) * p.splits * p.query_heads + h;  // run r: row0 + r * query_heads
+  int first_run, n;
+  runs_of(p, seq, &first_run, &n);
+  const int64_t row0 = static_cast<int64_t>(first_run) * p.query_heads + h;  // run r: row0 + r * query_heads
   const int d0 = blockIdx.y * kSlice + 4 * (tid & 15);
   const int d = p.c.head_dim;
   float big = -INFINITY;
@@ -142,28 +141,31 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, Plan* 
   p.groups_of_units = static_cast<int>((units + waves - 1) / waves);
   p.group_units = static_cast<int>((units + p.groups_of_units - 1) / p.groups_of_units);
 
-  int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
-  int64_t all = a.total_tokens > 0 ? a.total_tokens : longest * c.sequences;
-  if (all > longest * c.sequences) all = longest * c.sequences;
-  constexpr int64_t kWaves = 4096;
-  auto tiles_up = [](int64_t n) { return (n + kTile - 1) / kTile * kTile; };
-  int64_t chunk = tiles_up((all * units + kWaves - 1) / kWaves);
-  if (chunk < 64) chunk = 64;
-  if ((longest + chunk - 1) / chunk > kMaxSplits) chunk = tiles_up((longest + kMaxSplits - 1) / kMaxSplits);
-  p.chunk = static_cast<int>(chunk);
-  p.splits = static_cast<int>((longest + chunk - 1) / chunk);
-  if (p.splits < 1) p.splits = 1;
-  p.group_splits = waves / p.group_units;
-  if (p.group_splits > p.splits) p.group_splits = p.splits;
+  while ((1 << p.group_log2) < c.group_size) ++p.group_log2;
 
-  const size_t rows = static_cast<size_t>(c.sequences) * p.query_heads * p.splits;
-  out->o_bytes = p.splits > 1 ? aligned(rows * c.head_dim * sizeof(float)) : 0;
-  out->ml_bytes = p.splits > 1 ? aligned(rows * 2 * sizeof(float)) : 0;
-  p.score_stride = tiles_up(p.capacity);
+  auto tiles_of = [](int64_t n) { return (n + kTile - 1) / kTile; };
+  const int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
+  if (tiles_of(p.capacity) * c.sequences >= int64_t{1} << 31) return arg_error("sequences * capacity is past 2^37 slots");
+  int64_t all = tiles_of(longest) * c.sequences;  // stages to be worked on
+  if (a.total_tokens > 0 && a.total_tokens / kTile + c.sequences < all) all = a.total_tokens / kTile + c.sequences;
+  constexpr int64_t kWaves = 4096;
+  int64_t per = (all * units + kWaves - 1) / kWaves;
+  const int64_t least = (tiles_of(longest) + kMaxSplits - 1) / kMaxSplits;
+  if (per < least) per = least;
+  p.run_tiles = static_cast<int>(per);
+  p.runs = per >= tiles_of(longest) ? c.sequences : static_cast<int>(all / per + c.sequences);
+  p.group_runs = waves / p.group_units;
+  if (p.group_runs > p.runs) p.group_runs = p.runs;
+
+  const bool whole = p.runs <= c.sequences;
+  const size_t rows = static_cast<size_t>(p.runs) * p.query_heads;
+  out->o_bytes = whole ? 0 : aligned(rows * c.head_dim * sizeof(float));
+  out->ml_bytes = whole ? 0 : aligned(rows * 2 * sizeof(float));
+  p.score_stride = tiles_of(p.capacity) * kTile;
   out->score_bytes =
       a.accumulate ? static_cast<size_t>(c.sequences) * p.query_heads * p.score_stride * sizeof(float) : 0;
-  const int64_t wgs = static_cast<int64_t>(c.sequences) * ((p.splits + p.group_splits - 1) / p.group_splits);
-  if (wgs * waves * kWave > 0xFFFFFFFFll || static_cast<int64_t>(c.sequences) * p.query_heads * kThreads > 0xFFFFFFFFll)
+  if (static_cast<int64_t>(p.runs) * waves * kWave > 0xFFFFFFFFll ||
+      static_cast<int64_t>(c.sequences) * p.query_heads * kThreads > 0xFFFFFFFFll)
     return arg_error("too many sequences for one call");
   return 0;
 }
@@ -204,7 +206,7 @@ int launch_paged_decode(const kvssd_paged_cache& c, const kvssd_paged_decode_arg
                                      : plan.dp == 128 ? launch_paged_dims<2, 128>
                                                       : launch_paged_dims<2, 256>);
   if (int rc = launch(p, plan.gp, precise, stream)) return rc;
-  if (p.splits > 1)
+  if (p.runs > c.sequences)
     if (int rc = launch_paged_merge(p, stream)) return rc;
   if (a.accumulate) {
     const int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
