@@ -8,8 +8,7 @@
 // than those bytes take to arrive.
 //
 // Work split.  A wave owns one kv head, up to 16 / GP of its query heads (GP:
-// scale groups per head, rounded up to a power of two; NT such head tiles) and
-// one run of a sequence's slots, 64 slots (a stage) at a time.  The waves of a
+// scale groups per head, rounded up to a power of two) and one run of a sequence's slots, 64 slots (a stage) at a time.  The waves of a
 // workgroup take neighbouring kv heads of the same run, whose rows lie side by
 // side in a page, so that whole cache lines are used.  Waves do not meet: each
 // leaves an unnormalised partial (O, m, l), which paged_merge.hip joins.
@@ -246,6 +245,9 @@ __device__ __forceinline__ u32x4 key_operand(uint32_t x, int odd, const Masks& k
   }
 }
 
+// fp16 number e of packed pairs
+__device__ __forceinline__ float half_of(const uint32_t* w, int e) { return e % 2 ? half_hi(w[e / 2]) : half_lo(w[e / 2]); }
+
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
   return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
@@ -293,7 +295,6 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   constexpr int kSpan = DP / 4;            // dims of a lane in QK
   constexpr int kCols = DP / 16;           // PV column tiles
   constexpr int kParts = PREC ? 2 : 1;
-  constexpr int NT = 1;
   constexpr int kHeads = 16 / GP;          // query heads of a head tile
   constexpr float kF = kUnpackScale<BITS>;
   constexpr float kOff = kUnpackOffset<BITS>;
@@ -308,7 +309,6 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   const int run = scalar(blockIdx.x * p.group_runs + wave / p.group_units);
   const int unit = scalar(blockIdx.y * p.group_units + wave % p.group_units);
   const int kvh = scalar(unit / p.tiles);
-  const int set = unit - kvh * p.tiles;
   const kvssd_paged_cache& c = p.c;
   if (kvh >= c.kv_heads) return;
   const RunMap map = find_run(p, run);
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   const int64_t slot_bytes = static_cast<int64_t>(c.kv_heads) * row_bytes;
   const int64_t slot_scales = static_cast<int64_t>(c.kv_heads) * p.groups;
   const int own_g = col & (GP - 1);
-  const int gq0 = set * NT * kHeads;  // first query head of this wave within its kv head
+  const int head_first = (unit - kvh * p.tiles) * kHeads;  // first query head of this wave within its kv head
 
   // ---- copies of a stage
   const uint8_t* pk = c.packed_k + static_cast<int64_t>(kvh) * row_bytes;
@@ -441,12 +441,11 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   }
 
   // ---- query operand, its scale and the accumulator's initial value (while the first stage arrives)
-  u32x4 q[kParts][NT][kSlices];
-  float c_init[NT], s_factor[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int hh = gq0 + t * kHeads + col / GP;
-    const int64_t q0 = (static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq + (hh < p.gq ? hh : 0)) * d;
+  u32x4 q[kParts][kSlices];
+  const int head = head_first + col / GP;  // of the lane's column, within its kv head
+  const int64_t head0 = static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq;
+  float c_init, s_factor;
+  {
     float x[kSpan];
     float big = 0.0f;
     constexpr int kPieces = DP == 256 ? 2 : 1, kPiece = kSpan / kPieces;
@@ -454,10 +453,10 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     for (int g = 0; g < kPieces; ++g) {
       const int dim = g * 128 + lg * kPiece;
       float* v = x + g * kPiece;
-      query_span<kPiece>(p.query, p.query_dtype, q0 + (dim < d ? dim : 0), v);
+      query_span<kPiece>(p.query, p.query_dtype, (head0 + (head < p.gq ? head : 0)) * d + (dim < d ? dim : 0), v);
 #pragma unroll
       for (int i = 0; i < kPiece; ++i) big = fmaxf(big, fabsf(v[i]));
-      const bool mine = hh < p.gq && dim < d && dim >> p.group_log2 == own_g;
+      const bool mine = head < p.gq && dim < d && dim >> p.group_log2 == own_g;
 #pragma unroll
       for (int i = 0; i < kPiece; ++i) v[i] = mine ? v[i] : 0.0f;
     }
@@ -468,7 +467,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     const int up = 10 + 127 - ex;  // 2^up big in [2^10, 2^11)
     const float scale_up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + up) << 23);
     const float scale_down = __builtin_bit_cast(float, static_cast<uint32_t>(127 - up) << 23);
-    s_factor[t] = scale_down * (kF * p.scale_log2);
+    s_factor = scale_down * (kF * p.scale_log2);
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < kSlices; ++j)
@@ -478,18 +477,18 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
         const int lo = BITS == 4 ? j * 8 + w : j / 2 * 16 + j % 2 * 4 + w;
         const float a = x[lo] * scale_up, b = x[lo + (BITS == 4 ? 4 : 8)] * scale_up;
         const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
-        q[0][t][j][w] = pack_half2(ah, bh);
+        q[0][j][w] = pack_half2(ah, bh);
         sum += static_cast<float>(ah) + static_cast<float>(bh);
         if constexpr (PREC) {
           const _Float16 al = static_cast<_Float16>(a - static_cast<float>(ah));
           const _Float16 bl = static_cast<_Float16>(b - static_cast<float>(bh));
-          q[kParts - 1][t][j][w] = pack_half2(al, bl);
+          q[kParts - 1][j][w] = pack_half2(al, bl);
           sum += static_cast<float>(al) + static_cast<float>(bl);
         }
       }
     sum += __shfl_xor(sum, 16, kWave);
     sum += __shfl_xor(sum, 32, kWave);
-    c_init[t] = -kOff * sum;
+    c_init = -kOff * sum;
   }
 
   // ---- where the lane reads a stage's codes
@@ -507,15 +506,10 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   const Masks masks = make_masks(zero);
   const uint32_t m01 = 0x00030003u | zero, m23 = 0x000C000Cu | zero;
 
-  f32x4 acc[NT][kCols];
-  float m_ref[NT], l[NT];
+  f32x4 acc[kCols];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    m_ref[t] = -INFINITY;
-    l[t] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kCols; ++i) acc[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int i = 0; i < kCols; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m_ref = -INFINITY, l = 0.0f;
   int w_exp = -32;  // W = 2^(s - m_ref) sv, m_ref = maximum + w_exp: sv < 2^(w_exp + 9)
   bool first = true;
 
@@ -532,7 +526,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
         if (!(mask16 >> e & 1u)) svw[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
     }
     // ---- scores
-    f32x4 s_acc[NT][4];
+    f32x4 s_acc[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       uint32_t kw[kSpan * BITS / 32];
@@ -540,17 +534,14 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       __builtin_memcpy(kw, __builtin_assume_aligned(stage + key_at[u], kBytes), kBytes);
       if constexpr (DP == 256)
         __builtin_memcpy(kw + kBytes / 4, __builtin_assume_aligned(stage + (key_at[u] ^ (kRow / 2)), kBytes), kBytes);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) s_acc[t][u] = f32x4{c_init[t], c_init[t], c_init[t], c_init[t]};
+      f32x4 s = {c_init, c_init, c_init, c_init};
 #pragma unroll
       for (int j = 0; j < kSlices; ++j) {
         const u32x4 a = BITS == 4 ? key_operand<BITS>(kw[j], 0, masks) : key_operand<BITS>(kw[j / 2], j % 2, masks);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          s_acc[t][u] = mfma16(a, q[0][t][j], s_acc[t][u]);
-          if constexpr (PREC) s_acc[t][u] = mfma16(a, q[kParts - 1][t][j], s_acc[t][u]);
-        }
+        s = mfma16(a, q[0][j], s);
+        if constexpr (PREC) s = mfma16(a, q[kParts - 1][j], s);
       }
+      s_acc[u] = s;
     }
     uint32_t sv_top;
     {
@@ -560,102 +551,87 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       for (int i = 1; i < 8; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, svw[i] & 0x7FFF7FFFu));
       sv_top = m[0] > m[1] ? m[0] : m[1];
     }
-    float s2[NT][16];  // scores over s_factor, summed over the groups
+    float tv[16];  // log2 units above the reference
     bool over = static_cast<int>(sv_top >> 10) - 23 > w_exp;
+    float top = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float x = s_acc[t][e / 4][e % 4] * static_cast<float>(__builtin_bit_cast(half2v, skw[e / 2])[e % 2]);
-        if constexpr (GP > 1) x = dpp_add<0xB1>(x);
-        if constexpr (GP > 2) x = dpp_add<0x4E>(x);
-        if constexpr (GP > 4) x = dpp_add<0x141>(x);
-        if (kRagged && !(mask16 >> e & 1u)) x = -INFINITY;
-        s2[t][e] = x;
-        // (s_factor is negative or zero for a scale that is: the mask stays a mask below)
-        const float s = kRagged && !(mask16 >> e & 1u) ? -INFINITY : __builtin_fmaf(x, s_factor[t], -m_ref[t]);
-        top = fmaxf(top, s);
-      }
-      over = over || top > kLazy - static_cast<float>(w_exp);
+    for (int e = 0; e < 16; ++e) {
+      // products with an fp16 scale as fused multiply-adds of 0: one v_fma_mix each.  Opaque, so that the sums below
+      // take the rounded product (fused into one lane's sum, it would leave a head's lanes with different scores)
+      float x = __builtin_fmaf(s_acc[e / 4][e % 4], half_of(skw, e), 0.0f);
+      asm("" : "+v"(x));
+      if constexpr (GP > 1) x = dpp_add<0xB1>(x);
+      if constexpr (GP > 2) x = dpp_add<0x4E>(x);
+      if constexpr (GP > 4) x = dpp_add<0x141>(x);
+      s_acc[e / 4][e % 4] = x;
+      tv[e] = kRagged && !(mask16 >> e & 1u) ? -INFINITY : __builtin_fmaf(x, s_factor, -m_ref);
+      top = fmaxf(top, tv[e]);
     }
+    over = over || top > kLazy - static_cast<float>(w_exp);
     if (first || __any(over)) {
       // new reference points: the largest score so far and the largest value scale so far
-      int e_new = static_cast<int>(sv_top >> 10) - 23;
-      e_new = max(wave_most(e_new + 32) - 32, w_exp);
+      const int e_new = max(wave_most(static_cast<int>(sv_top >> 10) + 9) - 32, w_exp);
+      top = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float top = -INFINITY;
+      for (int e = 0; e < 16; ++e)
+        if (!kRagged || (mask16 >> e & 1u)) top = fmaxf(top, s_acc[e / 4][e % 4] * s_factor);
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      const float m_old = m_ref - static_cast<float>(w_exp);
+      const float ref = fmaxf(first ? -INFINITY : m_old, top) + static_cast<float>(e_new);
+      const float alpha = first ? 0.0f : (ref == m_ref ? 1.0f : exp2f(m_ref - ref));
+      m_ref = ref;
+      if (!first) {
+        l *= alpha;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (!kRagged || (mask16 >> e & 1u)) top = fmaxf(top, s2[t][e] * s_factor[t]);
-        top = fmaxf(top, __shfl_xor(top, 16, kWave));
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        const float m_old = m_ref[t] - static_cast<float>(w_exp);
-        const float ref = fmaxf(first ? -INFINITY : m_old, top) + static_cast<float>(e_new);
-        const float alpha = first ? 0.0f : (ref == m_ref[t] ? 1.0f : exp2f(m_ref[t] - ref));
-        m_ref[t] = ref;
-        if (!first) {
-          l[t] *= alpha;
+        for (int i = 0; i < 4; ++i) {
+          const float a = __shfl(alpha, 4 * lg + i, kWave);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = __shfl(alpha, 4 * lg + i, kWave);
-#pragma unroll
-            for (int k = 0; k < kCols; ++k) acc[t][k][i] *= a;
-          }
+          for (int k = 0; k < kCols; ++k) acc[k][i] *= a;
         }
       }
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        tv[e] = kRagged && !(mask16 >> e & 1u) ? -INFINITY : __builtin_fmaf(s_acc[e / 4][e % 4], s_factor, -m_ref);
       w_exp = e_new;
       first = false;
     }
-    if (p.scores != nullptr) {
+    if (p.scores != nullptr && own_g == 0 && head < p.gq) {
+      float* dst = p.scores + (head0 + head) * p.score_stride + base + 16 * lg;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int hh = gq0 + t * kHeads + col / GP;
-        if (own_g == 0 && hh < p.gq) {
-          float* dst = p.scores + (static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq + hh) * p.score_stride + base + 16 * lg;
+      for (int u = 0; u < 4; ++u) {
+        f32x4 v;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            f32x4 v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              v[i] = kRagged && !(mask16 >> (4 * u + i) & 1u) ? -INFINITY : s2[t][4 * u + i] * s_factor[t];
-            *reinterpret_cast<f32x4*>(dst + 4 * u) = v;
-          }
-        }
+        for (int i = 0; i < 4; ++i)
+          v[i] = kRagged && !(mask16 >> (4 * u + i) & 1u) ? -INFINITY : s_acc[u][i] * s_factor;
+        *reinterpret_cast<f32x4*>(dst + 4 * u) = v;
       }
     }
     // ---- weights: pairs (e, e + 4) of each step's 8 slots, the order of the values' pairs
-    u32x4 w[kParts][NT][2];
+    u32x4 w[kParts][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float sum = 0.0f;
-      float x[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float tv = kRagged && !(mask16 >> e & 1u) ? -INFINITY : __builtin_fmaf(s2[t][e], s_factor[t], -m_ref[t]);
-        const float pe = __builtin_amdgcn_exp2f(tv);
-        sum += pe;
-        x[e] = pe * static_cast<float>(__builtin_bit_cast(half2v, svw[e / 2])[e % 2]);
-        // one product in 32 bits for both parts: a first part rounded straight from the factors (v_fma_mixlo_f16)
-        // may be the other of its two neighbours, and the parts' sum then a step of it off
-        if constexpr (PREC) asm("" : "+v"(x[e]));
-      }
-      l[t] += sum;
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float a = x[8 * s + k], b = x[8 * s + k + 4];
-          const half2v hi = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
-          w[0][t][s][k] = __builtin_bit_cast(uint32_t, hi);
-          if constexpr (PREC) {
-            const half2v lo = {static_cast<_Float16>(a - static_cast<float>(hi[0])),
-                               static_cast<_Float16>(b - static_cast<float>(hi[1]))};
-            w[kParts - 1][t][s][k] = __builtin_bit_cast(uint32_t, lo);
-          }
-        }
+    for (int e = 0; e < 16; ++e) {
+      tv[e] = __builtin_amdgcn_exp2f(tv[e]);
+      l += tv[e];
     }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int e0 = 8 * s + k, e1 = e0 + 4;
+        if constexpr (PREC) {
+          // one product in 32 bits for both parts: a first part rounded straight from the factors (v_fma_mixlo_f16)
+          // may be the other of its two neighbours, and the parts' sum then a step of it off
+          float a = tv[e0] * half_of(svw, e0), b = tv[e1] * half_of(svw, e1);
+          asm("" : "+v"(a), "+v"(b));
+          const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
+          w[0][s][k] = pack_half2(ah, bh);
+          w[kParts - 1][s][k] = pack_half2(static_cast<_Float16>(a - static_cast<float>(ah)),
+                                           static_cast<_Float16>(b - static_cast<float>(bh)));
+        } else {
+          w[0][s][k] = wpair(tv[e0], half_of(svw, e0), tv[e1], half_of(svw, e1));
+        }
+      }
     // ---- weights times values: 8 bytes of a row a read, 16 (INT4) or 32 (INT2) dims
 #pragma unroll
     for (int r = 0; r < kRow / 8; ++r) {
@@ -666,11 +642,8 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
         for (int odd = 0; odd < (BITS == 4 ? 1 : 2); ++odd) {
           const u32x4 b = value_operand<BITS>(static_cast<uint32_t>(x[s]), odd, masks, m01, m23);
           const int tile = BITS == 4 ? r : 2 * r + odd;
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            acc[t][tile] = mfma16(w[0][t][s], b, acc[t][tile]);
-            if constexpr (PREC) acc[t][tile] = mfma16(w[kParts - 1][t][s], b, acc[t][tile]);
-          }
+          acc[tile] = mfma16(w[0][s], b, acc[tile]);
+          if constexpr (PREC) acc[tile] = mfma16(w[kParts - 1][s], b, acc[tile]);
         }
     }
   };
@@ -698,34 +671,36 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
 
   // ---- this run's partial, or the result where a sequence has one run
   const bool whole = p.runs <= c.sequences;
-  const int64_t head0 = static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq;
   const int64_t part0 = static_cast<int64_t>(run) * p.query_heads + kvh * p.gq;
+  l += __shfl_xor(l, 16, kWave);
+  l += __shfl_xor(l, 32, kWave);
+  // a column tile's dims are of one group gk; of the lane's rows 4 lg + i = (head, group) the kRows with that group
+  // hold them
+  constexpr int kRows = 4 / (GP < 4 ? GP : 4);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float lt = l[t] + __shfl_xor(l[t], 16, kWave);
-    lt += __shfl_xor(lt, 32, kWave);
+  for (int n = 0; n < kRows; ++n) {
+    const int h = GP >= 4 ? 4 * lg / GP : kRows * lg + n;  // within the head tile
+    const float l_head = __shfl(l, h * GP, kWave);
+    const float factor = !whole ? kF : l_head == 0.0f ? 0.0f : kF / l_head;
+    const bool has = head_first + h < p.gq;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 4 * lg + i;
-      const int hh = gq0 + t * kHeads + r / GP;
-      const float l_row = __shfl(lt, r, kWave);
-      const float inv = l_row == 0.0f ? 0.0f : kF / l_row;
-#pragma unroll
-      for (int k = 0; k < kCols; ++k) {
-        const int dim = BITS == 4 ? 16 * k + col : 32 * (k / 2) + 2 * col + k % 2;
-        if (hh >= p.gq || dim >= d || dim >> p.group_log2 != (r & (GP - 1))) continue;
-        if (whole) store_out(p.out, p.out_dtype, (head0 + hh) * d + dim, l_row == 0.0f ? 0.0f : acc[t][k][i] * inv);
-        else p.part_o[(part0 + hh) * d + dim] = kF * acc[t][k][i];
-      }
+    for (int k = 0; k < kCols; ++k) {
+      const int dim = BITS == 4 ? 16 * k + col : 32 * (k / 2) + 2 * col + k % 2;
+      const int gk = scalar((BITS == 4 ? 16 * k : 32 * (k / 2)) >> p.group_log2);
+      const int i = GP >= 4 ? gk & 3 : GP == 2 ? gk % 2 + 2 * n : n;
+      const float v01 = i & 1 ? acc[k][1] : acc[k][0], v23 = i & 1 ? acc[k][3] : acc[k][2];
+      const float v = (i & 2 ? v23 : v01) * factor;
+      if (!has || dim >= d || (GP == 8 && (lg & 1) != gk >> 2)) continue;
+      if (whole) store_out(p.out, p.out_dtype, (head0 + head_first + h) * d + dim, l_head == 0.0f ? 0.0f : v);
+      else p.part_o[(part0 + head_first + h) * d + dim] = v;
     }
-    const int hh = gq0 + t * kHeads + col / GP;
-    if (lg == 0 && own_g == 0 && hh < p.gq) {
-      if (whole) {
-        p.lse[head0 + hh] = lt == 0.0f ? -INFINITY : kLn2 * (m_ref[t] + log2f(lt));
-      } else {
-        p.part_ml[2 * (part0 + hh)] = m_ref[t];
-        p.part_ml[2 * (part0 + hh) + 1] = lt;
-      }
+  }
+  if (lg == 0 && own_g == 0 && head < p.gq) {
+    if (whole) {
+      p.lse[head0 + head] = l == 0.0f ? -INFINITY : kLn2 * (m_ref + log2f(l));
+    } else {
+      p.part_ml[2 * (part0 + head)] = m_ref;
+      p.part_ml[2 * (part0 + head) + 1] = l;
     }
   }
 }

@@ -148,8 +148,10 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, Plan* 
   if (tiles_of(p.capacity) * c.sequences >= int64_t{1} << 31) return arg_error("sequences * capacity is past 2^37 slots");
   int64_t all = tiles_of(longest) * c.sequences;  // stages to be worked on
   if (a.total_tokens > 0 && a.total_tokens / kTile + c.sequences < all) all = a.total_tokens / kTile + c.sequences;
-  constexpr int64_t kWaves = 4096;
-  int64_t per = (all * units + kWaves - 1) / kWaves;
+  // one round of workgroups: every CU holds one (its LDS)
+  const int64_t room = 256 * waves / units;  // runs
+  const int64_t cut = room - c.sequences > room / 2 ? room - c.sequences : (room + 1) / 2;
+  int64_t per = (all + cut - 1) / (cut > 0 ? cut : 1);
   const int64_t least = (tiles_of(longest) + kMaxSplits - 1) / kMaxSplits;
   if (per < least) per = least;
   p.run_tiles = static_cast<int>(per);
