@@ -13,12 +13,16 @@
 // side in a page, so that whole cache lines are used.  Waves do not meet: each
 // leaves an unnormalised partial (O, m, l), which paged_merge.hip joins.
 //
-// Copies.  A stage's codes go from memory straight to LDS (16 bytes a lane), one
-// stage ahead of the arithmetic, into the wave's own two buffers: 128 KB of a
-// CU in flight or in use without a register.  A row's 16-byte chunks are stored
-// in an order turned by the row's number, so that neither the key rows' nor the
-// value columns' reads meet in a bank.  Scales come through registers (one slot
-// a lane) and are laid out by group in LDS.
+// Copies.  Codes, scales and the query go from memory straight to LDS (16 or 4
+// bytes a lane), into the wave's own two buffers and without a register or a
+// barrier.  A stage's codes and scales are taken into registers when it begins,
+// and the copies of two stages on go to their place at once: between one and two
+// stages are always on the way, each awaited by the count of later copies
+// (vmcnt).  With one stage on the way, all awaited at once, 524,288 slots took
+// 133 us; with the waves' copies joined into rows of all kv heads, a barrier a
+// stage, 142.  A row's 16-byte chunks are stored in an order turned by the row's
+// number, so that neither the key rows' nor the value columns' reads meet in a
+// bank.  Scales are laid out by group in LDS when their stage begins.
 //
 // QK (v_mfma_f32_16x16x32_f16): rows = 16 slots' codes, columns = (query head,
 //   group): the query masked to one group, so that a column's sum is one group's
@@ -263,13 +267,13 @@ __device__ __forceinline__ void dma4_at(const uint8_t* src, uint32_t lds_dst) {
 
 // N consecutive query values (16-byte aligned) in 32 bits
 template <int N>
-__device__ __forceinline__ void query_span(const void* q, int dtype, int64_t at, float* v) {
+__device__ __forceinline__ void query_span(const uint8_t* q, int dtype, int at, float* v) {
   if (dtype == KVSSD_DTYPE_F32) {
-    __builtin_memcpy(v, __builtin_assume_aligned(static_cast<const float*>(q) + at, 16), 4 * N);
+    __builtin_memcpy(v, __builtin_assume_aligned(q + 4 * at, 16), 4 * N);
     return;
   }
   uint32_t w[N / 2];
-  __builtin_memcpy(w, __builtin_assume_aligned(static_cast<const uint16_t*>(q) + at, 16), 2 * N);
+  __builtin_memcpy(w, __builtin_assume_aligned(q + 2 * at, 16), 2 * N);
   if (dtype == KVSSD_DTYPE_F16) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = i % 2 ? half_hi(w[i / 2]) : half_lo(w[i / 2]);
@@ -281,9 +285,9 @@ __device__ __forceinline__ void query_span(const void* q, int dtype, int64_t at,
 
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// UNI: pages hold whole halves (32 slots) of a stage and rows whole 16-byte
-// chunks, so that a copy's rows have one uniform base; else every lane finds
-// its own row's address.
+// UNI: pages hold whole halves (32 slots) of a stage, rows whole 16-byte chunks
+// and a head's scales begin in a word alike in every row, so that a copy's rows
+// have one uniform base; else every lane finds its own row's address.
 template <int BITS, int DP, int GP, bool PREC, bool UNI>
 __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(PagedDecodeParams p) {
   constexpr int kWaves = decode_waves(DP);
@@ -299,7 +303,11 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   constexpr float kF = kUnpackScale<BITS>;
   constexpr float kOff = kUnpackOffset<BITS>;
   constexpr float kLazy = 6.0f;            // log2 units a score may exceed the reference by
+  // 4-byte words copied of a slot's scales of one head (two for one: a copy's slots are then of one half)
+  constexpr int kScaleWords = GP <= 4 ? 2 : 4, kScaleCopies = kScaleWords;
+  constexpr int kStageCopies = 2 * (kChunks + kScaleCopies);
   __shared__ __attribute__((aligned(1024))) uint8_t codes_lds[kWaves][2][2 * kArray];
+  __shared__ __attribute__((aligned(16))) uint32_t raw_lds[kWaves][2][2][kTile][kScaleWords];
   __shared__ __attribute__((aligned(16))) uint16_t scale_lds[kWaves][2][GP][kTile];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -323,7 +331,6 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   const int64_t slot_bytes = static_cast<int64_t>(c.kv_heads) * row_bytes;
   const int64_t slot_scales = static_cast<int64_t>(c.kv_heads) * p.groups;
   const int own_g = col & (GP - 1);
-  const int head_first = (unit - kvh * p.tiles) * kHeads;  // first query head of this wave within its kv head
 
   // ---- copies of a stage
   const uint8_t* pk = c.packed_k + static_cast<int64_t>(kvh) * row_bytes;
@@ -340,27 +347,15 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     const int lr = lane / kChunks;
     const int chunk = (lane % kChunks) ^ turned(n * kRowsOfCopy + lr);
     const int byte = chunk * 16 < row_bytes ? chunk * 16 : 0;  // (padding: the row's start again)
-    copy_at[n] = UNI ? static_cast<uint32_t>(lr * slot_bytes) + byte : byte;
+    copy_at[n] = UNI ? static_cast<uint32_t>((n * kRowsOfCopy % 32 + lr) * slot_bytes) + byte : byte;
   }
-  uint32_t scale_k[4], scale_v[4];  // of slot `lane` of the stage last issued
-  uint32_t live = 0;                // whether that slot takes part
-  auto load_scales = [&](const uint16_t* row, uint32_t* s) {
-    if (GP >= 4 && p.groups == 4) {
-      __builtin_memcpy(s, __builtin_assume_aligned(row, 8), 8);
-    } else if (GP == 2) {
-      __builtin_memcpy(s, __builtin_assume_aligned(row, 4), 4);
-    } else if (GP == 8 && p.groups == 8) {
-      __builtin_memcpy(s, __builtin_assume_aligned(row, 16), 16);
-    } else {
-#pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        const uint32_t x = row[g < p.groups ? g : 0];
-        s[g / 2] = g % 2 ? s[g / 2] | x << 16 : x;
-      }
-    }
-  };
-  const uint32_t lds0 = lds_addr(codes_lds[wave][0]);
-  // the page of the next half to be issued, fetched one half ahead
+  // the lane's scale word of a copy of 64 / kScaleWords slots (the last word there is, where there are fewer)
+  const int scale_slot = lane / kScaleWords;
+  const int scale_byte = 4 * min(lane % kScaleWords, (p.groups - 1) / 2);
+  const uint32_t codes0 = lds_addr(codes_lds[wave][0]);
+  const uint32_t raw0 = lds_addr(reinterpret_cast<const uint8_t*>(raw_lds[wave]));
+  const bool chunked = row_bytes % 16 == 0;
+  // The pages of the next stage's halves, fetched one stage before they are used
   int half_page = 0, half_off = 0;  // index into `pages`, slot within the page
   if constexpr (UNI) {
     half_page = scalar(begin / bt);
@@ -379,30 +374,32 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       }
     }
   };
-  auto issue = [&](int base, int buf) {
-    const uint32_t dst = lds0 + buf * (2 * kArray);
-    if constexpr (UNI) {
-      int64_t row[2];
-      bool ok[2];
+  // Whether a slot's scales begin in a word's upper half, for an odd number of groups.  The very last ones of a pool
+  // with an odd number of scales would end in a word past it: they are taken from one scale earlier on.
+  const bool odd_pool = p.groups % 2 && c.num_pages % 2 && bt % 2 && c.kv_heads % 2;
+  const int last_row = odd_pool && kvh == c.kv_heads - 1 ? c.num_pages * bt - 1 : -1;
+  auto upper = [&](int row) {
+    return p.groups % 2 && (((static_cast<uint32_t>(row) * c.kv_heads + kvh) & 1u) || row == last_row);
+  };
+  // A stage to be copied: rows of the pool (of its halves; of the lane's slot where not UNI), slots that take part,
+  // slots whose scales begin in a word's upper half
+  struct Stage {
+    int row[2];
+    uint64_t live, odd;
+  };
+  auto locate = [&](int base) {
+    Stage s;
+    if constexpr (UNI) {  // (an odd number of groups: of an even number of kv heads)
+      const int left = end - base;
+      s.live = left >= kTile ? ~0ull : (1ull << left) - 1;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        ok[h] = next_page[h] >= 0 && next_page[h] < c.num_pages;
-        row[h] = static_cast<int64_t>(ok[h] ? next_page[h] : 0) * bt + next_off[h];
+        const bool ok = static_cast<uint32_t>(next_page[h]) < static_cast<uint32_t>(c.num_pages);
+        s.row[h] = ok ? next_page[h] * bt + next_off[h] : 0;
+        if (!ok) s.live &= h ? 0xFFFFFFFFull : 0xFFFFFFFF00000000ull;
       }
-      const int64_t mine = (lane < 32 ? row[0] : row[1]) + (lane & 31);
-      load_scales(sk + mine * slot_scales, scale_k);
-      load_scales(sv + mine * slot_scales, scale_v);
-      live = base + lane < end && (lane < 32 ? ok[0] : ok[1]);
-#pragma unroll
-      for (int n = 0; n < kChunks; ++n) {
-        const int64_t at = (row[n * kRowsOfCopy / 32] + n * kRowsOfCopy % 32) * slot_bytes;
-        dma16<true>(pk + at, copy_at[n], dst + n * 1024);
-      }
-#pragma unroll
-      for (int n = 0; n < kChunks; ++n) {
-        const int64_t at = (row[n * kRowsOfCopy / 32] + n * kRowsOfCopy % 32) * slot_bytes;
-        dma16<true>(pv + at, copy_at[n], dst + kArray + n * 1024);
-      }
+      fetch_pages(base + kTile);
+      s.odd = p.groups & kvh & 1 ? ~0ull : 0;
     } else {
       const int slot = base + lane;
       int mine = -1;
@@ -410,40 +407,84 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
         const int page = pages[slot / bt];
         if (page >= 0 && page < c.num_pages) mine = page * bt + slot % bt;
       }
-      live = mine >= 0;
-      const int64_t row = max(mine, 0);
-      load_scales(sk + row * slot_scales, scale_k);
-      load_scales(sv + row * slot_scales, scale_v);
-      if (row_bytes % 16 == 0) {
+      s.live = __ballot(mine >= 0);
+      s.row[0] = s.row[1] = max(mine, 0);
+      s.odd = __ballot(upper(s.row[0]));
+    }
+    return s;
+  };
+  auto copy_codes = [&](const uint8_t* src, const Stage& s, uint32_t dst) {
+    if constexpr (UNI) {
+      const uint8_t* half[2] = {src + s.row[0] * slot_bytes, src + s.row[1] * slot_bytes};
 #pragma unroll
-        for (int n = 0; n < kChunks; ++n) {
-          const int64_t at = static_cast<int64_t>(__shfl(static_cast<int>(row), n * kRowsOfCopy + lane / kChunks, kWave)) * slot_bytes + copy_at[n];
-          dma16_at(pk + at, dst + n * 1024);
-          dma16_at(pv + at, dst + kArray + n * 1024);
-        }
-      } else {  // INT2 rows of an odd number of 8-byte pieces: 4 bytes a lane
-        constexpr int kUnits = kRow / 4;
-        for (int n = 0; n < kUnits; ++n) {
-          const int r = n * (kWave / kUnits) + lane / kUnits, unit = lane % kUnits;
-          int byte = ((unit / 4) ^ turned(r)) * 16 + unit % 4 * 4;
-          byte = byte < row_bytes ? byte : 0;
-          const int64_t at = static_cast<int64_t>(__shfl(static_cast<int>(row), r, kWave)) * slot_bytes + byte;
-          dma4_at(pk + at, dst + n * 256);
-          dma4_at(pv + at, dst + kArray + n * 256);
-        }
+      for (int n = 0; n < kChunks; ++n) dma16<false>(half[n * kRowsOfCopy / 32], copy_at[n], dst + n * 1024);
+    } else if (chunked) {
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) {
+        const int64_t row = __shfl(s.row[0], n * kRowsOfCopy + lane / kChunks, kWave);
+        dma16_at(src + row * slot_bytes + copy_at[n], dst + n * 1024);
+      }
+    } else {  // INT2 rows of an odd number of 8-byte pieces: 4 bytes a lane
+      constexpr int kUnits = kRow / 4;
+      for (int n = 0; n < kUnits; ++n) {
+        const int r = n * (kWave / kUnits) + lane / kUnits, part = lane % kUnits;
+        int byte = ((part / 4) ^ turned(r)) * 16 + part % 4 * 4;
+        byte = byte < row_bytes ? byte : 0;
+        const int64_t row = __shfl(s.row[0], r, kWave);
+        dma4_at(src + row * slot_bytes + byte, dst + n * 256);
       }
     }
   };
-  if (begin < end) {
-    if constexpr (UNI) fetch_pages(begin);
-    issue(begin, 0);
-    if constexpr (UNI) fetch_pages(begin + kTile);
+  const uint32_t scale_at = static_cast<uint32_t>(scale_slot * slot_scales * 2) + scale_byte;
+  auto copy_scales = [&](const uint16_t* scales, const Stage& s, uint32_t dst) {
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(scales);
+    constexpr int kSlots = kTile / kScaleCopies;  // of a copy: 32 or 16
+#pragma unroll
+    for (int n = 0; n < kScaleCopies; ++n) {
+      if constexpr (UNI) {
+        const int64_t row = s.row[n * kSlots / 32] + n * kSlots % 32;
+        dma4(src + row * slot_scales * 2 - (p.groups & kvh & 1) * 2, scale_at, dst + n * 256);
+      } else {
+        const int row = __shfl(s.row[0], n * kSlots + scale_slot, kWave);
+        dma4_at(src + row * slot_scales * 2 - (upper(row) ? 2 : 0) + scale_byte, dst + n * 256);
+      }
+    }
+  };
+  auto copy_stage = [&](const Stage& s, int buf) {
+    copy_scales(sk, s, raw0 + buf * 2 * (kScaleCopies * 256));
+    copy_scales(sv, s, raw0 + (buf * 2 + 1) * (kScaleCopies * 256));
+    copy_codes(pk, s, codes0 + buf * (2 * kArray));
+    copy_codes(pv, s, codes0 + buf * (2 * kArray) + kArray);
+  };
+
+  // ---- the query's rows first, into the second buffer (into both, before any stage, where they need them)
+  const int head_first = (unit - kvh * p.tiles) * kHeads;  // first query head of this wave within its kv head
+  const int64_t head0 = static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq;
+  const int query_item = p.query_dtype == KVSSD_DTYPE_F32 ? 4 : 2;
+  const int query_bytes = min(kHeads, p.gq - head_first) * d * query_item;
+  const bool crowded = query_bytes > 2 * kArray;
+  const int query_lds = crowded ? 0 : 2 * kArray;  // within the wave's buffers
+  {
+    const uint8_t* src = static_cast<const uint8_t*>(p.query) + (head0 + head_first) * d * query_item;
+    for (int n = 0; n * 1024 < query_bytes; ++n) {
+      const int at = n * 1024 + lane * 16;
+      dma16_at(src + (at < query_bytes ? at : 0), codes0 + query_lds + n * 1024);
+    }
   }
+  const int stages = (end - begin + kTile - 1) / kTile;
+  Stage now{}, next{};
+  if (stages > 0) {
+    if constexpr (UNI) fetch_pages(begin);
+    now = locate(begin);
+    if (!crowded) copy_stage(now, 0);
+  }
+  if (!crowded && stages > 0 && chunked) __builtin_amdgcn_s_waitcnt(vmcnt_wait(kStageCopies));
+  else __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
+  asm volatile("" ::: "memory");
 
   // ---- query operand, its scale and the accumulator's initial value (while the first stage arrives)
   u32x4 q[kParts][kSlices];
   const int head = head_first + col / GP;  // of the lane's column, within its kv head
-  const int64_t head0 = static_cast<int64_t>(seq) * p.query_heads + kvh * p.gq;
   float c_init, s_factor;
   {
     float x[kSpan];
@@ -453,7 +494,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     for (int g = 0; g < kPieces; ++g) {
       const int dim = g * 128 + lg * kPiece;
       float* v = x + g * kPiece;
-      query_span<kPiece>(p.query, p.query_dtype, (head0 + (head < p.gq ? head : 0)) * d + (dim < d ? dim : 0), v);
+      query_span<kPiece>(codes_lds[wave][0] + query_lds, p.query_dtype, (head < p.gq ? col / GP : 0) * d + (dim < d ? dim : 0), v);
 #pragma unroll
       for (int i = 0; i < kPiece; ++i) big = fmaxf(big, fabsf(v[i]));
       const bool mine = head < p.gq && dim < d && dim >> p.group_log2 == own_g;
@@ -490,6 +531,13 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     sum += __shfl_xor(sum, 32, kWave);
     c_init = -kOff * sum;
   }
+  // the query is read: the second stage may follow
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  if (crowded && stages > 0) copy_stage(now, 0);
+  if (stages > 1) {
+    next = locate(begin + kTile);
+    copy_stage(next, 1);
+  }
 
   // ---- where the lane reads a stage's codes
   int key_at[4];  // tile u: slot 16 (col / 4) + 4 u + col % 4 (and, in DP 256, chunks kChunks / 2 on)
@@ -513,35 +561,16 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   int w_exp = -32;  // W = 2^(s - m_ref) sv, m_ref = maximum + w_exp: sv < 2^(w_exp + 9)
   bool first = true;
 
-  auto compute = [&](int base, int buf, uint64_t live_mask, auto ragged_tag) {
+  constexpr int kLaneBytes = (DP == 256 ? 128 : DP) * BITS / 32;  // of a lane's piece of a key row: 16, 8 or 4
+  // a stage's weights from its scores; some of its slots may take no part (kRagged)
+  auto weigh = [&](int base, uint64_t live, f32x4 (&s_acc)[4], const uint32_t (&skw)[8], uint32_t (&svw)[8],
+                   u32x4 (&w)[kParts][2], auto ragged_tag) {
     constexpr bool kRagged = decltype(ragged_tag)::value;
-    const uint8_t* stage = codes_lds[wave][buf];
-    const uint32_t mask16 = static_cast<uint32_t>(live_mask >> (16 * lg)) & 0xFFFFu;  // slots 16 lg + e
-    uint32_t skw[8], svw[8];
-    __builtin_memcpy(skw, __builtin_assume_aligned(&scale_lds[wave][0][own_g][16 * lg], 16), 32);
-    __builtin_memcpy(svw, __builtin_assume_aligned(&scale_lds[wave][1][own_g][16 * lg], 16), 32);
+    const uint32_t mask16 = static_cast<uint32_t>(live >> (16 * lg)) & 0xFFFFu;  // slots 16 lg + e
     if constexpr (kRagged) {  // value scales of slots that take no part may be anything: 0 (codes are always finite)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (!(mask16 >> e & 1u)) svw[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
-    }
-    // ---- scores
-    f32x4 s_acc[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      uint32_t kw[kSpan * BITS / 32];
-      constexpr int kBytes = (DP == 256 ? 128 : DP) * BITS / 32;
-      __builtin_memcpy(kw, __builtin_assume_aligned(stage + key_at[u], kBytes), kBytes);
-      if constexpr (DP == 256)
-        __builtin_memcpy(kw + kBytes / 4, __builtin_assume_aligned(stage + (key_at[u] ^ (kRow / 2)), kBytes), kBytes);
-      f32x4 s = {c_init, c_init, c_init, c_init};
-#pragma unroll
-      for (int j = 0; j < kSlices; ++j) {
-        const u32x4 a = BITS == 4 ? key_operand<BITS>(kw[j], 0, masks) : key_operand<BITS>(kw[j / 2], j % 2, masks);
-        s = mfma16(a, q[0][j], s);
-        if constexpr (PREC) s = mfma16(a, q[kParts - 1][j], s);
-      }
-      s_acc[u] = s;
     }
     uint32_t sv_top;
     {
@@ -608,7 +637,6 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       }
     }
     // ---- weights: pairs (e, e + 4) of each step's 8 slots, the order of the values' pairs
-    u32x4 w[kParts][2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       tv[e] = __builtin_amdgcn_exp2f(tv[e]);
@@ -632,10 +660,71 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
           w[0][s][k] = wpair(tv[e0], half_of(svw, e0), tv[e1], half_of(svw, e1));
         }
       }
+  };
+
+  for (int i = 0, base = begin; i < stages; ++i, base += kTile) {
+    // the stage has landed
+    if (chunked && i + 1 < stages) __builtin_amdgcn_s_waitcnt(vmcnt_wait(kStageCopies));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
+    asm volatile("" ::: "memory");
+    const int buf = i & 1;
+    const uint8_t* stage = codes_lds[wave][buf];
+    uint32_t raw[2][kScaleWords + 1];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) __builtin_memcpy(raw[a], __builtin_assume_aligned(raw_lds[wave][buf][a][lane], 4 * kScaleWords), 4 * kScaleWords);
+    uint32_t kw[4][kSpan * BITS / 32];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      __builtin_memcpy(kw[u], __builtin_assume_aligned(stage + key_at[u], kLaneBytes), kLaneBytes);
+      if constexpr (DP == 256)
+        __builtin_memcpy(kw[u] + kLaneBytes / 4, __builtin_assume_aligned(stage + (key_at[u] ^ (kRow / 2)), kLaneBytes), kLaneBytes);
+    }
+    i32x2 vw[kRow / 8];
+#pragma unroll
+    for (int r = 0; r < kRow / 8; ++r) vw[r] = lds_read_tr4(stage, value_at + (((r / 2) ^ value_turn) * 16) + r % 2 * 8);
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      raw[a][kScaleWords] = 0;
+      if (p.groups % 2 && (now.odd >> lane & 1)) {
+#pragma unroll
+        for (int n = 0; n < kScaleWords; ++n) raw[a][n] = raw[a][n] >> 16 | raw[a][n + 1] << 16;
+      }
+#pragma unroll
+      for (int g = 0; g < GP; ++g)
+        scale_lds[wave][a][g][lane] = static_cast<uint16_t>(g < p.groups ? raw[a][g / 2] >> (16 * (g % 2)) : 0u);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    uint32_t skw[8], svw[8];
+    __builtin_memcpy(skw, __builtin_assume_aligned(&scale_lds[wave][0][own_g][16 * lg], 16), 32);
+    __builtin_memcpy(svw, __builtin_assume_aligned(&scale_lds[wave][1][own_g][16 * lg], 16), 32);
+    // it is read: the stage after the next may take its place
+    Stage later{};
+    if (i + 2 < stages) {
+      later = locate(base + 2 * kTile);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      copy_stage(later, buf);
+    }
+    // ---- scores
+    f32x4 s_acc[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      f32x4 s = {c_init, c_init, c_init, c_init};
+#pragma unroll
+      for (int j = 0; j < kSlices; ++j) {
+        const u32x4 a = BITS == 4 ? key_operand<BITS>(kw[u][j], 0, masks) : key_operand<BITS>(kw[u][j / 2], j % 2, masks);
+        s = mfma16(a, q[0][j], s);
+        if constexpr (PREC) s = mfma16(a, q[kParts - 1][j], s);
+      }
+      s_acc[u] = s;
+    }
+    u32x4 w[kParts][2];
+    if (now.live == ~0ull) weigh(base, now.live, s_acc, skw, svw, w, std::false_type{});
+    else weigh(base, now.live, s_acc, skw, svw, w, std::true_type{});
     // ---- weights times values: 8 bytes of a row a read, 16 (INT4) or 32 (INT2) dims
 #pragma unroll
     for (int r = 0; r < kRow / 8; ++r) {
-      const i32x2 x = lds_read_tr4(stage, value_at + (((r / 2) ^ value_turn) * 16) + r % 2 * 8);
+      const i32x2 x = vw[r];
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -646,27 +735,8 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
           if constexpr (PREC) acc[tile] = mfma16(w[kParts - 1][s], b, acc[tile]);
         }
     }
-  };
-
-  int buf = 0;
-  for (int base = begin; base < end; base += kTile, buf ^= 1) {
-    // the stage's copies (and scales) have landed, and nothing reads the buffer that the next one goes to
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-#pragma unroll
-    for (int g = 0; g < GP; ++g) {
-      scale_lds[wave][0][g][lane] = static_cast<uint16_t>(g < p.groups ? scale_k[g / 2] >> (16 * (g % 2)) : 0u);
-      scale_lds[wave][1][g][lane] = static_cast<uint16_t>(g < p.groups ? scale_v[g / 2] >> (16 * (g % 2)) : 0u);
-    }
-    const uint64_t live_mask = __ballot(live != 0);
-    if (base + kTile < end) {
-      issue(base + kTile, buf ^ 1);
-      if constexpr (UNI) fetch_pages(base + 2 * kTile);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (live_mask == ~0ull) compute(base, buf, live_mask, std::false_type{});
-    else compute(base, buf, live_mask, std::true_type{});
-    __builtin_amdgcn_wave_barrier();
+    now = next;
+    next = later;
   }
 
   // ---- this run's partial, or the result where a sequence has one run
@@ -710,7 +780,7 @@ int launch_paged_kernel(const PagedDecodeParams& p, hipStream_t stream) {
   const dim3 grid((p.runs + p.group_runs - 1) / p.group_runs, p.groups_of_units);
   const dim3 block(p.group_units * p.group_runs * kWave);
   if constexpr (DP * BITS >= 256) {
-    if (p.c.page_tokens % 32 == 0 && p.c.head_dim * BITS % 128 == 0) {
+    if (p.c.page_tokens % 32 == 0 && p.c.head_dim * BITS % 128 == 0 && !(p.groups % 2 && p.c.kv_heads % 2)) {
       hipLaunchKernelGGL((paged_decode_kernel<BITS, DP, GP, PREC, true>), grid, block, 0, stream, p);
       return hip_status(hipGetLastError(), "paged_decode launch");
     }
