@@ -24,28 +24,31 @@
 // number, so that neither the key rows' nor the value columns' reads meet in a
 // bank.  Scales are laid out by group in LDS when their stage begins.
 //
-// QK (v_mfma_f32_16x16x32_f16): rows = 16 slots' codes, columns = (query head,
-//   group): the query masked to one group, so that a column's sum is one group's
-//   and its scale multiplies in 32 bits afterwards.  A code enters as the fp16
-//   number 1 + c / 2^6 (INT4) or 1 + c / 2^2 (a bit operation for a pair); the
-//   offset's share, -(1 + mid/2^6) sum q, is the accumulator's initial value.
-//   The query is scaled by a power of two per head into fp16's range (exact for
-//   fp16 and bf16) and, with 32-bit results, taken as a sum of two fp16 parts.
-//   Tile u's row r is slot 16 (r / 4) + 4 u + r % 4: a lane's results are then
-//   its (head, group)'s scores of the 16 slots 16 (lane / 16) + e.
-// Softmax in the columns' lanes; the groups' shares meet by lane exchanges
-//   within 8 lanes.  The running maximum is lazy: scores up to 2^6 above the
-//   reference are summed as they are (no wave-wide maximum per stage); where one
-//   exceeds that, all lanes take the new maximum and rescale.  The reference
-//   also holds the exponent of the largest value scale met, so that W =
-//   2^(s - m) sv lies in fp16's normal range (at most 2^15) whatever the scales'
-//   size.
-// PV: rows = (head, group) weights W, columns = 16 dims, K = 32 slots.  The QK
-//   results' lanes are the A operand's, so W needs no exchange; V's codes come
-//   transposed from LDS (ds_read_b64_tr_b4: a dim's codes of 16 slots a lane)
-//   and enter as the exact numbers (c - mid) / 2^6: an offset taken out of the
-//   sums afterwards would cost a share of their precision that grows with the
-//   number of slots.  Of a column's 16 rows those of its own group count.
+// QK (v_mfma_f32_16x16x32_f16): one side is 16 slots' codes, the other (query
+//   head, group): the query masked to one group, so that a result is one group's
+//   share of a score and its scale multiplies in 32 bits afterwards.  A code
+//   enters as the fp16 number 1 + c / 2^6 (INT4) or 1 + c / 2^2 (a bit operation
+//   for a pair); the offset's share, -(1 + mid/2^6) sum q, is the accumulator's
+//   initial value.  The query is scaled by a power of two per head into fp16's
+//   range (exact for fp16 and bf16) and, with 32-bit results, taken as a sum of
+//   two fp16 parts.
+// Four groups and more (GP >= 4): rows = (head, group), columns = slots.  A lane
+//   holds a slot's shares of four groups and adds them itself; the softmax's 2^x
+//   go through LDS to the lanes that form the weights.  One or two groups: rows =
+//   slots, columns = (head, group), whose lanes are the weights' lanes; with two,
+//   the lanes of a head form the same scores twice.  (For four groups that form
+//   took 570 instructions a stage, this one 470.)
+// Softmax.  The running maximum is lazy: scores up to 2^6 above the reference are
+//   summed as they are (no wave-wide maximum per stage); where one exceeds that,
+//   all lanes take the new maximum and rescale.  The reference also holds the
+//   exponent of the largest value scale met, so that W = 2^(s - m) sv lies in
+//   fp16's normal range (at most 2^15) whatever the scales' size.
+// PV: rows = (head, group) weights W, columns = 16 dims, K = 32 slots: lane
+//   (row, lane / 16) forms those of the 16 slots 16 (lane / 16) + e.  V's codes
+//   come transposed from LDS (ds_read_b64_tr_b4: a dim's codes of 16 slots a
+//   lane) and enter as the exact numbers (c - mid) / 2^6: an offset taken out of
+//   the sums afterwards would cost a share of their precision that grows with
+//   the number of slots.  Of a column's 16 rows those of its own group count.
 //   Where 32-bit grade is asked for, W is a sum of two fp16 parts.
 #pragma once
 
@@ -308,7 +311,12 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   constexpr int kStageCopies = 2 * (kChunks + kScaleCopies);
   __shared__ __attribute__((aligned(1024))) uint8_t codes_lds[kWaves][2][2 * kArray];
   __shared__ __attribute__((aligned(16))) uint32_t raw_lds[kWaves][2][2][kTile][kScaleWords];
-  __shared__ __attribute__((aligned(16))) uint16_t scale_lds[kWaves][2][GP][kTile];
+  constexpr bool kSlotColumns = GP >= 4;   // QK with slots in the columns
+  // [keys (where they are rows), values][group][slot], and the softmax's powers [head][slot] (rows 16 bytes apart in
+  // the banks)
+  __shared__ __attribute__((aligned(16))) uint16_t scale_lds[kWaves][kSlotColumns ? 1 : 2][GP][kTile];
+  constexpr int kPowerRow = kTile + 4;
+  __shared__ __attribute__((aligned(16))) float power_lds[kWaves][kSlotColumns ? kHeads * kPowerRow : 1];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
@@ -531,6 +539,16 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     sum += __shfl_xor(sum, 32, kWave);
     c_init = -kOff * sum;
   }
+  // of the lane's own results: rows 4 lg + i, all of one head, or its column
+  f32x4 c_rows = {c_init, c_init, c_init, c_init};
+  int head_own = head;
+  if constexpr (kSlotColumns) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c_rows[i] = __shfl(c_init, 4 * lg + i, kWave);
+    s_factor = __shfl(s_factor, 4 * lg, kWave);
+    head_own = head_first + 4 * lg / GP;
+  }
+  asm("" : "+v"(c_rows));  // (kept in registers, not formed anew for every product)
   // the query is read: the second stage may follow
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   if (crowded && stages > 0) copy_stage(now, 0);
@@ -540,10 +558,11 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   }
 
   // ---- where the lane reads a stage's codes
-  int key_at[4];  // tile u: slot 16 (col / 4) + 4 u + col % 4 (and, in DP 256, chunks kChunks / 2 on)
+  // QK tile u's slots: 16 u + column, or row r: 16 (r / 4) + 4 u + r % 4 (and, in DP 256, chunks kChunks / 2 on)
+  int key_at[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const int slot = 16 * (col / 4) + 4 * u + col % 4;
+    const int slot = kSlotColumns ? 16 * u + col : 16 * (col / 4) + 4 * u + col % 4;
     constexpr int kLaneBytes = (DP == 256 ? 128 : DP) * BITS / 32;  // of a lane's piece: 16, 8 or 4
     key_at[u] = slot * kRow + ((lg * kLaneBytes / 16) ^ turned(slot)) * 16 + lg * kLaneBytes % 16;
   }
@@ -562,8 +581,29 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   bool first = true;
 
   constexpr int kLaneBytes = (DP == 256 ? 128 : DP) * BITS / 32;  // of a lane's piece of a key row: 16, 8 or 4
-  // a stage's weights from its scores; some of its slots may take no part (kRagged)
-  auto weigh = [&](int base, uint64_t live, f32x4 (&s_acc)[4], const uint32_t (&skw)[8], uint32_t (&svw)[8],
+  // weights of a lane's 16 slots: pairs (e, e + 4) of each step's 8, the order of the values' pairs
+  auto form_weights = [&](const float (&tv)[16], const uint32_t (&svw)[8], u32x4 (&w)[kParts][2]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int e0 = 8 * s + k, e1 = e0 + 4;
+        if constexpr (PREC) {
+          // one product in 32 bits for both parts: a first part rounded straight from the factors (v_fma_mixlo_f16)
+          // may be the other of its two neighbours, and the parts' sum then a step of it off
+          float a = tv[e0] * half_of(svw, e0), b = tv[e1] * half_of(svw, e1);
+          asm("" : "+v"(a), "+v"(b));
+          const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
+          w[0][s][k] = pack_half2(ah, bh);
+          w[kParts - 1][s][k] = pack_half2(static_cast<_Float16>(a - static_cast<float>(ah)),
+                                           static_cast<_Float16>(b - static_cast<float>(bh)));
+        } else {
+          w[0][s][k] = wpair(tv[e0], half_of(svw, e0), tv[e1], half_of(svw, e1));
+        }
+      }
+  };
+  // slots in the rows: the lane's column's weights of its slots 16 lg + e; some may take no part (kRagged)
+  auto weigh_rows = [&](int base, uint64_t live, f32x4 (&s_acc)[4], const uint32_t (&skw)[8], uint32_t (&svw)[8],
                    u32x4 (&w)[kParts][2], auto ragged_tag) {
     constexpr bool kRagged = decltype(ragged_tag)::value;
     const uint32_t mask16 = static_cast<uint32_t>(live >> (16 * lg)) & 0xFFFFu;  // slots 16 lg + e
@@ -590,8 +630,6 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       float x = __builtin_fmaf(s_acc[e / 4][e % 4], half_of(skw, e), 0.0f);
       asm("" : "+v"(x));
       if constexpr (GP > 1) x = dpp_add<0xB1>(x);
-      if constexpr (GP > 2) x = dpp_add<0x4E>(x);
-      if constexpr (GP > 4) x = dpp_add<0x141>(x);
       s_acc[e / 4][e % 4] = x;
       tv[e] = kRagged && !(mask16 >> e & 1u) ? -INFINITY : __builtin_fmaf(x, s_factor, -m_ref);
       top = fmaxf(top, tv[e]);
@@ -636,30 +674,65 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
         *reinterpret_cast<f32x4*>(dst + 4 * u) = v;
       }
     }
-    // ---- weights: pairs (e, e + 4) of each step's 8 slots, the order of the values' pairs
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       tv[e] = __builtin_amdgcn_exp2f(tv[e]);
       l += tv[e];
     }
+    form_weights(tv, svw, w);
+  };
+
+  // slots in the columns: the powers of the lane's slots 16 u + col, of one head, left in LDS
+  auto weigh_columns = [&](int base, uint64_t live, int e_stage, const f32x4 (&s_acc)[4], const uint32_t (&skw)[4][2],
+                           auto ragged_tag) {
+    constexpr bool kRagged = decltype(ragged_tag)::value;
+    float s[4], tv[4];
+    float top = -INFINITY;
+    bool out[4];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int u = 0; u < 4; ++u) {
+      float x = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int e0 = 8 * s + k, e1 = e0 + 4;
-        if constexpr (PREC) {
-          // one product in 32 bits for both parts: a first part rounded straight from the factors (v_fma_mixlo_f16)
-          // may be the other of its two neighbours, and the parts' sum then a step of it off
-          float a = tv[e0] * half_of(svw, e0), b = tv[e1] * half_of(svw, e1);
-          asm("" : "+v"(a), "+v"(b));
-          const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
-          w[0][s][k] = pack_half2(ah, bh);
-          w[kParts - 1][s][k] = pack_half2(static_cast<_Float16>(a - static_cast<float>(ah)),
-                                           static_cast<_Float16>(b - static_cast<float>(bh)));
-        } else {
-          w[0][s][k] = wpair(tv[e0], half_of(svw, e0), tv[e1], half_of(svw, e1));
-        }
+      for (int i = 0; i < 4; ++i) x = __builtin_fmaf(s_acc[u][i], half_of(skw[u], i), x);
+      if constexpr (GP == 8) x += __shfl_xor(x, 16, kWave);
+      out[u] = kRagged && !(live >> (16 * u + col) & 1);
+      s[u] = x;
+      tv[u] = out[u] ? -INFINITY : __builtin_fmaf(x, s_factor, -m_ref);
+      top = fmaxf(top, tv[u]);
+    }
+    if (first || __any(e_stage > w_exp || top > kLazy - static_cast<float>(w_exp))) {
+      // new reference points: the largest score so far and the largest value scale so far
+      const int e_new = max(wave_most(e_stage + 32) - 32, w_exp);
+      top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) top = out[u] ? top : fmaxf(top, s[u] * s_factor);
+      top = row_max16(top);
+      if constexpr (GP == 8) top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      const float m_old = m_ref - static_cast<float>(w_exp);
+      const float ref = fmaxf(first ? -INFINITY : m_old, top) + static_cast<float>(e_new);
+      const float alpha = first ? 0.0f : (ref == m_ref ? 1.0f : exp2f(m_ref - ref));
+      m_ref = ref;
+      if (!first) {
+        l *= alpha;
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) acc[k] *= alpha;  // (rows of the lane's own head)
       }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) tv[u] = out[u] ? -INFINITY : __builtin_fmaf(s[u], s_factor, -m_ref);
+      w_exp = e_new;
+      first = false;
+    }
+    if (p.scores != nullptr && (GP < 8 || lg % 2 == 0) && head_own < p.gq) {
+      float* dst = p.scores + (head0 + head_own) * p.score_stride + base + col;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) dst[16 * u] = out[u] ? -INFINITY : s[u] * s_factor;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float e = __builtin_amdgcn_exp2f(tv[u]);
+      l += e;
+      power_lds[wave][4 * lg / GP * kPowerRow + 16 * u + col] = e;
+    }
   };
 
   for (int i = 0, base = begin; i < stages; ++i, base += kTile) {
@@ -669,9 +742,30 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     asm volatile("" ::: "memory");
     const int buf = i & 1;
     const uint8_t* stage = codes_lds[wave][buf];
+    // Scales of slot `lane` as they were copied.  Groups that are fewer than GP, or begin in a word's upper half, are
+    // put in order first, the missing ones as zeros (nothing else may meet a sum of zero products).
+    const bool uneven = p.groups != GP;
     uint32_t raw[2][kScaleWords + 1];
 #pragma unroll
-    for (int a = 0; a < 2; ++a) __builtin_memcpy(raw[a], __builtin_assume_aligned(raw_lds[wave][buf][a][lane], 4 * kScaleWords), 4 * kScaleWords);
+    for (int a = kSlotColumns ? 1 : 0; a < 2; ++a)
+      __builtin_memcpy(raw[a], __builtin_assume_aligned(raw_lds[wave][buf][a][lane], 4 * kScaleWords), 4 * kScaleWords);
+    if (kSlotColumns && uneven)
+      __builtin_memcpy(raw[0], __builtin_assume_aligned(raw_lds[wave][buf][0][lane], 4 * kScaleWords), 4 * kScaleWords);
+    if (uneven || GP == 1) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        raw[a][kScaleWords] = 0;
+        if (now.odd >> lane & 1) {
+#pragma unroll
+          for (int n = 0; n < kScaleWords; ++n) raw[a][n] = raw[a][n] >> 16 | raw[a][n + 1] << 16;
+        }
+#pragma unroll
+        for (int n = 0; n < kScaleWords; ++n)
+          raw[a][n] = 2 * n + 1 < p.groups ? raw[a][n] : 2 * n < p.groups ? raw[a][n] & 0xFFFFu : 0u;
+      }
+      if constexpr (kSlotColumns)
+        __builtin_memcpy(__builtin_assume_aligned(raw_lds[wave][buf][0][lane], 4 * kScaleWords), raw[0], 4 * kScaleWords);
+    }
     uint32_t kw[4][kSpan * BITS / 32];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -683,21 +777,21 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
 #pragma unroll
     for (int r = 0; r < kRow / 8; ++r) vw[r] = lds_read_tr4(stage, value_at + (((r / 2) ^ value_turn) * 16) + r % 2 * 8);
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      raw[a][kScaleWords] = 0;
-      if (p.groups % 2 && (now.odd >> lane & 1)) {
-#pragma unroll
-        for (int n = 0; n < kScaleWords; ++n) raw[a][n] = raw[a][n] >> 16 | raw[a][n + 1] << 16;
-      }
+    for (int a = kSlotColumns ? 1 : 0; a < 2; ++a)
 #pragma unroll
       for (int g = 0; g < GP; ++g)
-        scale_lds[wave][a][g][lane] = static_cast<uint16_t>(g < p.groups ? raw[a][g / 2] >> (16 * (g % 2)) : 0u);
-    }
+        scale_lds[wave][kSlotColumns ? 0 : a][g][lane] = static_cast<uint16_t>(raw[a][g / 2] >> (16 * (g % 2)));
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    uint32_t skw[8], svw[8];
-    __builtin_memcpy(skw, __builtin_assume_aligned(&scale_lds[wave][0][own_g][16 * lg], 16), 32);
-    __builtin_memcpy(svw, __builtin_assume_aligned(&scale_lds[wave][1][own_g][16 * lg], 16), 32);
+    uint32_t skw[8], svw[8], sk_slot[4][2];
+    if constexpr (kSlotColumns) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        __builtin_memcpy(sk_slot[u], __builtin_assume_aligned(&raw_lds[wave][buf][0][16 * u + col][GP == 8 ? lg % 2 * 2 : 0], 8), 8);
+    } else {
+      __builtin_memcpy(skw, __builtin_assume_aligned(&scale_lds[wave][0][own_g][16 * lg], 16), 32);
+    }
+    __builtin_memcpy(svw, __builtin_assume_aligned(&scale_lds[wave][kSlotColumns ? 0 : 1][own_g][16 * lg], 16), 32);
     // it is read: the stage after the next may take its place
     Stage later{};
     if (i + 2 < stages) {
@@ -709,18 +803,42 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     f32x4 s_acc[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      f32x4 s = {c_init, c_init, c_init, c_init};
+      f32x4 s = c_rows;
 #pragma unroll
       for (int j = 0; j < kSlices; ++j) {
         const u32x4 a = BITS == 4 ? key_operand<BITS>(kw[u][j], 0, masks) : key_operand<BITS>(kw[u][j / 2], j % 2, masks);
-        s = mfma16(a, q[0][j], s);
-        if constexpr (PREC) s = mfma16(a, q[kParts - 1][j], s);
+#pragma unroll
+        for (int n = 0; n < kParts; ++n) s = kSlotColumns ? mfma16(q[n][j], a, s) : mfma16(a, q[n][j], s);
       }
       s_acc[u] = s;
     }
     u32x4 w[kParts][2];
-    if (now.live == ~0ull) weigh(base, now.live, s_acc, skw, svw, w, std::false_type{});
-    else weigh(base, now.live, s_acc, skw, svw, w, std::true_type{});
+    if constexpr (kSlotColumns) {
+      // exponent of the slot's largest value scale; none of a slot that takes no part, whose scales may be anything
+      // (its weights are 0, and so have its scales to be; codes are always finite)
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 m = __builtin_bit_cast(u16x2, raw[1][0] & 0x7FFF7FFFu);
+#pragma unroll
+      for (int n = 1; n < GP / 2; ++n) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, raw[1][n] & 0x7FFF7FFFu));
+      const int e_stage = (m[0] > m[1] ? m[0] >> 10 : m[1] >> 10) - 23;
+      if (now.live == ~0ull) {
+        weigh_columns(base, now.live, e_stage, s_acc, sk_slot, std::false_type{});
+      } else {
+        weigh_columns(base, now.live, now.live >> lane & 1 ? e_stage : -32, s_acc, sk_slot, std::true_type{});
+        const uint32_t mask16 = static_cast<uint32_t>(now.live >> (16 * lg)) & 0xFFFFu;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!(mask16 >> e & 1u)) svw[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      float powers[16];
+      __builtin_memcpy(powers, __builtin_assume_aligned(&power_lds[wave][col / GP * kPowerRow + 16 * lg], 16), 64);
+      form_weights(powers, svw, w);
+    } else {
+      if (now.live == ~0ull) weigh_rows(base, now.live, s_acc, skw, svw, w, std::false_type{});
+      else weigh_rows(base, now.live, s_acc, skw, svw, w, std::true_type{});
+    }
     // ---- weights times values: 8 bytes of a row a read, 16 (INT4) or 32 (INT2) dims
 #pragma unroll
     for (int r = 0; r < kRow / 8; ++r) {
@@ -742,15 +860,19 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   // ---- this run's partial, or the result where a sequence has one run
   const bool whole = p.runs <= c.sequences;
   const int64_t part0 = static_cast<int64_t>(run) * p.query_heads + kvh * p.gq;
-  l += __shfl_xor(l, 16, kWave);
-  l += __shfl_xor(l, 32, kWave);
+  if constexpr (kSlotColumns) {
+    l = row_sum16(l);
+  } else {
+    l += __shfl_xor(l, 16, kWave);
+    l += __shfl_xor(l, 32, kWave);
+  }
   // a column tile's dims are of one group gk; of the lane's rows 4 lg + i = (head, group) the kRows with that group
   // hold them
   constexpr int kRows = 4 / (GP < 4 ? GP : 4);
 #pragma unroll
   for (int n = 0; n < kRows; ++n) {
     const int h = GP >= 4 ? 4 * lg / GP : kRows * lg + n;  // within the head tile
-    const float l_head = __shfl(l, h * GP, kWave);
+    const float l_head = kSlotColumns ? l : __shfl(l, h * GP, kWave);
     const float factor = !whole ? kF : l_head == 0.0f ? 0.0f : kF / l_head;
     const bool has = head_first + h < p.gq;
 #pragma unroll
@@ -765,12 +887,12 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       else p.part_o[(part0 + head_first + h) * d + dim] = v;
     }
   }
-  if (lg == 0 && own_g == 0 && head < p.gq) {
+  if (kSlotColumns ? col == 0 && (GP < 8 || lg % 2 == 0) && head_own < p.gq : lg == 0 && own_g == 0 && head < p.gq) {
     if (whole) {
-      p.lse[head0 + head] = l == 0.0f ? -INFINITY : kLn2 * (m_ref + log2f(l));
+      p.lse[head0 + head_own] = l == 0.0f ? -INFINITY : kLn2 * (m_ref + log2f(l));
     } else {
-      p.part_ml[2 * (part0 + head)] = m_ref;
-      p.part_ml[2 * (part0 + head) + 1] = l;
+      p.part_ml[2 * (part0 + head_own)] = m_ref;
+      p.part_ml[2 * (part0 + head_own) + 1] = l;
     }
   }
 }
