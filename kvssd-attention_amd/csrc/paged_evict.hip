@@ -17,189 +17,525 @@
 namespace kvssd {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / kWave;
 constexpr int kBins = 2048;
+constexpr int kPasses = 3;
+constexpr int kOneThreads = 1024, kOneSlots = 8 * kOneThreads;  // a sequence of one workgroup
+constexpr int kChunkThreads = 256, kKeys = 8;                    // a chunk of one: kKeys slots a thread at a time
+constexpr int kChunkSlots = kKeys * kChunkThreads, kMostChunks = 1024;
+constexpr int kInnerMoves = 256;  // so few rows move within the selecting workgroup
+constexpr uint32_t kHeld = 0xFFFFFFFFu;
 
 struct EvictParams {
   kvssd_paged_cache c;
   int32_t* lengths_out;
   float* weights_out;
   int32_t* positions_out;
-  int32_t* counts;  // [sequences]: rows to move
-  int32_t* to;      // [sequences][most]
+  int32_t* counts;    // [sequences]: rows to move
+  int32_t* to;        // [sequences][most]
   int32_t* from;
-  int budget, sink, recent, capacity, most;
+  int32_t* state;     // [sequences][kState]
+  int32_t* hist;      // [sequences][kPasses][kBins]
+  int32_t* chunk;     // [sequences][chunks][4]: latest position; then slots above and equal to the threshold, by side
+  int budget, sink, recent, capacity, most, chunks, chunk_slots;
 };
+constexpr int kState = 2 * kPasses + 1;  // (key, need) after every pass, then the latest position
 
 __device__ __forceinline__ uint32_t weight_key(float w, int position, int sink, int64_t latest, int recent) {
-  if (position < sink || position > latest - recent) return 0xFFFFFFFFu;
+  if (position < sink || position > latest - recent) return kHeld;
   if (!(w == w)) w = -INFINITY;
   const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);  // -0 counts as 0
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Exclusive prefix count of `flag` over the workgroup's threads; *total: of all.
-__device__ __forceinline__ int prefix_count(bool flag, int* scratch, int* total) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const uint64_t mask = __ballot(flag);
-  if (lane == 0) scratch[wave] = __popcll(mask);
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    const int x = scratch[w];
-    before += w < wave ? x : 0;
-    all += x;
-  }
-  __syncthreads();
-  *total = all;
-  return before + __popcll(mask & ((1ull << lane) - 1));
+__device__ __forceinline__ int pass_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__device__ __forceinline__ uint32_t pass_above(int pass) { return pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u; }
+
+// Counts a key's digit; held keys, many and alike, once a wave.
+__device__ __forceinline__ void count_key(int* hist, uint32_t k, bool live, int pass, uint32_t key) {
+  const bool of = live && (k & pass_above(pass)) == key;
+  const uint64_t held = __ballot(of && k == kHeld);
+  const uint32_t digit = (k >> pass_shift(pass)) & (pass == 2 ? 1023u : 2047u);
+  if (of && k != kHeld) atomicAdd(&hist[digit], 1);
+  if (held != 0 && threadIdx.x % kWave == __builtin_ctzll(held)) atomicAdd(&hist[digit], __popcll(held));
 }
 
-__global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictParams p) {
+__device__ __forceinline__ int wave_inclusive(int x) {
+  const int lane = threadIdx.x % kWave;
+  for (int k = 1; k < kWave; k <<= 1) {
+    const int y = __shfl_up(x, k, kWave);
+    if (lane >= k) x += y;
+  }
+  return x;
+}
+
+// The bin, counted from the top, in which the need-th key lies, and the keys above it; -> key and need.
+template <int THREADS>
+__device__ __forceinline__ void find_digit(const int* hist, int pass, uint32_t& key, int& need, int* scratch) {
+  constexpr int kEach = kBins / THREADS;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  int c[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) sum += c[i] = hist[kBins - 1 - kEach * tid - i];
+  const int incl = wave_inclusive(sum);
+  if (lane == kWave - 1) scratch[wave] = incl;
+  __syncthreads();
+  int before = incl - sum;
+  for (int w = 0; w < wave; ++w) before += scratch[w];
+  int* found = scratch + THREADS / kWave;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (before < need && need <= before + c[i]) {
+      found[0] = kBins - 1 - kEach * tid - i;
+      found[1] = before;
+    }
+    before += c[i];
+  }
+  __syncthreads();
+  key |= static_cast<uint32_t>(found[0]) << pass_shift(pass);
+  need -= found[1];
+}
+
+// Exclusive prefix counts, in slot order, of flags over the slots j THREADS + thread, j < KEYS; total: of all.  The
+// counts of two kinds of flags go in a word's halves (at most 2^14 slots).
+template <int THREADS, int KEYS>
+__device__ __forceinline__ void prefix_counts(const uint32_t (&flag)[KEYS], uint32_t (&before)[KEYS], uint32_t& total,
+                                              uint32_t* scratch) {
+  constexpr int kWaves = THREADS / kWave, kEntries = KEYS * kWaves, kEach = (kEntries + kWave - 1) / kWave;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint64_t lower = (1ull << lane) - 1;
+  __syncthreads();  // (scratch is free)
+#pragma unroll
+  for (int j = 0; j < KEYS; ++j) {
+    const uint64_t a = __ballot(flag[j] & 0xFFFFu), b = __ballot(flag[j] >> 16);
+    before[j] = __popcll(a & lower) | __popcll(b & lower) << 16;
+    if (lane == 0) scratch[j * kWaves + wave] = __popcll(a) | __popcll(b) << 16;
+  }
+  __syncthreads();
+  uint32_t e[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int at = lane * kEach + i;
+    e[i] = sum;
+    sum += at < kEntries ? scratch[at] : 0;
+  }
+  const uint32_t incl = wave_inclusive(sum);
+  total = __shfl(incl, kWave - 1, kWave);
+#pragma unroll
+  for (int j = 0; j < KEYS; ++j) {
+    const int at = j * kWaves + wave;
+    uint32_t x = __shfl(incl - sum, at / kEach, kWave);
+#pragma unroll
+    for (int i = 1; i < kEach; ++i) {
+      const uint32_t y = __shfl(incl - sum + e[i], at / kEach, kWave);
+      x = at % kEach == i ? y : x;
+    }
+    before[j] += x;
+  }
+}
+
+// A wave moves slot f to slot t: codes of K and V, scales of every kv head, weight and position.
+__device__ __forceinline__ void move_slot(const EvictParams& p, int b, int t, int f) {
+  const int lane = threadIdx.x % kWave;
+  const kvssd_paged_cache& c = p.c;
+  const int64_t row = static_cast<int64_t>(b) * p.capacity;
+  if (lane == 0) {
+    p.weights_out[row + t] = c.weights[row + f];
+    p.positions_out[row + t] = c.positions[row + f];
+  }
+  const int32_t* pages = c.page_table + static_cast<int64_t>(b) * c.max_pages;
+  const int tp = pages[t / c.page_tokens], fp = pages[f / c.page_tokens];
+  if (tp < 0 || tp >= c.num_pages || fp < 0 || fp >= c.num_pages) return;
+  const int64_t code_bytes = static_cast<int64_t>(c.kv_heads) * c.head_dim * c.bits / 8;
+  const int64_t scale_count = static_cast<int64_t>(c.kv_heads) * (c.head_dim / c.group_size);
+  const int64_t dst = static_cast<int64_t>(tp) * c.page_tokens + t % c.page_tokens;
+  const int64_t src = static_cast<int64_t>(fp) * c.page_tokens + f % c.page_tokens;
+  for (int64_t at = lane * 8; at < code_bytes; at += kWave * 8) {  // rows are multiples of 8 bytes
+    *reinterpret_cast<uint64_t*>(c.packed_k + dst * code_bytes + at) =
+        *reinterpret_cast<const uint64_t*>(c.packed_k + src * code_bytes + at);
+    *reinterpret_cast<uint64_t*>(c.packed_v + dst * code_bytes + at) =
+        *reinterpret_cast<const uint64_t*>(c.packed_v + src * code_bytes + at);
+  }
+  for (int64_t at = lane; at < scale_count; at += kWave) {
+    c.scales_k[dst * scale_count + at] = c.scales_k[src * scale_count + at];
+    c.scales_v[dst * scale_count + at] = c.scales_v[src * scale_count + at];
+  }
+}
+
+__device__ __forceinline__ void clear_tail(const EvictParams& p, int64_t row, int begin, int end, int step) {
+  for (int s = begin + threadIdx.x; s < end; s += step) {
+    p.weights_out[row + s] = 0.0f;
+    p.positions_out[row + s] = -1;
+  }
+}
+
+// A sequence of at most kOneSlots slots in one workgroup: weights and positions are read once and stay in registers.
+template <bool INNER>
+__global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictParams p) {
+  constexpr int T = kOneThreads, K = kOneSlots / T;
   __shared__ int hist[kBins];
-  __shared__ int scratch[kWaves];
-  __shared__ int found[2];  // digit, keys above it
+  __shared__ uint32_t scratch[kOneSlots / kWave];
+  __shared__ int small[T / kWave + 2];
+  __shared__ int moves[2][INNER ? kInnerMoves : 1];
   const int b = blockIdx.x, tid = threadIdx.x;
   const int n = paged_length(p.c.lengths, b, p.capacity);
   const int m = n < p.budget ? n : p.budget;
   const int64_t row = static_cast<int64_t>(b) * p.capacity;
-  const float* weights = p.c.weights + row;
-  const int32_t* positions = p.c.positions + row;
-  float* weights_out = p.weights_out + row;
-  int32_t* positions_out = p.positions_out + row;
   if (tid == 0) p.lengths_out[b] = m;
-  for (int s = m + tid; s < p.capacity; s += kThreads) {
-    weights_out[s] = 0.0f;
-    positions_out[s] = -1;
-  }
-  if (n <= p.budget) {
-    for (int s = tid; s < n; s += kThreads) {
-      weights_out[s] = weights[s];
-      positions_out[s] = positions[s];
+  float w[K];
+  int pos[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    const int s = j * T + tid;
+    w[j] = 0.0f;
+    pos[j] = INT32_MIN;
+    if (s < n) {
+      w[j] = p.c.weights[row + s];
+      pos[j] = p.c.positions[row + s];
     }
-    if (tid == 0) p.counts[b] = 0;
+  }
+  clear_tail(p, row, m, p.capacity, T);
+  if (n <= p.budget) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      const int s = j * T + tid;
+      if (s < n) {
+        p.weights_out[row + s] = w[j];
+        p.positions_out[row + s] = pos[j];
+      }
+    }
+    if (!INNER && tid == 0) p.counts[b] = 0;
     return;
   }
-  // ---- the latest position
   int latest = INT32_MIN;
-  for (int s = tid; s < n; s += kThreads) latest = max(latest, positions[s]);
+#pragma unroll
+  for (int j = 0; j < K; ++j) latest = max(latest, pos[j]);
   for (int k = 1; k < kWave; k <<= 1) latest = max(latest, __shfl_xor(latest, k, kWave));
-  if (tid % kWave == 0) scratch[tid / kWave] = latest;
+  if (tid % kWave == 0) small[tid / kWave] = latest;
   __syncthreads();
-  for (int w = 0; w < kWaves; ++w) latest = max(latest, scratch[w]);
-  __syncthreads();
-  // ---- the threshold key, digit by digit from the top
+  for (int v = 0; v < T / kWave; ++v) latest = max(latest, small[v]);
+  uint32_t k[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) k[j] = weight_key(w[j], pos[j], p.sink, latest, p.recent);
   uint32_t key = 0;  // digits found so far
   int need = m;      // kept keys among those that share them
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const uint32_t digits = pass == 2 ? 1023u : 2047u;
-    const uint32_t above = pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
-    for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+  for (int pass = 0; pass < kPasses; ++pass) {
+    for (int i = tid; i < kBins; i += T) hist[i] = 0;
     __syncthreads();
-    for (int s = tid; s < n; s += kThreads) {
-      const uint32_t k = weight_key(weights[s], positions[s], p.sink, latest, p.recent);
-      if ((k & above) == key) atomicAdd(&hist[(k >> shift) & digits], 1);
-    }
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (j * T < n) count_key(hist, k[j], j * T + tid < n, pass, key);
     __syncthreads();
-    // bins in falling order, two a thread: the one in which the need-th key lies
-    const int i0 = kBins - 1 - 2 * tid;
-    const int c0 = hist[i0], c1 = hist[i0 - 1];
-    int sum = c0 + c1;
-    const int lane = tid % kWave, wave = tid / kWave;
-    int incl = sum;
-    for (int k = 1; k < kWave; k <<= 1) {
-      const int x = __shfl_up(incl, k, kWave);
-      if (lane >= k) incl += x;
-    }
-    if (lane == kWave - 1) scratch[wave] = incl;
-    __syncthreads();
-    int before = incl - sum;
-    for (int w = 0; w < wave; ++w) before += scratch[w];
-    if (before < need && need <= before + c0) {
-      found[0] = i0;
-      found[1] = before;
-    } else if (before + c0 < need && need <= before + sum) {
-      found[0] = i0 - 1;
-      found[1] = before + c0;
-    }
-    __syncthreads();
-    key |= static_cast<uint32_t>(found[0]) << shift;
-    need -= found[1];
+    find_digit<T>(hist, pass, key, need, small);
     __syncthreads();
   }
-  // ---- keys above the threshold stay, and the first `need` of those equal to it
-  int32_t* to = p.to + static_cast<int64_t>(b) * p.most;
-  int32_t* from = p.from + static_cast<int64_t>(b) * p.most;
-  int equal_before = 0, moved_to = 0, moved_from = 0;
-  for (int base = 0; base < n; base += kThreads) {
-    const int s = base + tid;
-    float w = 0.0f;
-    int pos = 0;
-    uint32_t k = 0;
-    if (s < n) {
-      w = weights[s];
-      pos = positions[s];
-      k = weight_key(w, pos, p.sink, latest, p.recent);
-    }
-    int total;
-    const bool equal = s < n && k == key;
-    const int rank = equal_before + prefix_count(equal, scratch, &total);
-    equal_before += total;
-    const bool kept = s < n && (k > key || (equal && rank < need));
-    const bool hole = s < m && !kept, far = s >= m && kept;
-    const int hole_rank = moved_to + prefix_count(hole, scratch, &total);
-    moved_to += total;
-    const int far_rank = moved_from + prefix_count(far, scratch, &total);
-    moved_from += total;
-    if (hole) to[hole_rank] = s;
-    if (far) from[far_rank] = s;
-    if (s < m && kept) {
-      weights_out[s] = w;
-      positions_out[s] = pos;
+  // keys above the threshold stay, and the first `need` of those equal to it
+  uint32_t flag[K], before[K], total;
+#pragma unroll
+  for (int j = 0; j < K; ++j) flag[j] = j * T + tid < n && k[j] == key;
+  prefix_counts<T>(flag, before, total, scratch);
+  bool kept[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    const int s = j * T + tid;
+    kept[j] = s < n && (k[j] > key || (k[j] == key && static_cast<int>(before[j]) < need));
+    flag[j] = s >= n ? 0 : s < m ? !kept[j] : kept[j] ? 0x10000u : 0;
+  }
+  prefix_counts<T>(flag, before, total, scratch);
+  int32_t* to = INNER ? moves[0] : p.to + static_cast<int64_t>(b) * p.most;
+  int32_t* from = INNER ? moves[INNER ? 1 : 0] : p.from + static_cast<int64_t>(b) * p.most;
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    const int s = j * T + tid;
+    if (flag[j] & 0xFFFFu) to[before[j] & 0xFFFFu] = s;
+    if (flag[j] >> 16) from[before[j] >> 16] = s;
+    if (s < m && kept[j]) {
+      p.weights_out[row + s] = w[j];
+      p.positions_out[row + s] = pos[j];
     }
   }
-  __syncthreads();  // (the lists, read below, were written by this workgroup)
-  for (int i = tid; i < moved_to; i += kThreads) {
-    const int t = to[i], f = from[i];
-    weights_out[t] = weights[f];
-    positions_out[t] = positions[f];
+  const int count = total >> 16;
+  if constexpr (INNER) {
+    __syncthreads();
+    for (int i = tid / kWave; i < count; i += T / kWave) move_slot(p, b, moves[0][i], moves[1][i]);
+  } else if (tid == 0) {
+    p.counts[b] = count;
   }
-  if (tid == 0) p.counts[b] = moved_to;
 }
 
-// A wave moves a row: codes of K and V, then scales, of every kv head.
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
   const int b = blockIdx.y;
-  const int lane = threadIdx.x % kWave;
-  const kvssd_paged_cache& c = p.c;
   const int count = p.counts[b];
-  const int32_t* pages = c.page_table + static_cast<int64_t>(b) * c.max_pages;
-  const int64_t code_bytes = static_cast<int64_t>(c.kv_heads) * c.head_dim * c.bits / 8;
-  const int64_t scale_count = static_cast<int64_t>(c.kv_heads) * (c.head_dim / c.group_size);
-  for (int i = blockIdx.x * 4 + threadIdx.x / kWave; i < count; i += gridDim.x * 4) {
-    const int t = p.to[static_cast<int64_t>(b) * p.most + i], f = p.from[static_cast<int64_t>(b) * p.most + i];
-    const int tp = pages[t / c.page_tokens], fp = pages[f / c.page_tokens];
-    if (tp < 0 || tp >= c.num_pages || fp < 0 || fp >= c.num_pages) continue;
-    const int64_t dst = static_cast<int64_t>(tp) * c.page_tokens + t % c.page_tokens;
-    const int64_t src = static_cast<int64_t>(fp) * c.page_tokens + f % c.page_tokens;
-    for (int64_t at = lane * 8; at < code_bytes; at += kWave * 8) {  // rows are multiples of 8 bytes
-      *reinterpret_cast<uint64_t*>(c.packed_k + dst * code_bytes + at) =
-          *reinterpret_cast<const uint64_t*>(c.packed_k + src * code_bytes + at);
-      *reinterpret_cast<uint64_t*>(c.packed_v + dst * code_bytes + at) =
-          *reinterpret_cast<const uint64_t*>(c.packed_v + src * code_bytes + at);
+  const int64_t at = static_cast<int64_t>(b) * p.most;
+  for (int i = blockIdx.x * 4 + threadIdx.x / kWave; i < count; i += gridDim.x * 4)
+    move_slot(p, b, p.to[at + i], p.from[at + i]);
+}
+
+// ---- longer sequences: a workgroup a chunk, a launch a step -------------------------------------------------------
+
+struct Chunk {
+  int b, nth, n, m, begin, end;  // slots [begin, end) of sequence b's n
+  int64_t row;
+};
+__device__ __forceinline__ Chunk chunk_of(const EvictParams& p) {
+  Chunk c;
+  c.b = blockIdx.x / p.chunks;
+  c.nth = blockIdx.x % p.chunks;
+  c.n = paged_length(p.c.lengths, c.b, p.capacity);
+  c.m = c.n < p.budget ? c.n : p.budget;
+  c.row = static_cast<int64_t>(c.b) * p.capacity;
+  c.begin = min(c.nth * p.chunk_slots, c.n);  // (below 2^31: at most 2^30 slots, and a chunk)
+  c.end = min(c.begin + p.chunk_slots, c.n);
+  return c;
+}
+
+// Step 1: a chunk's latest position; empty counts.
+__global__ __launch_bounds__(kChunkThreads) void evict_latest_kernel(EvictParams p) {
+  __shared__ int small[kChunkThreads / kWave];
+  const Chunk c = chunk_of(p);
+  const int tid = threadIdx.x;
+  int32_t* hist = p.hist + static_cast<int64_t>(c.b) * kPasses * kBins;
+  for (int i = c.nth * kChunkThreads + tid; i < kPasses * kBins; i += p.chunks * kChunkThreads) hist[i] = 0;
+  int latest = INT32_MIN;
+  for (int s = c.begin + tid; s < c.end; s += kChunkThreads) latest = max(latest, p.c.positions[c.row + s]);
+  for (int k = 1; k < kWave; k <<= 1) latest = max(latest, __shfl_xor(latest, k, kWave));
+  if (tid % kWave == 0) small[tid / kWave] = latest;
+  __syncthreads();
+  for (int v = 0; v < kChunkThreads / kWave; ++v) latest = max(latest, small[v]);
+  if (tid == 0) p.chunk[4 * static_cast<int64_t>(blockIdx.x)] = latest;
+}
+
+__device__ __forceinline__ uint32_t slot_key(const EvictParams& p, const Chunk& c, int s, int latest) {
+  return weight_key(p.c.weights[c.row + s], p.c.positions[c.row + s], p.sink, latest, p.recent);
+}
+
+// Steps 2 to 4: the sequence's counts of a digit; the digit before it is found first, by every workgroup.
+template <int PASS>
+__global__ __launch_bounds__(kChunkThreads) void evict_count_kernel(EvictParams p) {
+  constexpr int T = kChunkThreads;
+  __shared__ int counts[kBins];
+  __shared__ int small[T / kWave + 2];
+  const Chunk c = chunk_of(p);
+  if (c.n <= p.budget || c.begin >= c.end) return;
+  const int tid = threadIdx.x;
+  int32_t* hist = p.hist + static_cast<int64_t>(c.b) * kPasses * kBins;
+  int32_t* state = p.state + static_cast<int64_t>(c.b) * kState;
+  for (int i = tid; i < kBins; i += T) counts[i] = 0;
+  uint32_t key = 0;
+  int need = c.m, latest;
+  if constexpr (PASS == 0) {
+    latest = INT32_MIN;
+    for (int i = tid; i < p.chunks && i * p.chunk_slots < c.n; i += T)
+      latest = max(latest, p.chunk[4 * (static_cast<int64_t>(c.b) * p.chunks + i)]);
+    for (int k = 1; k < kWave; k <<= 1) latest = max(latest, __shfl_xor(latest, k, kWave));
+    if (tid % kWave == 0) small[tid / kWave] = latest;
+    __syncthreads();
+    for (int v = 0; v < T / kWave; ++v) latest = max(latest, small[v]);
+    if (c.nth == 0 && tid == 0) state[2 * kPasses] = latest;
+  } else {
+    latest = state[2 * kPasses];
+    if constexpr (PASS > 1) {
+      key = state[2 * (PASS - 2)];
+      need = state[2 * (PASS - 2) + 1];
     }
-    for (int64_t at = lane; at < scale_count; at += kWave) {
-      c.scales_k[dst * scale_count + at] = c.scales_k[src * scale_count + at];
-      c.scales_v[dst * scale_count + at] = c.scales_v[src * scale_count + at];
+    find_digit<T>(hist + (PASS - 1) * kBins, PASS - 1, key, need, small);
+    if (c.nth == 0 && tid == 0) {
+      state[2 * (PASS - 1)] = key;
+      state[2 * (PASS - 1) + 1] = need;
     }
   }
+  __syncthreads();
+  for (int base = c.begin; base < c.end; base += kChunkSlots) {
+    uint32_t k[kKeys];
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) {
+      const int s = base + j * T + tid;
+      k[j] = s < c.end ? slot_key(p, c, s, latest) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) count_key(counts, k[j], base + j * T + tid < c.end, PASS, key);
+  }
+  __syncthreads();
+  for (int i = tid; i < kBins; i += T)
+    if (counts[i] != 0) atomicAdd(&hist[PASS * kBins + i], counts[i]);  // (integers: any order)
+}
+
+// Step 5: a chunk's slots above and equal to the threshold, before the budget and from it on.
+__global__ __launch_bounds__(kChunkThreads) void evict_tally_kernel(EvictParams p) {
+  constexpr int T = kChunkThreads;
+  __shared__ int small[T / kWave + 2];
+  __shared__ int tally[4];
+  const Chunk c = chunk_of(p);
+  if (c.n <= p.budget || c.begin >= c.end) return;
+  const int tid = threadIdx.x;
+  int32_t* state = p.state + static_cast<int64_t>(c.b) * kState;
+  uint32_t key = state[2 * (kPasses - 2)];
+  int need = state[2 * (kPasses - 2) + 1];
+  const int latest = state[2 * kPasses];
+  if (tid < 4) tally[tid] = 0;
+  find_digit<T>(p.hist + (static_cast<int64_t>(c.b) * kPasses + kPasses - 1) * kBins, kPasses - 1, key, need, small);
+  if (c.nth == 0 && tid == 0) {
+    state[2 * (kPasses - 1)] = key;
+    state[2 * (kPasses - 1) + 1] = need;
+  }
+  int mine[4] = {0, 0, 0, 0};
+  for (int base = c.begin; base < c.end; base += kChunkSlots) {
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) {
+      const int s = base + j * T + tid;
+      const uint32_t k = s < c.end ? slot_key(p, c, s, latest) : 0;
+      const bool far = s >= c.m, above = s < c.end && k > key, equal = s < c.end && k == key;
+      mine[0] += __popcll(__ballot(above && !far));
+      mine[1] += __popcll(__ballot(above && far));
+      mine[2] += __popcll(__ballot(equal && !far));
+      mine[3] += __popcll(__ballot(equal && far));
+    }
+  }
+  if (tid % kWave == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) atomicAdd(&tally[i], mine[i]);
+  }
+  __syncthreads();
+  if (tid < 4) p.chunk[4 * static_cast<int64_t>(blockIdx.x) + tid] = tally[tid];
+}
+
+// Step 6: the kept slots' weights and positions, and the lists of the moves.
+__global__ __launch_bounds__(kChunkThreads) void evict_place_kernel(EvictParams p) {
+  constexpr int T = kChunkThreads;
+  __shared__ uint32_t scratch[kChunkSlots / kWave];
+  __shared__ int sums[3][T / kWave];
+  const Chunk c = chunk_of(p);
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  if (c.nth == 0 && tid == 0) p.lengths_out[c.b] = c.m;
+  const int64_t tail = static_cast<int64_t>(c.nth) * p.chunk_slots;
+  clear_tail(p, c.row, static_cast<int>(tail > c.m ? tail : c.m),
+             static_cast<int>(tail + p.chunk_slots < p.capacity ? tail + p.chunk_slots : p.capacity), T);
+  if (c.n <= p.budget) {
+    for (int s = c.begin + tid; s < c.end; s += T) {
+      p.weights_out[c.row + s] = p.c.weights[c.row + s];
+      p.positions_out[c.row + s] = p.c.positions[c.row + s];
+    }
+    if (c.nth == 0 && tid == 0) p.counts[c.b] = 0;
+    return;
+  }
+  const int32_t* state = p.state + static_cast<int64_t>(c.b) * kState;
+  const uint32_t key = state[2 * (kPasses - 1)];
+  const int need = state[2 * (kPasses - 1) + 1], latest = state[2 * kPasses];
+  // of the chunks before: slots equal to the threshold; then, from those, holes before the budget and kept slots past it
+  const int32_t* tallies = p.chunk + 4 * static_cast<int64_t>(c.b) * p.chunks;
+  int equal_before = 0, holes = 0, fars = 0;
+  for (int i0 = 0; i0 < c.nth && i0 * p.chunk_slots < c.n; i0 += T) {  // (the same number of times in every thread)
+    const int i = i0 + tid;
+    int above[2] = {0, 0}, equal[2] = {0, 0};
+    const bool of = i < c.nth && static_cast<int64_t>(i) * p.chunk_slots < c.n;
+    if (of) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        above[x] = tallies[4 * i + x];
+        equal[x] = tallies[4 * i + 2 + x];
+      }
+    }
+    const int incl = wave_inclusive(equal[0] + equal[1]);
+    __syncthreads();
+    if (lane == kWave - 1) sums[0][wave] = incl;
+    __syncthreads();
+    int at = equal_before + incl - equal[0] - equal[1];
+    for (int v = 0; v < T / kWave; ++v) {
+      at += v < wave ? sums[0][v] : 0;
+      equal_before += sums[0][v];
+    }
+    if (of) {
+      const int64_t first = static_cast<int64_t>(i) * p.chunk_slots;
+      const int64_t stop = first + p.chunk_slots < c.n ? first + p.chunk_slots : c.n;
+      const int near = static_cast<int>(first >= c.m ? 0 : (stop < c.m ? stop : c.m) - first);
+      const int kept_near = max(0, min(need - at, equal[0]));
+      holes += near - above[0] - kept_near;
+      fars += above[1] + max(0, min(need - at - equal[0], equal[1]));
+    }
+  }
+  for (int k = 1; k < kWave; k <<= 1) {
+    holes += __shfl_xor(holes, k, kWave);
+    fars += __shfl_xor(fars, k, kWave);
+  }
+  if (lane == 0) {
+    sums[1][wave] = holes;
+    sums[2][wave] = fars;
+  }
+  __syncthreads();
+  holes = fars = 0;
+  for (int v = 0; v < T / kWave; ++v) {
+    holes += sums[1][v];
+    fars += sums[2][v];
+  }
+  int32_t* to = p.to + static_cast<int64_t>(c.b) * p.most;
+  int32_t* from = p.from + static_cast<int64_t>(c.b) * p.most;
+  for (int base = c.begin; base < c.end; base += kChunkSlots) {
+    float w[kKeys];
+    int pos[kKeys];
+    uint32_t k[kKeys], flag[kKeys], before[kKeys], total;
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) {
+      const int s = base + j * T + tid;
+      w[j] = 0.0f;
+      pos[j] = 0;
+      if (s < c.end) {
+        w[j] = p.c.weights[c.row + s];
+        pos[j] = p.c.positions[c.row + s];
+      }
+      k[j] = weight_key(w[j], pos[j], p.sink, latest, p.recent);
+      flag[j] = s < c.end && k[j] == key;
+    }
+    prefix_counts<T>(flag, before, total, scratch);
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) {
+      const int s = base + j * T + tid;
+      const bool kept =
+          s < c.end && (k[j] > key || (k[j] == key && equal_before + static_cast<int>(before[j]) < need));
+      if (s < c.m && kept) {
+        p.weights_out[c.row + s] = w[j];
+        p.positions_out[c.row + s] = pos[j];
+      }
+      flag[j] = s >= c.end ? 0 : s < c.m ? !kept : kept ? 0x10000u : 0;
+    }
+    equal_before += total;
+    prefix_counts<T>(flag, before, total, scratch);
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) {
+      const int s = base + j * T + tid;
+      if (flag[j] & 0xFFFFu) to[holes + (before[j] & 0xFFFFu)] = s;
+      if (flag[j] >> 16) from[fars + (before[j] >> 16)] = s;
+    }
+    holes += total & 0xFFFFu;
+    fars += total >> 16;
+  }
+  if (c.end == c.n && c.begin < c.end && tid == 0) p.counts[c.b] = fars;
 }
 
 int most_moves(const kvssd_paged_cache& c, int budget) {
   const int64_t rest = paged_capacity(c) - budget;
   return static_cast<int>(rest < 0 ? 0 : rest < budget ? rest : budget);
+}
+
+// Workspace: chunked sequences' counts, then lengths and lists of the moves.
+struct EvictPlan {
+  bool one, inner;
+  int most, chunks, chunk_slots;
+  size_t words;
+};
+EvictPlan plan_evict(const kvssd_paged_cache& c, int budget) {
+  EvictPlan e{};
+  const int64_t capacity = paged_capacity(c);
+  e.most = most_moves(c, budget);
+  e.one = capacity <= kOneSlots;
+  e.inner = e.one && e.most <= kInnerMoves;
+  const size_t n = c.sequences;
+  if (e.inner) return e;
+  e.words = n * (1 + 2 * static_cast<size_t>(e.most));
+  if (e.one) return e;
+  const int64_t most_chunks = capacity / kChunkSlots / kMostChunks + 1;  // units of kChunkSlots a chunk
+  e.chunk_slots = static_cast<int>(most_chunks) * kChunkSlots;
+  e.chunks = static_cast<int>((capacity + e.chunk_slots - 1) / e.chunk_slots);
+  e.words += n * (kState + kPasses * kBins + 4 * static_cast<size_t>(e.chunks));
+  return e;
 }
 
 }  // namespace
@@ -214,12 +550,33 @@ int launch_paged_evict(const kvssd_paged_cache& c, const kvssd_paged_evict_args&
   p.sink = a.sink;
   p.recent = a.recent;
   p.capacity = static_cast<int>(paged_capacity(c));
-  p.most = most_moves(c, a.budget);
+  const EvictPlan plan = plan_evict(c, a.budget);
+  p.most = plan.most;
+  if (plan.inner) {
+    hipLaunchKernelGGL(evict_one_kernel<true>, dim3(c.sequences), dim3(kOneThreads), 0, stream, p);
+    return hip_status(hipGetLastError(), "evict launch");
+  }
+  const size_t n = c.sequences;
   p.counts = static_cast<int32_t*>(a.workspace);
-  p.to = p.counts + c.sequences;
-  p.from = p.to + static_cast<int64_t>(c.sequences) * p.most;
-  hipLaunchKernelGGL(evict_select_kernel, dim3(c.sequences), dim3(kThreads), 0, stream, p);
-  if (int rc = hip_status(hipGetLastError(), "evict_select launch")) return rc;
+  p.to = p.counts + n;
+  p.from = p.to + n * p.most;
+  if (plan.one) {
+    hipLaunchKernelGGL(evict_one_kernel<false>, dim3(c.sequences), dim3(kOneThreads), 0, stream, p);
+  } else {
+    p.chunks = plan.chunks;
+    p.chunk_slots = plan.chunk_slots;
+    p.state = p.from + n * p.most;
+    p.hist = p.state + n * kState;
+    p.chunk = p.hist + n * kPasses * kBins;
+    const dim3 grid(static_cast<unsigned>(n * plan.chunks)), block(kChunkThreads);
+    hipLaunchKernelGGL(evict_latest_kernel, grid, block, 0, stream, p);
+    hipLaunchKernelGGL(evict_count_kernel<0>, grid, block, 0, stream, p);
+    hipLaunchKernelGGL(evict_count_kernel<1>, grid, block, 0, stream, p);
+    hipLaunchKernelGGL(evict_count_kernel<2>, grid, block, 0, stream, p);
+    hipLaunchKernelGGL(evict_tally_kernel, grid, block, 0, stream, p);
+    hipLaunchKernelGGL(evict_place_kernel, grid, block, 0, stream, p);
+  }
+  if (int rc = hip_status(hipGetLastError(), "evict launch")) return rc;
   if (p.most == 0) return 0;
   for (int b0 = 0; b0 < c.sequences; b0 += 65535) {  // (a grid's second dimension)
     EvictParams q = p;
@@ -228,6 +585,10 @@ int launch_paged_evict(const kvssd_paged_cache& c, const kvssd_paged_evict_args&
     q.to += static_cast<int64_t>(b0) * p.most;
     q.from += static_cast<int64_t>(b0) * p.most;
     q.c.page_table += static_cast<int64_t>(b0) * c.max_pages;
+    q.c.weights += b0 * static_cast<int64_t>(p.capacity);
+    q.c.positions += b0 * static_cast<int64_t>(p.capacity);
+    q.weights_out += b0 * static_cast<int64_t>(p.capacity);
+    q.positions_out += b0 * static_cast<int64_t>(p.capacity);
     int blocks = (p.most + 3) / 4;
     const int cap = 8192 / nb < 1 ? 1 : 8192 / nb;
     blocks = blocks < cap ? blocks : cap;
@@ -250,9 +611,7 @@ int check_evict(const kvssd_paged_cache* cache, const kvssd_paged_evict_args* ar
     return arg_error("sink and recent must fit the budget");
   return 0;
 }
-size_t evict_bytes(const kvssd_paged_cache& c, int budget) {
-  return (static_cast<size_t>(c.sequences) + 2 * static_cast<size_t>(c.sequences) * most_moves(c, budget)) * sizeof(int32_t);
-}
+size_t evict_bytes(const kvssd_paged_cache& c, int budget) { return plan_evict(c, budget).words * sizeof(int32_t); }
 }  // namespace
 
 extern "C" {
@@ -276,7 +635,7 @@ __attribute__((visibility("default"))) int kvssd_hip_paged_evict(const kvssd_pag
       args->lengths_out == cache->lengths)
     return arg_error("eviction writes arrays of their own, not the cache's");
   const size_t need = evict_bytes(*cache, args->budget);
-  if (args->workspace == nullptr || args->workspace_bytes < need)
+  if (need > 0 && (args->workspace == nullptr || args->workspace_bytes < need))
     return arg_error("workspace too small: need " + std::to_string(need) + " bytes");
   return launch_paged_evict(*cache, *args, static_cast<hipStream_t>(stream));
 }

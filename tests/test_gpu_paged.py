@@ -503,6 +503,16 @@ EVICTS = [
 ]
 
 
+EVICTS += [  # several chunks of a sequence, chunks without a slot of it, the budget at a chunk's edge
+    ([8192, 8191, 1, 0, 5000], 4096, 4, 1000, 128, 1, 32, 4, "zeros"),
+    ([8193, 2048, 2049, 0, 1, 8192], 2048, 4, 100, 128, 1, 32, 2, "zeros"),
+    ([30000, 12345, 4097], 4096, 0, 50, 100, 1, 32, 2, "equal"),
+    ([30000, 16384, 10001], 10000, 3, 0, 64, 1, 32, 2, "odd"),
+    ([50000], 49999, 0, 0, 64, 1, 32, 2, "normal"),
+    ([50000, 9], 1, 1, 0, 64, 1, 32, 2, "heavy"),
+]
+
+
 @pytest.mark.parametrize("case", EVICTS, ids=lambda c: f"{c[0]}-{c[1]}-{c[8]}")
 @pytest.mark.parametrize("shuffled", [False, True])
 def test_eviction_keeps_and_moves_as_defined(cuda_device, case, shuffled):
@@ -566,6 +576,34 @@ def test_eviction_skips_pages_that_are_not_there(cuda_device):
     assert (got == want).all()
 
 
+def test_eviction_past_two_million_slots(cuda_device):
+    """More slots than the most chunks of the smallest size hold: two at a time in each."""
+    n, bt, budget = 2_200_000, 64, 1_000_001
+    rng = np.random.default_rng(32)
+    pages = -(-n // bt) + 1
+    pool = make_pool(rng, pages, bt, 1, 32, 32, 2)
+    table = make_table(rng, [n], bt, pages, pages)
+    w = rng.integers(0, 1 << 20, (1, pages * bt)).astype(np.float32)  # with equal ones
+    pos = np.arange(pages * bt, dtype=np.int32)[None]
+    batch = paged(cuda_device, pool, table, [n], 2, 32, w, pos)
+    lengths, new_w, new_p = evict_tokens(batch, budget, sink=5, recent=999)
+    held = (pos[0, :n] < 5) | (pos[0, :n] > n - 1 - 999)
+    order = np.lexsort((np.arange(n), -w[0, :n], ~held))
+    kept = np.zeros(n, bool)
+    kept[order[:budget]] = True
+    source = np.arange(budget)
+    source[~kept[:budget]] = budget + np.flatnonzero(kept[budget:])
+    assert lengths.tolist() == [budget]
+    assert np.array_equal(new_p.cpu().numpy()[0, :budget], pos[0, source]) and (new_p[0, budget:] == -1).all()
+    assert np.array_equal(new_w.cpu().numpy()[0, :budget], w[0, source]) and (new_w[0, budget:] == 0).all()
+    at = lambda s: table[0, s // bt].astype(np.int64) * bt + s % bt
+    slots = np.arange(n)
+    slots[:budget] = source
+    for name, a in zip(("packed_k", "packed_v", "scales_k", "scales_v"), pool):
+        got = getattr(batch, name).cpu().numpy().reshape(pages * bt, -1)[at(np.arange(n))]
+        assert (got.view(np.uint8) == a.reshape(pages * bt, -1)[at(slots)].view(np.uint8)).all(), name
+
+
 def test_eviction_graph(cuda_device):
     rng = np.random.default_rng(31)
     pool = make_pool(rng, 20, 16, 2, 64, 32, 4)
@@ -586,6 +624,31 @@ def test_eviction_graph(cuda_device):
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(a.packed_v, b.packed_v)
     del graph
+
+
+def test_eviction_of_long_sequences_in_a_graph(cuda_device):
+    rng = np.random.default_rng(33)
+    pool = make_pool(rng, 300, 128, 1, 32, 32, 2)
+    table = np.arange(300).reshape(2, 150)
+    pos = np.tile(np.arange(19200, dtype=np.int32), (2, 1))
+    a, b = (paged(cuda_device, pool, table, [19000, 9000], 2, 32, np.zeros((2, 19200), np.float32), pos) for _ in "ab")
+    evict_tokens(a, 8000, recent=5)
+    evict_tokens(b, 8000, recent=5)
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        got = evict_tokens(a, 8000, recent=5)
+    with torch.cuda.graph(second):
+        other = evict_tokens(a, 300, recent=5)
+    for r in range(4):
+        w = torch.from_numpy(rng.integers(0, 999, (2, 19200)).astype(np.float32))
+        a.weights.copy_(w)
+        b.weights.copy_(w)
+        for graph, have, budget in ((first, got, 8000), (second, other, 300)):
+            graph.replay()
+            want = evict_tokens(b, budget, recent=5)
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(have, want)) and torch.equal(a.packed_v, b.packed_v)
+    del first, second
 
 
 # --------------------------------------------------------------------------------------------- the operators together
