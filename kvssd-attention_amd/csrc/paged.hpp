@@ -38,4 +38,27 @@ __device__ __forceinline__ int paged_length(const int32_t* lengths, int b, int c
   return clamp_length(lengths[b], capacity);
 }
 
+// x of a lane before this one (0 where there is none): CTRL 0x110 + n, n lanes
+// before in the row of 16; 0x142 / 0x143, lane 15 of the row before / lane 31
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int lane_before(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_prefix(int x) {  // inclusive sum over the lanes
+  x += lane_before<0x111, 0xF>(x);
+  x += lane_before<0x112, 0xF>(x);
+  x += lane_before<0x114, 0xF>(x);
+  x += lane_before<0x118, 0xF>(x);
+  x += lane_before<0x142, 0xA>(x);
+  return x + lane_before<0x143, 0xC>(x);
+}
+__device__ __forceinline__ uint32_t wave_most(uint32_t x) {
+  x = max(x, static_cast<uint32_t>(lane_before<0x111, 0xF>(x)));
+  x = max(x, static_cast<uint32_t>(lane_before<0x112, 0xF>(x)));
+  x = max(x, static_cast<uint32_t>(lane_before<0x114, 0xF>(x)));
+  x = max(x, static_cast<uint32_t>(lane_before<0x118, 0xF>(x)));
+  x = max(x, static_cast<uint32_t>(lane_before<0x142, 0xA>(x)));
+  return __builtin_amdgcn_readlane(max(x, static_cast<uint32_t>(lane_before<0x143, 0xC>(x))), kWave - 1);
+}
+
 }  // namespace kvssd

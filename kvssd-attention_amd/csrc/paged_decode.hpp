@@ -100,29 +100,6 @@ struct RunMap {
   int nth;    // its place among the sequence's
 };
 
-// x of a lane before this one (0 where there is none): CTRL 0x110 + n, n lanes
-// before in the row of 16; 0x142 / 0x143, lane 15 of the row before / lane 31
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int lane_before(int x) {
-  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
-}
-__device__ __forceinline__ int wave_prefix(int x) {  // inclusive sum over the lanes
-  x += lane_before<0x111, 0xF>(x);
-  x += lane_before<0x112, 0xF>(x);
-  x += lane_before<0x114, 0xF>(x);
-  x += lane_before<0x118, 0xF>(x);
-  x += lane_before<0x142, 0xA>(x);
-  return x + lane_before<0x143, 0xC>(x);
-}
-__device__ __forceinline__ int wave_most(int x) {  // of numbers that are not negative
-  x = max(x, lane_before<0x111, 0xF>(x));
-  x = max(x, lane_before<0x112, 0xF>(x));
-  x = max(x, lane_before<0x114, 0xF>(x));
-  x = max(x, lane_before<0x118, 0xF>(x));
-  x = max(x, lane_before<0x142, 0xA>(x));
-  return __builtin_amdgcn_readlane(max(x, lane_before<0x143, 0xC>(x)), kWave - 1);
-}
-
 __device__ __forceinline__ int length_tiles(const PagedDecodeParams& p, int seq) {
   return seq < p.c.sequences ? (paged_length(p.c.lengths, seq, p.capacity) + kTile - 1) / kTile : 0;
 }
@@ -637,7 +614,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     over = over || top > kLazy - static_cast<float>(w_exp);
     if (first || __any(over)) {
       // new reference points: the largest score so far and the largest value scale so far
-      const int e_new = max(wave_most(static_cast<int>(sv_top >> 10) + 9) - 32, w_exp);
+      const int e_new = max(static_cast<int>(wave_most((sv_top >> 10) + 9)) - 32, w_exp);
       top = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -702,7 +679,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     }
     if (first || __any(e_stage > w_exp || top > kLazy - static_cast<float>(w_exp))) {
       // new reference points: the largest score so far and the largest value scale so far
-      const int e_new = max(wave_most(e_stage + 32) - 32, w_exp);
+      const int e_new = max(static_cast<int>(wave_most(e_stage + 32)) - 32, w_exp);
       top = -INFINITY;
 #pragma unroll
       for (int u = 0; u < 4; ++u) top = out[u] ? top : fmaxf(top, s[u] * s_factor);

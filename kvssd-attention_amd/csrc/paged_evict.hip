@@ -50,6 +50,8 @@ __device__ __forceinline__ uint32_t weight_key(float w, int position, int sink, 
 __device__ __forceinline__ int pass_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 __device__ __forceinline__ uint32_t pass_above(int pass) { return pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u; }
 
+__device__ __forceinline__ int scalar_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
+
 // Counts a key's digit; held keys, many and alike, once a wave.
 __device__ __forceinline__ void count_key(int* hist, uint32_t k, bool live, int pass, uint32_t key) {
   const bool of = live && (k & pass_above(pass)) == key;
@@ -59,13 +61,16 @@ __device__ __forceinline__ void count_key(int* hist, uint32_t k, bool live, int 
   if (held != 0 && threadIdx.x % kWave == __builtin_ctzll(held)) atomicAdd(&hist[digit], __popcll(held));
 }
 
-__device__ __forceinline__ int wave_inclusive(int x) {
-  const int lane = threadIdx.x % kWave;
-  for (int k = 1; k < kWave; k <<= 1) {
-    const int y = __shfl_up(x, k, kWave);
-    if (lane >= k) x += y;
-  }
-  return x;
+// The latest of the workgroup's threads' positions.
+template <int THREADS>
+__device__ __forceinline__ int latest_of(int x, int* scratch) {
+  const uint32_t most = wave_most(static_cast<uint32_t>(x) ^ 0x80000000u);
+  if (threadIdx.x % kWave == 0) scratch[threadIdx.x / kWave] = static_cast<int>(most ^ 0x80000000u);
+  __syncthreads();
+  int latest = scratch[0];
+#pragma unroll
+  for (int v = 1; v < THREADS / kWave; ++v) latest = max(latest, scratch[v]);
+  return latest;
 }
 
 // The bin, counted from the top, in which the need-th key lies, and the keys above it; -> key and need.
@@ -76,11 +81,12 @@ __device__ __forceinline__ void find_digit(const int* hist, int pass, uint32_t& 
   int c[kEach], sum = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) sum += c[i] = hist[kBins - 1 - kEach * tid - i];
-  const int incl = wave_inclusive(sum);
+  const int incl = wave_prefix(sum);
   if (lane == kWave - 1) scratch[wave] = incl;
   __syncthreads();
   int before = incl - sum;
-  for (int w = 0; w < wave; ++w) before += scratch[w];
+#pragma unroll
+  for (int w = 0; w < THREADS / kWave; ++w) before += w < wave ? scratch[w] : 0;
   int* found = scratch + THREADS / kWave;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
@@ -96,16 +102,17 @@ __device__ __forceinline__ void find_digit(const int* hist, int pass, uint32_t& 
 }
 
 // Exclusive prefix counts, in slot order, of flags over the slots j THREADS + thread, j < KEYS; total: of all.  The
-// counts of two kinds of flags go in a word's halves (at most 2^14 slots).
+// counts of two kinds of flags go in a word's halves (at most 2^14 slots).  Past `slots` there are none.
 template <int THREADS, int KEYS>
 __device__ __forceinline__ void prefix_counts(const uint32_t (&flag)[KEYS], uint32_t (&before)[KEYS], uint32_t& total,
-                                              uint32_t* scratch) {
+                                              uint32_t* scratch, int slots) {
   constexpr int kWaves = THREADS / kWave, kEntries = KEYS * kWaves, kEach = (kEntries + kWave - 1) / kWave;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave, wave = scalar_wave();
   const uint64_t lower = (1ull << lane) - 1;
   __syncthreads();  // (scratch is free)
 #pragma unroll
   for (int j = 0; j < KEYS; ++j) {
+    if (j * THREADS >= slots) break;
     const uint64_t a = __ballot(flag[j] & 0xFFFFu), b = __ballot(flag[j] >> 16);
     before[j] = __popcll(a & lower) | __popcll(b & lower) << 16;
     if (lane == 0) scratch[j * kWaves + wave] = __popcll(a) | __popcll(b) << 16;
@@ -116,48 +123,77 @@ __device__ __forceinline__ void prefix_counts(const uint32_t (&flag)[KEYS], uint
   for (int i = 0; i < kEach; ++i) {
     const int at = lane * kEach + i;
     e[i] = sum;
-    sum += at < kEntries ? scratch[at] : 0;
+    sum += at / kWaves * THREADS < slots && at < kEntries ? scratch[at] : 0;
   }
-  const uint32_t incl = wave_inclusive(sum);
-  total = __shfl(incl, kWave - 1, kWave);
+  const uint32_t incl = wave_prefix(sum);
+  total = __builtin_amdgcn_readlane(incl, kWave - 1);
 #pragma unroll
   for (int j = 0; j < KEYS; ++j) {
+    if (j * THREADS >= slots) break;
     const int at = j * kWaves + wave;
-    uint32_t x = __shfl(incl - sum, at / kEach, kWave);
+    uint32_t x = __builtin_amdgcn_readlane(incl - sum, at / kEach);
 #pragma unroll
     for (int i = 1; i < kEach; ++i) {
-      const uint32_t y = __shfl(incl - sum + e[i], at / kEach, kWave);
+      const uint32_t y = __builtin_amdgcn_readlane(incl - sum + e[i], at / kEach);
       x = at % kEach == i ? y : x;
     }
     before[j] += x;
   }
 }
 
-// A wave moves slot f to slot t: codes of K and V, scales of every kv head, weight and position.
-__device__ __forceinline__ void move_slot(const EvictParams& p, int b, int t, int f) {
+// A wave moves slots from[i] to slots to[i], first <= i < count, kRows at a time with every load before the first
+// store: codes of K and V, scales of every kv head, weights and positions.
+constexpr int kRows = 4;
+__device__ __forceinline__ void move_slots(const EvictParams& p, int b, const int32_t* to, const int32_t* from, int first,
+                                           int count) {
   const int lane = threadIdx.x % kWave;
   const kvssd_paged_cache& c = p.c;
   const int64_t row = static_cast<int64_t>(b) * p.capacity;
-  if (lane == 0) {
+  const int32_t* pages = c.page_table + static_cast<int64_t>(b) * c.max_pages;
+  const int code_bytes = c.kv_heads * (c.head_dim * c.bits / 8);  // a multiple of 8; (below 2^31: the row's elements are)
+  const int scale_count = c.kv_heads * (c.head_dim / c.group_size);
+  int64_t dst[kRows], src[kRows];
+  bool has[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int i = min(first + r, count - 1);
+    const int t = __builtin_amdgcn_readfirstlane(to[i]), f = __builtin_amdgcn_readfirstlane(from[i]);
+    const int tp = uniform_load(pages + t / c.page_tokens), fp = uniform_load(pages + f / c.page_tokens);
+    has[r] = first + r < count && tp >= 0 && tp < c.num_pages && fp >= 0 && fp < c.num_pages;
+    dst[r] = static_cast<int64_t>(tp) * c.page_tokens + t % c.page_tokens;
+    src[r] = static_cast<int64_t>(fp) * c.page_tokens + f % c.page_tokens;
+  }
+  for (int at = 0; at * 8 < code_bytes || at < scale_count; at += kWave) {
+    const int piece = at + lane, byte = 8 * piece;
+    uint64_t k[kRows], v[kRows];
+    uint16_t sk[kRows], sv[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (has[r] && byte < code_bytes) {
+        k[r] = *reinterpret_cast<const uint64_t*>(c.packed_k + src[r] * code_bytes + byte);
+        v[r] = *reinterpret_cast<const uint64_t*>(c.packed_v + src[r] * code_bytes + byte);
+      }
+      if (has[r] && piece < scale_count) {
+        sk[r] = c.scales_k[src[r] * scale_count + piece];
+        sv[r] = c.scales_v[src[r] * scale_count + piece];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (has[r] && byte < code_bytes) {
+        *reinterpret_cast<uint64_t*>(c.packed_k + dst[r] * code_bytes + byte) = k[r];
+        *reinterpret_cast<uint64_t*>(c.packed_v + dst[r] * code_bytes + byte) = v[r];
+      }
+      if (has[r] && piece < scale_count) {
+        c.scales_k[dst[r] * scale_count + piece] = sk[r];
+        c.scales_v[dst[r] * scale_count + piece] = sv[r];
+      }
+    }
+  }
+  if (lane < kRows && first + lane < count) {
+    const int t = to[first + lane], f = from[first + lane];
     p.weights_out[row + t] = c.weights[row + f];
     p.positions_out[row + t] = c.positions[row + f];
-  }
-  const int32_t* pages = c.page_table + static_cast<int64_t>(b) * c.max_pages;
-  const int tp = pages[t / c.page_tokens], fp = pages[f / c.page_tokens];
-  if (tp < 0 || tp >= c.num_pages || fp < 0 || fp >= c.num_pages) return;
-  const int64_t code_bytes = static_cast<int64_t>(c.kv_heads) * c.head_dim * c.bits / 8;
-  const int64_t scale_count = static_cast<int64_t>(c.kv_heads) * (c.head_dim / c.group_size);
-  const int64_t dst = static_cast<int64_t>(tp) * c.page_tokens + t % c.page_tokens;
-  const int64_t src = static_cast<int64_t>(fp) * c.page_tokens + f % c.page_tokens;
-  for (int64_t at = lane * 8; at < code_bytes; at += kWave * 8) {  // rows are multiples of 8 bytes
-    *reinterpret_cast<uint64_t*>(c.packed_k + dst * code_bytes + at) =
-        *reinterpret_cast<const uint64_t*>(c.packed_k + src * code_bytes + at);
-    *reinterpret_cast<uint64_t*>(c.packed_v + dst * code_bytes + at) =
-        *reinterpret_cast<const uint64_t*>(c.packed_v + src * code_bytes + at);
-  }
-  for (int64_t at = lane; at < scale_count; at += kWave) {
-    c.scales_k[dst * scale_count + at] = c.scales_k[src * scale_count + at];
-    c.scales_v[dst * scale_count + at] = c.scales_v[src * scale_count + at];
   }
 }
 
@@ -172,15 +208,12 @@ __device__ __forceinline__ void clear_tail(const EvictParams& p, int64_t row, in
 template <bool INNER>
 __global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictParams p) {
   constexpr int T = kOneThreads, K = kOneSlots / T;
-  __shared__ int hist[kBins];
+  __shared__ int hist[kPasses][kBins];
   __shared__ uint32_t scratch[kOneSlots / kWave];
   __shared__ int small[T / kWave + 2];
   __shared__ int moves[2][INNER ? kInnerMoves : 1];
   const int b = blockIdx.x, tid = threadIdx.x;
-  const int n = paged_length(p.c.lengths, b, p.capacity);
-  const int m = n < p.budget ? n : p.budget;
   const int64_t row = static_cast<int64_t>(b) * p.capacity;
-  if (tid == 0) p.lengths_out[b] = m;
   float w[K];
   int pos[K];
 #pragma unroll
@@ -188,13 +221,17 @@ __global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictParams p) {
     const int s = j * T + tid;
     w[j] = 0.0f;
     pos[j] = INT32_MIN;
-    if (s < n) {
+    if (s < p.capacity) {  // (not waiting for the length)
       w[j] = p.c.weights[row + s];
       pos[j] = p.c.positions[row + s];
     }
   }
-  clear_tail(p, row, m, p.capacity, T);
+  for (int i = tid; i < kPasses * kBins; i += T) hist[0][i] = 0;
+  const int n = paged_length(p.c.lengths, b, p.capacity);
+  const int m = n < p.budget ? n : p.budget;
+  if (tid == 0) p.lengths_out[b] = m;
   if (n <= p.budget) {
+    clear_tail(p, row, m, p.capacity, T);
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       const int s = j * T + tid;
@@ -208,66 +245,70 @@ __global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictParams p) {
   }
   int latest = INT32_MIN;
 #pragma unroll
-  for (int j = 0; j < K; ++j) latest = max(latest, pos[j]);
-  for (int k = 1; k < kWave; k <<= 1) latest = max(latest, __shfl_xor(latest, k, kWave));
-  if (tid % kWave == 0) small[tid / kWave] = latest;
-  __syncthreads();
-  for (int v = 0; v < T / kWave; ++v) latest = max(latest, small[v]);
+  for (int j = 0; j < K; ++j) latest = max(latest, j * T + tid < n ? pos[j] : INT32_MIN);
+  latest = latest_of<T>(latest, small);
   uint32_t k[K];
 #pragma unroll
   for (int j = 0; j < K; ++j) k[j] = weight_key(w[j], pos[j], p.sink, latest, p.recent);
   uint32_t key = 0;  // digits found so far
   int need = m;      // kept keys among those that share them
+#pragma unroll
   for (int pass = 0; pass < kPasses; ++pass) {
-    for (int i = tid; i < kBins; i += T) hist[i] = 0;
-    __syncthreads();
 #pragma unroll
     for (int j = 0; j < K; ++j)
-      if (j * T < n) count_key(hist, k[j], j * T + tid < n, pass, key);
+      if (j * T < n) count_key(hist[pass], k[j], j * T + tid < n, pass, key);
     __syncthreads();
-    find_digit<T>(hist, pass, key, need, small);
-    __syncthreads();
+    find_digit<T>(hist[pass], pass, key, need, small);
   }
   // keys above the threshold stay, and the first `need` of those equal to it
   uint32_t flag[K], before[K], total;
 #pragma unroll
   for (int j = 0; j < K; ++j) flag[j] = j * T + tid < n && k[j] == key;
-  prefix_counts<T>(flag, before, total, scratch);
+  prefix_counts<T>(flag, before, total, scratch, n);
   bool kept[K];
 #pragma unroll
   for (int j = 0; j < K; ++j) {
+    if (j * T >= n) break;
     const int s = j * T + tid;
     kept[j] = s < n && (k[j] > key || (k[j] == key && static_cast<int>(before[j]) < need));
     flag[j] = s >= n ? 0 : s < m ? !kept[j] : kept[j] ? 0x10000u : 0;
   }
-  prefix_counts<T>(flag, before, total, scratch);
+  prefix_counts<T>(flag, before, total, scratch, n);
   int32_t* to = INNER ? moves[0] : p.to + static_cast<int64_t>(b) * p.most;
   int32_t* from = INNER ? moves[INNER ? 1 : 0] : p.from + static_cast<int64_t>(b) * p.most;
 #pragma unroll
   for (int j = 0; j < K; ++j) {
+    if (j * T >= n) break;
     const int s = j * T + tid;
     if (flag[j] & 0xFFFFu) to[before[j] & 0xFFFFu] = s;
     if (flag[j] >> 16) from[before[j] >> 16] = s;
+  }
+  const int count = total >> 16;
+  if constexpr (INNER) {
+    __syncthreads();
+    for (int i = kRows * scalar_wave(); i < count; i += kRows * (T / kWave)) move_slots(p, b, moves[0], moves[1], i, count);
+  } else if (tid == 0) {
+    p.counts[b] = count;
+  }
+  // (last: a barrier waits for the stores before it)
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    if (j * T >= m) break;
+    const int s = j * T + tid;
     if (s < m && kept[j]) {
       p.weights_out[row + s] = w[j];
       p.positions_out[row + s] = pos[j];
     }
   }
-  const int count = total >> 16;
-  if constexpr (INNER) {
-    __syncthreads();
-    for (int i = tid / kWave; i < count; i += T / kWave) move_slot(p, b, moves[0][i], moves[1][i]);
-  } else if (tid == 0) {
-    p.counts[b] = count;
-  }
+  clear_tail(p, row, m, p.capacity, T);
 }
 
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
   const int b = blockIdx.y;
   const int count = p.counts[b];
   const int64_t at = static_cast<int64_t>(b) * p.most;
-  for (int i = blockIdx.x * 4 + threadIdx.x / kWave; i < count; i += gridDim.x * 4)
-    move_slot(p, b, p.to[at + i], p.from[at + i]);
+  for (int i = kRows * (blockIdx.x * 4 + scalar_wave()); i < count; i += kRows * 4 * gridDim.x)
+    move_slots(p, b, p.to + at, p.from + at, i, count);
 }
 
 // ---- longer sequences: a workgroup a chunk, a launch a step -------------------------------------------------------
@@ -297,10 +338,7 @@ __global__ __launch_bounds__(kChunkThreads) void evict_latest_kernel(EvictParams
   for (int i = c.nth * kChunkThreads + tid; i < kPasses * kBins; i += p.chunks * kChunkThreads) hist[i] = 0;
   int latest = INT32_MIN;
   for (int s = c.begin + tid; s < c.end; s += kChunkThreads) latest = max(latest, p.c.positions[c.row + s]);
-  for (int k = 1; k < kWave; k <<= 1) latest = max(latest, __shfl_xor(latest, k, kWave));
-  if (tid % kWave == 0) small[tid / kWave] = latest;
-  __syncthreads();
-  for (int v = 0; v < kChunkThreads / kWave; ++v) latest = max(latest, small[v]);
+  latest = latest_of<kChunkThreads>(latest, small);
   if (tid == 0) p.chunk[4 * static_cast<int64_t>(blockIdx.x)] = latest;
 }
 
@@ -326,10 +364,7 @@ __global__ __launch_bounds__(kChunkThreads) void evict_count_kernel(EvictParams 
     latest = INT32_MIN;
     for (int i = tid; i < p.chunks && i * p.chunk_slots < c.n; i += T)
       latest = max(latest, p.chunk[4 * (static_cast<int64_t>(c.b) * p.chunks + i)]);
-    for (int k = 1; k < kWave; k <<= 1) latest = max(latest, __shfl_xor(latest, k, kWave));
-    if (tid % kWave == 0) small[tid / kWave] = latest;
-    __syncthreads();
-    for (int v = 0; v < T / kWave; ++v) latest = max(latest, small[v]);
+    latest = latest_of<T>(latest, small);
     if (c.nth == 0 && tid == 0) state[2 * kPasses] = latest;
   } else {
     latest = state[2 * kPasses];
@@ -434,7 +469,7 @@ __global__ __launch_bounds__(kChunkThreads) void evict_place_kernel(EvictParams 
         equal[x] = tallies[4 * i + 2 + x];
       }
     }
-    const int incl = wave_inclusive(equal[0] + equal[1]);
+    const int incl = wave_prefix(equal[0] + equal[1]);
     __syncthreads();
     if (lane == kWave - 1) sums[0][wave] = incl;
     __syncthreads();
@@ -484,7 +519,7 @@ __global__ __launch_bounds__(kChunkThreads) void evict_place_kernel(EvictParams 
       k[j] = weight_key(w[j], pos[j], p.sink, latest, p.recent);
       flag[j] = s < c.end && k[j] == key;
     }
-    prefix_counts<T>(flag, before, total, scratch);
+    prefix_counts<T>(flag, before, total, scratch, kChunkSlots);
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) {
       const int s = base + j * T + tid;
@@ -497,7 +532,7 @@ __global__ __launch_bounds__(kChunkThreads) void evict_place_kernel(EvictParams 
       flag[j] = s >= c.end ? 0 : s < c.m ? !kept : kept ? 0x10000u : 0;
     }
     equal_before += total;
-    prefix_counts<T>(flag, before, total, scratch);
+    prefix_counts<T>(flag, before, total, scratch, kChunkSlots);
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) {
       const int s = base + j * T + tid;
@@ -589,8 +624,8 @@ int launch_paged_evict(const kvssd_paged_cache& c, const kvssd_paged_evict_args&
     q.c.positions += b0 * static_cast<int64_t>(p.capacity);
     q.weights_out += b0 * static_cast<int64_t>(p.capacity);
     q.positions_out += b0 * static_cast<int64_t>(p.capacity);
-    int blocks = (p.most + 3) / 4;
-    const int cap = 8192 / nb < 1 ? 1 : 8192 / nb;
+    int blocks = (p.most + 4 * kRows - 1) / (4 * kRows);
+    const int cap = 4096 / nb < 1 ? 1 : 4096 / nb;
     blocks = blocks < cap ? blocks : cap;
     hipLaunchKernelGGL(evict_move_kernel, dim3(blocks, nb), dim3(256), 0, stream, q);
   }

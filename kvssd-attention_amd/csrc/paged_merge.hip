@@ -80,28 +80,49 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
   if (tid == 0 && blockIdx.y == 0) p.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (big + log2f(total));
 }
 
+// A slot's weight: 2^(score - the head's sum) over its heads.  A workgroup takes 4 kWave slots; its waves take a
+// quarter of the heads each, kDeep rows of scores on the way at a time, and are joined in LDS in a fixed order.
 __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodeParams p) {
+  constexpr int kDeep = 8, kWaves = kThreads / kWave;
+  __shared__ f32x4 sums[kWaves][kWave];
   const int seq = blockIdx.y;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int length = paged_length(p.c.lengths, seq, p.capacity);
   const float* lse = p.lse + static_cast<int64_t>(seq) * p.query_heads;
-  for (int64_t t = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 4; t < length;
-       t += static_cast<int64_t>(gridDim.x) * kThreads * 4) {
-    const float* s = p.scores + static_cast<int64_t>(seq) * p.query_heads * p.score_stride + t;
+  const float* scores = p.scores + static_cast<int64_t>(seq) * p.query_heads * p.score_stride;
+  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * 4 * kWave; t0 < length;
+       t0 += static_cast<int64_t>(gridDim.x) * 4 * kWave) {
+    const int64_t t = t0 + 4 * lane;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int h = 0; h < p.query_heads; ++h) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(s + h * p.score_stride);
-      const float e = lse[h] * kLog2e;
-      if (e == -INFINITY) continue;  // no slot took part
+    if (t < length) {  // (rows are of whole 64 slots)
+      for (int h0 = wave; h0 < p.query_heads; h0 += kDeep * kWaves) {
+        f32x4 v[kDeep];
+        float e[kDeep];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] += exp2f(v[i] - e);
+        for (int i = 0; i < kDeep; ++i) {
+          const int h = h0 + i * kWaves;
+          e[i] = h < p.query_heads ? lse[h] * kLog2e : -INFINITY;
+          if (h < p.query_heads) v[i] = *reinterpret_cast<const f32x4*>(scores + h * p.score_stride + t);
+        }
+#pragma unroll
+        for (int i = 0; i < kDeep; ++i) {
+          if (e[i] == -INFINITY) continue;  // no such head, or none of its slots took part
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sum[x] += __builtin_amdgcn_exp2f(v[i][x] - e[i]);
+        }
+      }
     }
-    float* w = p.c.weights + static_cast<int64_t>(seq) * p.capacity + t;
+    sums[wave][lane] = sum;
+    __syncthreads();
+    // thread n: slot n of the workgroup's
+    float w = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (t + i < length) w[i] += sum[i];
+    for (int v = 0; v < kWaves; ++v) w += reinterpret_cast<const float*>(sums[v])[threadIdx.x];
+    if (t0 + threadIdx.x < length) p.c.weights[static_cast<int64_t>(seq) * p.capacity + t0 + threadIdx.x] += w;
+    __syncthreads();
   }
 }
+static_assert(kThreads == 4 * kWave, "a thread a slot");
 
 // Runs and shapes of a decode; the workspace's arrays as offsets from its start.
 struct Plan {
@@ -212,8 +233,8 @@ int launch_paged_decode(const kvssd_paged_cache& c, const kvssd_paged_decode_arg
     if (int rc = launch_paged_merge(p, stream)) return rc;
   if (a.accumulate) {
     const int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
-    const int64_t blocks = (longest + 4 * kThreads - 1) / (4 * kThreads);
-    hipLaunchKernelGGL(paged_weights_kernel, dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024), c.sequences),
+    const int64_t blocks = (longest + 4 * kWave - 1) / (4 * kWave);
+    hipLaunchKernelGGL(paged_weights_kernel, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), c.sequences),
                        dim3(kThreads), 0, stream, p);
     return hip_status(hipGetLastError(), "paged_weights launch");
   }
