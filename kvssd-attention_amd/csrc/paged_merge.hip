@@ -19,18 +19,22 @@ namespace kvssd {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSlice = 64;  // dims of a workgroup: 16 lanes of 4, 16 runs side by side
+constexpr int kFewRows = 1024;
 
+// LANES: lanes of a run, 4 dims each; kThreads / LANES runs side by side.  Many rows take all their dims in one
+// workgroup (64 sequences of 32 heads, 128 dims: 8.1 us, in two of 64 dims 10.6); few rows are spread over slices of
+// 64 (one sequence of 32 heads: 5.8 us, 6.7 in one).
+template <int LANES>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams p) {
   __shared__ float w_s[kMaxSplits];
   __shared__ float red[2][kThreads / kWave];
-  __shared__ f32x4 sum_s[kThreads / kWave][16];
+  __shared__ f32x4 sum_s[kThreads / kWave][LANES];
   const int seq = blockIdx.x / p.query_heads, h = blockIdx.x % p.query_heads;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   int first_run, n;
   runs_of(p, seq, &first_run, &n);
   const int64_t row0 = static_cast<int64_t>(first_run) * p.query_heads + h;  // run r: row0 + r * query_heads
-  const int d0 = blockIdx.y * kSlice + 4 * (tid & 15);
+  const int d0 = 4 * (blockIdx.y * LANES + tid % LANES);
   const int d = p.c.head_dim;
   float big = -INFINITY;
   for (int r = tid; r < n; r += kThreads) {
@@ -58,7 +62,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
     const float* o = p.part_o + row0 * d + d0;
     const int64_t step = static_cast<int64_t>(p.query_heads) * d;
 #pragma unroll 4
-    for (int r = tid / 16; r < n; r += kThreads / 16) {
+    for (int r = tid / LANES; r < n; r += kThreads / LANES) {
       const float w = w_s[r];
       const f32x4 v = *reinterpret_cast<const f32x4*>(o + r * step);
       if (w != 0.0f) acc += w * v;  // (NaN weights take part)
@@ -66,13 +70,13 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    acc[i] += __shfl_xor(acc[i], 16, kWave);
-    acc[i] += __shfl_xor(acc[i], 32, kWave);
+    if constexpr (LANES <= 16) acc[i] += __shfl_xor(acc[i], 16, kWave);
+    if constexpr (LANES <= 32) acc[i] += __shfl_xor(acc[i], 32, kWave);
   }
-  if (lane < 16) sum_s[wave][lane] = acc;
+  if (lane < LANES) sum_s[wave][lane] = acc;
   __syncthreads();
   const int64_t row = static_cast<int64_t>(seq) * p.query_heads + h;
-  if (tid < 16 && d0 < d) {
+  if (tid < LANES && d0 < d) {
     const f32x4 v = (sum_s[0][tid] + sum_s[1][tid]) + (sum_s[2][tid] + sum_s[3][tid]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) store_out(p.out, p.out_dtype, row * d + d0 + i, total == 0.0f ? 0.0f : v[i] / total);
@@ -196,8 +200,10 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, Plan* 
 }  // namespace
 
 int launch_paged_merge(const PagedDecodeParams& p, hipStream_t stream) {
-  const dim3 grid(p.c.sequences * p.query_heads, (p.c.head_dim + kSlice - 1) / kSlice);
-  hipLaunchKernelGGL(paged_merge_kernel, grid, dim3(kThreads), 0, stream, p);
+  const int rows = p.c.sequences * p.query_heads, d = p.c.head_dim;
+  if (rows < kFewRows || d <= 64) hipLaunchKernelGGL(paged_merge_kernel<16>, dim3(rows, (d + 63) / 64), dim3(kThreads), 0, stream, p);
+  else if (d <= 128) hipLaunchKernelGGL(paged_merge_kernel<32>, dim3(rows), dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL(paged_merge_kernel<64>, dim3(rows), dim3(kThreads), 0, stream, p);
   return hip_status(hipGetLastError(), "paged_merge launch");
 }
 
