@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTurns = 512;
-constexpr int kMaxTokens = 4;  // of a workgroup
+constexpr int kMaxTokens = 8;  // of a workgroup
 
 struct AppendParams {
   kvssd_paged_cache c;
@@ -32,7 +32,12 @@ struct AppendParams {
   int64_t tokens;
   int inverse, per_group, capacity;
   int words, lanes, groups;  // code words of a head's row, words of a group, groups of a row
-  int query_heads;
+  int query_heads, lanes_log2;
+  uint32_t of_token;  // code words of a token's keys and values
+  Divisor of_head;    // of a head
+  int width;          // threads side by side on a token's, log2
+  int row_bytes, row_scales;
+  Divisor of_query, items;    // items of a token's queries, of a head
 };
 
 // Sequence of token t: the b with offsets[b] <= t < offsets[b + 1], -1 if none.
@@ -47,60 +52,84 @@ __device__ __forceinline__ int sequence_of(const int32_t* offsets, int sequences
   return lo;
 }
 
-// A word's values: loaded, and rotated if `turns`.
+// A word's values: loaded, then rotated if `turns`.  Either half of a pair is own cos -+ other sin, so that a thread
+// forms its own half alone, with the sign on the other.
 template <typename T, int N, bool VEC>
-__device__ __forceinline__ void word_values(const T* x, int d0, const RotaryShape& s, const Turn* turns, float (&out)[N]) {
-  if constexpr (VEC) {  // no word mixes low, high and unturned values, and all loads are 16-byte aligned
-    T a[N];
-    load_values(x + d0, a);
-    if (turns == nullptr || d0 >= 2 * s.pairs) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) out[i] = to_f32(a[i]);
-    } else if (s.interleaved) {
-#pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        const Turn t = turns[d0 / 2 + i / 2];
-        out[i] = to_f32(store_cast<T>(turn_low(to_f32(a[i]), to_f32(a[i + 1]), t)));
-        out[i + 1] = to_f32(store_cast<T>(turn_high(to_f32(a[i]), to_f32(a[i + 1]), t)));
-      }
+struct Word {
+  T a[N], b[N];  // the values; their partners, in a half layout
+
+  __device__ __forceinline__ void load(const T* x, int d0, const RotaryShape& s, bool turned) {
+    if constexpr (VEC) {  // no word mixes low, high and unturned values, and all loads are 16-byte aligned
+      load_values(x + d0, a);
+      if (turned && d0 < 2 * s.pairs && !s.interleaved) load_values(x + (d0 >= s.pairs ? d0 - s.pairs : d0 + s.pairs), b);
     } else {
-      const bool high = d0 >= s.pairs;
-      const int p0 = high ? d0 - s.pairs : d0;
-      T b[N];
-      load_values(x + (high ? p0 : d0 + s.pairs), b);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const Turn t = turns[p0 + i];
-        const float own = to_f32(a[i]), other = to_f32(b[i]);
-        out[i] = to_f32(store_cast<T>(high ? turn_high(other, own, t) : turn_low(own, other, t)));
+        const int d = d0 + i;
+        a[i] = b[i] = x[d];
+        if (turned && d < 2 * s.pairs) b[i] = x[s.interleaved ? d ^ 1 : (d >= s.pairs ? d - s.pairs : d + s.pairs)];
       }
-    }
-  } else {
-    for (int i = 0; i < N; ++i) {
-      const int d = d0 + i;
-      const float own = to_f32(x[d]);
-      if (turns == nullptr || d >= 2 * s.pairs) {
-        out[i] = own;
-        continue;
-      }
-      const bool high = s.interleaved ? d % 2 : d >= s.pairs;
-      const int p = s.interleaved ? d / 2 : (high ? d - s.pairs : d);
-      const float other = to_f32(x[s.interleaved ? d ^ 1 : (high ? p : d + s.pairs)]);
-      out[i] = to_f32(store_cast<T>(high ? turn_high(other, own, turns[p]) : turn_low(own, other, turns[p])));
     }
   }
-}
+  static __device__ __forceinline__ float turn(float own, float other, bool high, Turn t) {
+    return to_f32(round_to<T>(turn_high(high ? other : -other, own, t)));
+  }
+  __device__ __forceinline__ void values(int d0, const RotaryShape& s, const Turn* turns, float (&out)[N]) const {
+    if (turns == nullptr || (VEC && d0 >= 2 * s.pairs)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) out[i] = to_f32(a[i]);
+    } else if constexpr (VEC) {
+      if (s.interleaved) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = turn(to_f32(a[i]), to_f32(a[i ^ 1]), i % 2, turns[turn_place(d0 / 2 + i / 2)]);
+      } else {
+        const bool high = d0 >= s.pairs;
+        const Turn* t = turns + turn_place(high ? d0 - s.pairs : d0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = turn(to_f32(a[i]), to_f32(b[i]), high, t[turn_place(i)]);  // (d0: a multiple of 8)
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int d = d0 + i;
+        const bool high = s.interleaved ? d % 2 : d >= s.pairs;
+        const int p = s.interleaved ? d / 2 : (high ? d - s.pairs : d);
+        out[i] = d < 2 * s.pairs ? turn(to_f32(a[i]), to_f32(b[i]), high, turns[turn_place(p)]) : to_f32(a[i]);
+      }
+    }
+  }
+};
 
 template <typename T, int BITS, bool VEC>
-__global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendParams p) {
+__global__ __launch_bounds__(kThreads, VEC ? 4 : 1) void paged_append_kernel(AppendParams p) {
   constexpr int kVals = 32 / BITS;
   constexpr int kItem = VEC ? 16 / sizeof(T) : 1;
-  __shared__ Turn turns[kMaxTurns];
+  __shared__ Turn turns[turn_place(kMaxTurns) + kMaxTokens];
   __shared__ int64_t row_s[kMaxTokens];  // row of the pool, -1: dropped
   __shared__ double position_s[kMaxTokens];
   const kvssd_paged_cache& c = p.c;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.per_group;
   const int n = static_cast<int>(p.tokens - t0 < p.per_group ? p.tokens - t0 : p.per_group);
+  // a thread's words lie at one place of every token that it takes
+  const uint32_t per_token = p.of_token, coded = per_token / 2;
+  const int first = threadIdx.x >> p.width, step = kThreads >> p.width;  // tokens
+  // its first item of the queries sets out now, the others one ahead
+  const bool in_place = p.query.data == p.query.out;
+  const uint32_t queries = static_cast<uint32_t>(n) * p.of_query.d;
+  struct Query {
+    RotaryItem<T, kItem> v;
+    int tok, head, item;
+  } next_query;
+  auto fetch_query = [&](uint32_t i) {
+    next_query.tok = p.of_query.quotient(i);
+    const uint32_t rest = i - next_query.tok * p.of_query.d;
+    next_query.head = p.items.quotient(rest);
+    next_query.item = rest - next_query.head * p.items.d;
+    next_query.v.load(p.shape, next_query.item,
+                      static_cast<const T*>(p.query.data) + (t0 + next_query.tok) * p.query.token_stride +
+                          next_query.head * p.query.head_stride, in_place);
+  };
+  if (threadIdx.x < queries) fetch_query(threadIdx.x);
   if (static_cast<int>(threadIdx.x) < n) {
     const int64_t t = t0 + threadIdx.x;
     const int b = p.offsets ? sequence_of(p.offsets, c.sequences, t) : static_cast<int>(t);
@@ -134,48 +163,47 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendParams p) 
     }
   }
   __syncthreads();
+  const int token_turns = turn_place(p.shape.pairs) + 1;
   if (p.frequencies) {
     for (int i = threadIdx.x; i < n * p.shape.pairs; i += kThreads)
-      turns[i] = make_turn(position_s[i / p.shape.pairs], p.frequencies[i % p.shape.pairs], p.magnitude, p.inverse);
+      turns[i / p.shape.pairs * token_turns + turn_place(i % p.shape.pairs)] =
+          make_turn(position_s[i / p.shape.pairs], p.frequencies[i % p.shape.pairs], p.magnitude, p.inverse);
     __syncthreads();
   }
-  const int coded = c.kv_heads * p.words;  // words of a token's keys, and of its values
-  const int per_token = 2 * coded + p.query_heads * p.shape.items;
-  for (int i = threadIdx.x; i < n * per_token; i += kThreads) {
-    const int tok = i / per_token;
-    int rest = i % per_token;
-    const Turn* turn = p.frequencies ? turns + tok * p.shape.pairs : nullptr;
-    if (rest < 2 * coded) {
+  for (uint32_t r = threadIdx.x & ((1u << p.width) - 1); r < per_token; r += 1u << p.width) {
+    const bool is_v = r >= coded, turned = p.frequencies != nullptr && !is_v;
+    const uint32_t rest = is_v ? r - coded : r;
+    const int head = p.of_head.quotient(rest), word = rest - head * p.of_head.d;
+    const int64_t stride = is_v ? p.values.token_stride : p.keys.token_stride;
+    const T* x = static_cast<const T*>(is_v ? p.values.data : p.keys.data) + t0 * stride +
+                 head * (is_v ? p.values.head_stride : p.keys.head_stride);
+    uint8_t* packed = (is_v ? c.packed_v : c.packed_k) + (head * p.words + word) * 4;
+    uint16_t* scales = (is_v ? c.scales_v : c.scales_k) + head * p.groups + (word >> p.lanes_log2);
+    const bool scaler = (word & (p.lanes - 1)) == 0;
+#pragma unroll 1
+    for (int tok = first; tok < n; tok += step) {
       const int64_t row = row_s[tok];
       if (row < 0) continue;  // the same for every lane of a group
-      const bool is_v = rest >= coded;
-      if (is_v) rest -= coded;
-      const int head = rest / p.words, word = rest % p.words;
-      const kvssd_heads& h = is_v ? p.values : p.keys;
-      const T* x = static_cast<const T*>(h.data) + (t0 + tok) * h.token_stride + head * h.head_stride;
+      Word<T, kVals, VEC> w;
+      w.load(x + tok * stride, word * kVals, p.shape, turned);
       float v[kVals];
-      word_values<T, kVals, VEC>(x, word * kVals, p.shape, is_v ? nullptr : turn, v);
+      w.values(word * kVals, p.shape, turned ? turns + tok * token_turns : nullptr, v);
       float amax = 0.0f;
 #pragma unroll
       for (int k = 0; k < kVals; ++k) amax = fmaxf(amax, fabsf(v[k]));
       const float s32 = group_scale<BITS>(lanes_max(amax, p.lanes));
       const uint32_t code = code_word<T, BITS>(v, s32);
-      const int64_t at = row * c.kv_heads + head;
-      uint8_t* packed = (is_v ? c.packed_v : c.packed_k) + (at * p.words + word) * 4;
-      __builtin_memcpy(__builtin_assume_aligned(packed, 4), &code, 4);
-      if ((word & (p.lanes - 1)) == 0)
-        (is_v ? c.scales_v : c.scales_k)[at * p.groups + word / p.lanes] =
-            __builtin_bit_cast(uint16_t, static_cast<_Float16>(s32));
-    } else {
-      rest -= 2 * coded;
-      const int head = rest / p.shape.items, item = rest % p.shape.items;
-      rotary_item<T, kItem>(p.shape, item,
-                            static_cast<const T*>(p.query.data) + (t0 + tok) * p.query.token_stride +
-                                head * p.query.head_stride,
-                            static_cast<T*>(p.query.out) + (t0 + tok) * p.query.out_token_stride +
-                                head * p.query.out_head_stride,
-                            turn);
+      __builtin_memcpy(__builtin_assume_aligned(packed + row * p.row_bytes, 4), &code, 4);
+      if (scaler) scales[row * p.row_scales] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(s32));
     }
+  }
+  for (uint32_t i = threadIdx.x; i < queries; i += kThreads) {
+    Query now = next_query;
+    if (i + kThreads < queries) fetch_query(i + kThreads);
+    now.v.store(p.shape, now.item,
+                static_cast<T*>(p.query.out) + (t0 + now.tok) * p.query.out_token_stride +
+                    now.head * p.query.out_head_stride,
+                turns + now.tok * token_turns, in_place);
   }
 }
 
@@ -192,7 +220,15 @@ void launch_typed(AppendParams& p, const kvssd_paged_append_args& a, hipStream_t
   }
   int per = p.shape.pairs ? kMaxTurns / p.shape.pairs : kMaxTokens;
   per = per < kMaxTokens ? per : kMaxTokens;
-  p.per_group = p.tokens >= 2048 ? per : 1;  // as the rotary kernel's
+  const int64_t share = p.tokens / 1024;  // four workgroups a CU
+  p.per_group = share < 1 ? 1 : share < per ? static_cast<int>(share) : per;
+  p.of_token = 2u * p.c.kv_heads * p.words;
+  while ((1u << p.width) < p.of_token && (1 << p.width) < kThreads) ++p.width;
+  p.row_bytes = p.c.kv_heads * p.words * 4;
+  p.row_scales = p.c.kv_heads * p.groups;
+  p.of_head = divisor(p.words);
+  p.items = divisor(p.shape.items);
+  p.of_query = divisor(int64_t{p.query_heads} * p.shape.items);
   const int64_t blocks = (p.tokens + p.per_group - 1) / p.per_group;
   const dim3 grid(static_cast<unsigned>(blocks > 0 ? blocks : 1));  // no token: lengths_out alone
   if (p.c.bits == 4) {
@@ -245,6 +281,7 @@ int launch_paged_append(const kvssd_paged_cache& c, const kvssd_paged_append_arg
   p.words = c.head_dim * c.bits / 32;
   p.lanes = c.group_size * c.bits / 32;
   p.groups = c.head_dim / c.group_size;
+  while ((1 << p.lanes_log2) < p.lanes) ++p.lanes_log2;
   if (a.rotary) {
     p.frequencies = a.rotary->frequencies;
     p.magnitude = a.rotary->magnitude;

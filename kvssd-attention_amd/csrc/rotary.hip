@@ -10,7 +10,7 @@ namespace kvssd {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTurns = 512;  // of a workgroup: 8 KB of LDS
+constexpr int kMaxTurns = 512, kMostTokens = 4;  // of a workgroup: 9 KB of LDS
 
 struct RotaryParams {
   const double* frequencies;
@@ -20,30 +20,46 @@ struct RotaryParams {
   RotaryShape shape;
   int64_t tokens;
   int count, inverse, positions_64, per_group;  // tokens of a workgroup
+  Divisor items, per_token[2];  // of a head, of a tensor's token
 };
 
 template <typename T, int PV>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p) {
-  __shared__ Turn turns[kMaxTurns];
+  __shared__ Turn turns[turn_place(kMaxTurns) + kMostTokens];
+  const int token_turns = turn_place(p.shape.pairs) + 1;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.per_group;
   const int n = static_cast<int>(p.tokens - t0 < p.per_group ? p.tokens - t0 : p.per_group);
   for (int i = threadIdx.x; i < n * p.shape.pairs; i += kThreads) {
     const int64_t t = t0 + i / p.shape.pairs;
     const double pos = p.positions_64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[t])
                                       : static_cast<double>(static_cast<const int32_t*>(p.positions)[t]);
-    turns[i] = make_turn(pos, p.frequencies[i % p.shape.pairs], p.magnitude, p.inverse);
+    turns[i / p.shape.pairs * token_turns + turn_place(i % p.shape.pairs)] =
+        make_turn(pos, p.frequencies[i % p.shape.pairs], p.magnitude, p.inverse);
   }
   __syncthreads();
   for (int k = 0; k < p.count; ++k) {
     const kvssd_heads& h = p.t[k];
-    const int per_token = h.heads * p.shape.items;
-    for (int i = threadIdx.x; i < n * per_token; i += kThreads) {
-      const int tok = i / per_token, rest = i % per_token;
-      const int head = rest / p.shape.items, item = rest % p.shape.items;
-      rotary_item<T, PV>(p.shape, item,
-                         static_cast<const T*>(h.data) + (t0 + tok) * h.token_stride + head * h.head_stride,
-                         static_cast<T*>(h.out) + (t0 + tok) * h.out_token_stride + head * h.out_head_stride,
-                         turns + tok * p.shape.pairs);
+    const bool in_place = h.data == h.out;
+    const uint32_t count = static_cast<uint32_t>(n) * p.per_token[k].d;
+    struct Next {
+      RotaryItem<T, PV> v;
+      int tok, head, item;
+    } next;
+    auto fetch = [&](uint32_t i) {
+      next.tok = p.per_token[k].quotient(i);
+      const uint32_t rest = i - next.tok * p.per_token[k].d;
+      next.head = p.items.quotient(rest);
+      next.item = rest - next.head * p.items.d;
+      next.v.load(p.shape, next.item,
+                  static_cast<const T*>(h.data) + (t0 + next.tok) * h.token_stride + next.head * h.head_stride, in_place);
+    };
+    if (threadIdx.x < count) fetch(threadIdx.x);
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+      Next now = next;
+      if (i + kThreads < count) fetch(i + kThreads);
+      now.v.store(p.shape, now.item,
+                  static_cast<T*>(h.out) + (t0 + now.tok) * h.out_token_stride + now.head * h.out_head_stride,
+                  turns + now.tok * token_turns, in_place);
     }
   }
 }
@@ -57,8 +73,10 @@ void launch_typed(RotaryParams& p, const kvssd_rotary_spec& r, hipStream_t strea
   int per = kMaxTurns / p.shape.pairs;  // >= 1: at most 512 pairs
   // long prompts: the sines of 4 tokens at a time give every thread one; short
   // ones: a workgroup a token, so that more CUs take part
-  per = p.tokens >= 2048 ? (per < 4 ? per : 4) : 1;
+  per = p.tokens >= 2048 ? (per < kMostTokens ? per : kMostTokens) : 1;
   p.per_group = per;
+  p.items = divisor(p.shape.items);
+  for (int k = 0; k < p.count; ++k) p.per_token[k] = divisor(static_cast<int64_t>(p.t[k].heads) * p.shape.items);
   const dim3 grid(static_cast<unsigned>((p.tokens + per - 1) / per));
   if (vec) hipLaunchKernelGGL((rotary_kernel<T, kVec>), grid, dim3(kThreads), 0, stream, p);
   else hipLaunchKernelGGL((rotary_kernel<T, 1>), grid, dim3(kThreads), 0, stream, p);

@@ -24,6 +24,10 @@ __device__ __forceinline__ Turn make_turn(double position, double frequency, dou
   return Turn{magnitude * c, inverse ? -(magnitude * s) : magnitude * s};
 }
 
+// A token's turns in LDS, one place left free after every 8: lanes that read the turns of words or items 8 pairs apart
+// then meet no bank twice (16 bytes each, 64 banks of 4).
+__host__ __device__ constexpr int turn_place(int pair) { return pair + pair / 8; }
+
 // (a, b) turned: a c - b s and b c + a s
 __device__ __forceinline__ float turn_low(double a, double b, Turn t) {
   return static_cast<float>(__builtin_fma(a, t.c, -(b * t.s)));
@@ -67,49 +71,70 @@ inline RotaryShape rotary_shape(const kvssd_rotary_spec& r, int pv) {
   return s;
 }
 
-// One item of a head: PV pairs turned (`turns` of the token), or PV values
-// passed through.  Every value is read and written by one thread only, so y
-// may be x.
+// x in type T, rounded to nearest even (a NaN stays one)
+template <typename T>
+__device__ __forceinline__ T round_to(float x) {
+  if constexpr (sizeof(T) == 2 && __is_same(T, uint16_t)) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+  else return static_cast<T>(x);
+}
+
+// One item of a head: PV pairs to turn, or PV values to pass through (a alone; none where y is x).  Every value is
+// read and written by one thread only, so y may be x.
 template <typename T, int PV>
-__device__ __forceinline__ void rotary_item(const RotaryShape& s, int item, const T* x, T* y, const Turn* turns) {
-  if (item >= s.turn_items) {
-    const int at = 2 * s.pairs + (item - s.turn_items) * PV;
-    if (x == y) return;
-    T v[PV];
-    load_values(x + at, v);
-    store_values(y + at, v);
-    return;
-  }
-  const int p0 = item * PV;
+struct RotaryItem {
   T a[PV], b[PV];
-  const int at0 = s.interleaved ? 2 * p0 : p0;
-  const int at1 = s.interleaved ? 2 * p0 + PV : s.pairs + p0;
-  load_values(x + at0, a);
-  load_values(x + at1, b);
-  T lo[PV], hi[PV];
-  if (s.interleaved) {
-#pragma unroll
-    for (int i = 0; i < PV; ++i) {
-      const T va = 2 * i < PV ? a[(2 * i) % PV] : b[(2 * i) % PV];
-      const T vb = 2 * i + 1 < PV ? a[(2 * i + 1) % PV] : b[(2 * i + 1) % PV];
-      const Turn t = turns[p0 + i];
-      const T l = store_cast<T>(turn_low(to_f32(va), to_f32(vb), t));
-      const T h = store_cast<T>(turn_high(to_f32(va), to_f32(vb), t));
-      if (2 * i < PV) lo[(2 * i) % PV] = l;
-      else hi[(2 * i) % PV] = l;
-      if (2 * i + 1 < PV) lo[(2 * i + 1) % PV] = h;
-      else hi[(2 * i + 1) % PV] = h;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < PV; ++i) {
-      const Turn t = turns[p0 + i];
-      lo[i] = store_cast<T>(turn_low(to_f32(a[i]), to_f32(b[i]), t));
-      hi[i] = store_cast<T>(turn_high(to_f32(a[i]), to_f32(b[i]), t));
-    }
+
+  static __device__ __forceinline__ int first(const RotaryShape& s, int item) {
+    return item >= s.turn_items ? 2 * s.pairs + (item - s.turn_items) * PV : s.interleaved ? 2 * item * PV : item * PV;
   }
-  store_values(y + at0, lo);
-  store_values(y + at1, hi);
+  __device__ __forceinline__ void load(const RotaryShape& s, int item, const T* x, bool in_place) {
+    const int at = first(s, item);
+    if (item < s.turn_items) load_values(x + at + (s.interleaved ? PV : s.pairs), b);
+    if (item < s.turn_items || !in_place) load_values(x + at, a);
+  }
+  // `turns` of the item's token
+  __device__ __forceinline__ void store(const RotaryShape& s, int item, T* y, const Turn* turns, bool in_place) {
+    const int at = first(s, item);
+    if (item >= s.turn_items) {
+      if (!in_place) store_values(y + at, a);
+      return;
+    }
+    const Turn* turn = turns + turn_place(item * PV);  // (PV pairs without a free place among them)
+    T lo[PV], hi[PV];
+    if (s.interleaved) {
+#pragma unroll
+      for (int i = 0; i < PV; ++i) {
+        const float va = to_f32(2 * i < PV ? a[(2 * i) % PV] : b[(2 * i) % PV]);
+        const float vb = to_f32(2 * i + 1 < PV ? a[(2 * i + 1) % PV] : b[(2 * i + 1) % PV]);
+        const T l = round_to<T>(turn_low(va, vb, turn[i])), h = round_to<T>(turn_high(va, vb, turn[i]));
+        if (2 * i < PV) lo[(2 * i) % PV] = l;
+        else hi[(2 * i) % PV] = l;
+        if (2 * i + 1 < PV) lo[(2 * i + 1) % PV] = h;
+        else hi[(2 * i + 1) % PV] = h;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PV; ++i) {
+        lo[i] = round_to<T>(turn_low(to_f32(a[i]), to_f32(b[i]), turn[i]));
+        hi[i] = round_to<T>(turn_high(to_f32(a[i]), to_f32(b[i]), turn[i]));
+      }
+    }
+    store_values(y + at, lo);
+    store_values(y + at + (s.interleaved ? PV : s.pairs), hi);
+  }
+};
+
+// Division of 32-bit numbers by one that the host knows.
+struct Divisor {
+  uint32_t d, m;  // m = 2^32 / d, rounded up
+  __device__ __forceinline__ uint32_t quotient(uint32_t x) const {
+    if (d == 1) return x;
+    const uint32_t q = __umulhi(x, m);  // right or one too many: x m / 2^32 is past x / d by less than 1
+    return q * d > x ? q - 1 : q;
+  }
+};
+inline Divisor divisor(int64_t d) {
+  return Divisor{static_cast<uint32_t>(d), d > 1 ? static_cast<uint32_t>(((uint64_t{1} << 32) + d - 1) / d) : 0};
 }
 
 // 16-byte loads of a heads tensor's values: its addresses and strides allow them
