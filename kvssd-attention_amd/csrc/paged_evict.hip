@@ -563,8 +563,7 @@ EvictPlan plan_evict(const kvssd_paged_cache& c, int budget) {
   e.one = capacity <= kOneSlots;
   e.inner = e.one && e.most <= kInnerMoves;
   const size_t n = c.sequences;
-  if (e.inner) return e;
-  e.words = n * (1 + 2 * static_cast<size_t>(e.most));
+  e.words = n * (1 + 2 * static_cast<size_t>(e.most));  // (also where no move's list leaves LDS: one size a budget)
   if (e.one) return e;
   const int64_t most_chunks = capacity / kChunkSlots / kMostChunks + 1;  // units of kChunkSlots a chunk
   e.chunk_slots = static_cast<int>(most_chunks) * kChunkSlots;
@@ -670,7 +669,7 @@ __attribute__((visibility("default"))) int kvssd_hip_paged_evict(const kvssd_pag
       args->lengths_out == cache->lengths)
     return arg_error("eviction writes arrays of their own, not the cache's");
   const size_t need = evict_bytes(*cache, args->budget);
-  if (need > 0 && (args->workspace == nullptr || args->workspace_bytes < need))
+  if (args->workspace == nullptr || args->workspace_bytes < need)
     return arg_error("workspace too small: need " + std::to_string(need) + " bytes");
   return launch_paged_evict(*cache, *args, static_cast<hipStream_t>(stream));
 }

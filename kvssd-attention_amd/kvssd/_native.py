@@ -195,6 +195,8 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
     translation-unit ids (``__hip_cuid_*``) for their device code, and a
     process that mapped two of them crashed at its first launches."""
     global _lib, _load_error, _loaded_from
+    if path is None and _lib is not None and _loaded_from == LIB_PATH:
+        return _lib
     want = LIB_PATH if path is None else Path(path).resolve()
     with _lock:
         if _lib is not None:

@@ -112,6 +112,7 @@ class PagedBatch:
         if self.page_table.ndim != 2 or self.lengths.shape != (self.page_table.shape[0],):
             raise ValueError("page_table must be [sequences,max_pages] and lengths [sequences]")
         slots = (self.page_table.shape[0], self.capacity)
+        device = self.packed_k.device
         for name, t, dtype in (
             ("packed KV", self.packed_k, torch.uint8), ("packed KV", self.packed_v, torch.uint8),
             ("scales", self.scales_k, torch.float16), ("scales", self.scales_v, torch.float16),
@@ -120,9 +121,9 @@ class PagedBatch:
         ):
             if t is None:
                 continue
-            if t.dtype != dtype:
+            if t.dtype is not dtype:
                 raise ValueError(f"{name} must be {str(dtype).removeprefix('torch.')}")
-            if t.device != self.packed_k.device:
+            if t.device != device:
                 raise ValueError("a paged cache must lie on one device")
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")

@@ -16,6 +16,7 @@ Takes over the role of the reference's CudaExtensionBackend
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from collections.abc import Sequence
 
@@ -44,6 +45,14 @@ def current_stream_handle(index: int) -> int:
 # without its lazy-initialisation check (the device is initialised by the time
 # a prepared decode exists).
 _CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(index: int):
+    """torch.cuda.device(index), or nothing to enter where that device is the current one."""
+    return _HERE if _CURRENT_DEVICE() == index else torch.cuda.device(index)
 
 
 def _index(device: torch.device) -> int:

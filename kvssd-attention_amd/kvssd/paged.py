@@ -25,9 +25,9 @@ import torch
 
 from . import _native
 from .backends import AttentionBackend, PackedBatch, PagedBatch, resolve_attention_backend
-from .backends.hip import current_stream_handle
+from .backends.hip import current_stream_handle, on_device
 from .backends.paged import native_cache
-from .rotary import _DTYPES, Rotary, check_heads, heads_of, refuse_grad
+from .rotary import _DTYPES, Rotary, check_heads, empty_heads, heads_of, refuse_grad
 
 
 def _gpu_index(batch: PagedBatch) -> int:
@@ -98,25 +98,24 @@ def append_tokens(
     elif _int32(lengths_out, "lengths_out", sequences, device) is not lengths_out:
         raise ValueError("lengths_out must be contiguous")
     keys, values = (t if t.stride(2) == 1 else t.contiguous() for t in (keys, values))
-    turned = None
-    args = _native.PagedAppendArgs(
-        heads_of(keys), heads_of(values), tokens=tokens, offsets=None if offsets is None else offsets.data_ptr(),
-        first_positions=None if first_positions is None else first_positions.data_ptr(),
-        lengths_out=lengths_out.data_ptr(), dtype=_DTYPES[dtype],
-    )
-    if rotary is not None:
-        args.rotary = ctypes.pointer(rotary.spec())
+    turned, turns = None, ()
     if query is not None:
         query = query if query.stride(2) == 1 else query.contiguous()
-        turned = torch.empty(query.shape, dtype=dtype, device=device)
+        turned = empty_heads(query)
         if query.shape[1]:
-            args.query = heads_of(query, turned)
+            turns = heads_of(query, turned)
+    args = _native.PagedAppendArgs(
+        heads_of(keys), heads_of(values), turns, tokens, None if offsets is None else offsets.data_ptr(),
+        None if first_positions is None else first_positions.data_ptr(),
+        None if rotary is None else ctypes.pointer(rotary.spec()), lengths_out.data_ptr(), _DTYPES[dtype], 0,
+    )
     cache = native_cache(batch)
-    with torch.cuda.device(index):
+    with on_device(index):
         rc = _native.load().kvssd_hip_paged_append(
             ctypes.addressof(cache), ctypes.addressof(args), current_stream_handle(index)
         )
-    _native.check(rc, "kvssd_hip_paged_append")
+    if rc:
+        _native.check(rc, "kvssd_hip_paged_append")
     return turned, lengths_out
 
 
@@ -151,10 +150,11 @@ def evict_tokens(
     where = ctypes.addressof(cache), ctypes.addressof(args)
     _native.check(lib.kvssd_hip_paged_evict_workspace_bytes(*where, ctypes.byref(need)), "kvssd_hip_paged_evict")
     work = torch.empty((need.value,), dtype=torch.uint8, device=batch.packed_k.device)
-    args.workspace, args.workspace_bytes = work.data_ptr(), work.numel()
-    with torch.cuda.device(index):
+    args.workspace, args.workspace_bytes = work.data_ptr(), need.value
+    with on_device(index):
         rc = lib.kvssd_hip_paged_evict(*where, current_stream_handle(index))
-    _native.check(rc, "kvssd_hip_paged_evict")
+    if rc:
+        _native.check(rc, "kvssd_hip_paged_evict")
     return lengths, weights, positions
 
 

@@ -23,10 +23,11 @@ from dataclasses import dataclass
 import torch
 
 from . import _native
-from .backends.hip import current_stream_handle
+from .backends.hip import current_stream_handle, on_device
 
 _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16, torch.float32: _native.DTYPE_F32}
 _KINDS = ("linear", "ntk", "yarn", "wavelength")
+_PAIR = _native.Heads * 2
 
 
 @dataclass(frozen=True)
@@ -119,19 +120,24 @@ def _overlaps_itself(t: torch.Tensor) -> bool:
     return False
 
 
-def heads_of(t: torch.Tensor, out: torch.Tensor | None = None) -> _native.Heads:
-    """kvssd_heads of a [tokens, heads, head_dim] tensor (its values of a head side by side)."""
-    s = t.stride()
+def heads_of(t: torch.Tensor, out: torch.Tensor | None = None) -> tuple:
+    """Fields of kvssd_heads of a [tokens, heads, head_dim] tensor (its values of a head side by side)."""
+    token, head, _ = t.stride()
     if out is None:
-        return _native.Heads(t.data_ptr(), None, s[0], s[1], 0, 0, t.shape[1], 0)
-    o = out.stride()
-    return _native.Heads(t.data_ptr(), out.data_ptr(), s[0], s[1], o[0], o[1], t.shape[1], 0)
+        return t.data_ptr(), None, token, head, 0, 0, t.shape[1], 0
+    out_token, out_head, _ = out.stride()
+    return t.data_ptr(), out.data_ptr(), token, head, out_token, out_head, t.shape[1], 0
+
+
+def empty_heads(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def check_heads(t: torch.Tensor, name: str, tokens: int, head_dim: int, dtype: torch.dtype, device: torch.device) -> None:
-    if t.ndim != 3 or t.shape[0] != tokens or t.shape[2] != head_dim:
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim:
         raise ValueError(f"{name} must be [{tokens}, heads, {head_dim}], got {tuple(t.shape)}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must have dtype {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
@@ -166,6 +172,8 @@ class Rotary:
         self.magnitude = 1.0 if scaling is None else scaling.magnitude
         host = torch.tensor(rotary_frequencies(rotary_dim, base, scaling), dtype=torch.float64)
         self.frequencies = host.to(device)
+        self._device = self.frequencies.device  # (with its index, on a GPU)
+        self._index = self._device.index if self._device.type == "cuda" else None
         self._specs = tuple(
             _native.RotarySpec(self.frequencies.data_ptr(), self.magnitude, head_dim, rotary_dim,
                                int(layout == "interleaved"), inverse)
@@ -185,8 +193,8 @@ class Rotary:
         inverse: bool = False,
         inplace: bool = False,
     ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
-        device = self.frequencies.device
-        if device.type != "cuda":
+        device, index = self._device, self._index
+        if index is None:
             raise ValueError(f"rotary positions require ROCm GPU tensors, got {device.type}")
         dtype, tokens = query.dtype, query.shape[0] if query.ndim else 0
         if dtype not in _DTYPES:
@@ -206,15 +214,15 @@ class Rotary:
             outs = tensors
         else:
             tensors = tuple(t if t.stride(2) == 1 else t.contiguous() for t in tensors)
-            outs = tuple(torch.empty(t.shape, dtype=dtype, device=device) for t in tensors)
+            outs = tuple(map(empty_heads, tensors))
         if tokens:
             positions = positions if positions.is_contiguous() else positions.contiguous()
-            heads = (_native.Heads * len(tensors))(*(heads_of(t, o) for t, o in zip(tensors, outs)))
-            index = device.index if device.index is not None else torch.cuda.current_device()
-            with torch.cuda.device(index):
+            heads = _PAIR(*map(heads_of, tensors, outs))
+            with on_device(index):
                 rc = _native.load().kvssd_hip_rotary(
-                    self._addresses[bool(inverse)], positions.data_ptr(), int(positions.dtype == torch.int64), tokens,
+                    self._addresses[bool(inverse)], positions.data_ptr(), int(positions.dtype is torch.int64), tokens,
                     _DTYPES[dtype], ctypes.addressof(heads), len(tensors), current_stream_handle(index),
                 )
-            _native.check(rc, "kvssd_hip_rotary")
+            if rc:
+                _native.check(rc, "kvssd_hip_rotary")
         return outs[0] if key is None else outs
