@@ -71,10 +71,12 @@ inline RotaryShape rotary_shape(const kvssd_rotary_spec& r, int pv) {
   return s;
 }
 
-// x in type T, rounded to nearest even (a NaN stays one)
+// x in type T, rounded to nearest even (a NaN stays one).  x is rounded to 32 bits already, and kept from the compiler,
+// which may otherwise round the 64-bit value before it to 16 bits at once: another result in 2^-17 of the values.
 template <typename T>
 __device__ __forceinline__ T round_to(float x) {
-  if constexpr (sizeof(T) == 2 && __is_same(T, uint16_t)) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+  if constexpr (sizeof(T) == 2) asm("" : "+v"(x));
+  if constexpr (__is_same(T, uint16_t)) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
   else return static_cast<T>(x);
 }
 

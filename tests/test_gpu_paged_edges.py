@@ -1,0 +1,232 @@
+"""The paged cache's operators at the edges of what a call may hold: thousands of sequences, shared pages, pools past
+4 GiB, queries of any alignment and stride, two host threads, and codes bit for bit over millions of values."""
+
+from __future__ import annotations
+
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+from kvssd import Rotary, append_tokens, evict_tokens
+from kvssd.backends import PagedBatch
+from kvssd.backends.hip import HipAttentionBackend
+from paged_oracle import as_double, attend, make_pool, make_table
+from test_gpu_paged import check_attention, paged
+
+pytestmark = pytest.mark.gpu
+
+
+MANY = [
+    # lengths, bits, query heads, kv heads, head_dim, page_tokens
+    ([0] * 99 + [20000], 4, 4, 1, 32, 64),  # one long sequence behind a wave of empty ones
+    ([20000] + [1] * 200, 2, 2, 2, 64, 32),
+    ([(37 * i) % 301 for i in range(130)], 4, 8, 2, 64, 16),
+    ([i % 3 for i in range(1500)], 4, 2, 1, 32, 8),
+    ([5] * 64, 2, 16, 8, 128, 64),
+    ([64 * i for i in range(65)], 4, 4, 4, 32, 64),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"{len(c[0])}-{max(c[0])}-int{c[1]}")
+def test_attention_over_many_sequences(cuda_device, case):
+    lengths, bits, qh, kvh, d, bt = case
+    rng = np.random.default_rng(len(lengths))
+    width = max(-(-n // bt) for n in lengths) + 1
+    pages = sum(-(-n // bt) for n in lengths) + 1
+    pool = make_pool(rng, pages, bt, kvh, d, 32, bits)
+    table = make_table(rng, lengths, bt, width, pages)
+    batch = paged(cuda_device, pool, table, lengths, bits, 32)
+    q = torch.from_numpy(rng.standard_normal((len(lengths), qh, d))).half().to(cuda_device)
+    want = attend(as_double(q), pool, table, lengths, bits, 0.125)
+    backend = HipAttentionBackend()
+    for hints in ({}, dict(max_length=max(lengths), total_tokens=sum(lengths)), dict(max_length=64, total_tokens=1)):
+        for out_dtype in (torch.float16, torch.float32):
+            out, lse = backend.run_paged(q, batch, 0.125, out_dtype=out_dtype, **hints)
+            check_attention(out, lse, want, d, max(lengths), out_dtype, out_dtype == torch.float32)
+
+
+def test_queries_of_any_alignment_and_stride(cuda_device):
+    rng = np.random.default_rng(50)
+    lengths = [100, 33]
+    pool = make_pool(rng, 12, 16, 2, 64, 32, 4)
+    table = make_table(rng, lengths, 16, 7, 12)
+    batch = paged(cuda_device, pool, table, lengths, 4, 32)
+    backend = HipAttentionBackend()
+    flat = torch.from_numpy(rng.standard_normal(2 * 8 * 64 + 8)).half().to(cuda_device)
+    for shift in (1, 3, 4):  # 2, 6 and 8 bytes past a 16-byte border
+        q = flat[shift:shift + 2 * 8 * 64].view(2, 8, 64)
+        run = backend.prepare_paged(q, batch, 0.1)
+        for a, b in zip(run(q), backend.run_paged(q.clone(), batch, 0.1)):
+            assert torch.equal(a, b)
+    strided = flat[:2 * 8 * 64].view(8, 2, 64).transpose(0, 1)
+    broadcast = flat[:64].view(1, 1, 64).expand(2, 8, 64)
+    for q in (strided, broadcast):
+        for a, b in zip(backend.run_paged(q, batch, 0.1), backend.run_paged(q.contiguous(), batch, 0.1)):
+            assert torch.equal(a, b)
+
+
+def test_sequences_may_share_pages(cuda_device):
+    rng = np.random.default_rng(51)
+    pool = make_pool(rng, 12, 32, 2, 64, 32, 4)
+    table = np.array([[3, 5, 7, -1], [3, 5, 8, 9], [3, 3, 3, 3]])
+    lengths = [70, 128, 100]
+    batch = paged(cuda_device, pool, table, lengths, 4, 32, np.zeros((3, 128), np.float32))
+    q = torch.from_numpy(rng.standard_normal((3, 4, 64))).half().to(cuda_device)
+    want = attend(as_double(q), pool, table, lengths, 4, 0.125)
+    out, lse = HipAttentionBackend().run_paged(q, batch, 0.125, accumulate=True)
+    check_attention(out, lse, want, 64, 128, torch.float32, True)
+    # a slot's weights are the sequence's own, shared page or not
+    sums = batch.weights.double().sum(1).cpu().numpy()
+    assert np.abs(sums - 4).max() < 4 * 2.0 ** -12 and (batch.weights[0, 70:] == 0).all()
+
+
+def test_two_threads_on_one_prepared_decode(cuda_device):
+    rng = np.random.default_rng(52)
+    lengths = [3000, 100]
+    pool = make_pool(rng, 50, 64, 2, 128, 32, 4)
+    table = make_table(rng, lengths, 64, 48, 50)
+    batch = paged(cuda_device, pool, table, lengths, 4, 32)
+    queries = torch.from_numpy(rng.standard_normal((2, 2, 8, 128))).half().to(cuda_device)
+    run = HipAttentionBackend().prepare_paged(queries[0], batch, 0.1)
+    want = [run(q) for q in queries]
+    got: list[list] = [[], []]
+
+    def work(i):
+        torch.cuda.set_device(cuda_device)
+        stream = torch.cuda.Stream(cuda_device)
+        stream.wait_stream(torch.cuda.default_stream(cuda_device))
+        with torch.cuda.stream(stream):
+            for _ in range(100):
+                got[i].append(run(queries[i]))
+        stream.synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    for i in range(2):
+        assert len(got[i]) == 100
+        for out, lse in got[i]:
+            assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+
+
+@pytest.mark.parametrize(("dtype", "bits", "layout", "kvh", "d", "counts"), [
+    (torch.bfloat16, 4, "half", 8, 128, [5000, 1, 3999]),      # eight tokens a workgroup
+    (torch.float16, 4, "interleaved", 8, 128, [9000]),
+    (torch.bfloat16, 2, "half", 3, 96, [4100, 0, 4101]),
+    (torch.float16, 2, "half", 16, 128, [2100, 200]),           # two, more words than threads
+    (torch.float32, 4, "half", 1, 32, [8192 + 5]),
+    (torch.float32, 2, "interleaved", 4, 64, [3000, 3000]),
+    (torch.bfloat16, 4, "half", 5, 256, [6000]),
+])
+def test_appended_codes_are_the_rotated_keys_over_millions_of_values(cuda_device, dtype, bits, layout, kvh, d, counts):
+    """A value rounded once to 16 bits, rather than to 32 and then to 16, differs in 2^-17 of the cases: too few for a
+    small test."""
+    total, bt = sum(counts), 128
+    width = max(-(-n // bt) for n in counts)
+    gen = torch.Generator(cuda_device).manual_seed(7)
+    shape = (len(counts) * width, bt, kvh)
+    rotary = Rotary(d, layout=layout, device=cuda_device)
+    k, v = (torch.randn((total, kvh, d), generator=gen, device=cuda_device).to(dtype) for _ in range(2))
+    q = torch.randn((total, 2, d), generator=gen, device=cuda_device).to(dtype)
+    offsets = torch.tensor([0, *np.cumsum(counts)], dtype=torch.int32, device=cuda_device)
+    first = torch.arange(len(counts), dtype=torch.int32, device=cuda_device) * 1000
+    batches = []
+    for _ in range(2):
+        codes = [torch.zeros((*shape, d * bits // 8), dtype=torch.uint8, device=cuda_device) for _ in "kv"]
+        scales = [torch.zeros((*shape, d // 32), dtype=torch.float16, device=cuda_device) for _ in "kv"]
+        table = torch.arange(len(counts) * width, dtype=torch.int32, device=cuda_device).view(len(counts), width)
+        batches.append(PagedBatch(*codes, *scales, table, torch.zeros_like(first), bits, 32))
+    turned, lengths = append_tokens(batches[0], k, v, offsets=offsets, rotary=rotary, query=q, first_positions=first)
+    position = torch.cat([torch.arange(n, device=cuda_device) + 1000 * i for i, n in enumerate(counts)])
+    tq, tk = rotary(position, q, k)
+    append_tokens(batches[1], tk, v, offsets=offsets)
+    assert lengths.tolist() == counts and torch.equal(turned, tq)
+    for name in ("packed_k", "packed_v", "scales_k", "scales_v"):
+        a, b = (getattr(x, name).view(torch.uint8) for x in batches)
+        assert torch.equal(a, b), (name, int((a != b).sum()))
+    # the rotation itself: 64 bits, rounded to 32 and then to the type (torch's conversions)
+    angle = position.double()[:, None, None] * rotary.frequencies
+    c, s, x = torch.cos(angle), torch.sin(angle), k.double()
+    a, b = (x[..., : d // 2], x[..., d // 2:]) if layout == "half" else (x[..., 0::2], x[..., 1::2])
+    lo, hi = a * c - b * s, b * c + a * s
+    want = torch.cat((lo, hi), -1) if layout == "half" else torch.stack((lo, hi), -1).flatten(-2)
+    # sines off by a few 2^-53 and a product fused or not: the 32-bit rounding hides all but a border's two sides
+    far = (tk.double() - want).abs() - want.abs() * torch.finfo(dtype).eps / 2 - (a.abs() + b.abs()).amax() * 2.0 ** -24
+    assert far.max() <= torch.finfo(dtype).smallest_normal
+
+
+def test_a_pool_past_4_gib(cuda_device):
+    """Pages at both ends of a pool whose code arrays pass 2^32 bytes; the same pages of a small pool beside them."""
+    pages, bt, kvh, d = 66000, 128, 8, 128
+    if torch.cuda.mem_get_info(cuda_device)[0] < 24 << 30:
+        pytest.skip("needs 24 GiB of GPU memory")
+    ends = [pages - 1, 0, pages - 2, 65537, pages - 3, 1]
+    assert (pages - 3) * bt * kvh * d // 2 > 1 << 32
+    big = PagedBatch(
+        *(torch.empty((pages, bt, kvh, d // 2), dtype=torch.uint8, device=cuda_device) for _ in "kv"),
+        *(torch.empty((pages, bt, kvh, d // 32), dtype=torch.float16, device=cuda_device) for _ in "kv"),
+        torch.tensor([ends[:3], ends[3:]], dtype=torch.int32, device=cuda_device),
+        torch.zeros(2, dtype=torch.int32, device=cuda_device), 4, 32,
+        torch.zeros((2, 3 * bt), device=cuda_device), torch.full((2, 3 * bt), -1, dtype=torch.int32, device=cuda_device),
+    )
+    small = PagedBatch(
+        *(torch.empty((6, *t.shape[1:]), dtype=t.dtype, device=cuda_device)
+          for t in (big.packed_k, big.packed_v, big.scales_k, big.scales_v)),
+        torch.arange(6, dtype=torch.int32, device=cuda_device).view(2, 3), big.lengths.clone(), 4, 32,
+        big.weights.clone(), big.positions.clone(),
+    )
+    gen = torch.Generator(cuda_device).manual_seed(3)
+    counts = [380, 300]
+    k, v = (torch.randn((680, kvh, d), generator=gen, device=cuda_device).bfloat16() for _ in range(2))
+    q = torch.randn((2, 32, d), generator=gen, device=cuda_device).bfloat16()
+    offsets = torch.tensor([0, 380, 680], dtype=torch.int32, device=cuda_device)
+    rotary, backend = Rotary(d, device=cuda_device), HipAttentionBackend()
+    results = []
+    for batch in (big, small):
+        _, lengths = append_tokens(batch, k, v, offsets=offsets, rotary=rotary)
+        batch.lengths.copy_(lengths)
+        first = backend.run_paged(q, batch, 0.1, accumulate=True)
+        lengths, weights, positions = evict_tokens(batch, 200, sink=2, recent=50)
+        batch.lengths.copy_(lengths)
+        second = backend.run_paged(q, batch, 0.1)
+        ids = batch.page_table.flatten().long()
+        results.append([*first, *second, lengths, weights, positions,
+                        *(t[ids] for t in (batch.packed_k, batch.packed_v, batch.scales_k, batch.scales_v))])
+    assert results[0][4].tolist() == [min(n, 200) for n in counts]
+    for i, (a, b) in enumerate(zip(*results)):
+        if i < 7:
+            assert torch.equal(a, b), i
+        else:  # slots past the appended ones hold whatever the memory held
+            n = [torch.arange(3 * bt) < c for c in counts]
+            used = torch.stack(n).view(6, bt).to(cuda_device)
+            assert torch.equal(a[used].view(torch.uint8), b[used].view(torch.uint8)), i
+
+
+def test_operators_run_on_another_stream(cuda_device):
+    rng = np.random.default_rng(53)
+    pool = make_pool(rng, 10, 32, 2, 64, 32, 4)
+    table = make_table(rng, [160, 160], 32, 5, 10)
+    slots = (2, 160)
+    pos = np.tile(np.arange(160, dtype=np.int32), (2, 1))
+    w = rng.uniform(0, 1, slots).astype(np.float32)
+    a, b = (paged(cuda_device, pool, table, [150, 60], 4, 32, w, pos) for _ in "ab")
+    k, v, q = (torch.from_numpy(rng.standard_normal((2, h, 64))).half().to(cuda_device) for h in (2, 2, 4))
+    rotary = Rotary(64, device=cuda_device)
+    results = []
+    side = torch.cuda.Stream(cuda_device)
+    torch.cuda.synchronize()
+    for batch, stream in ((a, torch.cuda.current_stream(cuda_device)), (b, side)):
+        with torch.cuda.stream(stream):
+            turned, lengths = append_tokens(batch, k, v, rotary=rotary, query=q)
+            batch.lengths.copy_(lengths)
+            out, lse = HipAttentionBackend().run_paged(turned, batch, 0.125, accumulate=True)
+            cut = evict_tokens(batch, 50, recent=8)
+            results.append([turned, lengths, out, lse, *cut, batch.packed_k, batch.scales_v, batch.weights])
+    torch.cuda.synchronize()
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
