@@ -86,16 +86,15 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
 
 // A slot's weight: 2^(score - the head's sum) over its heads.  A workgroup takes 4 kWave slots; its waves take a
 // quarter of the heads each, kDeep rows of scores on the way at a time, and are joined in LDS in a fixed order.
-__global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodeParams p) {
+__global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodeParams p, int blocks) {
   constexpr int kDeep = 8, kWaves = kThreads / kWave;
   __shared__ f32x4 sums[kWaves][kWave];
-  const int seq = blockIdx.y;
+  const int seq = blockIdx.x / blocks, nth = blockIdx.x % blocks;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int length = paged_length(p.c.lengths, seq, p.capacity);
   const float* lse = p.lse + static_cast<int64_t>(seq) * p.query_heads;
   const float* scores = p.scores + static_cast<int64_t>(seq) * p.query_heads * p.score_stride;
-  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * 4 * kWave; t0 < length;
-       t0 += static_cast<int64_t>(gridDim.x) * 4 * kWave) {
+  for (int64_t t0 = static_cast<int64_t>(nth) * 4 * kWave; t0 < length; t0 += static_cast<int64_t>(blocks) * 4 * kWave) {
     const int64_t t = t0 + 4 * lane;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     if (t < length) {  // (rows are of whole 64 slots)
@@ -239,9 +238,12 @@ int launch_paged_decode(const kvssd_paged_cache& c, const kvssd_paged_decode_arg
     if (int rc = launch_paged_merge(p, stream)) return rc;
   if (a.accumulate) {
     const int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
-    const int64_t blocks = (longest + 4 * kWave - 1) / (4 * kWave);
-    hipLaunchKernelGGL(paged_weights_kernel, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), c.sequences),
-                       dim3(kThreads), 0, stream, p);
+    // of a sequence; together fewer than 2^32 threads (a grid's second dimension would end at 65535 sequences)
+    const int64_t most = ((int64_t{1} << 24) - 1) / c.sequences;
+    int64_t blocks = (longest + 4 * kWave - 1) / (4 * kWave);
+    blocks = blocks < most ? blocks : most;
+    hipLaunchKernelGGL(paged_weights_kernel, dim3(static_cast<unsigned>(blocks * c.sequences)), dim3(kThreads), 0, stream,
+                       p, static_cast<int>(blocks));
     return hip_status(hipGetLastError(), "paged_weights launch");
   }
   return 0;

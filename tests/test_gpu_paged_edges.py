@@ -12,7 +12,7 @@ import torch
 from kvssd import Rotary, append_tokens, evict_tokens
 from kvssd.backends import PagedBatch
 from kvssd.backends.hip import HipAttentionBackend
-from paged_oracle import as_double, attend, make_pool, make_table
+from paged_oracle import as_double, attend, evict, make_pool, make_table
 from test_gpu_paged import check_attention, paged
 
 pytestmark = pytest.mark.gpu
@@ -45,6 +45,38 @@ def test_attention_over_many_sequences(cuda_device, case):
         for out_dtype in (torch.float16, torch.float32):
             out, lse = backend.run_paged(q, batch, 0.125, out_dtype=out_dtype, **hints)
             check_attention(out, lse, want, d, max(lengths), out_dtype, out_dtype == torch.float32)
+
+
+def test_seventy_thousand_sequences(cuda_device):
+    """More than a grid's second dimension holds, for the summed weights and for eviction's moves."""
+    n, bt, width = 70_000, 16, 40
+    rng = np.random.default_rng(54)
+    pool = make_pool(rng, 43, bt, 1, 32, 32, 2)
+    table = rng.integers(0, 3, (n, width)).astype(np.int32)  # (attention may share pages)
+    table[-1] = 3 + np.arange(width)
+    lengths = [i % 4 for i in range(n - 1)] + [width * bt]
+    slots = (n, width * bt)
+    pos = np.tile(np.arange(slots[1], dtype=np.int32), (n, 1))
+    batch = paged(cuda_device, pool, table, lengths, 2, 32, np.zeros(slots, np.float32), pos)
+    q = torch.from_numpy(rng.standard_normal((n, 1, 32))).half().to(cuda_device)
+    out, lse = HipAttentionBackend().run_paged(q, batch, 0.125, accumulate=True)
+    some = [0, 1, 2, 3, 65533, 65534, 65535, 65536, 65537, 65538, 65539, n - 2, n - 1]
+    want = attend(as_double(q[some]), pool, table[some], [lengths[i] for i in some], 2, 0.125, np.zeros((len(some), slots[1])))
+    check_attention(out[some], lse[some], want, 32, width * bt, torch.float32, True)
+    got = as_double(batch.weights[some])
+    assert np.abs(got - want["weights"]).max() < 2.0 ** -18  # (scores below 16: each off by less than 2^-19)
+    sums = batch.weights.double().sum(1).cpu().numpy()
+    assert np.abs(sums - (np.array(lengths) > 0)).max() < 2.0 ** -14
+    # a budget whose moves take a launch of their own; all but the last sequence are shorter
+    w = batch.weights.clone()
+    new_lengths, new_w, new_p = evict_tokens(batch, 300, recent=10)
+    assert torch.equal(new_lengths, batch.lengths.clamp(max=300))
+    source = evict(w[-1].cpu().numpy(), pos[-1], width * bt, 300, 0, 10)
+    assert new_p[-1, :300].tolist() == source and torch.equal(new_w[-1, :300], w[-1][source])
+    assert torch.equal(new_w[:-1, :4], w[:-1, :4])
+    old = torch.from_numpy(pool[0][3:].reshape(-1, 8))
+    assert torch.equal(batch.packed_k[3:].cpu().view(-1, 8)[:300], old[source])
+    assert torch.equal(batch.packed_k[:3].cpu(), torch.from_numpy(pool[0][:3]))
 
 
 def test_queries_of_any_alignment_and_stride(cuda_device):
