@@ -214,6 +214,7 @@ class PagedKVCache:
         self._pages: list[list[int]] = [[] for _ in range(sequences)]
         self.lengths = [0] * sequences  # slots in use, per sequence
         self.next_positions = [0] * sequences  # position of the next token, per sequence
+        self._plan: tuple | None = None  # of `attend`: what it was planned for, and the prepared decode
 
     @property
     def free_pages(self) -> int:
@@ -228,7 +229,10 @@ class PagedKVCache:
     def _resize(self, lengths: Sequence[int]) -> None:
         """Take or give back pages so that sequence b holds lengths[b] slots; nothing changes where the pool or a
         row of the page table is too small."""
-        want = [-(-n // self.page_tokens) for n in lengths]
+        room = self.page_tokens
+        if not any(n > len(have) * room or n <= (len(have) - 1) * room for n, have in zip(lengths, self._pages)):
+            return
+        want = [-(-n // room) for n in lengths]
         if max(want) > self.max_pages:
             raise ValueError(f"a sequence may hold at most {self.max_pages * self.page_tokens} tokens")
         back = sum(max(0, len(have) - n) for have, n in zip(self._pages, want))
@@ -262,14 +266,15 @@ class PagedKVCache:
     ) -> torch.Tensor | None:
         """Append counts[b] tokens to sequence b (default: one to each), as they lie in ``keys`` and ``values``
         [tokens, kv_heads, head_dim], sequence after sequence; returns the rotated query, if one was given."""
-        counts = [1] * self.sequences if counts is None else [int(n) for n in counts]
+        one = counts is None
+        counts = [1] * self.sequences if one else [int(n) for n in counts]
         if len(counts) != self.sequences or min(counts) < 0:
             raise ValueError("counts must hold one non-negative number per sequence")
         if keys.ndim != 3 or sum(counts) != keys.shape[0]:
             raise ValueError("counts must add up to the number of tokens")
         after = [n + more for n, more in zip(self.lengths, counts)]
         offsets = None
-        if any(n != 1 for n in counts):
+        if not one and any(n != 1 for n in counts):
             ends = [0]
             for n in counts:
                 ends.append(ends[-1] + n)
@@ -281,12 +286,14 @@ class PagedKVCache:
         self._resize(after)
         try:
             turned, lengths = append_tokens(
-                self.batch, keys, values, offsets=offsets, rotary=rotary, query=query, first_positions=first
+                self.batch, keys, values, offsets=offsets, rotary=rotary, query=query, first_positions=first,
+                lengths_out=self.batch.lengths if offsets is None else None,
             )
         except Exception:
             self._resize(held)
             raise
-        self.batch.lengths.copy_(lengths)
+        if offsets is not None:
+            self.batch.lengths.copy_(lengths)
         self.lengths = after
         self.next_positions = [n + more for n, more in zip(self.next_positions, counts)]
         return turned
@@ -302,16 +309,28 @@ class PagedKVCache:
         """(out, lse) of one query per sequence, [sequences, query_heads, head_dim]; see
         ``HipAttentionBackend.run_paged``.  The scale defaults to 1/sqrt(head_dim)."""
         scale = self.batch.head_dim ** -0.5 if sm_scale is None else sm_scale
-        hints = {}
-        if getattr(self.backend, "name", None) == "hip":
-            hints = dict(max_length=max(self.lengths), total_tokens=sum(self.lengths))
-        return self.backend.run_paged(query, self.batch, scale, out_dtype=out_dtype, accumulate=accumulate, **hints)
+        if getattr(self.backend, "name", None) != "hip":
+            return self.backend.run_paged(query, self.batch, scale, out_dtype=out_dtype, accumulate=accumulate)
+        # Checked and planned anew where the shape changes or the lengths have grown or shrunk by an eighth: between,
+        # the plan's hints are an eighth high at most, and the kernel goes by the lengths that there are.
+        shape = (query.shape, query.dtype, query.device, scale, out_dtype, accumulate)
+        longest, total = max(self.lengths), sum(self.lengths)
+        plan = self._plan
+        if plan is None or plan[0] != shape or not (plan[1] <= longest <= plan[2] and plan[3] <= total <= plan[4]):
+            hints = [n + n // 8 + 1 for n in (longest, total)]
+            run = self.backend.prepare_paged(
+                query, self.batch, scale, out_dtype=out_dtype, accumulate=accumulate, max_length=hints[0],
+                total_tokens=hints[1],
+            )
+            plan = self._plan = (shape, longest - longest // 8, hints[0], total - total // 8, hints[1], run)
+        return plan[5](query)
 
     def evict(self, budget: int, *, sink: int = 0, recent: int = 0) -> None:
         """Cut every sequence to at most ``budget`` tokens (:func:`evict_tokens`) and give back the pages behind."""
         lengths, weights, positions = evict_tokens(self.batch, budget, sink=sink, recent=recent)
         self.batch.lengths.copy_(lengths)
         self.batch = dataclasses.replace(self.batch, weights=weights, positions=positions)
+        self._plan = None  # (it holds the arrays that these take the place of)
         self.lengths = [min(n, budget) for n in self.lengths]
         self._resize(self.lengths)
 

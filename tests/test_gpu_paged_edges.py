@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from kvssd import Rotary, append_tokens, evict_tokens
+from kvssd import PagedKVCache, Rotary, append_tokens, evict_tokens
 from kvssd.backends import PagedBatch
 from kvssd.backends.hip import HipAttentionBackend
 from paged_oracle import as_double, attend, evict, make_pool, make_table
@@ -262,3 +262,41 @@ def test_operators_run_on_another_stream(cuda_device):
     torch.cuda.synchronize()
     for x, y in zip(*results):
         assert torch.equal(x, y)
+
+
+def test_a_cache_plans_anew_as_its_lengths_change(cuda_device):
+    rng = np.random.default_rng(55)
+    make = lambda h, n=2: torch.from_numpy(rng.standard_normal((n, h, 64))).half().to(cuda_device)  # noqa: E731
+    cache = PagedKVCache(60, 16, 2, 64, sequences=2, max_pages=30, track_weights=True, device=cuda_device)
+    backend = HipAttentionBackend()
+    plans = set()
+
+    def attend_and_check(query, **options):
+        out, lse = cache.attend(query, **options)
+        plans.add(id(cache._plan[5]))
+        keep.append(cache._plan)
+        want, want_lse = backend.run_paged(query, cache.batch, 64 ** -0.5, out_dtype=options.get("out_dtype"))
+        # a plan of other runs sums in another order: 32-bit grade, as elsewhere; 16-bit results by their rounding too
+        tol = dict(atol=2e-5, rtol=2e-5) if out.dtype == torch.float32 else dict(atol=2e-3, rtol=2.0 ** -10)
+        torch.testing.assert_close(out, want, **tol)
+        torch.testing.assert_close(lse, want_lse, atol=2e-5, rtol=2e-5)
+
+    keep: list = []
+    query = make(8)
+    attend_and_check(query)  # empty
+    cache.append(make(2, 40), make(2, 40), [37, 3])
+    for _ in range(150):
+        cache.append(make(2), make(2))
+        attend_and_check(query, accumulate=True)
+    assert 3 < len(plans) < 40
+    cache.evict(100, sink=2, recent=8)
+    assert cache.lengths == [100, 100] and cache.batch.lengths.tolist() == [100, 100]
+    attend_and_check(query, accumulate=True)
+    sums = cache.batch.weights.double().sum(1)
+    attend_and_check(query, accumulate=True)  # into the weights of the cut cache
+    assert ((cache.batch.weights.double().sum(1) - sums - 8).abs() < 1e-3).all()
+    cache.clear(0)
+    attend_and_check(query[:, :2].contiguous())
+    attend_and_check(query, out_dtype=torch.float16)
+    with pytest.raises(ValueError, match="query must be"):
+        cache.attend(query[:1])
