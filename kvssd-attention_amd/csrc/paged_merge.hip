@@ -21,9 +21,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kFewRows = 1024;
 
-// LANES: lanes of a run, 4 dims each; kThreads / LANES runs side by side.  Many rows take all their dims in one
-// workgroup (64 sequences of 32 heads, 128 dims: 8.1 us, in two of 64 dims 10.6); few rows are spread over slices of
-// 64 (one sequence of 32 heads: 5.8 us, 6.7 in one).
+// LANES: lanes of a run, 4 dims each; kThreads / LANES runs side by side.  Bound by its round trips: lengths, then
+// sums and partials together, then the joined row.  Many rows take all their dims in one workgroup (64 sequences of 32
+// heads, 128 dims: 6.9 us; 2.4 more in two of 64 dims), few are spread over slices of 64 (one sequence of 32 heads:
+// 4.1 us; 0.9 more in one).
 template <int LANES>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams p) {
   __shared__ float w_s[kMaxSplits];
@@ -36,11 +37,24 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
   const int64_t row0 = static_cast<int64_t>(first_run) * p.query_heads + h;  // run r: row0 + r * query_heads
   const int d0 = 4 * (blockIdx.y * LANES + tid % LANES);
   const int d = p.c.head_dim;
-  float big = -INFINITY;
-  for (int r = tid; r < n; r += kThreads) {
-    const float* ml = p.part_ml + 2 * (row0 + static_cast<int64_t>(r) * p.query_heads);
-    w_s[r] = ml[1] != 0.0f ? ml[0] : -INFINITY;  // (a NaN sum keeps its run)
-    if (ml[1] != 0.0f) big = fmaxf(big, ml[0]);
+  // the thread's first partials set out together, the sums behind them waiting for none
+  constexpr int kAhead = 4, kSide = kThreads / LANES;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2* ml = reinterpret_cast<const f32x2*>(p.part_ml) + row0;
+  const float* o = p.part_o + row0 * d + d0;
+  const int64_t step = static_cast<int64_t>(p.query_heads) * d;
+  f32x2 own = {-INFINITY, 0.0f};
+  if (tid < n) own = ml[static_cast<int64_t>(tid) * p.query_heads];
+  f32x4 ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int r = tid / LANES + i * kSide;
+    ahead[i] = r < n && d0 < d ? *reinterpret_cast<const f32x4*>(o + r * step) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  float big = own[1] != 0.0f ? own[0] : -INFINITY;  // (a NaN sum keeps its run)
+  for (int r = tid + kThreads; r < n; r += kThreads) {
+    const f32x2 x = ml[static_cast<int64_t>(r) * p.query_heads];
+    if (x[1] != 0.0f) big = fmaxf(big, x[0]);
   }
   big = wave_max(big);
   if (lane == 0) red[0][wave] = big;
@@ -48,24 +62,28 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
   big = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   float total = 0.0f;
   for (int r = tid; r < n; r += kThreads) {
-    const float l = p.part_ml[2 * (row0 + static_cast<int64_t>(r) * p.query_heads) + 1];
-    const float w = l != 0.0f ? exp2f(w_s[r] - big) : 0.0f;
+    const f32x2 x = r == tid ? own : ml[static_cast<int64_t>(r) * p.query_heads];
+    const float w = x[1] != 0.0f ? exp2f(x[0] - big) : 0.0f;
     w_s[r] = w;
-    total += w * l;
+    total += w * x[1];
   }
   total = wave_sum(total);
   if (lane == 0) red[1][wave] = total;
   __syncthreads();
   total = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int r = tid / LANES + i * kSide;
+    const float w = r < n ? w_s[r] : 0.0f;
+    if (w != 0.0f) acc += w * ahead[i];  // (NaN weights take part)
+  }
   if (d0 < d) {
-    const float* o = p.part_o + row0 * d + d0;
-    const int64_t step = static_cast<int64_t>(p.query_heads) * d;
 #pragma unroll 4
-    for (int r = tid / LANES; r < n; r += kThreads / LANES) {
+    for (int r = tid / LANES + kAhead * kSide; r < n; r += kSide) {
       const float w = w_s[r];
       const f32x4 v = *reinterpret_cast<const f32x4*>(o + r * step);
-      if (w != 0.0f) acc += w * v;  // (NaN weights take part)
+      if (w != 0.0f) acc += w * v;
     }
   }
 #pragma unroll
