@@ -1,13 +1,23 @@
 // New tokens into a paged packed cache: keys rotated, keys and values
 // quantised into their sequences' pages, queries rotated, in one launch.
 //
-// A workgroup takes one token (or a few of a prompt): where the token goes and
+// A workgroup takes one token (or up to 8 of a prompt): where the token goes and
 // its sines are formed once, then each thread takes words of codes (8 values
-// in INT4, 16 in INT2), those of a group side by side in the wave so that the
-// group's maximum is a few lane exchanges (quant_ops.hpp).  A key's word needs
+// in INT4, 16 in INT2) at one place of every token, so that its addresses are
+// formed once; those of a group lie side by side in the wave, and the group's
+// maximum is a few lane exchanges (quant_ops.hpp).  A key's word needs
 // the other half of its pairs: half layouts load it too (the lines are in the
 // cache, their neighbours' threads read them), so that no value passes between
-// threads between rotation and coding.  The rotated key is rounded to its type
+// threads between rotation and coding.
+//
+// Bound by its instructions on a prompt: 16,381 tokens of 8 kv heads of 128 in
+// bfloat16 into INT4 (86 MB in and out, 18 us at a copy's rate) take 31.5 us, of
+// which the vector units are busy 26 (a key's word ~200 instructions, 60 of them
+// 64-bit; a value's ~100); four tokens a workgroup take 2 us more.  A word loaded ahead of
+// the one that is coded changed nothing but the registers (35.3 and 35.9 us).
+// 4,097 tokens of 4 kv and 16 query heads of 64 in 32 bits into INT2: 13.9 us.
+// One token of each of 64 sequences: 6.2 us, four dependent reads.
+//  The rotated key is rounded to its type
 // first: the codes are those of a key rotated by kvssd_hip_rotary and quantised
 // by kvssd_hip_quantize, bit for bit.
 #include "paged.hpp"

@@ -6,10 +6,20 @@
 // Bound by the read of codes and scales (144 bytes a token and kv head in INT4
 // at head_dim 128); the arithmetic below is arranged to take fewer VALU cycles
 // than those bytes take to arrive.
+// Measured (one MI355X, this kernel alone; 8 kv and 32 query heads of 128 unless
+// said): INT4, 4 sequences of 131,000 to 262,144 tokens (899 MB) 173 us, 5.2 TB/s of
+// a plain read's 7.0; 64 ragged sequences up to 16,384 tokens (126 MB) 32.6 us; one of
+// 4,096 9.1 us, three round trips and one stage; INT2, 16 sequences up to 16,384,
+// 64 query heads, with the scores of every slot stored, 42 us, bound by its
+// instructions (two head tiles unpack every code twice).
+// 524,288 random-paged tokens (604 MB) take 133 us, 89 with every page in L2 and
+// 122 with the copies alone: what is left is how the 64-byte rows of a head arrive.
+// Two kv heads a wave, with whole 128-byte lines, need more registers than there
+// are (300 bytes a lane spilled).
 //
 // Work split.  A wave owns one kv head, up to 16 / GP of its query heads (GP:
-// scale groups per head, rounded up to a power of two) and one run of a sequence's slots, 64 slots (a stage) at a time.  The waves of a
-// workgroup take neighbouring kv heads of the same run, whose rows lie side by
+// scale groups per head, rounded up to a power of two) and one run of a
+// sequence's slots, 64 slots (a stage) at a time.  The waves of a workgroup take neighbouring kv heads of the same run, whose rows lie side by
 // side in a page, so that whole cache lines are used.  Waves do not meet: each
 // leaves an unnormalised partial (O, m, l), which paged_merge.hip joins.
 //
@@ -37,7 +47,8 @@
 //   go through LDS to the lanes that form the weights.  One or two groups: rows =
 //   slots, columns = (head, group), whose lanes are the weights' lanes; with two,
 //   the lanes of a head form the same scores twice.  (For four groups that form
-//   took 570 instructions a stage, this one 470.)
+//   took 543 vector instructions a stage, this one 418: 524,288 slots in L2 111 and
+//   89 us.)
 // Softmax.  The running maximum is lazy: scores up to 2^6 above the reference are
 //   summed as they are (no wave-wide maximum per stage); where one exceeds that,
 //   all lanes take the new maximum and rescale.  The reference also holds the
@@ -267,7 +278,8 @@ __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirst
 
 // UNI: pages hold whole halves (32 slots) of a stage, rows whole 16-byte chunks
 // and a head's scales begin in a word alike in every row, so that a copy's rows
-// have one uniform base; else every lane finds its own row's address.
+// have one uniform base; else every lane finds its own row's address (64 ragged
+// sequences 33.4 and 37.3 us, 899 MB 176 and 188).
 template <int BITS, int DP, int GP, bool PREC, bool UNI>
 __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(PagedDecodeParams p) {
   constexpr int kWaves = decode_waves(DP);

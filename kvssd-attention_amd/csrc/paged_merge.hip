@@ -11,6 +11,8 @@
 // Weights: slot t of sequence b gains sum over heads of 2^(s_bht - lse2_bh) from
 // the scores that the decode left (4 bytes a slot and head): a second pass
 // over the keys would read head_dim * bits / 8 + scales per kv head instead.
+// 16 sequences of 64 heads and up to 16,384 slots: 8.7 us (43 with a thread's heads
+// one after the other).
 #include "paged_decode.hpp"
 
 #include <string>
