@@ -330,7 +330,8 @@ typedef struct kvssd_paged_cache {
  * first_positions[b] + i (first_positions NULL: its slot).  Keys are rotated
  * (rotary not NULL) and rounded to their type, then keys and values are
  * quantised as by kvssd_hip_quantize.  Slots past the table's end are
- * dropped.  `query` (data NULL: none) is rotated by the same positions.
+ * dropped, and pages that are written may be named by one sequence only.
+ * `query` (data NULL: none) is rotated by the same positions.
  * Where the cache has them, the new slots' weights become 0 and their
  * positions are stored.  lengths_out[b] = lengths[b] + count, at most the
  * table's capacity; it may be the cache's own lengths where offsets is NULL. */
@@ -381,7 +382,8 @@ int kvssd_hip_paged_decode(const kvssd_paged_cache* cache, const kvssd_paged_dec
  * before it, so that only those rows are copied, in place.  lengths_out,
  * weights_out and positions_out (the cache's shapes, not its own arrays)
  * describe the result; slots past the new length get weight 0 and position
- * -1.  Needs the cache's weights and positions. */
+ * -1.  Needs the cache's weights and positions.  A page may be named by one
+ * sequence, and once, only. */
 typedef struct kvssd_paged_evict_args {
   int32_t budget, sink, recent, reserved;
   int32_t* lengths_out;

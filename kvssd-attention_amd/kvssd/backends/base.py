@@ -73,6 +73,9 @@ class PagedBatch:
       max_pages * page_tokens]``, each slot's summed attention weight and its
       token's position.
 
+    Several sequences may name the same page, to be attended; appending and
+    eviction write, and the pages they write have to be the sequence's own.
+
     No counterpart in the reference, whose batches are one sequence's blocks."""
 
     packed_k: torch.Tensor

@@ -60,7 +60,7 @@ def append_tokens(
     strides).  With ``offsets`` (int32 [sequences + 1]) tokens offsets[b] .. offsets[b+1]-1 belong to sequence b;
     without, there is one token a sequence.  A sequence's i-th new token goes to slot lengths[b] + i (dropped past
     the page table's end or where the table names no page) and has position first_positions[b] + i (int32
-    [sequences]; default: its slot).  With ``rotary`` the keys are turned by their positions and rounded to their
+    [sequences]; default: its slot).  The pages of those slots must be no other sequence's.  With ``rotary`` the keys are turned by their positions and rounded to their
     type before they are quantised, and so is ``query`` [tokens, query_heads, head_dim], if given.  Where the batch
     has them, the slots' positions are stored and their weights set to 0.
 
@@ -127,7 +127,8 @@ def evict_tokens(
     Kept are the slots whose position is below ``sink`` or among the last ``recent`` (above the sequence's largest
     position - recent), then those of the largest weights (NaN counts as -inf); of equals the lower slot, and
     ``budget`` in all.  The n-th kept slot at or past the budget moves into the n-th freed slot before it: only
-    those rows are copied, within the sequence's own pages.  The batch's own lengths, weights and positions stay as
+    those rows are copied, within the sequence's pages (which no other sequence, and no second place of the table,
+    may name).  The batch's own lengths, weights and positions stay as
     they are; the returned ones describe the cache after the cut (weight 0 and position -1 past the new length)."""
     batch.validate()
     index = _gpu_index(batch)
