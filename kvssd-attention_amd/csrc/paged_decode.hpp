@@ -109,17 +109,18 @@ struct RunMap {
   int tiles;  // stages of a run
   int seq;    // of run r; -1: there is no such run
   int nth;    // its place among the sequence's
+  int length;  // of the sequence (found with the run; in `runs_of`, not)
 };
 
-__device__ __forceinline__ int length_tiles(const PagedDecodeParams& p, int seq) {
-  return seq < p.c.sequences ? (paged_length(p.c.lengths, seq, p.capacity) + kTile - 1) / kTile : 0;
+__device__ __forceinline__ int length_of(const PagedDecodeParams& p, int seq) {
+  return seq < p.c.sequences ? paged_length(p.c.lengths, seq, p.capacity) : 0;
 }
-
-__device__ __forceinline__ int tiles_of_runs(const PagedDecodeParams& p) {
+// (`first`: the length of sequence `lane`, read once for all steps)
+__device__ __forceinline__ int tiles_of_runs(const PagedDecodeParams& p, int first) {
   const int lane = threadIdx.x % kWave;
-  int sum = 0, most = 0;
-  for (int s = lane; s - lane < p.c.sequences; s += kWave) {
-    const int n = length_tiles(p, s);
+  int sum = (first + kTile - 1) / kTile, most = sum;
+  for (int s = lane + kWave; s - lane < p.c.sequences; s += kWave) {
+    const int n = (length_of(p, s) + kTile - 1) / kTile;
     sum += n;
     most = max(most, n);
   }
@@ -131,20 +132,26 @@ __device__ __forceinline__ int tiles_of_runs(const PagedDecodeParams& p) {
 }
 
 __device__ __forceinline__ RunMap find_run(const PagedDecodeParams& p, int r) {
-  RunMap m{tiles_of_runs(p), -1, 0};
+  const int lane = threadIdx.x % kWave;
+  const int first = length_of(p, lane);
+  RunMap m{tiles_of_runs(p, first), -1, 0, 0};
   if (p.runs <= p.c.sequences) {
-    if (r < p.c.sequences) m.seq = r;
+    if (r < p.c.sequences) {
+      m.seq = r;
+      m.length = clamp_length(uniform_load(p.c.lengths + r), p.capacity);
+    }
     return m;
   }
-  const int lane = threadIdx.x % kWave;
   for (int s0 = 0; s0 < p.c.sequences; s0 += kWave) {
-    const int n = (length_tiles(p, s0 + lane) + m.tiles - 1) / m.tiles;
+    const int length = s0 == 0 ? first : length_of(p, s0 + lane);
+    const int n = ((length + kTile - 1) / kTile + m.tiles - 1) / m.tiles;
     const int upto = wave_prefix(n);
     const uint64_t past = __ballot(r < upto);
     if (past) {
       const int at = __builtin_ctzll(past);
       m.seq = s0 + at;
       m.nth = r - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
+      m.length = __builtin_amdgcn_readlane(length, at);
       return m;
     }
     r -= __builtin_amdgcn_readlane(upto, kWave - 1);
@@ -154,11 +161,13 @@ __device__ __forceinline__ RunMap find_run(const PagedDecodeParams& p, int r) {
 
 // first run of a sequence, and its number of runs
 __device__ __forceinline__ RunMap runs_of(const PagedDecodeParams& p, int seq, int* first, int* count) {
-  const RunMap m{tiles_of_runs(p), seq, 0};
   const int lane = threadIdx.x % kWave;
+  const int mine = length_of(p, lane);
+  const RunMap m{tiles_of_runs(p, mine), seq, 0, 0};
   int before = 0;
   for (int s0 = 0; s0 <= seq; s0 += kWave) {
-    const int n = (length_tiles(p, s0 + lane) + m.tiles - 1) / m.tiles;
+    const int length = s0 == 0 ? mine : length_of(p, s0 + lane);
+    const int n = ((length + kTile - 1) / kTile + m.tiles - 1) / m.tiles;
     const int upto = wave_prefix(n);
     if (seq < s0 + kWave) {
       *count = __builtin_amdgcn_readlane(n, seq - s0);
@@ -319,7 +328,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   const RunMap map = find_run(p, run);
   if (map.seq < 0) return;
   const int seq = scalar(map.seq);
-  const int length = clamp_length(uniform_load(c.lengths + seq), p.capacity);
+  const int length = scalar(map.length);
   const int begin = scalar(map.nth * map.tiles) * kTile;
   const int end = min(length, begin + scalar(map.tiles) * kTile);  // (at most 2^30 + 64 each)
 

@@ -149,7 +149,7 @@ class Rotary:
     ``rotary(positions, query, key)`` returns the turned query and key, each [tokens, heads, head_dim] in float16,
     bfloat16 or float32 with any token and head strides; ``positions`` is int32 or int64 [tokens].  Without a key it
     returns the query alone.  ``inverse`` turns back (the transpose, which is also the gradient's map);
-    ``inplace`` writes into the tensors given.  One launch on the current stream."""
+    ``inplace`` writes into the tensors given, which must share no element.  One launch on the current stream."""
 
     def __init__(
         self,
@@ -211,6 +211,8 @@ class Rotary:
             for t in tensors:
                 if t.stride(2) != 1 or _overlaps_itself(t):
                     raise ValueError("inplace needs values of a head side by side and no element twice")
+            if key is not None and key.data_ptr() == query.data_ptr() and key.numel() and query.numel():
+                raise ValueError("inplace needs a query and a key that share no element")
             outs = tensors
         else:
             tensors = tuple(t if t.stride(2) == 1 else t.contiguous() for t in tensors)

@@ -300,3 +300,18 @@ def test_a_cache_plans_anew_as_its_lengths_change(cuda_device):
     attend_and_check(query, out_dtype=torch.float16)
     with pytest.raises(ValueError, match="query must be"):
         cache.attend(query[:1])
+
+
+def test_inplace_rotation_of_one_tensor_twice_is_refused(cuda_device):
+    x = torch.randn((3, 4, 32), device=cuda_device)
+    positions = torch.arange(3, device=cuda_device)
+    rotary = Rotary(32, device=cuda_device)
+    before = x.clone()
+    with pytest.raises(ValueError, match="share no element"):
+        rotary(positions, x, x, inplace=True)
+    with pytest.raises(ValueError, match="share no element"):
+        rotary(positions, x, x[:, :1], inplace=True)
+    assert torch.equal(x, before)
+    both = rotary(positions, x, x)  # (into tensors of their own)
+    rotary(positions, x[:, :3], x[:, 3:], inplace=True)  # the slices of one tensor
+    assert torch.equal(x, both[0]) and torch.equal(both[0], both[1])
