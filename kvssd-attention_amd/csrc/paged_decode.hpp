@@ -7,15 +7,18 @@
 // at head_dim 128); the arithmetic below is arranged to take fewer VALU cycles
 // than those bytes take to arrive.
 // Measured (one MI355X, this kernel alone; 8 kv and 32 query heads of 128 unless
-// said): INT4, 4 sequences of 131,000 to 262,144 tokens (899 MB) 173 us, 5.2 TB/s of
+// said): INT4, 4 sequences of 131,000 to 262,144 tokens (899 MB) 148 us, 6.1 TB/s of
 // a plain read's 7.0; 64 ragged sequences up to 16,384 tokens (126 MB) 32.6 us; one of
 // 4,096 9.1 us, three round trips and one stage; INT2, 16 sequences up to 16,384,
 // 64 query heads, with the scores of every slot stored, 42 us, bound by its
 // instructions (two head tiles unpack every code twice).
-// 524,288 random-paged tokens (604 MB) take 133 us, 89 with every page in L2 and
-// 122 with the copies alone: what is left is how the 64-byte rows of a head arrive.
-// Two kv heads a wave, with whole 128-byte lines, need more registers than there
-// are (300 bytes a lane spilled).
+// 524,288 random-paged tokens (604 MB) take 116 us, 93 with every page in L2.  A
+// slot's codes of one head are half a line and its scales a sixteenth: waves that
+// drift apart fetch the same lines again from L2 (132 us; 105 without the scales).
+// Meeting before every second stage from the eighth on keeps them together (from
+// the first on 114 us, but 131,072 tokens then take 35.2 rather than 33.6).  Two kv
+// heads a wave, with whole lines, need more registers than there are (300 bytes a
+// lane spilled).
 //
 // Work split.  A wave owns one kv head, up to 16 / GP of its query heads (GP:
 // scale groups per head, rounded up to a power of two) and one run of a
@@ -288,7 +291,7 @@ __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirst
 // UNI: pages hold whole halves (32 slots) of a stage, rows whole 16-byte chunks
 // and a head's scales begin in a word alike in every row, so that a copy's rows
 // have one uniform base; else every lane finds its own row's address (64 ragged
-// sequences 33.4 and 37.3 us, 899 MB 176 and 188).
+// sequences 33.4 and 37.3 us).
 template <int BITS, int DP, int GP, bool PREC, bool UNI>
 __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(PagedDecodeParams p) {
   constexpr int kWaves = decode_waves(DP);
@@ -458,8 +461,8 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   };
   auto copy_stage = [&](const Stage& s, int buf) {
     copy_scales(sk, s, raw0 + buf * 2 * (kScaleCopies * 256));
-    copy_scales(sv, s, raw0 + (buf * 2 + 1) * (kScaleCopies * 256));
     copy_codes(pk, s, codes0 + buf * (2 * kArray));
+    copy_scales(sv, s, raw0 + (buf * 2 + 1) * (kScaleCopies * 256));
     copy_codes(pv, s, codes0 + buf * (2 * kArray) + kArray);
   };
 
@@ -733,6 +736,12 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     }
   };
 
+  // Waves of neighbouring kv heads, which share lines, meet before every second stage's copies, so that a line is still
+  // in L1 when its other readers come.  They begin in step: the first stages do without.  (All waves that are left have
+  // one run, and so as many meetings.)  Not in INT2 with several head tiles, which its instructions bind (16 sequences of
+  // 64 query heads: 42.5 us, 45 in step).
+  constexpr int kInStep = 8;
+  const bool in_step = p.group_units > 1 && p.group_runs == 1 && (BITS == 4 || p.tiles == 1);
   for (int i = 0, base = begin; i < stages; ++i, base += kTile) {
     // the stage has landed
     if (chunked && i + 1 < stages) __builtin_amdgcn_s_waitcnt(vmcnt_wait(kStageCopies));
@@ -795,6 +804,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     if (i + 2 < stages) {
       later = locate(base + 2 * kTile);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (in_step && i >= kInStep && buf == 0) __builtin_amdgcn_s_barrier();
       copy_stage(later, buf);
     }
     // ---- scores
