@@ -6,36 +6,37 @@
 // Bound by the read of codes and scales (144 bytes a token and kv head in INT4
 // at head_dim 128); the arithmetic below is arranged to take fewer VALU cycles
 // than those bytes take to arrive.
-// Measured (one MI355X, this kernel alone; 8 kv and 32 query heads of 128 unless
-// said): INT4, 4 sequences of 131,000 to 262,144 tokens (899 MB) 148 us, 6.1 TB/s of
-// a plain read's 7.0; 64 ragged sequences up to 16,384 tokens (126 MB) 32.6 us; one of
-// 4,096 9.1 us, three round trips and one stage; INT2, 16 sequences up to 16,384,
-// 64 query heads, with the scores of every slot stored, 42 us, bound by its
-// instructions (two head tiles unpack every code twice).
-// 524,288 random-paged tokens (604 MB) take 116 us, 93 with every page in L2.  A
-// slot's codes of one head are half a line and its scales a sixteenth: waves that
-// drift apart fetch the same lines again from L2 (132 us; 105 without the scales).
-// Meeting before every second stage from the eighth on keeps them together (from
-// the first on 114 us, but 131,072 tokens then take 35.2 rather than 33.6).  Two kv
-// heads a wave, with whole lines, need more registers than there are (300 bytes a
-// lane spilled).
+// Measured (one MI355X; 8 kv and 32 query heads of 128 unless said, with the join,
+// from memory): INT4, 4 sequences of 131,000 to 262,144 tokens (795 MB) 162 us,
+// 4.9 TB/s of a plain read's 7.0; 64 ragged sequences up to 16,384 tokens (126 MB)
+// 48 us; one of 4,096 tokens 12.2 us, round trips and one stage; INT2, 16 sequences up
+// to 16,384, 64 query heads, this kernel alone 42 us, bound by its instructions (two
+// head tiles unpack every code twice).
+// A slot's codes of one head are half a line and its scales a sixteenth: waves that
+// drift apart fetch the same lines again, some from memory (the 795 MB: 197 us, and
+// a third more fetched; 524,288 tokens 132 us, 105 without the scales).  They meet
+// before every stage's copies, which costs the arithmetic (524,288 tokens with every
+// page in L2: 89 us, 103 in step) less than it saves.  Meeting every second stage,
+// from the eighth on: 166 us, and 51.7 the 64 sequences.  Two kv heads a wave, with
+// whole lines, need more registers than there are (300 bytes a lane spilled).
 //
 // Work split.  A wave owns one kv head, up to 16 / GP of its query heads (GP:
 // scale groups per head, rounded up to a power of two) and one run of a
-// sequence's slots, 64 slots (a stage) at a time.  The waves of a workgroup take neighbouring kv heads of the same run, whose rows lie side by
-// side in a page, so that whole cache lines are used.  Waves do not meet: each
-// leaves an unnormalised partial (O, m, l), which paged_merge.hip joins.
+// sequence's slots, 64 slots (a stage) at a time.  The waves of a workgroup take
+// neighbouring kv heads of the same run, whose rows lie side by side in a page, so
+// that whole cache lines are used.  Waves pass each other nothing: each leaves an
+// unnormalised partial (O, m, l), which paged_merge.hip joins.
 //
 // Copies.  Codes, scales and the query go from memory straight to LDS (16 or 4
 // bytes a lane), into the wave's own two buffers and without a register or a
 // barrier.  A stage's codes and scales are taken into registers when it begins,
 // and the copies of two stages on go to their place at once: between one and two
 // stages are always on the way, each awaited by the count of later copies
-// (vmcnt).  With one stage on the way, all awaited at once, 524,288 slots took
-// 133 us; with the waves' copies joined into rows of all kv heads, a barrier a
-// stage, 142.  A row's 16-byte chunks are stored in an order turned by the row's
-// number, so that neither the key rows' nor the value columns' reads meet in a
-// bank.  Scales are laid out by group in LDS when their stage begins.
+// (vmcnt).  With the waves' copies joined into rows of all kv heads, awaited by all
+// at a barrier a stage, 524,288 slots took 142 us.  A row's 16-byte chunks are
+// stored in an order turned by the row's number, so that neither the key rows' nor
+// the value columns' reads meet in a bank.  Scales are laid out by group in LDS when
+// their stage begins.
 //
 // QK (v_mfma_f32_16x16x32_f16): one side is 16 slots' codes, the other (query
 //   head, group): the query masked to one group, so that a result is one group's
@@ -736,11 +737,9 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     }
   };
 
-  // Waves of neighbouring kv heads, which share lines, meet before every second stage's copies, so that a line is still
-  // in L1 when its other readers come.  They begin in step: the first stages do without.  (All waves that are left have
-  // one run, and so as many meetings.)  Not in INT2 with several head tiles, which its instructions bind (16 sequences of
-  // 64 query heads: 42.5 us, 45 in step).
-  constexpr int kInStep = 8;
+  // Waves of neighbouring kv heads, which share lines, meet before every stage's copies, so that a line is still in L1
+  // when its other readers come.  (All waves that are left have one run, and so as many meetings.)  Not in INT2 with
+  // several head tiles, which its instructions bind (16 sequences of 64 query heads: 42.5 us, 45 in step).
   const bool in_step = p.group_units > 1 && p.group_runs == 1 && (BITS == 4 || p.tiles == 1);
   for (int i = 0, base = begin; i < stages; ++i, base += kTile) {
     // the stage has landed
@@ -804,7 +803,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     if (i + 2 < stages) {
       later = locate(base + 2 * kTile);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (in_step && i >= kInStep && buf == 0) __builtin_amdgcn_s_barrier();
+      if (in_step) __builtin_amdgcn_s_barrier();
       copy_stage(later, buf);
     }
     // ---- scores
