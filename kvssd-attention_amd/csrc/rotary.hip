@@ -6,11 +6,11 @@
 // the next on its way while one is turned.
 //
 // Bound by memory: 8,187 tokens of 40 heads of 128 (168 MB in and out) take
-// 28.6 us where they lie in the last-level cache and 35.5 from HBM (4.7 TB/s,
+// 28.0 us where they lie in the last-level cache and 35.4 from HBM (4.7 TB/s,
 // a large copy's rate); with 32-bit products and sines the same.  4,099 tokens
-// of 28 heads of 256, a quarter of them turned (117 MB): 29.2 and 40.4 us.  All
+// of 28 heads of 256, a quarter of them turned (117 MB): 37 us from HBM.  All
 // heads' pairs before the values passed through, so that fewer waves form
-// products: 40.8, and 38.0 for the first shape.  One token's 64 sequences are
+// products: no faster there, and 38.0 for the first shape.  One token's 64 sequences are
 // the launch and three round trips: 5.2 us.
 #include "paged.hpp"
 #include "rotary_ops.hpp"
@@ -79,12 +79,16 @@ void launch_typed(RotaryParams& p, const kvssd_rotary_spec& r, hipStream_t strea
   bool vec = (r.rotary_dim / 2) % kVec == 0 && (r.head_dim - r.rotary_dim) % kVec == 0;
   for (int k = 0; k < p.count; ++k) vec = vec && heads_vector(p.t[k], sizeof(T), true);
   p.shape = rotary_shape(r, vec ? kVec : 1);
-  int per = kMaxTurns / p.shape.pairs;  // >= 1: at most 512 pairs
-  // long prompts: the sines of 4 tokens at a time give every thread one (8,187
-  // tokens of 64 pairs: 35.5 us, 40.2 a workgroup a token); short ones: a
-  // workgroup a token, so that more CUs take part
-  per = p.tokens >= 2048 ? (per < kMostTokens ? per : kMostTokens) : 1;
-  p.per_group = per;
+  // long prompts: as many tokens as give a thread about four items, whose sines
+  // then take few threads' time (8,187 tokens of 320 items: three a workgroup 35.4
+  // us, one 40.2; 4,099 of 784: one 37.0, four 40.4); short ones: a workgroup a
+  // token, so that more CUs take part
+  int64_t all = 0;
+  for (int k = 0; k < p.count; ++k) all += static_cast<int64_t>(p.t[k].heads) * p.shape.items;
+  int64_t per = p.tokens < 2048 ? 1 : all > 0 ? 4 * kThreads / all : kMostTokens;
+  per = per < 1 ? 1 : per > kMostTokens ? kMostTokens : per;
+  if (per > kMaxTurns / p.shape.pairs) per = kMaxTurns / p.shape.pairs;  // >= 1: at most 512 pairs
+  p.per_group = static_cast<int>(per);
   p.items = divisor(p.shape.items);
   for (int k = 0; k < p.count; ++k) p.per_token[k] = divisor(static_cast<int64_t>(p.t[k].heads) * p.shape.items);
   const dim3 grid(static_cast<unsigned>((p.tokens + per - 1) / per));
