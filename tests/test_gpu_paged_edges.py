@@ -315,3 +315,27 @@ def test_inplace_rotation_of_one_tensor_twice_is_refused(cuda_device):
     both = rotary(positions, x, x)  # (into tensors of their own)
     rotary(positions, x[:, :3], x[:, 3:], inplace=True)  # the slices of one tensor
     assert torch.equal(x, both[0]) and torch.equal(both[0], both[1])
+
+
+@pytest.mark.parametrize(("bits", "qh", "kvh", "d", "bt", "length"), [
+    (4, 9, 9, 64, 64, 60000),    # workgroups of five kv heads, the second with one too few
+    (2, 14, 7, 128, 32, 50000),  # seven waves, one workgroup over the heads
+    (4, 5, 5, 160, 24, 40000),   # three waves and two, slots' rows found lane by lane
+    (4, 24, 3, 128, 128, 90000),  # two head tiles a kv head
+])
+def test_long_runs_of_heads_that_fill_no_workgroup(cuda_device, bits, qh, kvh, d, bt, length):
+    rng = np.random.default_rng(56)
+    lengths = [length, 700]
+    width = -(-length // bt)
+    pages = width + -(-700 // bt)
+    pool = make_pool(rng, pages, bt, kvh, d, 32, bits)
+    table = make_table(rng, lengths, bt, width, pages)
+    batch = paged(cuda_device, pool, table, lengths, bits, 32)
+    q = torch.from_numpy(rng.standard_normal((2, qh, d))).bfloat16().to(cuda_device)
+    want = attend(as_double(q), pool, table, lengths, bits, d ** -0.5)
+    backend = HipAttentionBackend()
+    for out_dtype in (torch.bfloat16, torch.float32):
+        out, lse = backend.run_paged(q, batch, d ** -0.5, out_dtype=out_dtype)
+        check_attention(out, lse, want, d, length, out_dtype, out_dtype == torch.float32)
+        for a, b in zip((out, lse), backend.run_paged(q, batch, d ** -0.5, out_dtype=out_dtype)):
+            assert torch.equal(a, b)
