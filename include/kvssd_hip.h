@@ -303,8 +303,9 @@ int kvssd_hip_rotary(const kvssd_rotary_spec* spec, const void* positions, int p
 
 /* A paged packed cache.  Pool: packed_k/v uint8 [num_pages, page_tokens,
  * kv_heads, head_dim*bits/8] and scales fp16 [num_pages, page_tokens,
- * kv_heads, head_dim/group_size], C-contiguous, 16-byte aligned.  Slot s of
- * sequence b lies in page page_table[b][s / page_tokens], row
+ * kv_heads, head_dim/group_size], C-contiguous, 16-byte aligned (scales are
+ * read by words of 4 bytes: the last word of an odd number of scales whole).
+ * Slot s of sequence b lies in page page_table[b][s / page_tokens], row
  * s % page_tokens; sequence b holds slots 0 .. lengths[b]-1 (clamped to
  * [0, max_pages*page_tokens]).  Pages outside [0, num_pages) are skipped:
  * their slots are neither read nor written.  head_dim is a multiple of 32 up

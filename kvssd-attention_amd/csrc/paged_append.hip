@@ -266,8 +266,6 @@ int check_paged_cache(const kvssd_paged_cache* c) {
   if (paged_capacity(*c) > (int64_t{1} << 30)) return arg_error("a sequence may hold at most 2^30 slots");
   if (static_cast<int64_t>(c->num_pages) * c->page_tokens > (int64_t{1} << 30))
     return arg_error("a pool may hold at most 2^30 slots");
-  if (static_cast<int64_t>(c->num_pages) * c->page_tokens * c->kv_heads == 1 && (c->head_dim / c->group_size) % 2)
-    return arg_error("a pool of one row needs an even number of scale groups");  // (they are read 4 bytes at a time)
   if (!c->packed_k || !c->packed_v || !c->scales_k || !c->scales_v || !c->page_table || !c->lengths)
     return arg_error("a required buffer pointer is NULL");
   for (const void* ptr : {static_cast<const void*>(c->packed_k), static_cast<const void*>(c->packed_v),

@@ -384,13 +384,10 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       }
     }
   };
-  // Whether a slot's scales begin in a word's upper half, for an odd number of groups.  The very last ones of a pool
-  // with an odd number of scales would end in a word past it: they are taken from one scale earlier on.
-  const bool odd_pool = p.groups % 2 && c.num_pages % 2 && bt % 2 && c.kv_heads % 2;
-  const int last_row = odd_pool && kvh == c.kv_heads - 1 ? c.num_pages * bt - 1 : -1;
-  auto upper = [&](int row) {
-    return p.groups % 2 && (((static_cast<uint32_t>(row) * c.kv_heads + kvh) & 1u) || row == last_row);
-  };
+  // Whether a slot's scales begin in a word's upper half, for an odd number of groups: they are copied from the word's
+  // start, so that every address is a multiple of four (the arrays are).  The last scale of a pool that holds an odd
+  // number of them is copied with the two bytes behind the array, of the same aligned word; they are cut off below.
+  auto upper = [&](int row) { return p.groups % 2 && ((static_cast<uint32_t>(row) * c.kv_heads + kvh) & 1u); };
   // A stage to be copied: rows of the pool (of its halves; of the lane's slot where not UNI), slots that take part,
   // slots whose scales begin in a word's upper half
   struct Stage {

@@ -339,3 +339,34 @@ def test_long_runs_of_heads_that_fill_no_workgroup(cuda_device, bits, qh, kvh, d
         check_attention(out, lse, want, d, length, out_dtype, out_dtype == torch.float32)
         for a, b in zip((out, lse), backend.run_paged(q, batch, d ** -0.5, out_dtype=out_dtype)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize(("bits", "kvh", "d", "g", "bt", "pages"), [
+    (4, 1, 32, 32, 1, 1),    # one row, one scale
+    (4, 1, 64, 64, 7, 9),
+    (2, 3, 32, 32, 5, 11),
+    (4, 1, 96, 32, 1, 1),    # three groups
+    (4, 3, 96, 32, 7, 9),
+    (2, 1, 96, 32, 3, 25),
+    (4, 3, 160, 32, 5, 13),  # five
+    (2, 5, 224, 32, 9, 9),   # seven
+])
+def test_scales_that_end_an_odd_pool(cuda_device, bits, kvh, d, g, bt, pages):
+    """A pool with an odd number of scales, its last row in use: the last scale fills half a word, and what lies behind
+    the array (NaN here) has no part."""
+    rng = np.random.default_rng(57)
+    pool = list(make_pool(rng, pages, bt, kvh, d, g, bits))
+    for table, length in ((np.arange(pages)[None], pages * bt), (np.full((1, 1), pages - 1), bt)):  # all; the last page
+        lengths = [length]
+        batch = paged(cuda_device, pool, table, lengths, bits, g)
+        tails = []
+        for a in pool[2:]:
+            flat = torch.full((a.size + 8,), float("nan"), dtype=torch.float16, device=cuda_device)
+            flat[:a.size] = torch.from_numpy(a).flatten().to(cuda_device)
+            tails.append(flat[:a.size].view(a.shape))
+        batch = PagedBatch(batch.packed_k, batch.packed_v, *tails, batch.page_table, batch.lengths, bits, g)
+        q = torch.from_numpy(rng.standard_normal((1, 2 * kvh, d))).half().to(cuda_device)
+        want = attend(as_double(q), pool, table, lengths, bits, d ** -0.5)
+        for out_dtype in (torch.float16, torch.float32):
+            out, lse = HipAttentionBackend().run_paged(q, batch, d ** -0.5, out_dtype=out_dtype)
+            check_attention(out, lse, want, d, length, out_dtype, out_dtype == torch.float32)

@@ -336,3 +336,13 @@ def test_refused_caches(change, match):
 
 def test_rotary_and_cache_have_to_fit():
     assert Rotary(32, device="cpu").spec(True).inverse == 1 and Rotary(32, device="cpu").spec().inverse == 0
+
+
+def test_a_pool_of_one_row_is_taken_whatever_its_scales():
+    lib = _native.load()
+    for groups in (1, 2, 3):
+        cache = native(num_pages=1, page_tokens=1, kv_heads=1, max_pages=1, head_dim=32 * groups)
+        args, n = _native.PagedDecodeArgs(query_heads=1), ctypes.c_size_t(0)
+        _native.check(
+            lib.kvssd_hip_paged_decode_workspace_bytes(ctypes.byref(cache), ctypes.byref(args), ctypes.byref(n)), "decode"
+        )
