@@ -18,7 +18,6 @@ The functions launch on the current stream and never wait for the GPU.
 from __future__ import annotations
 
 import ctypes
-import dataclasses
 from collections.abc import Sequence
 
 import torch
@@ -327,11 +326,14 @@ class PagedKVCache:
         return plan[5](query)
 
     def evict(self, budget: int, *, sink: int = 0, recent: int = 0) -> None:
-        """Cut every sequence to at most ``budget`` tokens (:func:`evict_tokens`) and give back the pages behind."""
+        """Cut every sequence to at most ``budget`` tokens (:func:`evict_tokens`) and give back the pages behind.
+
+        ``batch`` keeps its arrays, so that decodes prepared before, and graphs of them, go on with the cut cache."""
+        longest = max(self.lengths)
         lengths, weights, positions = evict_tokens(self.batch, budget, sink=sink, recent=recent)
         self.batch.lengths.copy_(lengths)
-        self.batch = dataclasses.replace(self.batch, weights=weights, positions=positions)
-        self._plan = None  # (it holds the arrays that these take the place of)
+        self.batch.weights[:, :longest].copy_(weights[:, :longest])  # (none of the sequences has slots behind)
+        self.batch.positions[:, :longest].copy_(positions[:, :longest])
         self.lengths = [min(n, budget) for n in self.lengths]
         self._resize(self.lengths)
 

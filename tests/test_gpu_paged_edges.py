@@ -370,3 +370,34 @@ def test_scales_that_end_an_odd_pool(cuda_device, bits, kvh, d, g, bt, pages):
         for out_dtype in (torch.float16, torch.float32):
             out, lse = HipAttentionBackend().run_paged(q, batch, d ** -0.5, out_dtype=out_dtype)
             check_attention(out, lse, want, d, length, out_dtype, out_dtype == torch.float32)
+
+
+def test_decodes_prepared_before_a_cut_follow_the_cache(cuda_device):
+    """A prepared decode and a captured one go on after an eviction as a call made anew does, and add to the weights
+    that the next cut reads."""
+    rng = np.random.default_rng(58)
+    make = lambda n, h: torch.from_numpy(rng.standard_normal((n, h, 64))).half().to(cuda_device)  # noqa: E731
+    cache = PagedKVCache(24, 16, 2, 64, sequences=2, max_pages=12, track_weights=True, device=cuda_device)
+    backend, query = HipAttentionBackend(), make(2, 8)
+    run = backend.prepare_paged(query, cache.batch, 0.125, accumulate=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(query)
+    cache.append(make(250, 2), make(250, 2), [150, 100])
+    for r in range(3):
+        cache.attend(query, 0.125, accumulate=True)
+        cache.evict(80 - 20 * r, sink=2, recent=8)
+        assert cache.batch.lengths.tolist() == cache.lengths == [80 - 20 * r] * 2
+        want = backend.run_paged(query, cache.batch, 0.125)
+        sums = cache.batch.weights.double().sum(1)
+        for n in (1, 2):
+            if n == 1:
+                got = run(query)
+            else:
+                graph.replay()
+                got = captured
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+            # 8 heads' weights a call: each a sum of at most 80 numbers within 2^-17 of themselves
+            assert ((cache.batch.weights.double().sum(1) - sums - 8 * n).abs() < 16 * 2.0 ** -15).all()
+        cache.append(make(2, 2), make(2, 2))
+    del graph

@@ -346,3 +346,21 @@ def test_a_pool_of_one_row_is_taken_whatever_its_scales():
         _native.check(
             lib.kvssd_hip_paged_decode_workspace_bytes(ctypes.byref(cache), ctypes.byref(args), ctypes.byref(n)), "decode"
         )
+
+
+def test_a_cut_writes_into_the_arrays_that_there_are(monkeypatch):
+    cache = host_cache()
+    cache._resize([9, 2, 0])
+    cache.lengths = [9, 2, 0]
+    cache.batch.lengths.copy_(torch.tensor([9, 2, 0]))
+    before = cache.batch
+    arrays = {f.name: getattr(before, f.name) for f in dataclasses.fields(before)}
+    slots = before.weights.shape
+    cut = (torch.tensor([4, 2, 0], dtype=torch.int32), torch.arange(36.0).view(slots),
+           torch.arange(36, dtype=torch.int32).view(slots))
+    monkeypatch.setattr("kvssd.paged.evict_tokens", lambda *a, **k: cut)
+    cache.evict(4)
+    assert cache.batch is before and all(getattr(before, n) is a for n, a in arrays.items())
+    for got, want in zip((before.lengths, before.weights, before.positions), cut):
+        assert torch.equal(got[..., :9], want[..., :9])
+    assert cache.lengths == [4, 2, 0] and cache.free_pages == 4
