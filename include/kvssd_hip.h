@@ -288,7 +288,7 @@ typedef struct kvssd_rotary_spec {
  * in elements. */
 typedef struct kvssd_heads {
   const void* data;
-  void* out; /* where results go; may equal data with the same strides */
+  void* out; /* where results go; may equal data with the same strides, and shares no element with another tensor */
   int64_t token_stride, head_stride;
   int64_t out_token_stride, out_head_stride;
   int32_t heads;

@@ -120,6 +120,34 @@ def _overlaps_itself(t: torch.Tensor) -> bool:
     return False
 
 
+def _share_elements(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [tokens, heads, head_dim] tensors of one type, values of a head side by side and none of them there
+    twice, have an element in common."""
+    if not a.numel() or not b.numel():
+        return False
+    (n, h, d), (st, sh, _), (bn, bh, _), (bst, bsh, _) = a.shape, a.stride(), b.shape, b.stride()
+    size, first, second = a.itemsize, a.data_ptr(), b.data_ptr()
+    reach, b_reach = ((h - 1) * sh + d) * size, ((bh - 1) * bsh + d) * size  # bytes of a token, first value to last
+    if first + (n - 1) * st * size + reach <= second or second + (bn - 1) * bst * size + b_reach <= first:
+        return False
+    if st == bst > 0:  # slices of one projection: apart if their heads are, within a token's stride
+        ahead = (second - first) % (st * size)
+        if reach <= ahead <= st * size - b_reach:
+            return False
+    # the general case: no head of b may begin less than a head behind or before one of a
+    count = lambda m: torch.arange(m, device="cpu")  # noqa: E731
+    begins = [
+        (base + (count(t.shape[0])[:, None] * t.stride(0) + count(t.shape[1]) * t.stride(1)) * size).flatten()
+        for t, base in ((a, first), (b, second))
+    ]
+    begins[0] = begins[0].sort().values
+    at = torch.searchsorted(begins[0], begins[1])  # (begins[0][at - 1] < b <= begins[0][at])
+    last = begins[0].numel() - 1
+    behind = begins[1] - begins[0][(at - 1).clamp(min=0)] < d * size
+    before = begins[0][at.clamp(max=last)] - begins[1] < d * size
+    return bool(((at > 0) & behind).any() or ((at <= last) & before).any())
+
+
 def heads_of(t: torch.Tensor, out: torch.Tensor | None = None) -> tuple:
     """Fields of kvssd_heads of a [tokens, heads, head_dim] tensor (its values of a head side by side)."""
     token, head, _ = t.stride()
@@ -211,7 +239,7 @@ class Rotary:
             for t in tensors:
                 if t.stride(2) != 1 or _overlaps_itself(t):
                     raise ValueError("inplace needs values of a head side by side and no element twice")
-            if key is not None and key.data_ptr() == query.data_ptr() and key.numel() and query.numel():
+            if key is not None and _share_elements(query, key):
                 raise ValueError("inplace needs a query and a key that share no element")
             outs = tensors
         else:

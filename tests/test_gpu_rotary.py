@@ -174,3 +174,22 @@ def test_nothing_to_do_other_streams_and_captured(cuda_device):
         torch.cuda.synchronize()
         assert torch.equal(captured, eager), r
     del graph
+
+
+def test_inplace_rotation_of_overlapping_slices_is_refused(cuda_device):
+    rng = np.random.default_rng(12)
+    rot = Rotary(32, device=cuda_device)
+    pos = torch.arange(6, device=cuda_device)
+    x = torch.from_numpy(rng.standard_normal((6, 8, 32))).half().to(cuda_device)
+    before = x.clone()
+    for q, k in ((x[:, :5], x[:, 3:]), (x[:, 3:], x[:, :5]), (x[:, :3], x[:, 2:]), (x[:, ::2], x[:, 2:3])):
+        with pytest.raises(ValueError, match="share no element"):
+            rot(pos, q, k, inplace=True)
+    with pytest.raises(ValueError, match="share no element"):
+        rot(pos[:4], x[:4], x[2:], inplace=True)
+    assert torch.equal(x, before)
+    want = rot(pos, x)
+    for q, k in ((x[:, :5], x[:, 5:]), (x[:, 1::2], x[:, ::2])):  # slices that lie among each other
+        x.copy_(before)
+        rot(pos, q, k, inplace=True)
+        assert torch.equal(x, want)

@@ -3,12 +3,13 @@
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
 
 from kvssd import Rotary, RotaryScaling
-from kvssd.rotary import _overlaps_itself, refuse_grad, rotary_frequencies
+from kvssd.rotary import _overlaps_itself, _share_elements, refuse_grad, rotary_frequencies
 
 
 def test_plain_frequencies():
@@ -94,3 +95,37 @@ def test_tensors_that_hold_an_element_twice_are_seen():
     assert _overlaps_itself(t[:, :1].expand(4, 3, 8))
     assert _overlaps_itself(torch.zeros(20).as_strided((3, 2, 8), (4, 2, 1)))
     assert not _overlaps_itself(torch.zeros(0, 2, 8)) and not _overlaps_itself(t[:1].expand(1, 6, 8))
+
+
+def test_tensors_that_share_an_element_are_seen():
+    def shared(a, b):  # by the elements themselves
+        where = [{t.storage_offset() + i * t.stride(0) + h * t.stride(1) + x
+                  for i in range(t.shape[0]) for h in range(t.shape[1]) for x in range(t.shape[2])} for t in (a, b)]
+        return bool(where[0] & where[1])
+
+    flat = torch.zeros(4000)
+    x = flat[:960].view(5, 6, 32)
+    pairs = [
+        (x, x), (x[:, :5], x[:, 3:]), (x[:, :3], x[:, 2:]), (x[:, :3], x[:, 3:]), (x[:2], x[2:]), (x[:3], x[2:]),
+        (x[::2], x[1::2]), (x[::2], x[1:]), (x[:, ::2], x[:, 1::2]), (x[:, ::2], x[:, 2:3]), (x[:1], x[:1, 5:]),
+        (x[1:2, 4:], x[1:3, :4]), (x.transpose(0, 1)[:3], x.transpose(0, 1)[3:]), (x.transpose(0, 1), x[:, 5:]),
+        (x[..., :16], x[..., 16:]), (x[..., :17], x[..., 15:]), (x[:0], x), (x, torch.zeros(2, 3, 32)),
+        (x[:1].expand(1, 6, 32), x[1:, 2:]),
+    ]
+    rng = random.Random(3)
+    while len(pairs) < 2000:  # strides as they come, of tensors without an element twice
+        made = []
+        for _ in range(2):
+            n, h, d = rng.randint(1, 5), rng.randint(1, 4), 8
+            strides = rng.choice([(40, 8, 1), (64, 8, 1), (64, 16, 1), (8, 40, 1), (100, 20, 1), (33, 9, 1), (9, 50, 1)])
+            made.append(flat.as_strided((n, h, d), strides, rng.randint(0, 200)))
+        if not any(map(_overlaps_itself, made)):
+            pairs.append(tuple(made))
+    seen = [0, 0]
+    for a, b in pairs:
+        want = shared(a, b) and a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr()
+        assert _share_elements(a, b) == _share_elements(b, a) == want, (a.shape, a.stride(), b.shape, b.stride())
+        seen[want] += 1
+    assert min(seen) > 300
+    big = torch.zeros(8 * 48).view(1, 48, 8).expand(1, 48, 8)
+    assert not _share_elements(big[:, :40], big[:, 40:]) and _share_elements(big[:, :41], big[:, 40:])
