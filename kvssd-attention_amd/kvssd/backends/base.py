@@ -13,6 +13,17 @@ from dataclasses import dataclass
 from typing import Protocol, runtime_checkable
 
 import torch
+from torch.autograd import forward_ad
+
+
+def refuse_grad(*tensors: torch.Tensor | None) -> None:
+    """The generation operators have no derivative, backward or forward: say so, rather than cut the graph or drop a
+    tangent."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("this operator has no backward pass; call it under torch.no_grad() or on detached tensors")
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # (within forward_ad.dual_level only)
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise ValueError("this operator has no forward derivative; call it on the tensors' primal values")
 
 
 @dataclass(frozen=True)

@@ -12,7 +12,7 @@ import threading
 import torch
 
 from .. import _native
-from .base import PagedBatch
+from .base import PagedBatch, refuse_grad
 
 _BLOCK_BYTES = 16 << 20  # outputs allocated at a time, at most
 
@@ -94,8 +94,7 @@ class PreparedPagedDecode:
                 f"query {tuple(query.shape)} {query.dtype} on {query.device} does not match the prepared decode "
                 f"({tuple(self._qsize)} {self._qdtype} on {self._device})"
             )
-        if query.requires_grad and torch.is_grad_enabled():
-            raise ValueError("this operator has no backward pass; call it under torch.no_grad() or on detached tensors")
+        refuse_grad(query)
         if not query.is_contiguous() or query.data_ptr() % 16:  # the kernel reads 16 bytes at a time
             query = query.clone(memory_format=torch.contiguous_format)
         if torch._C._cuda_getDevice() != self._index:

@@ -23,6 +23,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _native
+from .backends.base import refuse_grad
 from .backends.hip import current_stream_handle, on_device
 
 _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16, torch.float32: _native.DTYPE_F32}
@@ -103,12 +104,6 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: RotarySc
         last = first + 0.001
     divided = [min(max((i - first) / (last - first), 0.0), 1.0) for i in range(rotary_dim // 2)]
     return [f / factor * t + f * (1.0 - t) for f, t in zip(plain, divided)]
-
-
-def refuse_grad(*tensors: torch.Tensor | None) -> None:
-    """The generation operators have no backward pass: say so, rather than cut the graph."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("this operator has no backward pass; call it under torch.no_grad() or on detached tensors")
 
 
 def _overlaps_itself(t: torch.Tensor) -> bool:

@@ -401,3 +401,27 @@ def test_decodes_prepared_before_a_cut_follow_the_cache(cuda_device):
             assert ((cache.batch.weights.double().sum(1) - sums - 8 * n).abs() < 16 * 2.0 ** -15).all()
         cache.append(make(2, 2), make(2, 2))
     del graph
+
+
+def test_tangents_are_refused_by_every_operator(cuda_device):
+    from torch.autograd import forward_ad
+
+    rng = np.random.default_rng(59)
+    pool = make_pool(rng, 4, 16, 2, 64, 32, 4)
+    batch = paged(cuda_device, pool, np.arange(4).reshape(2, 2), [20, 3], 4, 32)
+    k, q = (torch.from_numpy(rng.standard_normal((2, h, 64))).half().to(cuda_device) for h in (2, 4))
+    rotary, backend = Rotary(64, device=cuda_device), HipAttentionBackend()
+    run = backend.prepare_paged(q, batch, 0.125)
+    positions = torch.arange(2, device=cuda_device)
+    before = batch.packed_k.clone()
+    with forward_ad.dual_level():
+        dk, dq = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (k, q))
+        for call in (
+            lambda: rotary(positions, dq), lambda: rotary(positions, q, dk), lambda: append_tokens(batch, dk, k),
+            lambda: append_tokens(batch, k, dk), lambda: append_tokens(batch, k, k, rotary=rotary, query=dq),
+            lambda: run(dq), lambda: backend.run_paged(dq, batch, 0.125),
+        ):
+            with pytest.raises(ValueError, match="no forward derivative"):
+                call()
+        run(q)
+    assert torch.equal(batch.packed_k, before)

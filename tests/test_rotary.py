@@ -129,3 +129,19 @@ def test_tensors_that_share_an_element_are_seen():
     assert min(seen) > 300
     big = torch.zeros(8 * 48).view(1, 48, 8).expand(1, 48, 8)
     assert not _share_elements(big[:, :40], big[:, 40:]) and _share_elements(big[:, :41], big[:, 40:])
+
+
+def test_tangents_are_refused_not_dropped():
+    from torch.autograd import forward_ad
+
+    x = torch.zeros(2)
+    refuse_grad(x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(2))
+        refuse_grad(x, None)
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad(), pytest.raises(ValueError, match="no forward derivative"):
+                refuse_grad(None, dual)
+        refuse_grad(forward_ad.unpack_dual(dual).primal)
+    with pytest.raises(ValueError, match="no forward derivative"):
+        torch.func.jvp(lambda t: refuse_grad(t) or t, (x,), (torch.ones(2),))
