@@ -250,4 +250,7 @@ class Rotary:
                 )
             if rc:
                 _native.check(rc, "kvssd_hip_rotary")
+            if inplace:  # a graph that has saved them finds them changed, as after torch's own in-place operators
+                for t in tensors:
+                    torch.autograd.graph.increment_version(t)
         return outs[0] if key is None else outs

@@ -193,3 +193,23 @@ def test_inplace_rotation_of_overlapping_slices_is_refused(cuda_device):
         x.copy_(before)
         rot(pos, q, k, inplace=True)
         assert torch.equal(x, want)
+
+
+def test_a_graph_sees_that_its_tensor_was_rotated_in_place(cuda_device):
+    rot = Rotary(32, device=cuda_device)
+    pos = torch.arange(3, device=cuda_device)
+    w = torch.ones((3, 2, 32), device=cuda_device, requires_grad=True)
+    x, key = torch.randn((2, 3, 2, 32), device=cuda_device)
+    for tensors in ((x,), (key, x)):
+        y = (w * x).sum()  # (saves x)
+        rot(pos, *tensors, inplace=True)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    y = (w * x).sum()
+    rot(pos, x)
+    y.backward()
+    assert torch.equal(w.grad, x)
+    with torch.inference_mode():
+        z = torch.randn((3, 2, 32), device=cuda_device)
+        want = rot(pos, z)
+        assert torch.equal(rot(pos, z, inplace=True), want)
