@@ -353,8 +353,9 @@ int kvssd_hip_paged_append(const kvssd_paged_cache* cache, const kvssd_paged_app
  * out_query_dtype = 1) and lse fp32 [sequences, query_heads].  A sequence of
  * length 0 gives out = 0 and lse = -inf.  With `accumulate`, weights[b][s] +=
  * sum over the query heads of exp(score - lse).  max_length and total_tokens
- * size the split (0: the table's capacity, for every sequence); lengths beyond
- * them are answered all the same.  fp32 outputs come from 32-bit-grade
+ * size the split and, with `accumulate`, the workspace for the scores: 256
+ * bytes a query head for every 64 slots (0: the table's capacity, for every
+ * sequence); lengths beyond them are answered all the same.  fp32 outputs come from 32-bit-grade
  * arithmetic; 16-bit ones round the softmax weights times the value scales to
  * fp16. */
 typedef struct kvssd_paged_decode_args {

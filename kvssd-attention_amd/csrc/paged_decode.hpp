@@ -87,8 +87,8 @@ struct PagedDecodeParams {
   float* lse;
   float* part_o;
   float* part_ml;
-  float* scores;  // nullptr unless weights are summed: [sequences][query_heads][score_stride], log2 units
-  int64_t score_stride;
+  float* scores;  // nullptr unless weights are summed: [score_stages][query_heads][kTile], log2 units
+  int score_stages;  // of all sequences, one after the other; later ones have no place, and their scores are not kept
   int capacity;
   int run_tiles;    // stages of a run, unless the lengths call for more
   int runs;         // runs of all sequences that the grid and the workspace hold; == sequences: one run each
@@ -114,6 +114,7 @@ struct RunMap {
   int seq;    // of run r; -1: there is no such run
   int nth;    // its place among the sequence's
   int length;  // of the sequence (found with the run; in `runs_of`, not)
+  int before;  // stages of the sequences before it, where scores are kept (as `length`)
 };
 
 __device__ __forceinline__ int length_of(const PagedDecodeParams& p, int seq) {
@@ -135,14 +136,23 @@ __device__ __forceinline__ int tiles_of_runs(const PagedDecodeParams& p, int fir
   return max(p.run_tiles, max((sum + room - 1) / room, (most + kMaxSplits - 1) / kMaxSplits));
 }
 
+// Stages of the sequences before `seq` (fewer than 2^31 in all); `first` as there.
+__device__ __forceinline__ int stages_before(const PagedDecodeParams& p, int seq, int first) {
+  const int lane = threadIdx.x % kWave;
+  int sum = lane < seq ? (first + kTile - 1) / kTile : 0;
+  for (int s = lane + kWave; s - lane < seq; s += kWave) sum += s < seq ? (length_of(p, s) + kTile - 1) / kTile : 0;
+  return __builtin_amdgcn_readlane(wave_prefix(sum), kWave - 1);
+}
+
 __device__ __forceinline__ RunMap find_run(const PagedDecodeParams& p, int r) {
   const int lane = threadIdx.x % kWave;
   const int first = length_of(p, lane);
-  RunMap m{tiles_of_runs(p, first), -1, 0, 0};
+  RunMap m{tiles_of_runs(p, first), -1, 0, 0, 0};
   if (p.runs <= p.c.sequences) {
     if (r < p.c.sequences) {
       m.seq = r;
       m.length = clamp_length(uniform_load(p.c.lengths + r), p.capacity);
+      if (p.scores != nullptr) m.before = stages_before(p, r, first);
     }
     return m;
   }
@@ -156,6 +166,7 @@ __device__ __forceinline__ RunMap find_run(const PagedDecodeParams& p, int r) {
       m.seq = s0 + at;
       m.nth = r - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
       m.length = __builtin_amdgcn_readlane(length, at);
+      if (p.scores != nullptr) m.before = stages_before(p, m.seq, first);
       return m;
     }
     r -= __builtin_amdgcn_readlane(upto, kWave - 1);
@@ -167,7 +178,7 @@ __device__ __forceinline__ RunMap find_run(const PagedDecodeParams& p, int r) {
 __device__ __forceinline__ RunMap runs_of(const PagedDecodeParams& p, int seq, int* first, int* count) {
   const int lane = threadIdx.x % kWave;
   const int mine = length_of(p, lane);
-  const RunMap m{tiles_of_runs(p, mine), seq, 0, 0};
+  const RunMap m{tiles_of_runs(p, mine), seq, 0, 0, 0};
   int before = 0;
   for (int s0 = 0; s0 <= seq; s0 += kWave) {
     const int length = s0 == 0 ? mine : length_of(p, s0 + lane);
@@ -335,6 +346,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   const int length = scalar(map.length);
   const int begin = scalar(map.nth * map.tiles) * kTile;
   const int end = min(length, begin + scalar(map.tiles) * kTile);  // (at most 2^30 + 64 each)
+  const int score_stage = scalar(map.before) + begin / kTile;  // where the run's scores lie, if they are kept
 
   const int d = c.head_dim;
   const int row_bytes = d * BITS / 8;
@@ -602,7 +614,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       }
   };
   // slots in the rows: the lane's column's weights of its slots 16 lg + e; some may take no part (kRagged)
-  auto weigh_rows = [&](int base, uint64_t live, f32x4 (&s_acc)[4], const uint32_t (&skw)[8], uint32_t (&svw)[8],
+  auto weigh_rows = [&](float* rows, uint64_t live, f32x4 (&s_acc)[4], const uint32_t (&skw)[8], uint32_t (&svw)[8],
                    u32x4 (&w)[kParts][2], auto ragged_tag) {
     constexpr bool kRagged = decltype(ragged_tag)::value;
     const uint32_t mask16 = static_cast<uint32_t>(live >> (16 * lg)) & 0xFFFFu;  // slots 16 lg + e
@@ -662,8 +674,8 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       w_exp = e_new;
       first = false;
     }
-    if (p.scores != nullptr && own_g == 0 && head < p.gq) {
-      float* dst = p.scores + (head0 + head) * p.score_stride + base + 16 * lg;
+    if (rows != nullptr && own_g == 0 && head < p.gq) {
+      float* dst = rows + head * kTile + 16 * lg;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         f32x4 v;
@@ -682,7 +694,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   };
 
   // slots in the columns: the powers of the lane's slots 16 u + col, of one head, left in LDS
-  auto weigh_columns = [&](int base, uint64_t live, int e_stage, const f32x4 (&s_acc)[4], const uint32_t (&skw)[4][2],
+  auto weigh_columns = [&](float* rows, uint64_t live, int e_stage, const f32x4 (&s_acc)[4], const uint32_t (&skw)[4][2],
                            auto ragged_tag) {
     constexpr bool kRagged = decltype(ragged_tag)::value;
     float s[4], tv[4];
@@ -721,8 +733,8 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       w_exp = e_new;
       first = false;
     }
-    if (p.scores != nullptr && (GP < 8 || lg % 2 == 0) && head_own < p.gq) {
-      float* dst = p.scores + (head0 + head_own) * p.score_stride + base + col;
+    if (rows != nullptr && (GP < 8 || lg % 2 == 0) && head_own < p.gq) {
+      float* dst = rows + head_own * kTile + col;
 #pragma unroll
       for (int u = 0; u < 4; ++u) dst[16 * u] = out[u] ? -INFINITY : s[u] * s_factor;
     }
@@ -803,7 +815,10 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       if (in_step) __builtin_amdgcn_s_barrier();
       copy_stage(later, buf);
     }
-    // ---- scores
+    // ---- scores; where the kv head's are kept
+    float* rows = nullptr;
+    if (p.scores != nullptr && score_stage + i < p.score_stages)
+      rows = p.scores + (static_cast<int64_t>(score_stage + i) * p.query_heads + kvh * p.gq) * kTile;
     f32x4 s_acc[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -826,9 +841,9 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       for (int n = 1; n < GP / 2; ++n) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, raw[1][n] & 0x7FFF7FFFu));
       const int e_stage = (m[0] > m[1] ? m[0] >> 10 : m[1] >> 10) - 23;
       if (now.live == ~0ull) {
-        weigh_columns(base, now.live, e_stage, s_acc, sk_slot, std::false_type{});
+        weigh_columns(rows, now.live, e_stage, s_acc, sk_slot, std::false_type{});
       } else {
-        weigh_columns(base, now.live, now.live >> lane & 1 ? e_stage : -32, s_acc, sk_slot, std::true_type{});
+        weigh_columns(rows, now.live, now.live >> lane & 1 ? e_stage : -32, s_acc, sk_slot, std::true_type{});
         const uint32_t mask16 = static_cast<uint32_t>(now.live >> (16 * lg)) & 0xFFFFu;
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -840,8 +855,8 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       __builtin_memcpy(powers, __builtin_assume_aligned(&power_lds[wave][col / GP * kPowerRow + 16 * lg], 16), 64);
       form_weights(powers, svw, w);
     } else {
-      if (now.live == ~0ull) weigh_rows(base, now.live, s_acc, skw, svw, w, std::false_type{});
-      else weigh_rows(base, now.live, s_acc, skw, svw, w, std::true_type{});
+      if (now.live == ~0ull) weigh_rows(rows, now.live, s_acc, skw, svw, w, std::false_type{});
+      else weigh_rows(rows, now.live, s_acc, skw, svw, w, std::true_type{});
     }
     // ---- weights times values: 8 bytes of a row a read, 16 (INT4) or 32 (INT2) dims
 #pragma unroll

@@ -11,6 +11,10 @@
 // Weights: slot t of sequence b gains sum over heads of 2^(s_bht - lse2_bh) from
 // the scores that the decode left (4 bytes a slot and head): a second pass
 // over the keys would read head_dim * bits / 8 + scales per kv head instead.
+// Scores lie by stage, one sequence's behind the other's, in as many places as
+// the caller's hints make out (a page table has far more slots than its pool
+// where every sequence may grow into all of it); a stage past them, of lengths
+// past the hints, has its scores formed again here, a slot a lane.
 // 16 sequences of 64 heads and up to 16,384 slots: 8.7 us (43 with a thread's heads
 // one after the other).
 #include "paged_decode.hpp"
@@ -104,6 +108,32 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
   if (tid == 0 && blockIdx.y == 0) p.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (big + log2f(total));
 }
 
+__device__ __forceinline__ float query_value(const void* row, int dtype, int dim) {
+  if (dtype == KVSSD_DTYPE_F32) return load_query<float>(row, dim);
+  return dtype == KVSSD_DTYPE_F16 ? load_query<_Float16>(row, dim) : load_query<uint16_t>(row, dim);
+}
+
+// The score of a row of the pool for query head h of a sequence, log2 units.
+__device__ float row_score(const PagedDecodeParams& p, int seq, int h, int64_t row) {
+  const kvssd_paged_cache& c = p.c;
+  const int64_t at = row * c.kv_heads + h / p.gq;
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(c.packed_k + at * (c.head_dim * c.bits / 8));
+  const void* query = static_cast<const char*>(p.query) + (static_cast<int64_t>(seq) * p.query_heads + h) * c.head_dim *
+                                                              (p.query_dtype == KVSSD_DTYPE_F32 ? 4 : 2);
+  const int words = c.group_size * c.bits / 32, mask = (1 << c.bits) - 1, mid = 1 << (c.bits - 1);
+  float score = 0.0f;
+  for (int g = 0, dim = 0; g < p.groups; ++g) {
+    float sum = 0.0f;
+    for (int w = 0; w < words; ++w) {
+      uint32_t x = *codes++;
+      for (int i = 0; i < 32; i += c.bits, x >>= c.bits)
+        sum = __builtin_fmaf(query_value(query, p.query_dtype, dim++), static_cast<float>(static_cast<int>(x & mask) - mid), sum);
+    }
+    score = __builtin_fmaf(sum, half_bits_to_float(c.scales_k[at * p.groups + g]), score);
+  }
+  return score * p.scale_log2;
+}
+
 // A slot's weight: 2^(score - the head's sum) over its heads.  A workgroup takes 4 kWave slots; its waves take a
 // quarter of the heads each, kDeep rows of scores on the way at a time, and are joined in LDS in a fixed order.
 __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodeParams p, int blocks) {
@@ -112,12 +142,15 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodePara
   const int seq = blockIdx.x / blocks, nth = blockIdx.x % blocks;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int length = paged_length(p.c.lengths, seq, p.capacity);
+  if (static_cast<int64_t>(nth) * 4 * kWave >= length) return;
+  const int before = stages_before(p, seq, length_of(p, lane));
   const float* lse = p.lse + static_cast<int64_t>(seq) * p.query_heads;
-  const float* scores = p.scores + static_cast<int64_t>(seq) * p.query_heads * p.score_stride;
   for (int64_t t0 = static_cast<int64_t>(nth) * 4 * kWave; t0 < length; t0 += static_cast<int64_t>(blocks) * 4 * kWave) {
     const int64_t t = t0 + 4 * lane;
+    const int64_t stage = before + t / kTile;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (t < length) {  // (rows are of whole 64 slots)
+    if (t < length && stage < p.score_stages) {  // (rows are of whole 64 slots)
+      const float* scores = p.scores + stage * p.query_heads * kTile + t % kTile;
       for (int h0 = wave; h0 < p.query_heads; h0 += kDeep * kWaves) {
         f32x4 v[kDeep];
         float e[kDeep];
@@ -125,7 +158,7 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodePara
         for (int i = 0; i < kDeep; ++i) {
           const int h = h0 + i * kWaves;
           e[i] = h < p.query_heads ? lse[h] * kLog2e : -INFINITY;
-          if (h < p.query_heads) v[i] = *reinterpret_cast<const f32x4*>(scores + h * p.score_stride + t);
+          if (h < p.query_heads) v[i] = *reinterpret_cast<const f32x4*>(scores + h * kTile);
         }
 #pragma unroll
         for (int i = 0; i < kDeep; ++i) {
@@ -133,6 +166,20 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodePara
 #pragma unroll
           for (int x = 0; x < 4; ++x) sum[x] += __builtin_amdgcn_exp2f(v[i][x] - e[i]);
         }
+      }
+    } else if (t < length) {
+      for (int x = 0; x < 4 && t + x < length; ++x) {
+        const int slot = static_cast<int>(t) + x;
+        const int page = p.c.page_table[static_cast<int64_t>(seq) * p.c.max_pages + slot / p.c.page_tokens];
+        if (page < 0 || page >= p.c.num_pages) continue;
+        const int64_t row = static_cast<int64_t>(page) * p.c.page_tokens + slot % p.c.page_tokens;
+        float w = 0.0f;
+        for (int h = wave; h < p.query_heads; h += kWaves) {
+          const float e = lse[h] * kLog2e;
+          if (e != -INFINITY) w += __builtin_amdgcn_exp2f(row_score(p, seq, h, row) - e);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) sum[y] = y == x ? w : sum[y];
       }
     }
     sums[wave][lane] = sum;
@@ -207,9 +254,8 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, Plan* 
   const size_t rows = static_cast<size_t>(p.runs) * p.query_heads;
   out->o_bytes = whole ? 0 : aligned(rows * c.head_dim * sizeof(float));
   out->ml_bytes = whole ? 0 : aligned(rows * 2 * sizeof(float));
-  p.score_stride = tiles_of(p.capacity) * kTile;
-  out->score_bytes =
-      a.accumulate ? static_cast<size_t>(c.sequences) * p.query_heads * p.score_stride * sizeof(float) : 0;
+  p.score_stages = static_cast<int>(all);
+  out->score_bytes = a.accumulate ? static_cast<size_t>(all) * p.query_heads * kTile * sizeof(float) : 0;
   if (static_cast<int64_t>(p.runs) * waves * kWave > 0xFFFFFFFFll ||
       static_cast<int64_t>(c.sequences) * p.query_heads * kThreads > 0xFFFFFFFFll)
     return arg_error("too many sequences for one call");

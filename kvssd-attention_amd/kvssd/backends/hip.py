@@ -218,8 +218,8 @@ class HipAttentionBackend:
         ``out`` is fp32 unless ``out_dtype`` is the query's dtype.  A sequence of length 0 gives out = 0 and
         lse = -inf.  ``accumulate`` adds each slot's attention weight, summed over the query heads, to
         ``batch.weights``.  ``max_length`` and ``total_tokens``, the longest length and their sum where the caller
-        knows them (0: the page table's capacity), size the split over the sequences; lengths past them are answered
-        too."""
+        knows them (0: the page table's capacity), size the split over the sequences and, with ``accumulate``, the
+        workspace (4 bytes a slot and query head); lengths past them are answered too, their weights more slowly."""
         return PreparedPagedDecode(query, batch, sm_scale, out_dtype, accumulate, max_length, total_tokens, rows=1)(query)
 
     def prepare_paged(

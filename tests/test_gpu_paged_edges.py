@@ -425,3 +425,41 @@ def test_tangents_are_refused_by_every_operator(cuda_device):
                 call()
         run(q)
     assert torch.equal(batch.packed_k, before)
+
+
+@pytest.mark.parametrize(("lengths", "bits", "qh", "kvh", "d", "g", "bt", "dtype"), [
+    ([3000, 0, 64, 777], 4, 32, 8, 128, 32, 64, torch.bfloat16),
+    ([500, 1, 130], 2, 12, 2, 96, 32, 24, torch.float16),          # three groups, slots' rows found lane by lane
+    ([200, 65], 4, 6, 3, 256, 256, 40, torch.float32),
+    ([300, 40], 2, 2, 2, 64, 64, 32, torch.float32),
+    ([(37 * i) % 301 for i in range(130)], 4, 8, 2, 64, 32, 16, torch.float16),
+    ([5] * 70 + [20000], 4, 4, 1, 32, 32, 64, torch.bfloat16),
+])
+def test_weights_of_lengths_past_the_hints(cuda_device, lengths, bits, qh, kvh, d, g, bt, dtype):
+    """Scores have as many places as the hints make out; a slot past them gets the same weight, from its key."""
+    rng = np.random.default_rng(60)
+    width = max(-(-n // bt) for n in lengths) + 1
+    pages = sum(-(-n // bt) for n in lengths) + 1
+    pool = make_pool(rng, pages, bt, kvh, d, g, bits)
+    table = make_table(rng, lengths, bt, width, pages)
+    table[0, 1] = -1  # slots without a page
+    start = rng.uniform(0, 3, (len(lengths), width * bt)).astype(np.float32)
+    q = torch.from_numpy(rng.standard_normal((len(lengths), qh, d))).to(dtype).to(cuda_device)
+    scale = d ** -0.5
+    want = attend(as_double(q), pool, table, lengths, bits, scale, start)
+    u = 2.0 ** -24
+    e = 2 * (d + 16) * u * want["reach"] + (np.abs(want["lse"][np.isfinite(want["lse"])]).max() + 60) * 8 * u
+    added = want["weights"] - start
+    tol = added * (e + qh * u) * 2 + np.abs(want["weights"]) * u * 2
+    backend = HipAttentionBackend()
+    half = dict(max_length=max(lengths), total_tokens=sum(lengths) // 2)
+    for hints in ({}, dict(max_length=max(lengths), total_tokens=sum(lengths)), half, dict(max_length=1, total_tokens=1),
+                  dict(max_length=70), dict(total_tokens=1)):
+        batch = paged(cuda_device, pool, table, lengths, bits, g, start)
+        run = backend.prepare_paged(q, batch, scale, accumulate=True, **hints)
+        out, lse = run(q)
+        check_attention(out, lse, want, d, max(lengths), torch.float32, True)
+        got = as_double(batch.weights)
+        assert (np.abs(got - want["weights"]) <= tol).all(), hints
+        untouched = added == 0
+        assert (got[untouched] == start.astype(np.float64)[untouched]).all(), hints

@@ -364,3 +364,21 @@ def test_a_cut_writes_into_the_arrays_that_there_are(monkeypatch):
     for got, want in zip((before.lengths, before.weights, before.positions), cut):
         assert torch.equal(got[..., :9], want[..., :9])
     assert cache.lengths == [4, 2, 0] and cache.free_pages == 4
+
+
+def test_the_scores_workspace_goes_by_the_hints():
+    """16 sequences that may each grow into a whole pool of 262,144 slots (a table's row), 32 query heads."""
+    lib = _native.load()
+    cache = native(kv_heads=8, head_dim=128, num_pages=4096, page_tokens=64, sequences=16, max_pages=4096)
+    sizes = []
+    for accumulate in (0, 1):
+        for hints in ({}, dict(max_length=4700, total_tokens=70000), dict(total_tokens=70000), dict(max_length=4700)):
+            args, n = _native.PagedDecodeArgs(query_heads=32, accumulate=accumulate, **hints), ctypes.c_size_t(0)
+            _native.check(
+                lib.kvssd_hip_paged_decode_workspace_bytes(ctypes.byref(cache), ctypes.byref(args), ctypes.byref(n)), "decode"
+            )
+            sizes.append(n.value)
+    scores = [b - a for a, b in zip(sizes[:4], sizes[4:])]
+    stage = 32 * 64 * 4  # bytes of 64 slots' scores
+    assert scores[0] == 16 * 4096 * stage  # no hint: every slot of the table
+    assert scores[1] == scores[2] == (70000 // 64 + 16) * stage and scores[3] == 16 * 74 * stage
