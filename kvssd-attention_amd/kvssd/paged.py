@@ -195,6 +195,8 @@ class PagedKVCache:
         if max_pages < 1:
             raise ValueError("max_pages must be positive")
         device = torch.device(device)
+        if device.type == "cuda" and device.index is None:  # this GPU, whichever is the current one later on
+            device = torch.device("cuda", torch.cuda.current_device())
         self.device = device
         self.page_tokens, self.max_pages, self.sequences = page_tokens, max_pages, sequences
         self.backend = resolve_attention_backend(attention_backend, device)

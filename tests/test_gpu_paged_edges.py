@@ -463,3 +463,14 @@ def test_weights_of_lengths_past_the_hints(cuda_device, lengths, bits, qh, kvh, 
         assert (np.abs(got - want["weights"]) <= tol).all(), hints
         untouched = added == 0
         assert (got[untouched] == start.astype(np.float64)[untouched]).all(), hints
+
+
+def test_a_cache_of_an_unnumbered_device(cuda_device):
+    cache = PagedKVCache(4, 16, 1, 32, sequences=2, device="cuda")
+    assert cache.device == cache.batch.packed_k.device == cuda_device
+    x = torch.ones((5, 1, 32), device=cuda_device)
+    cache.append(x, x, [3, 2])
+    out, _ = cache.attend(torch.ones((2, 2, 32), device=cuda_device))
+    # a one is held as code 7 times the scale 1/7, which its rounding to fp16 puts off by at most 2^-11 of itself; the
+    # mean of equal values is that value to 32-bit grade
+    assert ((out - 1).abs() <= 2.0 ** -11 + 2.0 ** -16).all() and cache.batch.lengths.tolist() == [3, 2]

@@ -382,3 +382,21 @@ def test_the_scores_workspace_goes_by_the_hints():
     stage = 32 * 64 * 4  # bytes of 64 slots' scores
     assert scores[0] == 16 * 4096 * stage  # no hint: every slot of the table
     assert scores[1] == scores[2] == (70000 // 64 + 16) * stage and scores[3] == 16 * 74 * stage
+
+
+def test_a_cache_stays_on_the_gpu_that_was_current(monkeypatch):
+    made = []
+
+    class Stop(Exception):
+        pass
+
+    def resolve(name, device):
+        made.append(device)
+        raise Stop
+
+    monkeypatch.setattr("kvssd.paged.resolve_attention_backend", resolve)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    for device, want in (("cuda", "cuda:3"), ("cuda:1", "cuda:1"), ("cpu", "cpu")):
+        with pytest.raises(Stop):
+            host_cache(device=device)
+        assert made.pop() == torch.device(want)
