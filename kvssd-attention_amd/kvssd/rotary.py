@@ -98,6 +98,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: RotarySc
         """The (fractional) pair that makes this many turns in the original context."""
         return rotary_dim * math.log(scaling.original_positions / (turns * 2 * math.pi)) / (2 * math.log(base))
 
+    if pair_turning(low) <= 0:  # not even the first pair makes more
+        return [f / factor for f in plain]
     first = max(math.floor(pair_turning(high)), 0)
     last = min(math.ceil(pair_turning(low)), rotary_dim - 1)
     if last <= first:  # the ramp is a step

@@ -145,3 +145,17 @@ def test_tangents_are_refused_not_dropped():
         refuse_grad(forward_ad.unpack_dual(dual).primal)
     with pytest.raises(ValueError, match="no forward derivative"):
         torch.func.jvp(lambda t: refuse_grad(t) or t, (x,), (torch.ones(2),))
+
+
+@pytest.mark.parametrize("scaling", [
+    RotaryScaling("yarn", 8.0, 1), RotaryScaling("yarn", 8.0, 6), RotaryScaling("yarn", 4.0, 600, 100.0, 200.0),
+])
+def test_no_pair_of_a_short_context_makes_the_turns_that_it_would_stay_for(scaling):
+    plain = rotary_frequencies(16, 10000.0)
+    assert scaling.original_positions * plain[0] / (2 * math.pi) < scaling.bounds[0]
+    assert rotary_frequencies(16, 10000.0, scaling) == [f / scaling.factor for f in plain]
+
+
+def test_every_pair_of_a_long_context_stays_where_all_turn_often_enough():
+    scaling = RotaryScaling("yarn", 8.0, 1 << 40)
+    assert rotary_frequencies(16, 100.0, scaling) == rotary_frequencies(16, 100.0)
