@@ -332,7 +332,9 @@ typedef struct kvssd_paged_cache {
  * (rotary not NULL) and rounded to their type, then keys and values are
  * quantised as by kvssd_hip_quantize.  Slots past the table's end are
  * dropped, and pages that are written may be named by one sequence only.
- * `query` (data NULL: none) is rotated by the same positions.
+ * `query` (data NULL: none) is rotated by the same positions.  Tokens before
+ * offsets[0] and from offsets[sequences] on are no sequence's: dropped, their
+ * queries rotated as at position 0.
  * Where the cache has them, the new slots' weights become 0 and their
  * positions are stored.  lengths_out[b] = lengths[b] + count, at most the
  * table's capacity; it may be the cache's own lengths where offsets is NULL. */

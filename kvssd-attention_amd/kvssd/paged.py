@@ -59,9 +59,11 @@ def append_tokens(
     strides).  With ``offsets`` (int32 [sequences + 1]) tokens offsets[b] .. offsets[b+1]-1 belong to sequence b;
     without, there is one token a sequence.  A sequence's i-th new token goes to slot lengths[b] + i (dropped past
     the page table's end or where the table names no page) and has position first_positions[b] + i (int32
-    [sequences]; default: its slot).  The pages of those slots must be no other sequence's.  With ``rotary`` the keys are turned by their positions and rounded to their
-    type before they are quantised, and so is ``query`` [tokens, query_heads, head_dim], if given.  Where the batch
-    has them, the slots' positions are stored and their weights set to 0.
+    [sequences]; default: its slot).  The pages of those slots must be no other sequence's.  With ``rotary`` the keys
+    are turned by their positions and rounded to their type before they are quantised, and so is ``query`` [tokens,
+    query_heads, head_dim], if given.  Where the batch has them, the slots' positions are stored and their weights set
+    to 0.  Tokens of no sequence (before offsets[0], from offsets[sequences] on) are dropped, their queries turned as
+    at position 0.
 
     ``batch.lengths`` stays as it is unless it is passed as ``lengths_out`` (one token a sequence only); by default
     the new lengths are a new tensor."""

@@ -474,3 +474,25 @@ def test_a_cache_of_an_unnumbered_device(cuda_device):
     # a one is held as code 7 times the scale 1/7, which its rounding to fp16 puts off by at most 2^-11 of itself; the
     # mean of equal values is that value to 32-bit grade
     assert ((out - 1).abs() <= 2.0 ** -11 + 2.0 ** -16).all() and cache.batch.lengths.tolist() == [3, 2]
+
+
+def test_tokens_of_no_sequence_are_dropped(cuda_device):
+    """A padded batch: offsets that begin behind the first token and end before the last."""
+    from kvssd import RotaryScaling
+
+    rng = np.random.default_rng(61)
+    pool = make_pool(rng, 8, 16, 2, 64, 32, 4)
+    table = np.arange(8).reshape(2, 4)
+    slots = np.zeros((2, 64))
+    a, b = (paged(cuda_device, pool, table, [3, 14], 4, 32, slots.astype(np.float32) + 7, slots.astype(np.int32) - 1)
+            for _ in "ab")
+    k, v, q = (torch.from_numpy(rng.standard_normal((40, h, 64))).half().to(cuda_device) for h in (2, 2, 4))
+    rotary = Rotary(64, scaling=RotaryScaling("yarn", 4.0), device=cuda_device)
+    offsets = torch.tensor([5, 20, 31], dtype=torch.int32, device=cuda_device)
+    turned, lengths = append_tokens(a, k, v, offsets=offsets, rotary=rotary, query=q)
+    want, want_lengths = append_tokens(b, k[5:31], v[5:31], offsets=offsets - 5, rotary=rotary, query=q[5:31])
+    assert lengths.tolist() == want_lengths.tolist() == [18, 25] and torch.equal(turned[5:31], want)
+    for name in ("packed_k", "packed_v", "scales_k", "scales_v", "weights", "positions"):
+        assert torch.equal(getattr(a, name), getattr(b, name)), name
+    at_0 = rotary(torch.zeros(40, dtype=torch.int64, device=cuda_device), q)
+    assert torch.equal(turned[:5], at_0[:5]) and torch.equal(turned[31:], at_0[31:])
