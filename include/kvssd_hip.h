@@ -387,7 +387,9 @@ int kvssd_hip_paged_decode(const kvssd_paged_cache* cache, const kvssd_paged_dec
  * weights_out and positions_out (the cache's shapes, not its own arrays)
  * describe the result; slots past the new length get weight 0 and position
  * -1.  Needs the cache's weights and positions.  A page may be named by one
- * sequence, and once, only. */
+ * sequence, and once, only; every slot below the length of a sequence that is
+ * cut has to lie in a page of the pool (a row without one is not copied, and
+ * the slot that it was to fill keeps what it held). */
 typedef struct kvssd_paged_evict_args {
   int32_t budget, sink, recent, reserved;
   int32_t* lengths_out;

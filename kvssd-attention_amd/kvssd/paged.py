@@ -129,7 +129,9 @@ def evict_tokens(
     position - recent), then those of the largest weights (NaN counts as -inf); of equals the lower slot, and
     ``budget`` in all.  The n-th kept slot at or past the budget moves into the n-th freed slot before it: only
     those rows are copied, within the sequence's pages (which no other sequence, and no second place of the table,
-    may name).  The batch's own lengths, weights and positions stay as
+    may name).  Every slot of a sequence that is cut has to lie in a page of the pool: a row without one cannot move,
+    and the slot that it was to fill would keep an evicted token's under its own weight and position (attention and
+    append skip such slots; :class:`PagedKVCache` makes none).  The batch's own lengths, weights and positions stay as
     they are; the returned ones describe the cache after the cut (weight 0 and position -1 past the new length)."""
     batch.validate()
     index = _gpu_index(batch)

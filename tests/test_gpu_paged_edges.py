@@ -496,3 +496,30 @@ def test_tokens_of_no_sequence_are_dropped(cuda_device):
         assert torch.equal(getattr(a, name), getattr(b, name)), name
     at_0 = rotary(torch.zeros(40, dtype=torch.int64, device=cuda_device), q)
     assert torch.equal(turned[:5], at_0[:5]) and torch.equal(turned[31:], at_0[31:])
+
+
+@pytest.mark.parametrize(("lengths", "budget", "bt", "width"), [
+    ([300, 150, 20], 100, 24, 20), ([5000, 120], 4000, 64, 80), ([9000, 4100], 3000, 64, 200),
+], ids=["one", "rows moved apart", "chunks"])
+def test_attention_after_a_cut_is_over_the_kept_tokens(cuda_device, lengths, budget, bt, width):
+    rng = np.random.default_rng(62)
+    pages = sum(-(-n // bt) for n in lengths) + 1
+    pool = make_pool(rng, pages, bt, 2, 64, 32, 4)
+    table = make_table(rng, lengths, bt, width, pages)
+    slots = (len(lengths), width * bt)
+    w = np.exp(2 * rng.standard_normal(slots)).astype(np.float32)
+    pos = np.tile(np.arange(slots[1], dtype=np.int32), (len(lengths), 1))
+    batch = paged(cuda_device, pool, table, lengths, 4, 32, w, pos)
+    new_lengths, new_w, new_p = evict_tokens(batch, budget, sink=2, recent=50)
+    batch.lengths.copy_(new_lengths)
+    q = torch.from_numpy(rng.standard_normal((len(lengths), 4, 64))).half().to(cuda_device)
+    out, lse = HipAttentionBackend().run_paged(q, batch, 0.125)
+    # the kept slots' rows of the pool as it was, a page a token
+    kept = [evict(w[b], pos[b], n, budget, 2, 50) for b, n in enumerate(lengths)]
+    rows = np.full((len(lengths), max(map(len, kept))), -1)
+    for b, source in enumerate(kept):
+        rows[b, :len(source)] = [table[b, s // bt] * bt + s % bt for s in source]
+        assert new_p[b, :len(source)].tolist() == source and new_w[b, :len(source)].tolist() == w[b, source].tolist()
+    loose = [a.reshape(pages * bt, 1, *a.shape[2:]) for a in pool]
+    want = attend(as_double(q), loose, rows, [len(s) for s in kept], 4, 0.125)
+    check_attention(out, lse, want, 64, max(map(len, kept)), torch.float32, True)
