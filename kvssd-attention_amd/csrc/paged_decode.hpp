@@ -41,11 +41,13 @@
 // QK (v_mfma_f32_16x16x32_f16): one side is 16 slots' codes, the other (query
 //   head, group): the query masked to one group, so that a result is one group's
 //   share of a score and its scale multiplies in 32 bits afterwards.  A code
-//   enters as the fp16 number 1 + c / 2^6 (INT4) or 1 + c / 2^2 (a bit operation
-//   for a pair); the offset's share, -(1 + mid/2^6) sum q, is the accumulator's
-//   initial value.  The query is scaled by a power of two per head into fp16's
-//   range (exact for fp16 and bf16) and, with 32-bit results, taken as a sum of
-//   two fp16 parts.
+//   enters as the exact number (c - mid) / 2^6 (INT4) or / 2^2, as in PV.  (As
+//   1 + c / 2^6, with the offset's share taken out of the sum, it costs two
+//   instructions fewer a word, 161 for 163 us of the 795 MB, and the scores what
+//   the offset outweighs them by: the lse of up to 7 slots of 256 dims was off
+//   1.3e-6 of itself, 1.5e-7 now.)  The query is scaled by a power of two per
+//   head into fp16's range (exact for fp16 and bf16) and, with 32-bit results,
+//   taken as a sum of two fp16 parts.
 // Four groups and more (GP >= 4): rows = (head, group), columns = slots.  A lane
 //   holds a slot's shares of four groups and adds them itself; the softmax's 2^x
 //   go through LDS to the lanes that form the weights.  One or two groups: rows =
@@ -230,13 +232,14 @@ __device__ __forceinline__ uint32_t fma_pair(uint32_t v, _Float16 a, _Float16 b)
   return __builtin_bit_cast(uint32_t, r);
 }
 
-// A word of 8 slots' transposed codes (nibble e: slot e) as PV operand pairs
-// (e, e + 4): INT4, the dim's (c - 8) / 64; INT2, (c - 2) / 4 of the nibble's
-// even (odd = 0) or odd dim.  Codes stay where they are in their half, at
-// 1 + c / F for the F of that place; one fused multiply-add takes out the 1 and
-// the offset and brings all to one F, exactly.
+// A word's codes as operand pairs.  Values: 8 slots' transposed codes (nibble e:
+// slot e) as pairs (e, e + 4); INT4, the dim's (c - 8) / 64; INT2, (c - 2) / 4 of
+// the nibble's even (odd = 0) or odd dim.  Keys, the same bits: a row's codes
+// i and i + 4 of 8 (INT4), 2 i + odd and 2 i + odd + 8 of 16.  Codes stay where
+// they are in their half, at 1 + c / F for the F of that place; one fused
+// multiply-add takes out the 1 and the offset and brings all to one F, exactly.
 template <int BITS>
-__device__ __forceinline__ u32x4 value_operand(uint32_t x, int odd, const Masks& k, uint32_t m01, uint32_t m23) {
+__device__ __forceinline__ u32x4 code_operand(uint32_t x, int odd, const Masks& k, uint32_t m01, uint32_t m23) {
   const uint32_t y = x >> 8;
   if constexpr (BITS == 4) {
     const _Float16 f = 16.0f, fo = -16.125f, o = -1.125f;
@@ -250,17 +253,6 @@ __device__ __forceinline__ u32x4 value_operand(uint32_t x, int odd, const Masks&
     const _Float16 f0 = 64.0f, o0 = -64.5f, f1 = 4.0f, o1 = -4.5f;
     return u32x4{fma_pair(ao(x, m23), f0, o0), fma_pair(ao(x, k.m67), f1, o1), fma_pair(ao(y, m23), f0, o0),
                  fma_pair(ao(y, k.m67), f1, o1)};
-  }
-}
-
-// A word of key codes as QK operands, one (INT4) or two (INT2) slices
-template <int BITS>
-__device__ __forceinline__ u32x4 key_operand(uint32_t x, int odd, const Masks& k) {
-  if constexpr (BITS == 4) {
-    return u32x4{ao(x << 4, k.m47), ao(x, k.m47), ao(x >> 4, k.m47), ao(x >> 8, k.m47)};
-  } else {
-    if (odd == 0) return u32x4{ao(x << 8, k.m89), ao(x << 6, k.m89), ao(x << 4, k.m89), ao(x << 2, k.m89)};
-    return u32x4{ao(x, k.m89), ao(x >> 2, k.m89), ao(x >> 4, k.m89), ao(x >> 6, k.m89)};
   }
 }
 
@@ -317,7 +309,6 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   constexpr int kParts = PREC ? 2 : 1;
   constexpr int kHeads = 16 / GP;          // query heads of a head tile
   constexpr float kF = kUnpackScale<BITS>;
-  constexpr float kOff = kUnpackOffset<BITS>;
   constexpr float kLazy = 6.0f;            // log2 units a score may exceed the reference by
   // 4-byte words copied of a slot's scales of one head (two for one: a copy's slots are then of one half)
   constexpr int kScaleWords = GP <= 4 ? 2 : 4, kScaleCopies = kScaleWords;
@@ -501,10 +492,10 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   else __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
   asm volatile("" ::: "memory");
 
-  // ---- query operand, its scale and the accumulator's initial value (while the first stage arrives)
+  // ---- query operand and its scale (while the first stage arrives)
   u32x4 q[kParts][kSlices];
   const int head = head_first + col / GP;  // of the lane's column, within its kv head
-  float c_init, s_factor;
+  float s_factor;
   {
     float x[kSpan];
     float big = 0.0f;
@@ -528,38 +519,26 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     const float scale_up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + up) << 23);
     const float scale_down = __builtin_bit_cast(float, static_cast<uint32_t>(127 - up) << 23);
     s_factor = scale_down * (kF * p.scale_log2);
-    float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < kSlices; ++j)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        // the codes' order in key_operand: pairs (i, i + 4) of a word's 8, (i, i + 8) of its 16
-        const int lo = BITS == 4 ? j * 8 + w : j / 2 * 16 + j % 2 * 4 + w;
+        const int lo = BITS == 4 ? j * 8 + w : j / 2 * 16 + j % 2 + 2 * w;  // the codes' order in code_operand
         const float a = x[lo] * scale_up, b = x[lo + (BITS == 4 ? 4 : 8)] * scale_up;
         const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
         q[0][j][w] = pack_half2(ah, bh);
-        sum += static_cast<float>(ah) + static_cast<float>(bh);
         if constexpr (PREC) {
           const _Float16 al = static_cast<_Float16>(a - static_cast<float>(ah));
           const _Float16 bl = static_cast<_Float16>(b - static_cast<float>(bh));
           q[kParts - 1][j][w] = pack_half2(al, bl);
-          sum += static_cast<float>(al) + static_cast<float>(bl);
         }
       }
-    sum += __shfl_xor(sum, 16, kWave);
-    sum += __shfl_xor(sum, 32, kWave);
-    c_init = -kOff * sum;
   }
-  // of the lane's own results: rows 4 lg + i, all of one head, or its column
-  f32x4 c_rows = {c_init, c_init, c_init, c_init};
-  int head_own = head;
+  int head_own = head;  // of the lane's own results: rows 4 lg + i, all of one head, or its column
   if constexpr (kSlotColumns) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c_rows[i] = __shfl(c_init, 4 * lg + i, kWave);
     s_factor = __shfl(s_factor, 4 * lg, kWave);
     head_own = head_first + 4 * lg / GP;
   }
-  asm("" : "+v"(c_rows));  // (kept in registers, not formed anew for every product)
   // the query is read: the second stage may follow
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   if (crowded && stages > 0) copy_stage(now, 0);
@@ -822,10 +801,11 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     f32x4 s_acc[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      f32x4 s = c_rows;
+      f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int j = 0; j < kSlices; ++j) {
-        const u32x4 a = BITS == 4 ? key_operand<BITS>(kw[u][j], 0, masks) : key_operand<BITS>(kw[u][j / 2], j % 2, masks);
+        const u32x4 a = BITS == 4 ? code_operand<BITS>(kw[u][j], 0, masks, m01, m23)
+                                  : code_operand<BITS>(kw[u][j / 2], j % 2, masks, m01, m23);
 #pragma unroll
         for (int n = 0; n < kParts; ++n) s = kSlotColumns ? mfma16(q[n][j], a, s) : mfma16(a, q[n][j], s);
       }
@@ -866,7 +846,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int odd = 0; odd < (BITS == 4 ? 1 : 2); ++odd) {
-          const u32x4 b = value_operand<BITS>(static_cast<uint32_t>(x[s]), odd, masks, m01, m23);
+          const u32x4 b = code_operand<BITS>(static_cast<uint32_t>(x[s]), odd, masks, m01, m23);
           const int tile = BITS == 4 ? r : 2 * r + odd;
           acc[tile] = mfma16(w[0][s], b, acc[tile]);
           if constexpr (PREC) acc[tile] = mfma16(w[kParts - 1][s], b, acc[tile]);

@@ -523,3 +523,29 @@ def test_attention_after_a_cut_is_over_the_kept_tokens(cuda_device, lengths, bud
     loose = [a.reshape(pages * bt, 1, *a.shape[2:]) for a in pool]
     want = attend(as_double(q), loose, rows, [len(s) for s in kept], 4, 0.125)
     check_attention(out, lse, want, 64, max(map(len, kept)), torch.float32, True)
+
+
+@pytest.mark.parametrize(("bits", "d", "g"), [(4, 128, 32), (4, 128, 128), (4, 64, 32), (4, 256, 32), (2, 128, 32),
+                                              (2, 128, 64), (2, 256, 256), (2, 96, 32)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_scores_are_sums_of_what_the_codes_stand_for(cuda_device, bits, d, g, dtype):
+    """Keys of zeros but for one dim: the score is one product.  Were the codes' offset part of the sum, its rounding
+    would show: the query's values add up to a thousand times that product's last places."""
+    rng = np.random.default_rng(63)
+    mid, lengths = 1 << (bits - 1), [1, 40, 200]
+    pool = make_pool(rng, 12, 32, 2, d, g, bits)
+    codes = np.full((12, 32, 2, d), mid, np.uint8)
+    one = rng.integers(0, d, (12, 32, 2, 1))
+    np.put_along_axis(codes, one, mid + rng.choice([-1, 1], one.shape).astype(np.uint8), -1)
+    pool[0][...] = sum(codes[..., i::8 // bits] << (bits * i) for i in range(8 // bits))
+    pool[2][...] = 1.0
+    table = make_table(rng, lengths, 32, 7, 12)
+    batch = paged(cuda_device, pool, table, lengths, bits, g)
+    q = torch.from_numpy(rng.uniform(500, 2000, (3, 8, d))).to(dtype).to(cuda_device)
+    scale = 2.0 ** -8
+    want = attend(as_double(q), pool, table, lengths, bits, scale)
+    for out_dtype in (dtype, torch.float32):
+        _, lse = HipAttentionBackend().run_paged(q, batch, scale, out_dtype=out_dtype)
+        # scores exact but for their factor's two roundings; lse's own terms as elsewhere
+        err = np.abs(as_double(lse) - want["lse"])
+        assert (err <= (np.abs(want["lse"]) + 40) * 4 * 2.0 ** -24).all(), float(err.max())
