@@ -273,8 +273,8 @@ int kvssd_hip_memcpy_h2d_async(void* dst, const void* src, size_t bytes, void* s
  * (values i and i + rotary_dim / 2, or 2 i and 2 i + 1 where `interleaved`)
  * turns by p * frequencies[i] and is multiplied by `magnitude`; the other
  * values are left as they are.  `inverse` turns back (the rotation's
- * transpose).  Angles, sines and products are formed in 64 bits and rounded
- * once to the values' type. */
+ * transpose).  Angles, sines and products are formed in 64 bits and rounded to
+ * 32 bits, then to a 16-bit type. */
 typedef struct kvssd_rotary_spec {
   const double* frequencies; /* device, [rotary_dim / 2] */
   double magnitude;

@@ -15,7 +15,7 @@
 // which the vector units are busy 26 (a key's word ~200 instructions, 60 of them
 // 64-bit; a value's ~100); four tokens a workgroup take 2 us more.  A word loaded ahead of
 // the one that is coded changed nothing but the registers (35.3 and 35.9 us).
-// 4,097 tokens of 4 kv and 16 query heads of 64 in 32 bits into INT2: 13.9 us.
+// 4,097 tokens of 4 kv and 16 query heads of 64 in 32 bits into INT2: 13.9-15.2 us.
 // One token of each of 64 sequences: 6.2 us, four dependent reads.
 //  The rotated key is rounded to its type
 // first: the codes are those of a key rotated by kvssd_hip_rotary and quantised

@@ -10,8 +10,9 @@
 // from memory): INT4, 4 sequences of 131,000 to 262,144 tokens (795 MB) 162 us,
 // 4.9 TB/s of a plain read's 7.0; 64 ragged sequences up to 16,384 tokens (126 MB)
 // 48 us; one of 4,096 tokens 12.2 us, round trips and one stage; INT2, 16 sequences up
-// to 16,384, 64 query heads, this kernel alone 42 us, bound by its instructions (two
-// head tiles unpack every code twice).
+// to 16,384, 64 query heads, this kernel alone 45 us, bound by its instructions (two
+// head tiles unpack every code twice).  With 32-bit results, twice the products: 198,
+// 52 and 13.9 us.
 // A slot's codes of one head are half a line and its scales a sixteenth: waves that
 // drift apart fetch the same lines again, some from memory (the 795 MB: 197 us, and
 // a third more fetched; 524,288 tokens 132 us, 105 without the scales).  They meet
@@ -54,7 +55,7 @@
 //   slots, columns = (head, group), whose lanes are the weights' lanes; with two,
 //   the lanes of a head form the same scores twice.  (For four groups that form
 //   took 543 vector instructions a stage, this one 418: 524,288 slots in L2 111 and
-//   89 us.)
+//   89 us; 25 more in both since keys are centred.)
 // Softmax.  The running maximum is lazy: scores up to 2^6 above the reference are
 //   summed as they are (no wave-wide maximum per stage); where one exceeds that,
 //   all lanes take the new maximum and rescale.  The reference also holds the
@@ -294,8 +295,8 @@ __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirst
 
 // UNI: pages hold whole halves (32 slots) of a stage, rows whole 16-byte chunks
 // and a head's scales begin in a word alike in every row, so that a copy's rows
-// have one uniform base; else every lane finds its own row's address (64 ragged
-// sequences 33.4 and 37.3 us).
+// have one uniform base; else every lane finds its own row's address (whole passes
+// of the 64 ragged sequences 43.9 and 47.6 us, of the 795 MB 159 and 179).
 template <int BITS, int DP, int GP, bool PREC, bool UNI>
 __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(PagedDecodeParams p) {
   constexpr int kWaves = decode_waves(DP);

@@ -11,15 +11,19 @@
 // Attention does not depend on the slots' order (keys are rotated already),
 // and what is recent is read from the stored positions.
 //
-// Up to kOneSlots slots a sequence is one workgroup's, its weights and positions
-// in registers from one read: 64 sequences of 4,160 slots cut to 4,096 take
+// Where the page table has at most kOneSlots slots a sequence, used or not, a
+// sequence is one workgroup's, its weights and positions in registers from one
+// read: 64 sequences of 4,160 slots cut to 4,096 take
 // 17 us, moves included -- 0.9 until all is read, 0.5 for the latest position,
 // 2.1 + 1.3 + 1.3 for the digits (the first has few bins, and their counts meet),
 // 4.2 for ranks and lists, 3.7 for the moves' round trips, and the launch.  Longer
 // ones take a workgroup a chunk and a launch a step, each step's result found
 // again by every workgroup from the sequence's counts (8 KB): four sequences of
 // 65,545 to 131,072 slots cut to 16,384 take 40 us in six launches (425 us by one
-// workgroup each) and 27 for the moves, 122 MB at 4.6 TB/s.  Counts are integers,
+// workgroup each) and 27 for the moves, 122 MB at 4.6 TB/s.  The 64 sequences of
+// 4,160 slots take that way too where their table is wider: a call 17.0 us in a table
+// of 4,160 slots, 24.7 of 8,192, 48.6 of 8,256 and 79.6 of 131,072, over all of which
+// weights and positions are written.  Counts are integers,
 // so that the order in which atomics add them has no part in the result.
 #include "paged.hpp"
 

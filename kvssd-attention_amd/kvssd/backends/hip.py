@@ -233,7 +233,8 @@ class HipAttentionBackend:
         total_tokens: int = 0,
     ) -> PreparedPagedDecode:
         """Every check and plan of ``run_paged`` done once; calling the result with a query of that shape, dtype and
-        device decodes over the batch's arrays as they are at the call (what a decode loop repeats)."""
+        device decodes over the batch's arrays as they are at the call (what a decode loop repeats).  The results of up
+        to 64 calls (16 MB) are views of one allocation, which lives as long as any of them."""
         return PreparedPagedDecode(query, batch, sm_scale, out_dtype, accumulate, max_length, total_tokens)
 
     # ----------------------------------------------------------- merge ---

@@ -168,9 +168,11 @@ class PagedKVCache:
 
     Lengths and free pages are kept on the host (they follow from the calls, so that no call waits for the GPU),
     with a copy of the lengths on the device for the kernels.  ``track_weights`` keeps each slot's position and
-    summed attention weight, which :meth:`evict` needs.  One stream at a time: calls on different streams have to be
-    ordered by the caller.  :meth:`append` and :meth:`evict` change host state and so cannot be captured in a graph;
-    the operators under them can."""
+    summed attention weight, which :meth:`evict` needs: 8 bytes for each of the ``max_pages`` * ``page_tokens`` slots
+    that each sequence may grow to (``max_pages`` defaults to the whole pool), and a cut writes as many again.  From the
+    first cut on, positions differ from slots and are copied from the host at every append.  One stream at a time:
+    calls on different streams have to be ordered by the caller.  :meth:`append` and :meth:`evict` change host state and
+    so cannot be captured in a graph; the operators under them can."""
 
     def __init__(
         self,

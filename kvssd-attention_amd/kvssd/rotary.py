@@ -10,8 +10,8 @@ Pair i of a head -- values i and i + rotary_dim/2 (``layout="half"``) or 2i and
 2i + 1 (``"interleaved"``) -- is turned by the angle position * f_i and
 multiplied by the scaling's magnitude; values past ``rotary_dim`` stay.  Without
 scaling f_i = base^(-2i/rotary_dim).  Angles, sines and products have 64 bits,
-so that positions far past 32-bit angles' precision are exact; the result is
-rounded once to the values' type.
+so that positions far past 32-bit angles' precision keep theirs; the result is
+rounded to 32 bits and then, for 16-bit values, to their type.
 """
 
 from __future__ import annotations
