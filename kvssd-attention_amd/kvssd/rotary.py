@@ -131,17 +131,28 @@ def _share_elements(a: torch.Tensor, b: torch.Tensor) -> bool:
         ahead = (second - first) % (st * size)
         if reach <= ahead <= st * size - b_reach:
             return False
-    # the general case: no head of b may begin less than a head behind or before one of a
-    count = lambda m: torch.arange(m, device="cpu")  # noqa: E731
-    begins = [
-        (base + (count(t.shape[0])[:, None] * t.stride(0) + count(t.shape[1]) * t.stride(1)) * size).flatten()
-        for t, base in ((a, first), (b, second))
-    ]
-    begins[0] = begins[0].sort().values
-    at = torch.searchsorted(begins[0], begins[1])  # (begins[0][at - 1] < b <= begins[0][at])
-    last = begins[0].numel() - 1
-    behind = begins[1] - begins[0][(at - 1).clamp(min=0)] < d * size
-    before = begins[0][at.clamp(max=last)] - begins[1] < d * size
+    def heads_apart(t: torch.Tensor, first: int) -> torch.Tensor:
+        return first + torch.arange(t.shape[1], device="cpu") * (t.stride(1) * size)
+
+    # no head of b may begin less than a head (d values) before or behind one of a
+    begins, b_begins = heads_apart(a, first), heads_apart(b, second)
+    if st == bst or n == 1 or bn == 1:  # of each pair of heads, at the tokens where the two come closest
+        step = (bst if n == 1 else st) * size
+        ahead = b_begins - begins[:, None]
+        for extra in (0, 1):
+            tokens = (-ahead // step + extra).clamp(1 - n, bn - 1) if step else 0
+            if bool(((ahead + tokens * step).abs() < d * size).any()):
+                return True
+        return False
+    begins, b_begins = (
+        (torch.arange(t.shape[0], device="cpu")[:, None] * (t.stride(0) * size) + x).flatten()
+        for t, x in ((a, begins), (b, b_begins))
+    )
+    begins = begins.sort().values
+    at = torch.searchsorted(begins, b_begins)  # (begins[at - 1] < b_begins <= begins[at])
+    last = begins.numel() - 1
+    behind = b_begins - begins[(at - 1).clamp(min=0)] < d * size
+    before = begins[at.clamp(max=last)] - b_begins < d * size
     return bool(((at > 0) & behind).any() or ((at <= last) & before).any())
 
 
