@@ -54,9 +54,12 @@ class ReferenceAttentionBackend:
         sm_scale: float,
         out_dtype: torch.dtype | None = None,
         accumulate: bool = False,
+        max_length: int = 0,
+        total_tokens: int = 0,
     ) -> tuple[torch.Tensor, torch.Tensor]:
         """Attention of one query per sequence over its pages, sequence by sequence (what
-        HipAttentionBackend.run_paged computes); see there for the arguments."""
+        HipAttentionBackend.run_paged computes); see there for the arguments.  The hints have nothing to size here, and
+        weights are summed outside of any graph."""
         batch.validate()
         batch.validate_query(query)
         if accumulate and batch.weights is None:
@@ -86,7 +89,7 @@ class ReferenceAttentionBackend:
                 keys = keys * one.scales_k[0].float().repeat_interleave(batch.group_size, dim=-1)
                 grouped = query[b].float().reshape(keys.shape[1], -1, keys.shape[2])
                 scores = torch.matmul(grouped, keys.permute(1, 2, 0).contiguous()) * sm_scale
-                weights = torch.exp(scores - lse.reshape(*scores.shape[:2], 1)).sum((0, 1))
+                weights = torch.exp(scores - lse.reshape(*scores.shape[:2], 1)).sum((0, 1)).detach()
                 batch.weights[b, slots] += weights
         out = torch.stack(outs)
         return out.to(out_dtype or torch.float32), torch.stack(lses)

@@ -400,3 +400,12 @@ def test_a_cache_stays_on_the_gpu_that_was_current(monkeypatch):
         with pytest.raises(Stop):
             host_cache(device=device)
         assert made.pop() == torch.device(want)
+
+
+def test_the_portable_backend_takes_hints_and_keeps_weights_out_of_graphs():
+    batch, pool, table = small()
+    q = torch.from_numpy(np.random.default_rng(4).standard_normal((3, 4, 64))).float().requires_grad_()
+    out, _ = ReferenceAttentionBackend().run_paged(q, batch, 0.125, accumulate=True, max_length=33, total_tokens=53)
+    assert not batch.weights.requires_grad and batch.weights.sum().item() == pytest.approx(8.0, rel=1e-5)
+    out.sum().backward()  # (this backend has a backward pass)
+    assert torch.isfinite(q.grad).all() and (q.grad[1] == 0).all()
