@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define KVSSD_HIP_ABI_VERSION 6
+#define KVSSD_HIP_ABI_VERSION 7
 
 /* Query element types accepted by kvssd_hip_fused_decode (the reference
  * dispatches fp32/fp64/fp16/bf16 queries: csrc/fused_decode.cu:131-133). */
@@ -334,7 +334,9 @@ typedef struct kvssd_paged_cache {
  * dropped, and pages that are written may be named by one sequence only.
  * `query` (data NULL: none) is rotated by the same positions.  Tokens before
  * offsets[0] and from offsets[sequences] on are no sequence's: dropped, their
- * queries rotated as at position 0.
+ * queries rotated as at position 0.  With `parents` (int32 [tokens]) a
+ * sequence's tokens are a tree as in kvssd_hip_paged_tokens, and token i has
+ * position first_positions[b] (or lengths[b]) + its depth.
  * Where the cache has them, the new slots' weights become 0 and their
  * positions are stored.  lengths_out[b] = lengths[b] + count, at most the
  * table's capacity; it may be the cache's own lengths where offsets is NULL. */
@@ -343,6 +345,7 @@ typedef struct kvssd_paged_append_args {
   int64_t tokens;
   const int32_t* offsets;         /* [sequences + 1] or NULL */
   const int32_t* first_positions; /* [sequences] or NULL */
+  const int32_t* parents;         /* [tokens] or NULL */
   const kvssd_rotary_spec* rotary;
   int32_t* lengths_out; /* or NULL */
   int32_t dtype;        /* F16, BF16 or F32, of keys, values and query */
@@ -359,7 +362,8 @@ int kvssd_hip_paged_append(const kvssd_paged_cache* cache, const kvssd_paged_app
  * bytes a query head for every 64 slots (0: the table's capacity, for every
  * sequence); lengths beyond them are answered all the same.  fp32 outputs come from 32-bit-grade
  * arithmetic; 16-bit ones round the softmax weights times the value scales to
- * fp16. */
+ * fp16.  With window > 0 only the last `window` slots and the first `sink` take
+ * part (the others are not read); it does not go together with accumulate. */
 typedef struct kvssd_paged_decode_args {
   const void* query;
   void* out;
@@ -373,11 +377,70 @@ typedef struct kvssd_paged_decode_args {
   int32_t query_dtype;
   int32_t out_query_dtype;
   int32_t accumulate;
+  int32_t window; /* 0: every slot */
+  int32_t sink;
   int32_t reserved;
 } kvssd_paged_decode_args;
 int kvssd_hip_paged_decode_workspace_bytes(const kvssd_paged_cache* cache, const kvssd_paged_decode_args* args,
                                            size_t* bytes);
 int kvssd_hip_paged_decode(const kvssd_paged_cache* cache, const kvssd_paged_decode_args* args, void* stream);
+
+/* Attention of many new tokens a sequence over its slots, their own among
+ * them.  Token t of query [tokens, query_heads, head_dim] (F16, BF16 or F32)
+ * belongs to the sequence b with offsets[b] <= t < offsets[b+1]; its place
+ * i = t - offsets[b] is that of slot base + i, with n = offsets[b+1] -
+ * offsets[b] and base = lengths[b] - n: the tokens are the sequence's last n
+ * slots.  Without `parents` token i sees the slots up to its own, and slot t has
+ * position t.  With parents (int32 [tokens]) a sequence's tokens are a tree:
+ * token i is a child of its token parents[t], if that is 0 .. i-1, else of the
+ * slots before base; it sees those and its ancestors and itself, and has
+ * position base + depth (0 without a parent).  With window > 0 it sees of them
+ * only what lies above its position - window or below `sink`.
+ * out (fp32, or query_dtype with out_query_dtype = 1; [tokens, query_heads,
+ * head_dim], contiguous) and lse fp32 [tokens, query_heads]; a token that sees
+ * nothing, or of no sequence (before offsets[0], from offsets[sequences] on),
+ * gives out = 0 and lse = -inf.  max_length and total_tokens, of the lengths, size the split
+ * (0: the table's capacity, for every sequence); lengths beyond them are
+ * answered all the same.  Arithmetic as kvssd_hip_paged_decode's. */
+typedef struct kvssd_paged_tokens_args {
+  kvssd_heads query; /* query.out is not used */
+  void* out;
+  float* lse;
+  const int32_t* offsets; /* [sequences + 1] */
+  const int32_t* parents; /* [tokens] or NULL */
+  void* workspace; /* kvssd_hip_paged_tokens_workspace_bytes, 256-byte aligned */
+  size_t workspace_bytes;
+  double sm_scale;
+  int64_t tokens;
+  int64_t total_tokens;
+  int32_t max_length;
+  int32_t window; /* 0: everything */
+  int32_t sink;
+  int32_t query_dtype;
+  int32_t out_query_dtype;
+  int32_t reserved;
+} kvssd_paged_tokens_args;
+int kvssd_hip_paged_tokens_workspace_bytes(const kvssd_paged_cache* cache, const kvssd_paged_tokens_args* args,
+                                           size_t* bytes);
+int kvssd_hip_paged_tokens(const kvssd_paged_cache* cache, const kvssd_paged_tokens_args* args, void* stream);
+
+/* Keeps some of each sequence's last drafted[b] slots, the others are dropped:
+ * with base = lengths[b] - drafted[b] (clamped to [0, lengths[b]]), slot base + j
+ * takes the row (and weight and position, where the cache has them) of slot
+ * base + kept[b][j], and lengths_out[b] = base + m.  The list of a sequence is
+ * kept[b][0 .. m), which ends at the first entry that is not above the one
+ * before it or not within 0 .. drafted[b]-1, or at `width`.  Rows move in place:
+ * their pages may be named by no other sequence, and each of those slots has to
+ * lie in a page of the pool (a row without one does not move).  lengths_out may
+ * be the cache's own lengths. */
+typedef struct kvssd_paged_keep_args {
+  const int32_t* drafted; /* [sequences] */
+  const int32_t* kept;    /* [sequences, width] */
+  int32_t* lengths_out;
+  int32_t width;
+  int32_t reserved;
+} kvssd_paged_keep_args;
+int kvssd_hip_paged_keep(const kvssd_paged_cache* cache, const kvssd_paged_keep_args* args, void* stream);
 
 /* Cuts every sequence to at most `budget` slots.  Kept are, in this order, the
  * slots with a position below `sink` or above (largest position - recent), then

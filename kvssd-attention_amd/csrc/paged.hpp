@@ -38,6 +38,13 @@ __device__ __forceinline__ int paged_length(const int32_t* lengths, int b, int c
   return clamp_length(lengths[b], capacity);
 }
 
+// Parent of token i of a sequence's tree (whose entries begin at `parents`), -1 if it has none there: any entry that is
+// not an earlier token's.
+__device__ __forceinline__ int parent_of(const int32_t* parents, int i) {
+  const int up = parents[i];
+  return up < i ? max(up, -1) : -1;
+}
+
 // x of a lane before this one (0 where there is none): CTRL 0x110 + n, n lanes
 // before in the row of 16; 0x142 / 0x143, lane 15 of the row before / lane 31
 template <int CTRL, int ROWS>

@@ -37,6 +37,7 @@ struct AppendParams {
   double magnitude;
   const int32_t* offsets;
   const int32_t* first_positions;
+  const int32_t* parents;
   int32_t* lengths_out;
   RotaryShape shape;  // of the query's items
   int64_t tokens;
@@ -149,7 +150,12 @@ __global__ __launch_bounds__(kThreads, VEC ? 4 : 1) void paged_append_kernel(App
       const int64_t nth = p.offsets ? t - p.offsets[b] : 0;
       const int length = paged_length(c.lengths, b, p.capacity);
       const int64_t slot = length + nth;
-      const int64_t where = p.first_positions ? p.first_positions[b] + nth : slot;
+      int64_t where = (p.first_positions ? p.first_positions[b] : length) + nth;
+      if (p.parents && t >= nth) {  // the depth instead of nth
+        const int32_t* parents = p.parents + (t - nth);
+        where -= nth;
+        for (int up = parent_of(parents, static_cast<int>(nth)); up >= 0; up = parent_of(parents, up)) ++where;
+      }
       position = static_cast<double>(where);
       if (slot < p.capacity) {
         const int page = c.page_table[static_cast<int64_t>(b) * c.max_pages + slot / c.page_tokens];
@@ -283,6 +289,7 @@ int launch_paged_append(const kvssd_paged_cache& c, const kvssd_paged_append_arg
   p.query_heads = a.query.data ? a.query.heads : 0;
   p.offsets = a.offsets;
   p.first_positions = a.first_positions;
+  p.parents = a.parents;
   p.lengths_out = a.lengths_out;
   p.tokens = a.tokens;
   p.capacity = static_cast<int>(paged_capacity(c));

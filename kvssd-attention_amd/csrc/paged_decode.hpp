@@ -102,7 +102,21 @@ struct PagedDecodeParams {
   int groups;            // scale groups per head
   int group_log2;        // log2 of the group size
   float scale_log2;
+  int window, sink;      // window > 0: the last `window` slots and the first `sink` alone
 };
+
+// A window's sequence has stages that no slot is seen of, between the sinks' and the window's: they are left out, and
+// slots are counted without them from there on.  (Both borders are a stage's.)
+struct WindowGap {
+  int first;  // slot (and count) that the gap begins at; a multiple of kTile, as
+  int slots;  // the number of slots left out
+};
+__device__ __forceinline__ WindowGap window_gap(const PagedDecodeParams& p, int length) {
+  if (p.window == 0 || p.window >= length) return {0, 0};
+  const int seen = (length - p.window) / kTile * kTile;                // the window's first stage
+  const int first = min(seen, (min(p.sink, length) + kTile - 1) / kTile * kTile);  // (length is at most 2^30)
+  return {first, seen - first};
+}
 
 // Where the runs of a ragged batch lie.  Every sequence is cut into runs of the
 // same number of stages (its last may be shorter); run r of the batch is the
@@ -120,8 +134,10 @@ struct RunMap {
   int before;  // stages of the sequences before it, where scores are kept (as `length`)
 };
 
+// Slots of a sequence, without a window's gap
 __device__ __forceinline__ int length_of(const PagedDecodeParams& p, int seq) {
-  return seq < p.c.sequences ? paged_length(p.c.lengths, seq, p.capacity) : 0;
+  const int n = seq < p.c.sequences ? paged_length(p.c.lengths, seq, p.capacity) : 0;
+  return n - window_gap(p, n).slots;
 }
 // (`first`: the length of sequence `lane`, read once for all steps)
 __device__ __forceinline__ int tiles_of_runs(const PagedDecodeParams& p, int first) {
@@ -155,6 +171,7 @@ __device__ __forceinline__ RunMap find_run(const PagedDecodeParams& p, int r) {
     if (r < p.c.sequences) {
       m.seq = r;
       m.length = clamp_length(uniform_load(p.c.lengths + r), p.capacity);
+      m.length -= window_gap(p, m.length).slots;
       if (p.scores != nullptr) m.before = stages_before(p, r, first);
     }
     return m;
@@ -338,6 +355,14 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   const int length = scalar(map.length);
   const int begin = scalar(map.nth * map.tiles) * kTile;
   const int end = min(length, begin + scalar(map.tiles) * kTile);  // (at most 2^30 + 64 each)
+  // slot = count + gap.slots from gap.first on; of those, the window's begin at `seen`
+  WindowGap gap{0, 0};
+  int seen = 0;
+  if (p.window > 0) {
+    const int whole_length = clamp_length(uniform_load(c.lengths + seq), p.capacity);
+    gap = window_gap(p, whole_length);
+    seen = max(whole_length - p.window, 0);
+  }
   const int score_stage = scalar(map.before) + begin / kTile;  // where the run's scores lie, if they are kept
 
   const int d = c.head_dim;
@@ -371,12 +396,14 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   const bool chunked = row_bytes % 16 == 0;
   // The pages of the next stage's halves, fetched one stage before they are used
   int half_page = 0, half_off = 0;  // index into `pages`, slot within the page
-  if constexpr (UNI) {
-    half_page = scalar(begin / bt);
-    half_off = begin - half_page * bt;
-  }
+  auto seek = [&](int slot) {
+    half_page = scalar(slot / bt);
+    half_off = slot - half_page * bt;
+  };
+  if constexpr (UNI) seek(begin + (begin >= gap.first ? gap.slots : 0));
   int next_page[2] = {-1, -1}, next_off[2] = {0, 0};
   auto fetch_pages = [&](int base) {
+    if (gap.slots != 0 && base == gap.first) seek(base + gap.slots);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       next_page[h] = base + 32 * h < end ? uniform_load(pages + half_page) : -1;
@@ -400,6 +427,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   };
   auto locate = [&](int base) {
     Stage s;
+    const int first_slot = base + (base >= gap.first ? gap.slots : 0);
     if constexpr (UNI) {  // (an odd number of groups: of an even number of kv heads)
       const int left = end - base;
       s.live = left >= kTile ? ~0ull : (1ull << left) - 1;
@@ -409,12 +437,16 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
         s.row[h] = ok ? next_page[h] * bt + next_off[h] : 0;
         if (!ok) s.live &= h ? 0xFFFFFFFFull : 0xFFFFFFFF00000000ull;
       }
+      if (first_slot < seen) {
+        const int out = seen - first_slot, sinks = p.sink - first_slot;
+        s.live &= (out >= kTile ? 0ull : ~0ull << out) | (sinks <= 0 ? 0ull : sinks >= kTile ? ~0ull : (1ull << sinks) - 1);
+      }
       fetch_pages(base + kTile);
       s.odd = p.groups & kvh & 1 ? ~0ull : 0;
     } else {
-      const int slot = base + lane;
+      const int slot = first_slot + lane;
       int mine = -1;
-      if (slot < end) {
+      if (base + lane < end && (slot >= seen || slot < p.sink)) {
         const int page = pages[slot / bt];
         if (page >= 0 && page < c.num_pages) mine = page * bt + slot % bt;
       }

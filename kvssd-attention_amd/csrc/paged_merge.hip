@@ -208,6 +208,8 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, Plan* 
   if (!paged_dtype(a.query_dtype)) return arg_error("unsupported query dtype");
   if (a.out_query_dtype != 0 && a.out_query_dtype != 1) return arg_error("out_query_dtype must be 0 or 1");
   if (a.max_length < 0 || a.total_tokens < 0) return arg_error("max_length and total_tokens must be >= 0");
+  if (a.window < 0 || a.sink < 0) return arg_error("window and sink must be >= 0");
+  if (a.window > 0 && a.accumulate) return arg_error("weights are summed over whole sequences, not over a window");
   if (a.accumulate && !c.weights) return arg_error("accumulate needs a cache with weights");
   PagedDecodeParams& p = out->p;
   p = PagedDecodeParams{};
@@ -222,6 +224,8 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, Plan* 
   p.out_dtype = a.out_query_dtype ? a.query_dtype : KVSSD_DTYPE_F32;
   p.scale_log2 = static_cast<float>(a.sm_scale) * kLog2e;
   p.groups = c.head_dim / c.group_size;
+  p.window = a.window;
+  p.sink = a.sink;
   while (out->gp < p.groups) out->gp *= 2;
   const int heads = 16 / out->gp;
   p.tiles = (p.gq + heads - 1) / heads;
@@ -235,7 +239,11 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_decode_args& a, Plan* 
   while ((1 << p.group_log2) < c.group_size) ++p.group_log2;
 
   auto tiles_of = [](int64_t n) { return (n + kTile - 1) / kTile; };
-  const int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
+  int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
+  if (a.window > 0) {  // the window's stages and the sinks'
+    const int64_t seen = (tiles_of(a.window) + 1 + tiles_of(a.sink)) * kTile;
+    longest = longest < seen ? longest : seen;
+  }
   if (tiles_of(p.capacity) * c.sequences >= int64_t{1} << 31) return arg_error("sequences * capacity is past 2^37 slots");
   int64_t all = tiles_of(longest) * c.sequences;  // stages to be worked on
   if (a.total_tokens > 0 && a.total_tokens / kTile + c.sequences < all) all = a.total_tokens / kTile + c.sequences;

@@ -8,7 +8,7 @@ package's own.
 from .attention import packed_attention, reference_attention
 from .backends import available_attention_backends, resolve_attention_backend
 from .format import CacheSpec
-from .paged import PagedKVCache, append_tokens, evict_tokens
+from .paged import PagedKVCache, append_tokens, evict_tokens, keep_tokens
 from .pipeline import KVSSDPipeline
 from .quant import dequantize_tensor, quantize_tensor
 from .rotary import Rotary, RotaryScaling
@@ -28,6 +28,7 @@ __all__ = [
     "append_tokens",
     "dequantize_tensor",
     "evict_tokens",
+    "keep_tokens",
     "available_attention_backends",
     "available_storage_backends",
     "packed_attention",

@@ -23,7 +23,7 @@ LIB_PATH = Path(os.environ.get("KVSSD_HIP_LIBRARY") or Path(__file__).resolve().
 LIB_PATH_OVERRIDDEN = bool(os.environ.get("KVSSD_HIP_LIBRARY"))
 # the sources the in-tree build comes from (absent in an installed copy)
 BUILD_SCRIPT = Path(__file__).resolve().parent.parent / "csrc" / "build.py"
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_F64 = 0, 1, 2, 3
 KERNEL_AUTO, KERNEL_GENERAL, KERNEL_MFMA, KERNEL_STAGED = 0, 1, 2, 3
@@ -101,7 +101,7 @@ class PagedAppendArgs(ctypes.Structure):
 
     _fields_ = [
         ("keys", Heads), ("values", Heads), ("query", Heads), ("tokens", _LL), ("offsets", _P),
-        ("first_positions", _P), ("rotary", ctypes.POINTER(RotarySpec)), ("lengths_out", _P), ("dtype", _I32),
+        ("first_positions", _P), ("parents", _P), ("rotary", ctypes.POINTER(RotarySpec)), ("lengths_out", _P), ("dtype", _I32),
         ("reserved", _I32),
     ]
 
@@ -112,7 +112,25 @@ class PagedDecodeArgs(ctypes.Structure):
     _fields_ = [
         ("query", _P), ("out", _P), ("lse", _P), ("workspace", _P), ("workspace_bytes", ctypes.c_size_t),
         ("sm_scale", ctypes.c_double), ("total_tokens", _LL),
-    ] + [(n, _I32) for n in ("max_length", "query_heads", "query_dtype", "out_query_dtype", "accumulate", "reserved")]
+    ] + [
+        (n, _I32)
+        for n in ("max_length", "query_heads", "query_dtype", "out_query_dtype", "accumulate", "window", "sink", "reserved")
+    ]
+
+
+class PagedTokensArgs(ctypes.Structure):
+    """kvssd_paged_tokens_args."""
+
+    _fields_ = [
+        ("query", Heads), ("out", _P), ("lse", _P), ("offsets", _P), ("parents", _P), ("workspace", _P),
+        ("workspace_bytes", ctypes.c_size_t), ("sm_scale", ctypes.c_double), ("tokens", _LL), ("total_tokens", _LL),
+    ] + [(n, _I32) for n in ("max_length", "window", "sink", "query_dtype", "out_query_dtype", "reserved")]
+
+
+class PagedKeepArgs(ctypes.Structure):
+    """kvssd_paged_keep_args."""
+
+    _fields_ = [("drafted", _P), ("kept", _P), ("lengths_out", _P), ("width", _I32), ("reserved", _I32)]
 
 
 class PagedEvictArgs(ctypes.Structure):
@@ -153,6 +171,9 @@ SIGNATURES = {
     "kvssd_hip_paged_append": (_I, [_VP, _VP, _VP]),
     "kvssd_hip_paged_decode_workspace_bytes": (_I, [_VP, _VP, ctypes.POINTER(_SZ)]),
     "kvssd_hip_paged_decode": (_I, [_VP, _VP, _VP]),
+    "kvssd_hip_paged_tokens_workspace_bytes": (_I, [_VP, _VP, ctypes.POINTER(_SZ)]),
+    "kvssd_hip_paged_tokens": (_I, [_VP, _VP, _VP]),
+    "kvssd_hip_paged_keep": (_I, [_VP, _VP, _VP]),
     "kvssd_hip_paged_evict_workspace_bytes": (_I, [_VP, _VP, ctypes.POINTER(_SZ)]),
     "kvssd_hip_paged_evict": (_I, [_VP, _VP, _VP]),
     "kvssd_hip_read_probe": (_I, [_VP, _SZ, _VP, _SZ, _VP]),

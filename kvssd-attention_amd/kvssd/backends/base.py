@@ -154,6 +154,33 @@ class PagedBatch:
         if query.device != self.packed_k.device:
             raise ValueError("query and paged cache must share a device")
 
+    def validate_tokens(self, query: torch.Tensor) -> None:
+        """Of a query with many tokens a sequence."""
+        if query.ndim != 3:
+            raise ValueError("query must be [tokens, query_heads, head_dim]")
+        if query.shape[2] != self.head_dim:
+            raise ValueError("packed dimension does not match query head dimension")
+        if query.shape[1] == 0 or query.shape[1] % self.packed_k.shape[2]:
+            raise ValueError("query heads must be divisible by KV heads")
+        if query.device != self.packed_k.device:
+            raise ValueError("query and paged cache must share a device")
+
+    def validate_lists(self, tokens: int, offsets: torch.Tensor, parents: torch.Tensor | None) -> None:
+        """Of the sequences' places among ``tokens`` tokens and the tokens' parents."""
+        for name, t, count in (("offsets", offsets, self.lengths.shape[0] + 1), ("parents", parents, tokens)):
+            if t is None:
+                continue
+            if t.dtype != torch.int32 or t.shape != (count,) or t.device != self.lengths.device:
+                raise ValueError(f"{name} must be int32 [{count}] on {self.lengths.device}")
+
+    def validate_visible(self, window: int, sink: int, accumulate: bool = False) -> None:
+        if window < 0 or sink < 0:
+            raise ValueError("window and sink must be >= 0")
+        if window and accumulate:
+            raise ValueError("weights are summed over whole sequences, not over a window")
+        if accumulate and self.weights is None:
+            raise ValueError("accumulate needs a cache with weights")
+
 
 @runtime_checkable
 class AttentionBackend(Protocol):

@@ -24,7 +24,7 @@ import torch
 
 from .. import _native
 from .base import BackendAvailability, PackedBatch, PagedBatch
-from .paged import PreparedPagedDecode
+from .paged import PreparedPagedDecode, PreparedPagedTokens
 
 _device_state: dict[int, tuple[bool, str]] = {}
 
@@ -212,6 +212,8 @@ class HipAttentionBackend:
         accumulate: bool = False,
         max_length: int = 0,
         total_tokens: int = 0,
+        window: int = 0,
+        sink: int = 0,
     ) -> tuple[torch.Tensor, torch.Tensor]:
         """Attention of one query per sequence, [sequences, query_heads, head_dim], over its pages: (out, lse).
 
@@ -219,8 +221,14 @@ class HipAttentionBackend:
         lse = -inf.  ``accumulate`` adds each slot's attention weight, summed over the query heads, to
         ``batch.weights``.  ``max_length`` and ``total_tokens``, the longest length and their sum where the caller
         knows them (0: the page table's capacity), size the split over the sequences and, with ``accumulate``, the
-        workspace (4 bytes a slot and query head); lengths past them are answered too, their weights more slowly."""
-        return PreparedPagedDecode(query, batch, sm_scale, out_dtype, accumulate, max_length, total_tokens, rows=1)(query)
+        workspace (4 bytes a slot and query head); lengths past them are answered too, their weights more slowly.
+
+        With ``window`` > 0 the query sees its sequence's last ``window`` slots and the first ``sink`` alone, and no
+        others are read (pages that hold none of them may be gone from the table).  It does not go together with
+        ``accumulate``."""
+        return PreparedPagedDecode(
+            query, batch, sm_scale, out_dtype, accumulate, max_length, total_tokens, window, sink, rows=1
+        )(query)
 
     def prepare_paged(
         self,
@@ -231,11 +239,62 @@ class HipAttentionBackend:
         accumulate: bool = False,
         max_length: int = 0,
         total_tokens: int = 0,
+        window: int = 0,
+        sink: int = 0,
     ) -> PreparedPagedDecode:
         """Every check and plan of ``run_paged`` done once; calling the result with a query of that shape, dtype and
         device decodes over the batch's arrays as they are at the call (what a decode loop repeats).  The results of up
         to 64 calls (16 MB) are views of one allocation, which lives as long as any of them."""
-        return PreparedPagedDecode(query, batch, sm_scale, out_dtype, accumulate, max_length, total_tokens)
+        return PreparedPagedDecode(query, batch, sm_scale, out_dtype, accumulate, max_length, total_tokens, window, sink)
+
+    def run_paged_tokens(
+        self,
+        query: torch.Tensor,
+        batch: PagedBatch,
+        sm_scale: float,
+        offsets: torch.Tensor,
+        parents: torch.Tensor | None = None,
+        *,
+        window: int = 0,
+        sink: int = 0,
+        out_dtype: torch.dtype | None = None,
+        max_length: int = 0,
+        total_tokens: int = 0,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """Attention of many new tokens a sequence over its pages, their own among them: (out, lse).
+
+        Tokens offsets[b] .. offsets[b+1]-1 (int32 [sequences + 1]) of ``query`` [tokens, query_heads, head_dim] are
+        those of sequence b's last slots, whose keys and values are in the cache (``append_tokens``) and which
+        ``batch.lengths`` counts.  Without ``parents`` a token sees the slots up to its own, as in a prompt or a chunk
+        of one.  With ``parents`` (int32 [tokens]) a sequence's tokens are a tree: parents[t] is the place of token t's
+        parent among the sequence's tokens, which has to come before it; any other number makes t a child of the slots
+        before all of them.  A token sees those slots, its ancestors and itself, and its position is that of its depth.
+
+        With ``window`` > 0 a token sees of these only positions above its own - ``window``, and those below ``sink``;
+        slots that no token sees are not read.  Positions are the slots' numbers but for a tree's tokens.
+
+        ``out`` is [tokens, query_heads, head_dim], fp32 unless ``out_dtype`` is the query's dtype; a token that sees
+        nothing, or belongs to no sequence, gives out = 0 and lse = -inf.  ``max_length`` and ``total_tokens`` (of the
+        lengths, as in ``run_paged``) size the split.  The query may have any token and head strides."""
+        return PreparedPagedTokens(query, batch, sm_scale, out_dtype, window, sink, max_length, total_tokens, rows=1)(
+            query, offsets, parents
+        )
+
+    def prepare_paged_tokens(
+        self,
+        query: torch.Tensor,
+        batch: PagedBatch,
+        sm_scale: float,
+        *,
+        window: int = 0,
+        sink: int = 0,
+        out_dtype: torch.dtype | None = None,
+        max_length: int = 0,
+        total_tokens: int = 0,
+    ) -> PreparedPagedTokens:
+        """Every check and plan of ``run_paged_tokens`` done once, for a query of that shape: the result is called with
+        (query, offsets, parents or None); see ``prepare_paged``."""
+        return PreparedPagedTokens(query, batch, sm_scale, out_dtype, window, sink, max_length, total_tokens)
 
     # ----------------------------------------------------------- merge ---
     def merge_chunks(

@@ -1,7 +1,9 @@
 """One decode shape over a paged cache, its checks done once.
 
-Used by ``HipAttentionBackend.prepare_paged`` / ``run_paged``; as the prepared
-decode of a packed batch (``hip.py``), for batches of sequences in pages.
+Used by ``HipAttentionBackend.prepare_paged`` / ``run_paged`` (one token a
+sequence) and ``prepare_paged_tokens`` / ``run_paged_tokens`` (many); as the
+prepared decode of a packed batch (``hip.py``), for batches of sequences in
+pages.
 """
 
 from __future__ import annotations
@@ -40,9 +42,23 @@ class PreparedPagedDecode:
 
     _MAX_SLOTS = 8
 
-    def __init__(self, query, batch: PagedBatch, sm_scale, out_dtype, accumulate, max_length, total_tokens, rows=64):
+    def __init__(
+        self, query, batch: PagedBatch, sm_scale, out_dtype, accumulate, max_length, total_tokens, window=0, sink=0, rows=64
+    ):
         batch.validate()
         batch.validate_query(query)
+        batch.validate_visible(window, sink, accumulate)
+        self._check(query, out_dtype, max_length, total_tokens)
+        self._keep(query, batch, out_dtype)
+        self._args = _native.PagedDecodeArgs(
+            None, None, None, None, 0, float(sm_scale), int(total_tokens), int(min(max_length, 2**31 - 1)),
+            query.shape[1], _native.QUERY_DTYPES[query.dtype], int(self._out_dtype != torch.float32), int(accumulate),
+            min(window, 2**31 - 1), min(sink, 2**31 - 1), 0,
+        )
+        self._plan("kvssd_hip_paged_decode", query, rows)
+
+    @staticmethod
+    def _check(query, out_dtype, max_length, total_tokens) -> None:
         if query.device.type != "cuda":
             raise ValueError(f"HIP backend requires ROCm GPU tensors, got {query.device.type}")
         if query.dtype not in (torch.float16, torch.bfloat16, torch.float32):
@@ -51,8 +67,8 @@ class PreparedPagedDecode:
             raise ValueError(f"out_dtype must be torch.float32 or the query's dtype {query.dtype}, got {out_dtype}")
         if max_length < 0 or total_tokens < 0:
             raise ValueError("max_length and total_tokens must be >= 0")
-        if accumulate and batch.weights is None:
-            raise ValueError("accumulate needs a cache with weights")
+
+    def _keep(self, query, batch: PagedBatch, out_dtype) -> None:
         self._batch = batch  # keeps the arrays alive
         self._device = query.device
         self._index = query.device.index if query.device.index is not None else torch.cuda.current_device()
@@ -60,26 +76,24 @@ class PreparedPagedDecode:
         self._out_dtype = torch.float32 if out_dtype is None else out_dtype
         self._cache = native_cache(batch)
         self._cache_addr = ctypes.addressof(self._cache)
-        self._args = _native.PagedDecodeArgs(
-            None, None, None, None, 0, float(sm_scale), int(total_tokens), int(min(max_length, 2**31 - 1)),
-            query.shape[1], _native.QUERY_DTYPES[query.dtype], int(self._out_dtype != torch.float32), int(accumulate), 0,
-        )
+
+    def _plan(self, entry: str, query, rows: int) -> None:
         lib = _native.load()
         need = ctypes.c_size_t(0)
+        plan = getattr(lib, entry + "_workspace_bytes")
         _native.check(
-            lib.kvssd_hip_paged_decode_workspace_bytes(self._cache_addr, ctypes.addressof(self._args), ctypes.byref(need)),
-            "kvssd_hip_paged_decode_workspace_bytes",
+            plan(self._cache_addr, ctypes.addressof(self._args), ctypes.byref(need)), entry + "_workspace_bytes"
         )
         self._need = int(need.value)
-        self._fn = lib.kvssd_hip_paged_decode
+        self._entry, self._fn = entry, getattr(lib, entry)
         out_bytes = query.numel() * self._out_dtype.itemsize + 4 * query.shape[0] * query.shape[1]
-        self._rows = max(1, min(rows, _BLOCK_BYTES // out_bytes))
+        self._rows = max(1, min(rows, _BLOCK_BYTES // max(out_bytes, 1)))
         # (stream, thread): [args, its address, next row, outs, lses, workspace]
         self._slots: dict[tuple[int, int], list] = {}
 
     def _slot(self, old: list | None, rows: int) -> list:
         if old is None:
-            args = _native.PagedDecodeArgs.from_buffer_copy(self._args)
+            args = type(self._args).from_buffer_copy(self._args)
             work = torch.empty((max(self._need, 1),), dtype=torch.uint8, device=self._device)
             args.workspace, args.workspace_bytes = work.data_ptr(), work.numel()
         else:
@@ -88,21 +102,24 @@ class PreparedPagedDecode:
         lses = torch.empty((rows, *self._qsize[:2]), dtype=torch.float32, device=self._device).unbind(0)
         return [args, ctypes.addressof(args), 0, outs, lses, work]
 
-    def __call__(self, query: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    def _match(self, query: torch.Tensor) -> None:
         if query.dtype is not self._qdtype or query.shape != self._qsize or query.get_device() != self._index:
             raise ValueError(
                 f"query {tuple(query.shape)} {query.dtype} on {query.device} does not match the prepared decode "
                 f"({tuple(self._qsize)} {self._qdtype} on {self._device})"
             )
         refuse_grad(query)
+
+    def __call__(self, query: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        self._match(query)
         if not query.is_contiguous() or query.data_ptr() % 16:  # the kernel reads 16 bytes at a time
             query = query.clone(memory_format=torch.contiguous_format)
         if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self._index):
-                return self._launch(query)
-        return self._launch(query)
+                return self._launch(query.data_ptr())
+        return self._launch(query.data_ptr())
 
-    def _launch(self, query: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    def _launch(self, query, *lists: int | None) -> tuple[torch.Tensor, torch.Tensor]:
         from .hip import current_stream_handle
 
         handle = current_stream_handle(self._index)
@@ -118,8 +135,47 @@ class PreparedPagedDecode:
         row = slot[2]
         slot[2] = row + 1
         args, out, lse = slot[0], slot[3][row], slot[4][row]
-        args.query, args.out, args.lse = query.data_ptr(), out.data_ptr(), lse.data_ptr()
+        args.query, args.out, args.lse = query, out.data_ptr(), lse.data_ptr()
+        if lists:
+            args.offsets, args.parents = lists
         rc = self._fn(self._cache_addr, slot[1], handle)
         if rc:
-            _native.check(rc, "kvssd_hip_paged_decode")
+            _native.check(rc, self._entry)
         return out, lse
+
+
+class PreparedPagedTokens(PreparedPagedDecode):
+    """As PreparedPagedDecode for many new tokens a sequence: calling it with a query [tokens, query_heads, head_dim] of
+    the prepared shape (any token and head strides), the sequences' ``offsets`` in it and, for trees, the tokens'
+    ``parents`` returns a fresh (out, lse).  Workspaces and outputs as there."""
+
+    def __init__(self, query, batch: PagedBatch, sm_scale, out_dtype, window, sink, max_length, total_tokens, rows=64):
+        batch.validate()
+        batch.validate_tokens(query)
+        batch.validate_visible(window, sink)
+        self._check(query, out_dtype, max_length, total_tokens)
+        self._keep(query, batch, out_dtype)
+        heads = _native.Heads(None, None, 0, 0, 0, 0, query.shape[1], 0)
+        self._args = _native.PagedTokensArgs(
+            heads, None, None, None, None, None, 0, float(sm_scale), query.shape[0], int(total_tokens),
+            int(min(max_length, 2**31 - 1)), min(window, 2**31 - 1), min(sink, 2**31 - 1),
+            _native.QUERY_DTYPES[query.dtype], int(self._out_dtype != torch.float32), 0,
+        )
+        self._plan("kvssd_hip_paged_tokens", query, rows)
+
+    def __call__(
+        self, query: torch.Tensor, offsets: torch.Tensor, parents: torch.Tensor | None = None
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        self._match(query)
+        self._batch.validate_lists(query.shape[0], offsets, parents)
+        if query.stride(2) != 1:
+            query = query.contiguous()
+        offsets = offsets if offsets.is_contiguous() else offsets.contiguous()
+        if parents is not None and not parents.is_contiguous():
+            parents = parents.contiguous()
+        heads = _native.Heads(query.data_ptr(), None, query.stride(0), query.stride(1), 0, 0, query.shape[1], 0)
+        lists = offsets.data_ptr(), None if parents is None else parents.data_ptr()
+        if torch._C._cuda_getDevice() != self._index:
+            with torch.cuda.device(self._index):
+                return self._launch(heads, *lists)
+        return self._launch(heads, *lists)

@@ -8,9 +8,15 @@ holds many sequences:
   quantised by the framework's codec into their sequences' pages;
 * ``HipAttentionBackend.run_paged`` / ``prepare_paged`` -- one new token's
   attention per sequence, optionally summing each slot's attention weight;
+* ``run_paged_tokens`` / ``prepare_paged_tokens`` -- attention of many new tokens
+  a sequence: prompts, chunks of prompts, trees of drafted tokens;
+* :func:`keep_tokens` -- the accepted ones of a sequence's drafted tokens moved
+  together, the others dropped;
 * :func:`evict_tokens` -- every sequence cut to a budget of slots by that sum;
 * :class:`PagedKVCache` -- the pool, its free pages, the sequences' lengths and
-  positions, and the three operators over them.
+  positions, and these operators over them.
+
+Attention takes a sliding window and a few first tokens that stay visible.
 
 The functions launch on the current stream and never wait for the GPU.
 """
@@ -52,6 +58,7 @@ def append_tokens(
     query: torch.Tensor | None = None,
     first_positions: torch.Tensor | None = None,
     lengths_out: torch.Tensor | None = None,
+    parents: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor]:
     """Write new tokens behind their sequences' slots: (rotated query or None, new lengths).
 
@@ -64,6 +71,10 @@ def append_tokens(
     query_heads, head_dim], if given.  Where the batch has them, the slots' positions are stored and their weights set
     to 0.  Tokens of no sequence (before offsets[0], from offsets[sequences] on) are dropped, their queries turned as
     at position 0.
+
+    With ``parents`` (int32 [tokens]) a sequence's new tokens are a tree, as ``run_paged_tokens`` takes it: the i-th
+    goes to its slot all the same, and its position is the first's plus its depth (0 of a token whose parent is none of
+    the sequence's earlier new tokens).
 
     ``batch.lengths`` stays as it is unless it is passed as ``lengths_out`` (one token a sequence only); by default
     the new lengths are a new tensor."""
@@ -94,6 +105,8 @@ def append_tokens(
         raise ValueError("without offsets there is one token a sequence")
     if first_positions is not None:
         first_positions = _int32(first_positions, "first_positions", sequences, device)
+    if parents is not None:
+        parents = _int32(parents, "parents", tokens, device)
     if lengths_out is None:
         lengths_out = torch.empty_like(batch.lengths)
     elif _int32(lengths_out, "lengths_out", sequences, device) is not lengths_out:
@@ -108,6 +121,7 @@ def append_tokens(
     args = _native.PagedAppendArgs(
         heads_of(keys), heads_of(values), turns, tokens, None if offsets is None else offsets.data_ptr(),
         None if first_positions is None else first_positions.data_ptr(),
+        None if parents is None else parents.data_ptr(),
         None if rotary is None else ctypes.pointer(rotary.spec()), lengths_out.data_ptr(), _DTYPES[dtype], 0,
     )
     cache = native_cache(batch)
@@ -162,6 +176,41 @@ def evict_tokens(
     return lengths, weights, positions
 
 
+def keep_tokens(
+    batch: PagedBatch, drafted: torch.Tensor, kept: torch.Tensor, *, lengths_out: torch.Tensor | None = None
+) -> torch.Tensor:
+    """Keep some of each sequence's last ``drafted`` (int32 [sequences]) slots and drop the others: the new lengths.
+
+    ``kept`` (int32 [sequences, width]) lists the kept ones' places among them, ascending; a sequence's list ends at the
+    first entry that is not above the one before it or not a drafted token's (-1, say).  With base = length - drafted,
+    slot base + j takes the row of slot base + kept[b, j], and its weight and position where the cache has them; the new
+    length is base plus the list's.  Rows move in place, within the sequence's pages (which no other sequence may name),
+    and each of those slots has to lie in a page of the pool: a row without one does not move.
+
+    ``batch.lengths`` stays as it is unless it is passed as ``lengths_out``; by default the new lengths are a new
+    tensor."""
+    batch.validate()
+    index = _gpu_index(batch)
+    device, sequences = batch.packed_k.device, batch.lengths.shape[0]
+    drafted = _int32(drafted, "drafted", sequences, device)
+    if kept.dtype != torch.int32 or kept.ndim != 2 or kept.shape[0] != sequences or kept.device != device:
+        raise ValueError(f"kept must be int32 [{sequences}, width] on {device}")
+    kept = kept if kept.is_contiguous() else kept.contiguous()
+    if lengths_out is None:
+        lengths_out = torch.empty_like(batch.lengths)
+    elif _int32(lengths_out, "lengths_out", sequences, device) is not lengths_out:
+        raise ValueError("lengths_out must be contiguous")
+    args = _native.PagedKeepArgs(drafted.data_ptr(), kept.data_ptr(), lengths_out.data_ptr(), kept.shape[1], 0)
+    cache = native_cache(batch)
+    with on_device(index):
+        rc = _native.load().kvssd_hip_paged_keep(
+            ctypes.addressof(cache), ctypes.addressof(args), current_stream_handle(index)
+        )
+    if rc:
+        _native.check(rc, "kvssd_hip_paged_keep")
+    return lengths_out
+
+
 class PagedKVCache:
     """The packed cache of one layer for up to ``sequences`` sequences at a time, in pages that they take from a
     common pool as they grow and give back as they are cut or end.
@@ -171,8 +220,12 @@ class PagedKVCache:
     summed attention weight, which :meth:`evict` needs: 8 bytes for each of the ``max_pages`` * ``page_tokens`` slots
     that each sequence may grow to (``max_pages`` defaults to the whole pool), and a cut writes as many again.  From the
     first cut on, positions differ from slots and are copied from the host at every append.  One stream at a time:
-    calls on different streams have to be ordered by the caller.  :meth:`append` and :meth:`evict` change host state and
-    so cannot be captured in a graph; the operators under them can."""
+    calls on different streams have to be ordered by the caller.  :meth:`append`, :meth:`keep` and :meth:`evict` change
+    host state and so cannot be captured in a graph; the operators under them can.
+
+    A step with drafted tokens is :meth:`append` with their ``parents``, :meth:`attend_tokens` with the same, and
+    :meth:`keep` with each sequence's accepted path; until then the cache holds all of them, and only those calls and
+    :meth:`clear` are taken."""
 
     def __init__(
         self,
@@ -223,6 +276,10 @@ class PagedKVCache:
         self.lengths = [0] * sequences  # slots in use, per sequence
         self.next_positions = [0] * sequences  # position of the next token, per sequence
         self._plan: tuple | None = None  # of `attend`: what it was planned for, and the prepared decode
+        self._tokens_plan: tuple | None = None  # of `attend_tokens`, the same
+        # the last append's tokens of each sequence, while they can be kept in part, and whether they are a tree
+        self._latest: list[int] | None = None
+        self._drafting = False
 
     @property
     def free_pages(self) -> int:
@@ -263,6 +320,10 @@ class PagedKVCache:
             else:
                 self.batch.page_table[self._host_to_device(rows).long()] = self._host_to_device(table)
 
+    def _no_drafts(self) -> None:
+        if self._drafting:
+            raise RuntimeError("the cache holds drafted tokens; keep those that are accepted first")
+
     def append(
         self,
         keys: torch.Tensor,
@@ -271,9 +332,14 @@ class PagedKVCache:
         *,
         rotary: Rotary | None = None,
         query: torch.Tensor | None = None,
+        parents: torch.Tensor | Sequence[int] | None = None,
     ) -> torch.Tensor | None:
         """Append counts[b] tokens to sequence b (default: one to each), as they lie in ``keys`` and ``values``
-        [tokens, kv_heads, head_dim], sequence after sequence; returns the rotated query, if one was given."""
+        [tokens, kv_heads, head_dim], sequence after sequence; returns the rotated query, if one was given.
+
+        ``parents`` [tokens] (int32 on the cache's device, or numbers) makes each sequence's tokens a tree of drafted
+        ones (see :func:`append_tokens`), of which :meth:`keep` has to take those that are accepted next."""
+        self._no_drafts()
         one = counts is None
         counts = [1] * self.sequences if one else [int(n) for n in counts]
         if len(counts) != self.sequences or min(counts) < 0:
@@ -290,12 +356,15 @@ class PagedKVCache:
         first = None
         if self.next_positions != self.lengths:
             first = self._host_to_device(self.next_positions)
+        drafting = parents is not None
+        if drafting:
+            parents = self._parents(parents, keys.shape[0])
         held = list(self.lengths)
         self._resize(after)
         try:
             turned, lengths = append_tokens(
                 self.batch, keys, values, offsets=offsets, rotary=rotary, query=query, first_positions=first,
-                lengths_out=self.batch.lengths if offsets is None else None,
+                lengths_out=self.batch.lengths if offsets is None else None, parents=parents,
             )
         except Exception:
             self._resize(held)
@@ -304,7 +373,43 @@ class PagedKVCache:
             self.batch.lengths.copy_(lengths)
         self.lengths = after
         self.next_positions = [n + more for n, more in zip(self.next_positions, counts)]
+        self._latest, self._drafting = counts, drafting
         return turned
+
+    def _parents(self, parents: torch.Tensor | Sequence[int], tokens: int) -> torch.Tensor:
+        if not isinstance(parents, torch.Tensor):
+            parents = [int(x) for x in parents]
+            if len(parents) != tokens:
+                raise ValueError("parents must hold one number per token")
+            parents = self._host_to_device([x if -1 <= x < tokens else -1 for x in parents])
+        return parents
+
+    def keep(self, paths: Sequence[Sequence[int] | None]) -> None:
+        """Of the last append's tokens, keep paths[b] of sequence b -- their places among its tokens, ascending; of a
+        tree, a path from one without a parent down -- and drop the others (:func:`keep_tokens`); pages behind are given
+        back.  None keeps all, of a sequence whose tokens are no tree."""
+        counts = self._latest
+        if counts is None:
+            raise RuntimeError("there are no tokens to choose from: keep follows an append")
+        if len(paths) != self.sequences:
+            raise ValueError("paths must hold one list (or None) per sequence")
+        chosen = []
+        for path, n in zip(paths, counts):
+            if path is None and self._drafting and n > 1:
+                raise ValueError("a tree's tokens are kept by their path")
+            path = list(range(n)) if path is None else [int(x) for x in path]
+            if any(not 0 <= x < n for x in path) or any(a >= b for a, b in zip(path, path[1:])):
+                raise ValueError("a path must hold ascending places among the sequence's new tokens")
+            chosen.append(path)
+        width = max(len(path) for path in chosen)
+        drafted = self._host_to_device(counts)
+        kept = self._host_to_device([path + [-1] * (width - len(path)) for path in chosen])
+        keep_tokens(self.batch, drafted, kept.view(self.sequences, width), lengths_out=self.batch.lengths)
+        dropped = [n - len(path) for n, path in zip(counts, chosen)]
+        self.lengths = [n - less for n, less in zip(self.lengths, dropped)]
+        self.next_positions = [n - less for n, less in zip(self.next_positions, dropped)]
+        self._latest, self._drafting = None, False
+        self._resize(self.lengths)
 
     def attend(
         self,
@@ -313,36 +418,94 @@ class PagedKVCache:
         *,
         out_dtype: torch.dtype | None = None,
         accumulate: bool = False,
+        window: int = 0,
+        sink: int = 0,
     ) -> tuple[torch.Tensor, torch.Tensor]:
         """(out, lse) of one query per sequence, [sequences, query_heads, head_dim]; see
-        ``HipAttentionBackend.run_paged``.  The scale defaults to 1/sqrt(head_dim)."""
+        ``HipAttentionBackend.run_paged``.  The scale defaults to 1/sqrt(head_dim).  A ``window`` counts slots, and so is
+        taken as long as none was evicted only."""
+        self._no_drafts()
+        self._no_cuts(window)
         scale = self.batch.head_dim ** -0.5 if sm_scale is None else sm_scale
+        visible = dict(window=window, sink=sink) if window or sink else {}
         if getattr(self.backend, "name", None) != "hip":
-            return self.backend.run_paged(query, self.batch, scale, out_dtype=out_dtype, accumulate=accumulate)
-        # Checked and planned anew where the shape changes or the lengths have grown or shrunk by an eighth: between,
-        # the plan's hints are an eighth high at most, and the kernel goes by the lengths that there are.
-        shape = (query.shape, query.dtype, query.device, scale, out_dtype, accumulate)
+            return self.backend.run_paged(query, self.batch, scale, out_dtype=out_dtype, accumulate=accumulate, **visible)
+        shape = (query.shape, query.dtype, query.device, scale, out_dtype, accumulate, window, sink)
+        self._plan = self._planned(
+            self._plan, shape,
+            lambda **hints: self.backend.prepare_paged(
+                query, self.batch, scale, out_dtype=out_dtype, accumulate=accumulate, **hints, **visible
+            ),
+        )
+        return self._plan[5](query)
+
+    def _planned(self, plan: tuple | None, shape: tuple, prepare) -> tuple:
+        """Checked and planned anew where the shape changes or the lengths have grown or shrunk by an eighth: between,
+        the plan's hints are an eighth high at most, and the kernel goes by the lengths that there are."""
         longest, total = max(self.lengths), sum(self.lengths)
-        plan = self._plan
         if plan is None or plan[0] != shape or not (plan[1] <= longest <= plan[2] and plan[3] <= total <= plan[4]):
             hints = [n + n // 8 + 1 for n in (longest, total)]
-            run = self.backend.prepare_paged(
-                query, self.batch, scale, out_dtype=out_dtype, accumulate=accumulate, max_length=hints[0],
-                total_tokens=hints[1],
-            )
-            plan = self._plan = (shape, longest - longest // 8, hints[0], total - total // 8, hints[1], run)
-        return plan[5](query)
+            run = prepare(max_length=hints[0], total_tokens=hints[1])
+            plan = (shape, longest - longest // 8, hints[0], total - total // 8, hints[1], run)
+        return plan
+
+    def _no_cuts(self, window: int) -> None:
+        if window and self.next_positions != self.lengths:
+            raise ValueError("a window needs slots in the order of their positions, which eviction gives up")
+
+    def attend_tokens(
+        self,
+        query: torch.Tensor,
+        counts: Sequence[int] | None = None,
+        sm_scale: float | None = None,
+        *,
+        parents: torch.Tensor | Sequence[int] | None = None,
+        out_dtype: torch.dtype | None = None,
+        window: int = 0,
+        sink: int = 0,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """(out, lse) of each sequence's last counts[b] tokens (default: one of each), [tokens, query_heads, head_dim],
+        which are in the cache already: what a prompt's or a chunk's tokens see, or, with ``parents``, a tree's; see
+        ``HipAttentionBackend.run_paged_tokens``.  Weights are not summed.  Scale and window as in :meth:`attend`."""
+        self._no_cuts(window)
+        counts = [1] * self.sequences if counts is None else [int(n) for n in counts]
+        if len(counts) != self.sequences or min(counts) < 0:
+            raise ValueError("counts must hold one non-negative number per sequence")
+        if query.ndim != 3 or sum(counts) != query.shape[0]:
+            raise ValueError("counts must add up to the number of tokens")
+        if any(n > length for n, length in zip(counts, self.lengths)):
+            raise ValueError("a sequence holds fewer tokens than that")
+        if self._drafting and (parents is None or counts != self._latest):
+            raise RuntimeError("the cache holds drafted tokens; attend them with their parents, or keep the accepted ones")
+        ends = [0]
+        for n in counts:
+            ends.append(ends[-1] + n)
+        offsets = self._host_to_device(ends)
+        if parents is not None:
+            parents = self._parents(parents, query.shape[0])
+        scale = self.batch.head_dim ** -0.5 if sm_scale is None else sm_scale
+        visible = dict(window=window, sink=sink, out_dtype=out_dtype)
+        if getattr(self.backend, "name", None) != "hip":
+            return self.backend.run_paged_tokens(query, self.batch, scale, offsets, parents, **visible)
+        shape = (query.shape, query.dtype, query.device, scale, out_dtype, window, sink)
+        self._tokens_plan = self._planned(
+            self._tokens_plan, shape,
+            lambda **hints: self.backend.prepare_paged_tokens(query, self.batch, scale, **hints, **visible),
+        )
+        return self._tokens_plan[5](query, offsets, parents)
 
     def evict(self, budget: int, *, sink: int = 0, recent: int = 0) -> None:
         """Cut every sequence to at most ``budget`` tokens (:func:`evict_tokens`) and give back the pages behind.
 
         ``batch`` keeps its arrays, so that decodes prepared before, and graphs of them, go on with the cut cache."""
+        self._no_drafts()
         longest = max(self.lengths)
         lengths, weights, positions = evict_tokens(self.batch, budget, sink=sink, recent=recent)
         self.batch.lengths.copy_(lengths)
         self.batch.weights[:, :longest].copy_(weights[:, :longest])  # (none of the sequences has slots behind)
         self.batch.positions[:, :longest].copy_(positions[:, :longest])
         self.lengths = [min(n, budget) for n in self.lengths]
+        self._latest = None
         self._resize(self.lengths)
 
     def clear(self, sequence: int) -> None:
@@ -350,6 +513,8 @@ class PagedKVCache:
         if not 0 <= sequence < self.sequences:
             raise ValueError(f"sequence must lie in [0, {self.sequences})")
         self.lengths[sequence] = self.next_positions[sequence] = 0
+        if self._latest is not None:
+            self._latest[sequence] = 0
         self.batch.lengths[sequence].zero_()
         self._resize(self.lengths)
 
@@ -358,6 +523,7 @@ class PagedKVCache:
         page_tokens tokens each, all full but the last), positions counted from 0."""
         if not 0 <= sequence < self.sequences:
             raise ValueError(f"sequence must lie in [0, {self.sequences})")
+        self._no_drafts()
         if self.lengths[sequence]:
             raise ValueError("sequence is not empty")
         if (blocks.bits, blocks.group_size) != (self.batch.bits, self.batch.group_size):
@@ -380,4 +546,6 @@ class PagedKVCache:
             self.batch.positions[sequence, :length] = torch.arange(length, dtype=torch.int32, device=self.device)
             self.batch.weights[sequence, :length] = 0.0
         self.batch.lengths[sequence] = length
+        if self._latest is not None:
+            self._latest[sequence] = 0
         self.lengths[sequence] = self.next_positions[sequence] = length
