@@ -32,7 +32,7 @@ FASTCALL_OUT = PKG / ("_fastcall" + (sysconfig.get_config_var("EXT_SUFFIX") or "
 BUILD = HERE / "_build"
 SOURCES = ["abi.hip", "decode_general.hip", "decode_tile.hip", "decode_mfma.hip", "decode_staged.hip", "merge.hip", "codec.hip", "records.hip", "vllm_codec.hip",
            "rotary.hip", "paged_append.hip", *(f"paged_decode_int{b}_d{d}.hip" for b in (4, 2) for d in (64, 128, 256)), "paged_merge.hip",
-           "paged_evict.hip", "paged_tokens.hip", "paged_keep.hip"]
+           "paged_evict.hip", "paged_tokens.hip", *(f"paged_tokens_d{d}.hip" for d in (64, 128, 256)), "paged_keep.hip"]
 ARCH = "gfx950"
 
 COMMON = [

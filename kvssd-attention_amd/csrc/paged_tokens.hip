@@ -1,158 +1,169 @@
-// Attention of many new tokens a sequence over its packed pages, their own
-// among them: prompts and chunks of prompts (causal) and trees of drafted tokens,
-// with or without a sliding window and sinks.
+// Attention of many tokens a sequence: the plan, the join of a block's runs and
+// the C entry points.
 //
-//   s_it = sm_scale q_i.k_t over the slots t that token i sees,
-//   out_i = sum_t softmax(s_i)_t v_t,  lse_i = log sum_t e^s_it
-//
-// The plain form: a wave a (token, query head); a lane a slot for the scores, a
-// lane a few dims for the values.
-#include "paged_decode.hpp"
+// Join, per (token, query head): with partials (O_r unnormalised, m_r in log2
+// units, l_r) of the runs r of its block,
+//   M = max m_r, L = sum l_r 2^(m_r - M), out = sum O_r 2^(m_r - M) / L,
+//   lse = ln 2 (M + log2 L);
+// runs with l = 0 (nothing was seen) add nothing.
+#include "paged_tokens.hpp"
+
+#include <string>
 
 namespace kvssd {
 namespace {
 
-struct TokensParams {
-  kvssd_paged_cache c;
-  kvssd_heads query;
-  void* out;
-  float* lse;
-  const int32_t* offsets;
-  const int32_t* parents;
-  int64_t tokens;
-  int capacity, window, sink;
-  int query_heads, gq, query_dtype, out_dtype;
-  int groups, group_log2;
-  float scale_log2;
+constexpr int kThreads = 256;
+
+template <int DP>
+__global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedTokensParams p) {
+  const int kvh = blockIdx.x % p.c.kv_heads;
+  int first;
+  const TokenItem work = find_item<tokens_stage(DP)>(p, blockIdx.x / p.c.kv_heads, true, &first);
+  if (work.seq < 0 || work.runs == 1) return;
+  const int d = p.c.head_dim, lanes = d / 4;
+  const int rows = min(work.span.count * p.gq - work.block * p.block_rows, p.block_rows);
+  const int dim = threadIdx.x % lanes * 4;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const int64_t step = static_cast<int64_t>(p.c.kv_heads) * p.block_rows;  // rows between runs
+  for (int row = threadIdx.x / lanes; row < rows; row += kThreads / lanes) {
+    if (static_cast<int>(threadIdx.x) >= kThreads / lanes * lanes) break;
+    const int64_t at = (static_cast<int64_t>(first) * p.c.kv_heads + kvh) * p.block_rows + row;
+    const f32x2* ml = reinterpret_cast<const f32x2*>(p.part_ml) + at;
+    const float* o = p.part_o + at * d + dim;
+    float most = -INFINITY;
+#pragma unroll 4
+    for (int r = 0; r < work.runs; ++r) {
+      const f32x2 x = ml[r * step];
+      if (x[1] != 0.0f) most = fmaxf(most, x[0]);
+    }
+    float sum = 0.0f;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int r = 0; r < work.runs; ++r) {
+      const f32x2 x = ml[r * step];
+      const f32x4 v = *reinterpret_cast<const f32x4*>(o + r * step * d);
+      if (x[1] != 0.0f) {  // (a NaN sum takes part)
+        const float w = exp2f(x[0] - most);
+        sum += w * x[1];
+        acc += w * v;
+      }
+    }
+    const int in_seq = work.block * p.block_rows + row, token = in_seq / p.gq;
+    const int64_t to = (work.span.begin + token) * p.query_heads + kvh * p.gq + in_seq - token * p.gq;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_out(p.out, p.out_dtype, to * d + dim + i, sum == 0.0f ? 0.0f : acc[i] / sum);
+    if (dim == 0) p.lse[to] = sum == 0.0f ? -INFINITY : kLn2 * (most + log2f(sum));
+  }
+}
+
+size_t aligned(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+struct Plan {
+  PagedTokensParams p;
+  int dp, columns;
+  bool precise;
+  int64_t blocks;  // at most
+  size_t o_bytes, ml_bytes;
 };
 
-__device__ __forceinline__ float query_at(const void* q, int dtype, int64_t at) {
-  if (dtype == KVSSD_DTYPE_F32) return static_cast<const float*>(q)[at];
-  if (dtype == KVSSD_DTYPE_F16) return static_cast<float>(static_cast<const _Float16*>(q)[at]);
-  return __builtin_bit_cast(float, static_cast<uint32_t>(static_cast<const uint16_t*>(q)[at]) << 16);
-}
-
-__global__ __launch_bounds__(kWave) void paged_tokens_kernel(TokensParams p) {
-  const kvssd_paged_cache& c = p.c;
-  const int lane = threadIdx.x;
-  const int64_t t = blockIdx.x / p.query_heads;
-  const int h = blockIdx.x % p.query_heads, kvh = h / p.gq;
-  const int d = c.head_dim, mid = 1 << (c.bits - 1), mask = (1 << c.bits) - 1;
-  int seq = -1;
-  if (t >= p.offsets[0] && t < p.offsets[c.sequences]) {
-    int lo = 0, hi = c.sequences;
-    while (hi - lo > 1) {
-      const int at = (lo + hi) / 2;
-      if (p.offsets[at] <= t) lo = at;
-      else hi = at;
-    }
-    seq = lo;
-  }
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-  if (seq >= 0) {
-    const int begin = p.offsets[seq], n = p.offsets[seq + 1] - begin;
-    const int i = static_cast<int>(t - begin);
-    const int length = paged_length(c.lengths, seq, p.capacity);
-    const int base = length - n;
-    const int32_t* parents = p.parents ? p.parents + begin : nullptr;
-    int position = base + i;
-    if (parents != nullptr) {
-      position = base;
-      for (int up = parent_of(parents, i); up >= 0; up = parent_of(parents, up)) ++position;
-    }
-    const int32_t* pages = c.page_table + static_cast<int64_t>(seq) * c.max_pages;
-    const int64_t q0 = t * p.query.token_stride + h * p.query.head_stride;
-    for (int s0 = 0; s0 <= base + i; s0 += kWave) {
-      const int slot = s0 + lane;
-      bool seen = slot <= base + i && slot < length;
-      int where = slot;
-      if (seen && parents != nullptr && slot >= base) {
-        int x = i;
-        where = position;
-        while (x > slot - base) {
-          x = parent_of(parents, x);
-          --where;
-        }
-        seen = x == slot - base;
-      }
-      if (p.window > 0) seen = seen && (where > position - p.window || where < p.sink);
-      int64_t row = -1;
-      if (seen) {
-        const int page = pages[slot / c.page_tokens];
-        if (page >= 0 && page < c.num_pages) row = static_cast<int64_t>(page) * c.page_tokens + slot % c.page_tokens;
-      }
-      float score = -INFINITY;
-      if (row >= 0) {
-        const uint8_t* codes = c.packed_k + (row * c.kv_heads + kvh) * (d * c.bits / 8);
-        const uint16_t* scales = c.scales_k + (row * c.kv_heads + kvh) * p.groups;
-        score = 0.0f;
-        for (int g = 0; g < p.groups; ++g) {
-          float sum = 0.0f;
-          for (int x = 0; x < c.group_size; ++x) {
-            const int dim = g * c.group_size + x;
-            const int code = codes[dim * c.bits / 8] >> (dim * c.bits % 8) & mask;
-            sum = __builtin_fmaf(query_at(p.query.data, p.query_dtype, q0 + dim), static_cast<float>(code - mid), sum);
-          }
-          score = __builtin_fmaf(sum, half_bits_to_float(scales[g]), score);
-        }
-        score *= p.scale_log2;
-      }
-      const float m_new = fmaxf(m, wave_max(score));
-      const uint64_t live = __ballot(row >= 0);
-      if (live == 0) continue;
-      const float alpha = m == -INFINITY ? 0.0f : exp2f(m - m_new);
-      const float e = row >= 0 ? exp2f(score - (m_new == -INFINITY ? 0.0f : m_new)) : 0.0f;
-      m = m_new;
-      l = l * alpha + wave_sum(e);
-      for (int x = 0; x < 4; ++x) acc[x] *= alpha;
-      for (int k = 0; k < kWave; ++k) {
-        if (!(live >> k & 1)) continue;
-        const float w = __shfl(e, k, kWave);
-        const int64_t r = __shfl(row, k, kWave);
-        for (int x = 0; x < 4; ++x) {
-          const int dim = lane + x * kWave;
-          if (dim >= d) break;
-          const int code = c.packed_v[(r * c.kv_heads + kvh) * (d * c.bits / 8) + dim * c.bits / 8] >> (dim * c.bits % 8) & mask;
-          const float scale = half_bits_to_float(c.scales_v[(r * c.kv_heads + kvh) * p.groups + (dim >> p.group_log2)]);
-          acc[x] = __builtin_fmaf(w, static_cast<float>(code - mid) * scale, acc[x]);
-        }
-      }
-    }
-  }
-  const int64_t row = t * p.query_heads + h;
-  for (int x = 0; x < 4; ++x) {
-    const int dim = lane + x * kWave;
-    if (dim < d) store_out(p.out, p.out_dtype, row * d + dim, l == 0.0f ? 0.0f : acc[x] / l);
-  }
-  if (lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : kLn2 * (m + log2f(l));
-}
-
-int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, TokensParams* p) {
+int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* plan) {
   if (a.query.heads <= 0 || a.query.heads % c.kv_heads) return arg_error("query heads must be divisible by KV heads");
   if (!paged_dtype(a.query_dtype)) return arg_error("unsupported query dtype");
   if (a.out_query_dtype != 0 && a.out_query_dtype != 1) return arg_error("out_query_dtype must be 0 or 1");
   if (a.max_length < 0 || a.total_tokens < 0) return arg_error("max_length and total_tokens must be >= 0");
   if (a.window < 0 || a.sink < 0) return arg_error("window and sink must be >= 0");
-  if (a.tokens < 0 || a.tokens * a.query.heads > (int64_t{1} << 30)) return arg_error("too many tokens for one call");
-  *p = TokensParams{};
-  p->c = c;
-  p->query = a.query;
-  p->out = a.out;
-  p->lse = a.lse;
-  p->offsets = a.offsets;
-  p->parents = a.parents;
-  p->tokens = a.tokens;
-  p->capacity = static_cast<int>(paged_capacity(c));
-  p->window = a.window;
-  p->sink = a.sink;
-  p->query_heads = a.query.heads;
-  p->gq = a.query.heads / c.kv_heads;
-  p->query_dtype = a.query_dtype;
-  p->out_dtype = a.out_query_dtype ? a.query_dtype : KVSSD_DTYPE_F32;
-  p->groups = c.head_dim / c.group_size;
-  while ((1 << p->group_log2) < c.group_size) ++p->group_log2;
-  p->scale_log2 = static_cast<float>(a.sm_scale) * kLog2e;
+  if (a.tokens < 0 || a.tokens > (int64_t{1} << 30) || a.tokens * a.query.heads > (int64_t{1} << 30))
+    return arg_error("tokens * query heads must be at most 2^30");
+  *plan = Plan{};
+  PagedTokensParams& p = plan->p;
+  p.c = c;
+  p.query = a.query;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.offsets = a.offsets;
+  p.parents = a.parents;
+  p.tokens = a.tokens;
+  p.capacity = static_cast<int>(paged_capacity(c));
+  const int far = 1 << 30;  // as good as any larger one
+  p.window = a.window < far ? a.window : far;
+  p.sink = a.sink < far ? a.sink : far;
+  p.query_heads = a.query.heads;
+  p.gq = a.query.heads / c.kv_heads;
+  p.query_dtype = a.query_dtype;
+  p.out_dtype = a.out_query_dtype ? a.query_dtype : KVSSD_DTYPE_F32;
+  p.groups = c.head_dim / c.group_size;
+  while ((32 << p.slices_log2) < c.group_size) ++p.slices_log2;
+  p.scale_log2 = static_cast<float>(a.sm_scale) * kLog2e;
+  const int64_t item = static_cast<int64_t>(dtype_bytes(a.query_dtype));
+  p.vector_query = reinterpret_cast<uintptr_t>(a.query.data) % 16 == 0 && a.query.token_stride * item % 16 == 0 &&
+                   a.query.head_stride * item % 16 == 0;
+  plan->precise = p.out_dtype == KVSSD_DTYPE_F32 || p.query_dtype == KVSSD_DTYPE_F32;
+  plan->dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+  const int stage = tokens_stage(plan->dp);
+
+  // rows of a workgroup, after a sequence's rows on average
+  const int64_t each = (a.tokens * p.gq + c.sequences - 1) / c.sequences;
+  plan->columns = each > 128 && !plan->precise && plan->dp <= 128 ? 2 : 1;
+  p.row_tiles = each > 64 ? 4 : each > 32 ? 2 : 1;
+  const int tiles = stage / 32;
+  p.parts = kTokenWaves / p.row_tiles < tiles ? kTokenWaves / p.row_tiles : tiles;
+  p.block_rows = 32 * plan->columns * p.row_tiles;
+  plan->blocks = a.tokens * p.gq / p.block_rows + c.sequences + 2;
+
+  // runs, where blocks alone would leave compute units idle
+  auto stages = [&](int64_t n) { return (n + stage - 1) / stage; };
+  int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
+  int64_t total = a.total_tokens > 0 && a.total_tokens < longest * c.sequences ? a.total_tokens : longest * c.sequences;
+  if (p.window > 0) {
+    const int64_t seen = p.window + p.block_rows / p.gq + p.sink + 3 * stage;
+    longest = longest < seen ? longest : seen;
+    total = total < longest * c.sequences ? total : longest * c.sequences;
+  }
+  const int64_t likely = (each + p.block_rows - 1) / p.block_rows * c.sequences;  // blocks
+  const int64_t wanted = 512 / c.kv_heads;                                        // items
+  p.items = static_cast<int>(plan->blocks);
+  p.least_stages = 1 << 30;
+  if (likely < wanted) {
+    const int64_t work = (total / stage + c.sequences) * (likely / c.sequences);
+    int64_t size = (work + wanted - likely - 1) / (wanted - likely);
+    if (size < 2) size = 2;
+    if (size < stages(longest)) {
+      p.least_stages = static_cast<int>(size);
+      p.items = static_cast<int>(plan->blocks + work / size + 1);
+    }
+  }
+  if (static_cast<int64_t>(p.items) * c.kv_heads > (int64_t{1} << 23)) return arg_error("too many sequences or tokens for one call");
+  const bool split = p.least_stages < (1 << 30);
+  const size_t rows = split ? static_cast<size_t>(p.items) * c.kv_heads * p.block_rows : 0;
+  plan->o_bytes = aligned(rows * c.head_dim * sizeof(float));
+  plan->ml_bytes = aligned(rows * 2 * sizeof(float));
   return 0;
+}
+
+int launch_paged_tokens(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, hipStream_t stream) {
+  Plan plan;
+  if (int rc = plan_of(c, a, &plan)) return rc;
+  PagedTokensParams& p = plan.p;
+  const size_t need = plan.o_bytes + plan.ml_bytes;
+  if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need))
+    return arg_error("workspace too small: need " + std::to_string(need) + " bytes");
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 256) return arg_error("workspace must be 256-byte aligned");
+  if (reinterpret_cast<uintptr_t>(a.out) % 16) return arg_error("out must be 16-byte aligned");
+  p.part_o = static_cast<float*>(a.workspace);
+  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + plan.o_bytes);
+  const int64_t work = static_cast<int64_t>(p.items) * c.kv_heads;
+  const unsigned groups = static_cast<unsigned>(c.kv_heads % 2 ? work : (work + 15) / 16 * 16);
+  const auto launch = plan.dp == 64    ? launch_paged_tokens_dims<64>
+                      : plan.dp == 128 ? launch_paged_tokens_dims<128>
+                                       : launch_paged_tokens_dims<256>;
+  if (int rc = launch(p, plan.columns, plan.precise, groups, stream)) return rc;
+  if (need == 0) return 0;
+  const dim3 grid(static_cast<unsigned>(plan.blocks * c.kv_heads));
+  if (plan.dp == 64) hipLaunchKernelGGL(paged_tokens_merge_kernel<64>, grid, dim3(kThreads), 0, stream, p);
+  else if (plan.dp == 128) hipLaunchKernelGGL(paged_tokens_merge_kernel<128>, grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL(paged_tokens_merge_kernel<256>, grid, dim3(kThreads), 0, stream, p);
+  return hip_status(hipGetLastError(), "paged_tokens_merge launch");
 }
 
 }  // namespace
@@ -167,9 +178,9 @@ __attribute__((visibility("default"))) int kvssd_hip_paged_tokens_workspace_byte
                                                                                   size_t* bytes) {
   if (int rc = check_paged_cache(cache)) return rc;
   if (args == nullptr || bytes == nullptr) return arg_error("arguments are NULL");
-  TokensParams p;
-  if (int rc = plan_of(*cache, *args, &p)) return rc;
-  *bytes = 0;
+  Plan plan;
+  if (int rc = plan_of(*cache, *args, &plan)) return rc;
+  *bytes = plan.o_bytes + plan.ml_bytes;
   return 0;
 }
 
@@ -177,14 +188,9 @@ __attribute__((visibility("default"))) int kvssd_hip_paged_tokens(const kvssd_pa
                                                                   const kvssd_paged_tokens_args* args, void* stream) {
   if (int rc = check_paged_cache(cache)) return rc;
   if (args == nullptr) return arg_error("arguments are NULL");
-  TokensParams p;
-  if (int rc = plan_of(*cache, *args, &p)) return rc;
-  if (p.tokens == 0) return 0;
+  if (args->tokens == 0) return 0;
   if (!args->query.data || !args->out || !args->lse || !args->offsets) return arg_error("a required buffer pointer is NULL");
-  if (reinterpret_cast<uintptr_t>(args->workspace) % 256) return arg_error("workspace must be 256-byte aligned");
-  hipLaunchKernelGGL(paged_tokens_kernel, dim3(static_cast<unsigned>(p.tokens * p.query_heads)), dim3(kWave), 0,
-                     static_cast<hipStream_t>(stream), p);
-  return hip_status(hipGetLastError(), "paged_tokens launch");
+  return launch_paged_tokens(*cache, *args, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,759 @@
+// Attention of many new tokens a sequence over its packed pages, their own
+// among them: prompts and chunks of prompts (causal) and trees of drafted tokens,
+// with or without a sliding window and sinks.
+//
+//   s_it = sm_scale q_i.k_t over the slots t that token i sees,
+//   out_i = sum_t softmax(s_i)_t v_t,  lse_i = log sum_t e^s_it
+//
+// with k and v held as INT2/INT4 codes c and group scales, k = (c - mid) sk.
+//
+// Work split.  The rows of a kv head are its sequence's (token, query head) pairs,
+// a token's heads side by side.  A workgroup takes a block of them, 32 C a wave in
+// row_tiles waves, and a run of the slots that they see, a stage (8,192 numbers of
+// K and of V) at a time.  Its four waves unpack a stage together, each thread the 32
+// dims of one slot that it loaded while the stage before was worked on; where rows
+// fill fewer waves, waves share the stage's slots (parts) and are joined at the end.
+//
+// QK (v_mfma_f32_32x32x16_f16): rows = slots, columns = query rows, so that a lane
+//   holds 16 scores of one query row and softmax needs no exchange but between the
+//   wave's halves.  Codes enter exactly, as (c - mid) / 2^6 (INT4) or / 2^2; the
+//   products of 32 dims are taken apart and a group's scale multiplies in 32 bits.
+//   The query is scaled by a power of two per row into fp16's range (exact for
+//   fp16 and bf16); a 32-bit one is a sum of two fp16 parts.
+// Softmax.  The reference is lazy: it is moved (and sums rescaled) only where a score
+//   exceeds the range that fp16 weights have above it.  Weights are 2^8 at the
+//   reference's maximum, so that those below fp16's normal range are nothing beside it.
+// PV: rows = dims, columns = query rows, K = slots: the scores' lanes are the weights'
+//   lanes.  Values are codes times scale, rounded to fp16 (32-bit results: a sum of
+//   two fp16 parts, which hold it exactly, as they do the weights); scales are first
+//   multiplied by a power of two that puts the largest so far near fp16's top.
+//
+// A value scale that is not finite is left out of the products, where a masked row's
+// weight of 0 times it would be NaN, and makes its group of the rows that see it NaN.
+#pragma once
+
+#include "paged_decode.hpp"
+
+namespace kvssd {
+
+constexpr int kTokenWaves = 4;
+
+constexpr int tokens_stage(int dp) { return 8192 / dp; }  // slots: a thread's piece is 32 dims of one
+
+struct PagedTokensParams {
+  kvssd_paged_cache c;
+  kvssd_heads query;
+  void* out;
+  float* lse;
+  const int32_t* offsets;
+  const int32_t* parents;
+  float* part_o;   // [item][kv head][row][head_dim]
+  float* part_ml;  // [item][kv head][row][2]
+  int64_t tokens;
+  int capacity, window, sink;
+  int query_heads, gq, query_dtype, out_dtype;
+  int groups, slices_log2;  // scale groups of a head; 32-dim slices of a group
+  int vector_query;         // 16-byte loads of the query
+  int row_tiles, parts;     // of a workgroup: waves side by side on rows, on slots
+  int block_rows;           // rows of a workgroup
+  int items;                // (row block, run) pairs that the grid and the workspace hold
+  int least_stages;         // of a run, unless the lengths call for more
+  float scale_log2;
+};
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+// ds_read_b64_tr_b16: within each group of 16 lanes, lane j receives half j % 4 of lanes j / 4, j / 4 + 4, + 8 and + 12
+__device__ __forceinline__ u32x2 lds_read_tr16(const uint8_t* lds) {
+  typedef short i16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)lds));
+}
+
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// ---------------------------------------------------------------- the work ---
+
+// A sequence's tokens in the call; numbers `sequences` and one on are the tokens before and behind all of them, which
+// see nothing.
+struct TokenSpan {
+  int64_t begin;
+  int count;
+  int length;  // of the sequence, its new tokens included
+};
+
+__device__ __forceinline__ TokenSpan token_span(const PagedTokensParams& p, int s) {
+  const int last = p.c.sequences;
+  auto place = [&](int i) {
+    const int64_t at = p.offsets[i];
+    return at < 0 ? 0 : (at > p.tokens ? p.tokens : at);
+  };
+  if (s > last + 1) return {0, 0, 0};
+  const int64_t begin = s <= last ? (s == last ? 0 : place(s)) : place(last);
+  const int64_t end = s < last ? place(s + 1) : (s == last ? place(0) : p.tokens);
+  return {begin, end > begin ? static_cast<int>(end - begin) : 0, s < last ? paged_length(p.c.lengths, s, p.capacity) : 0};
+}
+
+__device__ __forceinline__ int blocks_of(const PagedTokensParams& p, const TokenSpan& s) {
+  return static_cast<int>((static_cast<int64_t>(s.count) * p.gq + p.block_rows - 1) / p.block_rows);
+}
+
+// Stages that a block's tokens see something of: those of the sinks, then from `second` to `end`.
+struct StageList {
+  int sinks, second, end;
+  __device__ __forceinline__ int count() const { return sinks + end - second; }
+  __device__ __forceinline__ int stage(int n) const { return n < sinks ? n : n - sinks + second; }
+};
+
+__device__ __forceinline__ StageList stages_of(const PagedTokensParams& p, const TokenSpan& s, int block, int stage_slots) {
+  const int base = s.length - s.count;
+  const int first = block * p.block_rows / p.gq;  // (fewer than 2^30 rows)
+  const int last = min((block * p.block_rows + p.block_rows - 1) / p.gq, s.count - 1);
+  const int hi = max(min(base + last + 1, s.length), 0);  // the first slot that none sees
+  StageList list{0, 0, (hi + stage_slots - 1) / stage_slots};
+  if (p.window > 0) {
+    const int at = (p.parents ? base : base + first) - p.window + 1;  // the first that one sees, but for sinks
+    list.second = min(max(at, 0) / stage_slots, list.end);
+    list.sinks = min((min(p.sink, hi) + stage_slots - 1) / stage_slots, list.second);
+  }
+  return list;
+}
+
+// Which work a workgroup does: its item, of the batch's, is run `run` of `runs` of a block of rows.
+struct TokenItem {
+  int seq, block, run, runs;
+  TokenSpan span;
+};
+
+// Every sequence's blocks are cut into the same number of runs, after the stages of its last one (which sees most, but
+// for borders).  p.least_stages comes from the caller's hints, and grows here where the lengths would need more items
+// than there are: sum of blocks * runs <= sum of blocks * stages / size + sum of blocks.
+template <int STAGE>
+__device__ __forceinline__ int runs_of_sequence(const PagedTokensParams& p, const TokenSpan& s, int blocks, int size) {
+  if (blocks == 0) return 0;
+  const int stages = stages_of(p, s, blocks - 1, STAGE).count();
+  return stages <= size ? 1 : (stages + size - 1) / size;
+}
+
+template <int STAGE>
+__device__ __forceinline__ int run_size(const PagedTokensParams& p) {
+  const int lane = threadIdx.x % kWave;
+  float work = 0.0f, blocks = 0.0f;
+  for (int s0 = 0; s0 < p.c.sequences + 2; s0 += kWave) {
+    const TokenSpan s = token_span(p, s0 + lane);
+    const int n = blocks_of(p, s);
+    if (n > 0) {
+      blocks += static_cast<float>(n);
+      work += static_cast<float>(n) * static_cast<float>(stages_of(p, s, n - 1, STAGE).count());
+    }
+  }
+  work = wave_sum(work);
+  blocks = wave_sum(blocks);
+  const float room = static_cast<float>(p.items) - blocks;
+  if (room < 1.0f) return 1 << 30;
+  const float least = work / room * 1.0001f + 1.0f;  // (sums of 24 bits)
+  return max(p.least_stages, least < 1e9f ? static_cast<int>(least) : 1 << 30);
+}
+
+// Item `item`; seq -1 where there are fewer.  `blocks_alone`: items are blocks.
+template <int STAGE>
+__device__ __forceinline__ TokenItem find_item(const PagedTokensParams& p, int item, bool blocks_alone, int* first) {
+  const int lane = threadIdx.x % kWave;
+  const int size = run_size<STAGE>(p);
+  int before = 0;  // items of the sequences before
+  for (int s0 = 0; s0 < p.c.sequences + 2; s0 += kWave) {
+    const TokenSpan s = token_span(p, s0 + lane);
+    const int blocks = blocks_of(p, s);
+    const int runs = runs_of_sequence<STAGE>(p, s, blocks, size);
+    const int n = blocks_alone ? blocks : blocks * runs;
+    const int upto = wave_prefix(n);
+    const uint64_t past = __ballot(item < upto);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      const int own = item - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
+      TokenItem t;
+      t.seq = s0 + at;
+      t.runs = __builtin_amdgcn_readlane(runs, at);
+      const int count = __builtin_amdgcn_readlane(blocks, at);
+      const int place = blocks_alone ? own : own / t.runs;
+      t.block = count - 1 - place;  // the longest first
+      t.run = blocks_alone ? 0 : own - place * t.runs;
+      t.span.begin = static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(s.begin), at));  // (below 2^30)
+      t.span.count = __builtin_amdgcn_readlane(s.count, at);
+      t.span.length = __builtin_amdgcn_readlane(s.length, at);
+      if (first != nullptr) {
+        const int all = wave_prefix(blocks * runs);
+        *first = before + __builtin_amdgcn_readlane(all, at) - count * t.runs + place * t.runs;
+      }
+      return t;
+    }
+    item -= __builtin_amdgcn_readlane(upto, kWave - 1);
+    before += __builtin_amdgcn_readlane(wave_prefix(blocks * runs), kWave - 1);
+  }
+  return TokenItem{-1, 0, 0, 1, {0, 0, 0}};
+}
+
+// Workgroup -> (item, kv head).  Workgroups go to the eight dies in turn, each with an L2 of its own; a line of codes
+// holds two neighbouring heads' rows (of 64 bytes), whose workgroups should so be of one die and near in time.
+__device__ __forceinline__ void place_of(const PagedTokensParams& p, int id, int* item, int* head) {
+  const int heads = p.c.kv_heads;
+  if (heads % 2) {
+    *item = id / heads;
+    *head = id - *item * heads;
+    return;
+  }
+  const int pair = id / 16 * 8 + id % 8;
+  *item = pair / (heads / 2);
+  *head = (pair - *item * (heads / 2)) * 2 + id / 8 % 2;
+}
+
+template <int DP>
+int launch_paged_tokens_dims(const PagedTokensParams& p, int columns, bool precise, unsigned groups, hipStream_t stream);
+template <>
+int launch_paged_tokens_dims<64>(const PagedTokensParams& p, int columns, bool precise, unsigned groups, hipStream_t stream);
+template <>
+int launch_paged_tokens_dims<128>(const PagedTokensParams& p, int columns, bool precise, unsigned groups, hipStream_t stream);
+template <>
+int launch_paged_tokens_dims<256>(const PagedTokensParams& p, int columns, bool precise, unsigned groups, hipStream_t stream);
+
+// ------------------------------------------------------------------ kernel ---
+
+// 32 codes as fp16 pairs (c - mid) / F in the dims' order
+template <int BITS>
+__device__ __forceinline__ void unpack_piece(const uint32_t* x, const Masks& k, uint32_t m01, uint32_t m23, u32x4 (&out)[4]) {
+  if constexpr (BITS == 4) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const u32x4 v = code_operand<4>(x[w], 0, k, m01, m23);  // dims (0, 4) (1, 5) (2, 6) (3, 7)
+      out[w] = u32x4{low_halves(v[0], v[1]), low_halves(v[2], v[3]), high_halves(v[0], v[1]), high_halves(v[2], v[3])};
+    }
+  } else {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const u32x4 a = code_operand<2>(x[w], 0, k, m01, m23), b = code_operand<2>(x[w], 1, k, m01, m23);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // dims (2 i, 2 i + 8) and (2 i + 1, 2 i + 9)
+        out[2 * w][i] = low_halves(a[i], b[i]);
+        out[2 * w + 1][i] = high_halves(a[i], b[i]);
+      }
+    }
+  }
+}
+
+// C: columns of 32 query rows a wave
+template <int DP, int C, bool PREC>
+__global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) void paged_tokens_kernel(PagedTokensParams p) {
+  constexpr int kStage = tokens_stage(DP);
+  constexpr int kSlices = DP / 32;
+  constexpr int kParts = PREC ? 2 : 1;
+  constexpr int kTiles = kStage / 32;             // of a stage
+  constexpr int kOwn = kStage / kTokenWaves;      // slots of a wave's pieces
+  constexpr int kValueRow = DP * 2 + 32;          // bytes; transposed reads of four rows meet in no bank
+  constexpr int kKeyBytes = DP * kStage * 2, kValueBytes = kValueRow * kStage;
+  constexpr float kBias = 8.0f, kRoom = 14.0f;    // log2 of a weight at the reference's maximum, and at most
+  constexpr int kPlain = 14;                      // exponent of the scales that the largest factor (2^15) serves
+  // keys: [chunk of 8 dims][slot] 16 bytes each, slots turned by their chunk; values: [part][slot][dim]
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kKeyBytes + kParts * kValueBytes];
+  __shared__ __attribute__((aligned(16))) uint16_t scale_lds[kSlices][kTiles][2][16];
+  __shared__ uint64_t live_lds[kTokenWaves], bad_lds[kTokenWaves];
+  __shared__ int top_lds[kTokenWaves];
+  uint8_t* const key_lds = lds;
+  uint8_t* const value_lds = lds + kKeyBytes;
+
+  const kvssd_paged_cache& c = p.c;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = scalar(tid / kWave);
+  const int col = lane & 31, half = lane >> 5;
+  int item, kvh;
+  place_of(p, blockIdx.x, &item, &kvh);
+  item = scalar(item);
+  kvh = scalar(kvh);
+  if (item >= p.items) return;
+  const TokenItem work = find_item<kStage>(p, item, false, nullptr);
+  if (work.seq < 0) return;
+  const int seq = scalar(work.seq), block = scalar(work.block), runs = scalar(work.runs);
+  const int count = scalar(work.span.count), length = scalar(work.span.length);
+  const int64_t token0 = scalar(static_cast<int>(work.span.begin));
+  const int base = length - count;
+  const int rows = count * p.gq;
+  StageList list{0, 0, 0};
+  int n_begin = 0, n_end = 0;
+  if (seq < c.sequences) {
+    list = stages_of(p, {token0, count, length}, block, kStage);
+    const int n = list.count();
+    const int run = scalar(work.run);
+    n_begin = static_cast<int>(static_cast<int64_t>(n) * run / runs);
+    n_end = static_cast<int>(static_cast<int64_t>(n) * (run + 1) / runs);
+  }
+
+  // ---- a thread's pieces: 32 dims of a slot
+  const int piece_slot = tid / kSlices, slice = tid % kSlices;
+  const int d = c.head_dim, row_bytes = d * c.bits / 8;
+  const bool has_dims = slice * 32 < d;
+  const int piece_bytes = 4 * c.bits;
+  const int group = slice >> p.slices_log2;
+  const int32_t* pages = c.page_table + static_cast<int64_t>(seq < c.sequences ? seq : 0) * c.max_pages;
+  struct Piece {
+    uint32_t k[4], v[4];
+    uint16_t sk, sv;
+    bool live;
+  } next{};
+  auto page_of = [&](int n) {  // of the piece's slot in the list's stage n; -1: none
+    const int slot = list.stage(n) * kStage + piece_slot;
+    return n < n_end && slot < length ? pages[slot / c.page_tokens] : -1;
+  };
+  auto load = [&](int n, int page) {
+    Piece x{};
+    if (n < n_end && page >= 0 && page < c.num_pages) {
+      const int slot = list.stage(n) * kStage + piece_slot;
+      const int64_t at = (static_cast<int64_t>(page) * c.page_tokens + slot % c.page_tokens) * c.kv_heads + kvh;
+      x.live = true;
+      if (has_dims) {
+        const int64_t byte = at * row_bytes + slice * piece_bytes;
+        if (c.bits == 4) {
+          __builtin_memcpy(x.k, __builtin_assume_aligned(c.packed_k + byte, 16), 16);
+          __builtin_memcpy(x.v, __builtin_assume_aligned(c.packed_v + byte, 16), 16);
+        } else {
+          __builtin_memcpy(x.k, __builtin_assume_aligned(c.packed_k + byte, 8), 8);
+          __builtin_memcpy(x.v, __builtin_assume_aligned(c.packed_v + byte, 8), 8);
+        }
+        x.sk = c.scales_k[at * p.groups + group];
+        x.sv = c.scales_v[at * p.groups + group];
+      }
+    }
+    return x;
+  };
+
+  // ---- the wave's rows
+  const int part = wave / p.row_tiles;
+  const bool active = part < p.parts;
+  const int wave_row0 = block * p.block_rows + (wave % p.row_tiles) * 32 * C;
+  u32x4 q[kParts][C][DP / 16];
+  float factor[C];
+  int own[C], place[C];  // a column's token among the sequence's, and its position
+  const bool two_parts = PREC && p.query_dtype == KVSSD_DTYPE_F32;
+  int page_next = page_of(n_begin);
+#pragma unroll
+  for (int x = 0; x < C; ++x) {
+    const int row = min(wave_row0 + 32 * x + col, rows - 1);
+    own[x] = row / p.gq;
+    const int head = kvh * p.gq + row - own[x] * p.gq;
+    place[x] = base + own[x];
+    if (p.parents != nullptr && seq < c.sequences) {
+      place[x] = base;
+      const int32_t* parents = p.parents + token0;
+      for (int up = parent_of(parents, own[x]); up >= 0; up = parent_of(parents, up)) ++place[x];
+    }
+    const int item_bytes = p.query_dtype == KVSSD_DTYPE_F32 ? 4 : 2;
+    const uint8_t* src = static_cast<const uint8_t*>(p.query.data) +
+                         ((token0 + own[x]) * p.query.token_stride + head * p.query.head_stride) * item_bytes;
+    float big = 0.0f;
+    auto span = [&](int j, float (&v)[8]) {  // dims 16 j + 8 half ..
+      const int dim = 16 * j + 8 * half;
+      if (!active || dim >= d) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      } else if (p.vector_query) {
+        query_span<8>(src, p.query_dtype, dim, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (p.query_dtype == KVSSD_DTYPE_F32) v[i] = reinterpret_cast<const float*>(src)[dim + i];
+          else if (p.query_dtype == KVSSD_DTYPE_F16) v[i] = static_cast<float>(reinterpret_cast<const _Float16*>(src)[dim + i]);
+          else v[i] = __builtin_bit_cast(float, static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(src)[dim + i]) << 16);
+        }
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < DP / 16; ++j) {
+      float v[8];
+      span(j, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(v[i]));
+    }
+    big = fmaxf(big, __shfl_xor(big, 32, kWave));
+    int ex = static_cast<int>((__builtin_bit_cast(uint32_t, big) >> 23) & 255u);
+    ex = ex < 12 ? 12 : (ex > 253 ? 253 : ex);
+    const int up = 10 + 127 - ex;  // 2^up big in [2^10, 2^11)
+    const float scale_up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + up) << 23);
+    const float scale_down = __builtin_bit_cast(float, static_cast<uint32_t>(127 - up) << 23);
+    factor[x] = scale_down * ((c.bits == 4 ? kUnpackScale<4> : kUnpackScale<2>) * p.scale_log2);
+#pragma unroll
+    for (int j = 0; j < DP / 16; ++j) {  // (the values again, from the cache: fewer registers)
+      float v[8];
+      span(j, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = v[2 * i] * scale_up, b = v[2 * i + 1] * scale_up;
+        const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
+        q[0][x][j][i] = pack_half2(ah, bh);
+        if constexpr (PREC)
+          q[kParts - 1][x][j][i] = pack_half2(static_cast<_Float16>(a - static_cast<float>(ah)),
+                                              static_cast<_Float16>(b - static_cast<float>(bh)));
+      }
+    }
+  }
+  // of the wave's rows: first and last token, as slots
+  const int own_lo = base + scalar(min(wave_row0, rows - 1) / p.gq);
+  const int own_hi = base + scalar(min(wave_row0 + 32 * C, rows) - 1) / p.gq;
+
+  uint32_t zero = 0;
+  asm("" : "+v"(zero));
+  const Masks masks = make_masks(zero);
+  const uint32_t m01 = 0x00030003u | zero, m23 = 0x000C000Cu | zero;
+  constexpr int kTurn = DP / 64;  // a slot's place among its chunk's: slot ^ (chunk / kTurn), for writes of 8 lanes
+  int top = kPlain;               // exponent that the accumulators' values are scaled by
+
+  auto unpack_stage = [&](const Piece& x) {
+    u32x4 codes[4];
+    if (c.bits == 4) unpack_piece<4>(x.k, masks, m01, m23, codes);
+    else unpack_piece<2>(x.k, masks, m01, m23, codes);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int chunk = 4 * slice + w;
+      *reinterpret_cast<u32x4*>(key_lds + (chunk * kStage + (piece_slot ^ (chunk / kTurn))) * 16) = codes[w];
+    }
+    const int in_tile = piece_slot % 32;
+    scale_lds[slice][piece_slot / 32][in_tile >> 2 & 1][(in_tile >> 3) * 4 + in_tile % 4] = x.sk;
+    const int ex = x.sv >> 10 & 31;
+    const bool bad = ex == 31;
+    const int most = max(top, static_cast<int>(wave_most(bad ? 0u : static_cast<uint32_t>(ex))));
+    const uint64_t live = __ballot(x.live), bads = __ballot(bad);
+    if (lane == 0) {
+      live_lds[wave] = live;
+      bad_lds[wave] = bads;
+      top_lds[wave] = most;
+    }
+    if (c.bits == 4) unpack_piece<4>(x.v, masks, m01, m23, codes);
+    else unpack_piece<2>(x.v, masks, m01, m23, codes);
+    const _Float16 up = __builtin_bit_cast(_Float16, static_cast<uint16_t>((44 - most) << 10));  // 2^(29 - most)
+    const _Float16 s = __builtin_bit_cast(_Float16, static_cast<uint16_t>(bad ? 0 : x.sv)) * up;
+    const half2v ss = {s, s};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      u32x4 hi, lo;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t pair = codes[w][i];  // (a bit cast of a vector's element takes the first one)
+        const half2v n = __builtin_bit_cast(half2v, pair);
+        const half2v v = n * ss;
+        hi[i] = __builtin_bit_cast(uint32_t, v);
+        if constexpr (PREC) lo[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, ss, -v));
+      }
+      uint8_t* dst = value_lds + piece_slot * kValueRow + slice * 64 + w * 16;
+      *reinterpret_cast<u32x4*>(dst) = hi;
+      if constexpr (PREC) *reinterpret_cast<u32x4*>(dst + kValueBytes) = lo;
+    }
+  };
+
+  // ---- the first stage
+  next = load(n_begin, page_next);
+  page_next = page_of(n_begin + 1);
+
+  f32x16 acc[C][kSlices];
+  float m[C], l[C];
+#pragma unroll
+  for (int x = 0; x < C; ++x) {
+    m[x] = -3.0e38f;
+    l[x] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i) acc[x][i] = f32x16{};
+  }
+
+  // where the lane reads: keys of slot 32 tile + col, values of slots 16 step + 4 half + (lane / 4) % 4, dims 16 (lane / 16 % 2) + 4 (lane % 4)
+  const uint8_t* const value_at = value_lds + (4 * half + (lane >> 2 & 3)) * kValueRow + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
+
+  unpack_stage(next);
+  __syncthreads();
+  for (int n = n_begin; n < n_end; ++n) {
+    // the next stage sets out
+    next = load(n + 1, page_next);
+    page_next = page_of(n + 2);
+    // ---- this stage
+    const int slot0 = list.stage(n) * kStage;
+    int tops[kTokenWaves];
+    bool all_live = true, any_bad = false;
+#pragma unroll
+    for (int w = 0; w < kTokenWaves; ++w) {
+      tops[w] = scalar(top_lds[w]);
+      all_live = all_live && live_lds[w] == ~0ull;
+      any_bad = any_bad || bad_lds[w] != 0;
+    }
+    all_live = scalar(all_live);
+    any_bad = scalar(any_bad);
+    const int top_new = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    if (top_new != top) {
+      const float less = __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - top_new) << 23);
+#pragma unroll
+      for (int x = 0; x < C; ++x)
+#pragma unroll
+        for (int i = 0; i < kSlices; ++i) acc[x][i] *= less;
+      top = top_new;
+    }
+    const bool even = tops[0] == top && tops[1] == top && tops[2] == top && tops[3] == top;
+    if (active) {
+      for (int tile = part; tile < kTiles; tile += p.parts) {
+        const int t0 = slot0 + 32 * tile, t1 = t0 + 31;
+        // whether every row of the wave sees all of the tile's slots, or none
+        const int reach_lo = p.parents ? base : own_lo;  // the lowest position; slots up to it are seen, but for the window
+        bool all = all_live && (p.parents ? t1 < base : t1 <= own_lo);
+        if (p.window > 0) {
+          all = all && (t0 > own_hi - p.window || t1 < p.sink);
+          if (t1 <= reach_lo - p.window && t0 >= p.sink) continue;
+        }
+        if (t0 > own_hi) continue;
+        // ---- scores
+        f32x16 s[C];
+#pragma unroll
+        for (int i = 0; i < kSlices; ++i) {
+          f32x16 dot[C];
+#pragma unroll
+          for (int x = 0; x < C; ++x) dot[x] = f32x16{};
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int chunk = 4 * i + 2 * j + half;
+            u32x4 a;
+            __builtin_memcpy(&a, __builtin_assume_aligned(key_lds + (chunk * kStage + ((32 * tile + col) ^ (chunk / kTurn))) * 16, 16), 16);
+#pragma unroll
+            for (int x = 0; x < C; ++x) {
+              dot[x] = mfma32(a, q[0][x][2 * i + j], dot[x]);
+              if constexpr (PREC) {
+                if (two_parts) dot[x] = mfma32(a, q[kParts - 1][x][2 * i + j], dot[x]);
+              }
+            }
+          }
+          uint32_t sk[8];
+          __builtin_memcpy(sk, __builtin_assume_aligned(scale_lds[i][tile][half], 16), 32);
+#pragma unroll
+          for (int x = 0; x < C; ++x)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[x][r] = __builtin_fmaf(dot[x][r], half_of(sk, r), i == 0 ? 0.0f : s[x][r]);
+        }
+        // ---- weights
+        u32x4 w[kParts][C][2];
+#pragma unroll
+        for (int x = 0; x < C; ++x) {
+          uint32_t seen = 0xFFFFu;  // of the lane's slots: bit r, slot 8 (r / 4) + 4 half + r % 4
+          if (!all) {
+            uint32_t bits = 0xFFFFFFFFu;  // of the tile's slots
+            const int before = p.parents ? base : base + own[x] + 1;  // slots below it are seen, but for the window
+            bits = before >= t0 + 32 ? bits : before <= t0 ? 0u : (1u << (before - t0)) - 1;
+            if (p.window > 0) {
+              const int low = place[x] - p.window + 1;  // slots from here on, or below the sinks' end
+              const uint32_t from = low <= t0 ? ~0u : low >= t0 + 32 ? 0u : ~0u << (low - t0);
+              const uint32_t sinks = p.sink >= t0 + 32 ? ~0u : p.sink <= t0 ? 0u : (1u << (p.sink - t0)) - 1;
+              bits &= from | sinks;
+            }
+            if (p.parents != nullptr && t1 >= base) {
+              const int32_t* parents = p.parents + token0;
+              int at = place[x];
+              for (int up = own[x]; up >= 0 && base + up >= t0; up = parent_of(parents, up), --at)
+                if (base + up <= t1 && (p.window == 0 || at > place[x] - p.window || at < p.sink)) bits |= 1u << (base + up - t0);
+            }
+            if (!all_live) {
+#pragma unroll
+              for (int w4 = 0; w4 < 32 / kOwn || w4 == 0; ++w4) {
+                // the tile's slots of one wave's pieces, kSlices lanes each
+                const int of_wave = (32 * tile) / kOwn + w4;
+                const uint64_t live = live_lds[of_wave];
+                constexpr int kHere = kOwn < 32 ? kOwn : 32;
+                for (int y = 0; y < kHere; ++y)
+                  if (!(live >> ((32 * tile % kOwn + y) * kSlices) & 1)) bits &= ~(1u << (w4 * kOwn + y));
+              }
+            }
+            bits >>= 4 * half;
+            seen = (bits & 0xFu) | (bits >> 4 & 0xF0u) | (bits >> 8 & 0xF00u) | (bits >> 12 & 0xF000u);
+          }
+          float most = -INFINITY;
+          float t[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) t[r] = __builtin_fmaf(s[x][r], factor[x], -m[x]);
+          if (!all) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t[r] = seen >> r & 1u ? t[r] : -INFINITY;
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) most = fmaxf(most, t[r]);
+          if (__any(most > kRoom)) {
+            float now = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) now = fmaxf(now, seen >> r & 1u ? s[x][r] * factor[x] : -INFINITY);
+            most = fmaxf(most, __shfl_xor(most, 32, kWave));
+            now = fmaxf(now, __shfl_xor(now, 32, kWave));
+            const float ref = most > kRoom ? now - kBias : m[x];
+            const float alpha = most > kRoom ? exp2f(m[x] - ref) : 1.0f;
+            m[x] = ref;
+            l[x] *= alpha;
+#pragma unroll
+            for (int i = 0; i < kSlices; ++i) acc[x][i] *= alpha;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              t[r] = seen >> r & 1u ? __builtin_fmaf(s[x][r], factor[x], -ref) : -INFINITY;
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            t[r] = __builtin_amdgcn_exp2f(t[r]);
+            l[x] += t[r];
+          }
+          if (any_bad) {
+            for (int y = 0; y < 32; ++y) {  // slots of the tile with a value scale that is not finite
+              const int of_wave = (32 * tile + y) / kOwn;
+              const uint32_t groups = static_cast<uint32_t>(bad_lds[of_wave] >> ((32 * tile + y) % kOwn * kSlices)) & ((1u << kSlices) - 1);
+              if (scalar(groups) == 0) continue;
+              const int r = (y >> 3) * 4 + y % 4;
+              const int here = half == (y >> 2 & 1) && (seen >> r & 1u);
+              const int sees = here | __shfl_xor(here, 32, kWave);
+#pragma unroll
+              for (int i = 0; i < kSlices; ++i)
+                if (sees && (groups >> i & 1u)) acc[x][i] += __builtin_nanf("");
+            }
+          }
+          if (!even) {  // values that were scaled by less than the largest so far
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int less = top - scalar(top_lds[(32 * tile + 8 * j) / kOwn]);
+              const float by = __builtin_bit_cast(float, static_cast<uint32_t>(127 - less) << 23);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) t[4 * j + i] *= by;
+            }
+          }
+#pragma unroll
+          for (int step = 0; step < 2; ++step)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float a = t[8 * step + 2 * k], b = t[8 * step + 2 * k + 1];
+              const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
+              w[0][x][step][k] = pack_half2(ah, bh);
+              if constexpr (PREC)
+                w[kParts - 1][x][step][k] = pack_half2(static_cast<_Float16>(a - static_cast<float>(ah)),
+                                                       static_cast<_Float16>(b - static_cast<float>(bh)));
+            }
+        }
+        // ---- weights times values
+#pragma unroll
+        for (int i = 0; i < kSlices; ++i)
+#pragma unroll
+          for (int step = 0; step < 2; ++step) {
+            const uint8_t* at = value_at + (32 * tile + 16 * step) * kValueRow + 64 * i;
+            const u32x2 lo = lds_read_tr16(at), hi = lds_read_tr16(at + 8 * kValueRow);
+            const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+            for (int x = 0; x < C; ++x) {
+              acc[x][i] = mfma32(v, w[0][x][step], acc[x][i]);
+              if constexpr (PREC) acc[x][i] = mfma32(v, w[kParts - 1][x][step], acc[x][i]);
+            }
+            if constexpr (PREC) {
+              const u32x2 lo2 = lds_read_tr16(at + kValueBytes), hi2 = lds_read_tr16(at + kValueBytes + 8 * kValueRow);
+              const u32x4 v2 = {lo2[0], lo2[1], hi2[0], hi2[1]};
+#pragma unroll
+              for (int x = 0; x < C; ++x) acc[x][i] = mfma32(v2, w[0][x][step], acc[x][i]);
+            }
+          }
+      }
+    }
+    __syncthreads();
+    if (n + 1 < n_end) unpack_stage(next);
+    __syncthreads();
+  }
+
+  // ---- waves of the same rows are joined (their halves of the slots in LDS, one after the other)
+#pragma unroll
+  for (int x = 0; x < C; ++x) l[x] += __shfl_xor(l[x], 32, kWave);
+  if (p.parts > 1) {
+    float* shared = reinterpret_cast<float*>(lds);  // [wave][C][kSlices * 16 + 2][lane], of one part at a time
+    constexpr int kRow = kSlices * 16 + 2;
+    static_assert(C > 1 || kTiles == 1 || 2 * kRow * kWave * 4 <= kKeyBytes + kParts * kValueBytes, "two row tiles' accumulators");
+    for (int other = 1; other < p.parts; ++other) {
+      __syncthreads();
+      float* mine = shared + (wave % p.row_tiles) * C * kRow * kWave + lane;
+      if (part == other) {
+#pragma unroll
+        for (int x = 0; x < C; ++x) {
+#pragma unroll
+          for (int i = 0; i < kSlices; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mine[(x * kRow + 16 * i + r) * kWave] = acc[x][i][r];
+          mine[(x * kRow + kRow - 2) * kWave] = m[x];
+          mine[(x * kRow + kRow - 1) * kWave] = l[x];
+        }
+      }
+      __syncthreads();
+      if (part == 0) {
+#pragma unroll
+        for (int x = 0; x < C; ++x) {
+          const float m2 = mine[(x * kRow + kRow - 2) * kWave], l2 = mine[(x * kRow + kRow - 1) * kWave];
+          // (a part that saw nothing has l = 0, and its reference counts for nothing)
+          const float ref = l2 == 0.0f ? m[x] : l[x] == 0.0f ? m2 : fmaxf(m[x], m2);
+          const float a = l[x] == 0.0f ? 0.0f : exp2f(m[x] - ref), b = l2 == 0.0f ? 0.0f : exp2f(m2 - ref);
+          m[x] = ref;
+          l[x] = l[x] * a + l2 * b;
+#pragma unroll
+          for (int i = 0; i < kSlices; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[x][i][r] = acc[x][i][r] * a + mine[(x * kRow + 16 * i + r) * kWave] * b;
+        }
+      }
+    }
+  }
+  if (part != 0) return;
+
+  // ---- the result, or the run's partial
+  const float unit = (c.bits == 4 ? kUnpackScale<4> : kUnpackScale<2>) *
+                     __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - 29) << 23);
+#pragma unroll
+  for (int x = 0; x < C; ++x) {
+    const int row = wave_row0 + 32 * x + col;
+    if (row >= rows) continue;
+    const int head = kvh * p.gq + row - own[x] * p.gq;
+    const int64_t at = (token0 + own[x]) * p.query_heads + head;
+    const int64_t part_at = (static_cast<int64_t>(item) * c.kv_heads + kvh) * p.block_rows + row - block * p.block_rows;
+    const bool whole = runs == 1;
+    const bool none = l[x] == 0.0f;
+    const float by = !whole ? unit : none ? 0.0f : unit / l[x];
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int dim = 32 * i + 8 * j + 4 * half;
+        if (dim >= d) continue;
+        f32x4 v;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) v[y] = whole && none ? 0.0f : acc[x][i][4 * j + y] * by;
+        if (!whole) {
+          *reinterpret_cast<f32x4*>(p.part_o + part_at * d + dim) = v;
+        } else if (p.out_dtype == KVSSD_DTYPE_F32) {
+          *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + at * d + dim) = v;
+        } else {
+          u32x2 o;
+          if (p.out_dtype == KVSSD_DTYPE_F16) {
+            o = u32x2{pack_half2(static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1])),
+                      pack_half2(static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3]))};
+          } else {
+            o = u32x2{store_cast<uint16_t>(v[0]) | static_cast<uint32_t>(store_cast<uint16_t>(v[1])) << 16,
+                      store_cast<uint16_t>(v[2]) | static_cast<uint32_t>(store_cast<uint16_t>(v[3])) << 16};
+          }
+          *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + at * d + dim) = o;
+        }
+      }
+    if (half == 0) {
+      if (whole) {
+        p.lse[at] = none ? -INFINITY : kLn2 * (m[x] + log2f(l[x]));
+      } else {
+        p.part_ml[2 * part_at] = m[x];
+        p.part_ml[2 * part_at + 1] = l[x];
+      }
+    }
+  }
+}
+
+template <int DP, int C, bool PREC>
+int launch_paged_tokens_kernel(const PagedTokensParams& p, unsigned groups, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_tokens_kernel<DP, C, PREC>), dim3(groups), dim3(kTokenWaves * kWave), 0, stream, p);
+  return hip_status(hipGetLastError(), "paged_tokens launch");
+}
+
+}  // namespace kvssd

@@ -1,0 +1,12 @@
+// Attention of many tokens a sequence, head_dim padded to 256.
+#include "paged_tokens.hpp"
+
+namespace kvssd {
+
+template <>
+int launch_paged_tokens_dims<256>(const PagedTokensParams& p, int columns, bool precise, unsigned groups, hipStream_t stream) {
+  return precise ? launch_paged_tokens_kernel<256, 1, true>(p, groups, stream)
+                 : launch_paged_tokens_kernel<256, 1, false>(p, groups, stream);
+}
+
+}  // namespace kvssd

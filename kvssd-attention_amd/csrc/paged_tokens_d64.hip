@@ -1,0 +1,13 @@
+// Attention of many tokens a sequence, head_dim padded to 64.
+#include "paged_tokens.hpp"
+
+namespace kvssd {
+
+template <>
+int launch_paged_tokens_dims<64>(const PagedTokensParams& p, int columns, bool precise, unsigned groups, hipStream_t stream) {
+  if (columns == 2) return launch_paged_tokens_kernel<64, 2, false>(p, groups, stream);
+  return precise ? launch_paged_tokens_kernel<64, 1, true>(p, groups, stream)
+                 : launch_paged_tokens_kernel<64, 1, false>(p, groups, stream);
+}
+
+}  // namespace kvssd
