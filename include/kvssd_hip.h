@@ -403,8 +403,8 @@ int kvssd_hip_paged_decode(const kvssd_paged_cache* cache, const kvssd_paged_dec
  * (0: the table's capacity, for every sequence); lengths beyond them are
  * answered all the same.  Arithmetic as kvssd_hip_paged_decode's. */
 typedef struct kvssd_paged_tokens_args {
-  kvssd_heads query; /* query.out is not used */
-  void* out;
+  kvssd_heads query; /* query.out is not used; the data, tokens and heads 16-byte aligned */
+  void* out;         /* 16-byte aligned */
   float* lse;
   const int32_t* offsets; /* [sequences + 1] */
   const int32_t* parents; /* [tokens] or NULL */

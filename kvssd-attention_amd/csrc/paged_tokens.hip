@@ -93,18 +93,16 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   p.query_dtype = a.query_dtype;
   p.out_dtype = a.out_query_dtype ? a.query_dtype : KVSSD_DTYPE_F32;
   p.groups = c.head_dim / c.group_size;
+  p.of_page = divisor(c.page_tokens);
   while ((32 << p.slices_log2) < c.group_size) ++p.slices_log2;
   p.scale_log2 = static_cast<float>(a.sm_scale) * kLog2e;
-  const int64_t item = static_cast<int64_t>(dtype_bytes(a.query_dtype));
-  p.vector_query = reinterpret_cast<uintptr_t>(a.query.data) % 16 == 0 && a.query.token_stride * item % 16 == 0 &&
-                   a.query.head_stride * item % 16 == 0;
   plan->precise = p.out_dtype == KVSSD_DTYPE_F32 || p.query_dtype == KVSSD_DTYPE_F32;
   plan->dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
   const int stage = tokens_stage(plan->dp);
 
   // rows of a workgroup, after a sequence's rows on average
   const int64_t each = (a.tokens * p.gq + c.sequences - 1) / c.sequences;
-  plan->columns = each > 128 && !plan->precise && plan->dp <= 128 ? 2 : 1;
+  plan->columns = 1;
   p.row_tiles = each > 64 ? 4 : each > 32 ? 2 : 1;
   const int tiles = stage / 32;
   p.parts = kTokenWaves / p.row_tiles < tiles ? kTokenWaves / p.row_tiles : tiles;
@@ -149,6 +147,8 @@ int launch_paged_tokens(const kvssd_paged_cache& c, const kvssd_paged_tokens_arg
   if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need))
     return arg_error("workspace too small: need " + std::to_string(need) + " bytes");
   if (reinterpret_cast<uintptr_t>(a.workspace) % 256) return arg_error("workspace must be 256-byte aligned");
+  if (!heads_vector(a.query, dtype_bytes(a.query_dtype), false))
+    return arg_error("query must be 16-byte aligned, as must its tokens and heads be");
   if (reinterpret_cast<uintptr_t>(a.out) % 16) return arg_error("out must be 16-byte aligned");
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + plan.o_bytes);

@@ -33,6 +33,7 @@
 #pragma once
 
 #include "paged_decode.hpp"
+#include "rotary_ops.hpp"
 
 namespace kvssd {
 
@@ -53,7 +54,7 @@ struct PagedTokensParams {
   int capacity, window, sink;
   int query_heads, gq, query_dtype, out_dtype;
   int groups, slices_log2;  // scale groups of a head; 32-dim slices of a group
-  int vector_query;         // 16-byte loads of the query
+  Divisor of_page;          // slots of a page
   int row_tiles, parts;     // of a workgroup: waves side by side on rows, on slots
   int block_rows;           // rows of a workgroup
   int items;                // (row block, run) pairs that the grid and the workspace hold
@@ -245,6 +246,14 @@ __device__ __forceinline__ void unpack_piece(const uint32_t* x, const Masks& k, 
   }
 }
 
+// s[r] = dot[r] * (scale of lane r of the lane's row of 16) + s[r]: the broadcast is the multiply-add's own operand
+template <int R>
+__device__ __forceinline__ void scale_rows(f32x16& s, const f32x16& dot, float scale, bool first) {
+  const float by = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, scale), 0x150 + R, 0xF, 0xF, true));
+  s[R] = first ? by * dot[R] : __builtin_fmaf(by, dot[R], s[R]);
+  if constexpr (R < 15) scale_rows<R + 1>(s, dot, scale, first);
+}
+
 // C: columns of 32 query rows a wave
 template <int DP, int C, bool PREC>
 __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) void paged_tokens_kernel(PagedTokensParams p) {
@@ -259,7 +268,7 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
   constexpr int kPlain = 14;                      // exponent of the scales that the largest factor (2^15) serves
   // keys: [chunk of 8 dims][slot] 16 bytes each, slots turned by their chunk; values: [part][slot][dim]
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kKeyBytes + kParts * kValueBytes];
-  __shared__ __attribute__((aligned(16))) uint16_t scale_lds[kSlices][kTiles][2][16];
+  __shared__ float scale_lds[kSlices][kTiles][2][16];  // keys': of slots 8 (i / 4) + 4 half + i % 4 of a tile
   __shared__ uint64_t live_lds[kTokenWaves], bad_lds[kTokenWaves];
   __shared__ int top_lds[kTokenWaves];
   uint8_t* const key_lds = lds;
@@ -295,8 +304,10 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
   const int d = c.head_dim, row_bytes = d * c.bits / 8;
   const bool has_dims = slice * 32 < d;
   const int piece_bytes = 4 * c.bits;
-  const int group = slice >> p.slices_log2;
   const int32_t* pages = c.page_table + static_cast<int64_t>(seq < c.sequences ? seq : 0) * c.max_pages;
+  // of the pool's row 0
+  const uint32_t slot_bytes = c.kv_heads * row_bytes, slot_scales = c.kv_heads * p.groups;
+  const uint32_t piece_at = kvh * row_bytes + slice * piece_bytes, scale_at = kvh * p.groups + (slice >> p.slices_log2);
   struct Piece {
     uint32_t k[4], v[4];
     uint16_t sk, sv;
@@ -304,16 +315,17 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
   } next{};
   auto page_of = [&](int n) {  // of the piece's slot in the list's stage n; -1: none
     const int slot = list.stage(n) * kStage + piece_slot;
-    return n < n_end && slot < length ? pages[slot / c.page_tokens] : -1;
+    return n < n_end && slot < length ? pages[p.of_page.quotient(slot)] : -1;
   };
   auto load = [&](int n, int page) {
     Piece x{};
     if (n < n_end && page >= 0 && page < c.num_pages) {
       const int slot = list.stage(n) * kStage + piece_slot;
-      const int64_t at = (static_cast<int64_t>(page) * c.page_tokens + slot % c.page_tokens) * c.kv_heads + kvh;
+      const uint32_t row = page * c.page_tokens + slot - p.of_page.quotient(slot) * c.page_tokens;
       x.live = true;
       if (has_dims) {
-        const int64_t byte = at * row_bytes + slice * piece_bytes;
+        const uint64_t byte = static_cast<uint64_t>(row) * slot_bytes + piece_at;
+        const uint64_t scale = static_cast<uint64_t>(row) * slot_scales + scale_at;
         if (c.bits == 4) {
           __builtin_memcpy(x.k, __builtin_assume_aligned(c.packed_k + byte, 16), 16);
           __builtin_memcpy(x.v, __builtin_assume_aligned(c.packed_v + byte, 16), 16);
@@ -321,8 +333,8 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
           __builtin_memcpy(x.k, __builtin_assume_aligned(c.packed_k + byte, 8), 8);
           __builtin_memcpy(x.v, __builtin_assume_aligned(c.packed_v + byte, 8), 8);
         }
-        x.sk = c.scales_k[at * p.groups + group];
-        x.sv = c.scales_v[at * p.groups + group];
+        x.sk = c.scales_k[scale];
+        x.sv = c.scales_v[scale];
       }
     }
     return x;
@@ -348,33 +360,35 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
       const int32_t* parents = p.parents + token0;
       for (int up = parent_of(parents, own[x]); up >= 0; up = parent_of(parents, up)) ++place[x];
     }
-    const int item_bytes = p.query_dtype == KVSSD_DTYPE_F32 ? 4 : 2;
-    const uint8_t* src = static_cast<const uint8_t*>(p.query.data) +
-                         ((token0 + own[x]) * p.query.token_stride + head * p.query.head_stride) * item_bytes;
+    const int64_t from = (token0 + own[x]) * p.query.token_stride + head * p.query.head_stride;
+    const bool wide = PREC && p.query_dtype == KVSSD_DTYPE_F32, bf16 = p.query_dtype == KVSSD_DTYPE_BF16;
+    u32x4 raw[DP / 16][kParts];  // dims 16 j + 8 half ..
     float big = 0.0f;
-    auto span = [&](int j, float (&v)[8]) {  // dims 16 j + 8 half ..
-      const int dim = 16 * j + 8 * half;
-      if (!active || dim >= d) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-      } else if (p.vector_query) {
-        query_span<8>(src, p.query_dtype, dim, v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (p.query_dtype == KVSSD_DTYPE_F32) v[i] = reinterpret_cast<const float*>(src)[dim + i];
-          else if (p.query_dtype == KVSSD_DTYPE_F16) v[i] = static_cast<float>(reinterpret_cast<const _Float16*>(src)[dim + i]);
-          else v[i] = __builtin_bit_cast(float, static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(src)[dim + i]) << 16);
+    auto value = [&](int j, int i) {
+      const uint32_t word = raw[j][i / 2 / 4][i / 2 % 4];
+      if constexpr (PREC) {
+        if (wide) {
+          const uint32_t whole = raw[j][i / 4][i % 4];
+          return __builtin_bit_cast(float, whole);
         }
       }
+      const float as_half = i % 2 ? half_hi(word) : half_lo(word);
+      return bf16 ? __builtin_bit_cast(float, i % 2 ? word & 0xFFFF0000u : word << 16) : as_half;
     };
 #pragma unroll
     for (int j = 0; j < DP / 16; ++j) {
-      float v[8];
-      span(j, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(v[i]));
+      const int dim = 16 * j + 8 * half;
+      raw[j][0] = raw[j][kParts - 1] = u32x4{0, 0, 0, 0};
+      if (active && dim < d) {
+        const uint8_t* src = static_cast<const uint8_t*>(p.query.data) + (from + dim) * (wide ? 4 : 2);
+        raw[j][0] = *reinterpret_cast<const u32x4*>(src);
+        if (wide) raw[j][kParts - 1] = *reinterpret_cast<const u32x4*>(src + 16);
+      }
     }
+#pragma unroll
+    for (int j = 0; j < DP / 16; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(value(j, i)));
     big = fmaxf(big, __shfl_xor(big, 32, kWave));
     int ex = static_cast<int>((__builtin_bit_cast(uint32_t, big) >> 23) & 255u);
     ex = ex < 12 ? 12 : (ex > 253 ? 253 : ex);
@@ -383,19 +397,16 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
     const float scale_down = __builtin_bit_cast(float, static_cast<uint32_t>(127 - up) << 23);
     factor[x] = scale_down * ((c.bits == 4 ? kUnpackScale<4> : kUnpackScale<2>) * p.scale_log2);
 #pragma unroll
-    for (int j = 0; j < DP / 16; ++j) {  // (the values again, from the cache: fewer registers)
-      float v[8];
-      span(j, v);
+    for (int j = 0; j < DP / 16; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float a = v[2 * i] * scale_up, b = v[2 * i + 1] * scale_up;
+        const float a = value(j, 2 * i) * scale_up, b = value(j, 2 * i + 1) * scale_up;
         const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
         q[0][x][j][i] = pack_half2(ah, bh);
         if constexpr (PREC)
           q[kParts - 1][x][j][i] = pack_half2(static_cast<_Float16>(a - static_cast<float>(ah)),
                                               static_cast<_Float16>(b - static_cast<float>(bh)));
       }
-    }
   }
   // of the wave's rows: first and last token, as slots
   const int own_lo = base + scalar(min(wave_row0, rows - 1) / p.gq);
@@ -418,7 +429,7 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
       *reinterpret_cast<u32x4*>(key_lds + (chunk * kStage + (piece_slot ^ (chunk / kTurn))) * 16) = codes[w];
     }
     const int in_tile = piece_slot % 32;
-    scale_lds[slice][piece_slot / 32][in_tile >> 2 & 1][(in_tile >> 3) * 4 + in_tile % 4] = x.sk;
+    scale_lds[slice][piece_slot / 32][in_tile >> 2 & 1][(in_tile >> 3) * 4 + in_tile % 4] = half_bits_to_float(x.sk);
     const int ex = x.sv >> 10 & 31;
     const bool bad = ex == 31;
     const int most = max(top, static_cast<int>(wave_most(bad ? 0u : static_cast<uint32_t>(ex))));
@@ -456,16 +467,190 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
 
   f32x16 acc[C][kSlices];
   float m[C], l[C];
+  float behind = 1.0f;  // what the accumulators are to be multiplied by, since the values' scale has changed
+  uint32_t poison[C];   // slices of a row that see a value scale that is not finite
 #pragma unroll
   for (int x = 0; x < C; ++x) {
     m[x] = -3.0e38f;
     l[x] = 0.0f;
+    poison[x] = 0;
 #pragma unroll
     for (int i = 0; i < kSlices; ++i) acc[x][i] = f32x16{};
   }
 
   // where the lane reads: keys of slot 32 tile + col, values of slots 16 step + 4 half + (lane / 4) % 4, dims 16 (lane / 16 % 2) + 4 (lane % 4)
   const uint8_t* const value_at = value_lds + (4 * half + (lane >> 2 & 3)) * kValueRow + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
+
+  // One tile of 32 slots.  `plain`: every row sees all of it, its values' scale is the accumulators' and finite.
+  auto work_tile = [&](int tile, int t0, bool plain, bool all_live, bool any_bad) {
+    const int t1 = t0 + 31;
+    // ---- scores
+    u32x4 key[2 * kSlices];
+    float sk[kSlices];
+    int at_col = 32 * tile + col;
+    asm volatile("" : "+v"(at_col));  // (a register for every turn of it would be kept otherwise)
+#pragma unroll
+    for (int i = 0; i < 2 * kSlices; ++i) {
+      const int turn = 2 * i / kTurn;  // (of chunks 2 i and 2 i + 1, one turn unless kTurn is 1)
+      const int slot = at_col ^ (kTurn == 1 ? turn + half : turn);
+      __builtin_memcpy(&key[i], __builtin_assume_aligned(key_lds + ((2 * i + half) * kStage + slot) * 16, 16), 16);
+    }
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i) sk[i] = scale_lds[i][tile][half][lane & 15];  // a slot's a lane, alike in the half's two rows
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16 s[C];
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i) {
+#pragma unroll
+      for (int x = 0; x < C; ++x) {
+        f32x16 dot = {};
+#pragma unroll
+        for (int j = 2 * i; j < 2 * i + 2; ++j) {
+          dot = mfma32(key[j], q[0][x][j], dot);
+          if constexpr (PREC) {
+            if (two_parts) dot = mfma32(key[j], q[kParts - 1][x][j], dot);
+          }
+        }
+        scale_rows<0>(s[x], dot, sk[i], i == 0);
+        asm volatile("" : "+v"(s[x]));  // here, and not where it is used: the products would all be kept until then
+      }
+    }
+    // ---- the values set out
+    constexpr int kAhead = DP <= 128 ? 2 * kSlices : kSlices;  // steps
+    u32x4 value[kAhead];
+    auto fetch = [&](int n) {  // step n % 2 of slice n / 2
+      const uint8_t* at = value_at + (32 * tile + 16 * (n % 2)) * kValueRow + 64 * (n / 2);
+      const u32x2 lo = lds_read_tr16(at), hi = lds_read_tr16(at + 8 * kValueRow);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) value[i] = fetch(i);
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- weights
+    u32x4 w[kParts][C][2];
+#pragma unroll
+    for (int x = 0; x < C; ++x) {
+      uint32_t seen = 0xFFFFu;  // of the lane's slots: bit r, slot 8 (r / 4) + 4 half + r % 4
+      if (!plain) {
+        uint32_t bits = 0xFFFFFFFFu;  // of the tile's slots
+        const int before = p.parents ? base : base + own[x] + 1;  // slots below it are seen, but for the window
+        bits = before >= t0 + 32 ? bits : before <= t0 ? 0u : (1u << (before - t0)) - 1;
+        if (p.window > 0) {
+          const int low = place[x] - p.window + 1;  // slots from here on, or below the sinks' end
+          const uint32_t from = low <= t0 ? ~0u : low >= t0 + 32 ? 0u : ~0u << (low - t0);
+          const uint32_t sinks = p.sink >= t0 + 32 ? ~0u : p.sink <= t0 ? 0u : (1u << (p.sink - t0)) - 1;
+          bits &= from | sinks;
+        }
+        if (p.parents != nullptr && t1 >= base) {
+          const int32_t* parents = p.parents + token0;
+          int at = place[x];
+          for (int up = own[x]; up >= 0 && base + up >= t0; up = parent_of(parents, up), --at)
+            if (base + up <= t1 && (p.window == 0 || at > place[x] - p.window || at < p.sink)) bits |= 1u << (base + up - t0);
+        }
+        if (!all_live) {
+#pragma unroll
+          for (int w4 = 0; w4 < 32 / kOwn || w4 == 0; ++w4) {
+            // the tile's slots of one wave's pieces, kSlices lanes each
+            const uint64_t live = live_lds[(32 * tile) / kOwn + w4];
+            constexpr int kHere = kOwn < 32 ? kOwn : 32;
+            for (int y = 0; y < kHere; ++y)
+              if (!(live >> ((32 * tile % kOwn + y) * kSlices) & 1)) bits &= ~(1u << (w4 * kOwn + y));
+          }
+        }
+        bits >>= 4 * half;
+        seen = (bits & 0xFu) | (bits >> 4 & 0xF0u) | (bits >> 8 & 0xF00u) | (bits >> 12 & 0xF000u);
+      }
+      float most = -INFINITY;
+      float t[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        t[r] = __builtin_fmaf(s[x][r], factor[x], -m[x]);
+      }
+      if (!plain) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t[r] = seen >> r & 1u ? t[r] : -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = fmaxf(most, t[r]);
+      if (__any(most > kRoom) || behind != 1.0f) {
+        float now = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) now = fmaxf(now, seen >> r & 1u ? s[x][r] * factor[x] : -INFINITY);
+        most = fmaxf(most, __shfl_xor(most, 32, kWave));
+        now = fmaxf(now, __shfl_xor(now, 32, kWave));
+        const float ref = most > kRoom ? now - kBias : m[x];
+        const float alpha = most > kRoom ? exp2f(m[x] - ref) : 1.0f;
+        m[x] = ref;
+        l[x] *= alpha;
+#pragma unroll
+        for (int i = 0; i < kSlices; ++i) acc[x][i] *= alpha * behind;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          t[r] = seen >> r & 1u ? __builtin_fmaf(s[x][r], factor[x], -ref) : -INFINITY;
+      }
+      float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        t[r] = __builtin_amdgcn_exp2f(t[r]);
+        sum[r % 2] += t[r];
+      }
+      l[x] += sum[0] + sum[1];
+      if (!plain) {
+        if (any_bad) {
+          for (int y = 0; y < 32; ++y) {  // slots of the tile with a value scale that is not finite
+            const int of_wave = (32 * tile + y) / kOwn;
+            const uint32_t groups = static_cast<uint32_t>(bad_lds[of_wave] >> ((32 * tile + y) % kOwn * kSlices)) & ((1u << kSlices) - 1);
+            if (scalar(groups) == 0) continue;
+            const int r = (y >> 3) * 4 + y % 4;
+            const int here = half == (y >> 2 & 1) && (seen >> r & 1u);
+            if (here | __shfl_xor(here, 32, kWave)) poison[x] |= groups;
+          }
+        }
+        // values that were scaled by less than the largest so far
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int less = top - scalar(top_lds[(32 * tile + 8 * j) / kOwn]);
+          const float by = __builtin_bit_cast(float, static_cast<uint32_t>(127 - less) << 23);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[4 * j + i] *= by;
+        }
+      }
+#pragma unroll
+      for (int step = 0; step < 2; ++step)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          typedef float f32x2 __attribute__((ext_vector_type(2)));
+          const f32x2 v = {t[8 * step + 2 * k], t[8 * step + 2 * k + 1]};
+          const half2v h = __builtin_convertvector(v, half2v);
+          w[0][x][step][k] = __builtin_bit_cast(uint32_t, h);
+          if constexpr (PREC) {
+            const half2v rest = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), half2v);
+            w[kParts - 1][x][step][k] = __builtin_bit_cast(uint32_t, rest);
+          }
+        }
+    }
+    behind = 1.0f;
+    // ---- weights times values
+#pragma unroll
+    for (int n = 0; n < 2 * kSlices; ++n) {
+      const int i = n / 2, step = n % 2;
+      const u32x4 v = value[n % kAhead];
+      if (n + kAhead < 2 * kSlices) value[n % kAhead] = fetch(n + kAhead);
+#pragma unroll
+      for (int x = 0; x < C; ++x) {
+        acc[x][i] = mfma32(v, w[0][x][step], acc[x][i]);
+        if constexpr (PREC) acc[x][i] = mfma32(v, w[kParts - 1][x][step], acc[x][i]);
+      }
+      if constexpr (PREC) {
+        const uint8_t* at = value_at + kValueBytes + (32 * tile + 16 * step) * kValueRow + 64 * i;
+        const u32x2 lo = lds_read_tr16(at), hi = lds_read_tr16(at + 8 * kValueRow);
+        const u32x4 v2 = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+        for (int x = 0; x < C; ++x) acc[x][i] = mfma32(v2, w[0][x][step], acc[x][i]);
+      }
+    }
+  };
 
   unpack_stage(next);
   __syncthreads();
@@ -487,11 +672,7 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
     any_bad = scalar(any_bad);
     const int top_new = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
     if (top_new != top) {
-      const float less = __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - top_new) << 23);
-#pragma unroll
-      for (int x = 0; x < C; ++x)
-#pragma unroll
-        for (int i = 0; i < kSlices; ++i) acc[x][i] *= less;
+      behind *= __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - top_new) << 23);
       top = top_new;
     }
     const bool even = tops[0] == top && tops[1] == top && tops[2] == top && tops[3] == top;
@@ -506,153 +687,7 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
           if (t1 <= reach_lo - p.window && t0 >= p.sink) continue;
         }
         if (t0 > own_hi) continue;
-        // ---- scores
-        f32x16 s[C];
-#pragma unroll
-        for (int i = 0; i < kSlices; ++i) {
-          f32x16 dot[C];
-#pragma unroll
-          for (int x = 0; x < C; ++x) dot[x] = f32x16{};
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int chunk = 4 * i + 2 * j + half;
-            u32x4 a;
-            __builtin_memcpy(&a, __builtin_assume_aligned(key_lds + (chunk * kStage + ((32 * tile + col) ^ (chunk / kTurn))) * 16, 16), 16);
-#pragma unroll
-            for (int x = 0; x < C; ++x) {
-              dot[x] = mfma32(a, q[0][x][2 * i + j], dot[x]);
-              if constexpr (PREC) {
-                if (two_parts) dot[x] = mfma32(a, q[kParts - 1][x][2 * i + j], dot[x]);
-              }
-            }
-          }
-          uint32_t sk[8];
-          __builtin_memcpy(sk, __builtin_assume_aligned(scale_lds[i][tile][half], 16), 32);
-#pragma unroll
-          for (int x = 0; x < C; ++x)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[x][r] = __builtin_fmaf(dot[x][r], half_of(sk, r), i == 0 ? 0.0f : s[x][r]);
-        }
-        // ---- weights
-        u32x4 w[kParts][C][2];
-#pragma unroll
-        for (int x = 0; x < C; ++x) {
-          uint32_t seen = 0xFFFFu;  // of the lane's slots: bit r, slot 8 (r / 4) + 4 half + r % 4
-          if (!all) {
-            uint32_t bits = 0xFFFFFFFFu;  // of the tile's slots
-            const int before = p.parents ? base : base + own[x] + 1;  // slots below it are seen, but for the window
-            bits = before >= t0 + 32 ? bits : before <= t0 ? 0u : (1u << (before - t0)) - 1;
-            if (p.window > 0) {
-              const int low = place[x] - p.window + 1;  // slots from here on, or below the sinks' end
-              const uint32_t from = low <= t0 ? ~0u : low >= t0 + 32 ? 0u : ~0u << (low - t0);
-              const uint32_t sinks = p.sink >= t0 + 32 ? ~0u : p.sink <= t0 ? 0u : (1u << (p.sink - t0)) - 1;
-              bits &= from | sinks;
-            }
-            if (p.parents != nullptr && t1 >= base) {
-              const int32_t* parents = p.parents + token0;
-              int at = place[x];
-              for (int up = own[x]; up >= 0 && base + up >= t0; up = parent_of(parents, up), --at)
-                if (base + up <= t1 && (p.window == 0 || at > place[x] - p.window || at < p.sink)) bits |= 1u << (base + up - t0);
-            }
-            if (!all_live) {
-#pragma unroll
-              for (int w4 = 0; w4 < 32 / kOwn || w4 == 0; ++w4) {
-                // the tile's slots of one wave's pieces, kSlices lanes each
-                const int of_wave = (32 * tile) / kOwn + w4;
-                const uint64_t live = live_lds[of_wave];
-                constexpr int kHere = kOwn < 32 ? kOwn : 32;
-                for (int y = 0; y < kHere; ++y)
-                  if (!(live >> ((32 * tile % kOwn + y) * kSlices) & 1)) bits &= ~(1u << (w4 * kOwn + y));
-              }
-            }
-            bits >>= 4 * half;
-            seen = (bits & 0xFu) | (bits >> 4 & 0xF0u) | (bits >> 8 & 0xF00u) | (bits >> 12 & 0xF000u);
-          }
-          float most = -INFINITY;
-          float t[16];
-#pragma unroll
-          for (int r = 0; r < 16; ++r) t[r] = __builtin_fmaf(s[x][r], factor[x], -m[x]);
-          if (!all) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) t[r] = seen >> r & 1u ? t[r] : -INFINITY;
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) most = fmaxf(most, t[r]);
-          if (__any(most > kRoom)) {
-            float now = -INFINITY;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) now = fmaxf(now, seen >> r & 1u ? s[x][r] * factor[x] : -INFINITY);
-            most = fmaxf(most, __shfl_xor(most, 32, kWave));
-            now = fmaxf(now, __shfl_xor(now, 32, kWave));
-            const float ref = most > kRoom ? now - kBias : m[x];
-            const float alpha = most > kRoom ? exp2f(m[x] - ref) : 1.0f;
-            m[x] = ref;
-            l[x] *= alpha;
-#pragma unroll
-            for (int i = 0; i < kSlices; ++i) acc[x][i] *= alpha;
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              t[r] = seen >> r & 1u ? __builtin_fmaf(s[x][r], factor[x], -ref) : -INFINITY;
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            t[r] = __builtin_amdgcn_exp2f(t[r]);
-            l[x] += t[r];
-          }
-          if (any_bad) {
-            for (int y = 0; y < 32; ++y) {  // slots of the tile with a value scale that is not finite
-              const int of_wave = (32 * tile + y) / kOwn;
-              const uint32_t groups = static_cast<uint32_t>(bad_lds[of_wave] >> ((32 * tile + y) % kOwn * kSlices)) & ((1u << kSlices) - 1);
-              if (scalar(groups) == 0) continue;
-              const int r = (y >> 3) * 4 + y % 4;
-              const int here = half == (y >> 2 & 1) && (seen >> r & 1u);
-              const int sees = here | __shfl_xor(here, 32, kWave);
-#pragma unroll
-              for (int i = 0; i < kSlices; ++i)
-                if (sees && (groups >> i & 1u)) acc[x][i] += __builtin_nanf("");
-            }
-          }
-          if (!even) {  // values that were scaled by less than the largest so far
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int less = top - scalar(top_lds[(32 * tile + 8 * j) / kOwn]);
-              const float by = __builtin_bit_cast(float, static_cast<uint32_t>(127 - less) << 23);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) t[4 * j + i] *= by;
-            }
-          }
-#pragma unroll
-          for (int step = 0; step < 2; ++step)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float a = t[8 * step + 2 * k], b = t[8 * step + 2 * k + 1];
-              const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
-              w[0][x][step][k] = pack_half2(ah, bh);
-              if constexpr (PREC)
-                w[kParts - 1][x][step][k] = pack_half2(static_cast<_Float16>(a - static_cast<float>(ah)),
-                                                       static_cast<_Float16>(b - static_cast<float>(bh)));
-            }
-        }
-        // ---- weights times values
-#pragma unroll
-        for (int i = 0; i < kSlices; ++i)
-#pragma unroll
-          for (int step = 0; step < 2; ++step) {
-            const uint8_t* at = value_at + (32 * tile + 16 * step) * kValueRow + 64 * i;
-            const u32x2 lo = lds_read_tr16(at), hi = lds_read_tr16(at + 8 * kValueRow);
-            const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-            for (int x = 0; x < C; ++x) {
-              acc[x][i] = mfma32(v, w[0][x][step], acc[x][i]);
-              if constexpr (PREC) acc[x][i] = mfma32(v, w[kParts - 1][x][step], acc[x][i]);
-            }
-            if constexpr (PREC) {
-              const u32x2 lo2 = lds_read_tr16(at + kValueBytes), hi2 = lds_read_tr16(at + kValueBytes + 8 * kValueRow);
-              const u32x4 v2 = {lo2[0], lo2[1], hi2[0], hi2[1]};
-#pragma unroll
-              for (int x = 0; x < C; ++x) acc[x][i] = mfma32(v2, w[0][x][step], acc[x][i]);
-            }
-          }
+        work_tile(tile, t0, all && even && !any_bad, all_live, any_bad);
       }
     }
     __syncthreads();
@@ -662,7 +697,11 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
 
   // ---- waves of the same rows are joined (their halves of the slots in LDS, one after the other)
 #pragma unroll
-  for (int x = 0; x < C; ++x) l[x] += __shfl_xor(l[x], 32, kWave);
+  for (int x = 0; x < C; ++x) {
+    l[x] += __shfl_xor(l[x], 32, kWave);
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i) acc[x][i] *= poison[x] >> i & 1u ? __builtin_nanf("") : behind;
+  }
   if (p.parts > 1) {
     float* shared = reinterpret_cast<float*>(lds);  // [wave][C][kSlices * 16 + 2][lane], of one part at a time
     constexpr int kRow = kSlices * 16 + 2;

@@ -168,8 +168,9 @@ class PreparedPagedTokens(PreparedPagedDecode):
     ) -> tuple[torch.Tensor, torch.Tensor]:
         self._match(query)
         self._batch.validate_lists(query.shape[0], offsets, parents)
-        if query.stride(2) != 1:
-            query = query.contiguous()
+        token, head, one = query.stride()
+        if one != 1 or query.data_ptr() % 16 or token * query.itemsize % 16 or head * query.itemsize % 16:
+            query = query.clone(memory_format=torch.contiguous_format)  # the kernel reads 16 bytes at a time
         offsets = offsets if offsets.is_contiguous() else offsets.contiguous()
         if parents is not None and not parents.is_contiguous():
             parents = parents.contiguous()
