@@ -15,11 +15,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <int DP>
+template <int STAGE>
 __global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedTokensParams p) {
   const int kvh = blockIdx.x % p.c.kv_heads;
   int first;
-  const TokenItem work = find_item<tokens_stage(DP)>(p, blockIdx.x / p.c.kv_heads, true, &first);
+  const TokenItem work = find_item<STAGE>(p, blockIdx.x / p.c.kv_heads, true, &first);
   if (work.seq < 0 || work.runs == 1) return;
   const int d = p.c.head_dim, lanes = d / 4;
   const int rows = min(work.span.count * p.gq - work.block * p.block_rows, p.block_rows);
@@ -61,7 +61,7 @@ size_t aligned(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 struct Plan {
   PagedTokensParams p;
-  int dp, columns;
+  int dp, waves, stage;
   bool precise;
   int64_t blocks;  // at most
   size_t o_bytes, ml_bytes;
@@ -98,15 +98,14 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   p.scale_log2 = static_cast<float>(a.sm_scale) * kLog2e;
   plan->precise = p.out_dtype == KVSSD_DTYPE_F32 || p.query_dtype == KVSSD_DTYPE_F32;
   plan->dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
-  const int stage = tokens_stage(plan->dp);
 
   // rows of a workgroup, after a sequence's rows on average
   const int64_t each = (a.tokens * p.gq + c.sequences - 1) / c.sequences;
-  plan->columns = 1;
-  p.row_tiles = each > 64 ? 4 : each > 32 ? 2 : 1;
-  const int tiles = stage / 32;
-  p.parts = kTokenWaves / p.row_tiles < tiles ? kTokenWaves / p.row_tiles : tiles;
-  p.block_rows = 32 * plan->columns * p.row_tiles;
+  plan->waves = each > 128 && !plan->precise && plan->dp <= 128 ? 8 : 4;
+  const int stage = plan->stage = tokens_stage(plan->dp, plan->waves);
+  p.row_tiles = each > 128 ? plan->waves : each > 64 ? 4 : each > 32 ? 2 : 1;
+  p.parts = plan->waves / p.row_tiles < stage / 32 ? plan->waves / p.row_tiles : stage / 32;
+  p.block_rows = 32 * p.row_tiles;
   plan->blocks = a.tokens * p.gq / p.block_rows + c.sequences + 2;
 
   // runs, where blocks alone would leave compute units idle
@@ -157,12 +156,13 @@ int launch_paged_tokens(const kvssd_paged_cache& c, const kvssd_paged_tokens_arg
   const auto launch = plan.dp == 64    ? launch_paged_tokens_dims<64>
                       : plan.dp == 128 ? launch_paged_tokens_dims<128>
                                        : launch_paged_tokens_dims<256>;
-  if (int rc = launch(p, plan.columns, plan.precise, groups, stream)) return rc;
+  if (int rc = launch(p, plan.waves, plan.precise, groups, stream)) return rc;
   if (need == 0) return 0;
   const dim3 grid(static_cast<unsigned>(plan.blocks * c.kv_heads));
-  if (plan.dp == 64) hipLaunchKernelGGL(paged_tokens_merge_kernel<64>, grid, dim3(kThreads), 0, stream, p);
-  else if (plan.dp == 128) hipLaunchKernelGGL(paged_tokens_merge_kernel<128>, grid, dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL(paged_tokens_merge_kernel<256>, grid, dim3(kThreads), 0, stream, p);
+  if (plan.stage == 256) hipLaunchKernelGGL(paged_tokens_merge_kernel<256>, grid, dim3(kThreads), 0, stream, p);
+  else if (plan.stage == 128) hipLaunchKernelGGL(paged_tokens_merge_kernel<128>, grid, dim3(kThreads), 0, stream, p);
+  else if (plan.stage == 64) hipLaunchKernelGGL(paged_tokens_merge_kernel<64>, grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL(paged_tokens_merge_kernel<32>, grid, dim3(kThreads), 0, stream, p);
   return hip_status(hipGetLastError(), "paged_tokens_merge launch");
 }
 

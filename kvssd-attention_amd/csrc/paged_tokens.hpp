@@ -37,9 +37,8 @@
 
 namespace kvssd {
 
-constexpr int kTokenWaves = 4;
-
-constexpr int tokens_stage(int dp) { return 8192 / dp; }  // slots: a thread's piece is 32 dims of one
+// slots of a stage: a thread of `waves` has a piece of 32 dims of one
+constexpr int tokens_stage(int dp, int waves) { return waves * 2048 / dp; }
 
 struct PagedTokensParams {
   kvssd_paged_cache c;
@@ -214,13 +213,13 @@ __device__ __forceinline__ void place_of(const PagedTokensParams& p, int id, int
 }
 
 template <int DP>
-int launch_paged_tokens_dims(const PagedTokensParams& p, int columns, bool precise, unsigned groups, hipStream_t stream);
+int launch_paged_tokens_dims(const PagedTokensParams& p, int waves, bool precise, unsigned groups, hipStream_t stream);
 template <>
-int launch_paged_tokens_dims<64>(const PagedTokensParams& p, int columns, bool precise, unsigned groups, hipStream_t stream);
+int launch_paged_tokens_dims<64>(const PagedTokensParams& p, int waves, bool precise, unsigned groups, hipStream_t stream);
 template <>
-int launch_paged_tokens_dims<128>(const PagedTokensParams& p, int columns, bool precise, unsigned groups, hipStream_t stream);
+int launch_paged_tokens_dims<128>(const PagedTokensParams& p, int waves, bool precise, unsigned groups, hipStream_t stream);
 template <>
-int launch_paged_tokens_dims<256>(const PagedTokensParams& p, int columns, bool precise, unsigned groups, hipStream_t stream);
+int launch_paged_tokens_dims<256>(const PagedTokensParams& p, int waves, bool precise, unsigned groups, hipStream_t stream);
 
 // ------------------------------------------------------------------ kernel ---
 
@@ -246,33 +245,57 @@ __device__ __forceinline__ void unpack_piece(const uint32_t* x, const Masks& k, 
   }
 }
 
-// s[r] = dot[r] * (scale of lane r of the lane's row of 16) + s[r]: the broadcast is the multiply-add's own operand
+// s[r] = dot[r] * (scale of lane r of the lane's row of 16) + s[r], r from R to 15
 template <int R>
-__device__ __forceinline__ void scale_rows(f32x16& s, const f32x16& dot, float scale, bool first) {
+__device__ __forceinline__ void scale_rows(float (&s)[16], const f32x16& dot, float scale) {
   const float by = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, scale), 0x150 + R, 0xF, 0xF, true));
-  s[R] = first ? by * dot[R] : __builtin_fmaf(by, dot[R], s[R]);
-  if constexpr (R < 15) scale_rows<R + 1>(s, dot, scale, first);
+  s[R] = by * dot[R];
+  if constexpr (R < 15) scale_rows<R + 1>(s, dot, scale);
+}
+// The same added to what v holds, here and now (else the products would all be kept to where v is used).  The compiler makes two instructions of each (a broadcast, a multiply-add); here the
+// broadcast is the multiply-add's operand.  What such assembly needs of its surroundings: the results of a matrix
+// instruction may be read some time after it only, which the compiler sees to at the first row's product, that it forms
+// itself and that the others take as an operand, so that they follow it; and a broadcast register must not have been
+// written just before, hence the s_nop.
+__device__ __forceinline__ void add_scaled_rows(float (&v)[16], const f32x16& dot, float scale) {
+  const float by = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, scale), 0x150, 0xF, 0xF, true));
+  v[0] = __builtin_fmaf(by, dot[0], v[0]);
+#define KVSSD_ROW(out, in, r) "v_fmac_f32_dpp " out ", %[scale], " in " row_newbcast:" #r " row_mask:0xf bank_mask:0xf bound_ctrl:1\n\t"
+  asm volatile("s_nop 1\n\t" KVSSD_ROW("%[s1]", "%[d1]", 1) KVSSD_ROW("%[s2]", "%[d2]", 2) KVSSD_ROW("%[s3]", "%[d3]", 3)
+                   KVSSD_ROW("%[s4]", "%[d4]", 4) KVSSD_ROW("%[s5]", "%[d5]", 5) KVSSD_ROW("%[s6]", "%[d6]", 6)
+                       KVSSD_ROW("%[s7]", "%[d7]", 7)
+               : [s1] "+v"(v[1]), [s2] "+v"(v[2]), [s3] "+v"(v[3]), [s4] "+v"(v[4]), [s5] "+v"(v[5]), [s6] "+v"(v[6]), [s7] "+v"(v[7])
+               : [scale] "v"(scale), [after] "v"(v[0]), [d1] "v"(dot[1]), [d2] "v"(dot[2]), [d3] "v"(dot[3]), [d4] "v"(dot[4]),
+                 [d5] "v"(dot[5]), [d6] "v"(dot[6]), [d7] "v"(dot[7]));
+  asm volatile("s_nop 1\n\t" KVSSD_ROW("%[s1]", "%[d1]", 8) KVSSD_ROW("%[s2]", "%[d2]", 9) KVSSD_ROW("%[s3]", "%[d3]", 10)
+                   KVSSD_ROW("%[s4]", "%[d4]", 11) KVSSD_ROW("%[s5]", "%[d5]", 12) KVSSD_ROW("%[s6]", "%[d6]", 13)
+                       KVSSD_ROW("%[s7]", "%[d7]", 14) KVSSD_ROW("%[s8]", "%[d8]", 15)
+               : [s1] "+v"(v[8]), [s2] "+v"(v[9]), [s3] "+v"(v[10]), [s4] "+v"(v[11]), [s5] "+v"(v[12]), [s6] "+v"(v[13]),
+                 [s7] "+v"(v[14]), [s8] "+v"(v[15])
+               : [scale] "v"(scale), [after] "v"(v[0]), [d1] "v"(dot[8]), [d2] "v"(dot[9]), [d3] "v"(dot[10]), [d4] "v"(dot[11]),
+                 [d5] "v"(dot[12]), [d6] "v"(dot[13]), [d7] "v"(dot[14]), [d8] "v"(dot[15]));
+#undef KVSSD_ROW
 }
 
-// C: columns of 32 query rows a wave
-template <int DP, int C, bool PREC>
-__global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) void paged_tokens_kernel(PagedTokensParams p) {
-  constexpr int kStage = tokens_stage(DP);
+// W: waves.  Small blocks take four, two workgroups a CU; large ones eight, which unpack a stage twice as long together.
+template <int DP, int W, bool PREC>
+__global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) void paged_tokens_kernel(PagedTokensParams p) {
+  constexpr int kStage = tokens_stage(DP, W);
   constexpr int kSlices = DP / 32;
   constexpr int kParts = PREC ? 2 : 1;
+  constexpr int kBuffers = PREC ? 1 : 2;          // stages in LDS: one is unpacked while another is worked on
   constexpr int kTiles = kStage / 32;             // of a stage
-  constexpr int kOwn = kStage / kTokenWaves;      // slots of a wave's pieces
+  constexpr int kOwn = kStage / W;                // slots of a wave's pieces
   constexpr int kValueRow = DP * 2 + 32;          // bytes; transposed reads of four rows meet in no bank
   constexpr int kKeyBytes = DP * kStage * 2, kValueBytes = kValueRow * kStage;
+  constexpr int kBytes = kKeyBytes + kParts * kValueBytes;
   constexpr float kBias = 8.0f, kRoom = 14.0f;    // log2 of a weight at the reference's maximum, and at most
   constexpr int kPlain = 14;                      // exponent of the scales that the largest factor (2^15) serves
   // keys: [chunk of 8 dims][slot] 16 bytes each, slots turned by their chunk; values: [part][slot][dim]
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kKeyBytes + kParts * kValueBytes];
-  __shared__ float scale_lds[kSlices][kTiles][2][16];  // keys': of slots 8 (i / 4) + 4 half + i % 4 of a tile
-  __shared__ uint64_t live_lds[kTokenWaves], bad_lds[kTokenWaves];
-  __shared__ int top_lds[kTokenWaves];
-  uint8_t* const key_lds = lds;
-  uint8_t* const value_lds = lds + kKeyBytes;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers][kBytes];
+  __shared__ float scale_lds[kBuffers][kSlices][kTiles][2][16];  // keys': of slots 8 (i / 4) + 4 half + i % 4 of a tile
+  __shared__ uint64_t live_lds[kBuffers][W], bad_lds[kBuffers][W];
+  __shared__ int top_lds[kBuffers][W];
 
   const kvssd_paged_cache& c = p.c;
   const int tid = threadIdx.x, lane = tid % kWave, wave = scalar(tid / kWave);
@@ -339,33 +362,32 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
     }
     return x;
   };
+  next = load(n_begin, page_of(n_begin));
+  int page_next = page_of(n_begin + 1);
 
   // ---- the wave's rows
   const int part = wave / p.row_tiles;
   const bool active = part < p.parts;
-  const int wave_row0 = block * p.block_rows + (wave % p.row_tiles) * 32 * C;
-  u32x4 q[kParts][C][DP / 16];
-  float factor[C];
-  int own[C], place[C];  // a column's token among the sequence's, and its position
-  const bool two_parts = PREC && p.query_dtype == KVSSD_DTYPE_F32;
-  int page_next = page_of(n_begin);
-#pragma unroll
-  for (int x = 0; x < C; ++x) {
-    const int row = min(wave_row0 + 32 * x + col, rows - 1);
-    own[x] = row / p.gq;
-    const int head = kvh * p.gq + row - own[x] * p.gq;
-    place[x] = base + own[x];
-    if (p.parents != nullptr && seq < c.sequences) {
-      place[x] = base;
-      const int32_t* parents = p.parents + token0;
-      for (int up = parent_of(parents, own[x]); up >= 0; up = parent_of(parents, up)) ++place[x];
-    }
-    const int64_t from = (token0 + own[x]) * p.query.token_stride + head * p.query.head_stride;
-    const bool wide = PREC && p.query_dtype == KVSSD_DTYPE_F32, bf16 = p.query_dtype == KVSSD_DTYPE_BF16;
+  const int wave_row0 = block * p.block_rows + (wave % p.row_tiles) * 32;
+  const int row = min(wave_row0 + col, rows - 1);
+  const int own = row / p.gq;  // the lane's token among the sequence's, and its position
+  int place = base + own;
+  if (p.parents != nullptr && seq < c.sequences) {
+    place = base;
+    const int32_t* parents = p.parents + token0;
+    for (int up = parent_of(parents, own); up >= 0; up = parent_of(parents, up)) ++place;
+  }
+  const int head = kvh * p.gq + row - own * p.gq;
+  u32x4 q[kParts][DP / 16];
+  float factor;
+  const bool wide = PREC && p.query_dtype == KVSSD_DTYPE_F32;
+  {
+    const int64_t from = (token0 + own) * p.query.token_stride + head * p.query.head_stride;
+    const bool bf16 = p.query_dtype == KVSSD_DTYPE_BF16;
     u32x4 raw[DP / 16][kParts];  // dims 16 j + 8 half ..
     float big = 0.0f;
     auto value = [&](int j, int i) {
-      const uint32_t word = raw[j][i / 2 / 4][i / 2 % 4];
+      const uint32_t word = raw[j][0][i / 2];
       if constexpr (PREC) {
         if (wide) {
           const uint32_t whole = raw[j][i / 4][i % 4];
@@ -395,22 +417,30 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
     const int up = 10 + 127 - ex;  // 2^up big in [2^10, 2^11)
     const float scale_up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + up) << 23);
     const float scale_down = __builtin_bit_cast(float, static_cast<uint32_t>(127 - up) << 23);
-    factor[x] = scale_down * ((c.bits == 4 ? kUnpackScale<4> : kUnpackScale<2>) * p.scale_log2);
+    factor = scale_down * ((c.bits == 4 ? kUnpackScale<4> : kUnpackScale<2>) * p.scale_log2);
+    // the keys' order of a chunk's dims: INT4 (0, 4) (1, 5) (2, 6) (3, 7), INT2 as they are
+    auto ordered = [&](u32x4 x) {
+      const u32x4 y = {low_halves(x[0], x[2]), high_halves(x[0], x[2]), low_halves(x[1], x[3]), high_halves(x[1], x[3])};
+      return c.bits == 4 ? y : x;
+    };
 #pragma unroll
-    for (int j = 0; j < DP / 16; ++j)
+    for (int j = 0; j < DP / 16; ++j) {
+      u32x4 hi, lo = {};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float a = value(j, 2 * i) * scale_up, b = value(j, 2 * i + 1) * scale_up;
         const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
-        q[0][x][j][i] = pack_half2(ah, bh);
+        hi[i] = pack_half2(ah, bh);
         if constexpr (PREC)
-          q[kParts - 1][x][j][i] = pack_half2(static_cast<_Float16>(a - static_cast<float>(ah)),
-                                              static_cast<_Float16>(b - static_cast<float>(bh)));
+          lo[i] = pack_half2(static_cast<_Float16>(a - static_cast<float>(ah)), static_cast<_Float16>(b - static_cast<float>(bh)));
       }
+      q[0][j] = ordered(hi);
+      if constexpr (PREC) q[kParts - 1][j] = ordered(lo);
+    }
   }
   // of the wave's rows: first and last token, as slots
   const int own_lo = base + scalar(min(wave_row0, rows - 1) / p.gq);
-  const int own_hi = base + scalar(min(wave_row0 + 32 * C, rows) - 1) / p.gq;
+  const int own_hi = base + scalar((min(wave_row0 + 32, rows) - 1) / p.gq);
 
   uint32_t zero = 0;
   asm("" : "+v"(zero));
@@ -419,25 +449,29 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
   constexpr int kTurn = DP / 64;  // a slot's place among its chunk's: slot ^ (chunk / kTurn), for writes of 8 lanes
   int top = kPlain;               // exponent that the accumulators' values are scaled by
 
-  auto unpack_stage = [&](const Piece& x) {
+  auto unpack_stage = [&](const Piece& x, int buf) {
     u32x4 codes[4];
-    if (c.bits == 4) unpack_piece<4>(x.k, masks, m01, m23, codes);
-    else unpack_piece<2>(x.k, masks, m01, m23, codes);
+    if (c.bits == 4) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) codes[w] = code_operand<4>(x.k[w], 0, masks, m01, m23);
+    } else {
+      unpack_piece<2>(x.k, masks, m01, m23, codes);
+    }
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const int chunk = 4 * slice + w;
-      *reinterpret_cast<u32x4*>(key_lds + (chunk * kStage + (piece_slot ^ (chunk / kTurn))) * 16) = codes[w];
+      *reinterpret_cast<u32x4*>(&lds[buf][(chunk * kStage + (piece_slot ^ (chunk / kTurn))) * 16]) = codes[w];
     }
     const int in_tile = piece_slot % 32;
-    scale_lds[slice][piece_slot / 32][in_tile >> 2 & 1][(in_tile >> 3) * 4 + in_tile % 4] = half_bits_to_float(x.sk);
+    scale_lds[buf][slice][piece_slot / 32][in_tile >> 2 & 1][(in_tile >> 3) * 4 + in_tile % 4] = half_bits_to_float(x.sk);
     const int ex = x.sv >> 10 & 31;
     const bool bad = ex == 31;
     const int most = max(top, static_cast<int>(wave_most(bad ? 0u : static_cast<uint32_t>(ex))));
     const uint64_t live = __ballot(x.live), bads = __ballot(bad);
     if (lane == 0) {
-      live_lds[wave] = live;
-      bad_lds[wave] = bads;
-      top_lds[wave] = most;
+      live_lds[buf][wave] = live;
+      bad_lds[buf][wave] = bads;
+      top_lds[buf][wave] = most;
     }
     if (c.bits == 4) unpack_piece<4>(x.v, masks, m01, m23, codes);
     else unpack_piece<2>(x.v, masks, m01, m23, codes);
@@ -455,343 +489,308 @@ __global__ __launch_bounds__(kTokenWaves * kWave, C == 1 && DP < 256 ? 2 : 1) vo
         hi[i] = __builtin_bit_cast(uint32_t, v);
         if constexpr (PREC) lo[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, ss, -v));
       }
-      uint8_t* dst = value_lds + piece_slot * kValueRow + slice * 64 + w * 16;
+      uint8_t* dst = &lds[buf][kKeyBytes + piece_slot * kValueRow + slice * 64 + w * 16];
       *reinterpret_cast<u32x4*>(dst) = hi;
       if constexpr (PREC) *reinterpret_cast<u32x4*>(dst + kValueBytes) = lo;
     }
   };
 
-  // ---- the first stage
-  next = load(n_begin, page_next);
-  page_next = page_of(n_begin + 1);
-
-  f32x16 acc[C][kSlices];
-  float m[C], l[C];
+  f32x16 acc[kSlices];
+#pragma unroll
+  for (int i = 0; i < kSlices; ++i) acc[i] = f32x16{};
+  float m = -3.0e38f, l = 0.0f;
   float behind = 1.0f;  // what the accumulators are to be multiplied by, since the values' scale has changed
-  uint32_t poison[C];   // slices of a row that see a value scale that is not finite
-#pragma unroll
-  for (int x = 0; x < C; ++x) {
-    m[x] = -3.0e38f;
-    l[x] = 0.0f;
-    poison[x] = 0;
-#pragma unroll
-    for (int i = 0; i < kSlices; ++i) acc[x][i] = f32x16{};
-  }
+  uint32_t poison = 0;  // slices of a row that see a value scale that is not finite
 
-  // where the lane reads: keys of slot 32 tile + col, values of slots 16 step + 4 half + (lane / 4) % 4, dims 16 (lane / 16 % 2) + 4 (lane % 4)
-  const uint8_t* const value_at = value_lds + (4 * half + (lane >> 2 & 3)) * kValueRow + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
+  // where the lane reads values: slots 16 step + 4 half + (lane / 4) % 4, dims 16 (lane / 16 % 2) + 4 (lane % 4)
+  const int value_at = kKeyBytes + (4 * half + (lane >> 2 & 3)) * kValueRow + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
 
   // One tile of 32 slots.  `plain`: every row sees all of it, its values' scale is the accumulators' and finite.
-  auto work_tile = [&](int tile, int t0, bool plain, bool all_live, bool any_bad) {
+  auto work_tile = [&](int buf, int tile, int t0, bool plain, bool all_live, bool any_bad) {
     const int t1 = t0 + 31;
+    const uint8_t* const stage = lds[buf];
     // ---- scores
-    u32x4 key[2 * kSlices];
-    float sk[kSlices];
+    constexpr int kKeys = DP <= 128 ? kSlices : kSlices / 2;  // slices whose keys are read together
+    float sk[kSlices], s[16];
     int at_col = 32 * tile + col;
     asm volatile("" : "+v"(at_col));  // (a register for every turn of it would be kept otherwise)
 #pragma unroll
-    for (int i = 0; i < 2 * kSlices; ++i) {
-      const int turn = 2 * i / kTurn;  // (of chunks 2 i and 2 i + 1, one turn unless kTurn is 1)
-      const int slot = at_col ^ (kTurn == 1 ? turn + half : turn);
-      __builtin_memcpy(&key[i], __builtin_assume_aligned(key_lds + ((2 * i + half) * kStage + slot) * 16, 16), 16);
-    }
+    for (int i = 0; i < kSlices; ++i) sk[i] = scale_lds[buf][i][tile][half][lane & 15];  // a slot's a lane, alike in the half's two rows
 #pragma unroll
-    for (int i = 0; i < kSlices; ++i) sk[i] = scale_lds[i][tile][half][lane & 15];  // a slot's a lane, alike in the half's two rows
-    __builtin_amdgcn_sched_barrier(0);
-    f32x16 s[C];
+    for (int first = 0; first < kSlices; first += kKeys) {
+      u32x4 key[2 * kKeys];
 #pragma unroll
-    for (int i = 0; i < kSlices; ++i) {
+      for (int i = 0; i < 2 * kKeys; ++i) {
+        const int chunk = 4 * first + 2 * i, turn = chunk / kTurn;  // (of this one and the next, one turn unless kTurn is 1)
+        const int slot = at_col ^ (kTurn == 1 ? turn + half : turn);
+        __builtin_memcpy(&key[i], __builtin_assume_aligned(stage + ((chunk + half) * kStage + slot) * 16, 16), 16);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x < C; ++x) {
+      for (int i = first; i < first + kKeys; ++i) {
         f32x16 dot = {};
 #pragma unroll
         for (int j = 2 * i; j < 2 * i + 2; ++j) {
-          dot = mfma32(key[j], q[0][x][j], dot);
+          dot = mfma32(key[j - 2 * first], q[0][j], dot);
           if constexpr (PREC) {
-            if (two_parts) dot = mfma32(key[j], q[kParts - 1][x][j], dot);
+            if (wide) dot = mfma32(key[j - 2 * first], q[kParts - 1][j], dot);
           }
         }
-        scale_rows<0>(s[x], dot, sk[i], i == 0);
-        asm volatile("" : "+v"(s[x]));  // here, and not where it is used: the products would all be kept until then
+        if (i == 0) scale_rows<0>(s, dot, sk[0]);
+        else add_scaled_rows(s, dot, sk[i]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     // ---- the values set out
-    constexpr int kAhead = DP <= 128 ? 2 * kSlices : kSlices;  // steps
+    constexpr int kAhead = PREC ? 2 : DP <= 128 ? 2 * kSlices : kSlices;  // steps
     u32x4 value[kAhead];
-    auto fetch = [&](int n) {  // step n % 2 of slice n / 2
-      const uint8_t* at = value_at + (32 * tile + 16 * (n % 2)) * kValueRow + 64 * (n / 2);
+    auto fetch = [&](int n, int from) {  // step n % 2 of slice n / 2
+      const uint8_t* at = stage + value_at + (32 * tile + 16 * (n % 2)) * kValueRow + 64 * (n / 2) + from;
       const u32x2 lo = lds_read_tr16(at), hi = lds_read_tr16(at + 8 * kValueRow);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) value[i] = fetch(i);
+    for (int i = 0; i < kAhead; ++i) value[i] = fetch(i, 0);
     __builtin_amdgcn_sched_barrier(0);
     // ---- weights
-    u32x4 w[kParts][C][2];
-#pragma unroll
-    for (int x = 0; x < C; ++x) {
-      uint32_t seen = 0xFFFFu;  // of the lane's slots: bit r, slot 8 (r / 4) + 4 half + r % 4
-      if (!plain) {
-        uint32_t bits = 0xFFFFFFFFu;  // of the tile's slots
-        const int before = p.parents ? base : base + own[x] + 1;  // slots below it are seen, but for the window
-        bits = before >= t0 + 32 ? bits : before <= t0 ? 0u : (1u << (before - t0)) - 1;
-        if (p.window > 0) {
-          const int low = place[x] - p.window + 1;  // slots from here on, or below the sinks' end
-          const uint32_t from = low <= t0 ? ~0u : low >= t0 + 32 ? 0u : ~0u << (low - t0);
-          const uint32_t sinks = p.sink >= t0 + 32 ? ~0u : p.sink <= t0 ? 0u : (1u << (p.sink - t0)) - 1;
-          bits &= from | sinks;
-        }
-        if (p.parents != nullptr && t1 >= base) {
-          const int32_t* parents = p.parents + token0;
-          int at = place[x];
-          for (int up = own[x]; up >= 0 && base + up >= t0; up = parent_of(parents, up), --at)
-            if (base + up <= t1 && (p.window == 0 || at > place[x] - p.window || at < p.sink)) bits |= 1u << (base + up - t0);
-        }
-        if (!all_live) {
-#pragma unroll
-          for (int w4 = 0; w4 < 32 / kOwn || w4 == 0; ++w4) {
-            // the tile's slots of one wave's pieces, kSlices lanes each
-            const uint64_t live = live_lds[(32 * tile) / kOwn + w4];
-            constexpr int kHere = kOwn < 32 ? kOwn : 32;
-            for (int y = 0; y < kHere; ++y)
-              if (!(live >> ((32 * tile % kOwn + y) * kSlices) & 1)) bits &= ~(1u << (w4 * kOwn + y));
-          }
-        }
-        bits >>= 4 * half;
-        seen = (bits & 0xFu) | (bits >> 4 & 0xF0u) | (bits >> 8 & 0xF00u) | (bits >> 12 & 0xF000u);
+    uint32_t seen = 0xFFFFu;  // of the lane's slots: bit r, slot 8 (r / 4) + 4 half + r % 4
+    if (!plain) {
+      uint32_t bits = 0xFFFFFFFFu;  // of the tile's slots
+      const int before = p.parents ? base : base + own + 1;  // slots below it are seen, but for the window
+      bits = before >= t0 + 32 ? bits : before <= t0 ? 0u : (1u << (before - t0)) - 1;
+      if (p.window > 0) {
+        const int low = place - p.window + 1;  // slots from here on, or below the sinks' end
+        const uint32_t from = low <= t0 ? ~0u : low >= t0 + 32 ? 0u : ~0u << (low - t0);
+        const uint32_t sinks = p.sink >= t0 + 32 ? ~0u : p.sink <= t0 ? 0u : (1u << (p.sink - t0)) - 1;
+        bits &= from | sinks;
       }
-      float most = -INFINITY;
-      float t[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        t[r] = __builtin_fmaf(s[x][r], factor[x], -m[x]);
+      if (p.parents != nullptr && t1 >= base) {
+        const int32_t* parents = p.parents + token0;
+        int at = place;
+        for (int up = own; up >= 0 && base + up >= t0; up = parent_of(parents, up), --at)
+          if (base + up <= t1 && (p.window == 0 || at > place - p.window || at < p.sink)) bits |= 1u << (base + up - t0);
       }
-      if (!plain) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) t[r] = seen >> r & 1u ? t[r] : -INFINITY;
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) most = fmaxf(most, t[r]);
-      if (__any(most > kRoom) || behind != 1.0f) {
-        float now = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) now = fmaxf(now, seen >> r & 1u ? s[x][r] * factor[x] : -INFINITY);
-        most = fmaxf(most, __shfl_xor(most, 32, kWave));
-        now = fmaxf(now, __shfl_xor(now, 32, kWave));
-        const float ref = most > kRoom ? now - kBias : m[x];
-        const float alpha = most > kRoom ? exp2f(m[x] - ref) : 1.0f;
-        m[x] = ref;
-        l[x] *= alpha;
-#pragma unroll
-        for (int i = 0; i < kSlices; ++i) acc[x][i] *= alpha * behind;
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          t[r] = seen >> r & 1u ? __builtin_fmaf(s[x][r], factor[x], -ref) : -INFINITY;
-      }
-      float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        t[r] = __builtin_amdgcn_exp2f(t[r]);
-        sum[r % 2] += t[r];
-      }
-      l[x] += sum[0] + sum[1];
-      if (!plain) {
-        if (any_bad) {
-          for (int y = 0; y < 32; ++y) {  // slots of the tile with a value scale that is not finite
-            const int of_wave = (32 * tile + y) / kOwn;
-            const uint32_t groups = static_cast<uint32_t>(bad_lds[of_wave] >> ((32 * tile + y) % kOwn * kSlices)) & ((1u << kSlices) - 1);
-            if (scalar(groups) == 0) continue;
-            const int r = (y >> 3) * 4 + y % 4;
-            const int here = half == (y >> 2 & 1) && (seen >> r & 1u);
-            if (here | __shfl_xor(here, 32, kWave)) poison[x] |= groups;
-          }
+      if (!all_live) {
+        constexpr int kHere = kOwn < 32 ? kOwn : 32;  // of the tile's slots, one wave's pieces; kSlices lanes each
+#pragma unroll 1
+        for (int y = 0; y < 32; ++y) {
+          const uint64_t live = live_lds[buf][(32 * tile + y) / kOwn];
+          if (!(live >> ((32 * tile + y) % kOwn * kSlices) & 1)) bits &= ~(1u << y);
         }
-        // values that were scaled by less than the largest so far
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int less = top - scalar(top_lds[(32 * tile + 8 * j) / kOwn]);
-          const float by = __builtin_bit_cast(float, static_cast<uint32_t>(127 - less) << 23);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) t[4 * j + i] *= by;
-        }
+        static_assert(kHere * kSlices <= kWave, "a wave's pieces");
       }
-#pragma unroll
-      for (int step = 0; step < 2; ++step)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          typedef float f32x2 __attribute__((ext_vector_type(2)));
-          const f32x2 v = {t[8 * step + 2 * k], t[8 * step + 2 * k + 1]};
-          const half2v h = __builtin_convertvector(v, half2v);
-          w[0][x][step][k] = __builtin_bit_cast(uint32_t, h);
-          if constexpr (PREC) {
-            const half2v rest = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), half2v);
-            w[kParts - 1][x][step][k] = __builtin_bit_cast(uint32_t, rest);
-          }
-        }
+      bits >>= 4 * half;
+      seen = (bits & 0xFu) | (bits >> 4 & 0xF0u) | (bits >> 8 & 0xF00u) | (bits >> 12 & 0xF000u);
     }
-    behind = 1.0f;
+    float most = -INFINITY;
+    float t[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t[r] = __builtin_fmaf(s[r], factor, -m);
+    if (!plain) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t[r] = seen >> r & 1u ? t[r] : -INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) most = fmaxf(most, t[r]);
+    if (__any(most > kRoom) || behind != 1.0f) {
+      float now = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) now = fmaxf(now, seen >> r & 1u ? s[r] * factor : -INFINITY);
+      most = fmaxf(most, __shfl_xor(most, 32, kWave));
+      now = fmaxf(now, __shfl_xor(now, 32, kWave));
+      const float ref = most > kRoom ? now - kBias : m;
+      const float alpha = most > kRoom ? exp2f(m - ref) : 1.0f;
+      m = ref;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < kSlices; ++i) acc[i] *= alpha * behind;
+      behind = 1.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t[r] = seen >> r & 1u ? __builtin_fmaf(s[r], factor, -ref) : -INFINITY;
+    }
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      t[r] = __builtin_amdgcn_exp2f(t[r]);
+      sum[r % 2] += t[r];
+    }
+    l += sum[0] + sum[1];
+    if (!plain) {
+      if (any_bad) {
+        for (int y = 0; y < 32; ++y) {  // slots of the tile with a value scale that is not finite
+          const uint64_t bads = bad_lds[buf][(32 * tile + y) / kOwn];
+          const uint32_t groups = static_cast<uint32_t>(bads >> ((32 * tile + y) % kOwn * kSlices)) & ((1u << kSlices) - 1);
+          if (scalar(groups) == 0) continue;
+          const int r = (y >> 3) * 4 + y % 4;
+          const int here = half == (y >> 2 & 1) && (seen >> r & 1u);
+          if (here | __shfl_xor(here, 32, kWave)) poison |= groups;
+        }
+      }
+      // values that were scaled by less than the largest so far
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int less = top - scalar(top_lds[buf][(32 * tile + 8 * j) / kOwn]);
+        const float by = __builtin_bit_cast(float, static_cast<uint32_t>(127 - less) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[4 * j + i] *= by;
+      }
+    }
+    u32x4 w[kParts][2];
+#pragma unroll
+    for (int step = 0; step < 2; ++step)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        const f32x2 v = {t[8 * step + 2 * k], t[8 * step + 2 * k + 1]};
+        const half2v h = __builtin_convertvector(v, half2v);
+        w[0][step][k] = __builtin_bit_cast(uint32_t, h);
+        if constexpr (PREC) {
+          const half2v rest = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), half2v);
+          w[kParts - 1][step][k] = __builtin_bit_cast(uint32_t, rest);
+        }
+      }
     // ---- weights times values
 #pragma unroll
     for (int n = 0; n < 2 * kSlices; ++n) {
       const int i = n / 2, step = n % 2;
       const u32x4 v = value[n % kAhead];
-      if (n + kAhead < 2 * kSlices) value[n % kAhead] = fetch(n + kAhead);
-#pragma unroll
-      for (int x = 0; x < C; ++x) {
-        acc[x][i] = mfma32(v, w[0][x][step], acc[x][i]);
-        if constexpr (PREC) acc[x][i] = mfma32(v, w[kParts - 1][x][step], acc[x][i]);
-      }
+      if (n + kAhead < 2 * kSlices) value[n % kAhead] = fetch(n + kAhead, 0);
+      acc[i] = mfma32(v, w[0][step], acc[i]);
       if constexpr (PREC) {
-        const uint8_t* at = value_at + kValueBytes + (32 * tile + 16 * step) * kValueRow + 64 * i;
-        const u32x2 lo = lds_read_tr16(at), hi = lds_read_tr16(at + 8 * kValueRow);
-        const u32x4 v2 = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-        for (int x = 0; x < C; ++x) acc[x][i] = mfma32(v2, w[0][x][step], acc[x][i]);
+        acc[i] = mfma32(v, w[kParts - 1][step], acc[i]);
+        acc[i] = mfma32(fetch(n, kValueBytes), w[0][step], acc[i]);
       }
     }
   };
 
-  unpack_stage(next);
+  // the stage after `n` into LDS, and the one after that on its way
+  auto advance = [&](int n) {
+    if (n + 1 < n_end) unpack_stage(next, kBuffers > 1 ? (n + 1 - n_begin) & 1 : 0);
+    next = load(n + 2, page_next);
+    page_next = page_of(n + 3);
+  };
+  advance(n_begin - 1);
   __syncthreads();
   for (int n = n_begin; n < n_end; ++n) {
-    // the next stage sets out
-    next = load(n + 1, page_next);
-    page_next = page_of(n + 2);
-    // ---- this stage
+    const int buf = kBuffers > 1 ? (n - n_begin) & 1 : 0;
     const int slot0 = list.stage(n) * kStage;
-    int tops[kTokenWaves];
+    int tops = 0, least = 31;
     bool all_live = true, any_bad = false;
 #pragma unroll
-    for (int w = 0; w < kTokenWaves; ++w) {
-      tops[w] = scalar(top_lds[w]);
-      all_live = all_live && live_lds[w] == ~0ull;
-      any_bad = any_bad || bad_lds[w] != 0;
+    for (int w = 0; w < W; ++w) {
+      const int e = scalar(top_lds[buf][w]);
+      tops = max(tops, e);
+      least = min(least, e);
+      all_live = all_live && live_lds[buf][w] == ~0ull;
+      any_bad = any_bad || bad_lds[buf][w] != 0;
     }
     all_live = scalar(all_live);
     any_bad = scalar(any_bad);
-    const int top_new = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
-    if (top_new != top) {
-      behind *= __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - top_new) << 23);
-      top = top_new;
+    if (tops != top) {
+      behind *= __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - tops) << 23);
+      top = tops;
     }
-    const bool even = tops[0] == top && tops[1] == top && tops[2] == top && tops[3] == top;
+    // (every other set of four waves unpacks first, so that a SIMD's two waves are not at the same thing)
+    if (kBuffers > 1 && W > 4 && wave / 4 % 2) advance(n);
     if (active) {
       for (int tile = part; tile < kTiles; tile += p.parts) {
         const int t0 = slot0 + 32 * tile, t1 = t0 + 31;
         // whether every row of the wave sees all of the tile's slots, or none
         const int reach_lo = p.parents ? base : own_lo;  // the lowest position; slots up to it are seen, but for the window
-        bool all = all_live && (p.parents ? t1 < base : t1 <= own_lo);
+        bool all = all_live && !any_bad && least == top && (p.parents ? t1 < base : t1 <= own_lo);
         if (p.window > 0) {
           all = all && (t0 > own_hi - p.window || t1 < p.sink);
           if (t1 <= reach_lo - p.window && t0 >= p.sink) continue;
         }
         if (t0 > own_hi) continue;
-        work_tile(tile, t0, all && even && !any_bad, all_live, any_bad);
+        work_tile(buf, tile, t0, all, all_live, any_bad);
       }
     }
-    __syncthreads();
-    if (n + 1 < n_end) unpack_stage(next);
+    if (kBuffers == 1) __syncthreads();
+    if (!(kBuffers > 1 && W > 4 && wave / 4 % 2)) advance(n);
     __syncthreads();
   }
 
-  // ---- waves of the same rows are joined (their halves of the slots in LDS, one after the other)
+  // ---- waves of the same rows are joined (their parts of the slots in LDS, one after the other)
+  l += __shfl_xor(l, 32, kWave);
 #pragma unroll
-  for (int x = 0; x < C; ++x) {
-    l[x] += __shfl_xor(l[x], 32, kWave);
-#pragma unroll
-    for (int i = 0; i < kSlices; ++i) acc[x][i] *= poison[x] >> i & 1u ? __builtin_nanf("") : behind;
-  }
+  for (int i = 0; i < kSlices; ++i) acc[i] *= poison >> i & 1u ? __builtin_nanf("") : behind;
   if (p.parts > 1) {
-    float* shared = reinterpret_cast<float*>(lds);  // [wave][C][kSlices * 16 + 2][lane], of one part at a time
     constexpr int kRow = kSlices * 16 + 2;
-    static_assert(C > 1 || kTiles == 1 || 2 * kRow * kWave * 4 <= kKeyBytes + kParts * kValueBytes, "two row tiles' accumulators");
+    static_assert(kTiles == 1 || W / 2 * kRow * kWave * 4 <= kBuffers * kBytes, "a part's accumulators");
+    float* mine = reinterpret_cast<float*>(lds[0]) + (wave % p.row_tiles) * kRow * kWave + lane;  // [row tile][kRow][lane]
     for (int other = 1; other < p.parts; ++other) {
       __syncthreads();
-      float* mine = shared + (wave % p.row_tiles) * C * kRow * kWave + lane;
       if (part == other) {
 #pragma unroll
-        for (int x = 0; x < C; ++x) {
+        for (int i = 0; i < kSlices; ++i)
 #pragma unroll
-          for (int i = 0; i < kSlices; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mine[(x * kRow + 16 * i + r) * kWave] = acc[x][i][r];
-          mine[(x * kRow + kRow - 2) * kWave] = m[x];
-          mine[(x * kRow + kRow - 1) * kWave] = l[x];
-        }
+          for (int r = 0; r < 16; ++r) mine[(16 * i + r) * kWave] = acc[i][r];
+        mine[(kRow - 2) * kWave] = m;
+        mine[(kRow - 1) * kWave] = l;
       }
       __syncthreads();
       if (part == 0) {
+        const float m2 = mine[(kRow - 2) * kWave], l2 = mine[(kRow - 1) * kWave];
+        // (a part that saw nothing has l = 0, and its reference counts for nothing)
+        const float ref = l2 == 0.0f ? m : l == 0.0f ? m2 : fmaxf(m, m2);
+        const float a = l == 0.0f ? 0.0f : exp2f(m - ref), b = l2 == 0.0f ? 0.0f : exp2f(m2 - ref);
+        m = ref;
+        l = l * a + l2 * b;
 #pragma unroll
-        for (int x = 0; x < C; ++x) {
-          const float m2 = mine[(x * kRow + kRow - 2) * kWave], l2 = mine[(x * kRow + kRow - 1) * kWave];
-          // (a part that saw nothing has l = 0, and its reference counts for nothing)
-          const float ref = l2 == 0.0f ? m[x] : l[x] == 0.0f ? m2 : fmaxf(m[x], m2);
-          const float a = l[x] == 0.0f ? 0.0f : exp2f(m[x] - ref), b = l2 == 0.0f ? 0.0f : exp2f(m2 - ref);
-          m[x] = ref;
-          l[x] = l[x] * a + l2 * b;
+        for (int i = 0; i < kSlices; ++i)
 #pragma unroll
-          for (int i = 0; i < kSlices; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[x][i][r] = acc[x][i][r] * a + mine[(x * kRow + 16 * i + r) * kWave] * b;
-        }
+          for (int r = 0; r < 16; ++r) acc[i][r] = acc[i][r] * a + mine[(16 * i + r) * kWave] * b;
       }
     }
   }
-  if (part != 0) return;
+  if (part != 0 || wave_row0 + col >= rows) return;
 
   // ---- the result, or the run's partial
+  const bool whole = runs == 1, none = l == 0.0f;
   const float unit = (c.bits == 4 ? kUnpackScale<4> : kUnpackScale<2>) *
                      __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - 29) << 23);
+  const int64_t at = (token0 + own) * p.query_heads + head;
+  const int64_t part_at = (static_cast<int64_t>(item) * c.kv_heads + kvh) * p.block_rows + row - block * p.block_rows;
+  const float by = !whole ? unit : none ? 0.0f : unit / l;
 #pragma unroll
-  for (int x = 0; x < C; ++x) {
-    const int row = wave_row0 + 32 * x + col;
-    if (row >= rows) continue;
-    const int head = kvh * p.gq + row - own[x] * p.gq;
-    const int64_t at = (token0 + own[x]) * p.query_heads + head;
-    const int64_t part_at = (static_cast<int64_t>(item) * c.kv_heads + kvh) * p.block_rows + row - block * p.block_rows;
-    const bool whole = runs == 1;
-    const bool none = l[x] == 0.0f;
-    const float by = !whole ? unit : none ? 0.0f : unit / l[x];
+  for (int i = 0; i < kSlices; ++i)
 #pragma unroll
-    for (int i = 0; i < kSlices; ++i)
+    for (int j = 0; j < 4; ++j) {
+      const int dim = 32 * i + 8 * j + 4 * half;
+      if (dim >= d) continue;
+      f32x4 v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int dim = 32 * i + 8 * j + 4 * half;
-        if (dim >= d) continue;
-        f32x4 v;
-#pragma unroll
-        for (int y = 0; y < 4; ++y) v[y] = whole && none ? 0.0f : acc[x][i][4 * j + y] * by;
-        if (!whole) {
-          *reinterpret_cast<f32x4*>(p.part_o + part_at * d + dim) = v;
-        } else if (p.out_dtype == KVSSD_DTYPE_F32) {
-          *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + at * d + dim) = v;
-        } else {
-          u32x2 o;
-          if (p.out_dtype == KVSSD_DTYPE_F16) {
-            o = u32x2{pack_half2(static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1])),
-                      pack_half2(static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3]))};
-          } else {
-            o = u32x2{store_cast<uint16_t>(v[0]) | static_cast<uint32_t>(store_cast<uint16_t>(v[1])) << 16,
-                      store_cast<uint16_t>(v[2]) | static_cast<uint32_t>(store_cast<uint16_t>(v[3])) << 16};
-          }
-          *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + at * d + dim) = o;
-        }
-      }
-    if (half == 0) {
-      if (whole) {
-        p.lse[at] = none ? -INFINITY : kLn2 * (m[x] + log2f(l[x]));
+      for (int y = 0; y < 4; ++y) v[y] = whole && none ? 0.0f : acc[i][4 * j + y] * by;
+      if (!whole) {
+        *reinterpret_cast<f32x4*>(p.part_o + part_at * d + dim) = v;
+      } else if (p.out_dtype == KVSSD_DTYPE_F32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + at * d + dim) = v;
       } else {
-        p.part_ml[2 * part_at] = m[x];
-        p.part_ml[2 * part_at + 1] = l[x];
+        u32x2 o;
+        if (p.out_dtype == KVSSD_DTYPE_F16) {
+          o = u32x2{pack_half2(static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1])),
+                    pack_half2(static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3]))};
+        } else {
+          o = u32x2{store_cast<uint16_t>(v[0]) | static_cast<uint32_t>(store_cast<uint16_t>(v[1])) << 16,
+                    store_cast<uint16_t>(v[2]) | static_cast<uint32_t>(store_cast<uint16_t>(v[3])) << 16};
+        }
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + at * d + dim) = o;
       }
+    }
+  if (half == 0) {
+    if (whole) {
+      p.lse[at] = none ? -INFINITY : kLn2 * (m + log2f(l));
+    } else {
+      p.part_ml[2 * part_at] = m;
+      p.part_ml[2 * part_at + 1] = l;
     }
   }
 }
 
-template <int DP, int C, bool PREC>
+template <int DP, int W, bool PREC>
 int launch_paged_tokens_kernel(const PagedTokensParams& p, unsigned groups, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_tokens_kernel<DP, C, PREC>), dim3(groups), dim3(kTokenWaves * kWave), 0, stream, p);
+  hipLaunchKernelGGL((paged_tokens_kernel<DP, W, PREC>), dim3(groups), dim3(W * kWave), 0, stream, p);
   return hip_status(hipGetLastError(), "paged_tokens launch");
 }
 
