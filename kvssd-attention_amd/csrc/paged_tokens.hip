@@ -104,7 +104,7 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   plan->waves = each > 128 && !plan->precise && plan->dp <= 128 ? 8 : 4;
   const int stage = plan->stage = tokens_stage(plan->dp, plan->waves);
   p.row_tiles = each > 128 ? plan->waves : each > 64 ? 4 : each > 32 ? 2 : 1;
-  p.parts = plan->waves / p.row_tiles < stage / 32 ? plan->waves / p.row_tiles : stage / 32;
+  p.parts = plan->waves / p.row_tiles < stage / 64 ? plan->waves / p.row_tiles : stage / 64;
   p.block_rows = 32 * p.row_tiles;
   plan->blocks = a.tokens * p.gq / p.block_rows + c.sequences + 2;
 
@@ -161,8 +161,7 @@ int launch_paged_tokens(const kvssd_paged_cache& c, const kvssd_paged_tokens_arg
   const dim3 grid(static_cast<unsigned>(plan.blocks * c.kv_heads));
   if (plan.stage == 256) hipLaunchKernelGGL(paged_tokens_merge_kernel<256>, grid, dim3(kThreads), 0, stream, p);
   else if (plan.stage == 128) hipLaunchKernelGGL(paged_tokens_merge_kernel<128>, grid, dim3(kThreads), 0, stream, p);
-  else if (plan.stage == 64) hipLaunchKernelGGL(paged_tokens_merge_kernel<64>, grid, dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL(paged_tokens_merge_kernel<32>, grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL(paged_tokens_merge_kernel<64>, grid, dim3(kThreads), 0, stream, p);
   return hip_status(hipGetLastError(), "paged_tokens_merge launch");
 }
 

@@ -37,8 +37,8 @@
 
 namespace kvssd {
 
-// slots of a stage: a thread of `waves` has a piece of 32 dims of one
-constexpr int tokens_stage(int dp, int waves) { return waves * 2048 / dp; }
+// slots of a stage, a multiple of 64: a thread of `waves` has a piece of 32 dims of one (of two, of long heads)
+constexpr int tokens_stage(int dp, int waves) { return waves * 2048 / dp < 64 ? 64 : waves * 2048 / dp; }
 
 struct PagedTokensParams {
   kvssd_paged_cache c;
@@ -245,35 +245,32 @@ __device__ __forceinline__ void unpack_piece(const uint32_t* x, const Masks& k, 
   }
 }
 
-// s[r] = dot[r] * (scale of lane r of the lane's row of 16) + s[r], r from R to 15
-template <int R>
+// s[r] = dot[r] * (scale of lane r of the lane's row of 16), r from R to END - 1
+template <int R, int END>
 __device__ __forceinline__ void scale_rows(float (&s)[16], const f32x16& dot, float scale) {
   const float by = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, scale), 0x150 + R, 0xF, 0xF, true));
   s[R] = by * dot[R];
-  if constexpr (R < 15) scale_rows<R + 1>(s, dot, scale);
+  if constexpr (R + 1 < END) scale_rows<R + 1, END>(s, dot, scale);
 }
-// The same added to what v holds, here and now (else the products would all be kept to where v is used).  The compiler makes two instructions of each (a broadcast, a multiply-add); here the
-// broadcast is the multiply-add's operand.  What such assembly needs of its surroundings: the results of a matrix
-// instruction may be read some time after it only, which the compiler sees to at the first row's product, that it forms
-// itself and that the others take as an operand, so that they follow it; and a broadcast register must not have been
-// written just before, hence the s_nop.
-__device__ __forceinline__ void add_scaled_rows(float (&v)[16], const f32x16& dot, float scale) {
-  const float by = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, scale), 0x150, 0xF, 0xF, true));
-  v[0] = __builtin_fmaf(by, dot[0], v[0]);
-#define KVSSD_ROW(out, in, r) "v_fmac_f32_dpp " out ", %[scale], " in " row_newbcast:" #r " row_mask:0xf bank_mask:0xf bound_ctrl:1\n\t"
-  asm volatile("s_nop 1\n\t" KVSSD_ROW("%[s1]", "%[d1]", 1) KVSSD_ROW("%[s2]", "%[d2]", 2) KVSSD_ROW("%[s3]", "%[d3]", 3)
-                   KVSSD_ROW("%[s4]", "%[d4]", 4) KVSSD_ROW("%[s5]", "%[d5]", 5) KVSSD_ROW("%[s6]", "%[d6]", 6)
-                       KVSSD_ROW("%[s7]", "%[d7]", 7)
+// The same added to what s holds, in rows 0 to 7 or 8 to 15.  The compiler makes two instructions of each (a broadcast, a
+// multiply-add); here the broadcast is the multiply-add's operand.  What such assembly needs of its surroundings: the
+// results of a matrix instruction may be read some time after it only, which the compiler sees to at the half's first
+// product, that it forms itself and that the others take as an operand, so that they follow it; and a broadcast register
+// must not have been written just before, hence the s_nop.
+template <int HALF>
+__device__ __forceinline__ void add_scaled_rows(float (&s)[16], const f32x16& dot, float scale) {
+  const float by =
+      __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, scale), 0x150 + 8 * HALF, 0xF, 0xF, true));
+  float* v = s + 8 * HALF;
+  constexpr int o = 8 * HALF;
+  v[0] = __builtin_fmaf(by, dot[o], v[0]);
+#define KVSSD_ROW(n, lo, hi) "v_fmac_f32_dpp %[s" #n "], %[scale], %[d" #n "] row_newbcast:%c[r" #n "] row_mask:0xf bank_mask:0xf bound_ctrl:1\n\t"
+  asm volatile("s_nop 1\n\t" KVSSD_ROW(1, 1, 9) KVSSD_ROW(2, 2, 10) KVSSD_ROW(3, 3, 11) KVSSD_ROW(4, 4, 12) KVSSD_ROW(5, 5, 13)
+                   KVSSD_ROW(6, 6, 14) KVSSD_ROW(7, 7, 15)
                : [s1] "+v"(v[1]), [s2] "+v"(v[2]), [s3] "+v"(v[3]), [s4] "+v"(v[4]), [s5] "+v"(v[5]), [s6] "+v"(v[6]), [s7] "+v"(v[7])
-               : [scale] "v"(scale), [after] "v"(v[0]), [d1] "v"(dot[1]), [d2] "v"(dot[2]), [d3] "v"(dot[3]), [d4] "v"(dot[4]),
-                 [d5] "v"(dot[5]), [d6] "v"(dot[6]), [d7] "v"(dot[7]));
-  asm volatile("s_nop 1\n\t" KVSSD_ROW("%[s1]", "%[d1]", 8) KVSSD_ROW("%[s2]", "%[d2]", 9) KVSSD_ROW("%[s3]", "%[d3]", 10)
-                   KVSSD_ROW("%[s4]", "%[d4]", 11) KVSSD_ROW("%[s5]", "%[d5]", 12) KVSSD_ROW("%[s6]", "%[d6]", 13)
-                       KVSSD_ROW("%[s7]", "%[d7]", 14) KVSSD_ROW("%[s8]", "%[d8]", 15)
-               : [s1] "+v"(v[8]), [s2] "+v"(v[9]), [s3] "+v"(v[10]), [s4] "+v"(v[11]), [s5] "+v"(v[12]), [s6] "+v"(v[13]),
-                 [s7] "+v"(v[14]), [s8] "+v"(v[15])
-               : [scale] "v"(scale), [after] "v"(v[0]), [d1] "v"(dot[8]), [d2] "v"(dot[9]), [d3] "v"(dot[10]), [d4] "v"(dot[11]),
-                 [d5] "v"(dot[12]), [d6] "v"(dot[13]), [d7] "v"(dot[14]), [d8] "v"(dot[15]));
+               : [scale] "v"(scale), [after] "v"(v[0]), [d1] "v"(dot[o + 1]), [d2] "v"(dot[o + 2]), [d3] "v"(dot[o + 3]),
+                 [d4] "v"(dot[o + 4]), [d5] "v"(dot[o + 5]), [d6] "v"(dot[o + 6]), [d7] "v"(dot[o + 7]), [r1] "n"(o + 1),
+                 [r2] "n"(o + 2), [r3] "n"(o + 3), [r4] "n"(o + 4), [r5] "n"(o + 5), [r6] "n"(o + 6), [r7] "n"(o + 7));
 #undef KVSSD_ROW
 }
 
@@ -285,7 +282,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   constexpr int kParts = PREC ? 2 : 1;
   constexpr int kBuffers = PREC ? 1 : 2;          // stages in LDS: one is unpacked while another is worked on
   constexpr int kTiles = kStage / 32;             // of a stage
-  constexpr int kOwn = kStage / W;                // slots of a wave's pieces
+  constexpr int kOwn = kWave / kSlices;           // slots of a wave's pieces at a time
+  constexpr int kGroups = kStage / kOwn;          // of so many slots
+  constexpr int kPieces = kGroups / W;            // of a thread
   constexpr int kValueRow = DP * 2 + 32;          // bytes; transposed reads of four rows meet in no bank
   constexpr int kKeyBytes = DP * kStage * 2, kValueBytes = kValueRow * kStage;
   constexpr int kBytes = kKeyBytes + kParts * kValueBytes;
@@ -294,8 +293,8 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   // keys: [chunk of 8 dims][slot] 16 bytes each, slots turned by their chunk; values: [part][slot][dim]
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers][kBytes];
   __shared__ float scale_lds[kBuffers][kSlices][kTiles][2][16];  // keys': of slots 8 (i / 4) + 4 half + i % 4 of a tile
-  __shared__ uint64_t live_lds[kBuffers][W], bad_lds[kBuffers][W];
-  __shared__ int top_lds[kBuffers][W];
+  __shared__ uint64_t live_lds[kBuffers][kGroups], bad_lds[kBuffers][kGroups];
+  __shared__ int top_lds[kBuffers][kGroups];
 
   const kvssd_paged_cache& c = p.c;
   const int tid = threadIdx.x, lane = tid % kWave, wave = scalar(tid / kWave);
@@ -323,7 +322,8 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   }
 
   // ---- a thread's pieces: 32 dims of a slot
-  const int piece_slot = tid / kSlices, slice = tid % kSlices;
+  const int first_slot = tid / kSlices, slice = tid % kSlices;
+  constexpr int kNext = W * kOwn;  // slots to the thread's next piece
   const int d = c.head_dim, row_bytes = d * c.bits / 8;
   const bool has_dims = slice * 32 < d;
   const int piece_bytes = 4 * c.bits;
@@ -335,15 +335,16 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     uint32_t k[4], v[4];
     uint16_t sk, sv;
     bool live;
-  } next{};
-  auto page_of = [&](int n) {  // of the piece's slot in the list's stage n; -1: none
-    const int slot = list.stage(n) * kStage + piece_slot;
+  } next[kPieces];
+  int page_next[kPieces];
+  auto page_of = [&](int n, int piece) {  // of the piece's slot in the list's stage n; -1: none
+    const int slot = list.stage(n) * kStage + first_slot + piece * kNext;
     return n < n_end && slot < length ? pages[p.of_page.quotient(slot)] : -1;
   };
-  auto load = [&](int n, int page) {
+  auto load = [&](int n, int piece, int page) {
     Piece x{};
     if (n < n_end && page >= 0 && page < c.num_pages) {
-      const int slot = list.stage(n) * kStage + piece_slot;
+      const int slot = list.stage(n) * kStage + first_slot + piece * kNext;
       const uint32_t row = page * c.page_tokens + slot - p.of_page.quotient(slot) * c.page_tokens;
       x.live = true;
       if (has_dims) {
@@ -362,8 +363,11 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     }
     return x;
   };
-  next = load(n_begin, page_of(n_begin));
-  int page_next = page_of(n_begin + 1);
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    next[i] = load(n_begin, i, page_of(n_begin, i));
+    page_next[i] = page_of(n_begin + 1, i);
+  }
 
   // ---- the wave's rows
   const int part = wave / p.row_tiles;
@@ -442,14 +446,15 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   const int own_lo = base + scalar(min(wave_row0, rows - 1) / p.gq);
   const int own_hi = base + scalar((min(wave_row0 + 32, rows) - 1) / p.gq);
 
-  uint32_t zero = 0;
-  asm("" : "+v"(zero));
-  const Masks masks = make_masks(zero);
-  const uint32_t m01 = 0x00030003u | zero, m23 = 0x000C000Cu | zero;
   constexpr int kTurn = DP / 64;  // a slot's place among its chunk's: slot ^ (chunk / kTurn), for writes of 8 lanes
   int top = kPlain;               // exponent that the accumulators' values are scaled by
 
-  auto unpack_stage = [&](const Piece& x, int buf) {
+  auto unpack_piece_into = [&](const Piece& x, int buf, int piece) {
+    const int piece_slot = first_slot + piece * kNext;
+    uint32_t zero = 0;
+    asm volatile("" : "+v"(zero));  // (masks live here only)
+    const Masks masks = make_masks(zero);
+    const uint32_t m01 = 0x00030003u | zero, m23 = 0x000C000Cu | zero;
     u32x4 codes[4];
     if (c.bits == 4) {
 #pragma unroll
@@ -469,9 +474,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     const int most = max(top, static_cast<int>(wave_most(bad ? 0u : static_cast<uint32_t>(ex))));
     const uint64_t live = __ballot(x.live), bads = __ballot(bad);
     if (lane == 0) {
-      live_lds[buf][wave] = live;
-      bad_lds[buf][wave] = bads;
-      top_lds[buf][wave] = most;
+      live_lds[buf][piece * W + wave] = live;
+      bad_lds[buf][piece * W + wave] = bads;
+      top_lds[buf][piece * W + wave] = most;
     }
     if (c.bits == 4) unpack_piece<4>(x.v, masks, m01, m23, codes);
     else unpack_piece<2>(x.v, masks, m01, m23, codes);
@@ -498,176 +503,206 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   f32x16 acc[kSlices];
 #pragma unroll
   for (int i = 0; i < kSlices; ++i) acc[i] = f32x16{};
-  float m = -3.0e38f, l = 0.0f;
+  float m = 0.0f, l = 0.0f;  // the reference, and the sum of the half's weights
   float behind = 1.0f;  // what the accumulators are to be multiplied by, since the values' scale has changed
   uint32_t poison = 0;  // slices of a row that see a value scale that is not finite
 
   // where the lane reads values: slots 16 step + 4 half + (lane / 4) % 4, dims 16 (lane / 16 % 2) + 4 (lane % 4)
   const int value_at = kKeyBytes + (4 * half + (lane >> 2 & 3)) * kValueRow + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
 
-  // One tile of 32 slots.  `plain`: every row sees all of it, its values' scale is the accumulators' and finite.
-  auto work_tile = [&](int buf, int tile, int t0, bool plain, bool all_live, bool any_bad) {
-    const int t1 = t0 + 31;
+  // Two tiles of 32 slots.  `plain`: every row sees all of them, their values' scale is the accumulators' and finite.
+  auto work_pair = [&](int buf, int tile, int t0, bool plain, bool all_live, bool any_bad) {
     const uint8_t* const stage = lds[buf];
-    // ---- scores
-    constexpr int kKeys = DP <= 128 ? kSlices : kSlices / 2;  // slices whose keys are read together
-    float sk[kSlices], s[16];
+    // ---- scores.  Steps: (slice, tile), the tiles in turn, so that a step's products are formed while those of the one
+    // before, of the other tile, are scaled
+    constexpr int kSteps = 2 * kSlices, kRing = 3;
+    float s[2][16], sk[kRing];
+    u32x4 key[kRing][2];
     int at_col = 32 * tile + col;
     asm volatile("" : "+v"(at_col));  // (a register for every turn of it would be kept otherwise)
+    auto read_keys = [&](int n) {
+      sk[n % kRing] = scale_lds[buf][n / 2][tile + n % 2][half][lane & 15];  // a slot's a lane, alike in the half's two rows
 #pragma unroll
-    for (int i = 0; i < kSlices; ++i) sk[i] = scale_lds[buf][i][tile][half][lane & 15];  // a slot's a lane, alike in the half's two rows
-#pragma unroll
-    for (int first = 0; first < kSlices; first += kKeys) {
-      u32x4 key[2 * kKeys];
-#pragma unroll
-      for (int i = 0; i < 2 * kKeys; ++i) {
-        const int chunk = 4 * first + 2 * i, turn = chunk / kTurn;  // (of this one and the next, one turn unless kTurn is 1)
-        const int slot = at_col ^ (kTurn == 1 ? turn + half : turn);
-        __builtin_memcpy(&key[i], __builtin_assume_aligned(stage + ((chunk + half) * kStage + slot) * 16, 16), 16);
+      for (int j = 0; j < 2; ++j) {
+        const int chunk = 4 * (n / 2) + 2 * j, turn = chunk / kTurn;  // (of this one and the next, one turn unless kTurn is 1)
+        const int slot = (at_col ^ (kTurn == 1 ? turn + half : turn)) + 32 * (n % 2);
+        __builtin_memcpy(&key[n % kRing][j], __builtin_assume_aligned(stage + ((chunk + half) * kStage + slot) * 16, 16), 16);
       }
+    };
+    auto product = [&](int n, int j, f32x16 to) {
+      to = mfma32(key[n % kRing][j], q[0][n / 2 * 2 + j], to);
+      if constexpr (PREC) {
+        if (wide) to = mfma32(key[n % kRing][j], q[kParts - 1][n / 2 * 2 + j], to);
+      }
+      return to;
+    };
+#pragma unroll
+    for (int n = 0; n < kRing; ++n) read_keys(n);
+    f32x16 dot[2];
+    dot[0] = product(0, 0, f32x16{});
+    dot[0] = product(0, 1, dot[0]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < kSteps; ++n) {
+      const bool more = n + 1 < kSteps;
+      const float by = sk[n % kRing];
+      if (n > 0 && n + kRing - 1 < kSteps) read_keys(n + kRing - 1);
+      if (more) dot[(n + 1) % 2] = product(n + 1, 0, f32x16{});
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = first; i < first + kKeys; ++i) {
-        f32x16 dot = {};
-#pragma unroll
-        for (int j = 2 * i; j < 2 * i + 2; ++j) {
-          dot = mfma32(key[j - 2 * first], q[0][j], dot);
-          if constexpr (PREC) {
-            if (wide) dot = mfma32(key[j - 2 * first], q[kParts - 1][j], dot);
-          }
-        }
-        if (i == 0) scale_rows<0>(s, dot, sk[0]);
-        else add_scaled_rows(s, dot, sk[i]);
-      }
+      if (n < 2) scale_rows<0, 8>(s[n % 2], dot[n % 2], by);
+      else add_scaled_rows<0>(s[n % 2], dot[n % 2], by);
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) dot[(n + 1) % 2] = product(n + 1, 1, dot[(n + 1) % 2]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (n < 2) scale_rows<8, 16>(s[n % 2], dot[n % 2], by);
+      else add_scaled_rows<1>(s[n % 2], dot[n % 2], by);
       __builtin_amdgcn_sched_barrier(0);
     }
-    // ---- the values set out
-    constexpr int kAhead = PREC ? 2 : DP <= 128 ? 2 * kSlices : kSlices;  // steps
+    // ---- the first tile's values set out
+    constexpr int kAhead = PREC ? 2 : DP <= 128 ? kSteps : kSlices;  // steps
     u32x4 value[kAhead];
-    auto fetch = [&](int n, int from) {  // step n % 2 of slice n / 2
-      const uint8_t* at = stage + value_at + (32 * tile + 16 * (n % 2)) * kValueRow + 64 * (n / 2) + from;
+    auto fetch = [&](int of, int n, int from) {  // of a tile, step n % 2 of slice n / 2
+      const uint8_t* at = stage + value_at + (32 * (tile + of) + 16 * (n % 2)) * kValueRow + 64 * (n / 2) + from;
       const u32x2 lo = lds_read_tr16(at), hi = lds_read_tr16(at + 8 * kValueRow);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) value[i] = fetch(i, 0);
+    for (int i = 0; i < kAhead; ++i) value[i] = fetch(0, i, 0);
     __builtin_amdgcn_sched_barrier(0);
-    // ---- weights
-    uint32_t seen = 0xFFFFu;  // of the lane's slots: bit r, slot 8 (r / 4) + 4 half + r % 4
+    // ---- weights: s is turned into log2 units above the reference, then into its powers
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[x][r] = __builtin_fmaf(s[x][r], factor, -m);
+    uint32_t seen[2];  // of the lane's slots: bit r, slot 8 (r / 4) + 4 half + r % 4
     if (!plain) {
-      uint32_t bits = 0xFFFFFFFFu;  // of the tile's slots
-      const int before = p.parents ? base : base + own + 1;  // slots below it are seen, but for the window
-      bits = before >= t0 + 32 ? bits : before <= t0 ? 0u : (1u << (before - t0)) - 1;
-      if (p.window > 0) {
-        const int low = place - p.window + 1;  // slots from here on, or below the sinks' end
-        const uint32_t from = low <= t0 ? ~0u : low >= t0 + 32 ? 0u : ~0u << (low - t0);
-        const uint32_t sinks = p.sink >= t0 + 32 ? ~0u : p.sink <= t0 ? 0u : (1u << (p.sink - t0)) - 1;
-        bits &= from | sinks;
-      }
-      if (p.parents != nullptr && t1 >= base) {
-        const int32_t* parents = p.parents + token0;
-        int at = place;
-        for (int up = own; up >= 0 && base + up >= t0; up = parent_of(parents, up), --at)
-          if (base + up <= t1 && (p.window == 0 || at > place - p.window || at < p.sink)) bits |= 1u << (base + up - t0);
-      }
-      if (!all_live) {
-        constexpr int kHere = kOwn < 32 ? kOwn : 32;  // of the tile's slots, one wave's pieces; kSlices lanes each
-#pragma unroll 1
-        for (int y = 0; y < 32; ++y) {
-          const uint64_t live = live_lds[buf][(32 * tile + y) / kOwn];
-          if (!(live >> ((32 * tile + y) % kOwn * kSlices) & 1)) bits &= ~(1u << y);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int s0 = t0 + 32 * x;
+        uint32_t bits = 0xFFFFFFFFu;  // of the tile's slots
+        const int before = p.parents ? base : base + own + 1;  // slots below it are seen, but for the window
+        bits = before >= s0 + 32 ? bits : before <= s0 ? 0u : (1u << (before - s0)) - 1;
+        if (p.window > 0) {
+          const int low = place - p.window + 1;  // slots from here on, or below the sinks' end
+          const uint32_t from = low <= s0 ? ~0u : low >= s0 + 32 ? 0u : ~0u << (low - s0);
+          const uint32_t sinks = p.sink >= s0 + 32 ? ~0u : p.sink <= s0 ? 0u : (1u << (p.sink - s0)) - 1;
+          bits &= from | sinks;
         }
-        static_assert(kHere * kSlices <= kWave, "a wave's pieces");
+        if (p.parents != nullptr && s0 + 31 >= base) {
+          const int32_t* parents = p.parents + token0;
+          int at = place;
+          for (int up = own; up >= 0 && base + up >= s0; up = parent_of(parents, up), --at)
+            if (base + up < s0 + 32 && (p.window == 0 || at > place - p.window || at < p.sink)) bits |= 1u << (base + up - s0);
+        }
+        if (!all_live) {
+#pragma unroll 1
+          for (int y = 0; y < 32; ++y) {
+            const uint64_t live = live_lds[buf][(32 * (tile + x) + y) / kOwn];  // of one wave's pieces; kSlices lanes a slot
+            if (!(live >> ((32 * (tile + x) + y) % kOwn * kSlices) & 1)) bits &= ~(1u << y);
+          }
+        }
+        bits >>= 4 * half;
+        seen[x] = (bits & 0xFu) | (bits >> 4 & 0xF0u) | (bits >> 8 & 0xF00u) | (bits >> 12 & 0xF000u);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[x][r] = seen[x] >> r & 1u ? s[x][r] : -INFINITY;
+        if (any_bad) {
+          for (int y = 0; y < 32; ++y) {  // slots of the tile with a value scale that is not finite
+            const uint64_t bads = bad_lds[buf][(32 * (tile + x) + y) / kOwn];
+            const uint32_t groups = static_cast<uint32_t>(bads >> ((32 * (tile + x) + y) % kOwn * kSlices)) & ((1u << kSlices) - 1);
+            if (scalar(groups) == 0) continue;
+            const int r = (y >> 3) * 4 + y % 4;
+            const int here = half == (y >> 2 & 1) && (seen[x] >> r & 1u);
+            if (here | __shfl_xor(here, 32, kWave)) poison |= groups;
+          }
+        }
       }
-      bits >>= 4 * half;
-      seen = (bits & 0xFu) | (bits >> 4 & 0xF0u) | (bits >> 8 & 0xF00u) | (bits >> 12 & 0xF000u);
     }
     float most = -INFINITY;
-    float t[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) t[r] = __builtin_fmaf(s[r], factor, -m);
-    if (!plain) {
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) t[r] = seen >> r & 1u ? t[r] : -INFINITY;
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) most = fmaxf(most, t[r]);
-    if (__any(most > kRoom) || behind != 1.0f) {
-      float now = -INFINITY;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) now = fmaxf(now, seen >> r & 1u ? s[r] * factor : -INFINITY);
+      for (int r = 0; r < 16; ++r) most = fmaxf(most, s[x][r]);
+    // a new reference where a weight would be too large, or where these are the first that the row sees
+    if (__any(most > kRoom || (l == 0.0f && most > -INFINITY)) || behind != 1.0f) {
       most = fmaxf(most, __shfl_xor(most, 32, kWave));
-      now = fmaxf(now, __shfl_xor(now, 32, kWave));
-      const float ref = most > kRoom ? now - kBias : m;
-      const float alpha = most > kRoom ? exp2f(m - ref) : 1.0f;
-      m = ref;
+      const bool none = l + __shfl_xor(l, 32, kWave) == 0.0f;
+      const bool moves = most > kRoom || (none && most > -INFINITY);
+      const float up = moves ? most - kBias : 0.0f;
+      const float alpha = none ? 0.0f : exp2f(-up);
+      m += up;
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < kSlices; ++i) acc[i] *= alpha * behind;
       behind = 1.0f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) t[r] = seen >> r & 1u ? __builtin_fmaf(s[r], factor, -ref) : -INFINITY;
-    }
-    float sum[2] = {0.0f, 0.0f};
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      t[r] = __builtin_amdgcn_exp2f(t[r]);
-      sum[r % 2] += t[r];
-    }
-    l += sum[0] + sum[1];
-    if (!plain) {
-      if (any_bad) {
-        for (int y = 0; y < 32; ++y) {  // slots of the tile with a value scale that is not finite
-          const uint64_t bads = bad_lds[buf][(32 * tile + y) / kOwn];
-          const uint32_t groups = static_cast<uint32_t>(bads >> ((32 * tile + y) % kOwn * kSlices)) & ((1u << kSlices) - 1);
-          if (scalar(groups) == 0) continue;
-          const int r = (y >> 3) * 4 + y % 4;
-          const int here = half == (y >> 2 & 1) && (seen >> r & 1u);
-          if (here | __shfl_xor(here, 32, kWave)) poison |= groups;
-        }
-      }
-      // values that were scaled by less than the largest so far
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int less = top - scalar(top_lds[buf][(32 * tile + 8 * j) / kOwn]);
-        const float by = __builtin_bit_cast(float, static_cast<uint32_t>(127 - less) << 23);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[4 * j + i] *= by;
-      }
+        for (int r = 0; r < 16; ++r) s[x][r] -= up;
     }
     u32x4 w[kParts][2];
+    auto powers = [&](float (&t)[16], int x) {
+      float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int step = 0; step < 2; ++step)
+      for (int r = 0; r < 16; ++r) {
+        t[r] = __builtin_amdgcn_exp2f(t[r]);
+        sum[r % 2] += t[r];
+      }
+      l += sum[0] + sum[1];
+      if (!plain) {  // values that were scaled by less than the largest so far
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        typedef float f32x2 __attribute__((ext_vector_type(2)));
-        const f32x2 v = {t[8 * step + 2 * k], t[8 * step + 2 * k + 1]};
-        const half2v h = __builtin_convertvector(v, half2v);
-        w[0][step][k] = __builtin_bit_cast(uint32_t, h);
-        if constexpr (PREC) {
-          const half2v rest = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), half2v);
-          w[kParts - 1][step][k] = __builtin_bit_cast(uint32_t, rest);
+        for (int j = 0; j < 4; ++j) {
+          const int less = top - scalar(top_lds[buf][(32 * (tile + x) + 8 * j) / kOwn]);
+          const float by = __builtin_bit_cast(float, static_cast<uint32_t>(127 - less) << 23);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[4 * j + i] *= by;
         }
       }
-    // ---- weights times values
+    };
+    auto operands = [&](const float (&t)[16]) {
 #pragma unroll
-    for (int n = 0; n < 2 * kSlices; ++n) {
-      const int i = n / 2, step = n % 2;
-      const u32x4 v = value[n % kAhead];
-      if (n + kAhead < 2 * kSlices) value[n % kAhead] = fetch(n + kAhead, 0);
-      acc[i] = mfma32(v, w[0][step], acc[i]);
-      if constexpr (PREC) {
-        acc[i] = mfma32(v, w[kParts - 1][step], acc[i]);
-        acc[i] = mfma32(fetch(n, kValueBytes), w[0][step], acc[i]);
+      for (int step = 0; step < 2; ++step)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          typedef float f32x2 __attribute__((ext_vector_type(2)));
+          const f32x2 v = {t[8 * step + 2 * k], t[8 * step + 2 * k + 1]};
+          const half2v h = __builtin_convertvector(v, half2v);
+          w[0][step][k] = __builtin_bit_cast(uint32_t, h);
+          if constexpr (PREC) {
+            const half2v rest = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), half2v);
+            w[kParts - 1][step][k] = __builtin_bit_cast(uint32_t, rest);
+          }
+        }
+    };
+    // ---- weights times values; the second tile's are read as the first one's are used
+    auto weigh = [&](int x) {
+#pragma unroll
+      for (int n = 0; n < kSteps; ++n) {
+        const int i = n / 2, step = n % 2, later = x * kSteps + n + kAhead;
+        const u32x4 v = value[n % kAhead];
+        acc[i] = mfma32(v, w[0][step], acc[i]);
+        if (later < 2 * kSteps) value[n % kAhead] = fetch(later / kSteps, later % kSteps, 0);
+        if constexpr (PREC) {
+          acc[i] = mfma32(v, w[kParts - 1][step], acc[i]);
+          acc[i] = mfma32(fetch(x, n, kValueBytes), w[0][step], acc[i]);
+        }
       }
-    }
+    };
+    powers(s[0], 0);
+    powers(s[1], 1);
+    operands(s[0]);
+    weigh(0);
+    operands(s[1]);
+    weigh(1);
   };
 
   // the stage after `n` into LDS, and the one after that on its way
   auto advance = [&](int n) {
-    if (n + 1 < n_end) unpack_stage(next, kBuffers > 1 ? (n + 1 - n_begin) & 1 : 0);
-    next = load(n + 2, page_next);
-    page_next = page_of(n + 3);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      if (n + 1 < n_end) unpack_piece_into(next[i], kBuffers > 1 ? (n + 1 - n_begin) & 1 : 0, i);
+      next[i] = load(n + 2, i, page_next[i]);
+      page_next[i] = page_of(n + 3, i);
+    }
   };
   advance(n_begin - 1);
   __syncthreads();
@@ -677,7 +712,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     int tops = 0, least = 31;
     bool all_live = true, any_bad = false;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
+    for (int w = 0; w < kGroups; ++w) {
       const int e = scalar(top_lds[buf][w]);
       tops = max(tops, e);
       least = min(least, e);
@@ -693,9 +728,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     // (every other set of four waves unpacks first, so that a SIMD's two waves are not at the same thing)
     if (kBuffers > 1 && W > 4 && wave / 4 % 2) advance(n);
     if (active) {
-      for (int tile = part; tile < kTiles; tile += p.parts) {
-        const int t0 = slot0 + 32 * tile, t1 = t0 + 31;
-        // whether every row of the wave sees all of the tile's slots, or none
+      for (int tile = 2 * part; tile < kTiles; tile += 2 * p.parts) {
+        const int t0 = slot0 + 32 * tile, t1 = t0 + 63;
+        // whether every row of the wave sees all of the tiles' slots, or none
         const int reach_lo = p.parents ? base : own_lo;  // the lowest position; slots up to it are seen, but for the window
         bool all = all_live && !any_bad && least == top && (p.parents ? t1 < base : t1 <= own_lo);
         if (p.window > 0) {
@@ -703,7 +738,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
           if (t1 <= reach_lo - p.window && t0 >= p.sink) continue;
         }
         if (t0 > own_hi) continue;
-        work_tile(buf, tile, t0, all, all_live, any_bad);
+        work_pair(buf, tile, t0, all, all_live, any_bad);
       }
     }
     if (kBuffers == 1) __syncthreads();
@@ -717,7 +752,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   for (int i = 0; i < kSlices; ++i) acc[i] *= poison >> i & 1u ? __builtin_nanf("") : behind;
   if (p.parts > 1) {
     constexpr int kRow = kSlices * 16 + 2;
-    static_assert(kTiles == 1 || W / 2 * kRow * kWave * 4 <= kBuffers * kBytes, "a part's accumulators");
+    static_assert(kTiles == 2 || W / 2 * kRow * kWave * 4 <= kBuffers * kBytes, "a part's accumulators");
     float* mine = reinterpret_cast<float*>(lds[0]) + (wave % p.row_tiles) * kRow * kWave + lane;  // [row tile][kRow][lane]
     for (int other = 1; other < p.parts; ++other) {
       __syncthreads();
