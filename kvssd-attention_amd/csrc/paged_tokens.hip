@@ -15,45 +15,80 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// A workgroup takes kThreads / (d / 4) rows at a time, of `rows` of a block: their runs' sums by a lane a run first, whose
+// weights go to LDS, then 4 dims a thread.
 template <int STAGE>
-__global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedTokensParams p) {
-  const int kvh = blockIdx.x % p.c.kv_heads;
+__global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedTokensParams p, int rows, int chunks) {
+  constexpr int kRuns = 1024, kSide = 32;  // weights at a time, of all rows at once; lanes of a row's sums
+  __shared__ float weights[kRuns];
+  __shared__ float most_s[kThreads / 8], sum_s[kThreads / 8];
+  const int chunk = blockIdx.x % chunks, kvh = blockIdx.x / chunks % p.c.kv_heads;
   int first;
-  const TokenItem work = find_item<STAGE>(p, blockIdx.x / p.c.kv_heads, true, &first);
+  const TokenItem work = find_item<STAGE>(p, blockIdx.x / chunks / p.c.kv_heads, true, &first);
   if (work.seq < 0 || work.runs == 1) return;
-  const int d = p.c.head_dim, lanes = d / 4;
-  const int rows = min(work.span.count * p.gq - work.block * p.block_rows, p.block_rows);
-  const int dim = threadIdx.x % lanes * 4;
+  const int d = p.c.head_dim, lanes = d / 4, side = kThreads / lanes;  // rows side by side: 4 to 32
+  const int end = min(min(work.span.count * p.gq - work.block * p.block_rows, p.block_rows), (chunk + 1) * rows);
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const int64_t step = static_cast<int64_t>(p.c.kv_heads) * p.block_rows;  // rows between runs
-  for (int row = threadIdx.x / lanes; row < rows; row += kThreads / lanes) {
-    if (static_cast<int>(threadIdx.x) >= kThreads / lanes * lanes) break;
-    const int64_t at = (static_cast<int64_t>(first) * p.c.kv_heads + kvh) * p.block_rows + row;
-    const f32x2* ml = reinterpret_cast<const f32x2*>(p.part_ml) + at;
-    const float* o = p.part_o + at * d + dim;
-    float most = -INFINITY;
-#pragma unroll 4
-    for (int r = 0; r < work.runs; ++r) {
-      const f32x2 x = ml[r * step];
-      if (x[1] != 0.0f) most = fmaxf(most, x[0]);
-    }
-    float sum = 0.0f;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int r = 0; r < work.runs; ++r) {
-      const f32x2 x = ml[r * step];
-      const f32x4 v = *reinterpret_cast<const f32x4*>(o + r * step * d);
-      if (x[1] != 0.0f) {  // (a NaN sum takes part)
-        const float w = exp2f(x[0] - most);
-        sum += w * x[1];
-        acc += w * v;
+  const int64_t at0 = (static_cast<int64_t>(first) * p.c.kv_heads + kvh) * p.block_rows;
+  const f32x2* ml = reinterpret_cast<const f32x2*>(p.part_ml);
+  const int tid = threadIdx.x, own = tid / lanes, dim = tid % lanes * 4;
+  for (int row0 = chunk * rows; row0 < end; row0 += side) {
+    // largest reference of each row, then its sum: 32 lanes a row, 8 rows at a time
+    for (int r0 = tid / kSide; r0 < side; r0 += kThreads / kSide) {
+      const bool has = row0 + r0 < end;
+      float most = -INFINITY, sum = 0.0f;
+      for (int n = tid % kSide; n < work.runs; n += kSide) {
+        const f32x2 x = has ? ml[at0 + row0 + r0 + n * step] : f32x2{0.0f, 0.0f};
+        if (x[1] != 0.0f) most = fmaxf(most, x[0]);  // (a NaN sum takes part)
+      }
+#pragma unroll
+      for (int k = 1; k < kSide; k *= 2) most = fmaxf(most, __shfl_xor(most, k, kWave));
+      for (int n = tid % kSide; n < work.runs; n += kSide) {
+        const f32x2 x = has ? ml[at0 + row0 + r0 + n * step] : f32x2{0.0f, 0.0f};
+        if (x[1] != 0.0f) sum += exp2f(x[0] - most) * x[1];
+      }
+#pragma unroll
+      for (int k = 1; k < kSide; k *= 2) sum += __shfl_xor(sum, k, kWave);
+      if (tid % kSide == 0) {
+        most_s[r0] = most;
+        sum_s[r0] = sum;
       }
     }
-    const int in_seq = work.block * p.block_rows + row, token = in_seq / p.gq;
-    const int64_t to = (work.span.begin + token) * p.query_heads + kvh * p.gq + in_seq - token * p.gq;
+    const int together = kRuns / side;  // runs
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int n0 = 0; n0 < work.runs; n0 += together) {
+      const int here = min(together, work.runs - n0);
+      __syncthreads();
+      for (int i = tid; i < side * here; i += kThreads) {
+        const int r = i / here, n = i - r * here;
+        float w = 0.0f;
+        if (row0 + r < end) {
+          const f32x2 x = ml[at0 + row0 + r + (n0 + n) * step];
+          if (x[1] != 0.0f) w = exp2f(x[0] - most_s[r]);
+        }
+        weights[r * together + n] = w;
+      }
+      __syncthreads();
+      if (own < side && row0 + own < end) {
+        const float* o = p.part_o + (at0 + row0 + own + n0 * step) * d + dim;
+#pragma unroll 8
+        for (int n = 0; n < here; ++n) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(o + n * step * d);
+          const float w = weights[own * together + n];
+          if (w != 0.0f) acc += w * v;  // (NaN weights take part)
+        }
+      }
+    }
+    if (own < side && row0 + own < end) {
+      const float sum = sum_s[own];
+      const int in_seq = work.block * p.block_rows + row0 + own, token = in_seq / p.gq;
+      const int64_t to = (work.span.begin + token) * p.query_heads + kvh * p.gq + in_seq - token * p.gq;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_out(p.out, p.out_dtype, to * d + dim + i, sum == 0.0f ? 0.0f : acc[i] / sum);
-    if (dim == 0) p.lse[to] = sum == 0.0f ? -INFINITY : kLn2 * (most + log2f(sum));
+      for (int i = 0; i < 4; ++i) store_out(p.out, p.out_dtype, to * d + dim + i, sum == 0.0f ? 0.0f : acc[i] / sum);
+      if (dim == 0) p.lse[to] = sum == 0.0f ? -INFINITY : kLn2 * (most_s[own] + log2f(sum));
+    }
+    __syncthreads();
   }
 }
 
@@ -130,7 +165,7 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
       p.items = static_cast<int>(plan->blocks + work / size + 1);
     }
   }
-  if (static_cast<int64_t>(p.items) * c.kv_heads > (int64_t{1} << 23)) return arg_error("too many sequences or tokens for one call");
+  if (static_cast<int64_t>(p.items) * c.kv_heads > (int64_t{1} << 22)) return arg_error("too many sequences or tokens for one call");
   const bool split = p.least_stages < (1 << 30);
   const size_t rows = split ? static_cast<size_t>(p.items) * c.kv_heads * p.block_rows : 0;
   plan->o_bytes = aligned(rows * c.head_dim * sizeof(float));
@@ -158,10 +193,13 @@ int launch_paged_tokens(const kvssd_paged_cache& c, const kvssd_paged_tokens_arg
                                        : launch_paged_tokens_dims<256>;
   if (int rc = launch(p, plan.waves, plan.precise, groups, stream)) return rc;
   if (need == 0) return 0;
-  const dim3 grid(static_cast<unsigned>(plan.blocks * c.kv_heads));
-  if (plan.stage == 256) hipLaunchKernelGGL(paged_tokens_merge_kernel<256>, grid, dim3(kThreads), 0, stream, p);
-  else if (plan.stage == 128) hipLaunchKernelGGL(paged_tokens_merge_kernel<128>, grid, dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL(paged_tokens_merge_kernel<64>, grid, dim3(kThreads), 0, stream, p);
+  // few blocks are spread over more workgroups
+  const int rows = plan.blocks * c.kv_heads * p.block_rows > 16384 ? 32 : kThreads / (c.head_dim / 4);
+  const int chunks = (p.block_rows + rows - 1) / rows;
+  const dim3 grid(static_cast<unsigned>(plan.blocks * c.kv_heads * chunks));
+  if (plan.stage == 256) hipLaunchKernelGGL(paged_tokens_merge_kernel<256>, grid, dim3(kThreads), 0, stream, p, rows, chunks);
+  else if (plan.stage == 128) hipLaunchKernelGGL(paged_tokens_merge_kernel<128>, grid, dim3(kThreads), 0, stream, p, rows, chunks);
+  else hipLaunchKernelGGL(paged_tokens_merge_kernel<64>, grid, dim3(kThreads), 0, stream, p, rows, chunks);
   return hip_status(hipGetLastError(), "paged_tokens_merge launch");
 }
 

@@ -223,24 +223,15 @@ int launch_paged_tokens_dims<256>(const PagedTokensParams& p, int waves, bool pr
 
 // ------------------------------------------------------------------ kernel ---
 
-// 32 codes as fp16 pairs (c - mid) / F in the dims' order
-template <int BITS>
-__device__ __forceinline__ void unpack_piece(const uint32_t* x, const Masks& k, uint32_t m01, uint32_t m23, u32x4 (&out)[4]) {
-  if constexpr (BITS == 4) {
+// 32 INT2 codes as fp16 pairs (c - 2) / 4 in the dims' order
+__device__ __forceinline__ void unpack_int2(const uint32_t* x, const Masks& k, uint32_t m01, uint32_t m23, u32x4 (&out)[4]) {
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const u32x4 v = code_operand<4>(x[w], 0, k, m01, m23);  // dims (0, 4) (1, 5) (2, 6) (3, 7)
-      out[w] = u32x4{low_halves(v[0], v[1]), low_halves(v[2], v[3]), high_halves(v[0], v[1]), high_halves(v[2], v[3])};
-    }
-  } else {
+  for (int w = 0; w < 2; ++w) {
+    const u32x4 a = code_operand<2>(x[w], 0, k, m01, m23), b = code_operand<2>(x[w], 1, k, m01, m23);
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const u32x4 a = code_operand<2>(x[w], 0, k, m01, m23), b = code_operand<2>(x[w], 1, k, m01, m23);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // dims (2 i, 2 i + 8) and (2 i + 1, 2 i + 9)
-        out[2 * w][i] = low_halves(a[i], b[i]);
-        out[2 * w + 1][i] = high_halves(a[i], b[i]);
-      }
+    for (int i = 0; i < 4; ++i) {  // dims (2 i, 2 i + 8) and (2 i + 1, 2 i + 9)
+      out[2 * w][i] = low_halves(a[i], b[i]);
+      out[2 * w + 1][i] = high_halves(a[i], b[i]);
     }
   }
 }
@@ -293,8 +284,10 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   // keys: [chunk of 8 dims][slot] 16 bytes each, slots turned by their chunk; values: [part][slot][dim]
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers][kBytes];
   __shared__ float scale_lds[kBuffers][kSlices][kTiles][2][16];  // keys': of slots 8 (i / 4) + 4 half + i % 4 of a tile
-  __shared__ uint64_t live_lds[kBuffers][kGroups], bad_lds[kBuffers][kGroups];
-  __shared__ int top_lds[kBuffers][kGroups];
+  __shared__ uint64_t live_lds[kBuffers][kGroups], bad_lds[kBuffers][kGroups];  // a bit a lane of a group's pieces
+  // of a group: exponent that its values are scaled by; whether slots take no part, or value scales are not finite
+  constexpr uint32_t kGaps = 256, kBad = 512;
+  __shared__ __attribute__((aligned(16))) uint32_t flags_lds[kBuffers][kGroups];
 
   const kvssd_paged_cache& c = p.c;
   const int tid = threadIdx.x, lane = tid % kWave, wave = scalar(tid / kWave);
@@ -336,37 +329,47 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     uint16_t sk, sv;
     bool live;
   } next[kPieces];
-  int page_next[kPieces];
-  auto page_of = [&](int n, int piece) {  // of the piece's slot in the list's stage n; -1: none
+  int page_next[kPieces], row_next[kPieces];  // of the stage after it: the page, and the row in it
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) next[i] = Piece{};
+  auto find = [&](int n, int piece) {  // of the piece's slot in the list's stage n; page -1: none
     const int slot = list.stage(n) * kStage + first_slot + piece * kNext;
-    return n < n_end && slot < length ? pages[p.of_page.quotient(slot)] : -1;
-  };
-  auto load = [&](int n, int piece, int page) {
-    Piece x{};
-    if (n < n_end && page >= 0 && page < c.num_pages) {
-      const int slot = list.stage(n) * kStage + first_slot + piece * kNext;
-      const uint32_t row = page * c.page_tokens + slot - p.of_page.quotient(slot) * c.page_tokens;
-      x.live = true;
-      if (has_dims) {
-        const uint64_t byte = static_cast<uint64_t>(row) * slot_bytes + piece_at;
-        const uint64_t scale = static_cast<uint64_t>(row) * slot_scales + scale_at;
-        if (c.bits == 4) {
-          __builtin_memcpy(x.k, __builtin_assume_aligned(c.packed_k + byte, 16), 16);
-          __builtin_memcpy(x.v, __builtin_assume_aligned(c.packed_v + byte, 16), 16);
-        } else {
-          __builtin_memcpy(x.k, __builtin_assume_aligned(c.packed_k + byte, 8), 8);
-          __builtin_memcpy(x.v, __builtin_assume_aligned(c.packed_v + byte, 8), 8);
-        }
-        x.sk = c.scales_k[scale];
-        x.sv = c.scales_v[scale];
-      }
+    page_next[piece] = -1;
+    if (n < n_end && slot < length) {
+      const int nth = p.of_page.quotient(slot);
+      row_next[piece] = slot - nth * c.page_tokens;
+      page_next[piece] = pages[nth];
     }
-    return x;
+  };
+  auto load = [&](int piece) {
+    Piece& x = next[piece];
+    const int page = page_next[piece];
+    x.live = page >= 0 && page < c.num_pages;
+    x.sk = x.sv = 0;
+    if (x.live && has_dims) {  // (other codes stay: any are finite, and their scales are 0)
+      const uint32_t row = page * c.page_tokens + row_next[piece];
+      const uint64_t byte = static_cast<uint64_t>(row) * slot_bytes + piece_at;
+      const uint64_t scale = static_cast<uint64_t>(row) * slot_scales + scale_at;
+      if (c.bits == 4) {
+        __builtin_memcpy(x.k, __builtin_assume_aligned(c.packed_k + byte, 16), 16);
+        __builtin_memcpy(x.v, __builtin_assume_aligned(c.packed_v + byte, 16), 16);
+      } else {
+        __builtin_memcpy(x.k, __builtin_assume_aligned(c.packed_k + byte, 8), 8);
+        __builtin_memcpy(x.v, __builtin_assume_aligned(c.packed_v + byte, 8), 8);
+      }
+      x.sk = c.scales_k[scale];
+      x.sv = c.scales_v[scale];
+    }
   };
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    next[i] = load(n_begin, i, page_of(n_begin, i));
-    page_next[i] = page_of(n_begin + 1, i);
+    row_next[i] = 0;
+    find(n_begin, i);
+  }
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    load(i);
+    find(n_begin + 1, i);
   }
 
   // ---- the wave's rows
@@ -456,12 +459,16 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     const Masks masks = make_masks(zero);
     const uint32_t m01 = 0x00030003u | zero, m23 = 0x000C000Cu | zero;
     u32x4 codes[4];
-    if (c.bits == 4) {
+    // dims of a chunk: INT4 (0, 4) (1, 5) (2, 6) (3, 7), INT2 in their order
+    auto unpack = [&](const uint32_t* from, u32x4 (&to)[4]) {
+      if (c.bits == 4) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) codes[w] = code_operand<4>(x.k[w], 0, masks, m01, m23);
-    } else {
-      unpack_piece<2>(x.k, masks, m01, m23, codes);
-    }
+        for (int w = 0; w < 4; ++w) to[w] = code_operand<4>(from[w], 0, masks, m01, m23);
+      } else {
+        unpack_int2(from, masks, m01, m23, to);
+      }
+    };
+    unpack(x.k, codes);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const int chunk = 4 * slice + w;
@@ -471,15 +478,15 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     scale_lds[buf][slice][piece_slot / 32][in_tile >> 2 & 1][(in_tile >> 3) * 4 + in_tile % 4] = half_bits_to_float(x.sk);
     const int ex = x.sv >> 10 & 31;
     const bool bad = ex == 31;
-    const int most = max(top, static_cast<int>(wave_most(bad ? 0u : static_cast<uint32_t>(ex))));
     const uint64_t live = __ballot(x.live), bads = __ballot(bad);
+    int most = top;
+    if (__any(!bad && ex > top)) most = static_cast<int>(wave_most(bad ? 0u : static_cast<uint32_t>(ex)));
     if (lane == 0) {
       live_lds[buf][piece * W + wave] = live;
       bad_lds[buf][piece * W + wave] = bads;
-      top_lds[buf][piece * W + wave] = most;
+      flags_lds[buf][piece * W + wave] = most | (live == ~0ull ? 0u : kGaps) | (bads != 0 ? kBad : 0u);
     }
-    if (c.bits == 4) unpack_piece<4>(x.v, masks, m01, m23, codes);
-    else unpack_piece<2>(x.v, masks, m01, m23, codes);
+    unpack(x.v, codes);
     const _Float16 up = __builtin_bit_cast(_Float16, static_cast<uint16_t>((44 - most) << 10));  // 2^(29 - most)
     const _Float16 s = __builtin_bit_cast(_Float16, static_cast<uint16_t>(bad ? 0 : x.sv)) * up;
     const half2v ss = {s, s};
@@ -651,7 +658,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       if (!plain) {  // values that were scaled by less than the largest so far
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int less = top - scalar(top_lds[buf][(32 * (tile + x) + 8 * j) / kOwn]);
+          const int less = top - scalar(flags_lds[buf][(32 * (tile + x) + 8 * j) / kOwn] & 31u);
           const float by = __builtin_bit_cast(float, static_cast<uint32_t>(127 - less) << 23);
 #pragma unroll
           for (int i = 0; i < 4; ++i) t[4 * j + i] *= by;
@@ -700,8 +707,8 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       if (n + 1 < n_end) unpack_piece_into(next[i], kBuffers > 1 ? (n + 1 - n_begin) & 1 : 0, i);
-      next[i] = load(n + 2, i, page_next[i]);
-      page_next[i] = page_of(n + 3, i);
+      load(i);
+      find(n + 3, i);
     }
   };
   advance(n_begin - 1);
@@ -709,18 +716,20 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   for (int n = n_begin; n < n_end; ++n) {
     const int buf = kBuffers > 1 ? (n - n_begin) & 1 : 0;
     const int slot0 = list.stage(n) * kStage;
-    int tops = 0, least = 31;
-    bool all_live = true, any_bad = false;
+    uint32_t flags = 0, highest = 0, lowest = 31;
+    {
+      uint32_t of[kGroups];
+      __builtin_memcpy(of, __builtin_assume_aligned(flags_lds[buf], 16), sizeof(of));
 #pragma unroll
-    for (int w = 0; w < kGroups; ++w) {
-      const int e = scalar(top_lds[buf][w]);
-      tops = max(tops, e);
-      least = min(least, e);
-      all_live = all_live && live_lds[buf][w] == ~0ull;
-      any_bad = any_bad || bad_lds[buf][w] != 0;
+      for (int w = 0; w < kGroups; ++w) {
+        flags |= of[w];
+        highest = max(highest, of[w] & 31u);
+        lowest = min(lowest, of[w] & 31u);
+      }
     }
-    all_live = scalar(all_live);
-    any_bad = scalar(any_bad);
+    const int tops = scalar(highest), least = scalar(lowest);
+    flags = scalar(flags);
+    const bool all_live = !(flags & kGaps), any_bad = flags & kBad;
     if (tops != top) {
       behind *= __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - tops) << 23);
       top = tops;
@@ -779,7 +788,20 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       }
     }
   }
-  if (part != 0 || wave_row0 + col >= rows) return;
+  if (part != 0) return;
+  if (c.bits == 4) {  // a chunk's dims lie 0, 4, 1, 5 in the lower half's lanes, 2, 6, 3, 7 in the upper one's
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const float v[4] = {acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]};
+        const auto even = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v[0]), __builtin_bit_cast(uint32_t, v[1]), false, false);
+        const auto odd = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v[2]), __builtin_bit_cast(uint32_t, v[3]), false, false);
+        const uint32_t lanes[4] = {even[0], odd[0], even[1], odd[1]};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[i][j + y] = __builtin_bit_cast(float, lanes[y]);
+      }
+  }
 
   // ---- the result, or the run's partial
   const bool whole = runs == 1, none = l == 0.0f;
@@ -788,6 +810,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   const int64_t at = (token0 + own) * p.query_heads + head;
   const int64_t part_at = (static_cast<int64_t>(item) * c.kv_heads + kvh) * p.block_rows + row - block * p.block_rows;
   const float by = !whole ? unit : none ? 0.0f : unit / l;
+  if (wave_row0 + col >= rows) return;
 #pragma unroll
   for (int i = 0; i < kSlices; ++i)
 #pragma unroll
