@@ -14,6 +14,7 @@ namespace kvssd {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kLeastStages = 2;  // of a run
 
 // A workgroup takes kThreads / (d / 4) rows at a time, of `rows` of a block: their runs' sums by a lane a run first, whose
 // weights go to LDS, then 4 dims a thread.
@@ -34,23 +35,31 @@ __global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedToken
   const f32x2* ml = reinterpret_cast<const f32x2*>(p.part_ml);
   const int tid = threadIdx.x, own = tid / lanes, dim = tid % lanes * 4;
   for (int row0 = chunk * rows; row0 < end; row0 += side) {
-    // largest reference of each row, then its sum: 32 lanes a row, 8 rows at a time
+    // largest reference of each row, then its sum: 32 lanes a row, 8 rows at a time, the first 64 runs kept in registers
     for (int r0 = tid / kSide; r0 < side; r0 += kThreads / kSide) {
-      const bool has = row0 + r0 < end;
-      float most = -INFINITY, sum = 0.0f;
-      for (int n = tid % kSide; n < work.runs; n += kSide) {
-        const f32x2 x = has ? ml[at0 + row0 + r0 + n * step] : f32x2{0.0f, 0.0f};
-        if (x[1] != 0.0f) most = fmaxf(most, x[0]);  // (a NaN sum takes part)
+      const f32x2* of = ml + at0 + row0 + r0;
+      const int runs = row0 + r0 < end ? work.runs : 0, n = tid % kSide;
+      f32x2 x[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) x[i] = n + i * kSide < runs ? of[(n + i * kSide) * step] : f32x2{-INFINITY, 0.0f};
+      float most = fmaxf(x[0][1] != 0.0f ? x[0][0] : -INFINITY, x[1][1] != 0.0f ? x[1][0] : -INFINITY);  // (a NaN sum takes part)
+      for (int i = n + 2 * kSide; i < runs; i += kSide) {
+        const f32x2 y = of[i * step];
+        if (y[1] != 0.0f) most = fmaxf(most, y[0]);
       }
 #pragma unroll
       for (int k = 1; k < kSide; k *= 2) most = fmaxf(most, __shfl_xor(most, k, kWave));
-      for (int n = tid % kSide; n < work.runs; n += kSide) {
-        const f32x2 x = has ? ml[at0 + row0 + r0 + n * step] : f32x2{0.0f, 0.0f};
-        if (x[1] != 0.0f) sum += exp2f(x[0] - most) * x[1];
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (x[i][1] != 0.0f) sum += exp2f(x[i][0] - most) * x[i][1];
+      for (int i = n + 2 * kSide; i < runs; i += kSide) {
+        const f32x2 y = of[i * step];
+        if (y[1] != 0.0f) sum += exp2f(y[0] - most) * y[1];
       }
 #pragma unroll
       for (int k = 1; k < kSide; k *= 2) sum += __shfl_xor(sum, k, kWave);
-      if (tid % kSide == 0) {
+      if (n == 0) {
         most_s[r0] = most;
         sum_s[r0] = sum;
       }
@@ -153,17 +162,19 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
     total = total < longest * c.sequences ? total : longest * c.sequences;
   }
   const int64_t likely = (each + p.block_rows - 1) / p.block_rows * c.sequences;  // blocks
-  const int64_t wanted = 512 / c.kv_heads;                                        // items
+  const int64_t work = (total / stage + c.sequences) * (likely / c.sequences);    // stages of all blocks
+  // workgroups that run at a time (LDS and registers); two rounds of them where blocks are few, four of more, whose
+  // lengths differ
+  const int64_t at_once = plan->waves == 4 && !plan->precise && plan->dp <= 128 ? 512 : 256;
+  const int64_t wanted = (likely * c.kv_heads < at_once ? 2 : 4) * at_once / c.kv_heads;
+  const int64_t cut = wanted - likely > wanted / 2 ? wanted - likely : (wanted + 1) / 2;
+  int64_t size = (work + cut - 1) / (cut > 0 ? cut : 1);
+  if (size < kLeastStages) size = kLeastStages;
   p.items = static_cast<int>(plan->blocks);
   p.least_stages = 1 << 30;
-  if (likely < wanted) {
-    const int64_t work = (total / stage + c.sequences) * (likely / c.sequences);
-    int64_t size = (work + wanted - likely - 1) / (wanted - likely);
-    if (size < 2) size = 2;
-    if (size < stages(longest)) {
-      p.least_stages = static_cast<int>(size);
-      p.items = static_cast<int>(plan->blocks + work / size + 1);
-    }
+  if (size < stages(longest)) {
+    p.least_stages = static_cast<int>(size);
+    p.items = static_cast<int>(plan->blocks + work / size + 1);
   }
   if (static_cast<int64_t>(p.items) * c.kv_heads > (int64_t{1} << 22)) return arg_error("too many sequences or tokens for one call");
   const bool split = p.least_stages < (1 << 30);

@@ -276,18 +276,26 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   constexpr int kOwn = kWave / kSlices;           // slots of a wave's pieces at a time
   constexpr int kGroups = kStage / kOwn;          // of so many slots
   constexpr int kPieces = kGroups / W;            // of a thread
-  constexpr int kValueRow = DP * 2 + 32;          // bytes; transposed reads of four rows meet in no bank
+  constexpr int kValueRow = DP * 2 + (DP == 64 ? 32 : 64);  // bytes; so (but for short heads) do transposed reads meet in no bank
   constexpr int kKeyBytes = DP * kStage * 2, kValueBytes = kValueRow * kStage;
   constexpr int kBytes = kKeyBytes + kParts * kValueBytes;
   constexpr float kBias = 8.0f, kRoom = 14.0f;    // log2 of a weight at the reference's maximum, and at most
   constexpr int kPlain = 14;                      // exponent of the scales that the largest factor (2^15) serves
-  // keys: [chunk of 8 dims][slot] 16 bytes each, slots turned by their chunk; values: [part][slot][dim]
+  // keys: [chunk of 8 dims][slot] 16 bytes each, slots turned by their slice; values: [part][slot][dim], the chunks of
+  // 8 dims of a slice turned by their slot's number: so do writes of 16 lanes meet in no bank either
+  constexpr int kTurn = 16 / kSlices;
+  auto value_turn = [](int slot, int slice) {
+    return DP == 128 ? slot & 3 : DP == 64 ? (slot & 1) + 2 * (slot >> 2 & 1) : (slot & 1) + 2 * (slice >> 2 & 1);
+  };
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers][kBytes];
   __shared__ float scale_lds[kBuffers][kSlices][kTiles][2][16];  // keys': of slots 8 (i / 4) + 4 half + i % 4 of a tile
   __shared__ uint64_t live_lds[kBuffers][kGroups], bad_lds[kBuffers][kGroups];  // a bit a lane of a group's pieces
   // of a group: exponent that its values are scaled by; whether slots take no part, or value scales are not finite
   constexpr uint32_t kGaps = 256, kBad = 512;
   __shared__ __attribute__((aligned(16))) uint32_t flags_lds[kBuffers][kGroups];
+
+  constexpr int kTree = 1024;  // tokens of a tree whose parents are kept in LDS
+  __shared__ int16_t parent_lds[kTree];
 
   const kvssd_paged_cache& c = p.c;
   const int tid = threadIdx.x, lane = tid % kWave, wave = scalar(tid / kWave);
@@ -312,6 +320,13 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     const int run = scalar(work.run);
     n_begin = static_cast<int>(static_cast<int64_t>(n) * run / runs);
     n_end = static_cast<int>(static_cast<int64_t>(n) * (run + 1) / runs);
+  }
+
+  // a tree's token above `i`, -1 if none
+  const bool tree = p.parents != nullptr && seq < c.sequences;
+  auto above = [&](int i) -> int { return i < kTree ? parent_lds[i] : parent_of(p.parents + token0, i); };
+  if (tree) {
+    for (int i = tid; i < min(count, kTree); i += W * kWave) parent_lds[i] = static_cast<int16_t>(parent_of(p.parents + token0, i));
   }
 
   // ---- a thread's pieces: 32 dims of a slot
@@ -379,10 +394,10 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   const int row = min(wave_row0 + col, rows - 1);
   const int own = row / p.gq;  // the lane's token among the sequence's, and its position
   int place = base + own;
-  if (p.parents != nullptr && seq < c.sequences) {
+  if (tree) {
+    __syncthreads();
     place = base;
-    const int32_t* parents = p.parents + token0;
-    for (int up = parent_of(parents, own); up >= 0; up = parent_of(parents, up)) ++place;
+    for (int up = above(own); up >= 0; up = above(up)) ++place;
   }
   const int head = kvh * p.gq + row - own * p.gq;
   u32x4 q[kParts][DP / 16];
@@ -449,7 +464,6 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   const int own_lo = base + scalar(min(wave_row0, rows - 1) / p.gq);
   const int own_hi = base + scalar((min(wave_row0 + 32, rows) - 1) / p.gq);
 
-  constexpr int kTurn = DP / 64;  // a slot's place among its chunk's: slot ^ (chunk / kTurn), for writes of 8 lanes
   int top = kPlain;               // exponent that the accumulators' values are scaled by
 
   auto unpack_piece_into = [&](const Piece& x, int buf, int piece) {
@@ -472,7 +486,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const int chunk = 4 * slice + w;
-      *reinterpret_cast<u32x4*>(&lds[buf][(chunk * kStage + (piece_slot ^ (chunk / kTurn))) * 16]) = codes[w];
+      *reinterpret_cast<u32x4*>(&lds[buf][(chunk * kStage + (piece_slot ^ slice * kTurn)) * 16]) = codes[w];
     }
     const int in_tile = piece_slot % 32;
     scale_lds[buf][slice][piece_slot / 32][in_tile >> 2 & 1][(in_tile >> 3) * 4 + in_tile % 4] = half_bits_to_float(x.sk);
@@ -501,7 +515,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
         hi[i] = __builtin_bit_cast(uint32_t, v);
         if constexpr (PREC) lo[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, ss, -v));
       }
-      uint8_t* dst = &lds[buf][kKeyBytes + piece_slot * kValueRow + slice * 64 + w * 16];
+      uint8_t* dst = &lds[buf][kKeyBytes + piece_slot * kValueRow + slice * 64 + (w ^ value_turn(piece_slot, slice)) * 16];
       *reinterpret_cast<u32x4*>(dst) = hi;
       if constexpr (PREC) *reinterpret_cast<u32x4*>(dst + kValueBytes) = lo;
     }
@@ -514,8 +528,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   float behind = 1.0f;  // what the accumulators are to be multiplied by, since the values' scale has changed
   uint32_t poison = 0;  // slices of a row that see a value scale that is not finite
 
-  // where the lane reads values: slots 16 step + 4 half + (lane / 4) % 4, dims 16 (lane / 16 % 2) + 4 (lane % 4)
-  const int value_at = kKeyBytes + (4 * half + (lane >> 2 & 3)) * kValueRow + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
+  // where the lane reads values: slots 16 step + 4 half + (lane / 4) % 4 (and 8 on), dims 16 (lane / 16 % 2) + 4 (lane % 4)
+  const int value_slot = 4 * half + (lane >> 2 & 3), value_chunk = (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
+  const int value_at = kKeyBytes + value_slot * kValueRow + (value_chunk ^ value_turn(value_slot, 0)) * 16 + (lane & 1) * 8;
 
   // Two tiles of 32 slots.  `plain`: every row sees all of them, their values' scale is the accumulators' and finite.
   auto work_pair = [&](int buf, int tile, int t0, bool plain, bool all_live, bool any_bad) {
@@ -529,12 +544,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     asm volatile("" : "+v"(at_col));  // (a register for every turn of it would be kept otherwise)
     auto read_keys = [&](int n) {
       sk[n % kRing] = scale_lds[buf][n / 2][tile + n % 2][half][lane & 15];  // a slot's a lane, alike in the half's two rows
+      const uint8_t* at = stage + ((4 * (n / 2) + half) * kStage + (at_col ^ n / 2 * kTurn) + 32 * (n % 2)) * 16;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int chunk = 4 * (n / 2) + 2 * j, turn = chunk / kTurn;  // (of this one and the next, one turn unless kTurn is 1)
-        const int slot = (at_col ^ (kTurn == 1 ? turn + half : turn)) + 32 * (n % 2);
-        __builtin_memcpy(&key[n % kRing][j], __builtin_assume_aligned(stage + ((chunk + half) * kStage + slot) * 16, 16), 16);
-      }
+      for (int j = 0; j < 2; ++j) __builtin_memcpy(&key[n % kRing][j], __builtin_assume_aligned(at + 2 * j * kStage * 16, 16), 16);
     };
     auto product = [&](int n, int j, f32x16 to) {
       to = mfma32(key[n % kRing][j], q[0][n / 2 * 2 + j], to);
@@ -569,7 +581,8 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     constexpr int kAhead = PREC ? 2 : DP <= 128 ? kSteps : kSlices;  // steps
     u32x4 value[kAhead];
     auto fetch = [&](int of, int n, int from) {  // of a tile, step n % 2 of slice n / 2
-      const uint8_t* at = stage + value_at + (32 * (tile + of) + 16 * (n % 2)) * kValueRow + 64 * (n / 2) + from;
+      const int start = value_turn(0, n / 2) ? value_at ^ value_turn(0, n / 2) * 16 : value_at;
+      const uint8_t* at = stage + start + (32 * (tile + of) + 16 * (n % 2)) * kValueRow + 64 * (n / 2) + from;
       const u32x2 lo = lds_read_tr16(at), hi = lds_read_tr16(at + 8 * kValueRow);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
@@ -587,7 +600,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       for (int x = 0; x < 2; ++x) {
         const int s0 = t0 + 32 * x;
         uint32_t bits = 0xFFFFFFFFu;  // of the tile's slots
-        const int before = p.parents ? base : base + own + 1;  // slots below it are seen, but for the window
+        const int before = tree ? base : base + own + 1;  // slots below it are seen, but for the window
         bits = before >= s0 + 32 ? bits : before <= s0 ? 0u : (1u << (before - s0)) - 1;
         if (p.window > 0) {
           const int low = place - p.window + 1;  // slots from here on, or below the sinks' end
@@ -595,10 +608,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
           const uint32_t sinks = p.sink >= s0 + 32 ? ~0u : p.sink <= s0 ? 0u : (1u << (p.sink - s0)) - 1;
           bits &= from | sinks;
         }
-        if (p.parents != nullptr && s0 + 31 >= base) {
-          const int32_t* parents = p.parents + token0;
+        if (tree && s0 + 31 >= base) {
           int at = place;
-          for (int up = own; up >= 0 && base + up >= s0; up = parent_of(parents, up), --at)
+          for (int up = own; up >= 0 && base + up >= s0; up = above(up), --at)
             if (base + up < s0 + 32 && (p.window == 0 || at > place - p.window || at < p.sink)) bits |= 1u << (base + up - s0);
         }
         if (!all_live) {
@@ -624,11 +636,10 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
         }
       }
     }
-    float most = -INFINITY;
+    float of[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) most = fmaxf(most, s[x][r]);
+    for (int r = 0; r < 32; ++r) of[r % 4] = fmaxf(of[r % 4], s[r / 16][r % 16]);
+    float most = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
     // a new reference where a weight would be too large, or where these are the first that the row sees
     if (__any(most > kRoom || (l == 0.0f && most > -INFINITY)) || behind != 1.0f) {
       most = fmaxf(most, __shfl_xor(most, 32, kWave));
@@ -647,14 +658,12 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
         for (int r = 0; r < 16; ++r) s[x][r] -= up;
     }
     u32x4 w[kParts][2];
-    auto powers = [&](float (&t)[16], int x) {
-      float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        t[r] = __builtin_amdgcn_exp2f(t[r]);
-        sum[r % 2] += t[r];
-      }
-      l += sum[0] + sum[1];
+    auto power = [&](int x, int r) {
+      s[x][r] = __builtin_amdgcn_exp2f(s[x][r]);
+      l += s[x][r];
+    };
+    auto operands = [&](int x) {
+      float (&t)[16] = s[x];
       if (!plain) {  // values that were scaled by less than the largest so far
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -664,8 +673,6 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
           for (int i = 0; i < 4; ++i) t[4 * j + i] *= by;
         }
       }
-    };
-    auto operands = [&](const float (&t)[16]) {
 #pragma unroll
       for (int step = 0; step < 2; ++step)
 #pragma unroll
@@ -680,26 +687,31 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
           }
         }
     };
-    // ---- weights times values; the second tile's are read as the first one's are used
-    auto weigh = [&](int x) {
-#pragma unroll
-      for (int n = 0; n < kSteps; ++n) {
-        const int i = n / 2, step = n % 2, later = x * kSteps + n + kAhead;
-        const u32x4 v = value[n % kAhead];
-        acc[i] = mfma32(v, w[0][step], acc[i]);
-        if (later < 2 * kSteps) value[n % kAhead] = fetch(later / kSteps, later % kSteps, 0);
-        if constexpr (PREC) {
-          acc[i] = mfma32(v, w[kParts - 1][step], acc[i]);
-          acc[i] = mfma32(fetch(x, n, kValueBytes), w[0][step], acc[i]);
-        }
+    // weights times values, step n of both tiles'; the later ones are read as these are used
+    auto weigh = [&](int n) {
+      const int i = n % kSteps / 2, step = n % 2, later = n + kAhead;
+      const u32x4 v = value[n % kAhead];
+      acc[i] = mfma32(v, w[0][step], acc[i]);
+      if (later < 2 * kSteps) value[n % kAhead] = fetch(later / kSteps, later % kSteps, 0);
+      if constexpr (PREC) {
+        acc[i] = mfma32(v, w[kParts - 1][step], acc[i]);
+        acc[i] = mfma32(fetch(n / kSteps, n % kSteps, kValueBytes), w[0][step], acc[i]);
       }
     };
-    powers(s[0], 0);
-    powers(s[1], 1);
-    operands(s[0]);
-    weigh(0);
-    operands(s[1]);
-    weigh(1);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) power(0, r);
+    operands(0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {  // beside the second tile's powers
+#pragma unroll
+      for (int n = r * kSteps / 16; n < (r + 1) * kSteps / 16; ++n) weigh(n);
+      power(1, r);
+      if (r % 2) __builtin_amdgcn_sched_barrier(0);
+    }
+    operands(1);
+#pragma unroll
+    for (int n = kSteps; n < 2 * kSteps; ++n) weigh(n);
   };
 
   // the stage after `n` into LDS, and the one after that on its way
@@ -734,14 +746,12 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       behind *= __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - tops) << 23);
       top = tops;
     }
-    // (every other set of four waves unpacks first, so that a SIMD's two waves are not at the same thing)
-    if (kBuffers > 1 && W > 4 && wave / 4 % 2) advance(n);
     if (active) {
       for (int tile = 2 * part; tile < kTiles; tile += 2 * p.parts) {
         const int t0 = slot0 + 32 * tile, t1 = t0 + 63;
         // whether every row of the wave sees all of the tiles' slots, or none
-        const int reach_lo = p.parents ? base : own_lo;  // the lowest position; slots up to it are seen, but for the window
-        bool all = all_live && !any_bad && least == top && (p.parents ? t1 < base : t1 <= own_lo);
+        const int reach_lo = tree ? base : own_lo;  // the lowest position; slots up to it are seen, but for the window
+        bool all = all_live && !any_bad && least == top && (tree ? t1 < base : t1 <= own_lo);
         if (p.window > 0) {
           all = all && (t0 > own_hi - p.window || t1 < p.sink);
           if (t1 <= reach_lo - p.window && t0 >= p.sink) continue;
@@ -751,7 +761,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       }
     }
     if (kBuffers == 1) __syncthreads();
-    if (!(kBuffers > 1 && W > 4 && wave / 4 % 2)) advance(n);
+    advance(n);
     __syncthreads();
   }
 
