@@ -14,90 +14,97 @@ namespace kvssd {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kLeastStages = 2;  // of a run
 
-// A workgroup takes kThreads / (d / 4) rows at a time, of `rows` of a block: their runs' sums by a lane a run first, whose
-// weights go to LDS, then 4 dims a thread.
+// `unit` threads (d / 4, up to a power of two) take every `splits`-th run of a row, 4 dims each, kAhead runs' sums read
+// before the first one's weight is known; a lane a run forms the weights.  With few rows, whose time is the latency of these
+// reads, a row's runs are split between the units of a workgroup (8 tokens of 4 heads at 4,096 tokens of context, 33 runs:
+// 6 us where one unit a row took 16).
 template <int STAGE>
-__global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedTokensParams p, int rows, int chunks) {
-  constexpr int kRuns = 1024, kSide = 32;  // weights at a time, of all rows at once; lanes of a row's sums
-  __shared__ float weights[kRuns];
+__global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedTokensParams p, int rows, int chunks, int unit_log2,
+                                                                      int splits_log2) {
+  constexpr int kAhead = 8;
+  __shared__ f32x4 acc_s[kThreads];
   __shared__ float most_s[kThreads / 8], sum_s[kThreads / 8];
   const int chunk = blockIdx.x % chunks, kvh = blockIdx.x / chunks % p.c.kv_heads;
   int first;
   const TokenItem work = find_item<STAGE>(p, blockIdx.x / chunks / p.c.kv_heads, true, &first);
   if (work.seq < 0 || work.runs == 1) return;
-  const int d = p.c.head_dim, lanes = d / 4, side = kThreads / lanes;  // rows side by side: 4 to 32
+  const int d = p.c.head_dim, tid = threadIdx.x;
+  const int unit = tid >> unit_log2, i = tid - (unit << unit_log2), dim = i * 4, size = 1 << unit_log2;
+  const int side_log2 = 8 - unit_log2 - splits_log2;  // rows side by side (of 256 threads)
+  const int own = unit & ((1 << side_log2) - 1), split = unit >> side_log2;
   const int end = min(min(work.span.count * p.gq - work.block * p.block_rows, p.block_rows), (chunk + 1) * rows);
   typedef float f32x2 __attribute__((ext_vector_type(2)));
-  const int64_t step = static_cast<int64_t>(p.c.kv_heads) * p.block_rows;  // rows between runs
-  const int64_t at0 = (static_cast<int64_t>(first) * p.c.kv_heads + kvh) * p.block_rows;
-  const f32x2* ml = reinterpret_cast<const f32x2*>(p.part_ml);
-  const int tid = threadIdx.x, own = tid / lanes, dim = tid % lanes * 4;
-  for (int row0 = chunk * rows; row0 < end; row0 += side) {
-    // largest reference of each row, then its sum: 32 lanes a row, 8 rows at a time, the first 64 runs kept in registers
-    for (int r0 = tid / kSide; r0 < side; r0 += kThreads / kSide) {
-      const f32x2* of = ml + at0 + row0 + r0;
-      const int runs = row0 + r0 < end ? work.runs : 0, n = tid % kSide;
-      f32x2 x[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) x[i] = n + i * kSide < runs ? of[(n + i * kSide) * step] : f32x2{-INFINITY, 0.0f};
-      float most = fmaxf(x[0][1] != 0.0f ? x[0][0] : -INFINITY, x[1][1] != 0.0f ? x[1][0] : -INFINITY);  // (a NaN sum takes part)
-      for (int i = n + 2 * kSide; i < runs; i += kSide) {
-        const f32x2 y = of[i * step];
-        if (y[1] != 0.0f) most = fmaxf(most, y[0]);
-      }
-#pragma unroll
-      for (int k = 1; k < kSide; k *= 2) most = fmaxf(most, __shfl_xor(most, k, kWave));
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (x[i][1] != 0.0f) sum += exp2f(x[i][0] - most) * x[i][1];
-      for (int i = n + 2 * kSide; i < runs; i += kSide) {
-        const f32x2 y = of[i * step];
-        if (y[1] != 0.0f) sum += exp2f(y[0] - most) * y[1];
-      }
-#pragma unroll
-      for (int k = 1; k < kSide; k *= 2) sum += __shfl_xor(sum, k, kWave);
-      if (n == 0) {
-        most_s[r0] = most;
-        sum_s[r0] = sum;
-      }
-    }
-    const int together = kRuns / side;  // runs
+  const int64_t step = static_cast<int64_t>(p.c.kv_heads) * p.block_rows << splits_log2;  // rows to the unit's next run
+  const int64_t at0 = (static_cast<int64_t>(first + split) * p.c.kv_heads + kvh) * p.block_rows;
+  const int runs = work.runs > split ? ((work.runs - 1 - split) >> splits_log2) + 1 : 0;  // of the unit
+  for (int row0 = chunk * rows; row0 < end; row0 += 1 << side_log2) {
+    const int row = row0 + own;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int n0 = 0; n0 < work.runs; n0 += together) {
-      const int here = min(together, work.runs - n0);
-      __syncthreads();
-      for (int i = tid; i < side * here; i += kThreads) {
-        const int r = i / here, n = i - r * here;
-        float w = 0.0f;
-        if (row0 + r < end) {
-          const f32x2 x = ml[at0 + row0 + r + (n0 + n) * step];
-          if (x[1] != 0.0f) w = exp2f(x[0] - most_s[r]);
+    float most = -INFINITY, sum = 0.0f;
+    if (row < end) {
+      const f32x2* ml = reinterpret_cast<const f32x2*>(p.part_ml) + at0 + row;
+      const float* o = p.part_o + (at0 + row) * d + dim;
+      float w = 0.0f;  // of the unit's run n0 / size * size + i
+      for (int n0 = 0; n0 < runs; n0 += kAhead) {
+        f32x4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+          if (n0 + k < runs && dim < d) v[k] = *reinterpret_cast<const f32x4*>(o + (n0 + k) * step * d);
+        if (n0 % size == 0) {
+          const f32x2 x = n0 + i < runs ? ml[(n0 + i) * step] : f32x2{-INFINITY, 0.0f};
+          float here = x[1] != 0.0f ? x[0] : -INFINITY;  // (a NaN sum takes part)
+          for (int k = 1; k < size; k *= 2) here = fmaxf(here, __shfl_xor(here, k, kWave));
+          here = fmaxf(here, most);
+          w = x[1] != 0.0f ? exp2f(x[0] - here) : 0.0f;
+          if (sum != 0.0f) {
+            const float scale = exp2f(most - here);
+            acc *= scale;
+            sum *= scale;
+          }
+          most = here;
+          float more = x[1] != 0.0f ? w * x[1] : 0.0f;
+          for (int k = 1; k < size; k *= 2) more += __shfl_xor(more, k, kWave);
+          sum += more;
         }
-        weights[r * together + n] = w;
-      }
-      __syncthreads();
-      if (own < side && row0 + own < end) {
-        const float* o = p.part_o + (at0 + row0 + own + n0 * step) * d + dim;
-#pragma unroll 8
-        for (int n = 0; n < here; ++n) {
-          const f32x4 v = *reinterpret_cast<const f32x4*>(o + n * step * d);
-          const float w = weights[own * together + n];
-          if (w != 0.0f) acc += w * v;  // (NaN weights take part)
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const float of = __shfl(w, n0 % size + k, size);
+          if (n0 + k < runs && of != 0.0f) acc += of * v[k];  // (NaN weights take part)
         }
       }
     }
-    if (own < side && row0 + own < end) {
-      const float sum = sum_s[own];
-      const int in_seq = work.block * p.block_rows + row0 + own, token = in_seq / p.gq;
+    if (splits_log2 > 0) {
+      acc_s[tid] = acc;
+      if (i == 0) {
+        most_s[unit] = most;
+        sum_s[unit] = sum;
+      }
+      __syncthreads();
+      if (split == 0) {
+        float all = -INFINITY;
+        for (int u = own; u < kThreads >> unit_log2; u += 1 << side_log2)
+          if (sum_s[u] != 0.0f) all = fmaxf(all, most_s[u]);
+        acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        sum = 0.0f;
+        for (int u = own; u < kThreads >> unit_log2; u += 1 << side_log2) {
+          if (sum_s[u] == 0.0f) continue;
+          const float of = exp2f(most_s[u] - all);
+          if (of == 0.0f) continue;
+          acc += of * acc_s[(u << unit_log2) + i];
+          sum += of * sum_s[u];
+        }
+        most = all;
+      }
+      __syncthreads();
+    }
+    if (split == 0 && row < end && dim < d) {
+      const int in_seq = work.block * p.block_rows + row, token = in_seq / p.gq;
       const int64_t to = (work.span.begin + token) * p.query_heads + kvh * p.gq + in_seq - token * p.gq;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) store_out(p.out, p.out_dtype, to * d + dim + i, sum == 0.0f ? 0.0f : acc[i] / sum);
-      if (dim == 0) p.lse[to] = sum == 0.0f ? -INFINITY : kLn2 * (most_s[own] + log2f(sum));
+      for (int x = 0; x < 4; ++x) store_out(p.out, p.out_dtype, to * d + dim + x, sum == 0.0f ? 0.0f : acc[x] / sum);
+      if (dim == 0) p.lse[to] = sum == 0.0f ? -INFINITY : kLn2 * (most + log2f(sum));
     }
-    __syncthreads();
   }
 }
 
@@ -145,9 +152,9 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
 
   // rows of a workgroup, after a sequence's rows on average
   const int64_t each = (a.tokens * p.gq + c.sequences - 1) / c.sequences;
-  plan->waves = each > 128 && !plan->precise && plan->dp <= 128 ? 8 : 4;
+  plan->waves = (each > 128 || each <= 32) && !plan->precise && plan->dp <= 128 ? 8 : 4;
   const int stage = plan->stage = tokens_stage(plan->dp, plan->waves);
-  p.row_tiles = each > 128 ? plan->waves : each > 64 ? 4 : each > 32 ? 2 : 1;
+  p.row_tiles = each > 128 ? plan->waves : each > 32 ? 4 : 1;
   p.parts = plan->waves / p.row_tiles < stage / 64 ? plan->waves / p.row_tiles : stage / 64;
   p.block_rows = 32 * p.row_tiles;
   plan->blocks = a.tokens * p.gq / p.block_rows + c.sequences + 2;
@@ -169,7 +176,8 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   const int64_t wanted = (likely * c.kv_heads < at_once ? 2 : 4) * at_once / c.kv_heads;
   const int64_t cut = wanted - likely > wanted / 2 ? wanted - likely : (wanted + 1) / 2;
   int64_t size = (work + cut - 1) / (cut > 0 ? cut : 1);
-  if (size < kLeastStages) size = kLeastStages;
+  if (size < 1) size = 1;
+  if (size < 2 && work * c.kv_heads > at_once) size = 2;  // (a run's start takes as long as a stage)
   p.items = static_cast<int>(plan->blocks);
   p.least_stages = 1 << 30;
   if (size < stages(longest)) {
@@ -204,13 +212,17 @@ int launch_paged_tokens(const kvssd_paged_cache& c, const kvssd_paged_tokens_arg
                                        : launch_paged_tokens_dims<256>;
   if (int rc = launch(p, plan.waves, plan.precise, groups, stream)) return rc;
   if (need == 0) return 0;
-  // few blocks are spread over more workgroups
-  const int rows = plan.blocks * c.kv_heads * p.block_rows > 16384 ? 32 : kThreads / (c.head_dim / 4);
+  int unit_log2 = 3;  // 8 to 64 threads a row
+  while ((4 << unit_log2) < c.head_dim) ++unit_log2;
+  // few rows' runs are split between units, and their rows spread over more workgroups
+  const bool few = plan.blocks * c.kv_heads * p.block_rows <= 16384;
+  const int splits_log2 = few ? 2 : 0, rows = few ? kThreads >> unit_log2 >> splits_log2 : 32;
   const int chunks = (p.block_rows + rows - 1) / rows;
   const dim3 grid(static_cast<unsigned>(plan.blocks * c.kv_heads * chunks));
-  if (plan.stage == 256) hipLaunchKernelGGL(paged_tokens_merge_kernel<256>, grid, dim3(kThreads), 0, stream, p, rows, chunks);
-  else if (plan.stage == 128) hipLaunchKernelGGL(paged_tokens_merge_kernel<128>, grid, dim3(kThreads), 0, stream, p, rows, chunks);
-  else hipLaunchKernelGGL(paged_tokens_merge_kernel<64>, grid, dim3(kThreads), 0, stream, p, rows, chunks);
+  const auto merge = plan.stage == 256   ? paged_tokens_merge_kernel<256>
+                     : plan.stage == 128 ? paged_tokens_merge_kernel<128>
+                                         : paged_tokens_merge_kernel<64>;
+  hipLaunchKernelGGL(merge, grid, dim3(kThreads), 0, stream, p, rows, chunks, unit_log2, splits_log2);
   return hip_status(hipGetLastError(), "paged_tokens_merge launch");
 }
 
