@@ -57,6 +57,17 @@ COMMON = [
 ]
 
 
+# flags of single sources
+MORE = {
+    # products' results in VGPRs also where a kernel may use accumulation
+    # registers: the VALU, which reads them at once, has to copy those first
+    # (two prompts of 1,024 tokens, heads of 256: 500 us became 430 in float16,
+    # 733 became 662 in float32)
+    f"paged_tokens_d{d}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+    for d in (128, 256)
+}
+
+
 HEADER = HERE.parent.parent / "include" / "kvssd_hip.h"
 BUILD_ID_MARK = b"kvssd-build-id:"
 
@@ -70,6 +81,7 @@ def source_hash() -> str:
     for f in files:
         h.update(f.name.encode() + b"\0" + f.read_bytes() + b"\0")
     h.update(" ".join(COMMON + SOURCES).encode())
+    h.update(repr(sorted(MORE.items())).encode())
     return h.hexdigest()[:16]
 
 
@@ -136,7 +148,7 @@ def build(jobs: int = 0, verbose: bool = False, timeline: bool = False) -> Path:
     if timeline:
         flags.append("-DKVSSD_TIMELINE")
     objs = [build_dir / (Path(s).stem + ".o") for s in SOURCES]
-    cmds = [[cc, *flags, "-c", str(HERE / s), "-o", str(o)] for s, o in zip(SOURCES, objs)]
+    cmds = [[cc, *flags, *MORE.get(s, []), "-c", str(HERE / s), "-o", str(o)] for s, o in zip(SOURCES, objs)]
     workers = jobs or min(len(cmds), os.cpu_count() or 1)
     with ThreadPoolExecutor(max_workers=workers) as pool:
         for fut in [pool.submit(_run, c, verbose) for c in cmds]:

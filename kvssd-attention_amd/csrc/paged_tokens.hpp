@@ -276,7 +276,6 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   constexpr int kOwn = kWave / kSlices;           // slots of a wave's pieces at a time
   constexpr int kGroups = kStage / kOwn;          // of so many slots
   constexpr int kPieces = kGroups / W;            // of a thread
-  constexpr bool kEarly = !(PREC && DP > 128);    // a stage's codes are read a stage ahead; there registers would not do
   constexpr int kValueRow = DP * 2 + (DP == 64 ? 32 : 64);  // bytes; so (but for short heads) do transposed reads meet in no bank
   constexpr int kKeyBytes = DP * kStage * 2, kValueBytes = kValueRow * kStage;
   constexpr int kBytes = kKeyBytes + kParts * kValueBytes;
@@ -297,9 +296,6 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
 
   constexpr int kTree = 1024;  // tokens of a tree whose parents are kept in LDS
   __shared__ int16_t parent_lds[kTree];
-  // the lower parts of the rows' first dims, where registers would not do: [wave][16 dims][lane]
-  constexpr int kRest = PREC && DP > 128 ? DP / 16 * 3 / 4 : 0;
-  __shared__ __attribute__((aligned(16))) u32x4 rest_lds[kRest > 0 ? W * kRest * kWave : 1];
 
   const kvssd_paged_cache& c = p.c;
   const int tid = threadIdx.x, lane = tid % kWave, wave = scalar(tid / kWave);
@@ -347,10 +343,10 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     uint32_t k[4], v[4];
     uint16_t sk, sv;
     bool live;
-  } next[kEarly ? kPieces : 1];
+  } next[kPieces];
   int page_next[kPieces], row_next[kPieces];  // of the stage after it: the page, and the row in it
 #pragma unroll
-  for (Piece& x : next) x = Piece{};
+  for (int i = 0; i < kPieces; ++i) next[i] = Piece{};
   auto find = [&](int n, int piece) {  // of the piece's slot in the list's stage n; page -1: none
     const int slot = list.stage(n) * kStage + first_slot + piece * kNext;
     page_next[piece] = -1;
@@ -361,7 +357,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     }
   };
   auto load = [&](int piece) {
-    Piece& x = next[kEarly ? piece : 0];
+    Piece& x = next[piece];
     const int page = page_next[piece];
     x.live = page >= 0 && page < c.num_pages;
     x.sk = x.sv = 0;
@@ -387,7 +383,6 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   }
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    if (!kEarly) continue;
     load(i);
     find(n_begin + 1, i);
   }
@@ -405,8 +400,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     for (int up = above(own); up >= 0; up = above(up)) ++place;
   }
   const int head = kvh * p.gq + row - own * p.gq;
-  u32x4 q[DP / 16], rest[DP / 16 - kRest];
-  auto query_rest = [&](int j) { return j < kRest ? rest_lds[(wave * kRest + j) * kWave + lane] : rest[j - kRest]; };
+  u32x4 q[kParts][DP / 16];
   float factor;
   const bool wide = PREC && p.query_dtype == KVSSD_DTYPE_F32;
   {
@@ -462,11 +456,8 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
         if constexpr (PREC)
           lo[i] = pack_half2(static_cast<_Float16>(a - static_cast<float>(ah)), static_cast<_Float16>(b - static_cast<float>(bh)));
       }
-      q[j] = ordered(hi);
-      if constexpr (PREC) {
-        if (j < kRest) rest_lds[(wave * kRest + j) * kWave + lane] = ordered(lo);
-        else rest[j - kRest] = ordered(lo);
-      }
+      q[0][j] = ordered(hi);
+      if constexpr (PREC) q[kParts - 1][j] = ordered(lo);
     }
   }
   // of the wave's rows: first and last token, as slots
@@ -558,9 +549,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       for (int j = 0; j < 2; ++j) __builtin_memcpy(&key[n % kRing][j], __builtin_assume_aligned(at + 2 * j * kStage * 16, 16), 16);
     };
     auto product = [&](int n, int j, f32x16 to) {
-      to = mfma32(key[n % kRing][j], q[n / 2 * 2 + j], to);
+      to = mfma32(key[n % kRing][j], q[0][n / 2 * 2 + j], to);
       if constexpr (PREC) {
-        if (DP > 128 || wide) to = mfma32(key[n % kRing][j], query_rest(n / 2 * 2 + j), to);
+        if (wide) to = mfma32(key[n % kRing][j], q[kParts - 1][n / 2 * 2 + j], to);
       }
       return to;
     };
@@ -587,7 +578,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       __builtin_amdgcn_sched_barrier(0);
     }
     // ---- the first tile's values set out
-    constexpr int kAhead = PREC ? (DP > 128 ? 1 : 2) : DP <= 128 ? kSteps : kSlices;  // steps
+    constexpr int kAhead = PREC ? 2 : kSteps;  // steps
     u32x4 value[kAhead];
     auto fetch = [&](int of, int n, int from) {  // of a tile, step n % 2 of slice n / 2
       const int start = value_turn(0, n / 2) ? value_at ^ value_turn(0, n / 2) * 16 : value_at;
@@ -727,10 +718,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   auto advance = [&](int n) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      if (!kEarly) load(i);  // (the page is found a stage ahead)
-      if (n + 1 < n_end) unpack_piece_into(next[kEarly ? i : 0], kBuffers > 1 ? (n + 1 - n_begin) & 1 : 0, i);
-      if (kEarly) load(i);
-      find(n + (kEarly ? 3 : 2), i);
+      if (n + 1 < n_end) unpack_piece_into(next[i], kBuffers > 1 ? (n + 1 - n_begin) & 1 : 0, i);
+      load(i);
+      find(n + 3, i);
     }
   };
   advance(n_begin - 1);
