@@ -15,6 +15,74 @@ namespace {
 
 constexpr int kThreads = 256;
 
+constexpr int kLocate = 1024;  // threads
+constexpr int kCounted = kWave - 2;  // sequences that a workgroup counts by itself, at one look
+
+// The items' and blocks' first numbers of every sequence, where they are so many that a workgroup should not count them by
+// itself: 64 at a time take about a microsecond of each (256 sequences of 8 tokens: 425 us without, 330 with it).
+template <int STAGE>
+__global__ __launch_bounds__(kLocate) void paged_tokens_locate_kernel(PagedTokensParams p) {
+  constexpr int kWaves = kLocate / kWave, kMost = 1 << 30;
+  __shared__ float work_s[kWaves], blocks_s[kWaves];
+  __shared__ int items_s[kWaves], sums_s[kWaves];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, sequences = p.c.sequences + 2;
+  float work = 0.0f, blocks = 0.0f;
+  for (int s = tid; s < sequences; s += kLocate) {
+    const TokenSpan span = token_span(p, s);
+    const int n = blocks_of(p, span);
+    if (n == 0) continue;
+    blocks += static_cast<float>(n);
+    work += static_cast<float>(n) * static_cast<float>(stages_of(p, span, n - 1, STAGE).count());
+  }
+  work = wave_sum(work);
+  blocks = wave_sum(blocks);
+  if (lane == 0) {
+    work_s[wave] = work;
+    blocks_s[wave] = blocks;
+  }
+  __syncthreads();
+  work = blocks = 0.0f;
+  for (int w = 0; w < kWaves; ++w) {
+    work += work_s[w];
+    blocks += blocks_s[w];
+  }
+  const int size = size_of_runs(p, work, blocks);
+  int32_t* const item_starts = p.starts;
+  int32_t* const block_starts = p.starts + sequences + 1;
+  if (tid == 0) p.starts[2 * sequences + 2] = size;
+  int items = 0, sums = 0;  // of the sequences before; more than a call takes count as 2^30
+  for (int s0 = 0; s0 < sequences; s0 += kLocate) {
+    const TokenSpan span = token_span(p, s0 + tid);  // (none behind the last)
+    const int n = blocks_of(p, span);
+    const int64_t all = static_cast<int64_t>(n) * runs_of_sequence<STAGE>(p, span, n, size);
+    const int own = all < (1 << 24) ? static_cast<int>(all) : 1 << 24;
+    const int item_end = wave_prefix(own), block_end = wave_prefix(n);
+    __syncthreads();
+    if (lane == kWave - 1) {
+      items_s[wave] = item_end;
+      sums_s[wave] = block_end;
+    }
+    __syncthreads();
+    int before = items, blocks_before = sums;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w == wave) {
+        before = items;
+        blocks_before = sums;
+      }
+      items = min(items + items_s[w], kMost);
+      sums = min(sums + sums_s[w], kMost);
+    }
+    if (s0 + tid < sequences) {
+      item_starts[s0 + tid] = min(before + item_end - own, kMost);
+      block_starts[s0 + tid] = min(blocks_before + block_end - n, kMost);
+    }
+  }
+  if (tid == 0) {
+    item_starts[sequences] = items;
+    block_starts[sequences] = sums;
+  }
+}
+
 // `unit` threads (d / 4, up to a power of two) take every `splits`-th run of a row, 4 dims each, kAhead runs' sums read
 // before the first one's weight is known; a lane a run forms the weights.  With few rows, whose time is the latency of these
 // reads, a row's runs are split between the units of a workgroup (8 tokens of 4 heads at 4,096 tokens of context, 33 runs:
@@ -115,7 +183,8 @@ struct Plan {
   int dp, waves, stage;
   bool precise;
   int64_t blocks;  // at most
-  size_t o_bytes, ml_bytes;
+  size_t o_bytes, ml_bytes, starts_bytes;
+  size_t bytes() const { return o_bytes + ml_bytes + starts_bytes; }
 };
 
 int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* plan) {
@@ -157,6 +226,7 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   p.row_tiles = each > 128 ? plan->waves : each > 32 ? 4 : 1;
   p.parts = plan->waves / p.row_tiles < stage / 64 ? plan->waves / p.row_tiles : stage / 64;
   p.block_rows = 32 * p.row_tiles;
+  p.block_log2 = 31 - __builtin_clz(p.block_rows);
   plan->blocks = a.tokens * p.gq / p.block_rows + c.sequences + 2;
 
   // runs, where blocks alone would leave compute units idle
@@ -189,6 +259,7 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   const size_t rows = split ? static_cast<size_t>(p.items) * c.kv_heads * p.block_rows : 0;
   plan->o_bytes = aligned(rows * c.head_dim * sizeof(float));
   plan->ml_bytes = aligned(rows * 2 * sizeof(float));
+  if (c.sequences > kCounted) plan->starts_bytes = aligned((2 * (static_cast<size_t>(c.sequences) + 3) + 1) * sizeof(int32_t));
   return 0;
 }
 
@@ -196,7 +267,7 @@ int launch_paged_tokens(const kvssd_paged_cache& c, const kvssd_paged_tokens_arg
   Plan plan;
   if (int rc = plan_of(c, a, &plan)) return rc;
   PagedTokensParams& p = plan.p;
-  const size_t need = plan.o_bytes + plan.ml_bytes;
+  const size_t need = plan.bytes();
   if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need))
     return arg_error("workspace too small: need " + std::to_string(need) + " bytes");
   if (reinterpret_cast<uintptr_t>(a.workspace) % 256) return arg_error("workspace must be 256-byte aligned");
@@ -205,13 +276,20 @@ int launch_paged_tokens(const kvssd_paged_cache& c, const kvssd_paged_tokens_arg
   if (reinterpret_cast<uintptr_t>(a.out) % 16) return arg_error("out must be 16-byte aligned");
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + plan.o_bytes);
+  const auto of_stage = [&](auto of256, auto of128, auto of64) { return plan.stage == 256 ? of256 : plan.stage == 128 ? of128 : of64; };
+  if (plan.starts_bytes > 0) {
+    p.starts = reinterpret_cast<int32_t*>(static_cast<char*>(a.workspace) + plan.o_bytes + plan.ml_bytes);
+    const auto locate = of_stage(paged_tokens_locate_kernel<256>, paged_tokens_locate_kernel<128>, paged_tokens_locate_kernel<64>);
+    hipLaunchKernelGGL(locate, dim3(1), dim3(kLocate), 0, stream, p);
+    if (int rc = hip_status(hipGetLastError(), "paged_tokens_locate launch")) return rc;
+  }
   const int64_t work = static_cast<int64_t>(p.items) * c.kv_heads;
   const unsigned groups = static_cast<unsigned>(c.kv_heads % 2 ? work : (work + 15) / 16 * 16);
   const auto launch = plan.dp == 64    ? launch_paged_tokens_dims<64>
                       : plan.dp == 128 ? launch_paged_tokens_dims<128>
                                        : launch_paged_tokens_dims<256>;
   if (int rc = launch(p, plan.waves, plan.precise, groups, stream)) return rc;
-  if (need == 0) return 0;
+  if (plan.o_bytes == 0) return 0;
   int unit_log2 = 3;  // 8 to 64 threads a row
   while ((4 << unit_log2) < c.head_dim) ++unit_log2;
   // few rows' runs are split between units, and their rows spread over more workgroups
@@ -219,9 +297,7 @@ int launch_paged_tokens(const kvssd_paged_cache& c, const kvssd_paged_tokens_arg
   const int splits_log2 = few ? 2 : 0, rows = few ? kThreads >> unit_log2 >> splits_log2 : 32;
   const int chunks = (p.block_rows + rows - 1) / rows;
   const dim3 grid(static_cast<unsigned>(plan.blocks * c.kv_heads * chunks));
-  const auto merge = plan.stage == 256   ? paged_tokens_merge_kernel<256>
-                     : plan.stage == 128 ? paged_tokens_merge_kernel<128>
-                                         : paged_tokens_merge_kernel<64>;
+  const auto merge = of_stage(paged_tokens_merge_kernel<256>, paged_tokens_merge_kernel<128>, paged_tokens_merge_kernel<64>);
   hipLaunchKernelGGL(merge, grid, dim3(kThreads), 0, stream, p, rows, chunks, unit_log2, splits_log2);
   return hip_status(hipGetLastError(), "paged_tokens_merge launch");
 }
@@ -240,7 +316,7 @@ __attribute__((visibility("default"))) int kvssd_hip_paged_tokens_workspace_byte
   if (args == nullptr || bytes == nullptr) return arg_error("arguments are NULL");
   Plan plan;
   if (int rc = plan_of(*cache, *args, &plan)) return rc;
-  *bytes = plan.o_bytes + plan.ml_bytes;
+  *bytes = plan.bytes();
   return 0;
 }
 

@@ -49,13 +49,15 @@ struct PagedTokensParams {
   const int32_t* parents;
   float* part_o;   // [item][kv head][row][head_dim]
   float* part_ml;  // [item][kv head][row][2]
+  int32_t* starts;  // of many sequences: first items [sequences + 3], first blocks [sequences + 3], the runs' size
   int64_t tokens;
   int capacity, window, sink;
   int query_heads, gq, query_dtype, out_dtype;
   int groups, slices_log2;  // scale groups of a head; 32-dim slices of a group
   Divisor of_page;          // slots of a page
   int row_tiles, parts;     // of a workgroup: waves side by side on rows, on slots
-  int block_rows;           // rows of a workgroup
+  int block_rows;           // rows of a workgroup, 2^block_log2
+  int block_log2;
   int items;                // (row block, run) pairs that the grid and the workspace hold
   int least_stages;         // of a run, unless the lengths call for more
   float scale_log2;
@@ -100,7 +102,9 @@ __device__ __forceinline__ TokenSpan token_span(const PagedTokensParams& p, int 
 }
 
 __device__ __forceinline__ int blocks_of(const PagedTokensParams& p, const TokenSpan& s) {
-  return static_cast<int>((static_cast<int64_t>(s.count) * p.gq + p.block_rows - 1) / p.block_rows);
+  // (2^24 of them are more than a call takes; so do their sums over a wave stay below 2^31, whatever the offsets)
+  const int64_t n = (static_cast<int64_t>(s.count) * p.gq + p.block_rows - 1) >> p.block_log2;
+  return static_cast<int>(n < (1 << 24) ? n : 1 << 24);
 }
 
 // Stages that a block's tokens see something of: those of the sinks, then from `second` to `end`.
@@ -140,6 +144,13 @@ __device__ __forceinline__ int runs_of_sequence(const PagedTokensParams& p, cons
   return stages <= size ? 1 : (stages + size - 1) / size;
 }
 
+__device__ __forceinline__ int size_of_runs(const PagedTokensParams& p, float work, float blocks) {
+  const float room = static_cast<float>(p.items) - blocks;
+  if (room < 1.0f) return 1 << 30;
+  const float least = work / room * 1.0001f + 1.0f;  // (sums of 24 bits)
+  return max(p.least_stages, least < 1e9f ? static_cast<int>(least) : 1 << 30);
+}
+
 template <int STAGE>
 __device__ __forceinline__ int run_size(const PagedTokensParams& p) {
   const int lane = threadIdx.x % kWave;
@@ -154,19 +165,41 @@ __device__ __forceinline__ int run_size(const PagedTokensParams& p) {
   }
   work = wave_sum(work);
   blocks = wave_sum(blocks);
-  const float room = static_cast<float>(p.items) - blocks;
-  if (room < 1.0f) return 1 << 30;
-  const float least = work / room * 1.0001f + 1.0f;  // (sums of 24 bits)
-  return max(p.least_stages, least < 1e9f ? static_cast<int>(least) : 1 << 30);
+  return size_of_runs(p, work, blocks);
 }
 
-// Item `item`; seq -1 where there are fewer.  `blocks_alone`: items are blocks.
+// What item `own` of a sequence is; `blocks_alone`: items are blocks.
+__device__ __forceinline__ TokenItem item_of(int seq, const TokenSpan& span, int blocks, int runs, int own, bool blocks_alone) {
+  const int place = blocks_alone || runs <= 1 ? own : own / runs;
+  return {seq, blocks - 1 - place, blocks_alone ? 0 : own - place * runs, runs, span};  // the longest first
+}
+
+// Item `item`; seq -1 where there are fewer.  first: of the item's first run.
 template <int STAGE>
 __device__ __forceinline__ TokenItem find_item(const PagedTokensParams& p, int item, bool blocks_alone, int* first) {
   const int lane = threadIdx.x % kWave;
+  const int sequences = p.c.sequences + 2;  // with the two of no sequence
+  if (p.starts) {
+    // the last one that starts at or before the item: 64 of them compared at a time
+    const int32_t* starts = p.starts + (blocks_alone ? sequences + 1 : 0);
+    if (item >= starts[sequences]) return TokenItem{-1, 0, 0, 1, {0, 0, 0}};
+    int at = 0;
+    for (int n = sequences; n > 1;) {
+      const int step = (n + kWave - 1) / kWave;
+      const bool upto = lane * step < n && starts[at + lane * step] <= item;
+      const int last = 63 - __builtin_clzll(__ballot(upto));  // (the first one does)
+      at += last * step;
+      n = min(step, n - last * step);
+    }
+    const TokenSpan span = token_span(p, at);
+    const int blocks = blocks_of(p, span), runs = runs_of_sequence<STAGE>(p, span, blocks, p.starts[2 * sequences + 2]);
+    const TokenItem t = item_of(at, span, blocks, runs, item - starts[at], blocks_alone);
+    if (first != nullptr) *first = p.starts[at] + (blocks - 1 - t.block) * runs;
+    return t;
+  }
   const int size = run_size<STAGE>(p);
   int before = 0;  // items of the sequences before
-  for (int s0 = 0; s0 < p.c.sequences + 2; s0 += kWave) {
+  for (int s0 = 0; s0 < sequences; s0 += kWave) {
     const TokenSpan s = token_span(p, s0 + lane);
     const int blocks = blocks_of(p, s);
     const int runs = runs_of_sequence<STAGE>(p, s, blocks, size);
@@ -176,19 +209,13 @@ __device__ __forceinline__ TokenItem find_item(const PagedTokensParams& p, int i
     if (past) {
       const int at = __builtin_ctzll(past);
       const int own = item - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
-      TokenItem t;
-      t.seq = s0 + at;
-      t.runs = __builtin_amdgcn_readlane(runs, at);
+      const TokenSpan span = {static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(s.begin), at)),  // (below 2^30)
+                              __builtin_amdgcn_readlane(s.count, at), __builtin_amdgcn_readlane(s.length, at)};
       const int count = __builtin_amdgcn_readlane(blocks, at);
-      const int place = blocks_alone ? own : own / t.runs;
-      t.block = count - 1 - place;  // the longest first
-      t.run = blocks_alone ? 0 : own - place * t.runs;
-      t.span.begin = static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(s.begin), at));  // (below 2^30)
-      t.span.count = __builtin_amdgcn_readlane(s.count, at);
-      t.span.length = __builtin_amdgcn_readlane(s.length, at);
+      const TokenItem t = item_of(s0 + at, span, count, __builtin_amdgcn_readlane(runs, at), own, blocks_alone);
       if (first != nullptr) {
         const int all = wave_prefix(blocks * runs);
-        *first = before + __builtin_amdgcn_readlane(all, at) - count * t.runs + place * t.runs;
+        *first = before + __builtin_amdgcn_readlane(all, at) - (t.block + 1) * t.runs;
       }
       return t;
     }
