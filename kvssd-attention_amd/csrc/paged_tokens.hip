@@ -102,7 +102,6 @@ __global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedToken
   const int side_log2 = 8 - unit_log2 - splits_log2;  // rows side by side (of 256 threads)
   const int own = unit & ((1 << side_log2) - 1), split = unit >> side_log2;
   const int end = min(min(work.span.count * p.gq - work.block * p.block_rows, p.block_rows), (chunk + 1) * rows);
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
   const int64_t step = static_cast<int64_t>(p.c.kv_heads) * p.block_rows << splits_log2;  // rows to the unit's next run
   const int64_t at0 = (static_cast<int64_t>(first + split) * p.c.kv_heads + kvh) * p.block_rows;
   const int runs = work.runs > split ? ((work.runs - 1 - split) >> splits_log2) + 1 : 0;  // of the unit
@@ -181,7 +180,7 @@ size_t aligned(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 struct Plan {
   PagedTokensParams p;
   int dp, waves, stage;
-  bool precise;
+  bool precise, own;  // `own`: every wave unpacks slots of its own
   int64_t blocks;  // at most
   size_t o_bytes, ml_bytes, starts_bytes;
   size_t bytes() const { return o_bytes + ml_bytes + starts_bytes; }
@@ -221,8 +220,9 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
 
   // rows of a workgroup, after a sequence's rows on average
   const int64_t each = (a.tokens * p.gq + c.sequences - 1) / c.sequences;
-  plan->waves = (each > 128 || each <= 32) && !plan->precise && plan->dp <= 128 ? 8 : 4;
-  const int stage = plan->stage = tokens_stage(plan->dp, plan->waves);
+  plan->own = each <= 32 && !plan->precise && plan->dp <= 128;
+  plan->waves = each > 128 && !plan->precise && plan->dp <= 128 ? 8 : 4;
+  const int stage = plan->stage = plan->own ? plan->waves * 64 : tokens_stage(plan->dp, plan->waves);
   p.row_tiles = each > 128 ? plan->waves : each > 32 ? 4 : 1;
   p.parts = plan->waves / p.row_tiles < stage / 64 ? plan->waves / p.row_tiles : stage / 64;
   p.block_rows = 32 * p.row_tiles;
@@ -242,7 +242,7 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   const int64_t work = (total / stage + c.sequences) * (likely / c.sequences);    // stages of all blocks
   // workgroups that run at a time (LDS and registers); two rounds of them where blocks are few, four of more, whose
   // lengths differ
-  const int64_t at_once = plan->waves == 4 && !plan->precise && plan->dp <= 128 ? 512 : 256;
+  const int64_t at_once = plan->waves == 4 && !plan->precise && plan->dp <= (plan->own ? 64 : 128) ? 512 : 256;
   const int64_t wanted = (likely * c.kv_heads < at_once ? 2 : 4) * at_once / c.kv_heads;
   const int64_t cut = wanted - likely > wanted / 2 ? wanted - likely : (wanted + 1) / 2;
   int64_t size = (work + cut - 1) / (cut > 0 ? cut : 1);
@@ -288,7 +288,7 @@ int launch_paged_tokens(const kvssd_paged_cache& c, const kvssd_paged_tokens_arg
   const auto launch = plan.dp == 64    ? launch_paged_tokens_dims<64>
                       : plan.dp == 128 ? launch_paged_tokens_dims<128>
                                        : launch_paged_tokens_dims<256>;
-  if (int rc = launch(p, plan.waves, plan.precise, groups, stream)) return rc;
+  if (int rc = launch(p, plan.waves, plan.precise, plan.own, groups, stream)) return rc;
   if (plan.o_bytes == 0) return 0;
   int unit_log2 = 3;  // 8 to 64 threads a row
   while ((4 << unit_log2) < c.head_dim) ++unit_log2;

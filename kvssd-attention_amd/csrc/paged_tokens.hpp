@@ -64,6 +64,7 @@ struct PagedTokensParams {
 };
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
@@ -78,6 +79,12 @@ __device__ __forceinline__ u32x2 lds_read_tr16(const uint8_t* lds) {
 
 __device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// two bf16, rounded to nearest, ties to even
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
 
 // ---------------------------------------------------------------- the work ---
 
@@ -240,13 +247,13 @@ __device__ __forceinline__ void place_of(const PagedTokensParams& p, int id, int
 }
 
 template <int DP>
-int launch_paged_tokens_dims(const PagedTokensParams& p, int waves, bool precise, unsigned groups, hipStream_t stream);
+int launch_paged_tokens_dims(const PagedTokensParams& p, int waves, bool precise, bool own, unsigned groups, hipStream_t stream);
 template <>
-int launch_paged_tokens_dims<64>(const PagedTokensParams& p, int waves, bool precise, unsigned groups, hipStream_t stream);
+int launch_paged_tokens_dims<64>(const PagedTokensParams& p, int waves, bool precise, bool own, unsigned groups, hipStream_t stream);
 template <>
-int launch_paged_tokens_dims<128>(const PagedTokensParams& p, int waves, bool precise, unsigned groups, hipStream_t stream);
+int launch_paged_tokens_dims<128>(const PagedTokensParams& p, int waves, bool precise, bool own, unsigned groups, hipStream_t stream);
 template <>
-int launch_paged_tokens_dims<256>(const PagedTokensParams& p, int waves, bool precise, unsigned groups, hipStream_t stream);
+int launch_paged_tokens_dims<256>(const PagedTokensParams& p, int waves, bool precise, bool own, unsigned groups, hipStream_t stream);
 
 // ------------------------------------------------------------------ kernel ---
 
@@ -293,18 +300,20 @@ __device__ __forceinline__ void add_scaled_rows(float (&s)[16], const f32x16& do
 }
 
 // W: waves.  Small blocks take four, two workgroups a CU; large ones eight, which unpack a stage twice as long together.
-template <int DP, int W, bool PREC>
-__global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) void paged_tokens_kernel(PagedTokensParams p) {
-  constexpr int kStage = tokens_stage(DP, W);
+template <int DP, int W, bool PREC, bool OWN>
+__global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) ? 2 : 1) void paged_tokens_kernel(PagedTokensParams p) {
+  constexpr int kStage = OWN ? 64 * W : tokens_stage(DP, W);
+  constexpr int kSlots = OWN ? 64 : kStage;       // of a buffer in LDS
   constexpr int kSlices = DP / 32;
   constexpr int kParts = PREC ? 2 : 1;
-  constexpr int kBuffers = PREC ? 1 : 2;          // stages in LDS: one is unpacked while another is worked on
-  constexpr int kTiles = kStage / 32;             // of a stage
+  // in LDS: stages, one of which is unpacked while another is worked on, or the waves' parts of one
+  constexpr int kBuffers = OWN ? W : PREC ? 1 : 2;
+  constexpr int kTiles = kSlots / 32;             // of a buffer
   constexpr int kOwn = kWave / kSlices;           // slots of a wave's pieces at a time
-  constexpr int kGroups = kStage / kOwn;          // of so many slots
-  constexpr int kPieces = kGroups / W;            // of a thread
+  constexpr int kGroups = kSlots / kOwn;          // of so many slots
+  constexpr int kPieces = OWN ? kGroups : kGroups / W;  // of a thread
   constexpr int kValueRow = DP * 2 + (DP == 64 ? 32 : 64);  // bytes; so (but for short heads) do transposed reads meet in no bank
-  constexpr int kKeyBytes = DP * kStage * 2, kValueBytes = kValueRow * kStage;
+  constexpr int kKeyBytes = DP * kSlots * 2, kValueBytes = kValueRow * kSlots;
   constexpr int kBytes = kKeyBytes + kParts * kValueBytes;
   constexpr float kBias = 8.0f, kRoom = 14.0f;    // log2 of a weight at the reference's maximum, and at most
   constexpr int kPlain = 14;                      // exponent of the scales that the largest factor (2^15) serves
@@ -357,8 +366,8 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   }
 
   // ---- a thread's pieces: 32 dims of a slot
-  const int first_slot = tid / kSlices, slice = tid % kSlices;
-  constexpr int kNext = W * kOwn;  // slots to the thread's next piece
+  const int first_slot = (OWN ? lane : tid) / kSlices, slice = tid % kSlices;  // in a buffer
+  constexpr int kNext = OWN ? kOwn : W * kOwn;  // slots to the thread's next piece
   const int d = c.head_dim, row_bytes = d * c.bits / 8;
   const bool has_dims = slice * 32 < d;
   const int piece_bytes = 4 * c.bits;
@@ -375,7 +384,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) next[i] = Piece{};
   auto find = [&](int n, int piece) {  // of the piece's slot in the list's stage n; page -1: none
-    const int slot = list.stage(n) * kStage + first_slot + piece * kNext;
+    const int slot = list.stage(n) * kStage + (OWN ? wave * kSlots : 0) + first_slot + piece * kNext;
     page_next[piece] = -1;
     if (n < n_end && slot < length) {
       const int nth = p.of_page.quotient(slot);
@@ -513,7 +522,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const int chunk = 4 * slice + w;
-      *reinterpret_cast<u32x4*>(&lds[buf][(chunk * kStage + (piece_slot ^ slice * kTurn)) * 16]) = codes[w];
+      *reinterpret_cast<u32x4*>(&lds[buf][(chunk * kSlots + (piece_slot ^ slice * kTurn)) * 16]) = codes[w];
     }
     const int in_tile = piece_slot % 32;
     scale_lds[buf][slice][piece_slot / 32][in_tile >> 2 & 1][(in_tile >> 3) * 4 + in_tile % 4] = half_bits_to_float(x.sk);
@@ -523,9 +532,10 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     int most = top;
     if (__any(!bad && ex > top)) most = static_cast<int>(wave_most(bad ? 0u : static_cast<uint32_t>(ex)));
     if (lane == 0) {
-      live_lds[buf][piece * W + wave] = live;
-      bad_lds[buf][piece * W + wave] = bads;
-      flags_lds[buf][piece * W + wave] = most | (live == ~0ull ? 0u : kGaps) | (bads != 0 ? kBad : 0u);
+      const int group = OWN ? piece : piece * W + wave;
+      live_lds[buf][group] = live;
+      bad_lds[buf][group] = bads;
+      flags_lds[buf][group] = most | (live == ~0ull ? 0u : kGaps) | (bads != 0 ? kBad : 0u);
     }
     unpack(x.v, codes);
     const _Float16 up = __builtin_bit_cast(_Float16, static_cast<uint16_t>((44 - most) << 10));  // 2^(29 - most)
@@ -571,9 +581,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     asm volatile("" : "+v"(at_col));  // (a register for every turn of it would be kept otherwise)
     auto read_keys = [&](int n) {
       sk[n % kRing] = scale_lds[buf][n / 2][tile + n % 2][half][lane & 15];  // a slot's a lane, alike in the half's two rows
-      const uint8_t* at = stage + ((4 * (n / 2) + half) * kStage + (at_col ^ n / 2 * kTurn) + 32 * (n % 2)) * 16;
+      const uint8_t* at = stage + ((4 * (n / 2) + half) * kSlots + (at_col ^ n / 2 * kTurn) + 32 * (n % 2)) * 16;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) __builtin_memcpy(&key[n % kRing][j], __builtin_assume_aligned(at + 2 * j * kStage * 16, 16), 16);
+      for (int j = 0; j < 2; ++j) __builtin_memcpy(&key[n % kRing][j], __builtin_assume_aligned(at + 2 * j * kSlots * 16, 16), 16);
     };
     auto product = [&](int n, int j, f32x16 to) {
       to = mfma32(key[n % kRing][j], q[0][n / 2 * 2 + j], to);
@@ -640,25 +650,20 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
           for (int up = own; up >= 0 && base + up >= s0; up = above(up), --at)
             if (base + up < s0 + 32 && (p.window == 0 || at > place - p.window || at < p.sink)) bits |= 1u << (base + up - s0);
         }
-        if (!all_live) {
-#pragma unroll 1
-          for (int y = 0; y < 32; ++y) {
-            const uint64_t live = live_lds[buf][(32 * (tile + x) + y) / kOwn];  // of one wave's pieces; kSlices lanes a slot
-            if (!(live >> ((32 * (tile + x) + y) % kOwn * kSlices) & 1)) bits &= ~(1u << y);
-          }
-        }
+        const int in_buffer = 32 * (tile + x) + col, group = in_buffer / kOwn, piece_lane = in_buffer % kOwn * kSlices;  // col's slot
+        if (!all_live) bits &= static_cast<uint32_t>(__ballot(live_lds[buf][group] >> piece_lane & 1));
         bits >>= 4 * half;
         seen[x] = (bits & 0xFu) | (bits >> 4 & 0xF0u) | (bits >> 8 & 0xF00u) | (bits >> 12 & 0xF000u);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[x][r] = seen[x] >> r & 1u ? s[x][r] : -INFINITY;
         if (any_bad) {
-          for (int y = 0; y < 32; ++y) {  // slots of the tile with a value scale that is not finite
-            const uint64_t bads = bad_lds[buf][(32 * (tile + x) + y) / kOwn];
-            const uint32_t groups = static_cast<uint32_t>(bads >> ((32 * (tile + x) + y) % kOwn * kSlices)) & ((1u << kSlices) - 1);
-            if (scalar(groups) == 0) continue;
+          const uint32_t bad_slices = static_cast<uint32_t>(bad_lds[buf][group] >> piece_lane) & ((1u << kSlices) - 1);
+#pragma unroll 1
+          for (uint32_t slots = static_cast<uint32_t>(__ballot(bad_slices != 0)); slots != 0; slots &= slots - 1) {
+            const int y = __builtin_ctz(slots);  // a slot of the tile with a value scale that is not finite
             const int r = (y >> 3) * 4 + y % 4;
             const int here = half == (y >> 2 & 1) && (seen[x] >> r & 1u);
-            if (here | __shfl_xor(here, 32, kWave)) poison |= groups;
+            if (here | __shfl_xor(here, 32, kWave)) poison |= __builtin_amdgcn_readlane(bad_slices, y);
           }
         }
       }
@@ -704,7 +709,6 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       for (int step = 0; step < 2; ++step)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          typedef float f32x2 __attribute__((ext_vector_type(2)));
           const f32x2 v = {t[8 * step + 2 * k], t[8 * step + 2 * k + 1]};
           const half2v h = __builtin_convertvector(v, half2v);
           w[0][step][k] = __builtin_bit_cast(uint32_t, h);
@@ -745,16 +749,16 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   auto advance = [&](int n) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      if (n + 1 < n_end) unpack_piece_into(next[i], kBuffers > 1 ? (n + 1 - n_begin) & 1 : 0, i);
+      if (n + 1 < n_end) unpack_piece_into(next[i], OWN ? wave : kBuffers > 1 ? (n + 1 - n_begin) & 1 : 0, i);
       load(i);
       find(n + 3, i);
     }
   };
   advance(n_begin - 1);
-  __syncthreads();
+  if (!OWN) __syncthreads();
   for (int n = n_begin; n < n_end; ++n) {
-    const int buf = kBuffers > 1 ? (n - n_begin) & 1 : 0;
-    const int slot0 = list.stage(n) * kStage;
+    const int buf = OWN ? wave : kBuffers > 1 ? (n - n_begin) & 1 : 0;
+    const int slot0 = list.stage(n) * kStage + (OWN ? wave * kSlots : 0);
     uint32_t flags = 0, highest = 0, lowest = 31;
     {
       uint32_t of[kGroups];
@@ -774,7 +778,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       top = tops;
     }
     if (active) {
-      for (int tile = 2 * part; tile < kTiles; tile += 2 * p.parts) {
+      for (int tile = OWN ? 0 : 2 * part; tile < kTiles; tile += 2 * (OWN ? 1 : p.parts)) {
         const int t0 = slot0 + 32 * tile, t1 = t0 + 63;
         // whether every row of the wave sees all of the tiles' slots, or none
         const int reach_lo = tree ? base : own_lo;  // the lowest position; slots up to it are seen, but for the window
@@ -789,16 +793,26 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     }
     if (kBuffers == 1) __syncthreads();
     advance(n);
-    __syncthreads();
+    if (!OWN) __syncthreads();  // (a wave's LDS operations are done in their order)
   }
 
   // ---- waves of the same rows are joined (their parts of the slots in LDS, one after the other)
+  if constexpr (OWN) {  // to one scale of the values
+    if (lane == 0) flags_lds[wave][0] = top;
+    __syncthreads();
+    uint32_t highest = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) highest = max(highest, flags_lds[w][0]);
+    const int tops = scalar(highest);
+    behind *= __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - tops) << 23);
+    top = tops;
+  }
   l += __shfl_xor(l, 32, kWave);
 #pragma unroll
   for (int i = 0; i < kSlices; ++i) acc[i] *= poison >> i & 1u ? __builtin_nanf("") : behind;
-  if (p.parts > 1) {
+  if (!OWN && p.parts > 1) {
     constexpr int kRow = kSlices * 16 + 2;
-    static_assert(kTiles == 2 || W / 2 * kRow * kWave * 4 <= kBuffers * kBytes, "a part's accumulators");
+    static_assert(OWN || kTiles == 2 || W / 2 * kRow * kWave * 4 <= kBuffers * kBytes, "a part's accumulators");
     float* mine = reinterpret_cast<float*>(lds[0]) + (wave % p.row_tiles) * kRow * kWave + lane;  // [row tile][kRow][lane]
     for (int other = 1; other < p.parts; ++other) {
       __syncthreads();
@@ -825,19 +839,54 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       }
     }
   }
-  if (part != 0) return;
+  constexpr int kQuads = 4 * kSlices;  // of four dims of a row: the accumulators of a lane
+  constexpr int kFinish = OWN ? kQuads / W : kQuads;  // of a wave
+  f32x4 quads[kFinish];
+  if constexpr (OWN) {  // every wave joins some of the dims
+    f32x4* all = reinterpret_cast<f32x4*>(lds[0]);  // [quad][part][lane]
+    f32x2* sums = reinterpret_cast<f32x2*>(all + kQuads * W * kWave);  // [part][lane]
+    static_assert((kQuads * 16 + 8) * W * kWave <= kBuffers * kBytes, "the parts' accumulators");
+    // (no wave reads what it has unpacked any more: they have met above)
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+      const f32x16& of = acc[q / 4];
+      all[(q * W + wave) * kWave + lane] = f32x4{of[q % 4 * 4], of[q % 4 * 4 + 1], of[q % 4 * 4 + 2], of[q % 4 * 4 + 3]};
+    }
+    sums[wave * kWave + lane] = f32x2{m, l};
+    __syncthreads();
+    f32x2 of[W];
+    float ref = -INFINITY;  // (a part that saw nothing has l = 0, and its reference counts for nothing)
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      of[w] = sums[w * kWave + lane];
+      if (of[w][1] != 0.0f) ref = fmaxf(ref, of[w][0]);
+    }
+    m = ref;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kFinish; ++i) quads[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float by = of[w][1] != 0.0f ? exp2f(of[w][0] - ref) : 0.0f;
+      l += of[w][1] != 0.0f ? of[w][1] * by : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kFinish; ++i) quads[i] += by * all[((wave * kFinish + i) * W + w) * kWave + lane];
+    }
+  } else {
+    if (part != 0) return;
+#pragma unroll
+    for (int i = 0; i < kFinish; ++i) quads[i] = f32x4{acc[i / 4][i % 4 * 4], acc[i / 4][i % 4 * 4 + 1], acc[i / 4][i % 4 * 4 + 2], acc[i / 4][i % 4 * 4 + 3]};
+  }
   if (c.bits == 4) {  // a chunk's dims lie 0, 4, 1, 5 in the lower half's lanes, 2, 6, 3, 7 in the upper one's
 #pragma unroll
-    for (int i = 0; i < kSlices; ++i)
+    for (int i = 0; i < kFinish; ++i) {
+      const float v[4] = {quads[i][0], quads[i][1], quads[i][2], quads[i][3]};
+      const auto even = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v[0]), __builtin_bit_cast(uint32_t, v[1]), false, false);
+      const auto odd = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v[2]), __builtin_bit_cast(uint32_t, v[3]), false, false);
+      const uint32_t lanes[4] = {even[0], odd[0], even[1], odd[1]};
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
-        const float v[4] = {acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]};
-        const auto even = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v[0]), __builtin_bit_cast(uint32_t, v[1]), false, false);
-        const auto odd = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v[2]), __builtin_bit_cast(uint32_t, v[3]), false, false);
-        const uint32_t lanes[4] = {even[0], odd[0], even[1], odd[1]};
-#pragma unroll
-        for (int y = 0; y < 4; ++y) acc[i][j + y] = __builtin_bit_cast(float, lanes[y]);
-      }
+      for (int y = 0; y < 4; ++y) quads[i][y] = __builtin_bit_cast(float, lanes[y]);
+    }
   }
 
   // ---- the result, or the run's partial
@@ -849,31 +898,28 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   const float by = !whole ? unit : none ? 0.0f : unit / l;
   if (wave_row0 + col >= rows) return;
 #pragma unroll
-  for (int i = 0; i < kSlices; ++i)
+  for (int i = 0; i < kFinish; ++i) {
+    const int dim = 8 * ((OWN ? wave * kFinish : 0) + i) + 4 * half;
+    if (dim >= d) continue;
+    f32x4 v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int dim = 32 * i + 8 * j + 4 * half;
-      if (dim >= d) continue;
-      f32x4 v;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) v[y] = whole && none ? 0.0f : acc[i][4 * j + y] * by;
-      if (!whole) {
-        *reinterpret_cast<f32x4*>(p.part_o + part_at * d + dim) = v;
-      } else if (p.out_dtype == KVSSD_DTYPE_F32) {
-        *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + at * d + dim) = v;
+    for (int y = 0; y < 4; ++y) v[y] = whole && none ? 0.0f : quads[i][y] * by;
+    if (!whole) {
+      *reinterpret_cast<f32x4*>(p.part_o + part_at * d + dim) = v;
+    } else if (p.out_dtype == KVSSD_DTYPE_F32) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + at * d + dim) = v;
+    } else {
+      u32x2 o;
+      if (p.out_dtype == KVSSD_DTYPE_F16) {
+        o = u32x2{pack_half2(static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1])),
+                  pack_half2(static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3]))};
       } else {
-        u32x2 o;
-        if (p.out_dtype == KVSSD_DTYPE_F16) {
-          o = u32x2{pack_half2(static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1])),
-                    pack_half2(static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3]))};
-        } else {
-          o = u32x2{store_cast<uint16_t>(v[0]) | static_cast<uint32_t>(store_cast<uint16_t>(v[1])) << 16,
-                    store_cast<uint16_t>(v[2]) | static_cast<uint32_t>(store_cast<uint16_t>(v[3])) << 16};
-        }
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + at * d + dim) = o;
+        o = u32x2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
       }
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + at * d + dim) = o;
     }
-  if (half == 0) {
+  }
+  if (half == 0 && (!OWN || wave == 0)) {
     if (whole) {
       p.lse[at] = none ? -INFINITY : kLn2 * (m + log2f(l));
     } else {
@@ -883,9 +929,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   }
 }
 
-template <int DP, int W, bool PREC>
+template <int DP, int W, bool PREC, bool OWN>
 int launch_paged_tokens_kernel(const PagedTokensParams& p, unsigned groups, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_tokens_kernel<DP, W, PREC>), dim3(groups), dim3(W * kWave), 0, stream, p);
+  hipLaunchKernelGGL((paged_tokens_kernel<DP, W, PREC, OWN>), dim3(groups), dim3(W * kWave), 0, stream, p);
   return hip_status(hipGetLastError(), "paged_tokens launch");
 }
 

@@ -4,9 +4,9 @@
 namespace kvssd {
 
 template <>
-int launch_paged_tokens_dims<256>(const PagedTokensParams& p, int waves, bool precise, unsigned groups, hipStream_t stream) {
-  return precise ? launch_paged_tokens_kernel<256, 4, true>(p, groups, stream)
-                 : launch_paged_tokens_kernel<256, 4, false>(p, groups, stream);
+int launch_paged_tokens_dims<256>(const PagedTokensParams& p, int waves, bool precise, bool, unsigned groups, hipStream_t stream) {
+  return precise ? launch_paged_tokens_kernel<256, 4, true, false>(p, groups, stream)
+                 : launch_paged_tokens_kernel<256, 4, false, false>(p, groups, stream);
 }
 
 }  // namespace kvssd

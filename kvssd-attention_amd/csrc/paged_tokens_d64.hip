@@ -4,10 +4,11 @@
 namespace kvssd {
 
 template <>
-int launch_paged_tokens_dims<64>(const PagedTokensParams& p, int waves, bool precise, unsigned groups, hipStream_t stream) {
-  if (waves == 8) return launch_paged_tokens_kernel<64, 8, false>(p, groups, stream);
-  return precise ? launch_paged_tokens_kernel<64, 4, true>(p, groups, stream)
-                 : launch_paged_tokens_kernel<64, 4, false>(p, groups, stream);
+int launch_paged_tokens_dims<64>(const PagedTokensParams& p, int waves, bool precise, bool own, unsigned groups, hipStream_t stream) {
+  if (own) return launch_paged_tokens_kernel<64, 4, false, true>(p, groups, stream);
+  if (waves == 8) return launch_paged_tokens_kernel<64, 8, false, false>(p, groups, stream);
+  return precise ? launch_paged_tokens_kernel<64, 4, true, false>(p, groups, stream)
+                 : launch_paged_tokens_kernel<64, 4, false, false>(p, groups, stream);
 }
 
 }  // namespace kvssd
