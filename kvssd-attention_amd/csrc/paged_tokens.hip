@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedToken
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
           const float of = __shfl(w, n0 % size + k, size);
-          if (n0 + k < runs && of != 0.0f) acc += of * v[k];  // (NaN weights take part)
+          if (n0 + k < runs) acc += of * v[k];  // (sums that are not finite take part whatever their weight, as slots' values do)
         }
       }
     }
@@ -157,7 +157,6 @@ __global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedToken
         for (int u = own; u < kThreads >> unit_log2; u += 1 << side_log2) {
           if (sum_s[u] == 0.0f) continue;
           const float of = exp2f(most_s[u] - all);
-          if (of == 0.0f) continue;
           acc += of * acc_s[(u << unit_log2) + i];
           sum += of * sum_s[u];
         }
@@ -234,7 +233,7 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   int64_t longest = a.max_length > 0 && a.max_length < p.capacity ? a.max_length : p.capacity;
   int64_t total = a.total_tokens > 0 && a.total_tokens < longest * c.sequences ? a.total_tokens : longest * c.sequences;
   if (p.window > 0) {
-    const int64_t seen = p.window + p.block_rows / p.gq + p.sink + 3 * stage;
+    const int64_t seen = int64_t{p.window} + p.block_rows / p.gq + p.sink + 3 * stage;
     longest = longest < seen ? longest : seen;
     total = total < longest * c.sequences ? total : longest * c.sequences;
   }

@@ -356,8 +356,8 @@ class PagedKVCache:
         first = None
         if self.next_positions != self.lengths:
             first = self._host_to_device(self.next_positions)
-        drafting = parents is not None
-        if drafting:
+        drafting = parents is not None and any(counts)
+        if parents is not None:
             parents = self._parents(parents, keys.shape[0])
         held = list(self.lengths)
         self._resize(after)
@@ -466,17 +466,20 @@ class PagedKVCache:
     ) -> tuple[torch.Tensor, torch.Tensor]:
         """(out, lse) of each sequence's last counts[b] tokens (default: one of each), [tokens, query_heads, head_dim],
         which are in the cache already: what a prompt's or a chunk's tokens see, or, with ``parents``, a tree's; see
-        ``HipAttentionBackend.run_paged_tokens``.  Weights are not summed.  Scale and window as in :meth:`attend`."""
+        ``HipAttentionBackend.run_paged_tokens``.  Weights are not summed.  Scale and window as in :meth:`attend`.
+        The lists are copied from the host, so that a call cannot be captured in a graph (that operator can)."""
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("attend_tokens copies lists from the host; capture run_paged_tokens")
         self._no_cuts(window)
         counts = [1] * self.sequences if counts is None else [int(n) for n in counts]
         if len(counts) != self.sequences or min(counts) < 0:
             raise ValueError("counts must hold one non-negative number per sequence")
+        if self._drafting and (parents is None or counts != self._latest):
+            raise RuntimeError("the cache holds drafted tokens; attend them with their parents, or keep the accepted ones")
         if query.ndim != 3 or sum(counts) != query.shape[0]:
             raise ValueError("counts must add up to the number of tokens")
         if any(n > length for n, length in zip(counts, self.lengths)):
             raise ValueError("a sequence holds fewer tokens than that")
-        if self._drafting and (parents is None or counts != self._latest):
-            raise RuntimeError("the cache holds drafted tokens; attend them with their parents, or keep the accepted ones")
         ends = [0]
         for n in counts:
             ends.append(ends[-1] + n)
@@ -515,6 +518,7 @@ class PagedKVCache:
         self.lengths[sequence] = self.next_positions[sequence] = 0
         if self._latest is not None:
             self._latest[sequence] = 0
+            self._drafting = self._drafting and any(self._latest)
         self.batch.lengths[sequence].zero_()
         self._resize(self.lengths)
 
