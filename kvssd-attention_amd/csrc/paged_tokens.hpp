@@ -569,6 +569,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
   const int value_slot = 4 * half + (lane >> 2 & 3), value_chunk = (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
   const int value_at = kKeyBytes + value_slot * kValueRow + (value_chunk ^ value_turn(value_slot, 0)) * 16 + (lane & 1) * 8;
 
+  // A wave that forms products goes first, scores before values: so do the two waves of a SIMD come to different parts of
+  // a pair, and one's products are formed beside the other's exponentials (chunks behind long contexts 1,585 -> 1,481 us,
+  // about half of it where all of a pair goes first).
   // Two tiles of 32 slots.  `plain`: every row sees all of them, their values' scale is the accumulators' and finite.
   auto work_pair = [&](int buf, int tile, int t0, bool plain, bool all_live, bool any_bad) {
     const uint8_t* const stage = lds[buf];
@@ -614,6 +617,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
       else add_scaled_rows<1>(s[n % 2], dot[n % 2], by);
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     // ---- the first tile's values set out
     constexpr int kAhead = PREC ? 2 : kSteps;  // steps
     u32x4 value[kAhead];
@@ -732,6 +736,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
 #pragma unroll
     for (int r = 0; r < 16; ++r) power(0, r);
     operands(0);
+    __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {  // beside the second tile's powers
@@ -788,7 +793,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
           if (t1 <= reach_lo - p.window && t0 >= p.sink) continue;
         }
         if (t0 > own_hi) continue;
+        __builtin_amdgcn_s_setprio(2);
         work_pair(buf, tile, t0, all, all_live, any_bad);
+        __builtin_amdgcn_s_setprio(0);
       }
     }
     if (kBuffers == 1) __syncthreads();
