@@ -19,7 +19,8 @@ constexpr int kLocate = 1024;  // threads
 constexpr int kCounted = kWave - 2;  // sequences that a workgroup counts by itself, at one look
 
 // The items' and blocks' first numbers of every sequence, where they are so many that a workgroup should not count them by
-// itself: 64 at a time take about a microsecond of each (256 sequences of 8 tokens: 425 us without, 330 with it).
+// itself, at about a microsecond for every 64 of them (256 sequences of 8 tokens: 425 us without this launch, 341 with it;
+// 64: no difference).  One workgroup, bound by the round trips of offsets and lengths.
 template <int STAGE>
 __global__ __launch_bounds__(kLocate) void paged_tokens_locate_kernel(PagedTokensParams p) {
   constexpr int kWaves = kLocate / kWave, kMost = 1 << 30;
@@ -83,10 +84,11 @@ __global__ __launch_bounds__(kLocate) void paged_tokens_locate_kernel(PagedToken
   }
 }
 
-// `unit` threads (d / 4, up to a power of two) take every `splits`-th run of a row, 4 dims each, kAhead runs' sums read
-// before the first one's weight is known; a lane a run forms the weights.  With few rows, whose time is the latency of these
-// reads, a row's runs are split between the units of a workgroup (8 tokens of 4 heads at 4,096 tokens of context, 33 runs:
-// 6 us where one unit a row took 16).
+// A row is `unit` threads' (d / 4, up to a power of two), 4 dims each, of every `splits`-th run, kAhead runs' sums read before
+// the first one's weight is known; a lane a run forms the weights.  With few rows, whose time is the latency of these reads,
+// a row's runs are split between the units of a workgroup (8 tokens of 4 heads at 4,096 tokens of context, 17 runs: 6.5 us;
+// 33 runs one after the other took 16).  With many it is bound by the partials' way through memory: 16 trees of up to 32
+// tokens 20 us.
 template <int STAGE>
 __global__ __launch_bounds__(kThreads) void paged_tokens_merge_kernel(PagedTokensParams p, int rows, int chunks, int unit_log2,
                                                                       int splits_log2) {
@@ -217,7 +219,8 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   plan->precise = p.out_dtype == KVSSD_DTYPE_F32 || p.query_dtype == KVSSD_DTYPE_F32;
   plan->dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
 
-  // rows of a workgroup, after a sequence's rows on average
+  // rows of a workgroup, after a sequence's rows on average: 256 where they fill half of them, 128 where they fill a quarter
+  // (16 trees of up to 32 tokens and 4 heads 152 us, in blocks of 64, of which two waves of four work, 190), else 32
   const int64_t each = (a.tokens * p.gq + c.sequences - 1) / c.sequences;
   plan->own = each <= 32 && !plan->precise && plan->dp <= 128;
   plan->waves = each > 128 && !plan->precise && plan->dp <= 128 ? 8 : 4;
@@ -240,7 +243,8 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   const int64_t likely = (each + p.block_rows - 1) / p.block_rows * c.sequences;  // blocks
   const int64_t work = (total / stage + c.sequences) * (likely / c.sequences);    // stages of all blocks
   // workgroups that run at a time (LDS and registers); two rounds of them where blocks are few, four of more, whose
-  // lengths differ
+  // lengths differ (8 tokens over 4,096: in runs of two stages 30 us, of three 32, of one, which are more than run at a time,
+  // 41; 16 trees in runs of 8, 15 and 28 stages 176, 152 and 151)
   const int64_t at_once = plan->waves == 4 && !plan->precise && plan->dp <= (plan->own ? 64 : 128) ? 512 : 256;
   const int64_t wanted = (likely * c.kv_heads < at_once ? 2 : 4) * at_once / c.kv_heads;
   const int64_t cut = wanted - likely > wanted / 2 ? wanted - likely : (wanted + 1) / 2;

@@ -8,11 +8,17 @@
 // with k and v held as INT2/INT4 codes c and group scales, k = (c - mid) sk.
 //
 // Work split.  The rows of a kv head are its sequence's (token, query head) pairs,
-// a token's heads side by side.  A workgroup takes a block of them, 32 C a wave in
-// row_tiles waves, and a run of the slots that they see, a stage (8,192 numbers of
-// K and of V) at a time.  Its four waves unpack a stage together, each thread the 32
-// dims of one slot that it loaded while the stage before was worked on; where rows
-// fill fewer waves, waves share the stage's slots (parts) and are joined at the end.
+// a token's heads side by side.  A workgroup takes a block of them, 32 a wave, and a
+// run of the slots that they see, a stage at a time.  Three forms, after the rows that
+// a sequence has on average:
+//   8 waves, 256 rows, stages of 16,384 numbers of K and of V (128 slots of heads of
+//     128), two of them in LDS: while one is worked on, the next, which each thread
+//     loaded a stage earlier (32 dims of a slot), is unpacked into the other;
+//   4 waves, 128 rows, stages of half that: two workgroups a CU.  Long heads take no
+//     more (registers), 32-bit results neither, with one stage in LDS;
+//   4 waves, 32 rows, every wave with 64 slots of its own (OWN), without a barrier, and
+//     joined at the end: with few rows a stage that all unpack feeds one or two waves
+//     (64 sequences of 8 tokens and 4 heads a kv head: 116 us, 129 with 8 such waves).
 //
 // QK (v_mfma_f32_32x32x16_f16): rows = slots, columns = query rows, so that a lane
 //   holds 16 scores of one query row and softmax needs no exchange but between the
@@ -28,6 +34,17 @@
 //   two fp16 parts, which hold it exactly, as they do the weights); scales are first
 //   multiplied by a power of two that puts the largest so far near fp16's top.
 //
+// Bound: a SIMD's instructions.  Two tiles of 32 slots of heads of 128 take a wave 32
+//   products (1,024 cycles) and some 370 vector instructions (4 cycles each), of which
+//   128 multiply scales in, 32 are exponentials (of two), 96 scale, sum and bound the
+//   scores; unpacking adds 150 a wave and stage.  Counted over chunks behind contexts
+//   of up to 32,768 tokens: products 35 % of the time, vector instructions 66 %, LDS
+//   conflicts 4 %.  8,187 tokens of 32 heads of 128 with a window of 1,024 take 274 us,
+//   472 TFLOP/s (a large fp16 product reaches 1,540 on this card); trees of 64 tokens
+//   over 65,536 to 131,072 slots 590 us, some 670 TFLOP/s.  16x16x32 products, which
+//   leave registers for more waves, scale twice as many results' lanes: 310 us for the
+//   former.
+//
 // A value scale that is not finite is left out of the products, where a masked row's
 // weight of 0 times it would be NaN, and makes its group of the rows that see it NaN.
 #pragma once
@@ -37,7 +54,7 @@
 
 namespace kvssd {
 
-// slots of a stage, a multiple of 64: a thread of `waves` has a piece of 32 dims of one (of two, of long heads)
+// slots of a stage that waves unpack together, a multiple of 64: a thread has a piece of 32 dims of one (of two, of long heads)
 constexpr int tokens_stage(int dp, int waves) { return waves * 2048 / dp < 64 ? 64 : waves * 2048 / dp; }
 
 struct PagedTokensParams {
@@ -299,7 +316,7 @@ __device__ __forceinline__ void add_scaled_rows(float (&s)[16], const f32x16& do
 #undef KVSSD_ROW
 }
 
-// W: waves.  Small blocks take four, two workgroups a CU; large ones eight, which unpack a stage twice as long together.
+// W: waves; PREC: 32-bit queries or results; OWN: waves with slots of their own.
 template <int DP, int W, bool PREC, bool OWN>
 __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) ? 2 : 1) void paged_tokens_kernel(PagedTokensParams p) {
   constexpr int kStage = OWN ? 64 * W : tokens_stage(DP, W);
