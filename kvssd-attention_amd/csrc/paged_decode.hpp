@@ -113,8 +113,10 @@ struct WindowGap {
   int first;  // slot (and count) that the gap begins at; a multiple of kTile, as
   int slots;  // the number of slots left out
 };
+// WINDOW: whether p.window may be more than 0
+template <bool WINDOW>
 __device__ __forceinline__ WindowGap window_gap(const PagedDecodeParams& p, int length) {
-  if (p.window == 0 || p.window >= length) return {0, 0};
+  if (!WINDOW || p.window == 0 || p.window >= length) return {0, 0};
   const int seen = (length - p.window) / kTile * kTile;                // the window's first stage
   const int first = min(seen, (min(p.sink, length) + kTile - 1) / kTile * kTile);  // (length is at most 2^30)
   return {first, seen - first};
@@ -137,16 +139,18 @@ struct RunMap {
 };
 
 // Slots of a sequence, without a window's gap
+template <bool WINDOW>
 __device__ __forceinline__ int length_of(const PagedDecodeParams& p, int seq) {
   const int n = seq < p.c.sequences ? paged_length(p.c.lengths, seq, p.capacity) : 0;
-  return n - window_gap(p, n).slots;
+  return n - window_gap<WINDOW>(p, n).slots;
 }
 // (`first`: the length of sequence `lane`, read once for all steps)
+template <bool WINDOW>
 __device__ __forceinline__ int tiles_of_runs(const PagedDecodeParams& p, int first) {
   const int lane = threadIdx.x % kWave;
   int sum = (first + kTile - 1) / kTile, most = sum;
   for (int s = lane + kWave; s - lane < p.c.sequences; s += kWave) {
-    const int n = (length_of(p, s) + kTile - 1) / kTile;
+    const int n = (length_of<WINDOW>(p, s) + kTile - 1) / kTile;
     sum += n;
     most = max(most, n);
   }
@@ -158,28 +162,30 @@ __device__ __forceinline__ int tiles_of_runs(const PagedDecodeParams& p, int fir
 }
 
 // Stages of the sequences before `seq` (fewer than 2^31 in all); `first` as there.
+template <bool WINDOW>
 __device__ __forceinline__ int stages_before(const PagedDecodeParams& p, int seq, int first) {
   const int lane = threadIdx.x % kWave;
   int sum = lane < seq ? (first + kTile - 1) / kTile : 0;
-  for (int s = lane + kWave; s - lane < seq; s += kWave) sum += s < seq ? (length_of(p, s) + kTile - 1) / kTile : 0;
+  for (int s = lane + kWave; s - lane < seq; s += kWave) sum += s < seq ? (length_of<WINDOW>(p, s) + kTile - 1) / kTile : 0;
   return __builtin_amdgcn_readlane(wave_prefix(sum), kWave - 1);
 }
 
+template <bool WINDOW>
 __device__ __forceinline__ RunMap find_run(const PagedDecodeParams& p, int r) {
   const int lane = threadIdx.x % kWave;
-  const int first = length_of(p, lane);
-  RunMap m{tiles_of_runs(p, first), -1, 0, 0, 0};
+  const int first = length_of<WINDOW>(p, lane);
+  RunMap m{tiles_of_runs<WINDOW>(p, first), -1, 0, 0, 0};
   if (p.runs <= p.c.sequences) {
     if (r < p.c.sequences) {
       m.seq = r;
       m.length = clamp_length(uniform_load(p.c.lengths + r), p.capacity);
-      m.length -= window_gap(p, m.length).slots;
-      if (p.scores != nullptr) m.before = stages_before(p, r, first);
+      m.length -= window_gap<WINDOW>(p, m.length).slots;
+      if (p.scores != nullptr) m.before = stages_before<WINDOW>(p, r, first);
     }
     return m;
   }
   for (int s0 = 0; s0 < p.c.sequences; s0 += kWave) {
-    const int length = s0 == 0 ? first : length_of(p, s0 + lane);
+    const int length = s0 == 0 ? first : length_of<WINDOW>(p, s0 + lane);
     const int n = ((length + kTile - 1) / kTile + m.tiles - 1) / m.tiles;
     const int upto = wave_prefix(n);
     const uint64_t past = __ballot(r < upto);
@@ -188,7 +194,7 @@ __device__ __forceinline__ RunMap find_run(const PagedDecodeParams& p, int r) {
       m.seq = s0 + at;
       m.nth = r - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
       m.length = __builtin_amdgcn_readlane(length, at);
-      if (p.scores != nullptr) m.before = stages_before(p, m.seq, first);
+      if (p.scores != nullptr) m.before = stages_before<WINDOW>(p, m.seq, first);
       return m;
     }
     r -= __builtin_amdgcn_readlane(upto, kWave - 1);
@@ -197,13 +203,14 @@ __device__ __forceinline__ RunMap find_run(const PagedDecodeParams& p, int r) {
 }
 
 // first run of a sequence, and its number of runs
+template <bool WINDOW>
 __device__ __forceinline__ RunMap runs_of(const PagedDecodeParams& p, int seq, int* first, int* count) {
   const int lane = threadIdx.x % kWave;
-  const int mine = length_of(p, lane);
-  const RunMap m{tiles_of_runs(p, mine), seq, 0, 0, 0};
+  const int mine = length_of<WINDOW>(p, lane);
+  const RunMap m{tiles_of_runs<WINDOW>(p, mine), seq, 0, 0, 0};
   int before = 0;
   for (int s0 = 0; s0 <= seq; s0 += kWave) {
-    const int length = s0 == 0 ? mine : length_of(p, s0 + lane);
+    const int length = s0 == 0 ? mine : length_of<WINDOW>(p, s0 + lane);
     const int n = ((length + kTile - 1) / kTile + m.tiles - 1) / m.tiles;
     const int upto = wave_prefix(n);
     if (seq < s0 + kWave) {
@@ -316,7 +323,8 @@ __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirst
 // and a head's scales begin in a word alike in every row, so that a copy's rows
 // have one uniform base; else every lane finds its own row's address (whole passes
 // of the 64 ragged sequences 43.9 and 47.6 us, of the 795 MB 159 and 179).
-template <int BITS, int DP, int GP, bool PREC, bool UNI>
+// WINDOW: a window's masks and gap; without, a pass is 2 % shorter (the 795 MB 166 and 169 us).
+template <int BITS, int DP, int GP, bool PREC, bool UNI, bool WINDOW>
 __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(PagedDecodeParams p) {
   constexpr int kWaves = decode_waves(DP);
   constexpr int kRow = DP * BITS / 8;      // bytes of a (padded) row in LDS
@@ -351,7 +359,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   const int kvh = scalar(unit / p.tiles);
   const kvssd_paged_cache& c = p.c;
   if (kvh >= c.kv_heads) return;
-  const RunMap map = find_run(p, run);
+  const RunMap map = find_run<WINDOW>(p, run);
   if (map.seq < 0) return;
   const int seq = scalar(map.seq);
   const int length = scalar(map.length);
@@ -360,9 +368,9 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   // slot = count + gap.slots from gap.first on; of those, the window's begin at `seen`
   WindowGap gap{0, 0};
   int seen = 0;
-  if (p.window > 0) {
+  if constexpr (WINDOW) {
     const int whole_length = clamp_length(uniform_load(c.lengths + seq), p.capacity);
-    gap = window_gap(p, whole_length);
+    gap = window_gap<WINDOW>(p, whole_length);
     seen = max(whole_length - p.window, 0);
   }
   const int score_stage = scalar(map.before) + begin / kTile;  // where the run's scores lie, if they are kept
@@ -402,10 +410,10 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     half_page = scalar(slot / bt);
     half_off = slot - half_page * bt;
   };
-  if constexpr (UNI) seek(begin + (begin >= gap.first ? gap.slots : 0));
+  if constexpr (UNI) seek(begin + (WINDOW && begin >= gap.first ? gap.slots : 0));
   int next_page[2] = {-1, -1}, next_off[2] = {0, 0};
   auto fetch_pages = [&](int base) {
-    if (gap.slots != 0 && base == gap.first) seek(base + gap.slots);
+    if (WINDOW && gap.slots != 0 && base == gap.first) seek(base + gap.slots);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       next_page[h] = base + 32 * h < end ? uniform_load(pages + half_page) : -1;
@@ -429,7 +437,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   };
   auto locate = [&](int base) {
     Stage s;
-    const int first_slot = base + (base >= gap.first ? gap.slots : 0);
+    const int first_slot = base + (WINDOW && base >= gap.first ? gap.slots : 0);
     if constexpr (UNI) {  // (an odd number of groups: of an even number of kv heads)
       const int left = end - base;
       s.live = left >= kTile ? ~0ull : (1ull << left) - 1;
@@ -439,7 +447,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
         s.row[h] = ok ? next_page[h] * bt + next_off[h] : 0;
         if (!ok) s.live &= h ? 0xFFFFFFFFull : 0xFFFFFFFF00000000ull;
       }
-      if (first_slot < seen) {
+      if (WINDOW && first_slot < seen) {
         const int out = seen - first_slot, sinks = p.sink - first_slot;
         s.live &= (out >= kTile ? 0ull : ~0ull << out) | (sinks <= 0 ? 0ull : sinks >= kTile ? ~0ull : (1ull << sinks) - 1);
       }
@@ -448,7 +456,7 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
     } else {
       const int slot = first_slot + lane;
       int mine = -1;
-      if (base + lane < end && (slot >= seen || slot < p.sink)) {
+      if (base + lane < end && (!WINDOW || slot >= seen || slot < p.sink)) {
         const int page = pages[slot / bt];
         if (page >= 0 && page < c.num_pages) mine = page * bt + slot % bt;
       }
@@ -931,23 +939,26 @@ __global__ __launch_bounds__(decode_waves(DP) * kWave) void paged_decode_kernel(
   }
 }
 
-template <int BITS, int DP, int GP, bool PREC>
+template <int BITS, int DP, int GP, bool PREC, bool WINDOW>
 int launch_paged_kernel(const PagedDecodeParams& p, hipStream_t stream) {
   const dim3 grid((p.runs + p.group_runs - 1) / p.group_runs, p.groups_of_units);
   const dim3 block(p.group_units * p.group_runs * kWave);
   if constexpr (DP * BITS >= 256) {
     if (p.c.page_tokens % 32 == 0 && p.c.head_dim * BITS % 128 == 0 && !(p.groups % 2 && p.c.kv_heads % 2)) {
-      hipLaunchKernelGGL((paged_decode_kernel<BITS, DP, GP, PREC, true>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((paged_decode_kernel<BITS, DP, GP, PREC, true, WINDOW>), grid, block, 0, stream, p);
       return hip_status(hipGetLastError(), "paged_decode launch");
     }
   }
-  hipLaunchKernelGGL((paged_decode_kernel<BITS, DP, GP, PREC, false>), grid, block, 0, stream, p);
+  hipLaunchKernelGGL((paged_decode_kernel<BITS, DP, GP, PREC, false, WINDOW>), grid, block, 0, stream, p);
   return hip_status(hipGetLastError(), "paged_decode launch");
 }
 
 template <int BITS, int DP, int GP>
 int launch_paged_shape(const PagedDecodeParams& p, bool precise, hipStream_t stream) {
-  return precise ? launch_paged_kernel<BITS, DP, GP, true>(p, stream) : launch_paged_kernel<BITS, DP, GP, false>(p, stream);
+  if (p.window > 0) {
+    return precise ? launch_paged_kernel<BITS, DP, GP, true, true>(p, stream) : launch_paged_kernel<BITS, DP, GP, false, true>(p, stream);
+  }
+  return precise ? launch_paged_kernel<BITS, DP, GP, true, false>(p, stream) : launch_paged_kernel<BITS, DP, GP, false, false>(p, stream);
 }
 
 }  // namespace kvssd

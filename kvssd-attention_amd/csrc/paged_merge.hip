@@ -39,7 +39,8 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedDecodeParams
   const int seq = blockIdx.x / p.query_heads, h = blockIdx.x % p.query_heads;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   int first_run, n;
-  runs_of(p, seq, &first_run, &n);
+  if (p.window > 0) runs_of<true>(p, seq, &first_run, &n);
+  else runs_of<false>(p, seq, &first_run, &n);
   const int64_t row0 = static_cast<int64_t>(first_run) * p.query_heads + h;  // run r: row0 + r * query_heads
   const int d0 = 4 * (blockIdx.y * LANES + tid % LANES);
   const int d = p.c.head_dim;
@@ -143,7 +144,7 @@ __global__ __launch_bounds__(kThreads) void paged_weights_kernel(PagedDecodePara
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int length = paged_length(p.c.lengths, seq, p.capacity);
   if (static_cast<int64_t>(nth) * 4 * kWave >= length) return;
-  const int before = stages_before(p, seq, length_of(p, lane));
+  const int before = stages_before<false>(p, seq, length_of<false>(p, lane));
   const float* lse = p.lse + static_cast<int64_t>(seq) * p.query_heads;
   for (int64_t t0 = static_cast<int64_t>(nth) * 4 * kWave; t0 < length; t0 += static_cast<int64_t>(blocks) * 4 * kWave) {
     const int64_t t = t0 + 4 * lane;
