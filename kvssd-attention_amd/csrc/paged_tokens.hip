@@ -224,9 +224,9 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   const int64_t each = (a.tokens * p.gq + c.sequences - 1) / c.sequences;
   plan->own = each <= 32 && !plan->precise && plan->dp <= 128;
   plan->waves = each > 128 && !plan->precise && plan->dp <= 128 ? 8 : 4;
-  const int stage = plan->stage = plan->own ? plan->waves * 64 : tokens_stage(plan->dp, plan->waves);
+  const int stage = plan->stage = plan->own ? plan->waves * 32 : tokens_stage(plan->dp, plan->waves);
   p.row_tiles = each > 128 ? plan->waves : each > 32 ? 4 : 1;
-  p.parts = plan->waves / p.row_tiles < stage / 64 ? plan->waves / p.row_tiles : stage / 64;
+  p.parts = plan->own || plan->waves / p.row_tiles < stage / 64 ? plan->waves / p.row_tiles : stage / 64;
   p.block_rows = 32 * p.row_tiles;
   p.block_log2 = 31 - __builtin_clz(p.block_rows);
   plan->blocks = a.tokens * p.gq / p.block_rows + c.sequences + 2;
@@ -245,7 +245,7 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   // workgroups that run at a time (LDS and registers); two rounds of them where blocks are few, four of more, whose
   // lengths differ (8 tokens over 4,096: in runs of two stages 30 us, of three 32, of one, which are more than run at a time,
   // 41; 16 trees in runs of 8, 15 and 28 stages 176, 152 and 151)
-  const int64_t at_once = plan->waves == 4 && !plan->precise && plan->dp <= (plan->own ? 64 : 128) ? 512 : 256;
+  const int64_t at_once = plan->waves == 4 && !plan->precise && plan->dp <= 128 ? 512 : 256;
   const int64_t wanted = (likely * c.kv_heads < at_once ? 2 : 4) * at_once / c.kv_heads;
   const int64_t cut = wanted - likely > wanted / 2 ? wanted - likely : (wanted + 1) / 2;
   int64_t size = (work + cut - 1) / (cut > 0 ? cut : 1);

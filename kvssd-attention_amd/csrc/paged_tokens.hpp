@@ -318,9 +318,10 @@ __device__ __forceinline__ void add_scaled_rows(float (&s)[16], const f32x16& do
 
 // W: waves; PREC: 32-bit queries or results; OWN: waves with slots of their own.
 template <int DP, int W, bool PREC, bool OWN>
-__global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) ? 2 : 1) void paged_tokens_kernel(PagedTokensParams p) {
-  constexpr int kStage = OWN ? 64 * W : tokens_stage(DP, W);
-  constexpr int kSlots = OWN ? 64 : kStage;       // of a buffer in LDS
+__global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) void paged_tokens_kernel(PagedTokensParams p) {
+  constexpr int kPair = OWN ? 1 : 2;              // tiles of 32 slots that a wave works on at a time
+  constexpr int kStage = OWN ? 32 * W : tokens_stage(DP, W);
+  constexpr int kSlots = OWN ? 32 : kStage;       // of a buffer in LDS
   constexpr int kSlices = DP / 32;
   constexpr int kParts = PREC ? 2 : 1;
   // in LDS: stages, one of which is unpacked while another is worked on, or the waves' parts of one
@@ -345,7 +346,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
   __shared__ uint64_t live_lds[kBuffers][kGroups], bad_lds[kBuffers][kGroups];  // a bit a lane of a group's pieces
   // of a group: exponent that its values are scaled by; whether slots take no part, or value scales are not finite
   constexpr uint32_t kGaps = 256, kBad = 512;
-  __shared__ __attribute__((aligned(16))) uint32_t flags_lds[kBuffers][kGroups];
+  __shared__ __attribute__((aligned(16))) uint32_t flags_lds[kBuffers][(kGroups + 3) / 4 * 4];
 
   constexpr int kTree = 1024;  // tokens of a tree whose parents are kept in LDS
   __shared__ int16_t parent_lds[kTree];
@@ -589,31 +590,31 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
   // A wave that forms products goes first, scores before values: so do the two waves of a SIMD come to different parts of
   // a pair, and one's products are formed beside the other's exponentials (chunks behind long contexts 1,585 -> 1,481 us,
   // about half of it where all of a pair goes first).
-  // Two tiles of 32 slots.  `plain`: every row sees all of them, their values' scale is the accumulators' and finite.
+  // A pair of tiles of 32 slots (or one).  `plain`: every row sees all of them, their values' scale is the accumulators' and finite.
   auto work_pair = [&](int buf, int tile, int t0, bool plain, bool all_live, bool any_bad) {
     const uint8_t* const stage = lds[buf];
     // ---- scores.  Steps: (slice, tile), the tiles in turn, so that a step's products are formed while those of the one
     // before, of the other tile, are scaled
-    constexpr int kSteps = 2 * kSlices, kRing = 3;
-    float s[2][16], sk[kRing];
+    constexpr int kSteps = kPair * kSlices, kRing = 3;
+    float s[kPair][16], sk[kRing];
     u32x4 key[kRing][2];
     int at_col = 32 * tile + col;
     asm volatile("" : "+v"(at_col));  // (a register for every turn of it would be kept otherwise)
     auto read_keys = [&](int n) {
-      sk[n % kRing] = scale_lds[buf][n / 2][tile + n % 2][half][lane & 15];  // a slot's a lane, alike in the half's two rows
-      const uint8_t* at = stage + ((4 * (n / 2) + half) * kSlots + (at_col ^ n / 2 * kTurn) + 32 * (n % 2)) * 16;
+      sk[n % kRing] = scale_lds[buf][n / kPair][tile + n % kPair][half][lane & 15];  // a slot's a lane, alike in the half's two rows
+      const uint8_t* at = stage + ((4 * (n / kPair) + half) * kSlots + (at_col ^ n / kPair * kTurn) + 32 * (n % kPair)) * 16;
 #pragma unroll
       for (int j = 0; j < 2; ++j) __builtin_memcpy(&key[n % kRing][j], __builtin_assume_aligned(at + 2 * j * kSlots * 16, 16), 16);
     };
     auto product = [&](int n, int j, f32x16 to) {
-      to = mfma32(key[n % kRing][j], q[0][n / 2 * 2 + j], to);
+      to = mfma32(key[n % kRing][j], q[0][n / kPair * 2 + j], to);
       if constexpr (PREC) {
-        if (wide) to = mfma32(key[n % kRing][j], q[kParts - 1][n / 2 * 2 + j], to);
+        if (wide) to = mfma32(key[n % kRing][j], q[kParts - 1][n / kPair * 2 + j], to);
       }
       return to;
     };
 #pragma unroll
-    for (int n = 0; n < kRing; ++n) read_keys(n);
+    for (int n = 0; n < kRing && n < kSteps; ++n) read_keys(n);
     f32x16 dot[2];
     dot[0] = product(0, 0, f32x16{});
     dot[0] = product(0, 1, dot[0]);
@@ -625,18 +626,19 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
       if (n > 0 && n + kRing - 1 < kSteps) read_keys(n + kRing - 1);
       if (more) dot[(n + 1) % 2] = product(n + 1, 0, f32x16{});
       __builtin_amdgcn_sched_barrier(0);
-      if (n < 2) scale_rows<0, 8>(s[n % 2], dot[n % 2], by);
-      else add_scaled_rows<0>(s[n % 2], dot[n % 2], by);
+      if (n < kPair) scale_rows<0, 8>(s[n % kPair], dot[n % 2], by);
+      else add_scaled_rows<0>(s[n % kPair], dot[n % 2], by);
       __builtin_amdgcn_sched_barrier(0);
       if (more) dot[(n + 1) % 2] = product(n + 1, 1, dot[(n + 1) % 2]);
       __builtin_amdgcn_sched_barrier(0);
-      if (n < 2) scale_rows<8, 16>(s[n % 2], dot[n % 2], by);
-      else add_scaled_rows<1>(s[n % 2], dot[n % 2], by);
+      if (n < kPair) scale_rows<8, 16>(s[n % kPair], dot[n % 2], by);
+      else add_scaled_rows<1>(s[n % kPair], dot[n % 2], by);
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
     // ---- the first tile's values set out
-    constexpr int kAhead = PREC ? 2 : kSteps;  // steps
+    constexpr int kValues = 2 * kSlices;  // steps of a tile
+    constexpr int kAhead = PREC ? 2 : kValues;
     u32x4 value[kAhead];
     auto fetch = [&](int of, int n, int from) {  // of a tile, step n % 2 of slice n / 2
       const int start = value_turn(0, n / 2) ? value_at ^ value_turn(0, n / 2) * 16 : value_at;
@@ -649,13 +651,13 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
     __builtin_amdgcn_sched_barrier(0);
     // ---- weights: s is turned into log2 units above the reference, then into its powers
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < kPair; ++x)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[x][r] = __builtin_fmaf(s[x][r], factor, -m);
-    uint32_t seen[2];  // of the lane's slots: bit r, slot 8 (r / 4) + 4 half + r % 4
+    uint32_t seen[kPair];  // of the lane's slots: bit r, slot 8 (r / 4) + 4 half + r % 4
     if (!plain) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < kPair; ++x) {
         const int s0 = t0 + 32 * x;
         uint32_t bits = 0xFFFFFFFFu;  // of the tile's slots
         const int before = tree ? base : base + own + 1;  // slots below it are seen, but for the window
@@ -691,7 +693,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
     }
     float of[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int r = 0; r < 32; ++r) of[r % 4] = fmaxf(of[r % 4], s[r / 16][r % 16]);
+    for (int r = 0; r < 16 * kPair; ++r) of[r % 4] = fmaxf(of[r % 4], s[r / 16][r % 16]);
     float most = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
     // a new reference where a weight would be too large, or where these are the first that the row sees
     if (__any(most > kRoom || (l == 0.0f && most > -INFINITY)) || behind != 1.0f) {
@@ -706,7 +708,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
       for (int i = 0; i < kSlices; ++i) acc[i] *= alpha * behind;
       behind = 1.0f;
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < kPair; ++x)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[x][r] -= up;
     }
@@ -741,13 +743,13 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
     };
     // weights times values, step n of both tiles'; the later ones are read as these are used
     auto weigh = [&](int n) {
-      const int i = n % kSteps / 2, step = n % 2, later = n + kAhead;
+      const int i = n % kValues / 2, step = n % 2, later = n + kAhead;
       const u32x4 v = value[n % kAhead];
       acc[i] = mfma32(v, w[0][step], acc[i]);
-      if (later < 2 * kSteps) value[n % kAhead] = fetch(later / kSteps, later % kSteps, 0);
+      if (later < kPair * kValues) value[n % kAhead] = fetch(later / kValues, later % kValues, 0);
       if constexpr (PREC) {
         acc[i] = mfma32(v, w[kParts - 1][step], acc[i]);
-        acc[i] = mfma32(fetch(n / kSteps, n % kSteps, kValueBytes), w[0][step], acc[i]);
+        acc[i] = mfma32(fetch(n / kValues, n % kValues, kValueBytes), w[0][step], acc[i]);
       }
     };
 #pragma unroll
@@ -755,16 +757,18 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
     operands(0);
     __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kPair == 2) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {  // beside the second tile's powers
+      for (int r = 0; r < 16; ++r) {  // beside the second tile's powers
 #pragma unroll
-      for (int n = r * kSteps / 16; n < (r + 1) * kSteps / 16; ++n) weigh(n);
-      power(1, r);
-      if (r % 2) __builtin_amdgcn_sched_barrier(0);
+        for (int n = r * kValues / 16; n < (r + 1) * kValues / 16; ++n) weigh(n);
+        power(kPair - 1, r);
+        if (r % 2) __builtin_amdgcn_sched_barrier(0);
+      }
+      operands(kPair - 1);
     }
-    operands(1);
 #pragma unroll
-    for (int n = kSteps; n < 2 * kSteps; ++n) weigh(n);
+    for (int n = (kPair - 1) * kValues; n < kPair * kValues; ++n) weigh(n);
   };
 
   // the stage after `n` into LDS, and the one after that on its way
@@ -801,7 +805,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !((PREC || OWN) && DP > 64) 
     }
     if (active) {
       for (int tile = OWN ? 0 : 2 * part; tile < kTiles; tile += 2 * (OWN ? 1 : p.parts)) {
-        const int t0 = slot0 + 32 * tile, t1 = t0 + 63;
+        const int t0 = slot0 + 32 * tile, t1 = t0 + 32 * kPair - 1;
         // whether every row of the wave sees all of the tiles' slots, or none
         const int reach_lo = tree ? base : own_lo;  // the lowest position; slots up to it are seen, but for the window
         bool all = all_live && !any_bad && least == top && (tree ? t1 < base : t1 <= own_lo);
