@@ -242,15 +242,16 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   }
   const int64_t likely = (each + p.block_rows - 1) / p.block_rows * c.sequences;  // blocks
   const int64_t work = (total / stage + c.sequences) * (likely / c.sequences);    // stages of all blocks
-  // workgroups that run at a time (LDS and registers); two rounds of them where blocks are few, four of more, whose
-  // lengths differ (8 tokens over 4,096: in runs of two stages 30 us, of three 32, of one, which are more than run at a time,
-  // 41; 16 trees in runs of 8, 15 and 28 stages 176, 152 and 151)
+  // workgroups that run at a time (LDS and registers); one or two rounds of them where blocks are few, four of more, whose
+  // lengths differ (8 tokens over 4,096 in runs of one stage, which are more than compute units, 25 us, of two 23, of three
+  // 25; 16 such trees over 1,000 to 2,000 in a round 45, in two 53, 64 in four 91, in two 89; 16 trees of up to 32 in runs
+  // of 8, 15 and 28 stages 176, 152 and 151)
   const int64_t at_once = plan->waves == 4 && !plan->precise && plan->dp <= 128 ? 512 : 256;
-  const int64_t wanted = (likely * c.kv_heads < at_once ? 2 : 4) * at_once / c.kv_heads;
+  const int64_t wanted = (likely * c.kv_heads >= at_once ? 4 : plan->own ? 1 : 2) * at_once / c.kv_heads;
   const int64_t cut = wanted - likely > wanted / 2 ? wanted - likely : (wanted + 1) / 2;
   int64_t size = (work + cut - 1) / (cut > 0 ? cut : 1);
   if (size < 1) size = 1;
-  if (size < 2 && work * c.kv_heads > at_once) size = 2;  // (a run's start takes as long as a stage)
+  if (size < 2 && work * c.kv_heads > 256) size = 2;  // (a run's start takes as long as two stages)
   p.items = static_cast<int>(plan->blocks);
   p.least_stages = 1 << 30;
   if (size < stages(longest)) {

@@ -16,9 +16,11 @@
 //     loaded a stage earlier (32 dims of a slot), is unpacked into the other;
 //   4 waves, 128 rows, stages of half that: two workgroups a CU.  Long heads take no
 //     more (registers), 32-bit results neither, with one stage in LDS;
-//   4 waves, 32 rows, every wave with 64 slots of its own (OWN), without a barrier, and
-//     joined at the end: with few rows a stage that all unpack feeds one or two waves
-//     (64 sequences of 8 tokens and 4 heads a kv head: 116 us, 129 with 8 such waves).
+//   4 waves, 32 rows, every wave with a tile of 32 slots of its own (OWN), without a
+//     barrier, two workgroups a CU, joined at the end: with few rows a stage that all
+//     unpack feeds one or two waves (64 sequences of 8 tokens and 4 heads a kv head
+//     91 us; 116 with 64 slots a wave, for which one workgroup has room; 129 with
+//     stages that eight waves unpack).
 //
 // QK (v_mfma_f32_32x32x16_f16): rows = slots, columns = query rows, so that a lane
 //   holds 16 scores of one query row and softmax needs no exchange but between the
