@@ -445,8 +445,8 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
 
   // ---- the wave's rows
   const int part = wave / p.row_tiles;
-  const bool active = part < p.parts;
   const int wave_row0 = block * p.block_rows + (wave % p.row_tiles) * 32;
+  const bool active = part < p.parts && wave_row0 < rows;  // (the others unpack alone)
   const int row = min(wave_row0 + col, rows - 1);
   const int own = row / p.gq;  // the lane's token among the sequence's, and its position
   int place = base + own;
