@@ -220,7 +220,8 @@ int plan_of(const kvssd_paged_cache& c, const kvssd_paged_tokens_args& a, Plan* 
   plan->dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
 
   // rows of a workgroup, after a sequence's rows on average: 256 where they fill half of them, 128 where they fill a quarter
-  // (16 trees of up to 32 tokens and 4 heads 152 us, in blocks of 64, of which two waves of four work, 190), else 32
+  // (16 trees of up to 32 tokens and 4 heads 126 us, in blocks of 32 151; 256 trees of 16 tokens 170 and 199, though 16 of
+  // them 97 and 85), else 32
   const int64_t each = (a.tokens * p.gq + c.sequences - 1) / c.sequences;
   plan->own = each <= 32 && !plan->precise && plan->dp <= 128;
   plan->waves = each > 128 && !plan->precise && plan->dp <= 128 ? 8 : 4;
