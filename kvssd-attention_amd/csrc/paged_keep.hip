@@ -73,16 +73,17 @@ __global__ __launch_bounds__(kThreads) void paged_keep_kernel(KeepParams p) {
     __syncthreads();
     for (int j = tid; j < most; j += kThreads) {
       const int node = kept[first + j], before = first + j > 0 ? kept[first + j - 1] : -1;
-      if (node <= before || node >= drafted) {
+      // An entry of an ascending list is not below its place.  One that is lies behind the list's end, where anything may
+      // stand; so do all that are negative, which would name slots before the sequence's.
+      if (node < first + j || node <= before || node >= drafted) {
         atomicMin(&end, j);
         continue;
       }
-      // (ascending up to here, or the list ends earlier: then this entry may be smaller than its place)
-      const int target = base + first + j, source = base + node;
+      const int target = base + first + j, source = base + node;  // base <= target <= source < length
       slot_from[j] = source;
       slot_to[j] = target;
       int r = -1, s = -1;
-      if (node != first + j && target < length) {
+      if (node != first + j) {
         r = row_of(source);
         s = row_of(target);
       }

@@ -9,9 +9,9 @@ import torch
 
 from kvssd import PagedKVCache, keep_tokens
 from kvssd.backends.hip import HipAttentionBackend
-from paged_oracle import as_double
+from paged_oracle import as_double, make_pool, make_table
 from test_gpu_paged_tokens import check, ints, paged, problem, random_parents
-from tokens_oracle import attend_tokens, chain, visible
+from tokens_oracle import attend_tokens, chain, keep, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -208,3 +208,44 @@ def test_a_step_of_trees_in_a_graph(cuda_device):
         assert torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(after, want_after)
         assert after.tolist() == [n - 8 + len(p) for n, p in zip(lengths, paths)]
         assert all(torch.equal(t, m) for t, m in zip(arrays, moved))
+
+
+def test_what_stands_behind_a_lists_end(cuda_device):
+    """A list ends at its first entry that is not above the one before it or not a drafted token's; what follows may be
+    anything, ascending numbers from far below 0 among it."""
+    rng = np.random.default_rng(78)
+    low, high = -2**31, 2**31 - 1
+    lists = [
+        [3, -2000000000, -1999999999, -1999999998],
+        [low, low + 1, low + 2, -1, 0, 1],
+        [-5, -4, -3, 0, 1, 2],
+        [0, 1, high, -7, -6, -5, 2, 3],
+        [2, 40, 41, -100000, -99999, 5, 6],
+        [0, 5, 5, 6, 7, 8, 9],
+        [1, 0, 4, 5, 6],
+        list(range(512)) + [-1] + list(range(-3000000, -2999913)),          # (600 entries)
+        list(range(0, 1024, 2)) + list(range(-88, 0)),
+        list(range(3, 603)),
+    ]
+    width = 600
+    kept = np.sort(rng.integers(low, high, (16, width)), axis=1).astype(np.int32)  # ascending numbers of any size
+    for b, x in enumerate(lists):
+        kept[b, :min(len(x), width)] = x[:width]
+    kept[11] = rng.integers(low, high, width)
+    kept[12] = rng.integers(-40, 40, width)
+    kept[13, :9] = [4, 5, 9, 20, 21, 22, 23, 24, 39]
+    drafted = [40] * 7 + [700, 1100, 650] + [40] * 4 + [0, high]
+    lengths = [50] * 7 + [900, 1200, 700] + [50] * 6
+    pages = sum(-(-n // 16) for n in lengths) + 2
+    pool = make_pool(rng, pages, 16, 2, 64, 32, 4)
+    table = make_table(rng, lengths, 16, 80, pages)
+    weights = rng.uniform(0, 3, (16, 1280)).astype(np.float32)
+    positions = rng.integers(0, 1 << 20, (16, 1280)).astype(np.int32)
+    batch = paged(cuda_device, pool, table, lengths, 4, 32, weights, positions)
+    want = keep(pool, table, lengths, drafted, kept, weights, positions)
+    got = keep_tokens(batch, ints(cuda_device, drafted), torch.from_numpy(kept).to(cuda_device))
+    assert got.tolist() == list(want[1])
+    assert (got - ints(cuda_device, lengths) + ints(cuda_device, drafted)).tolist()[:10] == [1, 0, 0, 2, 1, 2, 1, 512, 512, 600]
+    for a, b in zip((batch.packed_k, batch.packed_v, batch.scales_k, batch.scales_v), want[0]):
+        assert np.array_equal(a.cpu().numpy().view(np.uint8), b.view(np.uint8))
+    assert np.array_equal(batch.weights.cpu().numpy(), want[2]) and np.array_equal(batch.positions.cpu().numpy(), want[3])
