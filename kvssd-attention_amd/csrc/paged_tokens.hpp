@@ -773,6 +773,17 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     for (int n = (kPair - 1) * kValues; n < kPair * kValues; ++n) weigh(n);
   };
 
+  // What some lanes have written to LDS others may read from here on, and write over what they have read.  Waves with slots
+  // of their own exchange within the wave, whose LDS operations the hardware does in their order; the fence and the barrier
+  // (no instructions) hold the compiler to it.
+  auto meet = [&] {
+    if constexpr (OWN) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
+    }
+  };
   // the stage after `n` into LDS, and the one after that on its way
   auto advance = [&](int n) {
 #pragma unroll
@@ -783,7 +794,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     }
   };
   advance(n_begin - 1);
-  if (!OWN) __syncthreads();
+  meet();
   for (int n = n_begin; n < n_end; ++n) {
     const int buf = OWN ? wave : kBuffers > 1 ? (n - n_begin) & 1 : 0;
     const int slot0 = list.stage(n) * kStage + (OWN ? wave * kSlots : 0);
@@ -821,9 +832,9 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
         __builtin_amdgcn_s_setprio(0);
       }
     }
-    if (kBuffers == 1) __syncthreads();
+    if (OWN || kBuffers == 1) meet();
     advance(n);
-    if (!OWN) __syncthreads();  // (a wave's LDS operations are done in their order)
+    meet();
   }
 
   // ---- waves of the same rows are joined (their parts of the slots in LDS, one after the other)

@@ -249,3 +249,23 @@ def test_what_stands_behind_a_lists_end(cuda_device):
     for a, b in zip((batch.packed_k, batch.packed_v, batch.scales_k, batch.scales_v), want[0]):
         assert np.array_equal(a.cpu().numpy().view(np.uint8), b.view(np.uint8))
     assert np.array_equal(batch.weights.cpu().numpy(), want[2]) and np.array_equal(batch.positions.cpu().numpy(), want[3])
+
+
+@pytest.mark.parametrize(("d", "bits"), [(64, 4), (96, 2), (128, 4)])
+def test_few_tokens_repeat_bit_for_bit(cuda_device, d, bits):
+    """Waves that exchange keys, values and flags among their own lanes: the same bits in every pass, with slots that lie
+    in no page and a value scale that is not finite among them."""
+    rng, pool, table, lengths, offsets, q = problem(cuda_device, bits, 8, 2, d, 32, 32, [1500, 70, 0], [8, 6, 3], torch.float16, 79)
+    pool = tuple(x.copy() for x in pool)
+    table[0, [3, 17]] = -1
+    pool[3].reshape(-1, 2, d // 32)[table[0][9] * 32 + 5, 1, 1] = np.inf
+    batch = paged(cuda_device, pool, table, lengths, bits, 32)
+    off, up = ints(cuda_device, offsets), ints(cuda_device, random_parents(rng, [8, 6, 3]))
+    run = HipAttentionBackend().prepare_paged_tokens(q, batch, 0.1, out_dtype=torch.float16)
+    first, first_lse = run(q, off, up)
+    poisoned = torch.isnan(first)
+    assert poisoned[:8, 4:, 32:64].all() and poisoned.sum() == 8 * 4 * 32
+    for _ in range(50):
+        out, lse = run(q, off, up)
+        assert torch.equal(torch.nan_to_num(out), torch.nan_to_num(first)) and torch.equal(torch.isnan(out), poisoned)
+        assert torch.equal(lse, first_lse)
