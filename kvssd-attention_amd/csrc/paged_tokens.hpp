@@ -29,12 +29,17 @@
 //   The query is scaled by a power of two per row into fp16's range (exact for
 //   fp16 and bf16); a 32-bit one is a sum of two fp16 parts.
 // Softmax.  The reference is lazy: it is moved (and sums rescaled) only where a score
-//   exceeds the range that fp16 weights have above it.  Weights are 2^8 at the
-//   reference's maximum, so that those below fp16's normal range are nothing beside it.
+//   exceeds the range that fp16 weights have above it.  A weight is one fp16 number (32-bit
+//   results: two) whose smallest step is 2^-24, and 2^8 (2^14) or more at the row's maximum: it
+//   is off by 2^-11 (2^-22) of itself or by 2^-33 (2^-39) of the row's largest, which is more
+//   where it is below 2^-22 (2^-17) of that.
 // PV: rows = dims, columns = query rows, K = slots: the scores' lanes are the weights'
-//   lanes.  Values are codes times scale, rounded to fp16 (32-bit results: a sum of
-//   two fp16 parts, which hold it exactly, as they do the weights); scales are first
-//   multiplied by a power of two that puts the largest so far near fp16's top.
+//   lanes.  Values are codes times scale, rounded to fp16 once (32-bit results: a sum of two
+//   fp16 parts, which holds them exactly), whatever other scales the cache has.  Scales below
+//   2^8 are multiplied by 2^7 first: the smallest normal one, 2^-14, times the smallest code
+//   (in units of 2^-6 or 2^-2) is then 2^-13, in fp16's normal range, and the last place of
+//   any product, 2^-23, is in fp16's.  A run of stages with a larger one is gone through
+//   again for those alone, which are multiplied by 2^-1, so that it takes twice as long.
 //
 // Bound: a SIMD's instructions.  Two tiles of 32 slots of heads of 128 take a wave 32
 //   products (1,024 cycles) and some 370 vector instructions (4 cycles each), of which
@@ -335,8 +340,11 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   constexpr int kValueRow = DP * 2 + (DP == 64 ? 32 : 64);  // bytes; so (but for short heads) do transposed reads meet in no bank
   constexpr int kKeyBytes = DP * kSlots * 2, kValueBytes = kValueRow * kSlots;
   constexpr int kBytes = kKeyBytes + kParts * kValueBytes;
-  constexpr float kBias = 8.0f, kRoom = 14.0f;    // log2 of a weight at the reference's maximum, and at most
-  constexpr int kPlain = 14;                      // exponent of the scales that the largest factor (2^15) serves
+  // log2 of a weight at the reference's maximum, and at most.  (The smallest step is 2^-24: with 32-bit results 2^-38 of
+  // the former, at the price of references that move more often.)
+  constexpr float kBias = PREC ? 14.0f : 8.0f, kRoom = PREC ? 15.9f : 14.0f;
+  // value scales below kLarge, 2^8, times 2^7 and those from there on times 2^-1 have all their bits in fp16, times codes too
+  constexpr uint32_t kLarge = 23 << 10, kInfinite = 31 << 10;
   // keys: [chunk of 8 dims][slot] 16 bytes each, slots turned by their slice; values: [part][slot][dim], the chunks of
   // 8 dims of a slice turned by their slot's number: so do writes of 16 lanes meet in no bank either
   constexpr int kTurn = 16 / kSlices;
@@ -346,8 +354,8 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kBuffers][kBytes];
   __shared__ float scale_lds[kBuffers][kSlices][kTiles][2][16];  // keys': of slots 8 (i / 4) + 4 half + i % 4 of a tile
   __shared__ uint64_t live_lds[kBuffers][kGroups], bad_lds[kBuffers][kGroups];  // a bit a lane of a group's pieces
-  // of a group: exponent that its values are scaled by; whether slots take no part, or value scales are not finite
-  constexpr uint32_t kGaps = 256, kBad = 512;
+  // of a group: whether slots take no part, or value scales are not finite, or kLarge or more
+  constexpr uint32_t kGaps = 1, kBad = 2, kOver = 4;
   __shared__ __attribute__((aligned(16))) uint32_t flags_lds[kBuffers][(kGroups + 3) / 4 * 4];
 
   constexpr int kTree = 1024;  // tokens of a tree whose parents are kept in LDS
@@ -386,7 +394,8 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   }
 
   // ---- a thread's pieces: 32 dims of a slot
-  const int first_slot = (OWN ? lane : tid) / kSlices, slice = tid % kSlices;  // in a buffer
+  const int slice = tid % kSlices;
+  int first_slot = (OWN ? lane : tid) / kSlices;  // in a buffer
   constexpr int kNext = OWN ? kOwn : W * kOwn;  // slots to the thread's next piece
   const int d = c.head_dim, row_bytes = d * c.bits / 8;
   const bool has_dims = slice * 32 < d;
@@ -432,16 +441,19 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       x.sv = c.scales_v[scale];
     }
   };
+  auto begin = [&] {
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    row_next[i] = 0;
-    find(n_begin, i);
-  }
+    for (int i = 0; i < kPieces; ++i) {
+      row_next[i] = 0;
+      find(n_begin, i);
+    }
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    load(i);
-    find(n_begin + 1, i);
-  }
+    for (int i = 0; i < kPieces; ++i) {
+      load(i);
+      find(n_begin + 1, i);
+    }
+  };
+  begin();
 
   // ---- the wave's rows
   const int part = wave / p.row_tiles;
@@ -520,7 +532,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   const int own_lo = base + scalar(min(wave_row0, rows - 1) / p.gq);
   const int own_hi = base + scalar((min(wave_row0 + 32, rows) - 1) / p.gq);
 
-  int top = kPlain;               // exponent that the accumulators' values are scaled by
+  bool again = false;  // whether large value scales alone enter
 
   auto unpack_piece_into = [&](const Piece& x, int buf, int piece) {
     const int piece_slot = first_slot + piece * kNext;
@@ -546,20 +558,18 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     }
     const int in_tile = piece_slot % 32;
     scale_lds[buf][slice][piece_slot / 32][in_tile >> 2 & 1][(in_tile >> 3) * 4 + in_tile % 4] = half_bits_to_float(x.sk);
-    const int ex = x.sv >> 10 & 31;
-    const bool bad = ex == 31;
-    const uint64_t live = __ballot(x.live), bads = __ballot(bad);
-    int most = top;
-    if (__any(!bad && ex > top)) most = static_cast<int>(wave_most(bad ? 0u : static_cast<uint32_t>(ex)));
+    const uint32_t size = x.sv & 0x7FFFu;
+    const uint64_t live = __ballot(x.live), bads = __ballot(size >= kInfinite), overs = __ballot(size >= kLarge);
     if (lane == 0) {
       const int group = OWN ? piece : piece * W + wave;
       live_lds[buf][group] = live;
       bad_lds[buf][group] = bads;
-      flags_lds[buf][group] = most | (live == ~0ull ? 0u : kGaps) | (bads != 0 ? kBad : 0u);
+      flags_lds[buf][group] = (live == ~0ull ? 0u : kGaps) | (bads != 0 ? kBad : 0u) | (overs != bads ? kOver : 0u);
     }
     unpack(x.v, codes);
-    const _Float16 up = __builtin_bit_cast(_Float16, static_cast<uint16_t>((44 - most) << 10));  // 2^(29 - most)
-    const _Float16 s = __builtin_bit_cast(_Float16, static_cast<uint16_t>(bad ? 0 : x.sv)) * up;
+    const bool enters = again ? size - kLarge < kInfinite - kLarge : size < kLarge;
+    const _Float16 up = again ? static_cast<_Float16>(0.5f) : static_cast<_Float16>(128.0f);
+    const _Float16 s = __builtin_bit_cast(_Float16, static_cast<uint16_t>(enters ? x.sv : 0)) * up;
     const half2v ss = {s, s};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -582,7 +592,6 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
 #pragma unroll
   for (int i = 0; i < kSlices; ++i) acc[i] = f32x16{};
   float m = 0.0f, l = 0.0f;  // the reference, and the sum of the half's weights
-  float behind = 1.0f;  // what the accumulators are to be multiplied by, since the values' scale has changed
   uint32_t poison = 0;  // slices of a row that see a value scale that is not finite
 
   // where the lane reads values: slots 16 step + 4 half + (lane / 4) % 4 (and 8 on), dims 16 (lane / 16 % 2) + 4 (lane % 4)
@@ -592,7 +601,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
   // A wave that forms products goes first, scores before values: so do the two waves of a SIMD come to different parts of
   // a pair, and one's products are formed beside the other's exponentials (chunks behind long contexts 1,585 -> 1,481 us,
   // about half of it where all of a pair goes first).
-  // A pair of tiles of 32 slots (or one).  `plain`: every row sees all of them, their values' scale is the accumulators' and finite.
+  // A pair of tiles of 32 slots (or one).  `plain`: every row sees all of them, and their values' scales are finite.
   auto work_pair = [&](int buf, int tile, int t0, bool plain, bool all_live, bool any_bad) {
     const uint8_t* const stage = lds[buf];
     // ---- scores.  Steps: (slice, tile), the tiles in turn, so that a step's products are formed while those of the one
@@ -698,7 +707,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     for (int r = 0; r < 16 * kPair; ++r) of[r % 4] = fmaxf(of[r % 4], s[r / 16][r % 16]);
     float most = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
     // a new reference where a weight would be too large, or where these are the first that the row sees
-    if (__any(most > kRoom || (l == 0.0f && most > -INFINITY)) || behind != 1.0f) {
+    if (__any(most > kRoom || (l == 0.0f && most > -INFINITY))) {
       most = fmaxf(most, __shfl_xor(most, 32, kWave));
       const bool none = l + __shfl_xor(l, 32, kWave) == 0.0f;
       const bool moves = most > kRoom || (none && most > -INFINITY);
@@ -707,8 +716,7 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       m += up;
       l *= alpha;
 #pragma unroll
-      for (int i = 0; i < kSlices; ++i) acc[i] *= alpha * behind;
-      behind = 1.0f;
+      for (int i = 0; i < kSlices; ++i) acc[i] *= alpha;
 #pragma unroll
       for (int x = 0; x < kPair; ++x)
 #pragma unroll
@@ -721,15 +729,6 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
     };
     auto operands = [&](int x) {
       float (&t)[16] = s[x];
-      if (!plain) {  // values that were scaled by less than the largest so far
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int less = top - scalar(flags_lds[buf][(32 * (tile + x) + 8 * j) / kOwn] & 31u);
-          const float by = __builtin_bit_cast(float, static_cast<uint32_t>(127 - less) << 23);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) t[4 * j + i] *= by;
-        }
-      }
 #pragma unroll
       for (int step = 0; step < 2; ++step)
 #pragma unroll
@@ -793,64 +792,64 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
       find(n + 3, i);
     }
   };
-  advance(n_begin - 1);
-  meet();
-  for (int n = n_begin; n < n_end; ++n) {
-    const int buf = OWN ? wave : kBuffers > 1 ? (n - n_begin) & 1 : 0;
-    const int slot0 = list.stage(n) * kStage + (OWN ? wave * kSlots : 0);
-    uint32_t flags = 0, highest = 0, lowest = 31;
-    {
-      uint32_t of[kGroups];
-      __builtin_memcpy(of, __builtin_assume_aligned(flags_lds[buf], 16), sizeof(of));
-#pragma unroll
-      for (int w = 0; w < kGroups; ++w) {
-        flags |= of[w];
-        highest = max(highest, of[w] & 31u);
-        lowest = min(lowest, of[w] & 31u);
-      }
-    }
-    const int tops = scalar(highest), least = scalar(lowest);
-    flags = scalar(flags);
-    const bool all_live = !(flags & kGaps), any_bad = flags & kBad;
-    if (tops != top) {
-      behind *= __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - tops) << 23);
-      top = tops;
-    }
-    if (active) {
-      for (int tile = OWN ? 0 : 2 * part; tile < kTiles; tile += 2 * (OWN ? 1 : p.parts)) {
-        const int t0 = slot0 + 32 * tile, t1 = t0 + 32 * kPair - 1;
-        // whether every row of the wave sees all of the tiles' slots, or none
-        const int reach_lo = tree ? base : own_lo;  // the lowest position; slots up to it are seen, but for the window
-        bool all = all_live && !any_bad && least == top && (tree ? t1 < base : t1 <= own_lo);
-        if (p.window > 0) {
-          all = all && (t0 > own_hi - p.window || t1 < p.sink);
-          if (t1 <= reach_lo - p.window && t0 >= p.sink) continue;
-        }
-        if (t0 > own_hi) continue;
-        __builtin_amdgcn_s_setprio(2);
-        work_pair(buf, tile, t0, all, all_live, any_bad);
-        __builtin_amdgcn_s_setprio(0);
-      }
-    }
-    if (OWN || kBuffers == 1) meet();
-    advance(n);
+  for (;;) {
+    bool over = false;  // whether there are large value scales
+    advance(n_begin - 1);
     meet();
+    for (int n = n_begin; n < n_end; ++n) {
+      const int buf = OWN ? wave : kBuffers > 1 ? (n - n_begin) & 1 : 0;
+      const int slot0 = list.stage(n) * kStage + (OWN ? wave * kSlots : 0);
+      uint32_t flags = 0;
+      {
+        uint32_t of[kGroups];
+        __builtin_memcpy(of, __builtin_assume_aligned(flags_lds[buf], 16), sizeof(of));
+#pragma unroll
+        for (int w = 0; w < kGroups; ++w) flags |= of[w];
+      }
+      flags = scalar(flags);
+      const bool all_live = !(flags & kGaps), any_bad = flags & kBad;
+      over = over || (flags & kOver);
+      if (active) {
+        for (int tile = OWN ? 0 : 2 * part; tile < kTiles; tile += 2 * (OWN ? 1 : p.parts)) {
+          const int t0 = slot0 + 32 * tile, t1 = t0 + 32 * kPair - 1;
+          // whether every row of the wave sees all of the tiles' slots, or none
+          const int reach_lo = tree ? base : own_lo;  // the lowest position; slots up to it are seen, but for the window
+          bool all = all_live && !any_bad && (tree ? t1 < base : t1 <= own_lo);
+          if (p.window > 0) {
+            all = all && (t0 > own_hi - p.window || t1 < p.sink);
+            if (t1 <= reach_lo - p.window && t0 >= p.sink) continue;
+          }
+          if (t0 > own_hi) continue;
+          __builtin_amdgcn_s_setprio(2);
+          work_pair(buf, tile, t0, all, all_live, any_bad);
+          __builtin_amdgcn_s_setprio(0);
+        }
+      }
+      if (OWN || kBuffers == 1) meet();
+      advance(n);
+      meet();
+    }
+    // The large scales' turn, after the same stages: references stay, which hold for all of the scores, and so every weight
+    // is added to `l` a second time.  (A run of the workgroup's, or of a wave with slots of its own, without a scale of 2^8
+    // or more is through.)
+    if (__builtin_expect(again || !over, 1)) break;
+    again = true;
+    asm volatile("" : "+v"(first_slot));  // (what the start formed of it is not kept for this)
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i) acc[i] *= 1.0f / 256.0f;
+    begin();
+  }
+  if (again) {
+    l *= 0.5f;
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i) acc[i] *= 256.0f;
   }
 
   // ---- waves of the same rows are joined (their parts of the slots in LDS, one after the other)
-  if constexpr (OWN) {  // to one scale of the values
-    if (lane == 0) flags_lds[wave][0] = top;
-    __syncthreads();
-    uint32_t highest = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) highest = max(highest, flags_lds[w][0]);
-    const int tops = scalar(highest);
-    behind *= __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - tops) << 23);
-    top = tops;
-  }
+  if constexpr (OWN) __syncthreads();
   l += __shfl_xor(l, 32, kWave);
 #pragma unroll
-  for (int i = 0; i < kSlices; ++i) acc[i] *= poison >> i & 1u ? __builtin_nanf("") : behind;
+  for (int i = 0; i < kSlices; ++i) acc[i] *= poison >> i & 1u ? __builtin_nanf("") : 1.0f;
   if (!OWN && p.parts > 1) {
     constexpr int kRow = kSlices * 16 + 2;
     static_assert(OWN || kTiles == 2 || W / 2 * kRow * kWave * 4 <= kBuffers * kBytes, "a part's accumulators");
@@ -932,12 +931,16 @@ __global__ __launch_bounds__(W * kWave, DP < 256 && !(PREC && DP > 64) ? 2 : 1) 
 
   // ---- the result, or the run's partial
   const bool whole = runs == 1, none = l == 0.0f;
-  const float unit = (c.bits == 4 ? kUnpackScale<4> : kUnpackScale<2>) *
-                     __builtin_bit_cast(float, static_cast<uint32_t>(127 + top - 29) << 23);
-  const int64_t at = (token0 + own) * p.query_heads + head;
-  const int64_t part_at = (static_cast<int64_t>(item) * c.kv_heads + kvh) * p.block_rows + row - block * p.block_rows;
+  const float unit = (c.bits == 4 ? kUnpackScale<4> : kUnpackScale<2>) / 128.0f;  // (of the values' scales)
+  // (formed anew, the lane's number too: a register for each was kept since the query otherwise, and some in memory)
+  uint32_t none_before = 0;
+  asm volatile("" : "+v"(none_before));
+  const int own_row = wave_row0 + static_cast<int>(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none_before))) % 32;
+  if (own_row >= rows) return;
+  const int own_token = OWN ? own : own_row / p.gq;
+  const int64_t at = (token0 + own_token) * p.query_heads + kvh * p.gq + own_row - own_token * p.gq;
+  const int64_t part_at = (static_cast<int64_t>(item) * c.kv_heads + kvh) * p.block_rows + own_row - block * p.block_rows;
   const float by = !whole ? unit : none ? 0.0f : unit / l;
-  if (wave_row0 + col >= rows) return;
 #pragma unroll
   for (int i = 0; i < kFinish; ++i) {
     const int dim = 8 * ((OWN ? wave * kFinish : 0) + i) + 4 * half;
