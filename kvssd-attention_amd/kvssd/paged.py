@@ -280,6 +280,8 @@ class PagedKVCache:
         # the last append's tokens of each sequence, while they can be kept in part, and whether they are a tree
         self._latest: list[int] | None = None
         self._drafting = False
+        # of a tree: its parents, on the host or on their way there until the event, and the sequences' places among them
+        self._tree: tuple[list[int] | torch.Tensor, torch.cuda.Event | None, list[int]] | None = None
 
     @property
     def free_pages(self) -> int:
@@ -356,9 +358,10 @@ class PagedKVCache:
         first = None
         if self.next_positions != self.lengths:
             first = self._host_to_device(self.next_positions)
-        drafting = parents is not None and any(counts)
+        drafting, given = parents is not None and any(counts), None
         if parents is not None:
-            parents = self._parents(parents, keys.shape[0])
+            given = parents if isinstance(parents, torch.Tensor) else [int(x) for x in parents]
+            parents = self._parents(given, keys.shape[0])
         held = list(self.lengths)
         self._resize(after)
         try:
@@ -374,6 +377,7 @@ class PagedKVCache:
         self.lengths = after
         self.next_positions = [n + more for n, more in zip(self.next_positions, counts)]
         self._latest, self._drafting = counts, drafting
+        self._tree = self._tree_of(given, counts) if drafting else None
         return turned
 
     def _parents(self, parents: torch.Tensor | Sequence[int], tokens: int) -> torch.Tensor:
@@ -384,10 +388,45 @@ class PagedKVCache:
             parents = self._host_to_device([x if -1 <= x < tokens else -1 for x in parents])
         return parents
 
+    def _tree_of(self, parents: torch.Tensor | list[int], counts: Sequence[int]) -> tuple:
+        """What :meth:`keep` checks paths by.  A tensor on the GPU is on its way to the host when this returns."""
+        starts = [0]
+        for n in counts:
+            starts.append(starts[-1] + n)
+        if not isinstance(parents, torch.Tensor):
+            return parents, None, starts
+        if parents.device.type != "cuda":
+            return parents.tolist(), None, starts
+        with on_device(self.device.index):
+            host = torch.empty(parents.shape, dtype=parents.dtype, pin_memory=True)
+            host.copy_(parents, non_blocking=True)
+            copied = torch.cuda.Event()
+            copied.record()
+        return host, copied, starts
+
+    def _check_paths(self, paths: Sequence[Sequence[int]]) -> None:
+        """Kept tokens have the positions that follow the slots before them: they are a row's first ones, or each the
+        child of the one before it."""
+        if not self._drafting:
+            if any(path != list(range(len(path))) for path in paths):
+                raise ValueError("of tokens in a row the first ones are kept")
+            return
+        parents, copied, starts = self._tree
+        if copied is not None:
+            copied.synchronize()
+            parents = parents.tolist()
+            self._tree = parents, None, starts
+        for path, start in zip(paths, starts):
+            for above, x in zip([-1, *path], path):
+                up = parents[start + x]
+                if (up if 0 <= up < x else -1) != above:
+                    raise ValueError("a tree's path must lead from a token without a parent from child to child")
+
     def keep(self, paths: Sequence[Sequence[int] | None]) -> None:
-        """Of the last append's tokens, keep paths[b] of sequence b -- their places among its tokens, ascending; of a
-        tree, a path from one without a parent down -- and drop the others (:func:`keep_tokens`); pages behind are given
-        back.  None keeps all, of a sequence whose tokens are no tree."""
+        """Of the last append's tokens, keep paths[b] of sequence b -- their places among its tokens, ascending: of tokens
+        in a row the first ones, of a tree a path from one without a parent from child to child -- and drop the others
+        (:func:`keep_tokens`); pages behind are given back.  None keeps all, of a sequence whose tokens are no tree.  Where
+        the append's parents were a tensor, this waits until that append has read them."""
         counts = self._latest
         if counts is None:
             raise RuntimeError("there are no tokens to choose from: keep follows an append")
@@ -401,6 +440,7 @@ class PagedKVCache:
             if any(not 0 <= x < n for x in path) or any(a >= b for a, b in zip(path, path[1:])):
                 raise ValueError("a path must hold ascending places among the sequence's new tokens")
             chosen.append(path)
+        self._check_paths(chosen)
         width = max(len(path) for path in chosen)
         drafted = self._host_to_device(counts)
         kept = self._host_to_device([path + [-1] * (width - len(path)) for path in chosen])
@@ -408,7 +448,7 @@ class PagedKVCache:
         dropped = [n - len(path) for n, path in zip(counts, chosen)]
         self.lengths = [n - less for n, less in zip(self.lengths, dropped)]
         self.next_positions = [n - less for n, less in zip(self.next_positions, dropped)]
-        self._latest, self._drafting = None, False
+        self._latest, self._drafting, self._tree = None, False, None
         self._resize(self.lengths)
 
     def attend(

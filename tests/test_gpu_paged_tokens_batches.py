@@ -269,3 +269,24 @@ def test_few_tokens_repeat_bit_for_bit(cuda_device, d, bits):
         out, lse = run(q, off, up)
         assert torch.equal(torch.nan_to_num(out), torch.nan_to_num(first)) and torch.equal(torch.isnan(out), poisoned)
         assert torch.equal(lse, first_lse)
+
+
+def test_paths_of_a_tree_given_as_a_tensor(cuda_device):
+    """What is kept is checked by the parents that the append read, whatever has become of the tensor, on its stream too."""
+    cache = PagedKVCache(20, 16, 2, 64, sequences=2, device=cuda_device)
+    x = torch.randn(9, 2, 64, device=cuda_device, dtype=torch.float16)
+    parents = [-1, 0, 0, 1, 4] + [-1, 0, 1, 1]
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream(cuda_device)):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            wide = ints(cuda_device, np.repeat(parents, 2))
+            cache.append(x, x, [5, 4], parents=wide[::2])  # (any stride)
+            wide.fill_(-1)
+            held = list(cache.lengths)
+            for paths in ([[0, 3], []], [[4], [1]], [[0, 1, 2], []], [[0, 4], []], [[], [0, 1, 2, 3]]):
+                with pytest.raises(ValueError, match="from child to child"):
+                    cache.keep(paths)
+            assert cache.lengths == held == cache.batch.lengths.tolist()
+            cache.keep([[0, 1, 3], [0, 1, 3]])
+            assert cache.lengths == cache.next_positions == [held[0] - 2, held[1] - 1] == cache.batch.lengths.tolist()
+        torch.cuda.current_stream().wait_stream(stream)

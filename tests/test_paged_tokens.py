@@ -345,3 +345,42 @@ def test_attention_of_the_last_tokens(cache):
     for call in (lambda: cache.attend(q[:3], window=2), lambda: cache.attend_tokens(q[:3], window=2)):
         with pytest.raises(ValueError, match="slots in the order of their positions"):
             call()
+
+
+@pytest.mark.parametrize("path", [[1], [0, 2], [1, 2], [0, 1, 3], [2, 3]], ids=str)
+def test_tokens_in_a_row_are_kept_from_the_first_on(cache, path):
+    # a later one behind a gap would lie in a slot before its position, which the next token would get too
+    cache.append(rows(5), rows(5), [4, 1, 0])
+    with pytest.raises(ValueError, match="the first ones"):
+        cache.keep([path, None, None])
+    assert cache.lengths == cache.next_positions == [4, 1, 0] and cache.calls[-1][0] == "append"
+    cache.keep([[0, 1, 2], [], []])
+    assert cache.lengths == cache.next_positions == [3, 0, 0]
+
+
+@pytest.mark.parametrize("given", ["numbers", "tensor"])
+@pytest.mark.parametrize("path", [[1], [3], [0, 1, 2], [0, 3], [0, 1, 4], [5, 6], [0, 1, 3, 4], [4]], ids=str)
+def test_a_tree_is_kept_by_a_path_of_children(cache, path, given):
+    # 0 -> 1 -> 3, 0 -> 2, 4 -> 5, and 6 (a parent that is no earlier token is none); another sequence's 0 -> 1 -> 2
+    parents = [-1, 0, 0, 1, 4, 4, 9] + [-1, 0, 1]
+    cache.append(rows(4), rows(4), [2, 1, 1])
+    up = parents if given == "numbers" else torch.tensor(parents, dtype=torch.int32)
+    cache.append(rows(10), rows(10), [7, 0, 3], parents=up)
+    if given == "tensor":
+        up.fill_(-1)  # what the tokens' positions came from counts
+    refused = path != [4]
+    if refused:
+        with pytest.raises(ValueError, match="from child to child"):
+            cache.keep([path, [], [0, 1]])
+        assert cache.lengths == [9, 1, 4] and cache.calls[-1][0] == "append"
+    with pytest.raises(ValueError, match="from child to child"):
+        cache.keep([[0], [], [1, 2]])
+    if refused:
+        cache.keep([[0, 1, 3], [], [0, 1, 2]])
+        assert cache.lengths == cache.next_positions == [5, 1, 4]
+    else:
+        cache.clear(2)  # and with it its part of the tree
+        cache.keep([[4, 5], None, []])
+        assert cache.lengths == cache.next_positions == [4, 1, 0]
+    with pytest.raises(RuntimeError, match="follows an append"):
+        cache.keep([[], [], []])
