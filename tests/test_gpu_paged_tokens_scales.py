@@ -151,3 +151,39 @@ def test_weights_keep_their_bits_beside_a_large_scale(cuda_device, d, count):
     most = largest(pool, table, lengths, offsets, 4, parents, 0, 0, 8)
     out, lse = HipAttentionBackend().run_paged_tokens(q, batch, 3e-5, ints(cuda_device, offsets), ints(cuda_device, parents))
     check(out, lse, want, most, d, 5, torch.float32)  # (a token sees the 2 or 4 slots before, and itself)
+
+
+@pytest.mark.parametrize("out32", [False, True], ids=["own", "f32"])
+@pytest.mark.parametrize("count", [6, 40, 200])
+def test_large_scales_beside_pages_that_are_gone_and_scales_that_are_not_finite(cuda_device, count, out32):
+    """The second round of the stages: slots without a page take no part in it, what is infinite or NaN makes its group of
+    the rows that see it NaN and no other; keys that are NaN make whole rows so."""
+    rng, pool, table, lengths, offsets, q = problem(cuda_device, 4, 8, 2, 128, 32, 16, [500, 90], [count, 5], torch.float16, 84)
+    pool = tuple(x.copy() for x in pool)
+    table[0, [3, 11]] = -1
+
+    def scales(which, b, slot):
+        return pool[which].reshape(-1, 2, 4)[table[b][slot // 16] * 16 + slot % 16]
+
+    for slot in (20, 333, 500 + count // 2):
+        scales(3, 0, slot)[:] = 1e4
+    scales(3, 1, 92)[:, 2] = 300.0
+    clean = tuple(x.copy() for x in pool)
+    scales(3, 0, 500 + count - 2)[0, 1] = np.inf
+    scales(3, 1, 93)[1, 3] = np.nan
+    scales(2, 0, 500 + count - 1)[1, 0] = np.nan
+    most = largest(clean, np.maximum(table, 0), lengths, offsets, 4, None, 0, 0, 8)
+    dtype = torch.float32 if out32 else torch.float16
+    for window in (0, 200):
+        want = attend_tokens(as_double(q), clean, table, lengths, offsets, 4, 0.09, None, window)
+        out, lse = HipAttentionBackend().run_paged_tokens(q, paged(cuda_device, pool, table, lengths, 4, 32), 0.09,
+                                                          ints(cuda_device, offsets), window=window, out_dtype=dtype)
+        bad = np.zeros(out.shape, bool)
+        bad[count - 2:count, :4, 32:64] = True
+        bad[count + 3:, 4:, 96:] = True
+        bad[count - 1, 4:] = True
+        got = as_double(out)
+        assert np.array_equal(np.isnan(got), bad)
+        assert np.isnan(as_double(lse)[count - 1, 4:]).all() and np.isnan(as_double(lse)).sum() == 4
+        got[bad], lse[count - 1, 4:] = want["out"][bad], torch.from_numpy(want["lse"][count - 1, 4:]).to(lse)
+        check(torch.from_numpy(got), lse, want, most, 128, max(lengths), dtype)
