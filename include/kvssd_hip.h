@@ -399,7 +399,9 @@ int kvssd_hip_paged_decode(const kvssd_paged_cache* cache, const kvssd_paged_dec
  * out (fp32, or query_dtype with out_query_dtype = 1; [tokens, query_heads,
  * head_dim], contiguous) and lse fp32 [tokens, query_heads]; a token that sees
  * nothing, or of no sequence (before offsets[0], from offsets[sequences] on),
- * gives out = 0 and lse = -inf.  max_length and total_tokens, of the lengths, size the split
+ * gives out = 0 and lse = -inf.  offsets ascend: where they fall nothing is
+ * read or written out of bounds, but a token that they name twice (as two
+ * sequences', or as one's and none's) gets either result, or parts of both.  max_length and total_tokens, of the lengths, size the split
  * (0: the table's capacity, for every sequence); lengths beyond them are
  * answered all the same.  Arithmetic as kvssd_hip_paged_decode's. */
 typedef struct kvssd_paged_tokens_args {

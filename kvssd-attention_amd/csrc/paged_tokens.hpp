@@ -26,8 +26,9 @@
 //   holds 16 scores of one query row and softmax needs no exchange but between the
 //   wave's halves.  Codes enter exactly, as (c - mid) / 2^6 (INT4) or / 2^2; the
 //   products of 32 dims are taken apart and a group's scale multiplies in 32 bits.
-//   The query is scaled by a power of two per row into fp16's range (exact for
-//   fp16 and bf16); a 32-bit one is a sum of two fp16 parts.
+//   The query is scaled by a power of two per row into fp16's range, its largest element to
+//   2^10 or more (exact for fp16 and bf16 but for elements below 2^-24 of that one, which
+//   are off by 2^-35 of it); a 32-bit one is a sum of two fp16 parts.
 // Softmax.  The reference is lazy: it is moved (and sums rescaled) only where a score
 //   exceeds the range that fp16 weights have above it.  A weight is one fp16 number (32-bit
 //   results: two) whose smallest step is 2^-24, and 2^8 (2^14) or more at the row's maximum: it
@@ -41,16 +42,19 @@
 //   any product, 2^-23, is in fp16's.  A run of stages with a larger one is gone through
 //   again for those alone, which are multiplied by 2^-1, so that it takes twice as long.
 //
-// Bound: a SIMD's instructions.  Two tiles of 32 slots of heads of 128 take a wave 32
-//   products (1,024 cycles) and some 370 vector instructions (4 cycles each), of which
-//   128 multiply scales in, 32 are exponentials (of two), 96 scale, sum and bound the
-//   scores; unpacking adds 150 a wave and stage.  Counted over chunks behind contexts
-//   of up to 32,768 tokens: products 35 % of the time, vector instructions 66 %, LDS
-//   conflicts 4 %.  8,187 tokens of 32 heads of 128 with a window of 1,024 take 274 us,
-//   472 TFLOP/s (a large fp16 product reaches 1,540 on this card); trees of 64 tokens
-//   over 65,536 to 131,072 slots 590 us, some 670 TFLOP/s.  16x16x32 products, which
-//   leave registers for more waves, scale twice as many results' lanes: 310 us for the
-//   former.
+// Nearest bound: a SIMD's vector instructions.  Two tiles of 32 slots of heads of 128 take a
+//   wave 32 products (1,024 cycles) and, with its part of unpacking, some 410 vector
+//   instructions (4 cycles each), of which 128 multiply scales in, 32 are exponentials (of
+//   two), 96 scale, sum and bound the scores.  Counted over chunks behind contexts of up to
+//   32,768 tokens: products 36 % of the time, other vector instructions 58 %, LDS conflicts
+//   5 %.  The two kinds may run side by side, of a SIMD's two waves, so that their sum is no
+//   bound: each wave waits 29 % of its time, and the vector instructions alone would take 58 %
+//   of it all.  8,187 tokens of 32 heads of 128 with a window of 1,024 take 262 to 282 us,
+//   some 475 TFLOP/s (a large fp16 product reaches 1,540 on this card); trees of 64 tokens
+//   over 65,536 to 131,072 slots 570 us, some 720 TFLOP/s.  32-bit results, in four waves of
+//   512 registers each and one stage in LDS, take 2.3 to 2.7 times as long.  16x16x32 products, which
+//   leave registers for more waves, scale twice as many results' lanes: 310 us for the former
+//   where these took 292.
 //
 // A value scale that is not finite is left out of the products, where a masked row's
 // weight of 0 times it would be NaN, and makes its group of the rows that see it NaN.

@@ -265,7 +265,8 @@ class HipAttentionBackend:
 
         Tokens offsets[b] .. offsets[b+1]-1 (int32 [sequences + 1]) of ``query`` [tokens, query_heads, head_dim] are
         those of sequence b's last slots, whose keys and values are in the cache (``append_tokens``) and which
-        ``batch.lengths`` counts.  Without ``parents`` a token sees the slots up to its own, as in a prompt or a chunk
+        ``batch.lengths`` counts; offsets ascend (a token that falling ones name twice gets either result, or parts of
+        both).  Without ``parents`` a token sees the slots up to its own, as in a prompt or a chunk
         of one.  With ``parents`` (int32 [tokens]) a sequence's tokens are a tree: parents[t] is the place of token t's
         parent among the sequence's tokens, which has to come before it; any other number makes t a child of the slots
         before all of them.  A token sees those slots, its ancestors and itself, and its position is that of its depth.

@@ -290,3 +290,36 @@ def test_paths_of_a_tree_given_as_a_tensor(cuda_device):
             cache.keep([[0, 1, 3], [0, 1, 3]])
             assert cache.lengths == cache.next_positions == [held[0] - 2, held[1] - 1] == cache.batch.lengths.tolist()
         torch.cuda.current_stream().wait_stream(stream)
+
+
+@pytest.mark.parametrize("sequences", [4, 70])
+def test_offsets_that_fall(cuda_device, sequences):
+    """They name no tokens where they fall; tokens that are then named once, by a sequence or as none's, have their result."""
+    rng = np.random.default_rng(sequences + 80)
+    tokens = 60
+    before = rng.integers(10, 60, sequences).tolist()
+    _, pool, table, lengths, _, q = problem(cuda_device, 4, 4, 2, 64, 32, 16, before, [tokens] * sequences, torch.float16, 80)
+    q = q[:tokens]
+    batch = paged(cuda_device, pool, table, lengths, 4, 32)
+    for trial in range(6):
+        offsets = np.sort(rng.integers(-5, tokens + 10, sequences + 1))
+        at = int(rng.integers(0, sequences))
+        offsets[at], offsets[at + 1] = offsets[at + 1] + 3, offsets[at] - 2  # one pair the wrong way round
+        ends = np.clip(offsets, 0, tokens)
+        named, out, size = np.zeros(tokens, int), np.zeros(q.shape), np.zeros(q.shape)
+        lse, reach = np.full(q.shape[:2], -np.inf), 0.0
+        named[:ends[0]] += 1
+        named[ends[-1]:] += 1
+        for b in range(sequences):
+            a, e = int(ends[b]), int(ends[b + 1])
+            if e > a:
+                one = attend_tokens(as_double(q), pool, table[b:b + 1], lengths[b:b + 1], [a, e], 4, 0.125)
+                named[a:e] += 1
+                out[a:e], lse[a:e], size[a:e] = one["out"][a:e], one["lse"][a:e], one["size"][a:e]
+                reach = max(reach, one["reach"])
+        assert (named > 0).all() and (named == 1).any()
+        got, got_lse = HipAttentionBackend().run_paged_tokens(q, batch, 0.125, ints(cuda_device, offsets), out_dtype=torch.float16)
+        ok = torch.from_numpy(named == 1)
+        part = dict(out=out[named == 1], lse=lse[named == 1], size=size[named == 1], reach=reach)
+        check(got.cpu()[ok], got_lse.cpu()[ok], part, 64, 120, torch.float16, False)
+        assert not torch.isnan(got).any() and not torch.isnan(got_lse).any()
