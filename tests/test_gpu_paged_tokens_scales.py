@@ -1,5 +1,6 @@
-"""Value scales of any size beside each other in attention of many tokens, on the GPU against the 64-bit oracle: a large
-one that a row does not see takes no bits of that row's result, one that it sees takes its part.
+"""Value scales of any size beside each other in attention of many tokens and outside a single token's window, on the GPU
+against the 64-bit oracle: a large one that a row does not see takes no bits of that row's result, one that it sees takes
+its part.
 
 Tolerances: those of test_gpu_paged_tokens, which go by A = sum_t p_t |v_t| of the row itself, and one more.  A weight is
 one or two fp16 numbers, of which the row's largest is 2^8 to 2^14 (2^14 to 2^16 with 32-bit results) and the smallest
@@ -187,3 +188,31 @@ def test_large_scales_beside_pages_that_are_gone_and_scales_that_are_not_finite(
         assert np.isnan(as_double(lse)[count - 1, 4:]).all() and np.isnan(as_double(lse)).sum() == 4
         got[bad], lse[count - 1, 4:] = want["out"][bad], torch.from_numpy(want["lse"][count - 1, 4:]).to(lse)
         check(torch.from_numpy(got), lse, want, most, 128, max(lengths), dtype)
+
+
+@pytest.mark.parametrize("out32", [False, True], ids=["own", "f32"])
+@pytest.mark.parametrize("value", [np.nan, np.inf, 6.5e4], ids=str)
+@pytest.mark.parametrize(("qh", "kvh", "d", "bt", "bits"), [(32, 8, 128, 64, 4), (8, 2, 64, 20, 4), (10, 5, 96, 32, 2), (16, 2, 256, 128, 4)])
+def test_slots_outside_a_single_tokens_window_have_no_part(cuda_device, qh, kvh, d, bt, bits, value, out32):
+    """Keys' and values' scales of slots behind the sinks and before the window, in stages of which others are seen: the
+    same bits as with scales like all others there."""
+    lengths = [300, 77, 1000, 64]
+    rng, pool, table, _, offsets, q = problem(cuda_device, bits, qh, kvh, d, 32, bt, [n - 1 for n in lengths], [1] * 4,
+                                              torch.float16, 85, (1e-3, 1e-2))
+    dirty = tuple(x.copy() for x in pool)
+    window, sink = 50, 5
+    for b, length in enumerate(lengths):
+        for slot in range(sink, length - window):
+            row = table[b][slot // bt] * bt + slot % bt
+            dirty[3].reshape(-1, kvh, d // 32)[row] = value
+            if not np.isfinite(value):
+                dirty[2].reshape(-1, kvh, d // 32)[row] = value
+    dtype = torch.float32 if out32 else torch.float16
+    results = [
+        HipAttentionBackend().run_paged(q, paged(cuda_device, x, table, lengths, bits, 32), 3.0, window=window, sink=sink, out_dtype=dtype)
+        for x in (pool, dirty)
+    ]
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    want = attend_tokens(as_double(q), pool, table, lengths, offsets, bits, 3.0, None, window, sink)
+    most = largest(pool, table, lengths, offsets, bits, None, window, sink, qh)
+    check(*results[1], want, most, d, window + sink, dtype)
