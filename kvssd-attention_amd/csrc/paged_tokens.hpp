@@ -19,7 +19,7 @@
 //   4 waves, 32 rows, every wave with a tile of 32 slots of its own (OWN), without a
 //     barrier, two workgroups a CU, joined at the end: with few rows a stage that all
 //     unpack feeds one or two waves (64 sequences of 8 tokens and 4 heads a kv head
-//     91 us; 116 with 64 slots a wave, for which one workgroup has room; 129 with
+//     89 us; 116 with 64 slots a wave, for which one workgroup has room; 129 with
 //     stages that eight waves unpack).
 //
 // QK (v_mfma_f32_32x32x16_f16): rows = slots, columns = query rows, so that a lane
